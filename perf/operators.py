@@ -137,6 +137,14 @@ def _normal(g, *shape, scale=1.0):
     return torch.randn(*shape, generator=g, device=DEV) * scale
 
 
+def _power_of_two(top):
+    """The scale of a block of 8-bit states: the power of two at or above its
+    largest, 2^-126 at least, 0 for zeros."""
+    part, e = torch.frexp(top.double())
+    s = torch.ldexp(torch.ones_like(part), torch.where(part == 0.5, e - 1, e)).clamp_min(2.0 ** -126)
+    return torch.where(top > 0, s, 0.0).float()
+
+
 def prepare(case, seed):
     g = torch.Generator(device=DEV).manual_seed(int(seed))
     dt = DTYPES[case["dtype"]]
@@ -173,7 +181,7 @@ def prepare(case, seed):
         flat |= {"exp_avgs": m, "exp_avg_sqs": v}
     else:
         m, v = m.view(-1, BLOCK), v.view(-1, BLOCK)
-        sm, sv = m.abs().amax(1), v.amax(1)
+        sm, sv = _power_of_two(m.abs().amax(1)), _power_of_two(v.amax(1))
         flat |= {"exp_avgs": torch.round(127 * torch.sign(m) * (m.abs() / sm.clamp_min(1e-30)[:, None]).sqrt()).to(torch.int8).view(-1),
                  "exp_avg_sqs": torch.round(255 * (v / sv.clamp_min(1e-30)[:, None]).sqrt().sqrt()).to(torch.uint8).view(-1),
                  "exp_avg_scales": sm, "exp_avg_sq_scales": sv}
@@ -267,7 +275,7 @@ def _run_adamw(s):
         c = f["exp_avg_sqs"].double().view(-1, BLOCK) / 255
         vd = b2 * (c.square().square() * f["exp_avg_sq_scales"].double()[:, None]) + (1 - b2) * gd * gd
         m1, v1 = md.float().view(-1), vd.float().view(-1)
-        sm, sv = md.abs().amax(1).float(), vd.amax(1).float()
+        sm, sv = _power_of_two(md.abs().amax(1)), _power_of_two(vd.amax(1))
         top = torch.where(sm > 0, sm, 1.0).double()[:, None]
         cm = torch.round(127 * (md.abs() / top).sqrt()).clamp_max(127) * md.sign()
         top = torch.where(sv > 0, sv, 1.0).double()[:, None]
@@ -340,8 +348,8 @@ def _exact_adamw(s):
     update = (m / (1 - b1 ** t)) / ((v / (1 - b2 ** t)).sqrt() + HYPER["eps"])
     p = p - HYPER["lr"] * (HYPER["weight_decay"] * p + update)
     if s["case"]["bits"] == 8:
-        sm = m.abs().view(-1, BLOCK).max(dim=1).values.float().double().repeat_interleave(BLOCK)
-        sv = v.view(-1, BLOCK).max(dim=1).values.float().double().repeat_interleave(BLOCK)
+        sm = m.abs().view(-1, BLOCK).max(dim=1).values.log2().ceil().exp2().repeat_interleave(BLOCK)
+        sv = v.view(-1, BLOCK).max(dim=1).values.log2().ceil().exp2().repeat_interleave(BLOCK)
         c = torch.bucketize(m.abs() / sm.clamp_min(1e-300), _levels(127, 2)).double()
         m = m.sign() * (c / 127).square() * sm
         c = torch.bucketize(v / sv.clamp_min(1e-300), _levels(255, 4)).double()
