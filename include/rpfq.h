@@ -638,6 +638,123 @@ int rpfq_linear_f32_grad(const float* grad_y, const float* x, const float* w, in
                          float* grad_b, void* work, size_t work_bytes, void* stream);
 
 /*
+ * Codes and scales of rows in 8 bits: scale[m] = max|x[m]| / 127, codes[m][k] =
+ * rint(127 x[m][k] / max|x[m]|), ties to even (of the exact quotient), 0 for a
+ * row of zeros; a row with inf or NaN has scale NaN and codes 0.  x [M, K] of
+ * x_dtype; codes: rows of ld_codes bytes (>= K), zeros past K.  For the tokens
+ * and the output channels of rpfq_linear_int8.  No counterpart in the
+ * reference, whose activations are fake-quantized (quant_i.py:438-455).
+ */
+int rpfq_quantize_int8(const void* x, int x_dtype, int64_t M, int64_t K, int8_t* codes, int64_t ld_codes, float* scale,
+                       void* stream);
+
+/* Bytes of the device workspace of rpfq_linear_int8 (x_dtype, ld_w and the
+ * weight's address decide which copies it makes); 0 also where none is needed
+ * or the shape is not taken. */
+size_t rpfq_linear_int8_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t N, int64_t K, const int8_t* w,
+                                        int64_t ld_w);
+
+/*
+ * y[m][n] = (sum_k cx[m][k] w[n][k]) sx[m] w_scale[n] + bias[n], the sum exact
+ * in int32, the rest float32 rounded once to y_dtype.  x [M, K]: values of
+ * x_dtype that the call quantizes as rpfq_quantize_int8 (x_scale NULL), or codes
+ * (x_dtype = RPFQ_I8) with their scales x_scale [M].  w: N rows of ld_w bytes
+ * (>= K), read in place where w, ld_w and K are multiples of 16, else from a
+ * copy; w_scale [N], bias [N] or NULL float32.  K <= 131072.  work 256-byte
+ * aligned.  No counterpart in the reference: the 8-bit baseline of its layers.
+ */
+#define RPFQ_I8 3
+int rpfq_linear_int8(const void* x, int x_dtype, const float* x_scale, const int8_t* w, int64_t ld_w,
+                     const float* w_scale, const float* bias, int64_t M, int64_t N, int64_t K, void* y, int y_dtype,
+                     void* work, size_t work_bytes, void* stream);
+
+/* Cross entropy of a linear classifier over V classes, z = x w^T + bias:
+ *   loss_m = lse(z_m) - (1 - e) z_m[target_m] - (e / V) sum_v z_m[v],
+ * 0 where target_m = ignore_index, NaN where it is no class; e = smoothing. */
+#define RPFQ_REDUCE_NONE 0
+#define RPFQ_REDUCE_MEAN 1 /* over the rows that are not ignored; NaN if there are none */
+#define RPFQ_REDUCE_SUM 2
+typedef struct rpfq_ce_desc {
+    int64_t M, V, D; /* rows, classes, features */
+    int64_t ignore_index;
+    int32_t dtype;      /* of x [M, D] and w [V, D] */
+    int32_t bias_dtype; /* of bias [V] */
+    int32_t reduction;
+    float smoothing;    /* 0 .. 1 */
+} rpfq_ce_desc;
+
+/* Bytes of the device workspace of rpfq_linear_cross_entropy (backward = 0) or
+ * its gradient (1): there a piece of the logits' gradient, at most about 1 GiB
+ * whatever V is; 0 if the shape is not taken. */
+size_t rpfq_linear_cross_entropy_workspace_bytes(const rpfq_ce_desc* desc, int backward);
+
+/*
+ * loss: float32, [1], or [M] with RPFQ_REDUCE_NONE.  The logits are not kept:
+ * stat [2][M] (each row's maximum, and 1 / sum exp(z - maximum)) and coef [1]
+ * (the mean's factor) are what the gradient needs of them.
+ * float32 sums; float32 operands are multiplied as three bf16 terms each, at
+ * float32 accuracy.  x and w 16-byte aligned where D % 8 == 0, work 256-byte.
+ * Replaces F.cross_entropy(head(x), target) of the reference's training loop.
+ */
+int rpfq_linear_cross_entropy(const rpfq_ce_desc* desc, const void* x, const void* w, const void* bias,
+                              const int64_t* target, float* loss, float* stat, float* coef, void* work, size_t work_bytes,
+                              void* stream);
+
+/*
+ * Gradients of it: grad_x [M, D], grad_w [V, D] of dtype, grad_bias [V] of
+ * bias_dtype (each NULL if not wanted); grad_loss: float32 [1], or [M] with
+ * RPFQ_REDUCE_NONE; stat and coef as the forward wrote them.  Rows that are
+ * ignored have zero grad_x and no share of the other two, whatever x holds
+ * there.  Sums in a fixed order; the logits' gradient is rounded to 16 bits once
+ * between its two products (float32: not rounded).
+ */
+int rpfq_linear_cross_entropy_grad(const rpfq_ce_desc* desc, const void* x, const void* w, const void* bias,
+                                   const int64_t* target, const float* stat, const float* coef, const float* grad_loss,
+                                   void* grad_x, void* grad_w, void* grad_bias, void* work, size_t work_bytes,
+                                   void* stream);
+
+/* One tensor of an AdamW step.  State of 32 bits: float32 [numel], scales NULL;
+ * of 8 bits: int8 codes of the first moment, uint8 codes of the second, one
+ * float32 scale each per 256 elements:
+ *   m = s sgn(c) (c / 127)^2,  v = s (c / 255)^4,
+ * s the power of two at or above the block's largest (2^-126 at least). */
+typedef struct rpfq_adamw_tensor {
+    void* param;
+    const void* grad; /* of the parameter's type */
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;
+    float* exp_avg_sq_scale;
+    int64_t numel;
+} rpfq_adamw_tensor;
+
+typedef struct rpfq_adamw_hyper {
+    double lr, beta1, beta2, eps, weight_decay;
+} rpfq_adamw_hyper;
+
+/*
+ * AdamW with decoupled weight decay over `count` tensors (a host array; its
+ * tensors must not overlap), parameters and gradients of dtype:
+ *   t = ++*step;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps).
+ * step: device float32.  lr_device: the learning rate in device memory instead
+ * of hyper->lr, or NULL.  grad_scale: gradients are divided by it, or NULL.
+ * found_inf: nonzero leaves everything as it is, or NULL.  A gradient that is
+ * not finite makes its element NaN, with 8-bit states its block's states.
+ * work: 8 device floats.  The state in 8 bits: codes nearest to the value, the
+ * second moment's at least 1 where it is above 0.  No counterpart in the
+ * reference (its trainer takes torch's optimizers).
+ */
+int rpfq_adamw(const rpfq_adamw_tensor* tensors, int64_t count, int dtype, int state_bits, const rpfq_adamw_hyper* hyper,
+               float* step, const float* lr_device, const float* grad_scale, const float* found_inf, float* work,
+               void* stream);
+
+/* float32 values out[i][0 .. numel[i] - 1] of 8-bit states: codes[i] of the first
+ * (second[i] = 0) or second moment, their scales one per 256.  All arrays on the host. */
+int rpfq_adamw_state_values(const void* const* codes, const float* const* scales, const int64_t* numel, const int* second,
+                            float* const* out, int64_t count, void* stream);
+
+/*
  * rpfq_quantize_wide without a workspace argument and without any device
  * allocation: the float64 partials live in a static device array of this
  * library (64 KiB per GPU, held until the process ends), so the call makes

@@ -1,0 +1,301 @@
+// 8-bit integer layer: y[m, n] = (sum_k cx[m, k] cw[n, k]) sx[m] sw[n] + b[n],
+// cx = rint(127 x / max|x_m|) with sx = max|x_m| / 127 for each token, cw and sw
+// the same of each output channel of the weight, sums exact in int32.
+#include "tile_gemm.h"
+
+namespace rpfq {
+
+// ---------------------------------------------------------------------------
+// codes and scales of rows
+// ---------------------------------------------------------------------------
+// rint(127 x / top), ties to even, exactly: float32's own product is within
+// 2e-5 of the quotient, so where it is within 1e-4 of the middle of two codes
+// the quotient is compared with that middle in 64 bits, 254 |x| against
+// (2 c + 1) top, both exact there.  16-bit rows meet such ties in earnest (x =
+// top / 2 is 63.5).
+__device__ __forceinline__ int int8_code(float x, float top, float r) {
+    const float t = fabsf(x) * r;
+    float c = __builtin_rintf(t);
+    if (fabsf(fabsf(t - c) - 0.5f) < 1e-4f) {
+        c = floorf(t);
+        const double a = 254.0 * (double)fabsf(x), mid = (2.0 * (double)c + 1.0) * (double)top;
+        if (a > mid || (a == mid && ((int)c & 1))) c += 1.0f;
+    }
+    return (int)copysignf(c, x);
+}
+
+template <int DT>
+__device__ __forceinline__ float load1(const void* p, int64_t i) {
+    if (DT == RPFQ_F32) return reinterpret_cast<const float*>(p)[i];
+    if (DT == RPFQ_F16) return (float)reinterpret_cast<const _Float16*>(p)[i];
+    return bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
+    if constexpr (DT == RPFQ_F32) {
+        const f32x4* q = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + i);
+        const f32x4 a = q[0], b = q[1];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[t] = a[t], v[4 + t] = b[t];
+    } else {
+        const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if (DT == RPFQ_F16) {
+                const half2v h = __builtin_bit_cast(half2v, w[t]);
+                v[2 * t] = (float)h[0], v[2 * t + 1] = (float)h[1];
+            } else {
+                v[2 * t] = bf16_to_f32(w[t] & 0xffffu), v[2 * t + 1] = bf16_to_f32(w[t] >> 16);
+            }
+        }
+    }
+}
+
+// What a row's largest magnitude (its bits: NaN above inf above numbers)
+// makes of it: the scale to store, and (top, r) for int8_code, both times a
+// power of two where 127 / top would overflow.  inf or NaN: scale NaN.
+struct Int8Row {
+    float scale, top, r, lift;
+    __device__ __forceinline__ explicit Int8Row(uint32_t bits) {
+        const float mx = __uint_as_float(bits);
+        const bool fin = bits < 0x7f800000u, ok = fin && mx > 0.0f;
+        scale = fin ? mx / 127.0f : __uint_as_float(0x7fc00000u);
+        lift = ok && mx < 0x1p-60f ? 0x1p80f : 1.0f;
+        top = ok ? mx * lift : 1.0f;
+        r = ok ? 127.0f / top : 0.0f;
+    }
+    __device__ __forceinline__ int code(float x) const { return r > 0.0f ? int8_code(x * lift, top, r) : 0; }
+};
+
+// One wave a row, the row in registers: K <= 512 NC, 16-byte aligned rows.
+// Codes past K (up to ldq) are zero.  HBM bound: x once, a byte a value out.
+template <int DT, int NC>
+__global__ void __launch_bounds__(256) int8_rows_kernel(const void* x, int64_t M, int K, int8_t* q, int64_t ldq,
+                                                       float* scale) {
+    const int lane = threadIdx.x & 63;
+    const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (m >= M) return;
+    float v[NC][8];
+    uint32_t mx = 0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int c = 8 * (lane + 64 * i);
+        if (c < K) {
+            load8<DT>(x, m * K + c, v[i]);
+        } else {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) v[i][t] = 0.0f;
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t) mx = max(mx, __float_as_uint(v[i][t]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
+    const Int8Row row(mx);
+    if (lane == 0) scale[m] = row.scale;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int c = 8 * (lane + 64 * i);
+        if (c >= ldq) continue;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int t = 0; t < 8; ++t) w[t >> 2] |= (uint32_t)(row.code(v[i][t]) & 0xff) << (8 * (t & 3));
+        *reinterpret_cast<uint2*>(q + m * ldq + c) = make_uint2(w[0], w[1]);
+    }
+}
+
+// Any K and alignment: one workgroup a row, read twice (the second time from L2).
+template <int DT>
+__global__ void __launch_bounds__(256) int8_rows_any_kernel(const void* x, int64_t M, int64_t K, int8_t* q, int64_t ldq,
+                                                           float* scale) {
+    __shared__ uint32_t sm[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
+        uint32_t mx = 0;
+        for (int64_t k = threadIdx.x; k < K; k += 256) mx = max(mx, __float_as_uint(load1<DT>(x, m * K + k)) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
+        if (lane == 0) sm[wave] = mx;
+        __syncthreads();
+        const Int8Row row(max(max(sm[0], sm[1]), max(sm[2], sm[3])));
+        if (threadIdx.x == 0) scale[m] = row.scale;
+        for (int64_t k = threadIdx.x; k < ldq; k += 256)
+            q[m * ldq + k] = (int8_t)(k < K ? row.code(load1<DT>(x, m * K + k)) : 0);
+        __syncthreads();
+    }
+}
+
+// codes [N, K] of any K and alignment -> rows of ldq bytes, zeros past K
+__global__ void __launch_bounds__(256) int8_pad_kernel(const int8_t* src, int64_t lds_, int64_t K, int8_t* dst, int64_t ldq,
+                                                      int64_t total) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t n = i / ldq, k = i - n * ldq;
+        dst[i] = k < K ? src[n * lds_ + k] : (int8_t)0;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// product
+// ---------------------------------------------------------------------------
+struct Int8Args {
+    TileOperand x, w;
+    const float *sx, *sw, *bias;
+    void* y;
+    int64_t M, N, K;  // K bytes of a code row
+    int tiles_m, tiles_n, group, vec;
+};
+
+template <int MB, int YDT>
+__global__ void __launch_bounds__(256, 2) int8_gemm_kernel(Int8Args a) {
+    extern __shared__ __align__(16) char smem[];
+    using G = TileGemm<MB, false, false, MmaI8>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int mt, nt;
+    group_tile(xcd_tile(blockIdx.x, a.tiles_m * a.tiles_n), a.tiles_m, a.tiles_n, a.group, mt, nt);
+    const int64_t m0 = (int64_t)mt * 32 * MB, n0 = (int64_t)nt * 256;
+    intx16 acc[2][MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = intx16{0};
+    const int steps = (int)((a.K + 63) / 64);
+    G::run(a.x, a.w, m0, n0, a.K, a.K, steps, false, 0, steps, smem, wave, lane, acc);
+    const int64_t n = n0 + 64 * wave + 4 * (lane & 15);
+    f32x4 sw = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+        if (n + t < a.N) {
+            sw[t] = a.sw[n + t];
+            if (a.bias) b[t] = a.bias[n + t];
+        }
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        const int64_t mr = m0 + 32 * i + (lane & 31);
+        const float sx = a.sx[mr < a.M ? mr : a.M - 1];
+        tile_rows(smem + wave * kTileEpi, acc[0][i], acc[1][i], lane, [&](int v, int) { return (float)v * sx; },
+                  [&](int row, int, f32x4 v) {
+                      const int64_t m = m0 + 32 * i + row;
+                      if (m < a.M) tile_store4<YDT>(a.y, m * a.N, n, a.N, a.vec, v * sw + b);
+                  });
+    }
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+template <int DT>
+static hipError_t quantize_dt(const void* x, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale, hipStream_t s) {
+    const bool vec = K % 8 == 0 && ldq % 8 == 0 && ldq <= 4096 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(q) % 8 == 0;
+    const dim3 rows((unsigned)((M + 3) / 4));
+#define RPFQ_ROWS(NC) hipLaunchKernelGGL((int8_rows_kernel<DT, NC>), rows, dim3(256), 0, s, x, M, (int)K, q, ldq, scale)
+    if (vec && ldq <= 512) RPFQ_ROWS(1);
+    else if (vec && ldq <= 1024) RPFQ_ROWS(2);
+    else if (vec && ldq <= 2048) RPFQ_ROWS(4);
+    else if (vec) RPFQ_ROWS(8);
+    else
+        hipLaunchKernelGGL((int8_rows_any_kernel<DT>), dim3((unsigned)(M < 65536 ? M : 65536)), dim3(256), 0, s, x, M, K, q,
+                           ldq, scale);
+#undef RPFQ_ROWS
+    return hipGetLastError();
+}
+
+hipError_t launch_quantize_int8(const void* x, int dt, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale,
+                                hipStream_t s) {
+    switch (dt) {
+        case RPFQ_F32: return quantize_dt<RPFQ_F32>(x, M, K, q, ldq, scale, s);
+        case RPFQ_F16: return quantize_dt<RPFQ_F16>(x, M, K, q, ldq, scale, s);
+        default: return quantize_dt<RPFQ_BF16>(x, M, K, q, ldq, scale, s);
+    }
+}
+
+template <int MB, int YDT>
+static hipError_t gemm_go(Int8Args& a, hipStream_t s) {
+    using G = TileGemm<MB, false, false, MmaI8>;
+    static std::atomic<uint64_t> attr_done{0};
+    const hipError_t e = set_lds_attr_once(reinterpret_cast<const void*>(&int8_gemm_kernel<MB, YDT>), G::LDS, attr_done);
+    if (e != hipSuccess) return e;
+    a.tiles_m = (int)((a.M + 32 * MB - 1) / (32 * MB));
+    a.tiles_n = (int)((a.N + 255) / 256);
+    a.group = tile_group(a.tiles_n, 256 * a.K);
+    hipLaunchKernelGGL((int8_gemm_kernel<MB, YDT>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(256), G::LDS, s, a);
+    return hipGetLastError();
+}
+
+template <int YDT>
+static hipError_t gemm_y(Int8Args& a, hipStream_t s) {
+    if (a.M <= 32) return gemm_go<1, YDT>(a, s);
+    const int64_t tiles = (a.M + 127) / 128 * ((a.N + 255) / 256);
+    return tiles < device_cus() ? gemm_go<2, YDT>(a, s) : gemm_go<4, YDT>(a, s);
+}
+
+// x codes in `work` unless given; w copied there if its rows are not 16-byte aligned
+Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, bool quantize, bool pad_w) {
+    Int8Plan p = {};
+    p.ld = (K + 15) & ~(int64_t)15;
+    auto take = [&](size_t n) {
+        const size_t at = p.bytes;
+        p.bytes += (n + 255) & ~(size_t)255;
+        return at;
+    };
+    if (quantize) {
+        p.x_at = take((size_t)M * p.ld);
+        p.sx_at = take((size_t)M * 4);
+    }
+    if (pad_w) p.w_at = take((size_t)N * p.ld);
+    return p;
+}
+
+static hipError_t pad_codes(const int8_t* src, int64_t ld, int64_t K, int64_t rows, int8_t* dst, int64_t ldq, hipStream_t s) {
+    const int64_t total = rows * ldq, blocks = (total + 255) / 256;
+    hipLaunchKernelGGL(int8_pad_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, src, ld, K, dst, ldq,
+                       total);
+    return hipGetLastError();
+}
+
+hipError_t launch_linear_int8(const void* x, int xdt, const float* sx, const int8_t* w, int64_t ldw, const float* sw,
+                              const float* bias, int64_t M, int64_t N, int64_t K, void* y, int ydt, void* work,
+                              hipStream_t s) {
+    const bool quantize = xdt >= 0, pad_w = int8_pads(w, ldw, K);
+    // codes that come unaligned are copied as an unaligned weight is
+    const bool pad_x = !quantize && int8_pads(x, K, K);
+    const Int8Plan p = int8_plan(M, N, K, quantize || pad_x, pad_w);
+    char* wk = reinterpret_cast<char*>(work);
+    Int8Args a = {};
+    hipError_t e;
+    if (quantize || pad_x) {
+        int8_t* q = reinterpret_cast<int8_t*>(wk + p.x_at);
+        float* qs = reinterpret_cast<float*>(wk + p.sx_at);
+        e = quantize ? launch_quantize_int8(x, xdt, M, K, q, p.ld, qs, s)
+                     : pad_codes(reinterpret_cast<const int8_t*>(x), K, K, M, q, p.ld, s);
+        if (e != hipSuccess) return e;
+        a.x = {reinterpret_cast<const char*>(q), p.ld, 0, M};
+        a.sx = quantize ? qs : sx;
+    } else {
+        a.x = {reinterpret_cast<const char*>(x), K, 0, M};
+        a.sx = sx;
+    }
+    if (pad_w) {
+        int8_t* q = reinterpret_cast<int8_t*>(wk + p.w_at);
+        e = pad_codes(w, ldw, K, N, q, p.ld, s);
+        if (e != hipSuccess) return e;
+        a.w = {reinterpret_cast<const char*>(q), p.ld, 0, N};
+    } else {
+        a.w = {reinterpret_cast<const char*>(w), ldw, 0, N};
+    }
+    a.sw = sw;
+    a.bias = bias;
+    a.y = y;
+    a.M = M;
+    a.N = N;
+    a.K = p.ld;
+    const int es = ydt == RPFQ_F32 ? 4 : 2;
+    a.vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(y) % (4 * es) == 0;
+    switch (ydt) {
+        case RPFQ_F32: return gemm_y<RPFQ_F32>(a, s);
+        case RPFQ_F16: return gemm_y<RPFQ_F16>(a, s);
+        default: return gemm_y<RPFQ_BF16>(a, s);
+    }
+}
+
+}  // namespace rpfq

@@ -1,0 +1,785 @@
+// Softmax cross entropy of a linear classifier over many classes and its
+// gradient, without keeping the logits:
+//   z = x w^T + b,  loss_m = lse(z_m) - (1 - e) z_{m,t} - (e / V) sum_v z_{m,v},
+//   dz_m = g_m (softmax(z_m) - (1 - e) 1_t - e / V),
+//   dx = dz w,  dw = dz^T x,  db = sum_m dz_m.
+// Forward: the logits' tiles leave the matrix cores as a maximum and a sum of
+// exp(z - maximum) per row and tile (float32), joined by a pass over the tiles.
+// Kept are the row's maximum and the sum's reciprocal, not lse: that one's last
+// bit is 2^-20 of a probability near 1, which is most of dz where p - 1 is small.
+// Backward: the logits are formed again, a piece of the classes at a time; dz
+// of a piece goes to a workspace in 16 bits and meets w and x from there.
+//
+// Roundings to 16 bits: dz only, once (bf16 2^-9 of its value; fp16 2^-12, dz
+// times 2^15 so that probabilities down to 2^-29 stay normal), as the matrix
+// cores take it; the sums over classes and rows stay in float32 until the
+// gradients are rounded to their own type.  float32 operands go as three bf16
+// terms (tile_pair) and lose nothing.
+#include <cmath>
+
+#include "tile_gemm.h"
+
+namespace rpfq {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct CeArgs {
+    TileOperand x, w;          // [M, D], [V, D], K layout
+    const void* bias;          // [V] of bias_dt, or NULL
+    int bias_dt;
+    const int64_t* target;
+    int64_t M, V;              // rows, classes (w.count: those of a piece)
+    int64_t v0;                // first class of the piece
+    int64_t kb;                // bytes of k
+    int per, planes;
+    int tiles_m, tiles_n, group;
+    float smooth;
+    // forward
+    float2* part;              // [tiles_n][M] (maximum, sum of exp(z - maximum))
+    float* zsum;               // [tiles_n][M] sums of z, or NULL
+    float* zt;                 // [M] the target's logit
+    // backward
+    const float *stat, *rho;   // [2][M] maximum, 1 / sum; [M]
+    float dz_scale;
+    char* dz;                  // [planes][M][ldz bytes]
+    int64_t ldz, dz_plane;
+    float* colsum;             // [tiles_m][ldz / 2] or NULL
+};
+
+__device__ __forceinline__ float ce_load(const void* p, int dt, int64_t i) {
+    if (dt == RPFQ_F32) return reinterpret_cast<const float*>(p)[i];
+    if (dt == RPFQ_F16) return (float)reinterpret_cast<const _Float16*>(p)[i];
+    return bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+}
+
+// Adds the bias to a wave's block of logits and makes those past the last
+// class -inf: columns 32 j + 8 q + 4 g + t of the wave's 64, bias in LDS.
+template <int MB>
+__device__ __forceinline__ void ce_bias(floatx16 (&acc)[2][MB], const float* bias, int lane) {
+    const int g = lane >> 5;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 b = *reinterpret_cast<const f32x4*>(bias + 32 * j + 8 * q + 4 * g);
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc[j][i][4 * q + t] += b[t];
+        }
+}
+
+// The 256 biases of a tile to LDS: -inf past the last class.
+__device__ __forceinline__ void ce_stage_bias(const CeArgs& a, int64_t n0, float* sm) {
+    const int64_t n = n0 + threadIdx.x;
+    float b = n < a.w.count ? 0.0f : -__builtin_inff();
+    if (a.bias && n < a.w.count) b = ce_load(a.bias, a.bias_dt, a.v0 + n);
+    sm[threadIdx.x] = b;
+    __syncthreads();
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+template <int MB, class Mma>
+__global__ void __launch_bounds__(256, 2) ce_stats_kernel(CeArgs a) {
+    extern __shared__ __align__(16) char smem[];
+    using G = TileGemm<MB, false, false, Mma>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 31, g = lane >> 5;
+    int mt, nt;
+    group_tile(xcd_tile(blockIdx.x, a.tiles_m * a.tiles_n), a.tiles_m, a.tiles_n, a.group, mt, nt);
+    const int64_t m0 = (int64_t)mt * 32 * MB, n0 = (int64_t)nt * 256;
+    floatx16 acc[2][MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
+    const int steps = a.planes ? kPairs32 * a.per : a.per;
+    G::run(a.x, a.w, m0, n0, a.kb, a.kb, a.per, a.planes, 0, steps, smem, wave, lane, acc);
+    float* sb = reinterpret_cast<float*>(smem);
+    float* sp = sb + 256;  // [4 waves][32 MB rows][max, sum, sum of z]
+    ce_stage_bias(a, n0, sb);
+    ce_bias<MB>(acc, sb + 64 * wave, lane);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) mx = fmaxf(mx, acc[j][i][v]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float base = mx == -__builtin_inff() ? 0.0f : mx;
+        float sum = 0.0f, zs = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) sum += __builtin_amdgcn_exp2f((acc[j][i][v] - base) * kLog2e);
+        if (a.zsum) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int64_t n = n0 + 64 * wave + 32 * j + acc_row(v, g);
+                    zs += n < a.w.count ? acc[j][i][v] : 0.0f;
+                }
+            zs += __shfl_xor(zs, 32, 64);
+        }
+        sum += __shfl_xor(sum, 32, 64);
+        const int64_t m = m0 + 32 * i + r;
+        if (m < a.M) {
+            const int64_t t = a.target[m] - n0 - 64 * wave;
+            if (t >= 0 && t < 64 && n0 + 64 * wave + t < a.V) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (t == 32 * j + acc_row(v, g)) a.zt[m] = acc[j][i][v];
+            }
+        }
+        if (g == 0) {
+            float* d = sp + (wave * 32 * MB + 32 * i + r) * 3;
+            d[0] = mx;
+            d[1] = sum;
+            d[2] = zs;
+        }
+    }
+    __syncthreads();
+    const int row = threadIdx.x;
+    if (row < 32 * MB && m0 + row < a.M) {
+        float mx = -__builtin_inff(), sum = 0.0f, zs = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mx = fmaxf(mx, sp[(w * 32 * MB + row) * 3]);
+        // fmax passes over NaN: the sums keep it
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float* d = sp + (w * 32 * MB + row) * 3;
+            sum += d[0] == -__builtin_inff() ? d[1] : d[1] * __builtin_amdgcn_exp2f((d[0] - mx) * kLog2e);
+            zs += d[2];
+        }
+        a.part[(int64_t)nt * a.M + m0 + row] = make_float2(mx, sum);
+        if (a.zsum) a.zsum[(int64_t)nt * a.M + m0 + row] = zs;
+    }
+}
+
+struct CeJoin {
+    const float2* part;
+    const float* zsum;
+    const float* zt;
+    const int64_t* target;
+    int64_t M, V, ignore;
+    int tiles;
+    float smooth;
+    float* stat;  // [2][M]: maximum, 1 / sum of exp(z - maximum)
+    float* rows;  // [M] loss of each row, 0 where ignored
+};
+
+// lse and loss of a row from its tiles: 16 lanes a row, in a fixed order.
+__global__ void __launch_bounds__(256) ce_join_kernel(CeJoin a) {
+    const int64_t m = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
+    const int q = threadIdx.x >> 4;  // 16 parts of the tiles
+    __shared__ float sm[3][16][17];
+    float mx = -__builtin_inff(), sum = 0.0f, zs = 0.0f;
+    if (m < a.M)
+        for (int t = q; t < a.tiles; t += 16) {
+            const float2 p = a.part[(int64_t)t * a.M + m];
+            const float n = fmaxf(mx, p.x), base = n == -__builtin_inff() ? 0.0f : n;
+            sum = sum * __builtin_amdgcn_exp2f((mx - base) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - base) * kLog2e);
+            // a tile of -inf has sum 0, one with NaN has sum NaN whatever its maximum
+            if (p.x == -__builtin_inff() && p.y != p.y) sum = p.y;
+            mx = n;
+            if (a.zsum) zs += a.zsum[(int64_t)t * a.M + m];
+        }
+    const int c = threadIdx.x & 15;
+    sm[0][c][q] = mx;
+    sm[1][c][q] = sum;
+    sm[2][c][q] = zs;
+    __syncthreads();
+    if (q != 0 || m >= a.M) return;
+    float top = -__builtin_inff();
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, sm[0][c][i]);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    sum = zs = 0.0f;
+    for (int i = 0; i < 16; ++i) {
+        const float s = sm[1][c][i];
+        sum += s == 0.0f ? 0.0f : s * __builtin_amdgcn_exp2f((sm[0][c][i] - base) * kLog2e);
+        zs += sm[2][c][i];
+    }
+    const float more = logf(sum);  // lse - base
+    const int64_t t = a.target[m];
+    float loss = 0.0f;
+    if (t != a.ignore) {
+        if (t < 0 || t >= a.V) {
+            loss = __uint_as_float(0x7fc00000u);
+        } else {
+            loss = (1.0f - a.smooth) * ((base - a.zt[m]) + more);
+            if (a.zsum) loss += a.smooth * ((base - zs / (float)a.V) + more);
+        }
+    }
+    a.stat[m] = base;
+    a.stat[a.M + m] = 1.0f / sum;
+    a.rows[m] = loss;
+}
+
+// Sum (reduction 2) or mean (1) of the rows' losses in a fixed order, and the
+// factor that the gradient takes from it: coef[0] = 1 or 1 / count (0 where no
+// row counts: its rows then have no gradient, their mean is NaN).
+__global__ void __launch_bounds__(1024) ce_reduce_kernel(const float* rows, const int64_t* target, int64_t M, int64_t ignore,
+                                                         int reduction, float* loss, float* coef) {
+    __shared__ double sm[1024];
+    __shared__ int cm[1024];
+    const int t = threadIdx.x;
+    double s = 0.0;
+    int n = 0;
+    for (int64_t m = t; m < M; m += 1024) {
+        s += (double)rows[m];
+        n += target[m] != ignore;
+    }
+    sm[t] = s;
+    cm[t] = n;
+    __syncthreads();
+    for (int h = 512; h > 0; h >>= 1) {
+        if (t < h) {
+            sm[t] += sm[t + h];
+            cm[t] += cm[t + h];
+        }
+        __syncthreads();
+    }
+    if (t == 0) {
+        const double c = (double)cm[0];
+        if (reduction != 0) loss[0] = (float)(reduction == 1 ? sm[0] / c : sm[0]);
+        coef[0] = reduction == 1 ? (cm[0] ? (float)(1.0 / c) : 0.0f) : 1.0f;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+// rho[m], the weight of row m in dz (0: ignored, NaN: a target that is no
+// class), and factor[0], what the gradients are multiplied by in the end.
+// Reduction 0 divides the rows' gradients by the largest of them, so that dz
+// stays within [-1, 1].
+__global__ void __launch_bounds__(1024) ce_rho_kernel(const float* grad, const float* coef, const int64_t* target, int64_t M,
+                                                      int64_t V, int64_t ignore, int reduction, float undo, float* rho,
+                                                      float* factor) {
+    __shared__ float sm[1024];
+    const int t = threadIdx.x;
+    float top = 0.0f;
+    if (reduction == 0) {
+        for (int64_t m = t; m < M; m += 1024)
+            if (target[m] != ignore) top = fmaxf(top, fabsf(grad[m]));
+        sm[t] = top;
+        __syncthreads();
+        for (int h = 512; h > 0; h >>= 1) {
+            if (t < h) sm[t] = fmaxf(sm[t], sm[t + h]);
+            __syncthreads();
+        }
+        top = sm[0];
+        // no finite scale: the rows keep their gradients as they are
+        if (!(top > 0.0f) || top > 3.40282347e38f) top = 1.0f;
+    }
+    for (int64_t m = t; m < M; m += 1024) {
+        const int64_t c = target[m];
+        const float r = reduction == 0 ? grad[m] / top : 1.0f;
+        rho[m] = c == ignore ? 0.0f : c < 0 || c >= V ? __uint_as_float(0x7fc00000u) : r;
+    }
+    if (t == 0) factor[0] = (reduction == 0 ? top : grad[0] * coef[0]) * undo;
+}
+
+// x [M, D] as the operand of dw: rows that count nowhere are zeros, whatever
+// they hold (0 x NaN would reach every class), rows of ldx elements.
+__global__ void __launch_bounds__(256) ce_rows_kernel(const uint16_t* x, int64_t D, const int64_t* target, int64_t ignore,
+                                                      uint16_t* out, int64_t ldx, int64_t total8) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total8; i += (int64_t)gridDim.x * 256) {
+        const int64_t per = ldx / 8, m = i / per, d = (i - m * per) * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (!target || target[m] != ignore) {
+            if (D == ldx) {
+                v = *reinterpret_cast<const uint4*>(x + m * D + d);
+            } else {
+                uint16_t e[8];
+#pragma unroll
+                for (int t = 0; t < 8; ++t) e[t] = d + t < D ? x[m * D + d + t] : (uint16_t)0;
+                __builtin_memcpy(&v, e, 16);
+            }
+        }
+        *reinterpret_cast<uint4*>(out + i * 8) = v;
+    }
+}
+
+// float32 rows as three bf16 terms, each the top 8 bits of what is left: exact
+// for every finite value.  target: as in ce_rows_kernel, or NULL.
+__device__ __forceinline__ void split3(float v, uint16_t& h, uint16_t& m, uint16_t& l) {
+    const uint32_t u = __float_as_uint(v);
+    if ((u & 0x7fffffffu) > 0x7f800000u) {
+        h = 0x7fc0, m = l = 0;
+        return;
+    }
+    h = (uint16_t)(u >> 16);
+    const float r1 = (u & 0x7fffffffu) == 0x7f800000u ? 0.0f : v - __uint_as_float(u & 0xffff0000u);
+    m = (uint16_t)(__float_as_uint(r1) >> 16);
+    const float r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
+    l = (uint16_t)(__float_as_uint(r2) >> 16);
+}
+
+__global__ void __launch_bounds__(256) ce_planes_kernel(const float* x, int64_t rows, int64_t D, const int64_t* target,
+                                                        int64_t ignore, uint16_t* out, int64_t ld) {
+    const int64_t total = rows * (ld / 8), plane = rows * ld;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t per = ld / 8, m = i / per, d = (i - m * per) * 8;
+        uint16_t h[8], k[8], l[8];
+        const bool on = !target || target[m] != ignore;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) split3(on && d + t < D ? x[m * D + d + t] : 0.0f, h[t], k[t], l[t]);
+        __builtin_memcpy(out + i * 8, h, 16);
+        __builtin_memcpy(out + plane + i * 8, k, 16);
+        __builtin_memcpy(out + 2 * plane + i * 8, l, 16);
+    }
+}
+
+// dz of one piece of the classes.  DT: the type of dz (float32: three planes).
+template <int MB, class Mma, int DT>
+__global__ void __launch_bounds__(256, 2) ce_dz_kernel(CeArgs a) {
+    extern __shared__ __align__(16) char smem[];
+    using G = TileGemm<MB, false, false, Mma>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 31, c4 = 4 * (lane & 15);
+    int mt, nt;
+    group_tile(xcd_tile(blockIdx.x, a.tiles_m * a.tiles_n), a.tiles_m, a.tiles_n, a.group, mt, nt);
+    const int64_t m0 = (int64_t)mt * 32 * MB, n0 = (int64_t)nt * 256;
+    floatx16 acc[2][MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
+    const int steps = a.planes ? kPairs32 * a.per : a.per;
+    G::run(a.x, a.w, m0, n0, a.kb, a.kb, a.per, a.planes, 0, steps, smem, wave, lane, acc);
+    float* sb = reinterpret_cast<float*>(smem + 4 * kTileEpi);
+    ce_stage_bias(a, n0, sb);
+    ce_bias<MB>(acc, sb + 64 * wave, lane);
+    const float even = a.smooth / (float)a.V;
+    const int64_t n = n0 + 64 * wave + c4;  // the lane's columns in out()
+    f32x4 cs = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        const int64_t mr = m0 + 32 * i + r;
+        float top = 0.0f, inv = 0.0f, rho = 0.0f;
+        int t = -1;  // the target's column among the wave's
+        if (mr < a.M) {
+            top = a.stat[mr];
+            inv = a.stat[a.M + mr];
+            rho = a.rho[mr] * a.dz_scale;
+            const int64_t tt = a.target[mr] - a.v0 - n0 - 64 * wave;
+            t = tt >= 0 && tt < 64 ? (int)tt : -1;
+        }
+        tile_rows(
+            smem + wave * kTileEpi, acc[0][i], acc[1][i], lane,
+            [&](float z, int col) {
+                float p = __builtin_amdgcn_exp2f((z - top) * kLog2e) * inv - even;
+                if (col == t) p -= 1.0f - a.smooth;
+                return rho == 0.0f ? 0.0f : p * rho;
+            },
+            [&](int row, int, f32x4 v) {
+                const int64_t m = m0 + 32 * i + row;
+                if (m >= a.M || 2 * n >= a.ldz) return;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e >= a.w.count) v[e] = 0.0f;
+                cs += v;
+                char* d = a.dz + m * a.ldz + 2 * n;
+                if constexpr (DT == RPFQ_F32) {
+                    uint16_t h[4], k[4], l[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split3(v[e], h[e], k[e], l[e]);
+                    __builtin_memcpy(d, h, 8);
+                    __builtin_memcpy(d + a.dz_plane, k, 8);
+                    __builtin_memcpy(d + 2 * a.dz_plane, l, 8);
+                } else {
+                    uint2 o;
+                    o.x = DT == RPFQ_F16 ? cvt_pk(v[0], v[1]) : pack_bf2(v[0], v[1]);
+                    o.y = DT == RPFQ_F16 ? cvt_pk(v[2], v[3]) : pack_bf2(v[2], v[3]);
+                    *reinterpret_cast<uint2*>(d) = o;
+                }
+            });
+    }
+    if (a.colsum) {  // the lane's columns over the tile's rows
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            cs[e] += __shfl_xor(cs[e], 16, 64);
+            cs[e] += __shfl_xor(cs[e], 32, 64);
+        }
+        if (lane < 16 && 2 * n < a.ldz) *reinterpret_cast<f32x4*>(a.colsum + (int64_t)mt * (a.ldz / 2) + n) = cs;
+    }
+}
+
+struct CeGrad {
+    TileOperand r, c;
+    int64_t rk, ck;
+    int64_t M, N;     // rows, columns of the gradient
+    int per, steps, planes, splits;
+    int tiles_m, tiles_n, group;
+    float* part;      // [splits][M][ldp], or NULL: the gradient itself, rounded
+    int64_t ldp;
+    int add;          // part holds the pieces before
+    const float* factor;
+    void* out;        // [M, N]
+    int vec;
+};
+
+// One product of the gradient: dx (dz in K layout, w in T) or dw (dz and x in T).
+template <bool RT, class Mma, int DT>
+__global__ void __launch_bounds__(256, 2) ce_grad_kernel(CeGrad a) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr int MB = 4;
+    using G = TileGemm<MB, RT, true, Mma>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles = a.tiles_m * a.tiles_n;
+    const int unit = xcd_tile(blockIdx.x, tiles * a.splits), sp = unit / tiles;
+    int mt, nt;
+    group_tile(unit - sp * tiles, a.tiles_m, a.tiles_n, a.group, mt, nt);
+    const int64_t m0 = (int64_t)mt * 32 * MB, n0 = (int64_t)nt * 256;
+    const int s0 = (int)((int64_t)a.steps * sp / a.splits), s1 = (int)((int64_t)a.steps * (sp + 1) / a.splits);
+    floatx16 acc[2][MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
+    G::run(a.r, a.c, m0, n0, a.rk, a.ck, a.per, a.planes, s0, s1, smem, wave, lane, acc);
+    const int64_t n = n0 + 64 * wave + 4 * (lane & 15);
+    const float f = a.part ? 1.0f : a.factor[0];
+    float* part = a.part ? a.part + (int64_t)sp * a.M * a.ldp : nullptr;
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+        tile_rows(smem + wave * kTileEpi, acc[0][i], acc[1][i], lane, [&](float v, int) { return v; },
+                  [&](int row, int, f32x4 v) {
+                      const int64_t m = m0 + 32 * i + row;
+                      if (m >= a.M) return;
+                      if (part) {
+                          if (n >= a.ldp) return;
+                          f32x4* d = reinterpret_cast<f32x4*>(part + m * a.ldp + n);
+                          *d = a.add ? *d + v : v;
+                      } else {
+                          tile_store4<DT>(a.out, m * a.N, n, a.N, a.vec, v * f);
+                      }
+                  });
+}
+
+// out = factor * sum of the partials, in their order.
+template <int DT>
+__global__ void __launch_bounds__(256) ce_sum_kernel(const float* part, int parts, int64_t stride, int64_t rows, int64_t N,
+                                                     int64_t ldp, const float* factor, void* out, int vec) {
+    const float f = factor[0];
+    const int64_t per = ldp / 4, total = rows * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / per, n = (i - m * per) * 4;
+        const f32x4* p = reinterpret_cast<const f32x4*>(part + m * ldp + n);
+        f32x4 v = p[0];
+        for (int s = 1; s < parts; ++s) v += p[s * (stride / 4)];
+        tile_store4<DT>(out, m * N, n, N, vec, v * f);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// plan and launches
+// ---------------------------------------------------------------------------
+// Units of a product over `slots` workgroups at a time: the split of k with the
+// least rounds of work, a little for each partial that is written and read.
+static int ce_splits(int64_t tiles, int64_t steps) {
+    const int64_t slots = 2 * (int64_t)device_cus();
+    int best = 1;
+    double cost = 1e300;
+    for (int s = 1; s <= 16 && s <= steps; ++s) {
+        const int64_t rounds = (tiles * s + slots - 1) / slots;
+        const double c = (double)rounds * ((double)(steps + s - 1) / s + 8) + (s > 1 ? 4.0 * s * tiles / slots + 8 : 0.0);
+        if (c < cost) {
+            cost = c;
+            best = s;
+        }
+    }
+    return best;
+}
+
+// Classes of a piece: dz within kCePiece bytes, whole tiles, pieces alike.
+constexpr int64_t kCePiece = 1LL << 30;
+
+CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool backward) {
+    CePlan p = {};
+    const int planes = dt == RPFQ_F32 ? 3 : 1;
+    p.ldk = planes == 3 ? (D + 31) & ~(int64_t)31 : (D + 7) & ~(int64_t)7;
+    p.pad = planes == 3 || D % 8 != 0;
+    auto take = [&](int64_t n) {
+        const size_t at = p.bytes;
+        p.bytes += ((size_t)n + 255) & ~(size_t)255;
+        return at;
+    };
+    if (p.pad) {
+        p.x_at = take(2 * planes * M * p.ldk);
+        p.w_at = take(2 * planes * V * p.ldk);
+    }
+    p.tiles_v = (V + 255) / 256;
+    if (!backward) {
+        p.part_at = take(8 * p.tiles_v * M);
+        p.zsum_at = take(4 * p.tiles_v * M);
+        p.zt_at = take(4 * M);
+        p.rows_at = take(reduction ? 4 * M : 0);
+        return p;
+    }
+    if (!p.pad) p.x_at = take(2 * M * p.ldk);  // x without its ignored rows
+    p.rho_at = take(4 * M);
+    p.factor_at = take(4);
+    const int64_t fit = std::max<int64_t>(1, kCePiece / (2 * planes * M * 256));
+    p.pieces = (p.tiles_v + fit - 1) / fit;
+    p.piece = (p.tiles_v + p.pieces - 1) / p.pieces * 256;  // classes
+    if (p.piece > V) p.piece = (V + 7) & ~(int64_t)7;
+    p.dz_at = take(2 * planes * M * p.piece);
+    p.tiles_m = (M + 127) / 128;
+    p.col_at = take(4 * (M + 31) / 32 * p.piece);
+    // float32 partials, rows of whole 16 bytes
+    p.ldp = (D + 3) & ~(int64_t)3;
+    const int64_t tn = (D + 255) / 256, pairs = planes == 3 ? kPairs32 : 1;
+    p.dx_splits = ce_splits(p.tiles_m * tn, pairs * ((p.piece + 31) / 32));
+    p.dx_at = take(p.dx_splits > 1 || p.pieces > 1 ? 4 * p.dx_splits * M * p.ldp : 0);
+    p.dw_splits = ce_splits((p.piece + 127) / 128 * tn, pairs * ((M + 31) / 32));
+    p.dw_at = take(p.dw_splits > 1 ? 4 * p.dw_splits * p.piece * p.ldp : 0);
+    return p;
+}
+
+static unsigned blocks_of(int64_t n) { return (unsigned)(n < 1 ? 1 : n > 16384 ? 16384 : n); }
+
+// The operands of the logits: as they are, or padded / split copies in `work`.
+// target: rows of x that it ignores are zero (backward).
+static hipError_t ce_operands(const CePlan& p, int dt, const void* x, const void* w, int64_t M, int64_t V, int64_t D,
+                              char* wk, CeArgs& a, hipStream_t s) {
+    a.kb = 2 * p.ldk;
+    a.per = (int)((a.kb + 63) / 64);
+    a.planes = dt == RPFQ_F32;
+    a.x = {reinterpret_cast<const char*>(x), a.kb, 0, M};
+    a.w = {reinterpret_cast<const char*>(w), a.kb, 0, V};
+    if (!p.pad) return hipSuccess;
+    const void* src[2] = {x, w};
+    const int64_t rows[2] = {M, V};
+    const size_t at[2] = {p.x_at, p.w_at};
+    TileOperand* op[2] = {&a.x, &a.w};
+    for (int i = 0; i < 2; ++i) {
+        const int64_t total = rows[i] * (p.ldk / 8);
+        uint16_t* d = reinterpret_cast<uint16_t*>(wk + at[i]);
+        if (dt == RPFQ_F32)
+            hipLaunchKernelGGL(ce_planes_kernel, dim3(blocks_of((total + 255) / 256)), dim3(256), 0, s,
+                               reinterpret_cast<const float*>(src[i]), rows[i], D, (const int64_t*)nullptr, (int64_t)0, d, p.ldk);
+        else
+            hipLaunchKernelGGL(ce_rows_kernel, dim3(blocks_of((total + 255) / 256)), dim3(256), 0, s,
+                               reinterpret_cast<const uint16_t*>(src[i]), D, (const int64_t*)nullptr, (int64_t)0, d, p.ldk,
+                               total);
+        op[i]->p = reinterpret_cast<const char*>(d);
+        op[i]->plane = 2 * rows[i] * p.ldk;
+    }
+    return hipGetLastError();
+}
+
+template <class K>
+static hipError_t ce_lds(K kernel, int bytes, std::atomic<uint64_t>& done) {
+    return set_lds_attr_once(reinterpret_cast<const void*>(kernel), bytes, done);
+}
+
+template <int MB, class Mma>
+static hipError_t stats_go(CeArgs& a, hipStream_t s) {
+    using G = TileGemm<MB, false, false, Mma>;
+    static std::atomic<uint64_t> done{0};
+    const hipError_t e = ce_lds(&ce_stats_kernel<MB, Mma>, G::LDS, done);
+    if (e != hipSuccess) return e;
+    a.tiles_m = (int)((a.M + 32 * MB - 1) / (32 * MB));
+    a.tiles_n = (int)((a.w.count + 255) / 256);
+    a.group = tile_group(a.tiles_n, 256 * a.kb);
+    hipLaunchKernelGGL((ce_stats_kernel<MB, Mma>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(256), G::LDS, s, a);
+    return hipGetLastError();
+}
+
+template <class Mma>
+static hipError_t stats_mb(CeArgs& a, hipStream_t s) {
+    return a.M <= 32 ? stats_go<1, Mma>(a, s) : a.M <= 64 ? stats_go<2, Mma>(a, s) : stats_go<4, Mma>(a, s);
+}
+
+template <int MB, class Mma, int DT>
+static hipError_t dz_go(CeArgs& a, hipStream_t s) {
+    using G = TileGemm<MB, false, false, Mma>;
+    static std::atomic<uint64_t> done{0};
+    const hipError_t e = ce_lds(&ce_dz_kernel<MB, Mma, DT>, G::LDS, done);
+    if (e != hipSuccess) return e;
+    a.tiles_m = (int)((a.M + 32 * MB - 1) / (32 * MB));
+    a.tiles_n = (int)((a.w.count + 255) / 256);
+    a.group = tile_group(a.tiles_n, 256 * a.kb);
+    hipLaunchKernelGGL((ce_dz_kernel<MB, Mma, DT>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(256), G::LDS, s, a);
+    return hipGetLastError();
+}
+
+template <class Mma, int DT>
+static hipError_t dz_mb(CeArgs& a, hipStream_t s) {
+    return a.M <= 32 ? dz_go<1, Mma, DT>(a, s) : a.M <= 64 ? dz_go<2, Mma, DT>(a, s) : dz_go<4, Mma, DT>(a, s);
+}
+
+template <bool RT, class Mma, int DT>
+static hipError_t grad_go(CeGrad& a, hipStream_t s) {
+    using G = TileGemm<4, RT, true, Mma>;
+    static std::atomic<uint64_t> done{0};
+    const hipError_t e = ce_lds(&ce_grad_kernel<RT, Mma, DT>, G::LDS, done);
+    if (e != hipSuccess) return e;
+    a.tiles_m = (int)((a.M + 127) / 128);
+    a.tiles_n = (int)((a.N + 255) / 256);
+    a.group = a.tiles_n;
+    hipLaunchKernelGGL((ce_grad_kernel<RT, Mma, DT>), dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)), dim3(256), G::LDS, s,
+                       a);
+    return hipGetLastError();
+}
+
+static hipError_t ce_sum(int dt, const float* part, int parts, int64_t stride, int64_t rows, int64_t N, int64_t ldp,
+                         const float* factor, void* out, hipStream_t s) {
+    const int es = dt == RPFQ_F32 ? 4 : 2;
+    const int vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * es) == 0;
+    const dim3 grid(blocks_of((rows * (ldp / 4) + 255) / 256));
+    switch (dt) {
+        case RPFQ_F32:
+            hipLaunchKernelGGL(ce_sum_kernel<RPFQ_F32>, grid, dim3(256), 0, s, part, parts, stride, rows, N, ldp, factor, out, vec);
+            break;
+        case RPFQ_F16:
+            hipLaunchKernelGGL(ce_sum_kernel<RPFQ_F16>, grid, dim3(256), 0, s, part, parts, stride, rows, N, ldp, factor, out, vec);
+            break;
+        default:
+            hipLaunchKernelGGL(ce_sum_kernel<RPFQ_BF16>, grid, dim3(256), 0, s, part, parts, stride, rows, N, ldp, factor, out, vec);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_linear_ce(const CeCall& c, float* loss, float* stat, float* coef, void* work, hipStream_t s) {
+    const CePlan p = ce_plan(c.dtype, c.M, c.V, c.D, c.reduction, false);
+    char* wk = reinterpret_cast<char*>(work);
+    CeArgs a = {};
+    hipError_t e = ce_operands(p, c.dtype, c.x, c.w, c.M, c.V, c.D, wk, a, s);
+    if (e != hipSuccess) return e;
+    a.bias = c.bias;
+    a.bias_dt = c.bias_dtype;
+    a.target = c.target;
+    a.M = c.M;
+    a.V = c.V;
+    a.smooth = c.smooth;
+    a.part = reinterpret_cast<float2*>(wk + p.part_at);
+    a.zsum = c.smooth > 0.0f ? reinterpret_cast<float*>(wk + p.zsum_at) : nullptr;
+    a.zt = reinterpret_cast<float*>(wk + p.zt_at);
+    e = c.dtype == RPFQ_F16 ? stats_mb<MmaF16>(a, s) : stats_mb<MmaBf16>(a, s);
+    if (e != hipSuccess) return e;
+    float* rows = c.reduction ? reinterpret_cast<float*>(wk + p.rows_at) : loss;
+    const CeJoin j = {a.part, a.zsum, a.zt, c.target, c.M, c.V, c.ignore, (int)p.tiles_v, c.smooth, stat, rows};
+    hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)((c.M + 15) / 16)), dim3(256), 0, s, j);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if (c.reduction) {
+        hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(1024), 0, s, rows, c.target, c.M, c.ignore, c.reduction, loss, coef);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float* coef, const float* grad, void* gx, void* gw,
+                                 void* gb, void* work, hipStream_t s) {
+    const CePlan p = ce_plan(c.dtype, c.M, c.V, c.D, c.reduction, true);
+    char* wk = reinterpret_cast<char*>(work);
+    const int planes = c.dtype == RPFQ_F32 ? 3 : 1;
+    const int es = c.dtype == RPFQ_F32 ? 4 : 2;
+    CeArgs a = {};
+    hipError_t e = ce_operands(p, c.dtype, c.x, c.w, c.M, c.V, c.D, wk, a, s);
+    if (e != hipSuccess) return e;
+    float* rho = reinterpret_cast<float*>(wk + p.rho_at);
+    float* factor = reinterpret_cast<float*>(wk + p.factor_at);
+    const float scale = c.dtype == RPFQ_F16 ? 32768.0f : 1.0f;
+    hipLaunchKernelGGL(ce_rho_kernel, dim3(1), dim3(1024), 0, s, grad, coef, c.target, c.M, c.V, c.ignore, c.reduction,
+                       1.0f / scale, rho, factor);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    // x for dw: its ignored rows as zeros
+    TileOperand xz = a.x;
+    if (gw) {
+        uint16_t* d = reinterpret_cast<uint16_t*>(wk + p.x_at);
+        const int64_t total = c.M * (p.ldk / 8);
+        const dim3 grid(blocks_of((total + 255) / 256));
+        if (planes == 3)
+            hipLaunchKernelGGL(ce_planes_kernel, grid, dim3(256), 0, s, reinterpret_cast<const float*>(c.x), c.M, c.D, c.target,
+                               c.ignore, d, p.ldk);
+        else
+            hipLaunchKernelGGL(ce_rows_kernel, grid, dim3(256), 0, s, reinterpret_cast<const uint16_t*>(c.x), c.D, c.target,
+                               c.ignore, d, p.ldk, total);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        xz.p = reinterpret_cast<const char*>(d);
+        xz.plane = 2 * c.M * p.ldk;
+        a.x = xz;  // the logits of ignored rows are not looked at
+    }
+    a.bias = c.bias;
+    a.bias_dt = c.bias_dtype;
+    a.target = c.target;
+    a.M = c.M;
+    a.V = c.V;
+    a.smooth = c.smooth;
+    a.stat = stat;
+    a.rho = rho;
+    a.dz_scale = scale;
+    a.dz = wk + p.dz_at;
+    a.colsum = gb ? reinterpret_cast<float*>(wk + p.col_at) : nullptr;
+    const TileOperand w = a.w;
+    float* dxp = p.dx_splits > 1 || p.pieces > 1 ? reinterpret_cast<float*>(wk + p.dx_at) : nullptr;
+    for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
+        const int64_t n = std::min(p.piece, c.V - v0);
+        a.v0 = v0;
+        a.w.p = w.p + v0 * w.ld;
+        a.w.count = n;
+        a.ldz = 2 * ((n + 7) & ~(int64_t)7);
+        a.dz_plane = c.M * a.ldz;
+        e = c.dtype == RPFQ_F16 ? dz_mb<MmaF16, RPFQ_F16>(a, s)
+            : c.dtype == RPFQ_BF16 ? dz_mb<MmaBf16, RPFQ_BF16>(a, s) : dz_mb<MmaBf16, RPFQ_F32>(a, s);
+        if (e != hipSuccess) return e;
+        const TileOperand dzk = {a.dz, a.ldz, a.dz_plane, c.M}, dzt = {a.dz, a.ldz, a.dz_plane, n};
+        if (gx) {
+            CeGrad g = {};
+            g.r = dzk;
+            g.c = {a.w.p, w.ld, w.plane, p.ldk};
+            g.rk = a.ldz;
+            g.ck = n;
+            g.M = c.M;
+            g.N = c.D;
+            g.per = (int)((a.ldz + 63) / 64);
+            g.planes = a.planes;
+            g.steps = g.per * (g.planes ? kPairs32 : 1);
+            g.splits = p.dx_splits;
+            g.part = dxp;
+            g.ldp = p.ldp;
+            g.add = v0 > 0;
+            g.factor = factor;
+            g.out = gx;
+            g.vec = c.D % 4 == 0 && reinterpret_cast<uintptr_t>(gx) % (4 * es) == 0;
+            e = c.dtype == RPFQ_F16 ? grad_go<false, MmaF16, RPFQ_F16>(g, s)
+                : c.dtype == RPFQ_BF16 ? grad_go<false, MmaBf16, RPFQ_BF16>(g, s) : grad_go<false, MmaBf16, RPFQ_F32>(g, s);
+            if (e != hipSuccess) return e;
+        }
+        if (gw) {
+            CeGrad g = {};
+            g.r = dzt;
+            g.c = {xz.p, xz.ld, xz.plane, p.ldk};
+            g.rk = g.ck = c.M;
+            g.M = n;
+            g.N = c.D;
+            g.per = (int)((c.M + 31) / 32);
+            g.planes = a.planes;
+            g.steps = g.per * (g.planes ? kPairs32 : 1);
+            g.splits = p.dw_splits;
+            g.part = p.dw_splits > 1 ? reinterpret_cast<float*>(wk + p.dw_at) : nullptr;
+            g.ldp = p.ldp;
+            g.factor = factor;
+            g.out = reinterpret_cast<char*>(gw) + v0 * c.D * es;
+            g.vec = c.D % 4 == 0 && reinterpret_cast<uintptr_t>(g.out) % (4 * es) == 0;
+            e = c.dtype == RPFQ_F16 ? grad_go<true, MmaF16, RPFQ_F16>(g, s)
+                : c.dtype == RPFQ_BF16 ? grad_go<true, MmaBf16, RPFQ_BF16>(g, s) : grad_go<true, MmaBf16, RPFQ_F32>(g, s);
+            if (e != hipSuccess) return e;
+            if (g.part && (e = ce_sum(c.dtype, g.part, g.splits, n * p.ldp, n, c.D, p.ldp, factor, g.out, s)) != hipSuccess)
+                return e;
+        }
+        if (gb) {  // db: the column sums of the row tiles, as one row each
+            const int bs = c.bias_dtype == RPFQ_F32 ? 4 : 2;
+            e = ce_sum(c.bias_dtype, a.colsum, a.tiles_m, a.ldz / 2, 1, n, a.ldz / 2, factor,
+                       reinterpret_cast<char*>(gb) + v0 * bs, s);
+            if (e != hipSuccess) return e;
+        }
+    }
+    if (gx && dxp) return ce_sum(c.dtype, dxp, p.dx_splits, c.M * p.ldp, c.M, c.D, p.ldp, factor, gx, s);
+    return hipSuccess;
+}
+
+}  // namespace rpfq

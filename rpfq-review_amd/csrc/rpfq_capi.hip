@@ -80,6 +80,44 @@ int check_linear_f32(int64_t M, int64_t N, int64_t K) {
     return RPFQ_OK;
 }
 
+int check_ce(const rpfq_ce_desc* d) {
+    if (!d) return fail(RPFQ_ERR_NULL, "desc is NULL");
+    if (d->M <= 0 || d->V <= 0 || d->D <= 0)
+        return fail(RPFQ_ERR_SHAPE, "M=%lld V=%lld D=%lld must be positive", (long long)d->M, (long long)d->V, (long long)d->D);
+    if (d->M > (1LL << 22) || d->V > (1LL << 22) || d->D > (1LL << 16))
+        return fail(RPFQ_ERR_SHAPE, "M=%lld V=%lld exceed 2^22 or D=%lld 2^16", (long long)d->M, (long long)d->V, (long long)d->D);
+    if (!dtype_ok(d->dtype) || !dtype_ok(d->bias_dtype)) return fail(RPFQ_ERR_DTYPE, "unsupported dtype %d / %d", d->dtype, d->bias_dtype);
+    if (d->reduction < RPFQ_REDUCE_NONE || d->reduction > RPFQ_REDUCE_SUM) return fail(RPFQ_ERR_VALUE, "unknown reduction %d", d->reduction);
+    if (!(d->smoothing >= 0.0f && d->smoothing <= 1.0f)) return fail(RPFQ_ERR_VALUE, "smoothing %g is not within 0 .. 1", d->smoothing);
+    return RPFQ_OK;
+}
+
+int check_ce_operands(const rpfq_ce_desc* d, const void* x, const void* w, const void* bias, const void* work, size_t bytes,
+                      int backward) {
+    const size_t es = d->dtype == RPFQ_F32 ? 4 : 2;
+    if (!aligned(x, d->D % 8 == 0 ? 16 : es) || !aligned(w, d->D % 8 == 0 ? 16 : es) ||
+        (bias && !aligned(bias, d->bias_dtype == RPFQ_F32 ? 4 : 2)) || !aligned(work, 256))
+        return fail(RPFQ_ERR_ALIGN, "x and w must be 16-byte (D %% 8 == 0) and work 256-byte aligned");
+    const size_t need = rpfq_linear_cross_entropy_workspace_bytes(d, backward);
+    if (bytes < need) return fail(RPFQ_ERR_SHAPE, "workspace holds %zu bytes, need %zu", bytes, need);
+    return RPFQ_OK;
+}
+
+rpfq::CeCall ce_call(const rpfq_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* target) {
+    return {x, w, bias, d->dtype, d->bias_dtype, target, d->M, d->V, d->D, d->ignore_index, d->smoothing, d->reduction};
+}
+
+int check_int8(int64_t M, int64_t N, int64_t K, int x_dtype, int64_t ld_w) {
+    if (M <= 0 || N <= 0 || K <= 0)
+        return fail(RPFQ_ERR_SHAPE, "M=%lld N=%lld K=%lld must be positive", (long long)M, (long long)N, (long long)K);
+    if (M > (1LL << 30) || N > (1LL << 24) || K > 131072)
+        return fail(RPFQ_ERR_SHAPE, "M=%lld exceeds 2^30, N=%lld 2^24 or K=%lld 131072", (long long)M, (long long)N, (long long)K);
+    if ((M + 31) / 32 * ((N + 255) / 256) > (1LL << 30)) return fail(RPFQ_ERR_SHAPE, "M=%lld N=%lld: too many tiles", (long long)M, (long long)N);
+    if (!dtype_ok(x_dtype) && x_dtype != RPFQ_I8) return fail(RPFQ_ERR_DTYPE, "unsupported x dtype %d", x_dtype);
+    if (ld_w < K || ld_w > (1LL << 20)) return fail(RPFQ_ERR_SHAPE, "ld_w=%lld must be K=%lld .. 2^20", (long long)ld_w, (long long)K);
+    return RPFQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -720,6 +758,117 @@ int rpfq_linear_f32_grad(const float* grad_y, const float* x, const float* w, in
     return hip_status(rpfq::launch_linear_f32_grad(grad_y, x, w, M, N, K, w_parts, n_parts, x_scale, grad_x, grad_w,
                                                    grad_b, work, reinterpret_cast<hipStream_t>(stream)),
                       "rpfq_linear_f32_grad");
+}
+
+int rpfq_quantize_int8(const void* x, int x_dtype, int64_t M, int64_t K, int8_t* codes, int64_t ld_codes, float* scale,
+                       void* stream) {
+    if (!x || !codes || !scale) return fail(RPFQ_ERR_NULL, "rpfq_quantize_int8: NULL pointer argument");
+    if (!dtype_ok(x_dtype)) return fail(RPFQ_ERR_DTYPE, "unsupported x dtype %d", x_dtype);
+    if (M <= 0 || K <= 0 || M > (1LL << 30) || K > (1LL << 30))
+        return fail(RPFQ_ERR_SHAPE, "M=%lld K=%lld must be 1 .. 2^30", (long long)M, (long long)K);
+    if (ld_codes < K || ld_codes > (1LL << 30)) return fail(RPFQ_ERR_SHAPE, "ld_codes=%lld must be K .. 2^30", (long long)ld_codes);
+    if (!aligned(x, x_dtype == RPFQ_F32 ? 4 : 2) || !aligned(scale, 4)) return fail(RPFQ_ERR_ALIGN, "x and scale must be aligned to their elements");
+    return hip_status(rpfq::launch_quantize_int8(x, x_dtype, M, K, codes, ld_codes, scale, reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_quantize_int8");
+}
+
+size_t rpfq_linear_int8_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t N, int64_t K, const int8_t* w,
+                                        int64_t ld_w) {
+    if (check_int8(M, N, K, x_dtype, ld_w) != RPFQ_OK) return 0;
+    const bool copy_x = x_dtype != RPFQ_I8 || rpfq::int8_pads(reinterpret_cast<const int8_t*>(x), K, K);
+    return rpfq::int8_plan(M, N, K, copy_x, rpfq::int8_pads(w, ld_w, K)).bytes;
+}
+
+int rpfq_linear_int8(const void* x, int x_dtype, const float* x_scale, const int8_t* w, int64_t ld_w, const float* w_scale,
+                     const float* bias, int64_t M, int64_t N, int64_t K, void* y, int y_dtype, void* work,
+                     size_t work_bytes, void* stream) {
+    int rc = check_int8(M, N, K, x_dtype, ld_w);
+    if (rc) return rc;
+    if (!x || !w || !w_scale || !y) return fail(RPFQ_ERR_NULL, "rpfq_linear_int8: NULL pointer argument");
+    if ((x_dtype == RPFQ_I8) != (x_scale != nullptr)) return fail(RPFQ_ERR_NULL, "x_scale goes with int8 x, and only with it");
+    if (!dtype_ok(y_dtype)) return fail(RPFQ_ERR_DTYPE, "unsupported y dtype %d", y_dtype);
+    const size_t xs = x_dtype == RPFQ_I8 ? 1 : x_dtype == RPFQ_F32 ? 4 : 2, ys = y_dtype == RPFQ_F32 ? 4 : 2;
+    if (!aligned(x, xs) || !aligned(y, ys) || !aligned(w_scale, 4) || !aligned(bias, 4) || !aligned(x_scale, 4) || !aligned(work, 256))
+        return fail(RPFQ_ERR_ALIGN, "operands must be aligned to their elements and work to 256 bytes");
+    const size_t need = rpfq_linear_int8_workspace_bytes(x, x_dtype, M, N, K, w, ld_w);
+    if (need && !work) return fail(RPFQ_ERR_NULL, "rpfq_linear_int8: work is NULL");
+    if (work_bytes < need) return fail(RPFQ_ERR_SHAPE, "workspace holds %zu bytes, need %zu", work_bytes, need);
+    return hip_status(rpfq::launch_linear_int8(x, x_dtype == RPFQ_I8 ? -1 : x_dtype, x_scale, w, ld_w, w_scale, bias, M, N, K, y,
+                                               y_dtype, work, reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_linear_int8");
+}
+
+size_t rpfq_linear_cross_entropy_workspace_bytes(const rpfq_ce_desc* d, int backward) {
+    if (check_ce(d) != RPFQ_OK) return 0;
+    return rpfq::ce_plan(d->dtype, d->M, d->V, d->D, d->reduction, backward != 0).bytes;
+}
+
+int rpfq_linear_cross_entropy(const rpfq_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* target,
+                              float* loss, float* stat, float* coef, void* work, size_t work_bytes, void* stream) {
+    int rc = check_ce(d);
+    if (rc) return rc;
+    if (!x || !w || !target || !loss || !stat || !coef || !work)
+        return fail(RPFQ_ERR_NULL, "rpfq_linear_cross_entropy: NULL pointer argument");
+    if ((rc = check_ce_operands(d, x, w, bias, work, work_bytes, 0))) return rc;
+    return hip_status(rpfq::launch_linear_ce(ce_call(d, x, w, bias, target), loss, stat, coef, work,
+                                             reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_linear_cross_entropy");
+}
+
+int rpfq_linear_cross_entropy_grad(const rpfq_ce_desc* d, const void* x, const void* w, const void* bias,
+                                   const int64_t* target, const float* stat, const float* coef, const float* grad_loss,
+                                   void* grad_x, void* grad_w, void* grad_bias, void* work, size_t work_bytes, void* stream) {
+    int rc = check_ce(d);
+    if (rc) return rc;
+    if (!x || !w || !target || !stat || !coef || !grad_loss || !work || (!grad_x && !grad_w && !grad_bias))
+        return fail(RPFQ_ERR_NULL, "rpfq_linear_cross_entropy_grad: NULL pointer argument");
+    if ((rc = check_ce_operands(d, x, w, bias, work, work_bytes, 1))) return rc;
+    const size_t es = d->dtype == RPFQ_F32 ? 4 : 2;
+    if (!aligned(grad_x, es) || !aligned(grad_w, es) || !aligned(grad_bias, d->bias_dtype == RPFQ_F32 ? 4 : 2))
+        return fail(RPFQ_ERR_ALIGN, "gradients must be aligned to their elements");
+    return hip_status(rpfq::launch_linear_ce_grad(ce_call(d, x, w, bias, target), stat, coef, grad_loss, grad_x, grad_w, grad_bias,
+                                                  work, reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_linear_cross_entropy_grad");
+}
+
+int rpfq_adamw(const rpfq_adamw_tensor* tensors, int64_t count, int dtype, int state_bits, const rpfq_adamw_hyper* h,
+               float* step, const float* lr_device, const float* grad_scale, const float* found_inf, float* work,
+               void* stream) {
+    if (!h || !step || !work || (!tensors && count)) return fail(RPFQ_ERR_NULL, "rpfq_adamw: NULL pointer argument");
+    if (count < 0) return fail(RPFQ_ERR_SHAPE, "count=%lld must not be negative", (long long)count);
+    if (!dtype_ok(dtype)) return fail(RPFQ_ERR_DTYPE, "unsupported dtype %d", dtype);
+    if (state_bits != 8 && state_bits != 32) return fail(RPFQ_ERR_BITS, "state_bits=%d must be 8 or 32", state_bits);
+    if (!(h->lr >= 0.0) || !(h->eps >= 0.0) || !(h->weight_decay >= 0.0) || !(h->beta1 >= 0.0 && h->beta1 < 1.0) ||
+        !(h->beta2 >= 0.0 && h->beta2 < 1.0))
+        return fail(RPFQ_ERR_VALUE, "lr, eps, weight_decay must not be negative, betas within 0 .. 1");
+    const size_t es = dtype == RPFQ_F32 ? 4 : 2, ss = state_bits == 32 ? 4 : 1;
+    for (int64_t i = 0; i < count; ++i) {
+        const rpfq_adamw_tensor& t = tensors[i];
+        if (t.numel < 0 || t.numel > (1LL << 40)) return fail(RPFQ_ERR_SHAPE, "tensor %lld: numel=%lld", (long long)i, (long long)t.numel);
+        if (t.numel == 0) continue;
+        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return fail(RPFQ_ERR_NULL, "tensor %lld: NULL pointer", (long long)i);
+        if ((state_bits == 8) != (t.exp_avg_scale && t.exp_avg_sq_scale) || (!t.exp_avg_scale) != (!t.exp_avg_sq_scale))
+            return fail(RPFQ_ERR_NULL, "tensor %lld: scales go with 8-bit states, and only with them", (long long)i);
+        if (!aligned(t.param, es) || !aligned(t.grad, es) || !aligned(t.exp_avg, ss) || !aligned(t.exp_avg_sq, ss) ||
+            !aligned(t.exp_avg_scale, 4) || !aligned(t.exp_avg_sq_scale, 4))
+            return fail(RPFQ_ERR_ALIGN, "tensor %lld is not aligned to its elements", (long long)i);
+    }
+    return hip_status(rpfq::launch_adamw(tensors, count, dtype, state_bits, *h, step, lr_device, grad_scale, found_inf, work,
+                                         reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_adamw");
+}
+
+int rpfq_adamw_state_values(const void* const* codes, const float* const* scales, const int64_t* numel, const int* second,
+                            float* const* out, int64_t count, void* stream) {
+    if (count < 0) return fail(RPFQ_ERR_SHAPE, "count=%lld must not be negative", (long long)count);
+    if (count && (!codes || !scales || !numel || !second || !out)) return fail(RPFQ_ERR_NULL, "rpfq_adamw_state_values: NULL pointer argument");
+    for (int64_t i = 0; i < count; ++i) {
+        if (numel[i] < 0 || numel[i] > (1LL << 40)) return fail(RPFQ_ERR_SHAPE, "tensor %lld: numel=%lld", (long long)i, (long long)numel[i]);
+        if (numel[i] && (!codes[i] || !scales[i] || !out[i])) return fail(RPFQ_ERR_NULL, "tensor %lld: NULL pointer", (long long)i);
+        if (!aligned(scales[i], 4) || !aligned(out[i], 4)) return fail(RPFQ_ERR_ALIGN, "tensor %lld is not aligned to its elements", (long long)i);
+    }
+    return hip_status(rpfq::launch_adamw_values(codes, scales, numel, second, out, count, reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_adamw_state_values");
 }
 
 }  // extern "C"

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../../include/rpfq.h"
@@ -371,6 +372,51 @@ hipError_t launch_linear_f32(const float* x, const float* w, const float* bias, 
 hipError_t launch_linear_f32_grad(const float* gy, const float* x, const float* w, int64_t M, int64_t N, int64_t K,
                                   const float* parts, int nparts, const float* xscale, float* gx, float* gw, float* gb,
                                   void* work, hipStream_t s);
+// 8-bit integer layer (int8_linear.hip): offsets in its workspace.  Codes are
+// read in place where rows of ld bytes are 16-byte aligned and hold whole
+// 16-byte pieces, else from a padded copy.
+struct Int8Plan {
+    int64_t ld;  // row bytes of codes in the workspace
+    size_t x_at, sx_at, w_at, bytes;
+};
+inline bool int8_pads(const void* codes, int64_t ld, int64_t K) {
+    return K % 16 != 0 || ld % 16 != 0 || reinterpret_cast<uintptr_t>(codes) % 16 != 0;
+}
+Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, bool quantize, bool pad_w);
+hipError_t launch_quantize_int8(const void* x, int dt, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale,
+                                hipStream_t s);
+// xdt < 0: x holds codes and sx their scales
+hipError_t launch_linear_int8(const void* x, int xdt, const float* sx, const int8_t* w, int64_t ldw, const float* sw,
+                              const float* bias, int64_t M, int64_t N, int64_t K, void* y, int ydt, void* work,
+                              hipStream_t s);
+// cross entropy of a linear classifier (linear_ce.hip)
+struct CeCall {
+    const void *x, *w, *bias;  // [M, D], [V, D], [V] or NULL
+    int dtype, bias_dtype;
+    const int64_t* target;
+    int64_t M, V, D, ignore;
+    float smooth;
+    int reduction;  // 0 none, 1 mean, 2 sum
+};
+struct CePlan {
+    int64_t ldk, ldp;       // elements of a row of k; of float32 partials
+    bool pad;               // x and w are copied (rows of ldk, or three planes of them)
+    int64_t tiles_v, tiles_m, piece, pieces;
+    int dx_splits, dw_splits;
+    size_t x_at, w_at, part_at, zsum_at, zt_at, rows_at, rho_at, factor_at, dz_at, col_at, dx_at, dw_at, bytes;
+};
+CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool backward);
+hipError_t launch_linear_ce(const CeCall& c, float* loss, float* stat, float* coef, void* work, hipStream_t s);
+hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float* coef, const float* grad, void* gx, void* gw,
+                                 void* gb, void* work, hipStream_t s);
+// AdamW (adamw.hip): tensors of one launch (their table is a kernel argument)
+constexpr int kAdamTensors = 60;
+using AdamTensor = rpfq_adamw_tensor;
+using AdamHyper = rpfq_adamw_hyper;
+hipError_t launch_adamw(const AdamTensor* t, int64_t count, int pdt, int bits, const AdamHyper& h, float* step,
+                        const float* lr_dev, const float* grad_scale, const float* found_inf, float* coef, hipStream_t s);
+hipError_t launch_adamw_values(const void* const* codes, const float* const* scales, const int64_t* numel,
+                               const int* second, float* const* out, int64_t count, hipStream_t s);
 // adjoint blob (rpfq_kernels.hip) and the grad_x kernel (wide_adjoint.hip)
 hipError_t launch_wide_pack_adjoint(const rpfq_wide_desc& d, const WideGeom& g, const void* packed, void* adjoint,
                                     hipStream_t s);

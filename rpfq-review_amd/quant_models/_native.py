@@ -26,7 +26,8 @@ ERRORS = {
     6: "RPFQ_ERR_VALUE",
     7: "RPFQ_ERR_HIP",
 }
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, I8 = 0, 1, 2, 3
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 CB_AXIS, CB_SIGN, CB_PSK16, CB_TABLE = 0, 1, 2, 3
 QK_AXIS, QK_SIGN = 0, 1  # weight quantizer kinds of rpfq_quantize_wide
 FLAG_TILE_M128 = 1  # force the register-staged 128-row kernel
@@ -83,6 +84,14 @@ EXPORTED = (
     "rpfq_linear_f32_workspace_bytes",
     "rpfq_linear_f32",
     "rpfq_linear_f32_grad",
+    "rpfq_quantize_int8",
+    "rpfq_linear_int8_workspace_bytes",
+    "rpfq_linear_int8",
+    "rpfq_linear_cross_entropy_workspace_bytes",
+    "rpfq_linear_cross_entropy",
+    "rpfq_linear_cross_entropy_grad",
+    "rpfq_adamw",
+    "rpfq_adamw_state_values",
 )
 
 
@@ -110,6 +119,31 @@ class QuantDesc(ctypes.Structure):
         ("kind", ctypes.c_int32 * 2),
         ("steps", ctypes.c_int32 * 2),
     ]
+
+
+class CeDesc(ctypes.Structure):
+    """Mirror of struct rpfq_ce_desc."""
+
+    _fields_ = [
+        ("M", ctypes.c_int64),
+        ("V", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("ignore_index", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("reduction", ctypes.c_int32),
+        ("smoothing", ctypes.c_float),
+    ]
+
+
+class AdamWHyper(ctypes.Structure):
+    """Mirror of struct rpfq_adamw_hyper."""
+
+    _fields_ = [(name, ctypes.c_double) for name in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+
+
+# fields of struct rpfq_adamw_tensor, all of 8 bytes
+ADAMW_FIELDS = 7
 
 
 class RPFQError(RuntimeError):
@@ -190,8 +224,20 @@ def load() -> ctypes.CDLL:
         lib.rpfq_linear_f32_workspace_bytes.restype = sz
         lib.rpfq_linear_f32.argtypes = [vp, vp, vp, i64, i64, i64, vp, i32, vp, vp, vp, sz, vp]
         lib.rpfq_linear_f32_grad.argtypes = [vp, vp, vp, i64, i64, i64, vp, i32, vp, vp, vp, vp, vp, sz, vp]
+        lib.rpfq_quantize_int8.argtypes = [vp, i32, i64, i64, vp, i64, vp, vp]
+        lib.rpfq_linear_int8_workspace_bytes.argtypes = [vp, i32, i64, i64, i64, vp, i64]
+        lib.rpfq_linear_int8_workspace_bytes.restype = sz
+        lib.rpfq_linear_int8.argtypes = [vp, i32, vp, vp, i64, vp, vp, i64, i64, i64, vp, i32, vp, sz, vp]
+        cp = ctypes.POINTER(CeDesc)
+        lib.rpfq_linear_cross_entropy_workspace_bytes.argtypes = [cp, i32]
+        lib.rpfq_linear_cross_entropy_workspace_bytes.restype = sz
+        lib.rpfq_linear_cross_entropy.argtypes = [cp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        lib.rpfq_linear_cross_entropy_grad.argtypes = [cp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        lib.rpfq_adamw.argtypes = [vp, i64, i32, i32, ctypes.POINTER(AdamWHyper), vp, vp, vp, vp, vp, vp]
+        lib.rpfq_adamw_state_values.argtypes = [vp, vp, vp, vp, vp, i64, vp]
         for name in EXPORTED[2:]:
-            if name not in ("rpfq_wide_packed_bytes", "rpfq_wide_adjoint_bytes", "rpfq_quantize_workspace_bytes",
+            if name not in ("rpfq_linear_int8_workspace_bytes", "rpfq_linear_cross_entropy_workspace_bytes",
+                            "rpfq_wide_packed_bytes", "rpfq_wide_adjoint_bytes", "rpfq_quantize_workspace_bytes",
                             "rpfq_linear_f32_workspace_bytes", "rpfq_wide_dense_bytes"):
                 getattr(lib, name).restype = i32
         _lib = lib
@@ -242,6 +288,32 @@ def host():
             module = False
         _host = module
     return _host or None
+
+
+class on_device:
+    """Makes t's device the current one for the launches inside, where it is
+    another (the launches and the library's queries go to the current one)."""
+
+    __slots__ = ("want", "was")
+
+    def __init__(self, t: torch.Tensor):
+        self.want = t.get_device()
+
+    def __enter__(self):
+        self.was = torch._C._cuda_getDevice()
+        if self.was != self.want:
+            torch._C._cuda_setDevice(self.want)
+
+    def __exit__(self, *exc):
+        if self.was != self.want:
+            torch._C._cuda_setDevice(self.was)
+
+
+def require_same_device(first: torch.Tensor, **others) -> None:
+    require_device(first, *others.values())
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, expected {first.device}")
 
 
 def require_device(*tensors: torch.Tensor) -> None:

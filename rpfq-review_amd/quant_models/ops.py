@@ -846,6 +846,266 @@ def linear_f32_grad(grad_y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, w_pa
     return gx, gw
 
 
+def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes int8 [..., K], scale float32 [...]) of the rows of x
+    (rpfq_quantize_int8): scale = max|row| / 127, codes = rint(127 x /
+    max|row|) with ties to even.  A row with inf or NaN has scale NaN.  For
+    the tokens and, on a weight [N, K], the output channels of linear_int8."""
+    N.require_device(x)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("quantize_int8 takes rows of at least one value")
+    k = x.shape[-1]
+    x2 = _aligned_rows(x.detach().reshape(-1, k))
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if x2.shape[0]:
+        with N.on_device(x):
+            N.check("rpfq_quantize_int8", N.load().rpfq_quantize_int8(
+                x2.data_ptr(), N.dtype_code(x2.dtype), x2.shape[0], k, codes.data_ptr(), k, scale.data_ptr(),
+                N.stream_of(x2)))
+    return codes, scale
+
+
+def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
+                out_dtype: torch.dtype | None = None, x_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """y = (codes of x) weight^T, times each token's and each channel's scale,
+    plus bias, on [..., K] -> [..., N] (rpfq_linear_int8): the products and
+    sums exact in integers, the rest float32 rounded once to out_dtype
+    (default x.dtype).  x: float32, fp16 or bf16, quantized per token within
+    the call as quantize_int8 does, or int8 codes with their x_scale [...]
+    (out_dtype then says what y is).  weight int8 [N, K] (rows may be wider
+    apart: multiples of 16 bytes, K too, are read in place), weight_scale
+    float32 [N].  K <= 131072.  No gradient."""
+    N.require_same_device(x, weight=weight, weight_scale=weight_scale, bias=bias, x_scale=x_scale)
+    if weight.dtype != torch.int8 or weight.dim() != 2:
+        raise ValueError("weight must be int8 [N, K]")
+    n, k = weight.shape
+    if x.dim() == 0 or x.shape[-1] != k:
+        raise ValueError(f"expected last dim {k}, got {tuple(x.shape)}")
+    if weight_scale.shape != (n,) or weight_scale.dtype != torch.float32:
+        raise ValueError(f"weight_scale must be float32 of shape ({n},)")
+    if bias is not None and bias.shape != (n,):
+        raise ValueError(f"bias must have shape ({n},)")
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad()")
+    codes = x.dtype == torch.int8
+    if codes and (x_scale is None or out_dtype is None):
+        raise ValueError("int8 x takes its x_scale and an out_dtype")
+    if not codes and x_scale is not None:
+        raise ValueError("x_scale goes with int8 x")
+    if codes and (x_scale.shape != x.shape[:-1] or x_scale.dtype != torch.float32):
+        raise ValueError(f"x_scale must be float32 of shape {tuple(x.shape[:-1])}")
+    out_dtype = out_dtype or x.dtype
+    y = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=x.device)
+    ydt, xdt = N.dtype_code(out_dtype), N.I8 if codes else N.dtype_code(x.dtype)
+    if y.numel() == 0:
+        return y
+    x2 = _aligned_rows(x.reshape(-1, k))
+    m = x2.shape[0]
+    if weight.stride(1) != 1 and k > 1 or weight.stride(0) < k:
+        weight = weight.contiguous()
+    weight_scale = weight_scale.contiguous()
+    bias = None if bias is None else bias.detach().float().contiguous()
+    x_scale = None if x_scale is None else x_scale.contiguous()
+    lib = N.load()
+    ld = weight.stride(0) if n > 1 else max(k, weight.stride(0))
+    nwork = lib.rpfq_linear_int8_workspace_bytes(x2.data_ptr(), xdt, m, n, k, weight.data_ptr(), ld)
+    work = torch.empty(nwork, dtype=torch.uint8, device=x.device) if nwork else None
+    with N.on_device(x):
+        N.check("rpfq_linear_int8", lib.rpfq_linear_int8(
+            x2.data_ptr(), xdt, N.ptr(x_scale), weight.data_ptr(), ld, weight_scale.data_ptr(), N.ptr(bias), m, n, k,
+            y.data_ptr(), ydt, N.ptr(work), nwork, N.stream_of(x2)))
+    return y
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, ignore_index, smoothing, reduction):
+        m, d = x.shape
+        v = weight.shape[0]
+        desc = N.CeDesc(m, v, d, ignore_index, N.dtype_code(x.dtype),
+                        N.F32 if bias is None else N.dtype_code(bias.dtype), N.REDUCTIONS[reduction], smoothing)
+        stat = torch.empty(2 * m + 1, dtype=torch.float32, device=x.device)  # and the mean's factor
+        loss = torch.empty(m if reduction == "none" else (), dtype=torch.float32, device=x.device)
+        lib = N.load()
+        nwork = lib.rpfq_linear_cross_entropy_workspace_bytes(ctypes.byref(desc), 0)
+        if nwork == 0:
+            N.check("rpfq_linear_cross_entropy_workspace_bytes", 2)
+        work = torch.empty(nwork, dtype=torch.uint8, device=x.device)
+        with N.on_device(x):
+            N.check("rpfq_linear_cross_entropy", lib.rpfq_linear_cross_entropy(
+                ctypes.byref(desc), x.data_ptr(), weight.data_ptr(), N.ptr(bias), target.data_ptr(), loss.data_ptr(),
+                stat.data_ptr(), stat.data_ptr() + 8 * m, work.data_ptr(), nwork, N.stream_of(x)))
+        ctx.desc = desc
+        ctx.save_for_backward(x, weight, bias, target, stat)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, bias, target, stat = ctx.saved_tensors
+        desc = ctx.desc
+        want = ctx.needs_input_grad
+        gx = torch.empty_like(x) if want[0] else None
+        gw = torch.empty_like(weight) if want[1] else None
+        gb = torch.empty_like(bias) if bias is not None and want[2] else None
+        if gx is None and gw is None and gb is None:
+            return (None,) * 7
+        grad = grad.float().contiguous()
+        lib = N.load()
+        nwork = lib.rpfq_linear_cross_entropy_workspace_bytes(ctypes.byref(desc), 1)
+        work = torch.empty(nwork, dtype=torch.uint8, device=x.device)
+        with N.on_device(x):
+            N.check("rpfq_linear_cross_entropy_grad", lib.rpfq_linear_cross_entropy_grad(
+                ctypes.byref(desc), x.data_ptr(), weight.data_ptr(), N.ptr(bias), target.data_ptr(), stat.data_ptr(),
+                stat.data_ptr() + 8 * desc.M, grad.data_ptr(), N.ptr(gx), N.ptr(gw), N.ptr(gb), work.data_ptr(), nwork,
+                N.stream_of(x)))
+        return gx, gw, gb, None, None, None, None
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: torch.Tensor | None = None,
+                         *, ignore_index: int = -100, label_smoothing: float = 0.0,
+                         reduction: str = "mean") -> torch.Tensor:
+    """F.cross_entropy(F.linear(x, weight, bias), target) over V classes
+    without keeping the logits (rpfq_linear_cross_entropy and its gradient):
+    x [..., D], weight [V, D], bias [V], target int64 [...] -> float32 loss, a
+    scalar or [...] with reduction "none".  x and weight share a type (fp16,
+    bf16, float32); autocast casts them as it does for F.linear.  Rows with
+    target ignore_index have loss 0, no gradient and no share of the mean; a
+    target that is no class makes its row's loss and the gradients NaN.
+    Gradients of x, weight and bias, once differentiable; float32 sums in a
+    fixed order."""
+    N.require_same_device(x, weight=weight, target=target, bias=bias)
+    if reduction not in N.REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(N.REDUCTIONS)}, got {reduction!r}")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"label_smoothing must be within 0 .. 1, got {label_smoothing}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    v, d = weight.shape
+    if v == 0 or d == 0:
+        raise ValueError("weight must have at least one class and one feature")
+    if target.dtype != torch.int64 or target.shape != x.shape[:-1]:
+        raise ValueError(f"target must be int64 of shape {tuple(x.shape[:-1])}, got {target.dtype} {tuple(target.shape)}")
+    if bias is not None and bias.shape != (v,):
+        raise ValueError(f"bias must have shape ({v},)")
+    if torch.is_autocast_enabled("cuda"):
+        low = torch.get_autocast_dtype("cuda")
+        x, weight = x.to(low), weight.to(low)
+    if x.dtype != weight.dtype:
+        raise TypeError(f"x is {x.dtype}, weight {weight.dtype}: they must share a type")
+    for t in (x,) if bias is None else (x, bias):
+        N.dtype_code(t.dtype)
+    lead = target.shape
+    x2 = _aligned_rows(x.reshape(-1, d))
+    if x2.shape[0] == 0:  # as torch: the mean of nothing is NaN, its gradients zero
+        zero = x.float().sum() + 0.0 * weight[0, 0].float() + (0.0 if bias is None else 0.0 * bias[0].float())
+        zero = torch.where(torch.ones_like(zero, dtype=torch.bool), zero.new_zeros(()), zero)
+        return zero.expand(lead) if reduction == "none" else zero + math.nan if reduction == "mean" else zero
+    loss = _LinearCrossEntropy.apply(x2, _aligned_rows(weight), None if bias is None else bias.contiguous(),
+                                     target.reshape(-1).contiguous(), int(ignore_index), float(label_smoothing),
+                                     reduction)
+    return loss.reshape(lead) if reduction == "none" else loss
+
+
+# elements of an 8-bit optimizer state that share a scale
+STATE_BLOCK = 256
+
+
+def adamw(params, grads, exp_avgs, exp_avg_sqs, step: torch.Tensor, *, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+          weight_decay: float = 1e-2, exp_avg_scales=None, exp_avg_sq_scales=None,
+          grad_scale: torch.Tensor | None = None, found_inf: torch.Tensor | None = None) -> None:
+    """One AdamW step (decoupled weight decay) over lists of tensors, in place,
+    in one launch per 60 tensors (rpfq_adamw).  params and grads: contiguous,
+    of one type (float32, fp16, bf16); step: float32 device tensor of one
+    element, counted up by the call (so a captured step goes on when it is
+    replayed).  States: float32 exp_avgs and exp_avg_sqs of the parameters'
+    sizes, or 8-bit codes, int8 and uint8, with exp_avg_scales and
+    exp_avg_sq_scales: float32, one per 256 elements (new states: zeros).  lr:
+    a number, or a float32 device tensor that is read when the step runs.
+    grad_scale, found_inf: float32 device scalars, as torch.amp.GradScaler
+    passes them: gradients are divided by the one, a nonzero other leaves
+    parameters, states and step as they are.  The tensors must not overlap."""
+    params, grads, ms, vs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    n = len(params)
+    small = exp_avg_scales is not None
+    if small != (exp_avg_sq_scales is not None):
+        raise ValueError("8-bit states take both exp_avg_scales and exp_avg_sq_scales")
+    sm = list(exp_avg_scales) if small else []
+    sv = list(exp_avg_sq_scales) if small else []
+    if not len(grads) == len(ms) == len(vs) == n or small and not len(sm) == len(sv) == n:
+        raise ValueError("adamw: the lists must be of one length")
+    scalars = {"step": step, "grad_scale": grad_scale, "found_inf": found_inf}
+    lr_dev = lr if isinstance(lr, torch.Tensor) else None
+    scalars["lr"] = lr_dev
+    N.require_same_device(step, **scalars)
+    for name, t in scalars.items():
+        if t is not None and (t.dtype != torch.float32 or t.numel() != 1):
+            raise ValueError(f"{name} must be a float32 tensor of one element")
+    if n == 0:
+        raise ValueError("adamw: no tensors")
+    dtype, device = params[0].dtype, step.device
+    code = N.dtype_code(dtype)
+    mt, vt = (torch.int8, torch.uint8) if small else (torch.float32, torch.float32)
+    flat = []
+    for i, (p, g, m, v) in enumerate(zip(params, grads, ms, vs)):
+        size = p.numel()
+        if p.dtype != dtype or g.dtype != dtype or m.dtype != mt or v.dtype != vt:
+            raise TypeError(f"tensor {i}: parameters and gradients must be {dtype}, states {mt} and {vt}")
+        if g.shape != p.shape or m.numel() != size or v.numel() != size:
+            raise ValueError(f"tensor {i}: gradient or states do not have the parameter's size")
+        if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
+            raise ValueError(f"tensor {i}: parameters, gradients and states must be contiguous")
+        if not p.device == g.device == m.device == v.device == device:
+            raise ValueError(f"tensor {i} is not on {device}")
+        a = b = 0
+        if small:
+            blocks = -(-size // STATE_BLOCK)
+            for t in (sm[i], sv[i]):
+                if t.dtype != torch.float32 or t.numel() != blocks or not t.is_contiguous() or t.device != device:
+                    raise ValueError(f"tensor {i}: scales must be contiguous float32, one per {STATE_BLOCK} elements")
+            a, b = sm[i].data_ptr(), sv[i].data_ptr()
+        flat += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), a, b, size)
+    seen = [q for i in range(n) if flat[7 * i + 6] for q in (flat[7 * i], flat[7 * i + 2], flat[7 * i + 3])]
+    if len(set(seen)) != len(seen):
+        raise ValueError("adamw: a parameter or state is there twice")
+    hyper = N.AdamWHyper(0.0 if lr_dev is not None else float(lr), float(betas[0]), float(betas[1]), float(eps),
+                         float(weight_decay))
+    work = torch.empty(8, dtype=torch.float32, device=device)
+    table = (ctypes.c_int64 * len(flat))(*flat)
+    with N.on_device(step):
+        N.check("rpfq_adamw", N.load().rpfq_adamw(
+            table, n, code, 8 if small else 32, ctypes.byref(hyper), step.data_ptr(), N.ptr(lr_dev), N.ptr(grad_scale),
+            N.ptr(found_inf), work.data_ptr(), N.stream_of(step)))
+    # written behind torch's back: packed layers tell a changed weight by its version
+    torch.autograd.graph.increment_version(params + ms + vs + sm + sv + [step])
+
+
+def adamw_state_values(codes, scales) -> list[torch.Tensor]:
+    """float32 values of 8-bit AdamW states (rpfq_adamw_state_values), shaped as
+    the codes: int8 codes are first moments, uint8 codes second moments."""
+    codes, scales = list(codes), list(scales)
+    if len(codes) != len(scales):
+        raise ValueError("adamw_state_values: the lists must be of one length")
+    if not codes:
+        return []
+    for i, (c, s) in enumerate(zip(codes, scales)):
+        N.require_same_device(codes[0], **{f"codes {i}": c, f"scales {i}": s})
+        if c.dtype not in (torch.int8, torch.uint8) or not c.is_contiguous():
+            raise ValueError(f"codes {i} must be contiguous int8 or uint8")
+        if s.dtype != torch.float32 or not s.is_contiguous() or s.numel() != -(-c.numel() // STATE_BLOCK):
+            raise ValueError(f"scales {i} must be contiguous float32, one per {STATE_BLOCK} elements")
+    out = [torch.empty(c.shape, dtype=torch.float32, device=c.device) for c in codes]
+    n = len(codes)
+    vp, i64 = ctypes.c_void_p * n, ctypes.c_int64 * n
+    with N.on_device(codes[0]):
+        N.check("rpfq_adamw_state_values", N.load().rpfq_adamw_state_values(
+            vp(*[c.data_ptr() for c in codes]), vp(*[s.data_ptr() for s in scales]), i64(*[c.numel() for c in codes]),
+            (ctypes.c_int * n)(*[c.dtype == torch.uint8 for c in codes]), vp(*[t.data_ptr() for t in out]), n,
+            N.stream_of(codes[0])))
+    return out
+
+
 def make_desc(n_complex, k_complex, codebook, stages, block, rotation) -> N.WideDesc:
     d = N.WideDesc()
     d.n_complex = int(n_complex)
