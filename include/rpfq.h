@@ -690,8 +690,8 @@ size_t rpfq_linear_cross_entropy_workspace_bytes(const rpfq_ce_desc* desc, int b
 
 /*
  * loss: float32, [1], or [M] with RPFQ_REDUCE_NONE.  The logits are not kept:
- * stat [2][M] (each row's maximum, and 1 / sum exp(z - maximum)) and coef [1]
- * (the mean's factor) are what the gradient needs of them.
+ * stat [3][M] (each row's maximum, 1 / sum exp(z - maximum), the target's logit)
+ * and coef [1] (the mean's factor) are what the gradient needs of them.
  * float32 sums; float32 operands are multiplied as three bf16 terms each, at
  * float32 accuracy.  x and w 16-byte aligned where D % 8 == 0, work 256-byte.
  * Replaces F.cross_entropy(head(x), target) of the reference's training loop.

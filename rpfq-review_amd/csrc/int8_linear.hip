@@ -147,36 +147,65 @@ struct Int8Args {
     int tiles_m, tiles_n, group, vec;
 };
 
-template <int MB, int YDT>
-__global__ void __launch_bounds__(256, 2) int8_gemm_kernel(Int8Args a) {
+template <int MB, int WM, int S, int KB, int YDT>
+__global__ void __launch_bounds__(256 * WM, 2) int8_gemm_kernel(Int8Args a) {
     extern __shared__ __align__(16) char smem[];
-    using G = TileGemm<MB, false, false, MmaI8>;
+    using G = TileGemm<MB, WM, S, KB, false, false, MmaI8>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int mt, nt;
     group_tile(xcd_tile(blockIdx.x, a.tiles_m * a.tiles_n), a.tiles_m, a.tiles_n, a.group, mt, nt);
-    const int64_t m0 = (int64_t)mt * 32 * MB, n0 = (int64_t)nt * 256;
+    const int64_t m0 = (int64_t)mt * G::ROWS + 32 * MB * (wave >> 2), n0 = (int64_t)nt * 256, nw = n0 + 64 * (wave & 3);
     intx16 acc[2][MB];
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = intx16{0};
-    const int steps = (int)((a.K + 63) / 64);
-    G::run(a.x, a.w, m0, n0, a.K, a.K, steps, false, 0, steps, smem, wave, lane, acc);
-    const int64_t n = n0 + 64 * wave + 4 * (lane & 15);
-    f32x4 sw = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+    const int steps = (int)G::steps(a.K);
+    G::run(a.x, a.w, (int64_t)mt * G::ROWS, n0, a.K, a.K, steps, false, 0, steps, smem, wave, lane, acc);
+    char* epi = smem + wave * kTileEpi;
+    if constexpr (YDT == RPFQ_F32) {
+        const int64_t n = nw + 4 * (lane & 15);
+        f32x4 sw = {0, 0, 0, 0}, b = {0, 0, 0, 0};
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-        if (n + t < a.N) {
-            sw[t] = a.sw[n + t];
-            if (a.bias) b[t] = a.bias[n + t];
+        for (int t = 0; t < 4; ++t)
+            if (n + t < a.N) {
+                sw[t] = a.sw[n + t];
+                if (a.bias) b[t] = a.bias[n + t];
+            }
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            const int64_t mr = m0 + 32 * i + (lane & 31);
+            const float sx = a.sx[mr < a.M ? mr : a.M - 1];
+            tile_rows(epi, acc[0][i], acc[1][i], lane, [&](int v, int) { return (float)v * sx; },
+                      [&](int row, int, f32x4 v) {
+                          const int64_t m = m0 + 32 * i + row;
+                          if (m < a.M) tile_store4<YDT>(a.y, m * a.N, n, a.N, a.vec, v * sw + b);
+                      });
         }
+    } else {  // scales and biases of the tile's columns in LDS, as the accumulators hold them
+        float* col = reinterpret_cast<float*>(smem + G::WAVES * kTileEpi);
+        for (int c = threadIdx.x; c < 512; c += G::THREADS) {
+            const int64_t n = n0 + (c & 255);
+            col[c] = n >= a.N ? 0.0f : c < 256 ? a.sw[n] : a.bias ? a.bias[n] : 0.0f;
+        }
+        __syncthreads();
+        const float* mine = col + 64 * (wave & 3) + 4 * (lane >> 5);
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
-        const int64_t mr = m0 + 32 * i + (lane & 31);
-        const float sx = a.sx[mr < a.M ? mr : a.M - 1];
-        tile_rows(smem + wave * kTileEpi, acc[0][i], acc[1][i], lane, [&](int v, int) { return (float)v * sx; },
-                  [&](int row, int, f32x4 v) {
-                      const int64_t m = m0 + 32 * i + row;
-                      if (m < a.M) tile_store4<YDT>(a.y, m * a.N, n, a.N, a.vec, v * sw + b);
-                  });
+        for (int i = 0; i < MB; ++i) {
+            const int64_t mr = m0 + 32 * i + (lane & 31);
+            const float sx = a.sx[mr < a.M ? mr : a.M - 1];
+            tile_rows_half(
+                epi, acc[0][i], acc[1][i], lane,
+                [&](int v0, int v1, int v2, int v3, int j, int q) {
+                    const f32x4 w = *reinterpret_cast<const f32x4*>(mine + 32 * j + 8 * q);
+                    const f32x4 b = *reinterpret_cast<const f32x4*>(mine + 256 + 32 * j + 8 * q);
+                    const f32x4 v = (f32x4){(float)v0 * sx, (float)v1 * sx, (float)v2 * sx, (float)v3 * sx} * w + b;
+                    return make_uint2(tile_pack2<YDT>(v[0], v[1]), tile_pack2<YDT>(v[2], v[3]));
+                },
+                [] {},
+                [&](int row, int c, uint4 v) {
+                    const int64_t m = m0 + 32 * i + row;
+                    if (m < a.M) tile_store8(a.y, m * a.N, nw + c, a.N, a.vec, v);
+                });
+        }
     }
 }
 
@@ -209,24 +238,29 @@ hipError_t launch_quantize_int8(const void* x, int dt, int64_t M, int64_t K, int
     }
 }
 
-template <int MB, int YDT>
-static hipError_t gemm_go(Int8Args& a, hipStream_t s) {
-    using G = TileGemm<MB, false, false, MmaI8>;
-    static std::atomic<uint64_t> attr_done{0};
-    const hipError_t e = set_lds_attr_once(reinterpret_cast<const void*>(&int8_gemm_kernel<MB, YDT>), G::LDS, attr_done);
-    if (e != hipSuccess) return e;
-    a.tiles_m = (int)((a.M + 32 * MB - 1) / (32 * MB));
-    a.tiles_n = (int)((a.N + 255) / 256);
-    a.group = tile_group(a.tiles_n, 256 * a.K);
-    hipLaunchKernelGGL((int8_gemm_kernel<MB, YDT>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(256), G::LDS, s, a);
-    return hipGetLastError();
-}
+template <int YDT>
+struct Int8Go {
+    Int8Args& a;
+    hipStream_t s;
+    template <int MB, int WM, int S, int KB>
+    hipError_t run() {
+        using G = TileGemm<MB, WM, S, KB, false, false, MmaI8>;
+        static std::atomic<uint64_t> attr_done{0};
+        const auto kernel = &int8_gemm_kernel<MB, WM, S, KB, YDT>;
+        const hipError_t e = set_lds_attr_once(reinterpret_cast<const void*>(kernel), G::LDS, attr_done);
+        if (e != hipSuccess) return e;
+        a.tiles_m = (int)((a.M + G::ROWS - 1) / G::ROWS);
+        a.tiles_n = (int)((a.N + 255) / 256);
+        a.group = tile_group(a.tiles_n, 256 * a.K);
+        hipLaunchKernelGGL((int8_gemm_kernel<MB, WM, S, KB, YDT>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(G::THREADS),
+                           G::LDS, s, a);
+        return hipGetLastError();
+    }
+};
 
 template <int YDT>
 static hipError_t gemm_y(Int8Args& a, hipStream_t s) {
-    if (a.M <= 32) return gemm_go<1, YDT>(a, s);
-    const int64_t tiles = (a.M + 127) / 128 * ((a.N + 255) / 256);
-    return tiles < device_cus() ? gemm_go<2, YDT>(a, s) : gemm_go<4, YDT>(a, s);
+    return tile_dispatch(tile_form(a.M, a.N), Int8Go<YDT>{a, s});
 }
 
 // x codes in `work` unless given; w copied there if its rows are not 16-byte aligned
@@ -290,7 +324,7 @@ hipError_t launch_linear_int8(const void* x, int xdt, const float* sx, const int
     a.N = N;
     a.K = p.ld;
     const int es = ydt == RPFQ_F32 ? 4 : 2;
-    a.vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(y) % (4 * es) == 0;
+    a.vec = N % (16 / es) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
     switch (ydt) {
         case RPFQ_F32: return gemm_y<RPFQ_F32>(a, s);
         case RPFQ_F16: return gemm_y<RPFQ_F16>(a, s);

@@ -5,8 +5,9 @@
 //   dx = dz w,  dw = dz^T x,  db = sum_m dz_m.
 // Forward: the logits' tiles leave the matrix cores as a maximum and a sum of
 // exp(z - maximum) per row and tile (float32), joined by a pass over the tiles.
-// Kept are the row's maximum and the sum's reciprocal, not lse: that one's last
-// bit is 2^-20 of a probability near 1, which is most of dz where p - 1 is small.
+// Kept of a row are its maximum, the sum's reciprocal and the target's logit,
+// not lse: that one's last bit is 2^-20 of a probability near 1, which is most
+// of dz where p - 1 is small.
 // Backward: the logits are formed again, a piece of the classes at a time; dz
 // of a piece goes to a workspace in 16 bits and meets w and x from there.
 //
@@ -21,7 +22,22 @@
 
 namespace rpfq {
 
+// exp(z - a) as exp2(z log2e - a log2e), one fused operation a value, where a
+// is the rounded product wherever it is used again, so its rounding cancels.
+// log2e in float32 stands for 1.3e-8 too little of every logit, less than their
+// own rounding.  Past 2^100 (masks of a type's lowest value) a log2e could
+// overflow: there the difference comes first.
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kCeFar = 0x1p100f;
+__device__ __forceinline__ float ce_exp2(float z, float a2) { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -a2)); }
+// z - top of a logit against a row's maximum, in the units of exp2
+__device__ __forceinline__ float ce_gap_z(float z, float top) {
+    return fabsf(top) <= kCeFar ? __builtin_fmaf(z, kLog2e, -(top * kLog2e)) : (z - top) * kLog2e;
+}
+// (a - b) log2e as the two agree on it
+__device__ __forceinline__ float ce_gap(float a, float b) {
+    return fabsf(a) <= kCeFar && fabsf(b) <= kCeFar ? a * kLog2e - b * kLog2e : (a - b) * kLog2e;
+}
 
 struct CeArgs {
     TileOperand x, w;          // [M, D], [V, D], K layout
@@ -31,7 +47,7 @@ struct CeArgs {
     int64_t M, V;              // rows, classes (w.count: those of a piece)
     int64_t v0;                // first class of the piece
     int64_t kb;                // bytes of k
-    int per, planes;
+    int planes;
     int tiles_m, tiles_n, group;
     float smooth;
     // forward
@@ -39,7 +55,7 @@ struct CeArgs {
     float* zsum;               // [tiles_n][M] sums of z, or NULL
     float* zt;                 // [M] the target's logit
     // backward
-    const float *stat, *rho;   // [2][M] maximum, 1 / sum; [M]
+    const float *stat, *rho;   // [3][M] maximum, 1 / sum, the target's logit; [M]
     float dz_scale;
     char* dz;                  // [planes][M][ldz bytes]
     int64_t ldz, dz_plane;
@@ -69,65 +85,78 @@ __device__ __forceinline__ void ce_bias(floatx16 (&acc)[2][MB], const float* bia
         }
 }
 
-// The 256 biases of a tile to LDS: -inf past the last class.
-__device__ __forceinline__ void ce_stage_bias(const CeArgs& a, int64_t n0, float* sm) {
-    const int64_t n = n0 + threadIdx.x;
-    float b = n < a.w.count ? 0.0f : -__builtin_inff();
-    if (a.bias && n < a.w.count) b = ce_load(a.bias, a.bias_dt, a.v0 + n);
-    sm[threadIdx.x] = b;
+// The 256 biases of a tile to LDS, added to the accumulators of a wave: -inf
+// past the last class.  Tiles without either are left as they are.
+template <int MB>
+__device__ __forceinline__ void ce_logits(const CeArgs& a, int64_t n0, float* sm, int wave, int lane, floatx16 (&acc)[2][MB]) {
+    if (!a.bias && n0 + 256 <= a.w.count) return;
+    if (threadIdx.x < 256) {
+        const int64_t n = n0 + threadIdx.x;
+        float b = n < a.w.count ? 0.0f : -__builtin_inff();
+        if (a.bias && n < a.w.count) b = ce_load(a.bias, a.bias_dt, a.v0 + n);
+        sm[threadIdx.x] = b;
+    }
     __syncthreads();
+    ce_bias<MB>(acc, sm + 64 * (wave & 3), lane);
 }
 
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
-template <int MB, class Mma>
-__global__ void __launch_bounds__(256, 2) ce_stats_kernel(CeArgs a) {
+template <int MB, int WM, int S, int KB, class Mma>
+__global__ void __launch_bounds__(256 * WM, 2) ce_stats_kernel(CeArgs a) {
     extern __shared__ __align__(16) char smem[];
-    using G = TileGemm<MB, false, false, Mma>;
+    using G = TileGemm<MB, WM, S, KB, false, false, Mma>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 31, g = lane >> 5;
     int mt, nt;
     group_tile(xcd_tile(blockIdx.x, a.tiles_m * a.tiles_n), a.tiles_m, a.tiles_n, a.group, mt, nt);
-    const int64_t m0 = (int64_t)mt * 32 * MB, n0 = (int64_t)nt * 256;
+    const int64_t m0 = (int64_t)mt * G::ROWS, n0 = (int64_t)nt * 256, nw = n0 + 64 * (wave & 3);
     floatx16 acc[2][MB];
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
-    const int steps = a.planes ? kPairs32 * a.per : a.per;
-    G::run(a.x, a.w, m0, n0, a.kb, a.kb, a.per, a.planes, 0, steps, smem, wave, lane, acc);
+    const int per = (int)G::steps(a.kb), steps = a.planes ? kPairs32 * per : per;
+    G::run(a.x, a.w, m0, n0, a.kb, a.kb, per, a.planes, 0, steps, smem, wave, lane, acc);
     float* sb = reinterpret_cast<float*>(smem);
-    float* sp = sb + 256;  // [4 waves][32 MB rows][max, sum, sum of z]
-    ce_stage_bias(a, n0, sb);
-    ce_bias<MB>(acc, sb + 64 * wave, lane);
+    float* sp = sb + 256;  // [4 column waves][rows][max, sum, sum of z]
+    ce_logits<MB>(a, n0, sb, wave, lane, acc);
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
+        const int row = 32 * (MB * (wave >> 2) + i) + r;
         float mx = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int v = 0; v < 16; ++v) mx = fmaxf(mx, acc[j][i][v]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float base = mx == -__builtin_inff() ? 0.0f : mx;
         float sum = 0.0f, zs = 0.0f;
+        if (!__any(fabsf(mx) > kCeFar)) {
+            const float base = mx * kLog2e;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) sum += __builtin_amdgcn_exp2f((acc[j][i][v] - base) * kLog2e);
+                for (int v = 0; v < 16; ++v) sum += ce_exp2(acc[j][i][v], base);
+        } else {
+            const float base = mx == -__builtin_inff() ? 0.0f : mx;
+            const bool far = fabsf(base) > kCeFar;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    sum += far ? __builtin_amdgcn_exp2f((acc[j][i][v] - base) * kLog2e) : ce_exp2(acc[j][i][v], base * kLog2e);
+        }
         if (a.zsum) {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int64_t n = n0 + 64 * wave + 32 * j + acc_row(v, g);
-                    zs += n < a.w.count ? acc[j][i][v] : 0.0f;
-                }
+                for (int v = 0; v < 16; ++v) zs += nw + 32 * j + acc_row(v, g) < a.w.count ? acc[j][i][v] : 0.0f;
             zs += __shfl_xor(zs, 32, 64);
         }
         sum += __shfl_xor(sum, 32, 64);
-        const int64_t m = m0 + 32 * i + r;
+        const int64_t m = m0 + row;
         if (m < a.M) {
-            const int64_t t = a.target[m] - n0 - 64 * wave;
-            if (t >= 0 && t < 64 && n0 + 64 * wave + t < a.V) {
+            const int64_t t = a.target[m] - nw;
+            if (t >= 0 && t < 64 && nw + t < a.V) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -136,7 +165,7 @@ __global__ void __launch_bounds__(256, 2) ce_stats_kernel(CeArgs a) {
             }
         }
         if (g == 0) {
-            float* d = sp + (wave * 32 * MB + 32 * i + r) * 3;
+            float* d = sp + ((wave & 3) * G::ROWS + row) * 3;
             d[0] = mx;
             d[1] = sum;
             d[2] = zs;
@@ -144,15 +173,15 @@ __global__ void __launch_bounds__(256, 2) ce_stats_kernel(CeArgs a) {
     }
     __syncthreads();
     const int row = threadIdx.x;
-    if (row < 32 * MB && m0 + row < a.M) {
+    if (row < G::ROWS && m0 + row < a.M) {
         float mx = -__builtin_inff(), sum = 0.0f, zs = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) mx = fmaxf(mx, sp[(w * 32 * MB + row) * 3]);
+        for (int w = 0; w < 4; ++w) mx = fmaxf(mx, sp[(w * G::ROWS + row) * 3]);
         // fmax passes over NaN: the sums keep it
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float* d = sp + (w * 32 * MB + row) * 3;
-            sum += d[0] == -__builtin_inff() ? d[1] : d[1] * __builtin_amdgcn_exp2f((d[0] - mx) * kLog2e);
+            const float* d = sp + (w * G::ROWS + row) * 3;
+            sum += d[0] == -__builtin_inff() ? d[1] : d[1] * __builtin_amdgcn_exp2f(ce_gap(d[0], mx));
             zs += d[2];
         }
         a.part[(int64_t)nt * a.M + m0 + row] = make_float2(mx, sum);
@@ -168,7 +197,7 @@ struct CeJoin {
     int64_t M, V, ignore;
     int tiles;
     float smooth;
-    float* stat;  // [2][M]: maximum, 1 / sum of exp(z - maximum)
+    float* stat;  // [3][M]: maximum, 1 / sum of exp(z - maximum), the target's logit
     float* rows;  // [M] loss of each row, 0 where ignored
 };
 
@@ -182,9 +211,9 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeJoin a) {
         for (int t = q; t < a.tiles; t += 16) {
             const float2 p = a.part[(int64_t)t * a.M + m];
             const float n = fmaxf(mx, p.x), base = n == -__builtin_inff() ? 0.0f : n;
-            sum = sum * __builtin_amdgcn_exp2f((mx - base) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - base) * kLog2e);
             // a tile of -inf has sum 0, one with NaN has sum NaN whatever its maximum
-            if (p.x == -__builtin_inff() && p.y != p.y) sum = p.y;
+            const float add = p.y == 0.0f || p.y != p.y ? p.y : p.y * __builtin_amdgcn_exp2f(ce_gap(p.x, base));
+            sum = (sum == 0.0f ? 0.0f : sum * __builtin_amdgcn_exp2f(ce_gap(mx, base))) + add;
             mx = n;
             if (a.zsum) zs += a.zsum[(int64_t)t * a.M + m];
         }
@@ -200,22 +229,27 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeJoin a) {
     sum = zs = 0.0f;
     for (int i = 0; i < 16; ++i) {
         const float s = sm[1][c][i];
-        sum += s == 0.0f ? 0.0f : s * __builtin_amdgcn_exp2f((sm[0][c][i] - base) * kLog2e);
+        sum += s == 0.0f || s != s ? s : s * __builtin_amdgcn_exp2f(ce_gap(sm[0][c][i], base));
         zs += sm[2][c][i];
     }
-    const float more = logf(sum);  // lse - base
+    // lse in 64 bits, from the exponent that the sum is relative to
+    const double lse = fabsf(base) <= kCeFar ? ((double)(base * kLog2e) + log2((double)sum)) / (double)kLog2e
+                                             : (double)base + log((double)sum);
     const int64_t t = a.target[m];
+    const bool labelled = t >= 0 && t < a.V;
+    const float zt = labelled ? a.zt[m] : 0.0f;
     float loss = 0.0f;
     if (t != a.ignore) {
-        if (t < 0 || t >= a.V) {
-            loss = __uint_as_float(0x7fc00000u);
-        } else {
-            loss = (1.0f - a.smooth) * ((base - a.zt[m]) + more);
-            if (a.zsum) loss += a.smooth * ((base - zs / (float)a.V) + more);
+        loss = __uint_as_float(0x7fc00000u);
+        if (labelled) {
+            double d = (1.0 - (double)a.smooth) * (lse - (double)zt);
+            if (a.zsum) d += (double)a.smooth * (lse - (double)zs / (double)a.V);
+            loss = (float)d;
         }
     }
     a.stat[m] = base;
     a.stat[a.M + m] = 1.0f / sum;
+    a.stat[2 * a.M + m] = zt;
     a.rows[m] = loss;
 }
 
@@ -335,76 +369,129 @@ __global__ void __launch_bounds__(256) ce_planes_kernel(const float* x, int64_t 
     }
 }
 
+// Sums of 32 values over the 32 lanes of a half wave: lane r ends with the sum
+// of value r.  Each round halves the values: a lane keeps one half and hands
+// the other to its partner.
+__device__ __forceinline__ float ce_lane_sums(float (&v)[32], int lane) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+        const bool up = lane & m;
+#pragma unroll
+        for (int k = 0; k < m; ++k) {
+            const float give = up ? v[k] : v[k + m], keep = up ? v[k + m] : v[k];
+            v[k] = keep + __shfl_xor(give, m, 64);
+        }
+    }
+    return v[0];
+}
+
 // dz of one piece of the classes.  DT: the type of dz (float32: three planes).
-template <int MB, class Mma, int DT>
-__global__ void __launch_bounds__(256, 2) ce_dz_kernel(CeArgs a) {
+template <int MB, int WM, int S, int KB, class Mma, int DT>
+__global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
     extern __shared__ __align__(16) char smem[];
-    using G = TileGemm<MB, false, false, Mma>;
+    using G = TileGemm<MB, WM, S, KB, false, false, Mma>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 31, c4 = 4 * (lane & 15);
+    const int r = lane & 31, g = lane >> 5;
     int mt, nt;
     group_tile(xcd_tile(blockIdx.x, a.tiles_m * a.tiles_n), a.tiles_m, a.tiles_n, a.group, mt, nt);
-    const int64_t m0 = (int64_t)mt * 32 * MB, n0 = (int64_t)nt * 256;
+    const int64_t m0 = (int64_t)mt * G::ROWS, mw = m0 + 32 * MB * (wave >> 2);
+    const int64_t n0 = (int64_t)nt * 256, nw = n0 + 64 * (wave & 3);
     floatx16 acc[2][MB];
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
-    const int steps = a.planes ? kPairs32 * a.per : a.per;
-    G::run(a.x, a.w, m0, n0, a.kb, a.kb, a.per, a.planes, 0, steps, smem, wave, lane, acc);
-    float* sb = reinterpret_cast<float*>(smem + 4 * kTileEpi);
-    ce_stage_bias(a, n0, sb);
-    ce_bias<MB>(acc, sb + 64 * wave, lane);
+    const int per = (int)G::steps(a.kb), steps = a.planes ? kPairs32 * per : per;
+    G::run(a.x, a.w, m0, n0, a.kb, a.kb, per, a.planes, 0, steps, smem, wave, lane, acc);
+    char* epi = smem + wave * kTileEpi;
+    ce_logits<MB>(a, n0, reinterpret_cast<float*>(smem + G::WAVES * kTileEpi), wave, lane, acc);
     const float even = a.smooth / (float)a.V;
-    const int64_t n = n0 + 64 * wave + c4;  // the lane's columns in out()
-    f32x4 cs = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
-        const int64_t mr = m0 + 32 * i + r;
-        float top = 0.0f, inv = 0.0f, rho = 0.0f;
+        const int64_t mr = mw + 32 * i + r;
+        // rows that count nowhere: exp2(-inf) times 0
+        float top = __builtin_inff(), f = 0.0f, off = 0.0f, dzt = 0.0f;
         int t = -1;  // the target's column among the wave's
         if (mr < a.M) {
-            top = a.stat[mr];
-            inv = a.stat[a.M + mr];
-            rho = a.rho[mr] * a.dz_scale;
-            const int64_t tt = a.target[mr] - a.v0 - n0 - 64 * wave;
-            t = tt >= 0 && tt < 64 ? (int)tt : -1;
-        }
-        tile_rows(
-            smem + wave * kTileEpi, acc[0][i], acc[1][i], lane,
-            [&](float z, int col) {
-                float p = __builtin_amdgcn_exp2f((z - top) * kLog2e) * inv - even;
-                if (col == t) p -= 1.0f - a.smooth;
-                return rho == 0.0f ? 0.0f : p * rho;
-            },
-            [&](int row, int, f32x4 v) {
-                const int64_t m = m0 + 32 * i + row;
-                if (m >= a.M || 2 * n >= a.ldz) return;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e >= a.w.count) v[e] = 0.0f;
-                cs += v;
-                char* d = a.dz + m * a.ldz + 2 * n;
-                if constexpr (DT == RPFQ_F32) {
-                    uint16_t h[4], k[4], l[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) split3(v[e], h[e], k[e], l[e]);
-                    __builtin_memcpy(d, h, 8);
-                    __builtin_memcpy(d + a.dz_plane, k, 8);
-                    __builtin_memcpy(d + 2 * a.dz_plane, l, 8);
-                } else {
-                    uint2 o;
-                    o.x = DT == RPFQ_F16 ? cvt_pk(v[0], v[1]) : pack_bf2(v[0], v[1]);
-                    o.y = DT == RPFQ_F16 ? cvt_pk(v[2], v[3]) : pack_bf2(v[2], v[3]);
-                    *reinterpret_cast<uint2*>(d) = o;
+            const float rho = a.rho[mr] * a.dz_scale;
+            const int64_t tt = a.target[mr] - a.v0 - nw;
+            if (rho != 0.0f) {
+                const float inv = a.stat[a.M + mr];
+                top = a.stat[mr];
+                f = inv * rho;
+                off = even * rho;
+                if (tt >= 0 && tt < 64) {
+                    t = (int)tt;
+                    // p - 1 before the factors: what is left of a p near 1 keeps its bits
+                    dzt = (__builtin_amdgcn_exp2f(ce_gap_z(a.stat[2 * a.M + mr], top)) * inv - even - (1.0f - a.smooth)) * rho;
                 }
-            });
-    }
-    if (a.colsum) {  // the lane's columns over the tile's rows
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            cs[e] += __shfl_xor(cs[e], 16, 64);
-            cs[e] += __shfl_xor(cs[e], 32, 64);
+            }
         }
-        if (lane < 16 && 2 * n < a.ldz) *reinterpret_cast<f32x4*>(a.colsum + (int64_t)mt * (a.ldz / 2) + n) = cs;
+        const bool plain = !__any(fabsf(top) > kCeFar && top != __builtin_inff());
+        const float base = fabsf(top) > kCeFar && top != __builtin_inff() ? top : top * kLog2e;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const float z = acc[j][i][v];
+                const float e = plain ? ce_exp2(z, base) : __builtin_amdgcn_exp2f(ce_gap_z(z, top));
+                acc[j][i][v] = __builtin_fmaf(e, f, -off);
+            }
+        if (a.w.count - n0 < 256) {  // columns past the last class, for the operands' padding
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    if (nw + 32 * j + acc_row(v, g) >= a.w.count) acc[j][i][v] = 0.0f;
+        }
+        if (DT == RPFQ_F32 || a.colsum) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    if (t == 32 * j + acc_row(v, g)) acc[j][i][v] = dzt;
+        }
+        if constexpr (DT == RPFQ_F32) {
+            const int64_t n = nw + 4 * (lane & 15);
+            tile_rows(epi, acc[0][i], acc[1][i], lane, [](float v, int) { return v; },
+                      [&](int row, int, f32x4 v) {
+                          const int64_t m = mw + 32 * i + row;
+                          if (m >= a.M || 2 * n >= a.ldz) return;
+                          char* d = a.dz + m * a.ldz + 2 * n;
+                          uint16_t h[4], k[4], l[4];
+#pragma unroll
+                          for (int e = 0; e < 4; ++e) split3(v[e], h[e], k[e], l[e]);
+                          __builtin_memcpy(d, h, 8);
+                          __builtin_memcpy(d + a.dz_plane, k, 8);
+                          __builtin_memcpy(d + 2 * a.dz_plane, l, 8);
+                      });
+        } else {
+            tile_rows_half(
+                epi, acc[0][i], acc[1][i], lane,
+                [&](float a0, float a1, float a2, float a3, int, int) {
+                    return make_uint2(tile_pack2<DT>(a0, a1), tile_pack2<DT>(a2, a3));
+                },
+                [&] {
+                    if (t >= 0 && g == 0)
+                        *reinterpret_cast<uint16_t*>(epi + tile_half_at(r, t)) = (uint16_t)tile_pack2<DT>(dzt, 0.0f);
+                },
+                [&](int row, int c, uint4 v) {
+                    const int64_t m = mw + 32 * i + row, n = nw + c;
+                    if (m < a.M && 2 * n < a.ldz) *reinterpret_cast<uint4*>(a.dz + m * a.ldz + 2 * n) = v;
+                });
+        }
+    }
+    if (a.colsum) {  // the wave's columns over its rows
+        float cs[32];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                cs[16 * j + v] = acc[j][0][v];
+#pragma unroll
+                for (int i = 1; i < MB; ++i) cs[16 * j + v] += acc[j][i][v];
+            }
+        const float sum = ce_lane_sums(cs, lane);
+        const int64_t n = nw + 32 * (r >> 4) + acc_row(r & 15, g);
+        if (2 * n < a.ldz) a.colsum[((int64_t)mt * WM + (wave >> 2)) * (a.ldz / 2) + n] = sum;
     }
 }
 
@@ -412,7 +499,7 @@ struct CeGrad {
     TileOperand r, c;
     int64_t rk, ck;
     int64_t M, N;     // rows, columns of the gradient
-    int per, steps, planes, splits;
+    int planes, splits;
     int tiles_m, tiles_n, group;
     float* part;      // [splits][M][ldp], or NULL: the gradient itself, rounded
     int64_t ldp;
@@ -423,30 +510,30 @@ struct CeGrad {
 };
 
 // One product of the gradient: dx (dz in K layout, w in T) or dw (dz and x in T).
-template <bool RT, class Mma, int DT>
-__global__ void __launch_bounds__(256, 2) ce_grad_kernel(CeGrad a) {
+template <int MB, int WM, int S, int KB, bool RT, class Mma, int DT>
+__global__ void __launch_bounds__(256 * WM, 2) ce_grad_kernel(CeGrad a) {
     extern __shared__ __align__(16) char smem[];
-    constexpr int MB = 4;
-    using G = TileGemm<MB, RT, true, Mma>;
+    using G = TileGemm<MB, WM, S, KB, RT, true, Mma>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles = a.tiles_m * a.tiles_n;
     const int unit = xcd_tile(blockIdx.x, tiles * a.splits), sp = unit / tiles;
     int mt, nt;
     group_tile(unit - sp * tiles, a.tiles_m, a.tiles_n, a.group, mt, nt);
-    const int64_t m0 = (int64_t)mt * 32 * MB, n0 = (int64_t)nt * 256;
-    const int s0 = (int)((int64_t)a.steps * sp / a.splits), s1 = (int)((int64_t)a.steps * (sp + 1) / a.splits);
+    const int64_t m0 = (int64_t)mt * G::ROWS, mw = m0 + 32 * MB * (wave >> 2), n0 = (int64_t)nt * 256;
+    const int per = (int)G::steps(a.rk), steps = a.planes ? kPairs32 * per : per;
+    const int s0 = (int)((int64_t)steps * sp / a.splits), s1 = (int)((int64_t)steps * (sp + 1) / a.splits);
     floatx16 acc[2][MB];
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
-    G::run(a.r, a.c, m0, n0, a.rk, a.ck, a.per, a.planes, s0, s1, smem, wave, lane, acc);
-    const int64_t n = n0 + 64 * wave + 4 * (lane & 15);
+    G::run(a.r, a.c, m0, n0, a.rk, a.ck, per, a.planes, s0, s1, smem, wave, lane, acc);
+    const int64_t n = n0 + 64 * (wave & 3) + 4 * (lane & 15);
     const float f = a.part ? 1.0f : a.factor[0];
     float* part = a.part ? a.part + (int64_t)sp * a.M * a.ldp : nullptr;
 #pragma unroll
     for (int i = 0; i < MB; ++i)
         tile_rows(smem + wave * kTileEpi, acc[0][i], acc[1][i], lane, [&](float v, int) { return v; },
                   [&](int row, int, f32x4 v) {
-                      const int64_t m = m0 + 32 * i + row;
+                      const int64_t m = mw + 32 * i + row;
                       if (m >= a.M) return;
                       if (part) {
                           if (n >= a.ldp) return;
@@ -476,18 +563,27 @@ __global__ void __launch_bounds__(256) ce_sum_kernel(const float* part, int part
 // ---------------------------------------------------------------------------
 // plan and launches
 // ---------------------------------------------------------------------------
-// Units of a product over `slots` workgroups at a time: the split of k with the
-// least rounds of work, a little for each partial that is written and read.
-static int ce_splits(int64_t tiles, int64_t steps) {
-    const int64_t slots = 2 * (int64_t)device_cus();
-    int best = 1;
+// The form and the split of k (`steps` of 64 bytes) with the least time for a
+// gradient of rows x cols: rounds of the chip in units of a 256-row tile's step,
+// a few for a tile's start and end, and the partials' way through memory.
+static CeSplit ce_split(int64_t rows, int64_t cols, int64_t steps) {
+    const int64_t cus = device_cus(), tn = (cols + 255) / 256;
+    CeSplit best = {kTile128, 1};
     double cost = 1e300;
-    for (int s = 1; s <= 16 && s <= steps; ++s) {
-        const int64_t rounds = (tiles * s + slots - 1) / slots;
-        const double c = (double)rounds * ((double)(steps + s - 1) / s + 8) + (s > 1 ? 4.0 * s * tiles / slots + 8 : 0.0);
-        if (c < cost) {
-            cost = c;
-            best = s;
+    for (int s = 1; s <= 64 && (s == 1 || 4 * s <= steps); ++s) {
+        const double n = (double)((steps + s - 1) / s);
+        const double join = s > 1 ? 8.0 + (double)s * rows * cols * 8.0 / 2e6 : 0.0;
+        for (const TileForm f : {kTile64, kTile128Deep, kTile128, kTile256}) {
+            const int64_t tall = f == kTile64 ? 64 : f == kTile256 ? 256 : 128;
+            const int64_t units = (rows + tall - 1) / tall * tn * s;
+            double c;
+            if (f == kTile64 || f == kTile128Deep) c = units > cus ? 1e300 : n * (f == kTile64 ? 0.45 : 0.6) + 8.0;
+            else if (f == kTile128) c = (double)((units + 2 * cus - 1) / (2 * cus)) * (1.15 * n + 8.0);
+            else c = (double)((units + cus - 1) / cus) * (n + 10.0);
+            if (c + join < cost) {
+                cost = c + join;
+                best = {f, s};
+            }
         }
     }
     return best;
@@ -526,15 +622,14 @@ CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool back
     p.piece = (p.tiles_v + p.pieces - 1) / p.pieces * 256;  // classes
     if (p.piece > V) p.piece = (V + 7) & ~(int64_t)7;
     p.dz_at = take(2 * planes * M * p.piece);
-    p.tiles_m = (M + 127) / 128;
-    p.col_at = take(4 * (M + 31) / 32 * p.piece);
+    p.col_at = take(4 * ((M + 31) / 32 + 8) * p.piece);
     // float32 partials, rows of whole 16 bytes
     p.ldp = (D + 3) & ~(int64_t)3;
-    const int64_t tn = (D + 255) / 256, pairs = planes == 3 ? kPairs32 : 1;
-    p.dx_splits = ce_splits(p.tiles_m * tn, pairs * ((p.piece + 31) / 32));
-    p.dx_at = take(p.dx_splits > 1 || p.pieces > 1 ? 4 * p.dx_splits * M * p.ldp : 0);
-    p.dw_splits = ce_splits((p.piece + 127) / 128 * tn, pairs * ((M + 31) / 32));
-    p.dw_at = take(p.dw_splits > 1 ? 4 * p.dw_splits * p.piece * p.ldp : 0);
+    const int64_t pairs = planes == 3 ? kPairs32 : 1;
+    p.dx = ce_split(M, D, pairs * ((p.piece + 31) / 32));
+    p.dx_at = take(p.dx.splits > 1 || p.pieces > 1 ? 4 * p.dx.splits * M * p.ldp : 0);
+    p.dw = ce_split(p.piece, D, pairs * ((M + 31) / 32));
+    p.dw_at = take(p.dw.splits > 1 ? 4 * p.dw.splits * p.piece * p.ldp : 0);
     return p;
 }
 
@@ -545,7 +640,6 @@ static unsigned blocks_of(int64_t n) { return (unsigned)(n < 1 ? 1 : n > 16384 ?
 static hipError_t ce_operands(const CePlan& p, int dt, const void* x, const void* w, int64_t M, int64_t V, int64_t D,
                               char* wk, CeArgs& a, hipStream_t s) {
     a.kb = 2 * p.ldk;
-    a.per = (int)((a.kb + 63) / 64);
     a.planes = dt == RPFQ_F32;
     a.x = {reinterpret_cast<const char*>(x), a.kb, 0, M};
     a.w = {reinterpret_cast<const char*>(w), a.kb, 0, V};
@@ -575,54 +669,73 @@ static hipError_t ce_lds(K kernel, int bytes, std::atomic<uint64_t>& done) {
     return set_lds_attr_once(reinterpret_cast<const void*>(kernel), bytes, done);
 }
 
-template <int MB, class Mma>
-static hipError_t stats_go(CeArgs& a, hipStream_t s) {
-    using G = TileGemm<MB, false, false, Mma>;
-    static std::atomic<uint64_t> done{0};
-    const hipError_t e = ce_lds(&ce_stats_kernel<MB, Mma>, G::LDS, done);
-    if (e != hipSuccess) return e;
-    a.tiles_m = (int)((a.M + 32 * MB - 1) / (32 * MB));
-    a.tiles_n = (int)((a.w.count + 255) / 256);
-    a.group = tile_group(a.tiles_n, 256 * a.kb);
-    hipLaunchKernelGGL((ce_stats_kernel<MB, Mma>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(256), G::LDS, s, a);
-    return hipGetLastError();
-}
-
 template <class Mma>
-static hipError_t stats_mb(CeArgs& a, hipStream_t s) {
-    return a.M <= 32 ? stats_go<1, Mma>(a, s) : a.M <= 64 ? stats_go<2, Mma>(a, s) : stats_go<4, Mma>(a, s);
-}
-
-template <int MB, class Mma, int DT>
-static hipError_t dz_go(CeArgs& a, hipStream_t s) {
-    using G = TileGemm<MB, false, false, Mma>;
-    static std::atomic<uint64_t> done{0};
-    const hipError_t e = ce_lds(&ce_dz_kernel<MB, Mma, DT>, G::LDS, done);
-    if (e != hipSuccess) return e;
-    a.tiles_m = (int)((a.M + 32 * MB - 1) / (32 * MB));
-    a.tiles_n = (int)((a.w.count + 255) / 256);
-    a.group = tile_group(a.tiles_n, 256 * a.kb);
-    hipLaunchKernelGGL((ce_dz_kernel<MB, Mma, DT>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(256), G::LDS, s, a);
-    return hipGetLastError();
-}
+struct StatsGo {
+    CeArgs& a;
+    hipStream_t s;
+    template <int MB, int WM, int S, int KB>
+    hipError_t run() {
+        using G = TileGemm<MB, WM, S, KB, false, false, Mma>;
+        static std::atomic<uint64_t> done{0};
+        const hipError_t e = ce_lds(&ce_stats_kernel<MB, WM, S, KB, Mma>, G::LDS, done);
+        if (e != hipSuccess) return e;
+        a.tiles_m = (int)((a.M + G::ROWS - 1) / G::ROWS);
+        a.tiles_n = (int)((a.w.count + 255) / 256);
+        a.group = tile_group(a.tiles_n, 256 * a.kb);
+        hipLaunchKernelGGL((ce_stats_kernel<MB, WM, S, KB, Mma>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(G::THREADS),
+                           G::LDS, s, a);
+        return hipGetLastError();
+    }
+};
 
 template <class Mma, int DT>
-static hipError_t dz_mb(CeArgs& a, hipStream_t s) {
-    return a.M <= 32 ? dz_go<1, Mma, DT>(a, s) : a.M <= 64 ? dz_go<2, Mma, DT>(a, s) : dz_go<4, Mma, DT>(a, s);
-}
+struct DzGo {
+    CeArgs& a;
+    int& col_rows;  // rows of column sums that the launch leaves
+    hipStream_t s;
+    template <int MB, int WM, int S, int KB>
+    hipError_t run() {
+        using G = TileGemm<MB, WM, S, KB, false, false, Mma>;
+        static std::atomic<uint64_t> done{0};
+        const hipError_t e = ce_lds(&ce_dz_kernel<MB, WM, S, KB, Mma, DT>, G::LDS, done);
+        if (e != hipSuccess) return e;
+        a.tiles_m = (int)((a.M + G::ROWS - 1) / G::ROWS);
+        a.tiles_n = (int)((a.w.count + 255) / 256);
+        a.group = tile_group(a.tiles_n, 256 * a.kb);
+        col_rows = a.tiles_m * WM;
+        hipLaunchKernelGGL((ce_dz_kernel<MB, WM, S, KB, Mma, DT>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(G::THREADS),
+                           G::LDS, s, a);
+        return hipGetLastError();
+    }
+};
 
 template <bool RT, class Mma, int DT>
-static hipError_t grad_go(CeGrad& a, hipStream_t s) {
-    using G = TileGemm<4, RT, true, Mma>;
-    static std::atomic<uint64_t> done{0};
-    const hipError_t e = ce_lds(&ce_grad_kernel<RT, Mma, DT>, G::LDS, done);
-    if (e != hipSuccess) return e;
-    a.tiles_m = (int)((a.M + 127) / 128);
-    a.tiles_n = (int)((a.N + 255) / 256);
-    a.group = a.tiles_n;
-    hipLaunchKernelGGL((ce_grad_kernel<RT, Mma, DT>), dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)), dim3(256), G::LDS, s,
-                       a);
-    return hipGetLastError();
+struct GradGo {
+    CeGrad& a;
+    hipStream_t s;
+    template <int MB, int WM, int S, int KB>
+    hipError_t run() {
+        if constexpr (MB == 1) {
+            return hipErrorInvalidValue;  // ce_split takes 64 rows at least
+        } else {
+            using G = TileGemm<MB, WM, S, KB, RT, true, Mma>;
+            static std::atomic<uint64_t> done{0};
+            const hipError_t e = ce_lds(&ce_grad_kernel<MB, WM, S, KB, RT, Mma, DT>, G::LDS, done);
+            if (e != hipSuccess) return e;
+            a.tiles_m = (int)((a.M + G::ROWS - 1) / G::ROWS);
+            a.tiles_n = (int)((a.N + 255) / 256);
+            a.group = a.tiles_n;
+            hipLaunchKernelGGL((ce_grad_kernel<MB, WM, S, KB, RT, Mma, DT>), dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)),
+                               dim3(G::THREADS), G::LDS, s, a);
+            return hipGetLastError();
+        }
+    }
+};
+template <bool RT>
+static hipError_t ce_grad(int dt, TileForm form, CeGrad& g, hipStream_t s) {
+    return dt == RPFQ_F16    ? tile_dispatch(form, GradGo<RT, MmaF16, RPFQ_F16>{g, s})
+           : dt == RPFQ_BF16 ? tile_dispatch(form, GradGo<RT, MmaBf16, RPFQ_BF16>{g, s})
+                             : tile_dispatch(form, GradGo<RT, MmaBf16, RPFQ_F32>{g, s});
 }
 
 static hipError_t ce_sum(int dt, const float* part, int parts, int64_t stride, int64_t rows, int64_t N, int64_t ldp,
@@ -658,7 +771,8 @@ hipError_t launch_linear_ce(const CeCall& c, float* loss, float* stat, float* co
     a.part = reinterpret_cast<float2*>(wk + p.part_at);
     a.zsum = c.smooth > 0.0f ? reinterpret_cast<float*>(wk + p.zsum_at) : nullptr;
     a.zt = reinterpret_cast<float*>(wk + p.zt_at);
-    e = c.dtype == RPFQ_F16 ? stats_mb<MmaF16>(a, s) : stats_mb<MmaBf16>(a, s);
+    const TileForm form = tile_form(c.M, c.V);
+    e = c.dtype == RPFQ_F16 ? tile_dispatch(form, StatsGo<MmaF16>{a, s}) : tile_dispatch(form, StatsGo<MmaBf16>{a, s});
     if (e != hipSuccess) return e;
     float* rows = c.reduction ? reinterpret_cast<float*>(wk + p.rows_at) : loss;
     const CeJoin j = {a.part, a.zsum, a.zt, c.target, c.M, c.V, c.ignore, (int)p.tiles_v, c.smooth, stat, rows};
@@ -715,7 +829,7 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
     a.dz = wk + p.dz_at;
     a.colsum = gb ? reinterpret_cast<float*>(wk + p.col_at) : nullptr;
     const TileOperand w = a.w;
-    float* dxp = p.dx_splits > 1 || p.pieces > 1 ? reinterpret_cast<float*>(wk + p.dx_at) : nullptr;
+    float* dxp = p.dx.splits > 1 || p.pieces > 1 ? reinterpret_cast<float*>(wk + p.dx_at) : nullptr;
     for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
         const int64_t n = std::min(p.piece, c.V - v0);
         a.v0 = v0;
@@ -723,8 +837,11 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         a.w.count = n;
         a.ldz = 2 * ((n + 7) & ~(int64_t)7);
         a.dz_plane = c.M * a.ldz;
-        e = c.dtype == RPFQ_F16 ? dz_mb<MmaF16, RPFQ_F16>(a, s)
-            : c.dtype == RPFQ_BF16 ? dz_mb<MmaBf16, RPFQ_BF16>(a, s) : dz_mb<MmaBf16, RPFQ_F32>(a, s);
+        const TileForm form = tile_form(c.M, n);
+        int col_rows = 0;
+        e = c.dtype == RPFQ_F16    ? tile_dispatch(form, DzGo<MmaF16, RPFQ_F16>{a, col_rows, s})
+            : c.dtype == RPFQ_BF16 ? tile_dispatch(form, DzGo<MmaBf16, RPFQ_BF16>{a, col_rows, s})
+                                   : tile_dispatch(form, DzGo<MmaBf16, RPFQ_F32>{a, col_rows, s});
         if (e != hipSuccess) return e;
         const TileOperand dzk = {a.dz, a.ldz, a.dz_plane, c.M}, dzt = {a.dz, a.ldz, a.dz_plane, n};
         if (gx) {
@@ -735,18 +852,15 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
             g.ck = n;
             g.M = c.M;
             g.N = c.D;
-            g.per = (int)((a.ldz + 63) / 64);
             g.planes = a.planes;
-            g.steps = g.per * (g.planes ? kPairs32 : 1);
-            g.splits = p.dx_splits;
+            g.splits = p.dx.splits;
             g.part = dxp;
             g.ldp = p.ldp;
             g.add = v0 > 0;
             g.factor = factor;
             g.out = gx;
             g.vec = c.D % 4 == 0 && reinterpret_cast<uintptr_t>(gx) % (4 * es) == 0;
-            e = c.dtype == RPFQ_F16 ? grad_go<false, MmaF16, RPFQ_F16>(g, s)
-                : c.dtype == RPFQ_BF16 ? grad_go<false, MmaBf16, RPFQ_BF16>(g, s) : grad_go<false, MmaBf16, RPFQ_F32>(g, s);
+            e = ce_grad<false>(c.dtype, p.dx.form, g, s);
             if (e != hipSuccess) return e;
         }
         if (gw) {
@@ -756,29 +870,26 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
             g.rk = g.ck = c.M;
             g.M = n;
             g.N = c.D;
-            g.per = (int)((c.M + 31) / 32);
             g.planes = a.planes;
-            g.steps = g.per * (g.planes ? kPairs32 : 1);
-            g.splits = p.dw_splits;
-            g.part = p.dw_splits > 1 ? reinterpret_cast<float*>(wk + p.dw_at) : nullptr;
+            g.splits = p.dw.splits;
+            g.part = p.dw.splits > 1 ? reinterpret_cast<float*>(wk + p.dw_at) : nullptr;
             g.ldp = p.ldp;
             g.factor = factor;
             g.out = reinterpret_cast<char*>(gw) + v0 * c.D * es;
             g.vec = c.D % 4 == 0 && reinterpret_cast<uintptr_t>(g.out) % (4 * es) == 0;
-            e = c.dtype == RPFQ_F16 ? grad_go<true, MmaF16, RPFQ_F16>(g, s)
-                : c.dtype == RPFQ_BF16 ? grad_go<true, MmaBf16, RPFQ_BF16>(g, s) : grad_go<true, MmaBf16, RPFQ_F32>(g, s);
+            e = ce_grad<true>(c.dtype, p.dw.form, g, s);
             if (e != hipSuccess) return e;
             if (g.part && (e = ce_sum(c.dtype, g.part, g.splits, n * p.ldp, n, c.D, p.ldp, factor, g.out, s)) != hipSuccess)
                 return e;
         }
         if (gb) {  // db: the column sums of the row tiles, as one row each
             const int bs = c.bias_dtype == RPFQ_F32 ? 4 : 2;
-            e = ce_sum(c.bias_dtype, a.colsum, a.tiles_m, a.ldz / 2, 1, n, a.ldz / 2, factor,
+            e = ce_sum(c.bias_dtype, a.colsum, col_rows, a.ldz / 2, 1, n, a.ldz / 2, factor,
                        reinterpret_cast<char*>(gb) + v0 * bs, s);
             if (e != hipSuccess) return e;
         }
     }
-    if (gx && dxp) return ce_sum(c.dtype, dxp, p.dx_splits, c.M * p.ldp, c.M, c.D, p.ldp, factor, gx, s);
+    if (gx && dxp) return ce_sum(c.dtype, dxp, p.dx.splits, c.M * p.ldp, c.M, c.D, p.ldp, factor, gx, s);
     return hipSuccess;
 }
 

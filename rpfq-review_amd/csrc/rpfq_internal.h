@@ -389,6 +389,9 @@ hipError_t launch_quantize_int8(const void* x, int dt, int64_t M, int64_t K, int
 hipError_t launch_linear_int8(const void* x, int xdt, const float* sx, const int8_t* w, int64_t ldw, const float* sw,
                               const float* bias, int64_t M, int64_t N, int64_t K, void* y, int ydt, void* work,
                               hipStream_t s);
+// Forms of a tile product (tile_gemm.h): rows of a tile, or 128 of them with
+// more steps on their way.
+enum TileForm { kTile32, kTile64, kTile128Deep, kTile128, kTile256 };
 // cross entropy of a linear classifier (linear_ce.hip)
 struct CeCall {
     const void *x, *w, *bias;  // [M, D], [V, D], [V] or NULL
@@ -398,11 +401,15 @@ struct CeCall {
     float smooth;
     int reduction;  // 0 none, 1 mean, 2 sum
 };
+struct CeSplit {
+    TileForm form;  // of a gradient's product, and parts of its k
+    int splits;
+};
 struct CePlan {
     int64_t ldk, ldp;       // elements of a row of k; of float32 partials
     bool pad;               // x and w are copied (rows of ldk, or three planes of them)
-    int64_t tiles_v, tiles_m, piece, pieces;
-    int dx_splits, dw_splits;
+    int64_t tiles_v, piece, pieces;
+    CeSplit dx, dw;
     size_t x_at, w_at, part_at, zsum_at, zt_at, rows_at, rho_at, factor_at, dz_at, col_at, dx_at, dw_at, bytes;
 };
 CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool backward);

@@ -70,22 +70,26 @@ __device__ __forceinline__ intx4 tile_rsrc(const char* p) {
 }
 constexpr uint32_t kTileOut = 0x80000000u;  // an offset past every resource's end
 
-// W elements of one operand (a tile's rows or columns), 64 bytes of k a step.
-// K layout in LDS: W rows of 64 B, chunk c of 16 B at c ^ ((row >> 2) & 3), so 16
-// rows of one chunk (a read of half a wave) fall on all 64 banks once.  T
-// layout: 32 k rows of 2 W bytes, chunk c at c ^ ((k & 3) << 2) (64 columns: c ^
-// (k & 2) << 1): the 4 rows x 64 B of a transposed read on distinct banks.
-template <int W, bool T>
+// W elements of one operand (a tile's rows or columns), KB bytes of k a step.
+// K layout in LDS: W rows of KB bytes, chunk c of 16 at c ^ ((row >> 2) & 3) (KB =
+// 64) or c ^ ((row >> 1) & 7) (128): 16 rows of one chunk, what half a wave's
+// read takes, fall on all 64 banks once (5.7 clocks a 1-KB read, 16 to 32
+// unswizzled).  T layout: KB / 2 k rows of 2 W bytes, chunk c at c ^ ((k & 3) <<
+// 2) (64 columns: c ^ (k & 2) << 1): the 4 rows x 64 B of a transposed read on
+// distinct banks.
+template <int W, bool T, int WAVES, int KB>
 struct TileSide {
-    static constexpr int BYTES = W * 64;
-    static constexpr int LOADS = W / 64;        // DMA loads per wave and step, 1 KB each
-    static constexpr int CH = W / 8;            // T: chunks of a k row
+    static constexpr int BYTES = W * KB;
+    static constexpr int LOADS = W * KB / 1024 / WAVES;  // DMA loads per wave and step, 1 KB each
+    static constexpr int CH = W / 8;                     // T: chunks of a k row
+    static constexpr int KC = KB / 16;                   // K: chunks of a row
     uint32_t v[LOADS];
     uint32_t kpos[LOADS];  // K: byte of k within a step; T: k row within a step
     const char* base;
     int64_t ld, plane;
 
     static __device__ __forceinline__ int swz(int k) { return CH >= 16 ? (k & 3) << 2 : (k & 2) << 1; }
+    static __device__ __forceinline__ int kswz(int row) { return KC == 4 ? (row >> 2) & 3 : (row >> 1) & 7; }
 
     __device__ __forceinline__ void init(const TileOperand& o, int64_t first, int wave, int lane) {
         ld = o.ld;
@@ -99,7 +103,7 @@ struct TileSide {
                 kpos[j] = (uint32_t)k;
                 v[j] = first + 8 * c < o.count ? (uint32_t)(k * o.ld + c * 16) : kTileOut;
             } else {
-                const int row = piece * 16 + (lane >> 2), c = (lane & 3) ^ ((lane >> 4) & 3);
+                const int row = piece * (64 / KC) + lane / KC, c = (lane % KC) ^ kswz(row);
                 kpos[j] = (uint32_t)(c * 16);
                 v[j] = first + row < o.count ? (uint32_t)(row * o.ld + c * 16) : kTileOut;
             }
@@ -107,27 +111,31 @@ struct TileSide {
     }
     // step `ks` of plane pl (k: bytes of a row (K) or rows (T)) to LDS at `lds`
     __device__ __forceinline__ void issue(int ks, int pl, int64_t k, uint32_t lds, int wave) {
-        const intx4 rs = tile_rsrc(base + pl * plane + (T ? (int64_t)ks * 32 * ld : (int64_t)ks * 64));
-        const int64_t left64 = T ? k - (int64_t)ks * 32 : k - (int64_t)ks * 64;
-        const uint32_t left = (uint32_t)(left64 > 64 ? 64 : left64);
+        constexpr int PER = T ? KB / 2 : KB;
+        const intx4 rs = tile_rsrc(base + pl * plane + (T ? (int64_t)ks * PER * ld : (int64_t)ks * PER));
+        const int64_t left64 = k - (int64_t)ks * PER;
+        const uint32_t left = (uint32_t)(left64 > PER ? PER : left64);
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) dma_buffer(rs, kpos[j] < left ? v[j] : kTileOut, lds + (wave * LOADS + j) * 1024);
     }
-    // where lane l reads block 0 of substep 0; frag() adds the rest
-    static __device__ __forceinline__ uint32_t at(int lane) {
+    // where lane l reads block 0 of substep s of a stage at 0
+    static __device__ __forceinline__ uint32_t at(int lane, int s) {
         const int r = lane & 31, g = lane >> 5;
-        if (!T) return (uint32_t)(r * 64 + ((g ^ ((r >> 2) & 3)) * 16));
+        if (!T) return (uint32_t)(r * KB + (((2 * s + g) ^ kswz(r)) * 16));
         const int i16 = lane & 15, hf = (lane >> 4) & 1, k = 8 * g + (i16 >> 2);
         return (uint32_t)(k * 2 * W + ((2 * hf + ((i16 & 3) >> 1)) * 16) + (i16 & 1) * 8);
     }
     // 16 bytes of k of the lane's element of block b (32 elements), substep s
-    static __device__ __forceinline__ uint4 frag(uint32_t stage, uint32_t at, int b, int s, int lane) {
+    static __device__ __forceinline__ uint4 frag(uint32_t stage, const uint32_t (&at)[KB / 32], int b, int s, int lane) {
         if (!T) {
-            // chunk 2 s + g: the swizzle is an xor, so substep 1 flips bit 1
-            return __builtin_bit_cast(uint4, *((lds_i4_t)(stage + (at ^ (uint32_t)(s * 32)) + b * 2048)));
+            uint32_t a = stage + at[s];
+            // one register and 16-bit offsets from it: for addresses past 64 KB
+            // the compiler took 8-byte reads instead (1,050 -> 1,290 TFLOP/s)
+            asm("" : "+v"(a));
+            return __builtin_bit_cast(uint4, *((lds_i4_t)a + b * 2 * KB));
         } else {
             const int k = (lane & 15) >> 2;  // modulo 4: what the swizzle looks at
-            const uint32_t a = stage + ((at + b * 64) ^ (uint32_t)(swz(k) * 16)) + s * 32 * W;
+            const uint32_t a = stage + ((at[0] + b * 64) ^ (uint32_t)(swz(k) * 16)) + s * 32 * W;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)a);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)(a + 8 * W));
             return __builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -135,22 +143,33 @@ struct TileSide {
     }
 };
 
-// Workgroup of 4 waves: 32 MB rows x 256 columns, wave w the columns 64 w ..
-// 64 w + 63 of every row, acc[j][i] the 32 x 32 block of columns 32 j and rows
-// 32 i: lane (r, g) holds row r and columns acc_row(v, g).  Both operands go
-// global -> LDS by DMA, three stages of 64 bytes of k, two steps ahead; two
-// workgroups share a CU, so one's epilogue runs beside the other's products.
-template <int MB, bool RT, bool CT, class Mma>
+// Workgroup of 4 WM waves: 32 MB WM rows x 256 columns, wave w the columns 64
+// (w % 4) .. + 63 of rows 32 MB (w / 4) .. + 32 MB - 1, acc[j][i] the 32 x 32
+// block of its columns 32 j and rows 32 i: lane (r, g) holds row r and columns
+// acc_row(v, g).  Both operands go global -> LDS by DMA, in S stages of KB bytes
+// of k, S - 1 steps ahead.  The forms that are used (bf16, normal operands;
+// K = 768 / 8192, K layouts):
+//   256 x 256, KB 128, S 2, one workgroup a CU: 1,215 / 1,294 TFLOP/s.  Half the
+//     LDS fill per product of a 128-row tile, which is bound by it (48 of 64
+//     bytes a clock from the vector cache at full matrix rate);
+//   128 x 256, KB 64, S 3, two a CU: 1,040 / 1,010;
+//   S 6 of 64 bytes, one a CU: launches of fewer tiles than CUs, where a step
+//     otherwise waits for its DMA (0.74 us a step with S 3).
+template <int MB, int WM, int S, int KB, bool RT, bool CT, class Mma>
 struct TileGemm {
-    static constexpr int RW = MB == 1 ? 64 : 32 * MB;  // rows of R loaded (64 at least: one DMA load a wave)
-    using R = TileSide<RW, RT>;
-    using C = TileSide<256, CT>;
+    static constexpr int WAVES = 4 * WM, THREADS = 64 * WAVES, ROWS = 32 * MB * WM;
+    static constexpr int RW = ROWS < 64 ? 64 : ROWS;  // rows of R loaded: one DMA load a wave at least
+    using R = TileSide<RW, RT, WAVES, KB>;
+    using C = TileSide<256, CT, WAVES, KB>;
     using acc_t = typename Mma::acc_t;
+    static constexpr int SUB = KB / 32;
     static constexpr int STAGE = R::BYTES + C::BYTES;
-    static constexpr int LDS = 3 * STAGE;
+    static constexpr int LDS = S * STAGE;
     static constexpr int LOADS = R::LOADS + C::LOADS;
+    // steps of k (bytes of a row where an operand is in K layout, else rows)
+    static constexpr int64_t steps(int64_t k) { return RT && CT ? (k + KB / 2 - 1) / (KB / 2) : (k + KB - 1) / KB; }
 
-    // Adds steps s0 .. s1 - 1 of the product; a step is 64 bytes of k of one
+    // Adds steps s0 .. s1 - 1 of the product; a step is KB bytes of k of one
     // pair of planes, `per` steps a pair.  rk, ck: k of the operands as issue() takes it.
     static __device__ __forceinline__ void run(const TileOperand& ro, const TileOperand& co, int64_t m0, int64_t n0,
                                                int64_t rk, int64_t ck, int per, bool planes, int s0, int s1, char* smem,
@@ -160,6 +179,7 @@ struct TileGemm {
         rs.init(ro, m0, wave, lane);
         cs.init(co, n0, wave, lane);
         const uint32_t lds = lds_addr(smem);
+        const int wc = wave & 3, wr = wave >> 2;
         int pair = s0 / per, ks = s0 - pair * per;
         auto issue = [&](int st) {
             int rp = 0, cp = 0;
@@ -171,53 +191,80 @@ struct TileGemm {
                 ++pair;
             }
         };
-        const uint32_t ra = R::at(lane), ca = C::at(lane);
-        if (s0 < s1) issue(0);
-        if (s0 + 1 < s1) issue(1);
+        uint32_t ra[SUB], ca[SUB];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) ra[u] = R::at(lane, u), ca[u] = C::at(lane, u);
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i)
+            if (s0 + i < s1) issue(i);
         auto step = [&](int s, int st) {
-            if (s + 1 < s1)
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+            // the steps behind s may still be on their way
+            if (s + S - 2 < s1)
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * LOADS) : "memory");
             else
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if (s + 2 < s1) issue((st + 2) % 3);  // read a step ago, by every wave
+            if (s + S - 1 < s1) issue((st + S - 1) % S);  // read a step ago, by every wave
             const uint32_t rst = lds + st * STAGE, cst = rst + R::BYTES;
-            uint4 c0[2], c1[2], r0[MB], r1[MB];
+            uint4 cf[2][2], rf[2][MB];  // of a substep and the next
+            auto read = [&](int u, int p) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) c0[j] = C::frag(cst, ca, 2 * wave + j, 0, lane);
+                for (int j = 0; j < 2; ++j) cf[p][j] = C::frag(cst, ca, 2 * wc + j, u, lane);
 #pragma unroll
-            for (int i = 0; i < MB; ++i) r0[i] = R::frag(rst, ra, i, 0, lane);
+                for (int i = 0; i < MB; ++i) rf[p][i] = R::frag(rst, ra, MB * wr + i, u, lane);
+            };
+            read(0, 0);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) c1[j] = C::frag(cst, ca, 2 * wave + j, 1, lane);
+            for (int u = 0; u < SUB; ++u) {
+                if (u + 1 < SUB) read(u + 1, (u + 1) & 1);
 #pragma unroll
-            for (int i = 0; i < MB; ++i) r1[i] = R::frag(rst, ra, i, 1, lane);
+                for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[j][i] = Mma::mma(c0[j], r0[i], acc[j][i]);
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[j][i] = Mma::mma(c1[j], r1[i], acc[j][i]);
+                    for (int j = 0; j < 2; ++j) acc[j][i] = Mma::mma(cf[u & 1][j], rf[u & 1][i], acc[j][i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         };
         int s = s0;
-        for (; s + 3 <= s1; s += 3) {
-            step(s, 0);
-            step(s + 1, 1);
-            step(s + 2, 2);
-        }
-        if (s < s1) step(s, 0);
-        if (s + 1 < s1) step(s + 1, 1);
+        for (; s + S <= s1; s += S)
+#pragma unroll
+            for (int i = 0; i < S; ++i) step(s + i, i);
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i)
+            if (s + i < s1) step(s + i, i);
         __builtin_amdgcn_s_barrier();  // the stages are free for the epilogue
         asm volatile("" ::: "memory");
     }
 };
 
-// One wave's 32 x 64 block through 8 KB of LDS of its own: put(v) takes the
-// accumulators' values, then out(row, column, 4 values) is called for whole
-// 256-byte pieces of rows (16 lanes a row, 4 columns each).
+// The form of a launch of M x N outputs: one round of the chip on the smallest
+// tiles that fill it (64 rows, 32 for few rows; a step there waits on its DMA
+// and not on the products), else the cheaper of 128- and 256-row tiles, whose
+// rounds cost 1.15 to 1.
+inline TileForm tile_form(int64_t M, int64_t N) {
+    const int64_t cus = device_cus(), tn = (N + 255) / 256;
+    if (M <= 32) return kTile32;
+    if ((M + 63) / 64 * tn <= cus) return kTile64;
+    const int64_t t128 = (M + 127) / 128 * tn, t256 = (M + 255) / 256 * tn;
+    if (t128 <= cus) return kTile128Deep;
+    return 20 * ((t256 + cus - 1) / cus) <= 23 * ((t128 + 2 * cus - 1) / (2 * cus)) ? kTile256 : kTile128;
+}
+// go.run<MB, WM, S, KB>() of a form
+template <class Go>
+inline hipError_t tile_dispatch(TileForm f, Go go) {
+    switch (f) {
+        case kTile32: return go.template run<1, 1, 6, 64>();
+        case kTile64: return go.template run<2, 1, 6, 64>();
+        case kTile128Deep: return go.template run<4, 1, 6, 64>();
+        case kTile128: return go.template run<4, 1, 3, 64>();
+        default: return go.template run<4, 2, 2, 128>();
+    }
+}
+
+// One wave's 32 x 64 block through 8 KB of LDS of its own: value(v, column)
+// makes the accumulators' values, then out(row, column, 4 values) is called for
+// whole 256-byte pieces of rows (16 lanes a row, 4 columns each).
 template <class Acc, class F, class Out>
 __device__ __forceinline__ void tile_rows(char* epi, const Acc& a0, const Acc& a1, int lane, F value, Out out) {
     const int r = lane & 31, g = lane >> 5, c = lane & 15, row4 = lane >> 4;
@@ -240,7 +287,39 @@ __device__ __forceinline__ void tile_rows(char* epi, const Acc& a0, const Acc& a
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
 }
+
+// The same for 16-bit outputs, half the LDS: value4(4 values, column) packs four
+// columns to 8 bytes, patch() may change the staged block (its byte of row r,
+// column c: tile_half_at), out(row, column, 8 values) stores 128-byte pieces.
+__device__ __forceinline__ int tile_half_at(int r, int c) { return r * 128 + (((c >> 3) ^ ((r >> 1) & 7)) * 16) + (c & 7) * 2; }
+template <class Acc, class F, class P, class Out>
+__device__ __forceinline__ void tile_rows_half(char* epi, const Acc& a0, const Acc& a1, int lane, F value4, P patch, Out out) {
+    const int r = lane & 31, g = lane >> 5;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int c = 32 * j + 8 * q + 4 * g;
+            const Acc& a = j ? a1 : a0;
+            *reinterpret_cast<uint2*>(epi + tile_half_at(r, c)) = value4(a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3], j, q);
+        }
+    patch();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int row = 8 * j + (lane >> 3), c = 8 * (lane & 7);
+        out(row, c, *reinterpret_cast<const uint4*>(epi + tile_half_at(row, c)));
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
 constexpr int kTileEpi = 8192;  // a wave's LDS in tile_rows
+
+template <int YDT>
+__device__ __forceinline__ uint32_t tile_pack2(float a, float b) {
+    return YDT == RPFQ_F16 ? cvt_pk(a, b) : pack_bf2(a, b);
+}
 
 // 4 values to columns n .. n + 3 of a row of N (those below N): one store
 // where `vec` says that rows are 4-element aligned.
@@ -251,16 +330,28 @@ __device__ __forceinline__ void tile_store4(void* y, int64_t row_off, int64_t n,
         if constexpr (YDT == RPFQ_F32) {
             *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(y) + row_off + n) = v;
         } else {
-            uint2 o;
-            o.x = YDT == RPFQ_F16 ? cvt_pk(v[0], v[1]) : pack_bf2(v[0], v[1]);
-            o.y = YDT == RPFQ_F16 ? cvt_pk(v[2], v[3]) : pack_bf2(v[2], v[3]);
-            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(y) + row_off + n) = o;
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(y) + row_off + n) =
+                make_uint2(tile_pack2<YDT>(v[0], v[1]), tile_pack2<YDT>(v[2], v[3]));
         }
         return;
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t)
         if (n + t < N) store1<YDT>(y, row_off + n + t, v[t]);
+}
+
+// 8 16-bit values to columns n .. n + 7 of a row of N (those below N): one store
+// where `vec` says that rows are 16-byte aligned.
+__device__ __forceinline__ void tile_store8(void* y, int64_t row_off, int64_t n, int64_t N, bool vec, uint4 v) {
+    uint16_t* d = reinterpret_cast<uint16_t*>(y) + row_off + n;
+    if (vec) {
+        if (n < N) *reinterpret_cast<uint4*>(d) = v;
+        return;
+    }
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+        if (n + t < N) d[t] = (uint16_t)(w[t >> 1] >> (16 * (t & 1)));
 }
 
 }  // namespace rpfq

@@ -925,7 +925,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         v = weight.shape[0]
         desc = N.CeDesc(m, v, d, ignore_index, N.dtype_code(x.dtype),
                         N.F32 if bias is None else N.dtype_code(bias.dtype), N.REDUCTIONS[reduction], smoothing)
-        stat = torch.empty(2 * m + 1, dtype=torch.float32, device=x.device)  # and the mean's factor
+        stat = torch.empty(3 * m + 1, dtype=torch.float32, device=x.device)  # and the mean's factor
         loss = torch.empty(m if reduction == "none" else (), dtype=torch.float32, device=x.device)
         lib = N.load()
         nwork = lib.rpfq_linear_cross_entropy_workspace_bytes(ctypes.byref(desc), 0)
@@ -935,7 +935,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         with N.on_device(x):
             N.check("rpfq_linear_cross_entropy", lib.rpfq_linear_cross_entropy(
                 ctypes.byref(desc), x.data_ptr(), weight.data_ptr(), N.ptr(bias), target.data_ptr(), loss.data_ptr(),
-                stat.data_ptr(), stat.data_ptr() + 8 * m, work.data_ptr(), nwork, N.stream_of(x)))
+                stat.data_ptr(), stat.data_ptr() + 12 * m, work.data_ptr(), nwork, N.stream_of(x)))
         ctx.desc = desc
         ctx.save_for_backward(x, weight, bias, target, stat)
         return loss
@@ -958,7 +958,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         with N.on_device(x):
             N.check("rpfq_linear_cross_entropy_grad", lib.rpfq_linear_cross_entropy_grad(
                 ctypes.byref(desc), x.data_ptr(), weight.data_ptr(), N.ptr(bias), target.data_ptr(), stat.data_ptr(),
-                stat.data_ptr() + 8 * desc.M, grad.data_ptr(), N.ptr(gx), N.ptr(gw), N.ptr(gb), work.data_ptr(), nwork,
+                stat.data_ptr() + 12 * desc.M, grad.data_ptr(), N.ptr(gx), N.ptr(gw), N.ptr(gb), work.data_ptr(), nwork,
                 N.stream_of(x)))
         return gx, gw, gb, None, None, None, None
 
