@@ -147,6 +147,9 @@ struct Int8Args {
     int tiles_m, tiles_n, group, vec;
 };
 
+template <class G>
+constexpr int kInt8Lds = G::LDS + 768 * 4;
+
 template <int MB, int WM, int S, int KB, int YDT>
 __global__ void __launch_bounds__(256 * WM, 2) int8_gemm_kernel(Int8Args a) {
     extern __shared__ __align__(16) char smem[];
@@ -159,39 +162,37 @@ __global__ void __launch_bounds__(256 * WM, 2) int8_gemm_kernel(Int8Args a) {
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = intx16{0};
     const int steps = (int)G::steps(a.K);
-    G::run(a.x, a.w, (int64_t)mt * G::ROWS, n0, a.K, a.K, steps, false, 0, steps, smem, wave, lane, acc);
+    // scales and biases of the tile's columns and scales of its rows
+    float* col = reinterpret_cast<float*>(smem + G::LDS);
+    G::run(a.x, a.w, (int64_t)mt * G::ROWS, n0, a.K, a.K, steps, false, 0, steps, smem, wave, lane, acc, [&] {
+        for (int c = threadIdx.x; c < 256; c += G::THREADS) {
+            const int64_t n = n0 + c;
+            col[c] = n < a.N ? a.sw[n] : 0.0f;
+            col[256 + c] = n < a.N && a.bias ? a.bias[n] : 0.0f;
+            const int64_t m = (int64_t)mt * G::ROWS + c;
+            if (c < G::ROWS) col[512 + c] = m < a.M ? a.sx[m] : 0.0f;
+        }
+    });
+    const float* sxs = col + 512 + 32 * MB * (wave >> 2) + (lane & 31);
     char* epi = smem + wave * kTileEpi;
     if constexpr (YDT == RPFQ_F32) {
         const int64_t n = nw + 4 * (lane & 15);
-        f32x4 sw = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-            if (n + t < a.N) {
-                sw[t] = a.sw[n + t];
-                if (a.bias) b[t] = a.bias[n + t];
-            }
+        const float* mine = col + 64 * (wave & 3) + 4 * (lane & 15);
+        const f32x4 sw = *reinterpret_cast<const f32x4*>(mine), b = *reinterpret_cast<const f32x4*>(mine + 256);
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
-            const int64_t mr = m0 + 32 * i + (lane & 31);
-            const float sx = a.sx[mr < a.M ? mr : a.M - 1];
+            const float sx = sxs[32 * i];
             tile_rows(epi, acc[0][i], acc[1][i], lane, [&](int v, int) { return (float)v * sx; },
                       [&](int row, int, f32x4 v) {
                           const int64_t m = m0 + 32 * i + row;
                           if (m < a.M) tile_store4<YDT>(a.y, m * a.N, n, a.N, a.vec, v * sw + b);
                       });
         }
-    } else {  // scales and biases of the tile's columns in LDS, as the accumulators hold them
-        float* col = reinterpret_cast<float*>(smem + G::WAVES * kTileEpi);
-        for (int c = threadIdx.x; c < 512; c += G::THREADS) {
-            const int64_t n = n0 + (c & 255);
-            col[c] = n >= a.N ? 0.0f : c < 256 ? a.sw[n] : a.bias ? a.bias[n] : 0.0f;
-        }
-        __syncthreads();
+    } else {
         const float* mine = col + 64 * (wave & 3) + 4 * (lane >> 5);
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
-            const int64_t mr = m0 + 32 * i + (lane & 31);
-            const float sx = a.sx[mr < a.M ? mr : a.M - 1];
+            const float sx = sxs[32 * i];
             tile_rows_half(
                 epi, acc[0][i], acc[1][i], lane,
                 [&](int v0, int v1, int v2, int v3, int j, int q) {
@@ -247,13 +248,13 @@ struct Int8Go {
         using G = TileGemm<MB, WM, S, KB, false, false, MmaI8>;
         static std::atomic<uint64_t> attr_done{0};
         const auto kernel = &int8_gemm_kernel<MB, WM, S, KB, YDT>;
-        const hipError_t e = set_lds_attr_once(reinterpret_cast<const void*>(kernel), G::LDS, attr_done);
+        const hipError_t e = set_lds_attr_once(reinterpret_cast<const void*>(kernel), kInt8Lds<G>, attr_done);
         if (e != hipSuccess) return e;
         a.tiles_m = (int)((a.M + G::ROWS - 1) / G::ROWS);
         a.tiles_n = (int)((a.N + 255) / 256);
         a.group = tile_group(a.tiles_n, 256 * a.K);
         hipLaunchKernelGGL((int8_gemm_kernel<MB, WM, S, KB, YDT>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(G::THREADS),
-                           G::LDS, s, a);
+                           kInt8Lds<G>, s, a);
         return hipGetLastError();
     }
 };

@@ -39,6 +39,14 @@ __device__ __forceinline__ float ce_gap(float a, float b) {
     return fabsf(a) <= kCeFar && fabsf(b) <= kCeFar ? a * kLog2e - b * kLog2e : (a - b) * kLog2e;
 }
 
+// What the gradients are multiplied by in the end.
+struct CeFactor {
+    const float* grad;  // of the loss, [1]
+    const float* coef;  // the mean's factor, or NULL
+    float undo;         // of dz's scale
+    __device__ __forceinline__ float operator()() const { return grad[0] * (coef ? coef[0] : 1.0f) * undo; }
+};
+
 struct CeArgs {
     TileOperand x, w;          // [M, D], [V, D], K layout
     const void* bias;          // [V] of bias_dt, or NULL
@@ -55,11 +63,15 @@ struct CeArgs {
     float* zsum;               // [tiles_n][M] sums of z, or NULL
     float* zt;                 // [M] the target's logit
     // backward
-    const float *stat, *rho;   // [3][M] maximum, 1 / sum, the target's logit; [M]
+    const float* stat;         // [3][M] maximum, 1 / sum, the target's logit
+    const float* rho;          // [M] weights of the rows in dz, or NULL: 1
+    int64_t ignore;
     float dz_scale;
+    char* xz;                  // x without its ignored rows, to be written here; or NULL
     char* dz;                  // [planes][M][ldz bytes]
     int64_t ldz, dz_plane;
-    float* colsum;             // [tiles_m][ldz / 2] or NULL
+    int64_t n8;                // columns of dz that are written: the piece's, in whole 16 bytes
+    float* colsum;             // [row waves][n8] or NULL
 };
 
 __device__ __forceinline__ float ce_load(const void* p, int dt, int64_t i) {
@@ -85,19 +97,28 @@ __device__ __forceinline__ void ce_bias(floatx16 (&acc)[2][MB], const float* bia
         }
 }
 
-// The 256 biases of a tile to LDS, added to the accumulators of a wave: -inf
-// past the last class.  Tiles without either are left as they are.
-template <int MB>
-__device__ __forceinline__ void ce_logits(const CeArgs& a, int64_t n0, float* sm, int wave, int lane, floatx16 (&acc)[2][MB]) {
-    if (!a.bias && n0 + 256 <= a.w.count) return;
-    if (threadIdx.x < 256) {
-        const int64_t n = n0 + threadIdx.x;
-        float b = n < a.w.count ? 0.0f : -__builtin_inff();
-        if (a.bias && n < a.w.count) b = ce_load(a.bias, a.bias_dt, a.v0 + n);
-        sm[threadIdx.x] = b;
-    }
-    __syncthreads();
-    ce_bias<MB>(acc, sm + 64 * (wave & 3), lane);
+// What the epilogues keep in LDS past the stages: the biases of a tile's
+// columns, -inf past the last class, and of dz's rows what they need.
+struct CeRow {
+    float top;  // the maximum
+    float f;    // p's factor; 0: a row that counts nowhere, NaN: one whose target is no class
+    float off;  // what is taken off every class
+    float dzt;  // dz of the target
+};
+template <int ROWS>
+struct CeLds {
+    float bias[256];
+    CeRow row[ROWS];
+    int t[ROWS];  // the target's column in the tile, or -1
+};
+
+__device__ __forceinline__ bool ce_biased(const CeArgs& a, int64_t n0) { return a.bias || n0 + 256 > a.w.count; }
+__device__ __forceinline__ void ce_stage_bias(const CeArgs& a, int64_t n0, float* sm) {
+    if (!ce_biased(a, n0) || threadIdx.x >= 256) return;
+    const int64_t n = n0 + threadIdx.x;
+    float b = n < a.w.count ? 0.0f : -__builtin_inff();
+    if (a.bias && n < a.w.count) b = ce_load(a.bias, a.bias_dt, a.v0 + n);
+    sm[threadIdx.x] = b;
 }
 
 // ---------------------------------------------------------------------------
@@ -116,10 +137,10 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_stats_kernel(CeArgs a) {
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
     const int per = (int)G::steps(a.kb), steps = a.planes ? kPairs32 * per : per;
-    G::run(a.x, a.w, m0, n0, a.kb, a.kb, per, a.planes, 0, steps, smem, wave, lane, acc);
-    float* sb = reinterpret_cast<float*>(smem);
-    float* sp = sb + 256;  // [4 column waves][rows][max, sum, sum of z]
-    ce_logits<MB>(a, n0, sb, wave, lane, acc);
+    float* sb = reinterpret_cast<float*>(smem + G::LDS);
+    G::run(a.x, a.w, m0, n0, a.kb, a.kb, per, a.planes, 0, steps, smem, wave, lane, acc, [&] { ce_stage_bias(a, n0, sb); });
+    float* sp = reinterpret_cast<float*>(smem);  // [4 column waves][rows][max, sum, sum of z]
+    if (ce_biased(a, n0)) ce_bias<MB>(acc, sb + 64 * (wave & 3), lane);
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
         const int row = 32 * (MB * (wave >> 2) + i) + r;
@@ -197,76 +218,21 @@ struct CeJoin {
     int64_t M, V, ignore;
     int tiles;
     float smooth;
+    int reduction;
     float* stat;  // [3][M]: maximum, 1 / sum of exp(z - maximum), the target's logit
     float* rows;  // [M] loss of each row, 0 where ignored
+    float* loss;  // the sum or the mean of them
+    float* coef;
 };
-
-// lse and loss of a row from its tiles: 16 lanes a row, in a fixed order.
-__global__ void __launch_bounds__(256) ce_join_kernel(CeJoin a) {
-    const int64_t m = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
-    const int q = threadIdx.x >> 4;  // 16 parts of the tiles
-    __shared__ float sm[3][16][17];
-    float mx = -__builtin_inff(), sum = 0.0f, zs = 0.0f;
-    if (m < a.M)
-        for (int t = q; t < a.tiles; t += 16) {
-            const float2 p = a.part[(int64_t)t * a.M + m];
-            const float n = fmaxf(mx, p.x), base = n == -__builtin_inff() ? 0.0f : n;
-            // a tile of -inf has sum 0, one with NaN has sum NaN whatever its maximum
-            const float add = p.y == 0.0f || p.y != p.y ? p.y : p.y * __builtin_amdgcn_exp2f(ce_gap(p.x, base));
-            sum = (sum == 0.0f ? 0.0f : sum * __builtin_amdgcn_exp2f(ce_gap(mx, base))) + add;
-            mx = n;
-            if (a.zsum) zs += a.zsum[(int64_t)t * a.M + m];
-        }
-    const int c = threadIdx.x & 15;
-    sm[0][c][q] = mx;
-    sm[1][c][q] = sum;
-    sm[2][c][q] = zs;
-    __syncthreads();
-    if (q != 0 || m >= a.M) return;
-    float top = -__builtin_inff();
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, sm[0][c][i]);
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    sum = zs = 0.0f;
-    for (int i = 0; i < 16; ++i) {
-        const float s = sm[1][c][i];
-        sum += s == 0.0f || s != s ? s : s * __builtin_amdgcn_exp2f(ce_gap(sm[0][c][i], base));
-        zs += sm[2][c][i];
-    }
-    // lse in 64 bits, from the exponent that the sum is relative to
-    const double lse = fabsf(base) <= kCeFar ? ((double)(base * kLog2e) + log2((double)sum)) / (double)kLog2e
-                                             : (double)base + log((double)sum);
-    const int64_t t = a.target[m];
-    const bool labelled = t >= 0 && t < a.V;
-    const float zt = labelled ? a.zt[m] : 0.0f;
-    float loss = 0.0f;
-    if (t != a.ignore) {
-        loss = __uint_as_float(0x7fc00000u);
-        if (labelled) {
-            double d = (1.0 - (double)a.smooth) * (lse - (double)zt);
-            if (a.zsum) d += (double)a.smooth * (lse - (double)zs / (double)a.V);
-            loss = (float)d;
-        }
-    }
-    a.stat[m] = base;
-    a.stat[a.M + m] = 1.0f / sum;
-    a.stat[2 * a.M + m] = zt;
-    a.rows[m] = loss;
-}
+constexpr int64_t kCeFewRows = 128;
 
 // Sum (reduction 2) or mean (1) of the rows' losses in a fixed order, and the
-// factor that the gradient takes from it: coef[0] = 1 or 1 / count (0 where no
-// row counts: its rows then have no gradient, their mean is NaN).
-__global__ void __launch_bounds__(1024) ce_reduce_kernel(const float* rows, const int64_t* target, int64_t M, int64_t ignore,
-                                                         int reduction, float* loss, float* coef) {
+// factor that the gradient takes from it: coef = 1 or 1 / count (0 where no row
+// counts: its rows then have no gradient, their mean is NaN).
+__device__ __forceinline__ void ce_reduce(const CeJoin& a, double s, int n) {
     __shared__ double sm[1024];
     __shared__ int cm[1024];
     const int t = threadIdx.x;
-    double s = 0.0;
-    int n = 0;
-    for (int64_t m = t; m < M; m += 1024) {
-        s += (double)rows[m];
-        n += target[m] != ignore;
-    }
     sm[t] = s;
     cm[t] = n;
     __syncthreads();
@@ -279,68 +245,110 @@ __global__ void __launch_bounds__(1024) ce_reduce_kernel(const float* rows, cons
     }
     if (t == 0) {
         const double c = (double)cm[0];
-        if (reduction != 0) loss[0] = (float)(reduction == 1 ? sm[0] / c : sm[0]);
-        coef[0] = reduction == 1 ? (cm[0] ? (float)(1.0 / c) : 0.0f) : 1.0f;
+        a.loss[0] = (float)(a.reduction == 1 ? sm[0] / c : sm[0]);
+        a.coef[0] = a.reduction == 1 ? (cm[0] ? (float)(1.0 / c) : 0.0f) : 1.0f;
     }
+}
+
+__global__ void __launch_bounds__(1024) ce_reduce_kernel(CeJoin a) {
+    double s = 0.0;
+    int n = 0;
+    for (int64_t m = threadIdx.x; m < a.M; m += 1024) {
+        s += (double)a.rows[m];
+        n += a.target[m] != a.ignore;
+    }
+    ce_reduce(a, s, n);
+}
+
+// lse and loss of a row from its tiles: 16 threads a row, in a fixed order.
+// ALL: one workgroup takes all rows and reduces them.
+template <bool ALL>
+__global__ void __launch_bounds__(1024) ce_join_kernel(CeJoin a) {
+    const int c = threadIdx.x & 63, q = threadIdx.x >> 6;  // row, one of 16 parts of the tiles
+    __shared__ float sm[3][64][17];
+    double total = 0.0;
+    int count = 0;
+    for (int64_t m0 = ALL ? 0 : (int64_t)blockIdx.x * 64; m0 < (ALL ? a.M : (int64_t)blockIdx.x * 64 + 64); m0 += 64) {
+        const int64_t m = m0 + c;
+        float mx = -__builtin_inff(), sum = 0.0f, zs = 0.0f;
+        if (m < a.M)
+            for (int t = q; t < a.tiles; t += 16) {
+                const float2 p = a.part[(int64_t)t * a.M + m];
+                const float n = fmaxf(mx, p.x), base = n == -__builtin_inff() ? 0.0f : n;
+                // a tile of -inf has sum 0, one with NaN has sum NaN whatever its maximum
+                const float add = p.y == 0.0f || p.y != p.y ? p.y : p.y * __builtin_amdgcn_exp2f(ce_gap(p.x, base));
+                sum = (sum == 0.0f ? 0.0f : sum * __builtin_amdgcn_exp2f(ce_gap(mx, base))) + add;
+                mx = n;
+                if (a.zsum) zs += a.zsum[(int64_t)t * a.M + m];
+            }
+        sm[0][c][q] = mx;
+        sm[1][c][q] = sum;
+        sm[2][c][q] = zs;
+        __syncthreads();
+        if (q == 0 && m < a.M) {
+            float top = -__builtin_inff();
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, sm[0][c][i]);
+            const float base = top == -__builtin_inff() ? 0.0f : top;
+            sum = zs = 0.0f;
+            for (int i = 0; i < 16; ++i) {
+                const float s = sm[1][c][i];
+                sum += s == 0.0f || s != s ? s : s * __builtin_amdgcn_exp2f(ce_gap(sm[0][c][i], base));
+                zs += sm[2][c][i];
+            }
+            // lse in 64 bits, from the exponent that the sum is relative to
+            const double lse = fabsf(base) <= kCeFar ? ((double)(base * kLog2e) + log2((double)sum)) / (double)kLog2e
+                                                     : (double)base + log((double)sum);
+            const int64_t t = a.target[m];
+            const bool labelled = t >= 0 && t < a.V;
+            const float zt = labelled ? a.zt[m] : 0.0f;
+            float loss = 0.0f;
+            if (t != a.ignore) {
+                loss = __uint_as_float(0x7fc00000u);
+                if (labelled) {
+                    double d = (1.0 - (double)a.smooth) * (lse - (double)zt);
+                    if (a.zsum) d += (double)a.smooth * (lse - (double)zs / (double)a.V);
+                    loss = (float)d;
+                }
+                ++count;
+            }
+            a.stat[m] = base;
+            a.stat[a.M + m] = 1.0f / sum;
+            a.stat[2 * a.M + m] = zt;
+            if (!ALL) a.rows[m] = loss;
+            total += (double)loss;
+        }
+        __syncthreads();
+    }
+    if (ALL) ce_reduce(a, total, count);
 }
 
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
-// rho[m], the weight of row m in dz (0: ignored, NaN: a target that is no
-// class), and factor[0], what the gradients are multiplied by in the end.
-// Reduction 0 divides the rows' gradients by the largest of them, so that dz
-// stays within [-1, 1].
-__global__ void __launch_bounds__(1024) ce_rho_kernel(const float* grad, const float* coef, const int64_t* target, int64_t M,
-                                                      int64_t V, int64_t ignore, int reduction, float undo, float* rho,
-                                                      float* factor) {
+// reduction none: rho[m] = grad[m] over the largest of the rows that count, so
+// that dz stays within [-1, 1], and that largest, factor[0].
+__global__ void __launch_bounds__(1024) ce_rho_kernel(const float* grad, const int64_t* target, int64_t M, int64_t ignore,
+                                                      float* rho, float* factor) {
     __shared__ float sm[1024];
     const int t = threadIdx.x;
     float top = 0.0f;
-    if (reduction == 0) {
-        for (int64_t m = t; m < M; m += 1024)
-            if (target[m] != ignore) top = fmaxf(top, fabsf(grad[m]));
-        sm[t] = top;
+    for (int64_t m = t; m < M; m += 1024)
+        if (target[m] != ignore) top = fmaxf(top, fabsf(grad[m]));
+    sm[t] = top;
+    __syncthreads();
+    for (int h = 512; h > 0; h >>= 1) {
+        if (t < h) sm[t] = fmaxf(sm[t], sm[t + h]);
         __syncthreads();
-        for (int h = 512; h > 0; h >>= 1) {
-            if (t < h) sm[t] = fmaxf(sm[t], sm[t + h]);
-            __syncthreads();
-        }
-        top = sm[0];
-        // no finite scale: the rows keep their gradients as they are
-        if (!(top > 0.0f) || top > 3.40282347e38f) top = 1.0f;
     }
-    for (int64_t m = t; m < M; m += 1024) {
-        const int64_t c = target[m];
-        const float r = reduction == 0 ? grad[m] / top : 1.0f;
-        rho[m] = c == ignore ? 0.0f : c < 0 || c >= V ? __uint_as_float(0x7fc00000u) : r;
-    }
-    if (t == 0) factor[0] = (reduction == 0 ? top : grad[0] * coef[0]) * undo;
+    top = sm[0];
+    // no finite scale: the rows keep their gradients as they are
+    if (!(top > 0.0f) || top > 3.40282347e38f) top = 1.0f;
+    for (int64_t m = t; m < M; m += 1024) rho[m] = grad[m] / top;
+    if (t == 0) factor[0] = top;
 }
 
-// x [M, D] as the operand of dw: rows that count nowhere are zeros, whatever
-// they hold (0 x NaN would reach every class), rows of ldx elements.
-__global__ void __launch_bounds__(256) ce_rows_kernel(const uint16_t* x, int64_t D, const int64_t* target, int64_t ignore,
-                                                      uint16_t* out, int64_t ldx, int64_t total8) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total8; i += (int64_t)gridDim.x * 256) {
-        const int64_t per = ldx / 8, m = i / per, d = (i - m * per) * 8;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (!target || target[m] != ignore) {
-            if (D == ldx) {
-                v = *reinterpret_cast<const uint4*>(x + m * D + d);
-            } else {
-                uint16_t e[8];
-#pragma unroll
-                for (int t = 0; t < 8; ++t) e[t] = d + t < D ? x[m * D + d + t] : (uint16_t)0;
-                __builtin_memcpy(&v, e, 16);
-            }
-        }
-        *reinterpret_cast<uint4*>(out + i * 8) = v;
-    }
-}
-
-// float32 rows as three bf16 terms, each the top 8 bits of what is left: exact
-// for every finite value.  target: as in ce_rows_kernel, or NULL.
+// A float32 as three bf16 terms, each the top 8 bits of what is left: exact for
+// every finite value.
 __device__ __forceinline__ void split3(float v, uint16_t& h, uint16_t& m, uint16_t& l) {
     const uint32_t u = __float_as_uint(v);
     if ((u & 0x7fffffffu) > 0x7f800000u) {
@@ -354,34 +362,62 @@ __device__ __forceinline__ void split3(float v, uint16_t& h, uint16_t& m, uint16
     l = (uint16_t)(__float_as_uint(r2) >> 16);
 }
 
-__global__ void __launch_bounds__(256) ce_planes_kernel(const float* x, int64_t rows, int64_t D, const int64_t* target,
-                                                        int64_t ignore, uint16_t* out, int64_t ld) {
-    const int64_t total = rows * (ld / 8), plane = rows * ld;
+// x [M, D] and w [V, D] as operands: rows of ld elements, float32 as three planes
+// of bf16 terms.  target: rows of x that it ignores are zeros, whatever they
+// hold (0 x NaN would reach every class of dw); NULL: all rows as they are.
+struct CeCopy {
+    const void* src[2];
+    uint16_t* dst[2];
+    int64_t rows[2];
+    int64_t D, ld;
+    const int64_t* target;
+    int64_t ignore;
+};
+template <bool F32>
+__global__ void __launch_bounds__(256) ce_copy_kernel(CeCopy a) {
+    const int64_t per = a.ld / 8, first = a.rows[0] * per, total = first + a.rows[1] * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t per = ld / 8, m = i / per, d = (i - m * per) * 8;
-        uint16_t h[8], k[8], l[8];
-        const bool on = !target || target[m] != ignore;
+        const int k = i >= first;
+        const int64_t at = k ? i - first : i, m = at / per, d = (at - m * per) * 8;
+        const bool on = k || !a.target || a.target[m] != a.ignore;
+        uint16_t* out = a.dst[k] + at * 8;
+        if constexpr (F32) {
+            const float* x = reinterpret_cast<const float*>(a.src[k]);
+            const int64_t plane = a.rows[k] * a.ld;
+            uint16_t h[8], mid[8], l[8];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) split3(on && d + t < D ? x[m * D + d + t] : 0.0f, h[t], k[t], l[t]);
-        __builtin_memcpy(out + i * 8, h, 16);
-        __builtin_memcpy(out + plane + i * 8, k, 16);
-        __builtin_memcpy(out + 2 * plane + i * 8, l, 16);
+            for (int t = 0; t < 8; ++t) split3(on && d + t < a.D ? x[m * a.D + d + t] : 0.0f, h[t], mid[t], l[t]);
+            __builtin_memcpy(out, h, 16);
+            __builtin_memcpy(out + plane, mid, 16);
+            __builtin_memcpy(out + 2 * plane, l, 16);
+        } else {
+            const uint16_t* x = reinterpret_cast<const uint16_t*>(a.src[k]);
+            uint16_t e[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) e[t] = on && d + t < a.D ? x[m * a.D + d + t] : (uint16_t)0;
+            __builtin_memcpy(out, e, 16);
+        }
     }
 }
 
 // Sums of 32 values over the 32 lanes of a half wave: lane r ends with the sum
 // of value r.  Each round halves the values: a lane keeps one half and hands
 // the other to its partner.
-__device__ __forceinline__ float ce_lane_sums(float (&v)[32], int lane) {
+template <int M>
+__device__ __forceinline__ void ce_lane_round(float (&v)[32], int lane) {
+    const bool up = lane & M;
 #pragma unroll
-    for (int m = 16; m > 0; m >>= 1) {
-        const bool up = lane & m;
-#pragma unroll
-        for (int k = 0; k < m; ++k) {
-            const float give = up ? v[k] : v[k + m], keep = up ? v[k + m] : v[k];
-            v[k] = keep + __shfl_xor(give, m, 64);
-        }
+    for (int k = 0; k < M; ++k) {
+        const float give = up ? v[k] : v[k + M], keep = up ? v[k + M] : v[k];
+        v[k] = keep + __shfl_xor(give, M, 64);
     }
+}
+__device__ __forceinline__ float ce_lane_sums(float (&v)[32], int lane) {
+    ce_lane_round<16>(v, lane);
+    ce_lane_round<8>(v, lane);
+    ce_lane_round<4>(v, lane);
+    ce_lane_round<2>(v, lane);
+    ce_lane_round<1>(v, lane);
     return v[0];
 }
 
@@ -400,33 +436,54 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
     const int per = (int)G::steps(a.kb), steps = a.planes ? kPairs32 * per : per;
-    G::run(a.x, a.w, m0, n0, a.kb, a.kb, per, a.planes, 0, steps, smem, wave, lane, acc);
-    char* epi = smem + wave * kTileEpi;
-    ce_logits<MB>(a, n0, reinterpret_cast<float*>(smem + G::WAVES * kTileEpi), wave, lane, acc);
+    CeLds<G::ROWS>& sh = *reinterpret_cast<CeLds<G::ROWS>*>(smem + G::LDS);
     const float even = a.smooth / (float)a.V;
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-        const int64_t mr = mw + 32 * i + r;
-        // rows that count nowhere: exp2(-inf) times 0
-        float top = __builtin_inff(), f = 0.0f, off = 0.0f, dzt = 0.0f;
-        int t = -1;  // the target's column among the wave's
-        if (mr < a.M) {
-            const float rho = a.rho[mr] * a.dz_scale;
-            const int64_t tt = a.target[mr] - a.v0 - nw;
-            if (rho != 0.0f) {
-                const float inv = a.stat[a.M + mr];
-                top = a.stat[mr];
-                f = inv * rho;
-                off = even * rho;
-                if (tt >= 0 && tt < 64) {
-                    t = (int)tt;
+    G::run(a.x, a.w, m0, n0, a.kb, a.kb, per, a.planes, 0, steps, smem, wave, lane, acc, [&] {
+        ce_stage_bias(a, n0, sh.bias);
+        if (threadIdx.x < G::ROWS) {
+            const int64_t m = m0 + threadIdx.x;
+            CeRow row = {0.0f, 0.0f, 0.0f, 0.0f};
+            int t = -1;
+            if (m < a.M) {
+                const int64_t label = a.target[m], at = label - a.v0 - n0;
+                const float inv = a.stat[a.M + m], zt = a.stat[2 * a.M + m], own = a.rho ? a.rho[m] : 1.0f;
+                row.top = a.stat[m];
+                const float rho = label == a.ignore             ? 0.0f
+                                  : label < 0 || label >= a.V ? __uint_as_float(0x7fc00000u)
+                                                                : own * a.dz_scale;
+                if (rho != 0.0f) {
+                    row.f = inv * rho;
+                    row.off = even * rho;
+                    if (at >= 0 && at < 256) t = (int)at;
                     // p - 1 before the factors: what is left of a p near 1 keeps its bits
-                    dzt = (__builtin_amdgcn_exp2f(ce_gap_z(a.stat[2 * a.M + mr], top)) * inv - even - (1.0f - a.smooth)) * rho;
+                    row.dzt = (__builtin_amdgcn_exp2f(ce_gap_z(zt, row.top)) * inv - even - (1.0f - a.smooth)) * rho;
                 }
             }
+            sh.row[threadIdx.x] = row;
+            sh.t[threadIdx.x] = t;
         }
-        const bool plain = !__any(fabsf(top) > kCeFar && top != __builtin_inff());
-        const float base = fabsf(top) > kCeFar && top != __builtin_inff() ? top : top * kLog2e;
+        if (a.xz) {  // the row tile's share of x, a part of it for each column tile
+            const uint32_t per16 = (uint32_t)(a.kb / 16), rows = (uint32_t)(a.M - m0 < G::ROWS ? a.M - m0 : G::ROWS);
+            const uint32_t all = rows * per16, share = (all + a.tiles_n - 1) / a.tiles_n;
+            const uint32_t end = (nt + 1) * share < all ? (nt + 1) * share : all;
+            for (uint32_t i = nt * share + threadIdx.x; i < end; i += G::THREADS) {
+                const int64_t m = m0 + i / per16, at = m * a.kb + (i % per16) * 16;
+                const uint4 v = *reinterpret_cast<const uint4*>(a.x.p + at);
+                *reinterpret_cast<uint4*>(a.xz + at) = a.target[m] != a.ignore ? v : make_uint4(0, 0, 0, 0);
+            }
+        }
+    });
+    char* epi = smem + wave * kTileEpi;
+    if (ce_biased(a, n0)) ce_bias<MB>(acc, sh.bias + 64 * (wave & 3), lane);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        const CeRow row = sh.row[32 * (MB * (wave >> 2) + i) + r];
+        const float top = row.top, f = row.f, off = row.off, dzt = row.dzt;
+        // the target's column among the wave's
+        int t = sh.t[32 * (MB * (wave >> 2) + i) + r] - 64 * (wave & 3);
+        t = t >= 0 && t < 64 ? t : -1;
+        const bool plain = !__any(fabsf(top) > kCeFar);
+        const float base = top * kLog2e;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -435,6 +492,12 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
                 const float e = plain ? ce_exp2(z, base) : __builtin_amdgcn_exp2f(ce_gap_z(z, top));
                 acc[j][i][v] = __builtin_fmaf(e, f, -off);
             }
+        if (__any(f == 0.0f)) {  // whatever such a row holds
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) acc[j][i][v] = f == 0.0f ? 0.0f : acc[j][i][v];
+        }
         if (a.w.count - n0 < 256) {  // columns past the last class, for the operands' padding
 #pragma unroll
             for (int j = 0; j < 2; ++j)
@@ -454,7 +517,7 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
             tile_rows(epi, acc[0][i], acc[1][i], lane, [](float v, int) { return v; },
                       [&](int row, int, f32x4 v) {
                           const int64_t m = mw + 32 * i + row;
-                          if (m >= a.M || 2 * n >= a.ldz) return;
+                          if (m >= a.M || n >= a.n8) return;
                           char* d = a.dz + m * a.ldz + 2 * n;
                           uint16_t h[4], k[4], l[4];
 #pragma unroll
@@ -475,7 +538,7 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
                 },
                 [&](int row, int c, uint4 v) {
                     const int64_t m = mw + 32 * i + row, n = nw + c;
-                    if (m < a.M && 2 * n < a.ldz) *reinterpret_cast<uint4*>(a.dz + m * a.ldz + 2 * n) = v;
+                    if (m < a.M && n < a.n8) *reinterpret_cast<uint4*>(a.dz + m * a.ldz + 2 * n) = v;
                 });
         }
     }
@@ -491,7 +554,7 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
             }
         const float sum = ce_lane_sums(cs, lane);
         const int64_t n = nw + 32 * (r >> 4) + acc_row(r & 15, g);
-        if (2 * n < a.ldz) a.colsum[((int64_t)mt * WM + (wave >> 2)) * (a.ldz / 2) + n] = sum;
+        if (n < a.n8) a.colsum[((int64_t)mt * WM + (wave >> 2)) * a.n8 + n] = sum;
     }
 }
 
@@ -504,7 +567,7 @@ struct CeGrad {
     float* part;      // [splits][M][ldp], or NULL: the gradient itself, rounded
     int64_t ldp;
     int add;          // part holds the pieces before
-    const float* factor;
+    CeFactor factor;
     void* out;        // [M, N]
     int vec;
 };
@@ -525,9 +588,9 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_grad_kernel(CeGrad a) {
     floatx16 acc[2][MB];
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
-    G::run(a.r, a.c, m0, n0, a.rk, a.ck, per, a.planes, s0, s1, smem, wave, lane, acc);
+    G::run(a.r, a.c, m0, n0, a.rk, a.ck, per, a.planes, s0, s1, smem, wave, lane, acc, [] {});
     const int64_t n = n0 + 64 * (wave & 3) + 4 * (lane & 15);
-    const float f = a.part ? 1.0f : a.factor[0];
+    const float f = a.part ? 1.0f : a.factor();
     float* part = a.part ? a.part + (int64_t)sp * a.M * a.ldp : nullptr;
 #pragma unroll
     for (int i = 0; i < MB; ++i)
@@ -548,14 +611,22 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_grad_kernel(CeGrad a) {
 // out = factor * sum of the partials, in their order.
 template <int DT>
 __global__ void __launch_bounds__(256) ce_sum_kernel(const float* part, int parts, int64_t stride, int64_t rows, int64_t N,
-                                                     int64_t ldp, const float* factor, void* out, int vec) {
-    const float f = factor[0];
+                                                     int64_t ldp, CeFactor factor, void* out, int vec) {
+    const float f = factor();
     const int64_t per = ldp / 4, total = rows * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t m = i / per, n = (i - m * per) * 4;
         const f32x4* p = reinterpret_cast<const f32x4*>(part + m * ldp + n);
         f32x4 v = p[0];
-        for (int s = 1; s < parts; ++s) v += p[s * (stride / 4)];
+        int s = 1;
+        for (; s + 8 <= parts; s += 8) {  // eight loads on their way, added in order
+            f32x4 w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = p[(s + k) * (stride / 4)];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v += w[k];
+        }
+        for (; s < parts; ++s) v += p[s * (stride / 4)];
         tile_store4<DT>(out, m * N, n, N, vec, v * f);
     }
 }
@@ -564,22 +635,23 @@ __global__ void __launch_bounds__(256) ce_sum_kernel(const float* part, int part
 // plan and launches
 // ---------------------------------------------------------------------------
 // The form and the split of k (`steps` of 64 bytes) with the least time for a
-// gradient of rows x cols: rounds of the chip in units of a 256-row tile's step,
-// a few for a tile's start and end, and the partials' way through memory.
+// gradient of rows x cols: rounds of the chip in units of a 256-row tile's step
+// (0.9 us), a few for a tile's start and end, and the partials' way through
+// memory (about 5 TB/s, and a launch).
 static CeSplit ce_split(int64_t rows, int64_t cols, int64_t steps) {
     const int64_t cus = device_cus(), tn = (cols + 255) / 256;
     CeSplit best = {kTile128, 1};
     double cost = 1e300;
     for (int s = 1; s <= 64 && (s == 1 || 4 * s <= steps); ++s) {
         const double n = (double)((steps + s - 1) / s);
-        const double join = s > 1 ? 8.0 + (double)s * rows * cols * 8.0 / 2e6 : 0.0;
+        const double join = s > 1 ? 7.0 + (double)s * rows * cols * 8.0 / 4.5e6 : 0.0;
         for (const TileForm f : {kTile64, kTile128Deep, kTile128, kTile256}) {
             const int64_t tall = f == kTile64 ? 64 : f == kTile256 ? 256 : 128;
             const int64_t units = (rows + tall - 1) / tall * tn * s;
             double c;
-            if (f == kTile64 || f == kTile128Deep) c = units > cus ? 1e300 : n * (f == kTile64 ? 0.45 : 0.6) + 8.0;
-            else if (f == kTile128) c = (double)((units + 2 * cus - 1) / (2 * cus)) * (1.15 * n + 8.0);
-            else c = (double)((units + cus - 1) / cus) * (n + 10.0);
+            if (f == kTile64 || f == kTile128Deep) c = units > cus ? 1e300 : n * (f == kTile64 ? 0.38 : 0.48) + 4.0;
+            else if (f == kTile128) c = (double)((units + 2 * cus - 1) / (2 * cus)) * (1.15 * n + 5.0);
+            else c = (double)((units + cus - 1) / cus) * (n + 5.0);
             if (c + join < cost) {
                 cost = c + join;
                 best = {f, s};
@@ -591,6 +663,12 @@ static CeSplit ce_split(int64_t rows, int64_t cols, int64_t steps) {
 
 // Classes of a piece: dz within kCePiece bytes, whole tiles, pieces alike.
 constexpr int64_t kCePiece = 1LL << 30;
+// Bytes of a row of dz with n classes: 16-byte pieces, and not a multiple of 4
+// KB, where a tile's rows would all lie on the same channels.
+static int64_t ce_ldz(int64_t n) {
+    const int64_t ld = 2 * ((n + 7) & ~(int64_t)7);
+    return ld % 4096 == 0 ? ld + 256 : ld;
+}
 
 CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool backward) {
     CePlan p = {};
@@ -621,7 +699,7 @@ CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool back
     p.pieces = (p.tiles_v + fit - 1) / fit;
     p.piece = (p.tiles_v + p.pieces - 1) / p.pieces * 256;  // classes
     if (p.piece > V) p.piece = (V + 7) & ~(int64_t)7;
-    p.dz_at = take(2 * planes * M * p.piece);
+    p.dz_at = take(planes * M * (2 * p.piece + 256));
     p.col_at = take(4 * ((M + 31) / 32 + 8) * p.piece);
     // float32 partials, rows of whole 16 bytes
     p.ldp = (D + 3) & ~(int64_t)3;
@@ -636,31 +714,34 @@ CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool back
 static unsigned blocks_of(int64_t n) { return (unsigned)(n < 1 ? 1 : n > 16384 ? 16384 : n); }
 
 // The operands of the logits: as they are, or padded / split copies in `work`.
-// target: rows of x that it ignores are zero (backward).
-static hipError_t ce_operands(const CePlan& p, int dt, const void* x, const void* w, int64_t M, int64_t V, int64_t D,
-                              char* wk, CeArgs& a, hipStream_t s) {
+// target: rows of x that it ignores are zero there (backward).
+static hipError_t ce_operands(const CePlan& p, const CeCall& c, const int64_t* target, char* wk, CeArgs& a, hipStream_t s) {
     a.kb = 2 * p.ldk;
-    a.planes = dt == RPFQ_F32;
-    a.x = {reinterpret_cast<const char*>(x), a.kb, 0, M};
-    a.w = {reinterpret_cast<const char*>(w), a.kb, 0, V};
+    a.planes = c.dtype == RPFQ_F32;
+    a.x = {reinterpret_cast<const char*>(c.x), a.kb, 0, c.M};
+    a.w = {reinterpret_cast<const char*>(c.w), a.kb, 0, c.V};
+    a.bias = c.bias;
+    a.bias_dt = c.bias_dtype;
+    a.target = c.target;
+    a.M = c.M;
+    a.V = c.V;
+    a.smooth = c.smooth;
+    a.ignore = c.ignore;
     if (!p.pad) return hipSuccess;
-    const void* src[2] = {x, w};
-    const int64_t rows[2] = {M, V};
-    const size_t at[2] = {p.x_at, p.w_at};
-    TileOperand* op[2] = {&a.x, &a.w};
-    for (int i = 0; i < 2; ++i) {
-        const int64_t total = rows[i] * (p.ldk / 8);
-        uint16_t* d = reinterpret_cast<uint16_t*>(wk + at[i]);
-        if (dt == RPFQ_F32)
-            hipLaunchKernelGGL(ce_planes_kernel, dim3(blocks_of((total + 255) / 256)), dim3(256), 0, s,
-                               reinterpret_cast<const float*>(src[i]), rows[i], D, (const int64_t*)nullptr, (int64_t)0, d, p.ldk);
-        else
-            hipLaunchKernelGGL(ce_rows_kernel, dim3(blocks_of((total + 255) / 256)), dim3(256), 0, s,
-                               reinterpret_cast<const uint16_t*>(src[i]), D, (const int64_t*)nullptr, (int64_t)0, d, p.ldk,
-                               total);
-        op[i]->p = reinterpret_cast<const char*>(d);
-        op[i]->plane = 2 * rows[i] * p.ldk;
-    }
+    const CeCopy k = {{c.x, c.w},
+                      {reinterpret_cast<uint16_t*>(wk + p.x_at), reinterpret_cast<uint16_t*>(wk + p.w_at)},
+                      {c.M, c.V},
+                      c.D,
+                      p.ldk,
+                      target,
+                      c.ignore};
+    const dim3 grid(blocks_of(((c.M + c.V) * (p.ldk / 8) + 255) / 256));
+    if (a.planes) hipLaunchKernelGGL(ce_copy_kernel<true>, grid, dim3(256), 0, s, k);
+    else hipLaunchKernelGGL(ce_copy_kernel<false>, grid, dim3(256), 0, s, k);
+    a.x.p = wk + p.x_at;
+    a.w.p = wk + p.w_at;
+    a.x.plane = 2 * c.M * p.ldk;
+    a.w.plane = 2 * c.V * p.ldk;
     return hipGetLastError();
 }
 
@@ -677,13 +758,13 @@ struct StatsGo {
     hipError_t run() {
         using G = TileGemm<MB, WM, S, KB, false, false, Mma>;
         static std::atomic<uint64_t> done{0};
-        const hipError_t e = ce_lds(&ce_stats_kernel<MB, WM, S, KB, Mma>, G::LDS, done);
+        const hipError_t e = ce_lds(&ce_stats_kernel<MB, WM, S, KB, Mma>, G::LDS + 1024, done);
         if (e != hipSuccess) return e;
         a.tiles_m = (int)((a.M + G::ROWS - 1) / G::ROWS);
         a.tiles_n = (int)((a.w.count + 255) / 256);
         a.group = tile_group(a.tiles_n, 256 * a.kb);
         hipLaunchKernelGGL((ce_stats_kernel<MB, WM, S, KB, Mma>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(G::THREADS),
-                           G::LDS, s, a);
+                           G::LDS + 1024, s, a);
         return hipGetLastError();
     }
 };
@@ -696,15 +777,16 @@ struct DzGo {
     template <int MB, int WM, int S, int KB>
     hipError_t run() {
         using G = TileGemm<MB, WM, S, KB, false, false, Mma>;
+        constexpr int lds = G::LDS + (int)sizeof(CeLds<G::ROWS>);
         static std::atomic<uint64_t> done{0};
-        const hipError_t e = ce_lds(&ce_dz_kernel<MB, WM, S, KB, Mma, DT>, G::LDS, done);
+        const hipError_t e = ce_lds(&ce_dz_kernel<MB, WM, S, KB, Mma, DT>, lds, done);
         if (e != hipSuccess) return e;
         a.tiles_m = (int)((a.M + G::ROWS - 1) / G::ROWS);
         a.tiles_n = (int)((a.w.count + 255) / 256);
         a.group = tile_group(a.tiles_n, 256 * a.kb);
         col_rows = a.tiles_m * WM;
         hipLaunchKernelGGL((ce_dz_kernel<MB, WM, S, KB, Mma, DT>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(G::THREADS),
-                           G::LDS, s, a);
+                           lds, s, a);
         return hipGetLastError();
     }
 };
@@ -715,7 +797,7 @@ struct GradGo {
     hipStream_t s;
     template <int MB, int WM, int S, int KB>
     hipError_t run() {
-        if constexpr (MB == 1) {
+        if constexpr (MB == 1 && WM == 1) {
             return hipErrorInvalidValue;  // ce_split takes 64 rows at least
         } else {
             using G = TileGemm<MB, WM, S, KB, RT, true, Mma>;
@@ -739,7 +821,7 @@ static hipError_t ce_grad(int dt, TileForm form, CeGrad& g, hipStream_t s) {
 }
 
 static hipError_t ce_sum(int dt, const float* part, int parts, int64_t stride, int64_t rows, int64_t N, int64_t ldp,
-                         const float* factor, void* out, hipStream_t s) {
+                         CeFactor factor, void* out, hipStream_t s) {
     const int es = dt == RPFQ_F32 ? 4 : 2;
     const int vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * es) == 0;
     const dim3 grid(blocks_of((rows * (ldp / 4) + 255) / 256));
@@ -760,14 +842,8 @@ hipError_t launch_linear_ce(const CeCall& c, float* loss, float* stat, float* co
     const CePlan p = ce_plan(c.dtype, c.M, c.V, c.D, c.reduction, false);
     char* wk = reinterpret_cast<char*>(work);
     CeArgs a = {};
-    hipError_t e = ce_operands(p, c.dtype, c.x, c.w, c.M, c.V, c.D, wk, a, s);
+    hipError_t e = ce_operands(p, c, nullptr, wk, a, s);
     if (e != hipSuccess) return e;
-    a.bias = c.bias;
-    a.bias_dt = c.bias_dtype;
-    a.target = c.target;
-    a.M = c.M;
-    a.V = c.V;
-    a.smooth = c.smooth;
     a.part = reinterpret_cast<float2*>(wk + p.part_at);
     a.zsum = c.smooth > 0.0f ? reinterpret_cast<float*>(wk + p.zsum_at) : nullptr;
     a.zt = reinterpret_cast<float*>(wk + p.zt_at);
@@ -775,11 +851,17 @@ hipError_t launch_linear_ce(const CeCall& c, float* loss, float* stat, float* co
     e = c.dtype == RPFQ_F16 ? tile_dispatch(form, StatsGo<MmaF16>{a, s}) : tile_dispatch(form, StatsGo<MmaBf16>{a, s});
     if (e != hipSuccess) return e;
     float* rows = c.reduction ? reinterpret_cast<float*>(wk + p.rows_at) : loss;
-    const CeJoin j = {a.part, a.zsum, a.zt, c.target, c.M, c.V, c.ignore, (int)p.tiles_v, c.smooth, stat, rows};
-    hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)((c.M + 15) / 16)), dim3(256), 0, s, j);
+    const CeJoin j = {a.part, a.zsum, a.zt, c.target, c.M, c.V, c.ignore, (int)p.tiles_v, c.smooth, c.reduction, stat, rows, loss,
+                      coef};
+    // few rows: the sum over them by the same workgroup (one launch less, 4 us)
+    if (c.reduction && c.M <= kCeFewRows) {
+        hipLaunchKernelGGL(ce_join_kernel<true>, dim3(1), dim3(1024), 0, s, j);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(ce_join_kernel<false>, dim3((unsigned)((c.M + 63) / 64)), dim3(1024), 0, s, j);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     if (c.reduction) {
-        hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(1024), 0, s, rows, c.target, c.M, c.ignore, c.reduction, loss, coef);
+        hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(1024), 0, s, j);
         e = hipGetLastError();
     }
     return e;
@@ -789,42 +871,26 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
                                  void* gb, void* work, hipStream_t s) {
     const CePlan p = ce_plan(c.dtype, c.M, c.V, c.D, c.reduction, true);
     char* wk = reinterpret_cast<char*>(work);
-    const int planes = c.dtype == RPFQ_F32 ? 3 : 1;
     const int es = c.dtype == RPFQ_F32 ? 4 : 2;
     CeArgs a = {};
-    hipError_t e = ce_operands(p, c.dtype, c.x, c.w, c.M, c.V, c.D, wk, a, s);
+    hipError_t e = ce_operands(p, c, c.target, wk, a, s);
     if (e != hipSuccess) return e;
-    float* rho = reinterpret_cast<float*>(wk + p.rho_at);
-    float* factor = reinterpret_cast<float*>(wk + p.factor_at);
     const float scale = c.dtype == RPFQ_F16 ? 32768.0f : 1.0f;
-    hipLaunchKernelGGL(ce_rho_kernel, dim3(1), dim3(1024), 0, s, grad, coef, c.target, c.M, c.V, c.ignore, c.reduction,
-                       1.0f / scale, rho, factor);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    // x for dw: its ignored rows as zeros
-    TileOperand xz = a.x;
-    if (gw) {
-        uint16_t* d = reinterpret_cast<uint16_t*>(wk + p.x_at);
-        const int64_t total = c.M * (p.ldk / 8);
-        const dim3 grid(blocks_of((total + 255) / 256));
-        if (planes == 3)
-            hipLaunchKernelGGL(ce_planes_kernel, grid, dim3(256), 0, s, reinterpret_cast<const float*>(c.x), c.M, c.D, c.target,
-                               c.ignore, d, p.ldk);
-        else
-            hipLaunchKernelGGL(ce_rows_kernel, grid, dim3(256), 0, s, reinterpret_cast<const uint16_t*>(c.x), c.D, c.target,
-                               c.ignore, d, p.ldk, total);
+    CeFactor factor = {grad, c.reduction == 1 ? coef : nullptr, 1.0f / scale};
+    if (c.reduction == 0) {
+        float* rho = reinterpret_cast<float*>(wk + p.rho_at);
+        float* top = reinterpret_cast<float*>(wk + p.factor_at);
+        hipLaunchKernelGGL(ce_rho_kernel, dim3(1), dim3(1024), 0, s, grad, c.target, c.M, c.ignore, rho, top);
         if ((e = hipGetLastError()) != hipSuccess) return e;
-        xz.p = reinterpret_cast<const char*>(d);
-        xz.plane = 2 * c.M * p.ldk;
-        a.x = xz;  // the logits of ignored rows are not looked at
+        a.rho = rho;
+        factor.grad = top;
     }
-    a.bias = c.bias;
-    a.bias_dt = c.bias_dtype;
-    a.target = c.target;
-    a.M = c.M;
-    a.V = c.V;
-    a.smooth = c.smooth;
+    TileOperand xz = a.x;  // x of dw: its ignored rows as zeros
+    if (gw && !p.pad) {
+        xz.p = wk + p.x_at;
+        a.xz = wk + p.x_at;
+    }
     a.stat = stat;
-    a.rho = rho;
     a.dz_scale = scale;
     a.dz = wk + p.dz_at;
     a.colsum = gb ? reinterpret_cast<float*>(wk + p.col_at) : nullptr;
@@ -835,7 +901,8 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         a.v0 = v0;
         a.w.p = w.p + v0 * w.ld;
         a.w.count = n;
-        a.ldz = 2 * ((n + 7) & ~(int64_t)7);
+        a.ldz = ce_ldz(n);
+        a.n8 = (n + 7) & ~(int64_t)7;
         a.dz_plane = c.M * a.ldz;
         const TileForm form = tile_form(c.M, n);
         int col_rows = 0;
@@ -843,12 +910,13 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
             : c.dtype == RPFQ_BF16 ? tile_dispatch(form, DzGo<MmaBf16, RPFQ_BF16>{a, col_rows, s})
                                    : tile_dispatch(form, DzGo<MmaBf16, RPFQ_F32>{a, col_rows, s});
         if (e != hipSuccess) return e;
+        a.xz = nullptr;  // written with the first piece
         const TileOperand dzk = {a.dz, a.ldz, a.dz_plane, c.M}, dzt = {a.dz, a.ldz, a.dz_plane, n};
         if (gx) {
             CeGrad g = {};
             g.r = dzk;
             g.c = {a.w.p, w.ld, w.plane, p.ldk};
-            g.rk = a.ldz;
+            g.rk = 2 * a.n8;
             g.ck = n;
             g.M = c.M;
             g.N = c.D;
@@ -884,7 +952,7 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         }
         if (gb) {  // db: the column sums of the row tiles, as one row each
             const int bs = c.bias_dtype == RPFQ_F32 ? 4 : 2;
-            e = ce_sum(c.bias_dtype, a.colsum, col_rows, a.ldz / 2, 1, n, a.ldz / 2, factor,
+            e = ce_sum(c.bias_dtype, a.colsum, col_rows, a.n8, 1, n, a.n8, factor,
                        reinterpret_cast<char*>(gb) + v0 * bs, s);
             if (e != hipSuccess) return e;
         }

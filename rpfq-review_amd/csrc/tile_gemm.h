@@ -153,8 +153,9 @@ struct TileSide {
 //     LDS fill per product of a 128-row tile, which is bound by it (48 of 64
 //     bytes a clock from the vector cache at full matrix rate);
 //   128 x 256, KB 64, S 3, two a CU: 1,040 / 1,010;
-//   S 6 of 64 bytes, one a CU: launches of fewer tiles than CUs, where a step
-//     otherwise waits for its DMA (0.74 us a step with S 3).
+//   64 x 256 and 128 x 256 of eight waves, KB 128, S 3, one a CU: launches of
+//     fewer tiles than CUs (333 x 10,007 x 2,496: 27 and 34 us; four waves with
+//     S 6 of 64 bytes 40 and 43).
 template <int MB, int WM, int S, int KB, bool RT, bool CT, class Mma>
 struct TileGemm {
     static constexpr int WAVES = 4 * WM, THREADS = 64 * WAVES, ROWS = 32 * MB * WM;
@@ -170,10 +171,13 @@ struct TileGemm {
     static constexpr int64_t steps(int64_t k) { return RT && CT ? (k + KB / 2 - 1) / (KB / 2) : (k + KB - 1) / KB; }
 
     // Adds steps s0 .. s1 - 1 of the product; a step is KB bytes of k of one
-    // pair of planes, `per` steps a pair.  rk, ck: k of the operands as issue() takes it.
+    // pair of planes, `per` steps a pair.  rk, ck: k of the operands as issue()
+    // takes it.  meanwhile(): what the epilogue wants in LDS past the stages,
+    // loaded while the first steps are on their way (s0 < s1).
+    template <class F>
     static __device__ __forceinline__ void run(const TileOperand& ro, const TileOperand& co, int64_t m0, int64_t n0,
                                                int64_t rk, int64_t ck, int per, bool planes, int s0, int s1, char* smem,
-                                               int wave, int lane, acc_t (&acc)[2][MB]) {
+                                               int wave, int lane, acc_t (&acc)[2][MB], F meanwhile) {
         R rs;
         C cs;
         rs.init(ro, m0, wave, lane);
@@ -197,6 +201,7 @@ struct TileGemm {
 #pragma unroll
         for (int i = 0; i < S - 1; ++i)
             if (s0 + i < s1) issue(i);
+        meanwhile();
         auto step = [&](int s, int st) {
             // the steps behind s may still be on their way
             if (s + S - 2 < s1)
@@ -254,9 +259,9 @@ inline TileForm tile_form(int64_t M, int64_t N) {
 template <class Go>
 inline hipError_t tile_dispatch(TileForm f, Go go) {
     switch (f) {
-        case kTile32: return go.template run<1, 1, 6, 64>();
-        case kTile64: return go.template run<2, 1, 6, 64>();
-        case kTile128Deep: return go.template run<4, 1, 6, 64>();
+        case kTile32: return go.template run<1, 1, 3, 128>();
+        case kTile64: return go.template run<1, 2, 3, 128>();
+        case kTile128Deep: return go.template run<2, 2, 3, 128>();
         case kTile128: return go.template run<4, 1, 3, 64>();
         default: return go.template run<4, 2, 2, 128>();
     }
