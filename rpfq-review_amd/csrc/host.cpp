@@ -8,12 +8,17 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/autocast_mode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstring>
+#include <vector>
 
 #include "../../include/rpfq.h"
 
@@ -29,7 +34,9 @@ constexpr double kMostOps = 1.5e9;
 #define RPFQ_HOST_CALLS(X)                                                                              \
     X(rpfq_wide_linear_kernel) X(rpfq_row_scales) X(rpfq_wide_linear_scaled)                            \
     X(rpfq_layer_norm_wide_linear_fusable) X(rpfq_layer_norm_wide_linear) X(rpfq_act_quant_wide_linear) \
-    X(rpfq_attention)
+    X(rpfq_attention) X(rpfq_last_error) X(rpfq_linear_int8_workspace_bytes) X(rpfq_linear_int8)        \
+    X(rpfq_linear_cross_entropy_workspace_bytes) X(rpfq_linear_cross_entropy)                           \
+    X(rpfq_linear_cross_entropy_grad) X(rpfq_adamw)
 struct Api {
 #define X(f) decltype(&::f) f;
     RPFQ_HOST_CALLS(X)
@@ -254,6 +261,266 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+bool needs_grad(const at::Tensor* t) { return t && t->defined() && at::GradMode::is_enabled() && t->requires_grad(); }
+
+// Tensors that stand for others (vmap, dual numbers) are left to torch's own rules.
+bool transformed(const at::Tensor& t) {
+    constexpr c10::DispatchKeySet keys{c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                       c10::DispatchKey::Batched, c10::DispatchKey::Functionalize};
+    return t.key_set().has_any(keys) || t._fw_grad(0).defined();
+}
+
+at::ScalarType dtype_or(PyObject* o, at::ScalarType t) {
+    if (o == Py_None) return t;
+    return THPDtype_Check(o) ? reinterpret_cast<THPDtype*>(o)->scalar_type : at::ScalarType::Undefined;
+}
+
+void* stream_on(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+// linear_int8(x, weight, weight_scale, bias, out_dtype)
+PyObject* linear_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const float *scale, *bias;
+    const at::Tensor* x = n == 5 && api.rpfq_linear_int8 ? plain(a[0]) : nullptr;
+    const at::Tensor* w = x ? plain(a[1]) : nullptr;
+    if (!w || x->dim() < 1 || w->dim() != 2 || w->scalar_type() != at::kChar || x->size(-1) != w->size(1) || !rows16(*x) ||
+        x->numel() == 0 || (w->size(1) > 1 && w->stride(1) != 1) || w->size(0) < 1 || transformed(*x))
+        Py_RETURN_NONE;
+    const int64_t out = w->size(0), k = w->size(1), m = x->numel() / k;
+    const int64_t ld = out > 1 ? w->stride(0) : std::max(k, w->stride(0));
+    const at::ScalarType yt = dtype_or(a[4], x->scalar_type());
+    const int xdt = dtype_code(x->scalar_type()), ydt = dtype_code(yt);
+    const at::Tensor* b = a[3] == Py_None ? nullptr : plain(a[3]);
+    if (xdt < 0 || ydt < 0 || ld < k || !vec(a[2], out, &scale) || !scale || !vec(a[3], out, &bias) || needs_grad(x) ||
+        needs_grad(b) || w->device() != x->device() || plain(a[2])->device() != x->device() ||
+        (b && b->device() != x->device()) || plain(a[2])->dim() != 1 || (b && b->dim() != 1))
+        Py_RETURN_NONE;
+    at::Tensor y;
+    int rc;
+    {
+        Unlocked u;
+        const c10::DeviceGuard guard(x->device());
+        c10::SmallVector<int64_t, 6> shape(x->sizes().begin(), x->sizes().end());
+        shape.back() = out;
+        y = at::empty(shape, x->options().dtype(yt));
+        const int8_t* wp = reinterpret_cast<const int8_t*>(w->data_ptr());
+        const size_t bytes = api.rpfq_linear_int8_workspace_bytes(x->data_ptr(), xdt, m, out, k, wp, ld);
+        at::Tensor work;
+        if (bytes) work = at::empty({(int64_t)bytes}, x->options().dtype(at::kByte));
+        rc = api.rpfq_linear_int8(x->data_ptr(), xdt, nullptr, wp, ld, scale, bias, m, out, k, y.data_ptr(), ydt,
+                                  bytes ? work.data_ptr() : nullptr, bytes, stream_on(*x));
+    }
+    return done(rc, y);
+    END_HANDLE_TH_ERRORS
+}
+
+// The cross entropy of a classifier under autograd, as ops._LinearCrossEntropy.
+struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
+    static rpfq_ce_desc describe(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, int64_t ignore,
+                                 double smoothing, int64_t reduction) {
+        return {x.size(0), w.size(0), x.size(1), ignore, dtype_code(x.scalar_type()),
+                bias.defined() ? dtype_code(bias.scalar_type()) : RPFQ_F32, (int32_t)reduction, (float)smoothing};
+    }
+    static void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+    // (loss, stat)
+    static std::pair<at::Tensor, at::Tensor> loss(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target,
+                                                  const at::Tensor& bias, const rpfq_ce_desc& d) {
+        const c10::DeviceGuard guard(x.device());
+        const auto f32 = x.options().dtype(at::kFloat).requires_grad(false);
+        at::Tensor stat = at::empty({3 * d.M + 1}, f32);
+        at::Tensor out = d.reduction == RPFQ_REDUCE_NONE ? at::empty({d.M}, f32) : at::empty({}, f32);
+        const size_t bytes = api.rpfq_linear_cross_entropy_workspace_bytes(&d, 0);
+        at::Tensor work = at::empty({(int64_t)bytes}, f32.dtype(at::kByte));
+        float* s = stat.data_ptr<float>();
+        const int rc = api.rpfq_linear_cross_entropy(&d, x.data_ptr(), w.data_ptr(), ptr(bias), target.data_ptr<int64_t>(),
+                                                     out.data_ptr<float>(), s, s + 3 * d.M, work.data_ptr(), bytes,
+                                                     stream_on(x));
+        TORCH_CHECK(rc == RPFQ_OK, "rpfq_linear_cross_entropy: ", api.rpfq_last_error());
+        return {out, stat};
+    }
+
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
+                              const at::Tensor& target, const std::optional<at::Tensor>& given, int64_t ignore,
+                              double smoothing, int64_t reduction) {
+        const at::Tensor bias = given ? *given : at::Tensor();
+        auto [out, stat] = loss(x, w, target, bias, describe(x, w, bias, ignore, smoothing, reduction));
+        ctx->save_for_backward({x, w, target, bias, stat});
+        ctx->saved_data["ignore"] = ignore;
+        ctx->saved_data["smoothing"] = smoothing;
+        ctx->saved_data["reduction"] = reduction;
+        return out;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &w = saved[1], &target = saved[2], &bias = saved[3], &stat = saved[4];
+        const c10::DeviceGuard guard(x.device());
+        const rpfq_ce_desc d = describe(x, w, bias, ctx->saved_data["ignore"].toInt(), ctx->saved_data["smoothing"].toDouble(),
+                                        ctx->saved_data["reduction"].toInt());
+        torch::autograd::variable_list out(7);
+        at::Tensor gx, gw, gb;
+        {
+            const at::NoGradGuard plain_results;
+            const at::Tensor g = grads[0].to(at::kFloat).contiguous();
+            if (ctx->needs_input_grad(0)) gx = at::empty(x.sizes(), x.options());
+            if (ctx->needs_input_grad(1)) gw = at::empty(w.sizes(), w.options());
+            if (bias.defined() && ctx->needs_input_grad(3)) gb = at::empty(bias.sizes(), bias.options());
+            if (!gx.defined() && !gw.defined() && !gb.defined()) return out;
+            const size_t bytes = api.rpfq_linear_cross_entropy_workspace_bytes(&d, 1);
+            at::Tensor work = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+            const float* s = stat.const_data_ptr<float>();
+            const int rc = api.rpfq_linear_cross_entropy_grad(&d, x.data_ptr(), w.data_ptr(), ptr(bias),
+                                                              target.data_ptr<int64_t>(), s, s + 3 * d.M,
+                                                              g.const_data_ptr<float>(), ptr(gx), ptr(gw), ptr(gb),
+                                                              work.data_ptr(), bytes, stream_on(x));
+            TORCH_CHECK(rc == RPFQ_OK, "rpfq_linear_cross_entropy_grad: ", api.rpfq_last_error());
+        }
+        out[0] = gx;
+        out[1] = gw;
+        out[3] = gb;
+        if (at::GradMode::is_enabled()) {  // create_graph: these gradients cannot be differentiated again
+            auto error = std::make_shared<torch::autograd::DelayedError>(
+                "linear_cross_entropy is differentiable once", (int)out.size());
+            torch::autograd::variable_list wrapped(out.size());
+            for (size_t i = 0; i < out.size(); ++i)
+                if (out[i].defined()) {
+                    at::Tensor t = out[i].detach();
+                    t.requires_grad_(true);
+                    wrapped[i] = t;
+                }
+            return (*error)(std::move(wrapped));
+        }
+        return out;
+    }
+};
+
+// linear_cross_entropy(x, weight, target, bias, ignore_index, smoothing, reduction)
+PyObject* linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t ignore, reduction;
+    const at::Tensor* x = n == 7 && api.rpfq_linear_cross_entropy ? plain(a[0]) : nullptr;
+    const at::Tensor* w = x ? plain(a[1]) : nullptr;
+    const at::Tensor* t = w ? plain(a[2]) : nullptr;
+    const at::Tensor* b = a[3] == Py_None ? nullptr : plain(a[3]);
+    if (!t || (a[3] != Py_None && !b) || !number(a[4], &ignore) || !number(a[6], &reduction)) Py_RETURN_NONE;
+    const double smoothing = PyFloat_AsDouble(a[5]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    const at::Tensor none;
+    const at::Tensor& bias = b ? *b : none;
+    if (x->dim() != 2 || w->dim() != 2 || x->size(1) != w->size(1) || x->numel() == 0 || w->numel() == 0 || t->dim() != 1 ||
+        t->scalar_type() != at::kLong || t->size(0) != x->size(0) || !t->is_contiguous() ||
+        x->scalar_type() != w->scalar_type() || dtype_code(x->scalar_type()) < 0 || !rows16(*x) || !rows16(*w) ||
+        w->device() != x->device() || t->device() != x->device() || !(smoothing >= 0.0 && smoothing <= 1.0) || reduction < 0 ||
+        reduction > 2 || at::autocast::is_autocast_enabled(at::kCUDA) || transformed(*x) || transformed(*w) ||
+        (b && (b->dim() != 1 || b->size(0) != w->size(0) || !b->is_contiguous() || dtype_code(b->scalar_type()) < 0 ||
+               b->device() != x->device() || transformed(*b))))
+        Py_RETURN_NONE;
+    const rpfq_ce_desc d = CrossEntropy::describe(*x, *w, bias, ignore, smoothing, reduction);
+    if (!api.rpfq_linear_cross_entropy_workspace_bytes(&d, 0)) Py_RETURN_NONE;
+    at::Tensor y;
+    {
+        Unlocked u;
+        if (needs_grad(x) || needs_grad(w) || needs_grad(b))
+            y = CrossEntropy::apply(*x, *w, *t, b ? std::optional<at::Tensor>(*b) : std::nullopt, ignore, smoothing, reduction);
+        else
+            y = CrossEntropy::loss(*x, *w, *t, bias, d).first;
+    }
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// The tensors of a list, or false where it is not a list of plain ones.
+bool tensors(PyObject* list, std::vector<const at::Tensor*>& out) {
+    if (!PyList_CheckExact(list)) return false;
+    const Py_ssize_t n = PyList_GET_SIZE(list);
+    out.resize(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject* o = PyList_GET_ITEM(list, i);
+        if (!THPVariable_Check(o)) return false;  // parameters among them
+        const at::Tensor& t = THPVariable_Unpack(o);
+        if (!t.is_cuda() || t.layout() != at::kStrided || !t.is_contiguous() || t.is_inference() || t.is_neg() || t.is_conj() ||
+            t.key_set().has(c10::DispatchKey::Python))
+            return false;
+        out[i] = &t;
+    }
+    return true;
+}
+
+// adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, step,
+//       (lr, beta1, beta2, eps, weight_decay), lr, grad_scale, found_inf): True where
+// the step was taken; lists of scales are empty with 32-bit states.
+PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    std::vector<const at::Tensor*> p, g, m, v, sm, sv;
+    if (n != 11 || !api.rpfq_adamw || !tensors(a[0], p) || !tensors(a[1], g) || !tensors(a[2], m) || !tensors(a[3], v) ||
+        !tensors(a[4], sm) || !tensors(a[5], sv) || p.empty() || !PyTuple_CheckExact(a[7]) || PyTuple_GET_SIZE(a[7]) != 5)
+        Py_RETURN_NONE;
+    const size_t count = p.size();
+    const bool small = !sm.empty();
+    if (g.size() != count || m.size() != count || v.size() != count || sm.size() != (small ? count : 0) || sv.size() != sm.size())
+        Py_RETURN_NONE;
+    rpfq_adamw_hyper h;
+    double* field = &h.lr;
+    for (int i = 0; i < 5; ++i) field[i] = PyFloat_AsDouble(PyTuple_GET_ITEM(a[7], i));
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    const at::Tensor* scalar[4];  // step, lr, grad_scale, found_inf
+    for (int i = 0; i < 4; ++i) {
+        PyObject* o = a[i == 0 ? 6 : 7 + i];
+        scalar[i] = o == Py_None ? nullptr : plain(o);
+        if (o == Py_None ? i == 0 : !scalar[i] || scalar[i]->scalar_type() != at::kFloat || scalar[i]->numel() != 1) Py_RETURN_NONE;
+    }
+    const at::Device device = scalar[0]->device();
+    for (int i = 1; i < 4; ++i)
+        if (scalar[i] && scalar[i]->device() != device) Py_RETURN_NONE;
+    const at::ScalarType type = p[0]->scalar_type();
+    const int code = dtype_code(type);
+    if (code < 0 || scalar[0]->is_inference()) Py_RETURN_NONE;
+    std::vector<rpfq_adamw_tensor> table(count);
+    std::vector<const void*> seen;
+    seen.reserve(3 * count);
+    for (size_t i = 0; i < count; ++i) {
+        const int64_t size = p[i]->numel();
+        if (p[i]->scalar_type() != type || g[i]->scalar_type() != type || g[i]->sizes() != p[i]->sizes() ||
+            m[i]->scalar_type() != (small ? at::kChar : at::kFloat) || v[i]->scalar_type() != (small ? at::kByte : at::kFloat) ||
+            m[i]->numel() != size || v[i]->numel() != size || p[i]->device() != device || g[i]->device() != device ||
+            m[i]->device() != device || v[i]->device() != device)
+            Py_RETURN_NONE;
+        rpfq_adamw_tensor& t = table[i];
+        t = {p[i]->data_ptr(), g[i]->data_ptr(), m[i]->data_ptr(), v[i]->data_ptr(), nullptr, nullptr, size};
+        if (small) {
+            for (const at::Tensor* s : {sm[i], sv[i]})
+                if (s->scalar_type() != at::kFloat || s->numel() != (size + 255) / 256 || s->device() != device) Py_RETURN_NONE;
+            t.exp_avg_scale = sm[i]->data_ptr<float>();
+            t.exp_avg_sq_scale = sv[i]->data_ptr<float>();
+        }
+        if (size) seen.insert(seen.end(), {t.param, t.exp_avg, t.exp_avg_sq});
+    }
+    std::sort(seen.begin(), seen.end());
+    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_NONE;
+    int rc;
+    {
+        Unlocked u;
+        const c10::DeviceGuard guard(device);
+        at::Tensor work = at::empty({8}, scalar[0]->options().requires_grad(false));
+        auto at_ = [&](int i) { return scalar[i] ? scalar[i]->data_ptr<float>() : nullptr; };
+        rc = api.rpfq_adamw(table.data(), (int64_t)count, code, small ? 8 : 32, &h, at_(0), at_(1), at_(2), at_(3),
+                            work.data_ptr<float>(), stream_on(*scalar[0]));
+    }
+    if (rc != RPFQ_OK) Py_RETURN_NONE;
+    for (const auto* list : {&p, &m, &v, &sm, &sv})
+        for (const at::Tensor* t : *list) t->unsafeGetTensorImpl()->bump_version();
+    scalar[0]->unsafeGetTensorImpl()->bump_version();
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(addresses): the functions named by CALLS, in that order.
 PyObject* bind(PyObject*, PyObject* addresses) {
     Api next;
@@ -278,6 +545,9 @@ PyMethodDef methods[] = {
     {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear)), METH_FASTCALL, nullptr},
     {"layer_norm_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm_linear)), METH_FASTCALL, nullptr},
     {"act_quant_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(act_quant_linear)), METH_FASTCALL, nullptr},
+    {"linear_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_int8)), METH_FASTCALL, nullptr},
+    {"linear_cross_entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_cross_entropy)), METH_FASTCALL, nullptr},
+    {"adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -876,6 +876,11 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     (out_dtype then says what y is).  weight int8 [N, K] (rows may be wider
     apart: multiples of 16 bytes, K too, are read in place), weight_scale
     float32 [N].  K <= 131072.  No gradient."""
+    host = N.host()
+    if host is not None and x_scale is None:
+        y = host.linear_int8(x, weight, weight_scale, bias, out_dtype)
+        if y is not None:
+            return y
     N.require_same_device(x, weight=weight, weight_scale=weight_scale, bias=bias, x_scale=x_scale)
     if weight.dtype != torch.int8 or weight.dim() != 2:
         raise ValueError("weight must be int8 [N, K]")
@@ -975,6 +980,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     target that is no class makes its row's loss and the gradients NaN.
     Gradients of x, weight and bias, once differentiable; float32 sums in a
     fixed order."""
+    host = N.host()
+    if host is not None:
+        loss = host.linear_cross_entropy(x, weight, target, bias, ignore_index, label_smoothing, N.REDUCTIONS.get(reduction))
+        if loss is not None:
+            return loss
     N.require_same_device(x, weight=weight, target=target, bias=bias)
     if reduction not in N.REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(N.REDUCTIONS)}, got {reduction!r}")
@@ -1033,6 +1043,12 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, step: torch.Tensor, *, lr=1e-3, 
         raise ValueError("8-bit states take both exp_avg_scales and exp_avg_sq_scales")
     sm = list(exp_avg_scales) if small else []
     sv = list(exp_avg_sq_scales) if small else []
+    host = N.host()
+    if host is not None:
+        lr_dev = lr if isinstance(lr, torch.Tensor) else None
+        if host.adamw(params, grads, ms, vs, sm, sv, step, (0.0 if lr_dev is not None else lr, *betas, eps, weight_decay),
+                      lr_dev, grad_scale, found_inf):
+            return
     if not len(grads) == len(ms) == len(vs) == n or small and not len(sm) == len(sv) == n:
         raise ValueError("adamw: the lists must be of one length")
     scalars = {"step": step, "grad_scale": grad_scale, "found_inf": found_inf}

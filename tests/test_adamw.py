@@ -10,6 +10,17 @@ import pytest
 import torch
 
 DEV = "cuda"
+
+
+@pytest.fixture(autouse=True, params=["native", "ctypes"])
+def host_path(request, monkeypatch):
+    """Every test on the native host path and on the Python one behind it."""
+    if request.param == "ctypes":
+        from quant_models import _native
+
+        monkeypatch.setattr(_native, "host", lambda: None)
+
+
 HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 E24 = 2.0 ** -24
 SIZES = [(1,), (3,), (255,), (256,), (257,), (64, 33), (4096,), (4097,), (1000, 13), (5, 0), (3, 5, 7), (70000,)]

@@ -8,6 +8,17 @@ import pytest
 import torch
 
 DEV = "cuda"
+
+
+@pytest.fixture(autouse=True, params=["native", "ctypes"])
+def host_path(request, monkeypatch):
+    """Every test on the native host path and on the Python one behind it."""
+    if request.param == "ctypes":
+        from quant_models import _native
+
+        monkeypatch.setattr(_native, "host", lambda: None)
+
+
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 

@@ -13,6 +13,17 @@ import torch
 import torch.nn.functional as F
 
 DEV = "cuda"
+
+
+@pytest.fixture(autouse=True, params=["native", "ctypes"])
+def host_path(request, monkeypatch):
+    """Every test on the native host path and on the Python one behind it."""
+    if request.param == "ctypes":
+        from quant_models import _native
+
+        monkeypatch.setattr(_native, "host", lambda: None)
+
+
 HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 ROUND = {torch.float32: 2.0 ** -22, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}  # of dz
 
