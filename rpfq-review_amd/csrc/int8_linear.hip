@@ -210,9 +210,121 @@ __global__ void __launch_bounds__(256 * WM, 2) int8_gemm_kernel(Int8Args a) {
     }
 }
 
+// Few rows (M <= 16, serving's single tokens): one launch, x quantized by every
+// workgroup (its codes in LDS, M K <= kInt8FewCodes), the weights streamed once.
+// Workgroup = 16 channels; its four waves take a quarter of K each in steps of
+// 64 (v_mfma_i32_16x16x64_i8, the rows past M zero), whose loads are all
+// independent, and add up their int32 sums in LDS.  Bound by the latency of
+// two reads, x and the weights, and by HBM for large weights.  1 x 768 -> 1000
+// fp16 3.9 us; quantizer and tile kernel 3 + 7.
+constexpr int64_t kInt8FewCodes = 32768;
+struct Int8Few {
+    const void* x;
+    const int8_t* w;
+    const float *sw, *bias;
+    void* y;
+    int64_t ldw, N;
+    int M, K;
+};
+constexpr int int8_few_pitch(int64_t K) { return (int)((K + 63) / 64 * 64 + 16); }
+
+template <int XDT, int YDT>
+__global__ void __launch_bounds__(256) int8_few_kernel(Int8Few a) {
+    extern __shared__ __align__(16) char smem[];
+    __shared__ float sx[16];
+    __shared__ int part[4][16][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const int steps = (a.K + 63) / 64, pitch = int8_few_pitch(a.K);
+    // weights of this wave's first steps, on their way while x is quantized
+    const int s0 = steps * wave / 4, s1 = steps * (wave + 1) / 4;
+    const int64_t row = n0 + r < a.N ? n0 + r : a.N - 1;
+    const int8_t* wp = a.w + row * a.ldw + 16 * g;
+    auto load = [&](int s) {  // K is a multiple of 16: a lane's 16 bytes are in the row or past it
+        intx4 v = {0, 0, 0, 0};
+        if (s < s1 && 64 * s + 16 * g < a.K) v = *reinterpret_cast<const intx4*>(wp + 64 * s);
+        return v;
+    };
+    constexpr int AHEAD = 8;
+    intx4 w[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) w[i] = load(s0 + i);
+    int8_t* codes = reinterpret_cast<int8_t*>(smem);  // [16][pitch]
+    for (int m = wave; m < a.M; m += 4) {
+        uint32_t mx = 0;
+        for (int k = 8 * lane; k < a.K; k += 512) {
+            float v[8];
+            load8<XDT>(a.x, (int64_t)m * a.K + k, v);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) mx = max(mx, __float_as_uint(v[t]) & 0x7fffffffu);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
+        const Int8Row q(mx);
+        if (lane == 0) sx[m] = q.scale;
+        for (int k = 8 * lane; k < 64 * steps; k += 512) {
+            uint32_t c[2] = {0, 0};
+            if (k < a.K) {
+                float v[8];
+                load8<XDT>(a.x, (int64_t)m * a.K + k, v);
+#pragma unroll
+                for (int t = 0; t < 8; ++t) c[t >> 2] |= (uint32_t)(q.code(v[t]) & 0xff) << (8 * (t & 3));
+            }
+            *reinterpret_cast<uint2*>(codes + m * pitch + k) = make_uint2(c[0], c[1]);
+        }
+    }
+    __syncthreads();
+    intx4 acc = {0, 0, 0, 0};
+    const bool used = r < a.M;
+    for (int s = s0; s < s1; s += AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (s + i >= s1) break;
+            intx4 x = {0, 0, 0, 0};
+            if (used) x = *reinterpret_cast<const intx4*>(codes + r * pitch + 64 * (s + i) + 16 * g);
+            const intx4 v = w[i];
+            w[i] = load(s + i + AHEAD);
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, x, acc, 0, 0, 0);
+        }
+    }
+    // acc[t]: channel 4 g + t, row r
+#pragma unroll
+    for (int t = 0; t < 4; ++t) part[wave][4 * g + t][r] = acc[t];
+    __syncthreads();
+    const int c = threadIdx.x & 15, m = threadIdx.x >> 4;
+    const int64_t n = n0 + c;
+    if (m < a.M && n < a.N) {
+        const int sum = part[0][c][m] + part[1][c][m] + part[2][c][m] + part[3][c][m];
+        const float v = (float)sum * sx[m] * a.sw[n];
+        store1<YDT>(a.y, (int64_t)m * a.N + n, a.bias ? v + a.bias[n] : v);
+    }
+}
+
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
+bool int8_few(const void* x, int xdt, int64_t M, int64_t K, const int8_t* w, int64_t ldw) {
+    return xdt >= 0 && M <= 16 && (M + 15) / 16 * 16 * int8_few_pitch(K) <= 140 * 1024 && M * K <= kInt8FewCodes &&
+           !int8_pads(w, ldw, K) && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+}
+
+template <int XDT, int YDT>
+static hipError_t few_go(const Int8Few& a, hipStream_t s) {
+    static std::atomic<uint64_t> attr_done{0};
+    const hipError_t e = set_lds_attr_once(reinterpret_cast<const void*>(&int8_few_kernel<XDT, YDT>), 140 * 1024, attr_done);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((int8_few_kernel<XDT, YDT>), dim3((unsigned)((a.N + 15) / 16)), dim3(256), a.M * int8_few_pitch(a.K), s, a);
+    return hipGetLastError();
+}
+template <int XDT>
+static hipError_t few_y(const Int8Few& a, int ydt, hipStream_t s) {
+    switch (ydt) {
+        case RPFQ_F32: return few_go<XDT, RPFQ_F32>(a, s);
+        case RPFQ_F16: return few_go<XDT, RPFQ_F16>(a, s);
+        default: return few_go<XDT, RPFQ_BF16>(a, s);
+    }
+}
+
 template <int DT>
 static hipError_t quantize_dt(const void* x, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale, hipStream_t s) {
     const bool vec = K % 8 == 0 && ldq % 8 == 0 && ldq <= 4096 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
@@ -291,6 +403,14 @@ static hipError_t pad_codes(const int8_t* src, int64_t ld, int64_t K, int64_t ro
 hipError_t launch_linear_int8(const void* x, int xdt, const float* sx, const int8_t* w, int64_t ldw, const float* sw,
                               const float* bias, int64_t M, int64_t N, int64_t K, void* y, int ydt, void* work,
                               hipStream_t s) {
+    if (int8_few(x, xdt, M, K, w, ldw)) {
+        const Int8Few f = {x, w, sw, bias, y, ldw, N, (int)M, (int)K};
+        switch (xdt) {
+            case RPFQ_F32: return few_y<RPFQ_F32>(f, ydt, s);
+            case RPFQ_F16: return few_y<RPFQ_F16>(f, ydt, s);
+            default: return few_y<RPFQ_BF16>(f, ydt, s);
+        }
+    }
     const bool quantize = xdt >= 0, pad_w = int8_pads(w, ldw, K);
     // codes that come unaligned are copied as an unaligned weight is
     const bool pad_x = !quantize && int8_pads(x, K, K);

@@ -382,6 +382,8 @@ struct Int8Plan {
 inline bool int8_pads(const void* codes, int64_t ld, int64_t K) {
     return K % 16 != 0 || ld % 16 != 0 || reinterpret_cast<uintptr_t>(codes) % 16 != 0;
 }
+// whether few rows go in one launch without a workspace
+bool int8_few(const void* x, int xdt, int64_t M, int64_t K, const int8_t* w, int64_t ldw);
 Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, bool quantize, bool pad_w);
 hipError_t launch_quantize_int8(const void* x, int dt, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale,
                                 hipStream_t s);

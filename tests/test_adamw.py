@@ -132,6 +132,39 @@ def test_step_matches_its_definition(dtype, bits, count):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("b1,b2", [(0.9, 0.999), (0.5, 0.5), (0.0, 0.99), (0.95, 0.9)])
+def test_codes_over_many_magnitudes(b1, b2):
+    """400,000 elements: blocks of zeros, without a gradient, of gradients that
+    nearly cancel the moment, of tiny and huge scales, single large values."""
+    from quant_models import ops
+
+    g = _gen(21)
+    blocks, n = 1600, 1600 * 256 - 37
+    c = torch.randint(-127, 128, (n,), device=DEV, generator=g, dtype=torch.int8)
+    u = torch.randint(0, 256, (n,), device=DEV, generator=g, dtype=torch.uint8)
+    s = torch.exp2(torch.randint(-60, 8, (blocks,), device=DEV, generator=g).float())
+    r = torch.exp2(torch.randint(-100, 12, (blocks,), device=DEV, generator=g).float())
+    of = torch.arange(n, device=DEV) // 256
+    kind = of % 8
+    grad = torch.randn(n, device=DEV, generator=g) * s[of] * 10.0 ** torch.randint(-3, 3, (n,), device=DEV, generator=g)
+    c[kind == 0], u[kind == 0], grad[kind == 0] = 0, 0, 0
+    grad[kind == 1] = 0
+    m = _values(c, s)
+    near = (-m * (b1 / (1 - b1)) * (1 + 1e-4 * torch.randn(n, device=DEV, generator=g))).float()
+    grad[kind == 2] = near[kind == 2]
+    c[kind == 3], u[kind == 3] = 0, 0
+    c[(kind == 4) & (torch.arange(n, device=DEV) % 256 != 9)] = 0
+    grad[kind == 5] = grad[kind == 5] * 1e-25
+    s[5::16], r[5::16], u[kind == 6] = 2.0 ** -126, 2.0 ** -126, 1
+    p = torch.zeros(n, device=DEV)
+    cm, sm, cv, sv = _encode(b1 * _values(c, s) + (1 - b1) * grad.double(),
+                             b2 * _values(u, r) + (1 - b2) * grad.double() * grad.double())
+    ops.adamw([p], [grad], [c], [u], torch.ones(1, device=DEV), betas=(b1, b2), exp_avg_scales=[s], exp_avg_sq_scales=[r])
+    assert torch.equal(s, sm) and torch.equal(r, sv)
+    assert torch.equal(c, cm) and torch.equal(u, cv)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_first_steps_from_zero_states(bits):
     """New states are zeros; 20 steps of a noisy gradient stay near 64-bit AdamW

@@ -86,7 +86,7 @@ def test_codes_of_extreme_rows():
 
 SHAPES = [(1, 1, 1), (1, 768, 1000), (2, 16, 3), (8, 1024, 333), (16, 515, 64), (17, 768, 257), (31, 64, 31), (32, 80, 256),
           (33, 48, 255), (64, 130, 500), (65, 1024, 4), (129, 768, 1000), (300, 4096, 72), (777, 515, 333), (1576, 768, 2304),
-          (3, 20000, 40), (40, 9000, 17)]
+          (3, 20000, 40), (40, 9000, 17), (16, 2048, 100), (2, 16384, 33), (1, 32768, 20), (5, 48, 17), (16, 2064, 40)]
 
 
 @pytest.mark.gpu
