@@ -574,10 +574,12 @@ def grad_x_bench(m: int, steps: int) -> int:
 
 
 def train_bench(cfg_name: str, batch: int, steps: int, warmup: int, act_quant: bool, modes=("hip", "torch"),
-                amp: bool = False):
+                amp: bool = False, optimizer: str = "sgd", loss_kind: str = "torch"):
     """Quantization-aware training steps of the configured model (float32,
     or with amp the forward under fp16 autocast and a gradient scaler as the
-    reference trainer's --amp runs it; rotation at the family default, SGD):
+    reference trainer's --amp runs it; rotation at the family default, SGD or
+    AdamW with states in 32 or 8 bits; the head's logits and torch's cross
+    entropy, or the two in one without the logits):
     forward with every Linear
     quantized from its float32 master weight, backward with straight-through
     gradients, optimizer step.  'hip' runs the weight quantizer and the act
@@ -600,22 +602,30 @@ def train_bench(cfg_name: str, batch: int, steps: int, warmup: int, act_quant: b
         torch.manual_seed(seed)
         model = qm.create_model(name, img_size=img, quant_method_u="complex_phase_v2",
                                 quant_method_w="complex_phase_v2", enable_act_quant=act_quant).cuda().train()
-        opt = torch.optim.SGD(model.parameters(), lr=1e-4, momentum=0.9)
+        if optimizer == "sgd":
+            opt = torch.optim.SGD(model.parameters(), lr=1e-4, momentum=0.9)
+        else:
+            opt = qm.AdamW(model.parameters(), lr=1e-4, state_bits=8 if optimizer == "adamw8" else 32)
         g = torch.Generator(device="cuda").manual_seed(seed)
         x = torch.randn(batch, 3, img, img, device="cuda", generator=g)
         labels = torch.randint(0, 1000, (batch,), device="cuda", generator=g)
 
         scaler = torch.amp.GradScaler("cuda") if amp else None
 
+        def model_loss():
+            if loss_kind == "fused":
+                return qm.classifier_loss(model, x, labels)
+            return F.cross_entropy(model(x), labels)
+
         def step():
             opt.zero_grad(set_to_none=True)
             if scaler is None:
-                loss = F.cross_entropy(model(x), labels)
+                loss = model_loss()
                 loss.backward()
                 opt.step()
                 return loss
             with torch.autocast("cuda", dtype=torch.float16):
-                loss = F.cross_entropy(model(x), labels)
+                loss = model_loss()
             scaler.scale(loss).backward()
             scaler.step(opt)
             scaler.update()
@@ -658,11 +668,11 @@ def train_bench(cfg_name: str, batch: int, steps: int, warmup: int, act_quant: b
     quant_i.QAT_PACKED_GRAD = os.environ.get("RPFQ_QAT_PACKED_GRAD", "0")
     first = out[modes[0]]
     prec = "fp16 autocast" if amp else "float32"
-    print(json.dumps({"metric": f"QAT training images/s {desc}, {prec}, SGD", "value": first["images_per_s"],
+    print(json.dumps({"metric": f"QAT training images/s {desc}, {prec}, {optimizer.replace('sgd', 'SGD')}", "value": first["images_per_s"],
                       "unit": "images/s", "n_gpus": 1, "steps": steps, "warmup": warmup,
                       "ms_per_step": first["ms_per_step"], "higher_is_better": True, "data": "synthetic",
                       "config": {"workload": cfg_name, "batch": batch, "act_quant": act_quant, "mode": modes[0],
-                                 "amp": amp},
+                                 "amp": amp, "optimizer": optimizer, "loss": loss_kind},
                       "modes": out}))
     return 0
 
@@ -790,6 +800,9 @@ def main() -> int:
     ap.add_argument("--train", action="store_true",
                     help="time quantization-aware training steps (HIP quantizer vs torch ops) instead")
     ap.add_argument("--train-modes", default="hip,hip_pgrad,torch")
+    ap.add_argument("--optimizer", default="sgd", choices=("sgd", "adamw", "adamw8"), help="with --train")
+    ap.add_argument("--loss", default="torch", choices=("torch", "fused"),
+                    help="with --train: logits and torch's cross entropy, or the loss without the logits")
     ap.add_argument("--amp", action="store_true", help="with --train: fp16 autocast forward and a gradient scaler")
     ap.add_argument("--no-bf16-line", action="store_true",
                     help="skip the bf16-activation sub-block of the default (fp16) bench line")
@@ -803,7 +816,7 @@ def main() -> int:
         return vs_library_bench(args.batch * 197 if args.batch else 50432, args.steps)
     if args.train:
         return train_bench(args.config, args.batch or 64, args.steps, args.warmup, args.act_quant,
-                           tuple(args.train_modes.split(",")), amp=args.amp)
+                           tuple(args.train_modes.split(",")), amp=args.amp, optimizer=args.optimizer, loss_kind=args.loss)
     if args.stream_sweep:
         shapes = None if not args.stream_shapes else set(args.stream_shapes.split(","))
         if shapes and not shapes <= set(STREAM_SHAPES):

@@ -659,8 +659,9 @@ size_t rpfq_linear_int8_workspace_bytes(const void* x, int x_dtype, int64_t M, i
  * in int32, the rest float32 rounded once to y_dtype.  x [M, K]: values of
  * x_dtype that the call quantizes as rpfq_quantize_int8 (x_scale NULL), or codes
  * (x_dtype = RPFQ_I8) with their scales x_scale [M].  w: N rows of ld_w bytes
- * (>= K), read in place where w, ld_w and K are multiples of 16, else from a
- * copy; w_scale [N], bias [N] or NULL float32.  K <= 131072.  work 256-byte
+ * (>= K), read in place where w and ld_w are multiples of 16 and ld_w holds K
+ * rounded up to 16 (whose bytes past K may be anything, in the last row too),
+ * else from a copy; w_scale [N], bias [N] or NULL float32.  K <= 131072.  work 256-byte
  * aligned.  No counterpart in the reference: the 8-bit baseline of its layers.
  */
 #define RPFQ_I8 3

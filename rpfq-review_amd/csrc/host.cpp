@@ -288,6 +288,11 @@ PyObject* linear_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Py_RETURN_NONE;
     const int64_t out = w->size(0), k = w->size(1), m = x->numel() / k;
     const int64_t ld = out > 1 ? w->stride(0) : std::max(k, w->stride(0));
+    // rows are read in whole 16 bytes: the last one's too have to be there (rows
+    // of exactly K that do not fill them are copied by the library)
+    if (ld >= (k + 15) / 16 * 16 &&
+        (size_t)(w->storage_offset() + (out - 1) * ld + (k + 15) / 16 * 16) > w->storage().nbytes())
+        Py_RETURN_NONE;
     const at::ScalarType yt = dtype_or(a[4], x->scalar_type());
     const int xdt = dtype_code(x->scalar_type()), ydt = dtype_code(yt);
     const at::Tensor* b = a[3] == Py_None ? nullptr : plain(a[3]);

@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(256) int8_few_kernel(Int8Few a) {
     const int s0 = steps * wave / 4, s1 = steps * (wave + 1) / 4;
     const int64_t row = n0 + r < a.N ? n0 + r : a.N - 1;
     const int8_t* wp = a.w + row * a.ldw + 16 * g;
-    auto load = [&](int s) {  // K is a multiple of 16: a lane's 16 bytes are in the row or past it
+    auto load = [&](int s) {  // a lane's 16 bytes begin in the row (which holds K in whole 16 bytes) or past it
         intx4 v = {0, 0, 0, 0};
         if (s < s1 && 64 * s + 16 * g < a.K) v = *reinterpret_cast<const intx4*>(wp + 64 * s);
         return v;
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(256) int8_few_kernel(Int8Few a) {
 // launches
 // ---------------------------------------------------------------------------
 bool int8_few(const void* x, int xdt, int64_t M, int64_t K, const int8_t* w, int64_t ldw) {
-    return xdt >= 0 && M <= 16 && (M + 15) / 16 * 16 * int8_few_pitch(K) <= 140 * 1024 && M * K <= kInt8FewCodes &&
+    return xdt >= 0 && M <= 16 && K % 8 == 0 && (M + 15) / 16 * 16 * int8_few_pitch(K) <= 140 * 1024 && M * K <= kInt8FewCodes &&
            !int8_pads(w, ldw, K) && reinterpret_cast<uintptr_t>(x) % 16 == 0;
 }
 

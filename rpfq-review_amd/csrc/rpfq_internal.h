@@ -373,14 +373,15 @@ hipError_t launch_linear_f32_grad(const float* gy, const float* x, const float* 
                                   const float* parts, int nparts, const float* xscale, float* gx, float* gw, float* gb,
                                   void* work, hipStream_t s);
 // 8-bit integer layer (int8_linear.hip): offsets in its workspace.  Codes are
-// read in place where rows of ld bytes are 16-byte aligned and hold whole
-// 16-byte pieces, else from a padded copy.
+// read in place where rows of ld bytes are 16-byte aligned and hold K in whole
+// 16-byte pieces (a weight's past K meet codes of x that are 0), else from a
+// padded copy.
 struct Int8Plan {
     int64_t ld;  // row bytes of codes in the workspace
     size_t x_at, sx_at, w_at, bytes;
 };
 inline bool int8_pads(const void* codes, int64_t ld, int64_t K) {
-    return K % 16 != 0 || ld % 16 != 0 || reinterpret_cast<uintptr_t>(codes) % 16 != 0;
+    return ld < ((K + 15) & ~(int64_t)15) || ld % 16 != 0 || reinterpret_cast<uintptr_t>(codes) % 16 != 0;
 }
 // whether few rows go in one launch without a workspace
 bool int8_few(const void* x, int xdt, int64_t M, int64_t K, const int8_t* w, int64_t ldw);

@@ -16,7 +16,9 @@ from .quant_i import (  # noqa: F401
 from .quant_rpfq_deit import *  # noqa: F401,F403
 from .quant_rpfq_swin import *  # noqa: F401,F403
 from .quant_rpfq_vit import *  # noqa: F401,F403
+from .int8 import Int8Linear  # noqa: F401
 from .registry import create_model, is_model, list_models, register_model  # noqa: F401
+from .training import AdamW, classifier_loss  # noqa: F401
 from . import torch_ops  # noqa: F401,E402  (registers torch.ops.rpfq.*)
 
 __all__ = [
@@ -24,6 +26,9 @@ __all__ = [
     "ComplexWeightQuantizer",
     "ComplexActivationQuantizer",
     "SUPPORTED_QUANT_METHODS",
+    "Int8Linear",
+    "AdamW",
+    "classifier_loss",
     "create_model",
     "is_model",
     "list_models",

@@ -8,6 +8,7 @@ import torch.nn as nn
 
 from . import _native as N
 from . import packing as P
+from .int8 import Int8Linear
 from .quant_i import QATLinearComplexPhase
 
 
@@ -33,12 +34,13 @@ def load_synthetic_codes(model: nn.Module, seed: int, codebook: int = N.CB_AXIS,
 def prepare_inference(model: nn.Module, device="cuda", dtype: torch.dtype = torch.float16) -> nn.Module:
     """eval(), move to `device`, pack every quantized layer once, and cast the
     remaining (non-quantized) parameters and buffers to `dtype`.  Quantized
-    layers keep their float32 master weight and bias."""
+    layers keep their float32 master weight and bias, 8-bit ones (to_int8)
+    their codes, scales and bias."""
     model.eval().to(device)
     for _, layer in quant_layers(model):
         layer.packed(torch.device(device))
     for m in model.modules():
-        if isinstance(m, QATLinearComplexPhase):
+        if isinstance(m, (QATLinearComplexPhase, Int8Linear)):
             continue
         for name, p in list(m.named_parameters(recurse=False)):
             p.data = p.data.to(dtype)
@@ -46,6 +48,22 @@ def prepare_inference(model: nn.Module, device="cuda", dtype: torch.dtype = torc
             if b is not None and b.is_floating_point():
                 setattr(m, name, b.to(dtype))
     return model
+
+
+def to_int8(model: nn.Module, skip=()) -> int:
+    """Replace every linear layer of `model` (nn.Linear and phase-quantized
+    ones, from their float weights) by its 8-bit baseline Int8Linear, but those
+    named in `skip` (names of named_modules(); a name covers what is below
+    it).  For inference; returns the number of layers."""
+    edges = []
+    for name, parent in model.named_modules():
+        for child_name, child in parent.named_children():
+            full = f"{name}.{child_name}" if name else child_name
+            if isinstance(child, nn.Linear) and not any(full == s or full.startswith(s + ".") for s in skip):
+                edges.append((parent, child_name, child))
+    for parent, name, child in edges:
+        setattr(parent, name, Int8Linear.from_linear(child))
+    return len(edges)
 
 
 def packed_code_bytes(model: nn.Module) -> int:

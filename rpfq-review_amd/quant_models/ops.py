@@ -873,9 +873,9 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     sums exact in integers, the rest float32 rounded once to out_dtype
     (default x.dtype).  x: float32, fp16 or bf16, quantized per token within
     the call as quantize_int8 does, or int8 codes with their x_scale [...]
-    (out_dtype then says what y is).  weight int8 [N, K] (rows may be wider
-    apart: multiples of 16 bytes, K too, are read in place), weight_scale
-    float32 [N].  K <= 131072.  No gradient."""
+    (out_dtype then says what y is).  weight int8 [N, K] (read in place where
+    its rows lie a multiple of 16 bytes apart that holds K, as a slice of wider
+    rows does; else from a copy of it), weight_scale float32 [N].  K <= 131072.  No gradient."""
     host = N.host()
     if host is not None and x_scale is None:
         y = host.linear_int8(x, weight, weight_scale, bias, out_dtype)
@@ -907,7 +907,9 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         return y
     x2 = _aligned_rows(x.reshape(-1, k))
     m = x2.shape[0]
-    if weight.stride(1) != 1 and k > 1 or weight.stride(0) < k:
+    # rows are read in whole 16 bytes: the last one's too have to be there
+    end = weight.storage_offset() + (n - 1) * weight.stride(0) + -(-k // 16) * 16
+    if weight.stride(1) != 1 and k > 1 or weight.stride(0) < k or end > weight.untyped_storage().nbytes():
         weight = weight.contiguous()
     weight_scale = weight_scale.contiguous()
     bias = None if bias is None else bias.detach().float().contiguous()

@@ -681,6 +681,25 @@ class QATLinearComplexPhase(nn.Linear):
             x = torch.cat((qr, qi), dim=-1)
         return _linear(x, q_weight, self.bias)
 
+    def training_operands(self, x: torch.Tensor):
+        """(x, weight, bias) whose F.linear is the training forward: the
+        fake-quantized activations and A_q, with their straight-through
+        gradients.  For callers that take the product with something else
+        (training.classifier_loss: the head with the loss)."""
+        spec = self._hip_qat_spec(x)
+        if spec is not None:
+            q_weight = _HipWideQuantSTE.apply(self.weight, self.quantizer_u.rotation_angle,
+                                              self.quantizer_w.rotation_angle, spec, None)
+        else:
+            q_weight = self.quantized_weight()
+        if self.act_quantizer is not None:
+            if spec is not None and x.dtype == torch.float32:
+                x = _HipActQuantSTE.apply(x, self.act_quantizer.num_bits)
+            else:
+                h = self.in_features // 2
+                x = torch.cat(self.act_quantizer(x[..., :h], x[..., h:]), dim=-1)
+        return x, q_weight, self.bias
+
     # -- packed HIP path ------------------------------------------------------
     def load_packed(self, codes: "P.LayerCodes") -> None:
         """Run this layer from externally supplied code planes and scales

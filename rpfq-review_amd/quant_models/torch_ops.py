@@ -24,6 +24,8 @@ contract is registered here, running the HIP kernels of librpfq.so:
   gradient on the same blob (rpfq_wide_linear_grad_x, after relaying its
   codes out with rpfq_wide_pack_adjoint per call) and the bias gradient as
   the column sum (the reference operator's backward, kernel.py:585-588).
+* ``torch.ops.rpfq.linear_int8(x, weight, weight_scale, bias)``: the 8-bit
+  baseline (rpfq_linear_int8), x quantized per token; inference only.
 * ``torch.ops.rpfq.act_quant(x, num_bits)``: ActivationQuantSTE's forward
   (quant_i.py:438-455) on [..., 2K'] features.
 
@@ -155,3 +157,16 @@ def act_quant(x: torch.Tensor, num_bits: int) -> torch.Tensor:
 @act_quant.register_fake
 def _(x, num_bits):
     return torch.empty_like(x)
+
+
+@torch.library.custom_op("rpfq::linear_int8", mutates_args=())
+def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                bias: Optional[torch.Tensor]) -> torch.Tensor:
+    from . import ops
+
+    return ops.linear_int8(x, weight, weight_scale, bias)
+
+
+@linear_int8.register_fake
+def _(x, weight, weight_scale, bias):
+    return x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0],))

@@ -1,0 +1,211 @@
+"""Training steps of the quantized classifiers: AdamW over all tensors in a
+few launches, with states in 32 or in 8 bits, and the loss of a model's head
+without its logits.
+"""
+from __future__ import annotations
+
+from collections import defaultdict
+
+import torch
+import torch.nn as nn
+
+from .quant_i import QATLinearComplexPhase
+from .swin_transformer import SwinTransformer
+from .vision_transformer import VisionTransformer, VisionTransformerDistilled
+
+
+# ---------------------------------------------------------------------------
+# loss
+# ---------------------------------------------------------------------------
+def head_operands(layer: nn.Module, x: torch.Tensor):
+    """(x, weight, bias) whose linear map is layer(x) in training: a
+    phase-quantized layer's activations and weight as its training forward
+    quantizes them (straight-through gradients), nn.Linear's as they are."""
+    if isinstance(layer, QATLinearComplexPhase):
+        return layer.training_operands(x)
+    if type(layer) is not nn.Linear:
+        raise TypeError(f"classifier_loss takes a linear head, got {type(layer).__name__}")
+    return x, layer.weight, layer.bias
+
+
+def classifier_loss(model: nn.Module, images: torch.Tensor, labels: torch.Tensor, *, ignore_index: int = -100,
+                    label_smoothing: float = 0.0, reduction: str = "mean") -> torch.Tensor:
+    """F.cross_entropy(model(images), labels, ...) of a ViT, DeiT or Swin
+    model (this package's, phase-quantized or not) without its logits: the
+    model's features, then ops.linear_cross_entropy with the head's weight.
+    A distilled DeiT's two heads are averaged, as its eval output is; in
+    distilled training the model returns two outputs, which this does not
+    take."""
+    from . import ops
+
+    if isinstance(model, VisionTransformerDistilled):
+        if model.distilled_training and model.training:
+            raise ValueError("classifier_loss: distilled training has a loss for each head")
+        f = model.forward_features(images)
+        # (head(a) + head_dist(b)) / 2 as one layer of both weights on [a, b] / 2
+        parts = [head_operands(h, v) for h, v in ((model.head, f[:, 0]), (model.head_dist, f[:, 1]))]
+        x = torch.cat([p[0] for p in parts], -1) * 0.5
+        weight = torch.cat([p[1].to(p[0].dtype) if not torch.is_autocast_enabled("cuda") else p[1] for p in parts], -1)
+        biases = [p[2] for p in parts if p[2] is not None]
+        bias = sum(biases) * 0.5 if biases else None
+    elif isinstance(model, VisionTransformer):
+        x, weight, bias = head_operands(model.head, model.forward_head(model.forward_features(images), pre_logits=True))
+    elif isinstance(model, SwinTransformer):
+        x, weight, bias = head_operands(model.head.fc, model.forward_features(images).mean(dim=(1, 2)))
+    else:
+        raise TypeError(f"classifier_loss takes a VisionTransformer or SwinTransformer, got {type(model).__name__}")
+    if x.dtype != weight.dtype and not torch.is_autocast_enabled("cuda"):
+        weight = weight.to(x.dtype)
+    return ops.linear_cross_entropy(x, weight, labels, bias, ignore_index=ignore_index, label_smoothing=label_smoothing,
+                                    reduction=reduction)
+
+
+# ---------------------------------------------------------------------------
+# optimizer
+# ---------------------------------------------------------------------------
+def _flat(t: torch.Tensor, what: str) -> torch.Tensor:
+    """t's memory as it lies, for tensors without gaps (any order of dimensions)."""
+    if t.is_contiguous():
+        return t
+    expect = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda p: p[1]):
+        if stride != expect:
+            raise ValueError(f"AdamW: {what} of shape {tuple(t.shape)} and strides {t.stride()} has gaps or overlaps")
+        expect *= size
+    return t.as_strided((t.numel(),), (1,))
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's step (decoupled weight decay) on the device kernel
+    (ops.adamw): one launch per 60 tensors of a type.  state_bits 32: float32
+    moments; 8: codes of 8 bits with one scale per 256 elements, 2.03 bytes an
+    element instead of 8.  Parameters on the device, float32, fp16 or bf16
+    (moments and update in float32).  lr may be a float32 device tensor of one
+    element.  The steps are counted on the device, so step() can be captured
+    into a graph once the states exist; torch.amp.GradScaler's scale and its
+    skipped steps are taken on the device too.  state_dict() and
+    load_state_dict() keep the states' types."""
+
+    _step_supports_amp_scaling = True
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 state_bits: int = 32):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"eps and weight_decay must not be negative, got {eps} and {weight_decay}")
+        if not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"betas must be within 0 .. 1, got {betas}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def _new_state(self, p: torch.Tensor, bits: int, steps: dict) -> dict:
+        # parameters that start together share one count (and so a launch)
+        state = {"step": steps.setdefault((p.device, "new"), torch.zeros(1, dtype=torch.float32, device=p.device))}
+        if bits == 32:
+            state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+            state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        else:
+            from . import ops
+
+            blocks = -(-p.numel() // ops.STATE_BLOCK)
+            state["exp_avg"] = torch.zeros_like(p, dtype=torch.int8)
+            state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.uint8)
+            for name in ("exp_avg_scale", "exp_avg_sq_scale"):
+                state[name] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        from . import ops
+
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        grad_scale, found_inf = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        # all parameters that share a count, and those of them that step now
+        sharing, stepping, fresh = defaultdict(int), defaultdict(list), {}
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is not None:
+                    if p.grad.is_sparse:
+                        raise RuntimeError("AdamW does not take sparse gradients")
+                    if not p.is_cuda:
+                        raise ValueError("AdamW takes device parameters only")
+                    if not self.state[p]:
+                        self.state[p] = self._new_state(p, group["state_bits"], fresh)
+                    stepping[id(self.state[p]["step"])].append(p)
+                if p in self.state and self.state[p]:
+                    sharing[id(self.state[p]["step"])] += 1
+        for key, params in stepping.items():
+            if len(params) < sharing[key]:  # the others do not step: a count of their own for these
+                count = self.state[params[0]]["step"].clone()
+                for p in params:
+                    self.state[p]["step"] = count
+        for group in self.param_groups:
+            calls = defaultdict(list)
+            for p in group["params"]:
+                if p.grad is not None:
+                    calls[(id(self.state[p]["step"]), p.dtype)].append(p)
+            for params in calls.values():
+                step = self.state[params[0]]["step"]
+                # a count belongs to one call: another group's or type's takes a copy
+                if any(self.state[q]["step"] is step for g in self.param_groups for q in g["params"]
+                       if q in self.state and self.state[q] and (g is not group or q.dtype != params[0].dtype)):
+                    step = step.clone()
+                    for p in params:
+                        self.state[p]["step"] = step
+                self._launch(ops, params, step, group, grad_scale, found_inf)
+        return loss
+
+    def _launch(self, ops, params, step, group, grad_scale, found_inf):
+        lists = defaultdict(list)
+        for p in params:
+            state, g = self.state[p], p.grad
+            if g.stride() != p.stride():
+                g = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
+            lists["params"].append(_flat(p, "a parameter"))
+            lists["grads"].append(_flat(g, "a gradient"))
+            lists["exp_avgs"].append(_flat(state["exp_avg"], "a state"))
+            lists["exp_avg_sqs"].append(_flat(state["exp_avg_sq"], "a state"))
+            if group["state_bits"] == 8:
+                lists["exp_avg_scales"].append(state["exp_avg_scale"])
+                lists["exp_avg_sq_scales"].append(state["exp_avg_sq_scale"])
+        device = params[0].device
+        there = [None if t is None else t.to(device=device, dtype=torch.float32) for t in (grad_scale, found_inf)]
+        ops.adamw(step=step, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                  grad_scale=there[0], found_inf=there[1], **lists)
+
+    def state_values(self, p: torch.Tensor):
+        """(first, second) moment of a parameter as float32 tensors."""
+        from . import ops
+
+        state = self.state[p]
+        if "exp_avg_scale" not in state:
+            return state["exp_avg"], state["exp_avg_sq"]
+        flat = [_flat(state[k], "a state").reshape(-1) for k in ("exp_avg", "exp_avg_sq")]
+        values = ops.adamw_state_values(flat, [state["exp_avg_scale"], state["exp_avg_sq_scale"]])
+        return tuple(v.as_strided(p.shape, p.stride()) for v in values)
+
+    def load_state_dict(self, state_dict) -> None:
+        """As torch's, but the states keep their types (codes stay codes,
+        moments float32), and parameters of one count share it again."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        counts = {}
+        for i, p in zip(saved, params):
+            source = state_dict["state"].get(i)
+            if not source:
+                continue
+            for name, value in source.items():
+                if name == "step":
+                    at = float(value)
+                    value = counts.setdefault((p.device, at), torch.full((1,), at, dtype=torch.float32, device=p.device))
+                elif isinstance(value, torch.Tensor):
+                    moved = value.to(p.device)
+                    value = torch.empty_strided(p.shape, p.stride(), dtype=value.dtype, device=p.device).copy_(moved) \
+                        if value.shape == p.shape and name in ("exp_avg", "exp_avg_sq") else moved.clone()
+                self.state[p][name] = value
