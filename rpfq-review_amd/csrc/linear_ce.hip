@@ -563,7 +563,7 @@ struct CeGrad {
     int64_t rk, ck;
     int64_t M, N;     // rows, columns of the gradient
     int planes, splits;
-    int tiles_m, tiles_n, group;
+    int tiles_m, tiles_n;
     float* part;      // [splits][M][ldp], or NULL: the gradient itself, rounded
     int64_t ldp;
     int add;          // part holds the pieces before
@@ -574,14 +574,13 @@ struct CeGrad {
 
 // One product of the gradient: dx (dz in K layout, w in T) or dw (dz and x in T).
 template <int MB, int WM, int S, int KB, bool RT, class Mma, int DT>
-__global__ void __launch_bounds__(256 * WM, 2) ce_grad_kernel(CeGrad a) {
-    extern __shared__ __align__(16) char smem[];
+__device__ __forceinline__ void ce_grad_unit(const CeGrad& a, int bid, char* smem) {
     using G = TileGemm<MB, WM, S, KB, RT, true, Mma>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles = a.tiles_m * a.tiles_n;
-    const int unit = xcd_tile(blockIdx.x, tiles * a.splits), sp = unit / tiles;
+    const int unit = xcd_tile(bid, tiles * a.splits), sp = unit / tiles;
     int mt, nt;
-    group_tile(unit - sp * tiles, a.tiles_m, a.tiles_n, a.group, mt, nt);
+    group_tile(unit - sp * tiles, a.tiles_m, a.tiles_n, a.tiles_n, mt, nt);
     const int64_t m0 = (int64_t)mt * G::ROWS, mw = m0 + 32 * MB * (wave >> 2), n0 = (int64_t)nt * 256;
     const int per = (int)G::steps(a.rk), steps = a.planes ? kPairs32 * per : per;
     const int s0 = (int)((int64_t)steps * sp / a.splits), s1 = (int)((int64_t)steps * (sp + 1) / a.splits);
@@ -606,6 +605,23 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_grad_kernel(CeGrad a) {
                           tile_store4<DT>(a.out, m * a.N, n, a.N, a.vec, v * f);
                       }
                   });
+}
+
+// Both products of a piece's dz in one launch: dx (dz in K layout, w in T) and dw
+// (dz and x in T), the longer units first and the others into their last round
+// (2,048 x 20,000 x 1,024 fp16: 1.2 and 1.0 rounds of the chip apart, 227 us).
+struct CeGrads {
+    CeGrad g[2];   // dx, dw; splits = 0: not wanted
+    int units[2];
+    int first;     // whose units come first
+};
+template <int MB, int WM, int S, int KB, class Mma, int DT>
+__global__ void __launch_bounds__(256 * WM, 2) ce_grads_kernel(CeGrads a) {
+    extern __shared__ __align__(16) char smem[];
+    const int bid = blockIdx.x, lead = a.units[a.first];
+    const int k = bid < lead ? a.first : 1 - a.first, at = bid < lead ? bid : bid - lead;
+    if (k == 0) ce_grad_unit<MB, WM, S, KB, false, Mma, DT>(a.g[0], at, smem);
+    else ce_grad_unit<MB, WM, S, KB, true, Mma, DT>(a.g[1], at, smem);
 }
 
 // out = factor * sum of the partials, in their order.
@@ -634,27 +650,40 @@ __global__ void __launch_bounds__(256) ce_sum_kernel(const float* part, int part
 // ---------------------------------------------------------------------------
 // plan and launches
 // ---------------------------------------------------------------------------
-// The form and the split of k (`steps` of 64 bytes) with the least time for a
-// gradient of rows x cols: rounds of the chip in units of a 256-row tile's step
-// (0.9 us), a few for a tile's start and end, and the partials' way through
-// memory (about 5 TB/s, and a launch).
-static CeSplit ce_split(int64_t rows, int64_t cols, int64_t steps) {
-    const int64_t cus = device_cus(), tn = (cols + 255) / 256;
-    CeSplit best = {kTile128, 1};
+// The form of the two gradients' launch, dx of M x D over V classes and dw of V
+// x D over M rows, and the splits of their k (in steps of 64 bytes) that take
+// the least time: the longest unit or the chip's share of all and half a unit,
+// in steps of a 256-row tile (0.9 us), and the partials' way through memory
+// (about 5 TB/s, and a launch).
+static CeSplit ce_split(int64_t M, int64_t V, int64_t D, int64_t pairs) {
+    const int64_t cus = device_cus(), tn = (D + 255) / 256, kx = pairs * ((V + 31) / 32), kw = pairs * ((M + 31) / 32);
+    static constexpr int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64};
+    CeSplit best = {kTile128, 1, 1};
     double cost = 1e300;
-    for (int s = 1; s <= 64 && (s == 1 || 4 * s <= steps); ++s) {
-        const double n = (double)((steps + s - 1) / s);
-        const double join = s > 1 ? 7.0 + (double)s * rows * cols * 8.0 / 4.5e6 : 0.0;
-        for (const TileForm f : {kTile64, kTile128Deep, kTile128, kTile256}) {
-            const int64_t tall = f == kTile64 ? 64 : f == kTile256 ? 256 : 128;
-            const int64_t units = (rows + tall - 1) / tall * tn * s;
-            double c;
-            if (f == kTile64 || f == kTile128Deep) c = units > cus ? 1e300 : n * (f == kTile64 ? 0.38 : 0.48) + 4.0;
-            else if (f == kTile128) c = (double)((units + 2 * cus - 1) / (2 * cus)) * (1.15 * n + 5.0);
-            else c = (double)((units + cus - 1) / cus) * (n + 5.0);
-            if (c + join < cost) {
-                cost = c + join;
-                best = {f, s};
+    struct {
+        TileForm form;
+        int rows, slots;
+        double step, start;
+    } const forms[] = {{kTile64, 64, 1, 0.38, 4.0}, {kTile128Deep, 128, 1, 0.48, 4.0}, {kTile128, 128, 2, 1.15, 6.0}, {kTile256, 256, 1, 1.0, 5.0}};
+    for (const auto& f : forms) {
+        const int64_t slots = f.slots * cus;
+        for (const int sx : kSplits) {
+            if (sx > 1 && 4 * sx > kx) break;
+            for (const int sw : kSplits) {
+                if (sw > 1 && 4 * sw > kw) break;
+                const double nx = (double)((kx + sx - 1) / sx) * f.step + f.start, nw = (double)((kw + sw - 1) / sw) * f.step + f.start;
+                const double ux = (double)((M + f.rows - 1) / f.rows * tn * sx), uw = (double)((V + f.rows - 1) / f.rows * tn * sw);
+                const double longest = nx > nw ? nx : nw, rounds = (ux * nx + uw * nw) / (double)slots;
+                // the deep forms are for one round: more of them wait on the LDS fill
+                if (ux + uw > (double)slots && (f.form == kTile64 || f.form == kTile128Deep)) continue;
+                double c = ux + uw <= (double)slots ? longest : rounds + 0.5 * (nx < nw ? nx : nw);
+                if (c < longest) c = longest;
+                if (sx > 1) c += 7.0 + (double)sx * M * D * 8.0 / 4.5e6;
+                if (sw > 1) c += 7.0 + (double)sw * V * D * 8.0 / 4.5e6;
+                if (c < cost) {
+                    cost = c;
+                    best = {f.form, sx, sw};
+                }
             }
         }
     }
@@ -704,10 +733,9 @@ CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool back
     // float32 partials, rows of whole 16 bytes
     p.ldp = (D + 3) & ~(int64_t)3;
     const int64_t pairs = planes == 3 ? kPairs32 : 1;
-    p.dx = ce_split(M, D, pairs * ((p.piece + 31) / 32));
-    p.dx_at = take(p.dx.splits > 1 || p.pieces > 1 ? 4 * p.dx.splits * M * p.ldp : 0);
-    p.dw = ce_split(p.piece, D, pairs * ((M + 31) / 32));
-    p.dw_at = take(p.dw.splits > 1 ? 4 * p.dw.splits * p.piece * p.ldp : 0);
+    p.grad = ce_split(M, p.piece, D, pairs);
+    p.dx_at = take(p.grad.dx > 1 || p.pieces > 1 ? 4 * p.grad.dx * M * p.ldp : 0);
+    p.dw_at = take(p.grad.dw > 1 ? 4 * p.grad.dw * p.piece * p.ldp : 0);
     return p;
 }
 
@@ -791,33 +819,40 @@ struct DzGo {
     }
 };
 
-template <bool RT, class Mma, int DT>
+template <class Mma, int DT>
 struct GradGo {
-    CeGrad& a;
+    CeGrads& a;
     hipStream_t s;
     template <int MB, int WM, int S, int KB>
     hipError_t run() {
         if constexpr (MB == 1 && WM == 1) {
             return hipErrorInvalidValue;  // ce_split takes 64 rows at least
         } else {
-            using G = TileGemm<MB, WM, S, KB, RT, true, Mma>;
+            using X = TileGemm<MB, WM, S, KB, false, true, Mma>;
+            using W = TileGemm<MB, WM, S, KB, true, true, Mma>;
+            static_assert(X::LDS == W::LDS, "one launch");
             static std::atomic<uint64_t> done{0};
-            const hipError_t e = ce_lds(&ce_grad_kernel<MB, WM, S, KB, RT, Mma, DT>, G::LDS, done);
+            const hipError_t e = ce_lds(&ce_grads_kernel<MB, WM, S, KB, Mma, DT>, X::LDS, done);
             if (e != hipSuccess) return e;
-            a.tiles_m = (int)((a.M + G::ROWS - 1) / G::ROWS);
-            a.tiles_n = (int)((a.N + 255) / 256);
-            a.group = a.tiles_n;
-            hipLaunchKernelGGL((ce_grad_kernel<MB, WM, S, KB, RT, Mma, DT>), dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)),
-                               dim3(G::THREADS), G::LDS, s, a);
+            double length[2];
+            for (int k = 0; k < 2; ++k) {
+                CeGrad& g = a.g[k];
+                g.tiles_m = (int)((g.M + X::ROWS - 1) / X::ROWS);
+                g.tiles_n = (int)((g.N + 255) / 256);
+                a.units[k] = g.tiles_m * g.tiles_n * g.splits;
+                length[k] = g.splits ? (double)(k ? W::steps(g.rk) : X::steps(g.rk)) / g.splits : 0.0;
+            }
+            a.first = length[1] > length[0];
+            hipLaunchKernelGGL((ce_grads_kernel<MB, WM, S, KB, Mma, DT>), dim3((unsigned)(a.units[0] + a.units[1])),
+                               dim3(X::THREADS), X::LDS, s, a);
             return hipGetLastError();
         }
     }
 };
-template <bool RT>
-static hipError_t ce_grad(int dt, TileForm form, CeGrad& g, hipStream_t s) {
-    return dt == RPFQ_F16    ? tile_dispatch(form, GradGo<RT, MmaF16, RPFQ_F16>{g, s})
-           : dt == RPFQ_BF16 ? tile_dispatch(form, GradGo<RT, MmaBf16, RPFQ_BF16>{g, s})
-                             : tile_dispatch(form, GradGo<RT, MmaBf16, RPFQ_F32>{g, s});
+static hipError_t ce_grads(int dt, TileForm form, CeGrads& g, hipStream_t s) {
+    return dt == RPFQ_F16    ? tile_dispatch(form, GradGo<MmaF16, RPFQ_F16>{g, s})
+           : dt == RPFQ_BF16 ? tile_dispatch(form, GradGo<MmaBf16, RPFQ_BF16>{g, s})
+                             : tile_dispatch(form, GradGo<MmaBf16, RPFQ_F32>{g, s});
 }
 
 static hipError_t ce_sum(int dt, const float* part, int parts, int64_t stride, int64_t rows, int64_t N, int64_t ldp,
@@ -895,7 +930,7 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
     a.dz = wk + p.dz_at;
     a.colsum = gb ? reinterpret_cast<float*>(wk + p.col_at) : nullptr;
     const TileOperand w = a.w;
-    float* dxp = p.dx.splits > 1 || p.pieces > 1 ? reinterpret_cast<float*>(wk + p.dx_at) : nullptr;
+    float* dxp = p.grad.dx > 1 || p.pieces > 1 ? reinterpret_cast<float*>(wk + p.dx_at) : nullptr;
     for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
         const int64_t n = std::min(p.piece, c.V - v0);
         a.v0 = v0;
@@ -912,44 +947,34 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         if (e != hipSuccess) return e;
         a.xz = nullptr;  // written with the first piece
         const TileOperand dzk = {a.dz, a.ldz, a.dz_plane, c.M}, dzt = {a.dz, a.ldz, a.dz_plane, n};
-        if (gx) {
-            CeGrad g = {};
-            g.r = dzk;
-            g.c = {a.w.p, w.ld, w.plane, p.ldk};
-            g.rk = 2 * a.n8;
-            g.ck = n;
-            g.M = c.M;
-            g.N = c.D;
-            g.planes = a.planes;
-            g.splits = p.dx.splits;
-            g.part = dxp;
-            g.ldp = p.ldp;
-            g.add = v0 > 0;
-            g.factor = factor;
-            g.out = gx;
-            g.vec = c.D % 4 == 0 && reinterpret_cast<uintptr_t>(gx) % (4 * es) == 0;
-            e = ce_grad<false>(c.dtype, p.dx.form, g, s);
-            if (e != hipSuccess) return e;
-        }
-        if (gw) {
-            CeGrad g = {};
-            g.r = dzt;
-            g.c = {xz.p, xz.ld, xz.plane, p.ldk};
-            g.rk = g.ck = c.M;
-            g.M = n;
-            g.N = c.D;
-            g.planes = a.planes;
-            g.splits = p.dw.splits;
-            g.part = p.dw.splits > 1 ? reinterpret_cast<float*>(wk + p.dw_at) : nullptr;
-            g.ldp = p.ldp;
-            g.factor = factor;
-            g.out = reinterpret_cast<char*>(gw) + v0 * c.D * es;
-            g.vec = c.D % 4 == 0 && reinterpret_cast<uintptr_t>(g.out) % (4 * es) == 0;
-            e = ce_grad<true>(c.dtype, p.dw.form, g, s);
-            if (e != hipSuccess) return e;
-            if (g.part && (e = ce_sum(c.dtype, g.part, g.splits, n * p.ldp, n, c.D, p.ldp, factor, g.out, s)) != hipSuccess)
-                return e;
-        }
+        CeGrads both = {};
+        CeGrad &dx = both.g[0], &dw = both.g[1];
+        dx.planes = dw.planes = a.planes;
+        dx.N = dw.N = c.D;
+        dx.ldp = dw.ldp = p.ldp;
+        dx.factor = dw.factor = factor;
+        dx.r = dzk;
+        dx.c = {a.w.p, w.ld, w.plane, p.ldk};
+        dx.rk = 2 * a.n8;
+        dx.ck = n;
+        dx.M = c.M;
+        dx.splits = gx ? p.grad.dx : 0;
+        dx.part = dxp;
+        dx.add = v0 > 0;
+        dx.out = gx;
+        dx.vec = c.D % 4 == 0 && reinterpret_cast<uintptr_t>(gx) % (4 * es) == 0;
+        dw.r = dzt;
+        dw.c = {xz.p, xz.ld, xz.plane, p.ldk};
+        dw.rk = dw.ck = c.M;
+        dw.M = n;
+        dw.splits = gw ? p.grad.dw : 0;
+        dw.part = p.grad.dw > 1 ? reinterpret_cast<float*>(wk + p.dw_at) : nullptr;
+        dw.out = gw ? reinterpret_cast<char*>(gw) + v0 * c.D * es : nullptr;
+        dw.vec = c.D % 4 == 0 && reinterpret_cast<uintptr_t>(dw.out) % (4 * es) == 0;
+        if ((gx || gw) && (e = ce_grads(c.dtype, p.grad.form, both, s)) != hipSuccess) return e;
+        if (gw && dw.part &&
+            (e = ce_sum(c.dtype, dw.part, dw.splits, n * p.ldp, n, c.D, p.ldp, factor, dw.out, s)) != hipSuccess)
+            return e;
         if (gb) {  // db: the column sums of the row tiles, as one row each
             const int bs = c.bias_dtype == RPFQ_F32 ? 4 : 2;
             e = ce_sum(c.bias_dtype, a.colsum, col_rows, a.n8, 1, n, a.n8, factor,
@@ -957,7 +982,7 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
             if (e != hipSuccess) return e;
         }
     }
-    if (gx && dxp) return ce_sum(c.dtype, dxp, p.dx.splits, c.M * p.ldp, c.M, c.D, p.ldp, factor, gx, s);
+    if (gx && dxp) return ce_sum(c.dtype, dxp, p.grad.dx, c.M * p.ldp, c.M, c.D, p.ldp, factor, gx, s);
     return hipSuccess;
 }
 

@@ -405,14 +405,14 @@ struct CeCall {
     int reduction;  // 0 none, 1 mean, 2 sum
 };
 struct CeSplit {
-    TileForm form;  // of a gradient's product, and parts of its k
-    int splits;
+    TileForm form;  // of the gradients' products
+    int dx, dw;     // parts of their k
 };
 struct CePlan {
     int64_t ldk, ldp;       // elements of a row of k; of float32 partials
     bool pad;               // x and w are copied (rows of ldk, or three planes of them)
     int64_t tiles_v, piece, pieces;
-    CeSplit dx, dw;
+    CeSplit grad;
     size_t x_at, w_at, part_at, zsum_at, zt_at, rows_at, rho_at, factor_at, dz_at, col_at, dx_at, dw_at, bytes;
 };
 CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool backward);
