@@ -446,6 +446,10 @@ hipError_t launch_linear_int8(const void* x, int xdt, const float* sx, const int
     a.K = p.ld;
     const int es = ydt == RPFQ_F32 ? 4 : 2;
     a.vec = N % (16 / es) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+    // an output larger than the 256-MB cache behind the L2 goes past both, which
+    // leaves them to the operands (50,432 x 4,096: 289 -> 277 us); a smaller one
+    // is what the next layer reads
+    if (a.vec && M * N * es > 256LL << 20) a.vec = 2;
     switch (ydt) {
         case RPFQ_F32: return gemm_y<RPFQ_F32>(a, s);
         case RPFQ_F16: return gemm_y<RPFQ_F16>(a, s);

@@ -346,11 +346,13 @@ __device__ __forceinline__ void tile_store4(void* y, int64_t row_off, int64_t n,
 }
 
 // 8 16-bit values to columns n .. n + 7 of a row of N (those below N): one store
-// where `vec` says that rows are 16-byte aligned.
-__device__ __forceinline__ void tile_store8(void* y, int64_t row_off, int64_t n, int64_t N, bool vec, uint4 v) {
+// where `vec` says that rows are 16-byte aligned, past the caches where it is 2.
+__device__ __forceinline__ void tile_store8(void* y, int64_t row_off, int64_t n, int64_t N, int vec, uint4 v) {
     uint16_t* d = reinterpret_cast<uint16_t*>(y) + row_off + n;
     if (vec) {
-        if (n < N) *reinterpret_cast<uint4*>(d) = v;
+        if (n >= N) return;
+        if (vec == 2) __builtin_nontemporal_store(__builtin_bit_cast(intx4, v), reinterpret_cast<intx4*>(d));
+        else *reinterpret_cast<uint4*>(d) = v;
         return;
     }
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
