@@ -53,6 +53,18 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
     }
 }
 
+// The same at any alignment of the elements.
+template <int DT>
+__device__ __forceinline__ void load8_any(const void* p, int64_t i, float (&v)[8]) {
+    if constexpr (DT == RPFQ_F32) {
+        __builtin_memcpy(v, reinterpret_cast<const float*>(p) + i, 32);
+    } else {
+        uint4 u;
+        __builtin_memcpy(&u, reinterpret_cast<const uint16_t*>(p) + i, 16);
+        load8<DT>(&u, 0, v);
+    }
+}
+
 // What a row's largest magnitude (its bits: NaN above inf above numbers)
 // makes of it: the scale to store, and (top, r) for int8_code, both times a
 // power of two where 127 / top would overflow.  inf or NaN: scale NaN.
@@ -127,13 +139,23 @@ __global__ void __launch_bounds__(256) int8_rows_any_kernel(const void* x, int64
     }
 }
 
-// codes [N, K] of any K and alignment -> rows of ldq bytes, zeros past K
-__global__ void __launch_bounds__(256) int8_pad_kernel(const int8_t* src, int64_t lds_, int64_t K, int8_t* dst, int64_t ldq,
-                                                      int64_t total) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t n = i / ldq, k = i - n * ldq;
-        dst[i] = k < K ? src[n * lds_ + k] : (int8_t)0;
-    }
+// codes [rows, K] of any K and alignment -> rows of ldq bytes, zeros past K: a
+// wave a row, 16 bytes a lane.
+__global__ void __launch_bounds__(256) int8_pad_kernel(const int8_t* src, int64_t ld, int64_t K, int8_t* dst, int64_t ldq,
+                                                      int64_t rows) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (int64_t)gridDim.x * 4)
+        for (int64_t k = 16 * lane; k < ldq; k += 1024) {
+            int8_t e[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+            if (k + 16 <= K) {
+                __builtin_memcpy(e, src + n * ld + k, 16);
+            } else {
+#pragma unroll
+                for (int t = 0; t < 16; ++t)
+                    if (k + t < K) e[t] = src[n * ld + k + t];
+            }
+            __builtin_memcpy(dst + n * ldq + k, e, 16);
+        }
 }
 
 // ---------------------------------------------------------------------------
@@ -252,9 +274,18 @@ __global__ void __launch_bounds__(256) int8_few_kernel(Int8Few a) {
     int8_t* codes = reinterpret_cast<int8_t*>(smem);  // [16][pitch]
     for (int m = wave; m < a.M; m += 4) {
         uint32_t mx = 0;
+        auto piece = [&](int k, float (&v)[8]) {  // 8 values of the row, zeros past its end
+            const int64_t at = (int64_t)m * a.K + k;
+            if (k + 8 <= a.K) {
+                load8_any<XDT>(a.x, at, v);
+            } else {
+#pragma unroll
+                for (int t = 0; t < 8; ++t) v[t] = k + t < a.K ? load1<XDT>(a.x, at + t) : 0.0f;
+            }
+        };
         for (int k = 8 * lane; k < a.K; k += 512) {
             float v[8];
-            load8<XDT>(a.x, (int64_t)m * a.K + k, v);
+            piece(k, v);
 #pragma unroll
             for (int t = 0; t < 8; ++t) mx = max(mx, __float_as_uint(v[t]) & 0x7fffffffu);
         }
@@ -266,7 +297,7 @@ __global__ void __launch_bounds__(256) int8_few_kernel(Int8Few a) {
             uint32_t c[2] = {0, 0};
             if (k < a.K) {
                 float v[8];
-                load8<XDT>(a.x, (int64_t)m * a.K + k, v);
+                piece(k, v);
 #pragma unroll
                 for (int t = 0; t < 8; ++t) c[t >> 2] |= (uint32_t)(q.code(v[t]) & 0xff) << (8 * (t & 3));
             }
@@ -303,9 +334,8 @@ __global__ void __launch_bounds__(256) int8_few_kernel(Int8Few a) {
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-bool int8_few(const void* x, int xdt, int64_t M, int64_t K, const int8_t* w, int64_t ldw) {
-    return xdt >= 0 && M <= 16 && K % 8 == 0 && (M + 15) / 16 * 16 * int8_few_pitch(K) <= 140 * 1024 && M * K <= kInt8FewCodes &&
-           !int8_pads(w, ldw, K) && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+static bool int8_few(int xdt, int64_t M, int64_t K) {
+    return xdt >= 0 && M <= 16 && M * int8_few_pitch(K) <= 140 * 1024 && M * K <= kInt8FewCodes;
 }
 
 template <int XDT, int YDT>
@@ -376,34 +406,47 @@ static hipError_t gemm_y(Int8Args& a, hipStream_t s) {
     return tile_dispatch(tile_form(a.M, a.N), Int8Go<YDT>{a, s});
 }
 
-// x codes in `work` unless given; w copied there if its rows are not 16-byte aligned
-Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, bool quantize, bool pad_w) {
+// x codes in `work` unless given, or few; w copied there if its rows are not whole 16-byte pieces
+Int8Plan int8_plan(const void* x, int xdt, int64_t M, int64_t N, int64_t K, const int8_t* w, int64_t ldw) {
     Int8Plan p = {};
     p.ld = (K + 15) & ~(int64_t)15;
+    p.few = int8_few(xdt, M, K);
+    p.pad_w = int8_pads(w, ldw, K);
+    p.copy_x = !p.few && (xdt >= 0 || int8_pads(reinterpret_cast<const int8_t*>(x), K, K));
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
         p.bytes += (n + 255) & ~(size_t)255;
         return at;
     };
-    if (quantize) {
+    if (p.copy_x) {
         p.x_at = take((size_t)M * p.ld);
         p.sx_at = take((size_t)M * 4);
     }
-    if (pad_w) p.w_at = take((size_t)N * p.ld);
+    if (p.pad_w) p.w_at = take((size_t)N * p.ld);
     return p;
 }
 
 static hipError_t pad_codes(const int8_t* src, int64_t ld, int64_t K, int64_t rows, int8_t* dst, int64_t ldq, hipStream_t s) {
-    const int64_t total = rows * ldq, blocks = (total + 255) / 256;
-    hipLaunchKernelGGL(int8_pad_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, src, ld, K, dst, ldq,
-                       total);
+    const int64_t blocks = (rows + 3) / 4;
+    hipLaunchKernelGGL(int8_pad_kernel, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, src, ld, K, dst, ldq,
+                       rows);
     return hipGetLastError();
 }
 
 hipError_t launch_linear_int8(const void* x, int xdt, const float* sx, const int8_t* w, int64_t ldw, const float* sw,
                               const float* bias, int64_t M, int64_t N, int64_t K, void* y, int ydt, void* work,
                               hipStream_t s) {
-    if (int8_few(x, xdt, M, K, w, ldw)) {
+    const Int8Plan p = int8_plan(x, xdt, M, N, K, w, ldw);
+    char* wk = reinterpret_cast<char*>(work);
+    hipError_t e;
+    if (p.pad_w) {
+        int8_t* q = reinterpret_cast<int8_t*>(wk + p.w_at);
+        e = pad_codes(w, ldw, K, N, q, p.ld, s);
+        if (e != hipSuccess) return e;
+        w = q;
+        ldw = p.ld;
+    }
+    if (p.few) {
         const Int8Few f = {x, w, sw, bias, y, ldw, N, (int)M, (int)K};
         switch (xdt) {
             case RPFQ_F32: return few_y<RPFQ_F32>(f, ydt, s);
@@ -411,32 +454,19 @@ hipError_t launch_linear_int8(const void* x, int xdt, const float* sx, const int
             default: return few_y<RPFQ_BF16>(f, ydt, s);
         }
     }
-    const bool quantize = xdt >= 0, pad_w = int8_pads(w, ldw, K);
-    // codes that come unaligned are copied as an unaligned weight is
-    const bool pad_x = !quantize && int8_pads(x, K, K);
-    const Int8Plan p = int8_plan(M, N, K, quantize || pad_x, pad_w);
-    char* wk = reinterpret_cast<char*>(work);
     Int8Args a = {};
-    hipError_t e;
-    if (quantize || pad_x) {
+    a.x = {reinterpret_cast<const char*>(x), K, 0, M};
+    a.w = {reinterpret_cast<const char*>(w), ldw, 0, N};
+    a.sx = sx;
+    if (p.copy_x) {
         int8_t* q = reinterpret_cast<int8_t*>(wk + p.x_at);
         float* qs = reinterpret_cast<float*>(wk + p.sx_at);
-        e = quantize ? launch_quantize_int8(x, xdt, M, K, q, p.ld, qs, s)
+        // codes that come unaligned are copied as an unaligned weight is
+        e = xdt >= 0 ? launch_quantize_int8(x, xdt, M, K, q, p.ld, qs, s)
                      : pad_codes(reinterpret_cast<const int8_t*>(x), K, K, M, q, p.ld, s);
         if (e != hipSuccess) return e;
         a.x = {reinterpret_cast<const char*>(q), p.ld, 0, M};
-        a.sx = quantize ? qs : sx;
-    } else {
-        a.x = {reinterpret_cast<const char*>(x), K, 0, M};
-        a.sx = sx;
-    }
-    if (pad_w) {
-        int8_t* q = reinterpret_cast<int8_t*>(wk + p.w_at);
-        e = pad_codes(w, ldw, K, N, q, p.ld, s);
-        if (e != hipSuccess) return e;
-        a.w = {reinterpret_cast<const char*>(q), p.ld, 0, N};
-    } else {
-        a.w = {reinterpret_cast<const char*>(w), ldw, 0, N};
+        if (xdt >= 0) a.sx = qs;
     }
     a.sw = sw;
     a.bias = bias;

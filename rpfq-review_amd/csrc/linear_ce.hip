@@ -14,8 +14,8 @@
 // Roundings to 16 bits: dz only, once (bf16 2^-9 of its value; fp16 2^-12, dz
 // times 2^15 so that probabilities down to 2^-29 stay normal), as the matrix
 // cores take it; the sums over classes and rows stay in float32 until the
-// gradients are rounded to their own type.  float32 operands go as three bf16
-// terms (tile_pair) and lose nothing.
+// gradients are rounded to their own type.  float32 operands lose nothing:
+// many rows go as three bf16 terms (tile_pair), few as they are (kCeDirectRows).
 #include <cmath>
 
 #include "tile_gemm.h"
@@ -372,30 +372,55 @@ struct CeCopy {
     int64_t D, ld;
     const int64_t* target;
     int64_t ignore;
+    int lanes;
 };
-template <bool F32>
+// MODE 0: 16-bit rows, 1: planes, 2: float32 rows.  `lanes` (a power of two) take
+// a row, 8 elements each; whole pieces are read at once, at any alignment of
+// their elements.
+template <int MODE>
 __global__ void __launch_bounds__(256) ce_copy_kernel(CeCopy a) {
-    const int64_t per = a.ld / 8, first = a.rows[0] * per, total = first + a.rows[1] * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int k = i >= first;
-        const int64_t at = k ? i - first : i, m = at / per, d = (at - m * per) * 8;
+    const int lane = threadIdx.x & (a.lanes - 1), per = (int)(a.ld / 8);
+    const int64_t rows = a.rows[0] + a.rows[1], step = (int64_t)gridDim.x * (256 / a.lanes);
+    for (int64_t at = (int64_t)blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes; at < rows; at += step) {
+        const int k = at >= a.rows[0];
+        const int64_t m = k ? at - a.rows[0] : at;
         const bool on = k || !a.target || a.target[m] != a.ignore;
-        uint16_t* out = a.dst[k] + at * 8;
-        if constexpr (F32) {
-            const float* x = reinterpret_cast<const float*>(a.src[k]);
-            const int64_t plane = a.rows[k] * a.ld;
-            uint16_t h[8], mid[8], l[8];
+        for (int i = lane; i < per; i += a.lanes) {
+            const int64_t d = 8 * i;
+            uint16_t* out = a.dst[k] + (m * a.ld + d) * (MODE == 2 ? 2 : 1);
+            if constexpr (MODE == 0) {
+                const uint16_t* x = reinterpret_cast<const uint16_t*>(a.src[k]) + m * a.D + d;
+                uint16_t e[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (on && d + 8 <= a.D) {
+                    __builtin_memcpy(e, x, 16);
+                } else if (on) {
 #pragma unroll
-            for (int t = 0; t < 8; ++t) split3(on && d + t < a.D ? x[m * a.D + d + t] : 0.0f, h[t], mid[t], l[t]);
-            __builtin_memcpy(out, h, 16);
-            __builtin_memcpy(out + plane, mid, 16);
-            __builtin_memcpy(out + 2 * plane, l, 16);
-        } else {
-            const uint16_t* x = reinterpret_cast<const uint16_t*>(a.src[k]);
-            uint16_t e[8];
+                    for (int t = 0; t < 8; ++t)
+                        if (d + t < a.D) e[t] = x[t];
+                }
+                __builtin_memcpy(out, e, 16);
+            } else {
+                const float* x = reinterpret_cast<const float*>(a.src[k]) + m * a.D + d;
+                float e[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (on && d + 8 <= a.D) {
+                    __builtin_memcpy(e, x, 32);
+                } else if (on) {
 #pragma unroll
-            for (int t = 0; t < 8; ++t) e[t] = on && d + t < a.D ? x[m * a.D + d + t] : (uint16_t)0;
-            __builtin_memcpy(out, e, 16);
+                    for (int t = 0; t < 8; ++t)
+                        if (d + t < a.D) e[t] = x[t];
+                }
+                if constexpr (MODE == 2) {
+                    __builtin_memcpy(out, e, 32);
+                } else {
+                    const int64_t plane = a.rows[k] * a.ld;
+                    uint16_t h[8], mid[8], l[8];
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) split3(e[t], h[t], mid[t], l[t]);
+                    __builtin_memcpy(out, h, 16);
+                    __builtin_memcpy(out + plane, mid, 16);
+                    __builtin_memcpy(out + 2 * plane, l, 16);
+                }
+            }
         }
     }
 }
@@ -518,6 +543,10 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
                       [&](int row, int, f32x4 v) {
                           const int64_t m = mw + 32 * i + row;
                           if (m >= a.M || n >= a.n8) return;
+                          if constexpr (Mma::ES == 4) {
+                              *reinterpret_cast<f32x4*>(a.dz + m * a.ldz + 4 * n) = v;
+                              return;
+                          }
                           char* d = a.dz + m * a.ldz + 2 * n;
                           uint16_t h[4], k[4], l[4];
 #pragma unroll
@@ -655,8 +684,10 @@ __global__ void __launch_bounds__(256) ce_sum_kernel(const float* part, int part
 // the least time: the longest unit or the chip's share of all and half a unit,
 // in steps of a 256-row tile (0.9 us), and the partials' way through memory
 // (about 5 TB/s, and a launch).
-static CeSplit ce_split(int64_t M, int64_t V, int64_t D, int64_t pairs) {
-    const int64_t cus = device_cus(), tn = (D + 255) / 256, kx = pairs * ((V + 31) / 32), kw = pairs * ((M + 31) / 32);
+static CeSplit ce_split(int64_t M, int64_t V, int64_t D, int planes, int es) {
+    // float32 as it is: twice the steps, each eight times as long
+    const int64_t cost16 = planes == 3 ? kPairs32 : es == 4 ? 16 : 1, least = es == 4 ? 16 : 4;
+    const int64_t cus = device_cus(), tn = (D + 255) / 256, kx = cost16 * ((V + 31) / 32), kw = cost16 * ((M + 31) / 32);
     static constexpr int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64};
     CeSplit best = {kTile128, 1, 1};
     double cost = 1e300;
@@ -668,9 +699,9 @@ static CeSplit ce_split(int64_t M, int64_t V, int64_t D, int64_t pairs) {
     for (const auto& f : forms) {
         const int64_t slots = f.slots * cus;
         for (const int sx : kSplits) {
-            if (sx > 1 && 4 * sx > kx) break;
+            if (sx > 1 && least * sx > kx) break;
             for (const int sw : kSplits) {
-                if (sw > 1 && 4 * sw > kw) break;
+                if (sw > 1 && least * sw > kw) break;
                 const double nx = (double)((kx + sx - 1) / sx) * f.step + f.start, nw = (double)((kw + sw - 1) / sw) * f.step + f.start;
                 const double ux = (double)((M + f.rows - 1) / f.rows * tn * sx), uw = (double)((V + f.rows - 1) / f.rows * tn * sw);
                 const double longest = nx > nw ? nx : nw, rounds = (ux * nx + uw * nw) / (double)slots;
@@ -694,14 +725,24 @@ static CeSplit ce_split(int64_t M, int64_t V, int64_t D, int64_t pairs) {
 constexpr int64_t kCePiece = 1LL << 30;
 // Bytes of a row of dz with n classes: 16-byte pieces, and not a multiple of 4
 // KB, where a tile's rows would all lie on the same channels.
-static int64_t ce_ldz(int64_t n) {
-    const int64_t ld = 2 * ((n + 7) & ~(int64_t)7);
+static int64_t ce_ldz(int64_t n, int es) {
+    const int64_t ld = es * ((n + 7) & ~(int64_t)7);
     return ld % 4096 == 0 ? ld + 256 : ld;
 }
 
+// float32 products of few rows: as they are, on the float32 matrix
+// instructions.  Three planes of both operands cost 20 bytes an element of w and
+// pass, whatever M is, but from about 256 rows on their products are 1.2 to 1.6
+// times as fast (loss and gradients, us, planes -> direct: 50,000 classes x 1,024,
+// 16 rows 649 -> 270, 128 773 -> 545, 256 1,017 -> 997, 512 1,626 -> 1,936;
+// 10,008 x 768, 64 rows 185 -> 163, 256 both 221, 1,024 492 -> 677).
+constexpr int64_t kCeDirectRows = 256;
+
 CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool backward) {
     CePlan p = {};
-    const int planes = dt == RPFQ_F32 ? 3 : 1;
+    const bool direct = dt == RPFQ_F32 && M <= kCeDirectRows;
+    const int planes = p.planes = dt == RPFQ_F32 && !direct ? 3 : 1;
+    const int es = p.es = direct ? 4 : 2;
     p.ldk = planes == 3 ? (D + 31) & ~(int64_t)31 : (D + 7) & ~(int64_t)7;
     p.pad = planes == 3 || D % 8 != 0;
     auto take = [&](int64_t n) {
@@ -710,8 +751,8 @@ CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool back
         return at;
     };
     if (p.pad) {
-        p.x_at = take(2 * planes * M * p.ldk);
-        p.w_at = take(2 * planes * V * p.ldk);
+        p.x_at = take(es * planes * M * p.ldk);
+        p.w_at = take(es * planes * V * p.ldk);
     }
     p.tiles_v = (V + 255) / 256;
     if (!backward) {
@@ -721,19 +762,18 @@ CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool back
         p.rows_at = take(reduction ? 4 * M : 0);
         return p;
     }
-    if (!p.pad) p.x_at = take(2 * M * p.ldk);  // x without its ignored rows
+    if (!p.pad) p.x_at = take(es * M * p.ldk);  // x without its ignored rows
     p.rho_at = take(4 * M);
     p.factor_at = take(4);
-    const int64_t fit = std::max<int64_t>(1, kCePiece / (2 * planes * M * 256));
+    const int64_t fit = std::max<int64_t>(1, kCePiece / (es * planes * M * 256));
     p.pieces = (p.tiles_v + fit - 1) / fit;
     p.piece = (p.tiles_v + p.pieces - 1) / p.pieces * 256;  // classes
     if (p.piece > V) p.piece = (V + 7) & ~(int64_t)7;
-    p.dz_at = take(planes * M * (2 * p.piece + 256));
+    p.dz_at = take(planes * M * (es * p.piece + 256));
     p.col_at = take(4 * ((M + 31) / 32 + 8) * p.piece);
     // float32 partials, rows of whole 16 bytes
     p.ldp = (D + 3) & ~(int64_t)3;
-    const int64_t pairs = planes == 3 ? kPairs32 : 1;
-    p.grad = ce_split(M, p.piece, D, pairs);
+    p.grad = ce_split(M, p.piece, D, planes, es);
     p.dx_at = take(p.grad.dx > 1 || p.pieces > 1 ? 4 * p.grad.dx * M * p.ldp : 0);
     p.dw_at = take(p.grad.dw > 1 ? 4 * p.grad.dw * p.piece * p.ldp : 0);
     return p;
@@ -744,8 +784,8 @@ static unsigned blocks_of(int64_t n) { return (unsigned)(n < 1 ? 1 : n > 16384 ?
 // The operands of the logits: as they are, or padded / split copies in `work`.
 // target: rows of x that it ignores are zero there (backward).
 static hipError_t ce_operands(const CePlan& p, const CeCall& c, const int64_t* target, char* wk, CeArgs& a, hipStream_t s) {
-    a.kb = 2 * p.ldk;
-    a.planes = c.dtype == RPFQ_F32;
+    a.kb = p.es * p.ldk;
+    a.planes = p.planes == 3;
     a.x = {reinterpret_cast<const char*>(c.x), a.kb, 0, c.M};
     a.w = {reinterpret_cast<const char*>(c.w), a.kb, 0, c.V};
     a.bias = c.bias;
@@ -756,19 +796,23 @@ static hipError_t ce_operands(const CePlan& p, const CeCall& c, const int64_t* t
     a.smooth = c.smooth;
     a.ignore = c.ignore;
     if (!p.pad) return hipSuccess;
+    int lanes = 1;
+    while (lanes < 64 && 8 * lanes < p.ldk) lanes *= 2;
     const CeCopy k = {{c.x, c.w},
                       {reinterpret_cast<uint16_t*>(wk + p.x_at), reinterpret_cast<uint16_t*>(wk + p.w_at)},
                       {c.M, c.V},
                       c.D,
                       p.ldk,
                       target,
-                      c.ignore};
-    const dim3 grid(blocks_of(((c.M + c.V) * (p.ldk / 8) + 255) / 256));
-    if (a.planes) hipLaunchKernelGGL(ce_copy_kernel<true>, grid, dim3(256), 0, s, k);
-    else hipLaunchKernelGGL(ce_copy_kernel<false>, grid, dim3(256), 0, s, k);
+                      c.ignore,
+                      lanes};
+    const dim3 grid(blocks_of(((c.M + c.V) * lanes + 255) / 256));
+    if (a.planes) hipLaunchKernelGGL(ce_copy_kernel<1>, grid, dim3(256), 0, s, k);
+    else if (p.es == 4) hipLaunchKernelGGL(ce_copy_kernel<2>, grid, dim3(256), 0, s, k);
+    else hipLaunchKernelGGL(ce_copy_kernel<0>, grid, dim3(256), 0, s, k);
     a.x.p = wk + p.x_at;
     a.w.p = wk + p.w_at;
-    a.x.plane = 2 * c.M * p.ldk;
+    a.x.plane = 2 * c.M * p.ldk;  // planes are 16-bit
     a.w.plane = 2 * c.V * p.ldk;
     return hipGetLastError();
 }
@@ -849,8 +893,9 @@ struct GradGo {
         }
     }
 };
-static hipError_t ce_grads(int dt, TileForm form, CeGrads& g, hipStream_t s) {
-    return dt == RPFQ_F16    ? tile_dispatch(form, GradGo<MmaF16, RPFQ_F16>{g, s})
+static hipError_t ce_grads(int dt, bool direct, TileForm form, CeGrads& g, hipStream_t s) {
+    return direct            ? tile_dispatch(form, GradGo<MmaF32, RPFQ_F32>{g, s})
+           : dt == RPFQ_F16  ? tile_dispatch(form, GradGo<MmaF16, RPFQ_F16>{g, s})
            : dt == RPFQ_BF16 ? tile_dispatch(form, GradGo<MmaBf16, RPFQ_BF16>{g, s})
                              : tile_dispatch(form, GradGo<MmaBf16, RPFQ_F32>{g, s});
 }
@@ -883,7 +928,9 @@ hipError_t launch_linear_ce(const CeCall& c, float* loss, float* stat, float* co
     a.zsum = c.smooth > 0.0f ? reinterpret_cast<float*>(wk + p.zsum_at) : nullptr;
     a.zt = reinterpret_cast<float*>(wk + p.zt_at);
     const TileForm form = tile_form(c.M, c.V);
-    e = c.dtype == RPFQ_F16 ? tile_dispatch(form, StatsGo<MmaF16>{a, s}) : tile_dispatch(form, StatsGo<MmaBf16>{a, s});
+    e = p.es == 4              ? tile_dispatch(form, StatsGo<MmaF32>{a, s})
+        : c.dtype == RPFQ_F16 ? tile_dispatch(form, StatsGo<MmaF16>{a, s})
+                              : tile_dispatch(form, StatsGo<MmaBf16>{a, s});
     if (e != hipSuccess) return e;
     float* rows = c.reduction ? reinterpret_cast<float*>(wk + p.rows_at) : loss;
     const CeJoin j = {a.part, a.zsum, a.zt, c.target, c.M, c.V, c.ignore, (int)p.tiles_v, c.smooth, c.reduction, stat, rows, loss,
@@ -936,12 +983,13 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         a.v0 = v0;
         a.w.p = w.p + v0 * w.ld;
         a.w.count = n;
-        a.ldz = ce_ldz(n);
+        a.ldz = ce_ldz(n, p.es);
         a.n8 = (n + 7) & ~(int64_t)7;
         a.dz_plane = c.M * a.ldz;
         const TileForm form = tile_form(c.M, n);
         int col_rows = 0;
-        e = c.dtype == RPFQ_F16    ? tile_dispatch(form, DzGo<MmaF16, RPFQ_F16>{a, col_rows, s})
+        e = p.es == 4              ? tile_dispatch(form, DzGo<MmaF32, RPFQ_F32>{a, col_rows, s})
+            : c.dtype == RPFQ_F16  ? tile_dispatch(form, DzGo<MmaF16, RPFQ_F16>{a, col_rows, s})
             : c.dtype == RPFQ_BF16 ? tile_dispatch(form, DzGo<MmaBf16, RPFQ_BF16>{a, col_rows, s})
                                    : tile_dispatch(form, DzGo<MmaBf16, RPFQ_F32>{a, col_rows, s});
         if (e != hipSuccess) return e;
@@ -955,7 +1003,7 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         dx.factor = dw.factor = factor;
         dx.r = dzk;
         dx.c = {a.w.p, w.ld, w.plane, p.ldk};
-        dx.rk = 2 * a.n8;
+        dx.rk = p.es * a.n8;
         dx.ck = n;
         dx.M = c.M;
         dx.splits = gx ? p.grad.dx : 0;
@@ -971,7 +1019,7 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         dw.part = p.grad.dw > 1 ? reinterpret_cast<float*>(wk + p.dw_at) : nullptr;
         dw.out = gw ? reinterpret_cast<char*>(gw) + v0 * c.D * es : nullptr;
         dw.vec = c.D % 4 == 0 && reinterpret_cast<uintptr_t>(dw.out) % (4 * es) == 0;
-        if ((gx || gw) && (e = ce_grads(c.dtype, p.grad.form, both, s)) != hipSuccess) return e;
+        if ((gx || gw) && (e = ce_grads(c.dtype, p.es == 4, p.grad.form, both, s)) != hipSuccess) return e;
         if (gw && dw.part &&
             (e = ce_sum(c.dtype, dw.part, dw.splits, n * p.ldp, n, c.D, p.ldp, factor, dw.out, s)) != hipSuccess)
             return e;

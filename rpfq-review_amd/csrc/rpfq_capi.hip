@@ -775,9 +775,7 @@ int rpfq_quantize_int8(const void* x, int x_dtype, int64_t M, int64_t K, int8_t*
 size_t rpfq_linear_int8_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t N, int64_t K, const int8_t* w,
                                         int64_t ld_w) {
     if (check_int8(M, N, K, x_dtype, ld_w) != RPFQ_OK) return 0;
-    if (rpfq::int8_few(x, x_dtype == RPFQ_I8 ? -1 : x_dtype, M, K, w, ld_w)) return 0;
-    const bool copy_x = x_dtype != RPFQ_I8 || rpfq::int8_pads(reinterpret_cast<const int8_t*>(x), K, K);
-    return rpfq::int8_plan(M, N, K, copy_x, rpfq::int8_pads(w, ld_w, K)).bytes;
+    return rpfq::int8_plan(x, x_dtype == RPFQ_I8 ? -1 : x_dtype, M, N, K, w, ld_w).bytes;
 }
 
 int rpfq_linear_int8(const void* x, int x_dtype, const float* x_scale, const int8_t* w, int64_t ld_w, const float* w_scale,

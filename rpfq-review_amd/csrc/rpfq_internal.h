@@ -378,14 +378,13 @@ hipError_t launch_linear_f32_grad(const float* gy, const float* x, const float* 
 // padded copy.
 struct Int8Plan {
     int64_t ld;  // row bytes of codes in the workspace
+    bool few, copy_x, pad_w;
     size_t x_at, sx_at, w_at, bytes;
 };
 inline bool int8_pads(const void* codes, int64_t ld, int64_t K) {
     return ld < ((K + 15) & ~(int64_t)15) || ld % 16 != 0 || reinterpret_cast<uintptr_t>(codes) % 16 != 0;
 }
-// whether few rows go in one launch without a workspace
-bool int8_few(const void* x, int xdt, int64_t M, int64_t K, const int8_t* w, int64_t ldw);
-Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, bool quantize, bool pad_w);
+Int8Plan int8_plan(const void* x, int xdt, int64_t M, int64_t N, int64_t K, const int8_t* w, int64_t ldw);
 hipError_t launch_quantize_int8(const void* x, int dt, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale,
                                 hipStream_t s);
 // xdt < 0: x holds codes and sx their scales
@@ -409,6 +408,7 @@ struct CeSplit {
     int dx, dw;     // parts of their k
 };
 struct CePlan {
+    int es, planes;         // bytes of an operand's element, bf16 terms of a float32
     int64_t ldk, ldp;       // elements of a row of k; of float32 partials
     bool pad;               // x and w are copied (rows of ldk, or three planes of them)
     int64_t tiles_v, piece, pieces;

@@ -15,29 +15,46 @@ typedef __attribute__((address_space(3))) s16x4* lds_s4_t;
 typedef __attribute__((address_space(3))) const intx4* lds_i4_t;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// The 32 x 32 products: 32 bytes of k a row (16 halves, 32 int8).
+// The 32 x 32 products: 32 bytes of k a row (16 halves, 32 int8, 8 floats), ES
+// bytes an element.
 struct MmaF16 {
     using acc_t = floatx16;
+    static constexpr int ES = 2;
     static __device__ __forceinline__ acc_t mma(uint4 a, uint4 b, acc_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
     }
 };
 struct MmaBf16 {
     using acc_t = floatx16;
+    static constexpr int ES = 2;
     static __device__ __forceinline__ acc_t mma(uint4 a, uint4 b, acc_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
 };
 struct MmaI8 {
     using acc_t = intx16;
+    static constexpr int ES = 1;
     static __device__ __forceinline__ acc_t mma(uint4 a, uint4 b, acc_t c) {
         return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(intx4, a), __builtin_bit_cast(intx4, b), c, 0, 0, 0);
     }
 };
 
+// float32 as it is, 1/16 of the 16-bit rate: lane (r, g) holds k = 4 (2 s + g) + t
+// in both operands, one of them a step.
+struct MmaF32 {
+    using acc_t = floatx16;
+    static constexpr int ES = 4;
+    static __device__ __forceinline__ acc_t mma(uint4 a, uint4 b, acc_t c) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[t], y[t], c, 0, 0, 0);
+        return c;
+    }
+};
+
 // One operand of a product.  K layout: `count` rows of `k_bytes` at p + row ld.
-// T layout: k rows at p + k ld of `count` 2-byte elements.  p, ld, k_bytes (K)
-// and 2 count (T) are multiples of 16 bytes.  Planes (float32 as three bf16
+// T layout: k rows at p + k ld of `count` elements.  p, ld, k_bytes (K) and the
+// bytes of count (T) are multiples of 16.  Planes (float32 as three bf16
 // terms) lie `plane` bytes apart.
 struct TileOperand {
     const char* p;
@@ -76,32 +93,35 @@ constexpr uint32_t kTileOut = 0x80000000u;  // an offset past every resource's e
 // read takes, fall on all 64 banks once (5.7 clocks a 1-KB read, 16 to 32
 // unswizzled).  T layout: KB / 2 k rows of 2 W bytes, chunk c at c ^ ((k & 3) <<
 // 2) (64 columns: c ^ (k & 2) << 1): the 4 rows x 64 B of a transposed read on
-// distinct banks.
-template <int W, bool T, int WAVES, int KB>
+// distinct banks.  T layout of float32: KB / 4 rows of 4 W bytes, read a value at
+// a time; chunk c at c ^ 8 where k & 4, so the two halves of a wave, four rows
+// apart, fall on different banks.
+template <int W, bool T, int WAVES, int KB, int ES>
 struct TileSide {
     static constexpr int BYTES = W * KB;
     static constexpr int LOADS = W * KB / 1024 / WAVES;  // DMA loads per wave and step, 1 KB each
-    static constexpr int CH = W / 8;                     // T: chunks of a k row
+    static constexpr int CH = W * ES / 16;               // T: chunks of a k row
+    static constexpr int PER = T ? KB / ES : KB;         // k of a step: rows (T) or bytes of a row
     static constexpr int KC = KB / 16;                   // K: chunks of a row
     uint32_t v[LOADS];
     uint32_t kpos[LOADS];  // K: byte of k within a step; T: k row within a step
     const char* base;
     int64_t ld, plane;
 
-    static __device__ __forceinline__ int swz(int k) { return CH >= 16 ? (k & 3) << 2 : (k & 2) << 1; }
+    static __device__ __forceinline__ int swz(int k) { return ES == 4 ? (k & 4) << 1 : CH >= 16 ? (k & 3) << 2 : (k & 2) << 1; }
     static __device__ __forceinline__ int kswz(int row) { return KC == 4 ? (row >> 2) & 3 : (row >> 1) & 7; }
 
     __device__ __forceinline__ void init(const TileOperand& o, int64_t first, int wave, int lane) {
         ld = o.ld;
         plane = o.plane;
-        base = o.p + (T ? first * 2 : first * o.ld);
+        base = o.p + (T ? first * ES : first * o.ld);
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
             const int piece = wave * LOADS + j;
             if (T) {
                 const int k = piece * (64 / CH) + lane / CH, c = (lane % CH) ^ swz(k);
                 kpos[j] = (uint32_t)k;
-                v[j] = first + 8 * c < o.count ? (uint32_t)(k * o.ld + c * 16) : kTileOut;
+                v[j] = first + (16 / ES) * c < o.count ? (uint32_t)(k * o.ld + c * 16) : kTileOut;
             } else {
                 const int row = piece * (64 / KC) + lane / KC, c = (lane % KC) ^ kswz(row);
                 kpos[j] = (uint32_t)(c * 16);
@@ -111,7 +131,6 @@ struct TileSide {
     }
     // step `ks` of plane pl (k: bytes of a row (K) or rows (T)) to LDS at `lds`
     __device__ __forceinline__ void issue(int ks, int pl, int64_t k, uint32_t lds, int wave) {
-        constexpr int PER = T ? KB / 2 : KB;
         const intx4 rs = tile_rsrc(base + pl * plane + (T ? (int64_t)ks * PER * ld : (int64_t)ks * PER));
         const int64_t left64 = k - (int64_t)ks * PER;
         const uint32_t left = (uint32_t)(left64 > PER ? PER : left64);
@@ -122,6 +141,7 @@ struct TileSide {
     static __device__ __forceinline__ uint32_t at(int lane, int s) {
         const int r = lane & 31, g = lane >> 5;
         if (!T) return (uint32_t)(r * KB + (((2 * s + g) ^ kswz(r)) * 16));
+        if (ES == 4) return (uint32_t)(4 * g * 4 * W + r * 4);
         const int i16 = lane & 15, hf = (lane >> 4) & 1, k = 8 * g + (i16 >> 2);
         return (uint32_t)(k * 2 * W + ((2 * hf + ((i16 & 3) >> 1)) * 16) + (i16 & 1) * 8);
     }
@@ -133,6 +153,12 @@ struct TileSide {
             // the compiler took 8-byte reads instead (1,050 -> 1,290 TFLOP/s)
             asm("" : "+v"(a));
             return __builtin_bit_cast(uint4, *((lds_i4_t)a + b * 2 * KB));
+        } else if constexpr (ES == 4) {
+            const uint32_t a = stage + ((at[0] + b * 128) ^ (uint32_t)(lane >> 5 << 7)) + s * 32 * W;
+            uint32_t v[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) v[t] = *((lds_u32_t)(a + t * 4 * W));
+            return make_uint4(v[0], v[1], v[2], v[3]);
         } else {
             const int k = (lane & 15) >> 2;  // modulo 4: what the swizzle looks at
             const uint32_t a = stage + ((at[0] + b * 64) ^ (uint32_t)(swz(k) * 16)) + s * 32 * W;
@@ -160,15 +186,15 @@ template <int MB, int WM, int S, int KB, bool RT, bool CT, class Mma>
 struct TileGemm {
     static constexpr int WAVES = 4 * WM, THREADS = 64 * WAVES, ROWS = 32 * MB * WM;
     static constexpr int RW = ROWS < 64 ? 64 : ROWS;  // rows of R loaded: one DMA load a wave at least
-    using R = TileSide<RW, RT, WAVES, KB>;
-    using C = TileSide<256, CT, WAVES, KB>;
+    using R = TileSide<RW, RT, WAVES, KB, Mma::ES>;
+    using C = TileSide<256, CT, WAVES, KB, Mma::ES>;
     using acc_t = typename Mma::acc_t;
     static constexpr int SUB = KB / 32;
     static constexpr int STAGE = R::BYTES + C::BYTES;
     static constexpr int LDS = S * STAGE;
     static constexpr int LOADS = R::LOADS + C::LOADS;
-    // steps of k (bytes of a row where an operand is in K layout, else rows)
-    static constexpr int64_t steps(int64_t k) { return RT && CT ? (k + KB / 2 - 1) / (KB / 2) : (k + KB - 1) / KB; }
+    // steps of R's k (bytes of a row in K layout, rows in T)
+    static constexpr int64_t steps(int64_t k) { return (k + R::PER - 1) / R::PER; }
 
     // Adds steps s0 .. s1 - 1 of the product; a step is KB bytes of k of one
     // pair of planes, `per` steps a pair.  rk, ck: k of the operands as issue()
