@@ -658,7 +658,8 @@ size_t rpfq_linear_int8_workspace_bytes(const void* x, int x_dtype, int64_t M, i
  * y[m][n] = (sum_k cx[m][k] w[n][k]) sx[m] w_scale[n] + bias[n], the sum exact
  * in int32, the rest float32 rounded once to y_dtype.  x [M, K]: values of
  * x_dtype that the call quantizes as rpfq_quantize_int8 (x_scale NULL), or codes
- * (x_dtype = RPFQ_I8) with their scales x_scale [M].  w: N rows of ld_w bytes
+ * (x_dtype = RPFQ_I8) with their scales x_scale [M].  Codes are -127 .. 127 (with
+ * -128 in both operands the largest K is 131071).  w: N rows of ld_w bytes
  * (>= K), read in place where w and ld_w are multiples of 16 and ld_w holds K
  * rounded up to 16 (whose bytes past K may be anything, in the last row too),
  * else from a copy; w_scale [N], bias [N] or NULL float32.  K <= 131072.  work 256-byte
@@ -686,15 +687,16 @@ typedef struct rpfq_ce_desc {
 
 /* Bytes of the device workspace of rpfq_linear_cross_entropy (backward = 0) or
  * its gradient (1): there a piece of the logits' gradient, at most about 1 GiB
- * whatever V is; 0 if the shape is not taken. */
+ * whatever V is; 0 if the shape is not taken (M or V above 2^22, M V above
+ * 2^39, D above 2^16). */
 size_t rpfq_linear_cross_entropy_workspace_bytes(const rpfq_ce_desc* desc, int backward);
 
 /*
  * loss: float32, [1], or [M] with RPFQ_REDUCE_NONE.  The logits are not kept:
  * stat [3][M] (each row's maximum, 1 / sum exp(z - maximum), the target's logit)
  * and coef [1] (the mean's factor) are what the gradient needs of them.
- * float32 sums; float32 operands are multiplied as three bf16 terms each, at
- * float32 accuracy.  x and w 16-byte aligned where D % 8 == 0, work 256-byte.
+ * float32 sums; float32 operands are multiplied at float32 accuracy (up to 256
+ * rows as they are, more as three bf16 terms each).  x and w 16-byte aligned where D % 8 == 0, work 256-byte.
  * Replaces F.cross_entropy(head(x), target) of the reference's training loop.
  */
 int rpfq_linear_cross_entropy(const rpfq_ce_desc* desc, const void* x, const void* w, const void* bias,

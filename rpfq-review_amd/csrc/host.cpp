@@ -13,7 +13,10 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -357,7 +360,25 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
         return out;
     }
 
+    // Under capture: whether the engine would next add to a leaf on the default
+    // stream, where an eager graph that is still alive has bound it; joining that
+    // stream to the capture ends the process, not the call.
+    static bool leaves_capture() {
+        if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return false;
+        const auto* inputs = torch::autograd::get_current_graph_task_exec_info();
+        const auto node = torch::autograd::get_current_node();
+        if (!node || (inputs && !inputs->empty())) return false;  // autograd.grad adds to no leaf
+        for (const auto& edge : node->next_edges())
+            if (dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) {
+                const auto s = edge.function->stream();
+                if (s && s->id() == 0) return true;  // the default stream
+            }
+        return false;
+    }
+
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!leaves_capture(), "linear_cross_entropy: backward under capture while an eager graph of the same leaves is "
+                    "alive: let go of its outputs first");
         const auto saved = ctx->get_saved_variables();
         const at::Tensor &x = saved[0], &w = saved[1], &target = saved[2], &bias = saved[3], &stat = saved[4];
         const c10::DeviceGuard guard(x.device());
@@ -488,8 +509,9 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int code = dtype_code(type);
     if (code < 0 || scalar[0]->is_inference()) Py_RETURN_NONE;
     std::vector<rpfq_adamw_tensor> table(count);
-    std::vector<const void*> seen;
+    std::vector<std::pair<const char*, const char*>> seen;  // what the step writes
     seen.reserve(3 * count);
+    const int64_t es = p[0]->element_size(), ss = small ? 1 : 4;
     for (size_t i = 0; i < count; ++i) {
         const int64_t size = p[i]->numel();
         if (p[i]->scalar_type() != type || g[i]->scalar_type() != type || g[i]->sizes() != p[i]->sizes() ||
@@ -505,10 +527,17 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
             t.exp_avg_scale = sm[i]->data_ptr<float>();
             t.exp_avg_sq_scale = sv[i]->data_ptr<float>();
         }
-        if (size) seen.insert(seen.end(), {t.param, t.exp_avg, t.exp_avg_sq});
+        auto writes = [&](const void* at, int64_t bytes) {
+            const char* c = reinterpret_cast<const char*>(at);
+            if (bytes) seen.emplace_back(c, c + bytes);
+        };
+        writes(t.param, size * es);
+        writes(t.exp_avg, size * ss);
+        writes(t.exp_avg_sq, size * ss);
     }
     std::sort(seen.begin(), seen.end());
-    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_NONE;
+    for (size_t i = 1; i < seen.size(); ++i)
+        if (seen[i].first < seen[i - 1].second) Py_RETURN_NONE;
     int rc;
     {
         Unlocked u;

@@ -87,34 +87,34 @@ template <int DT, int NC>
 __global__ void __launch_bounds__(256) int8_rows_kernel(const void* x, int64_t M, int K, int8_t* q, int64_t ldq,
                                                        float* scale) {
     const int lane = threadIdx.x & 63;
-    const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (m >= M) return;
-    float v[NC][8];
-    uint32_t mx = 0;
+    for (int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); m < M; m += (int64_t)gridDim.x * 4) {
+        float v[NC][8];
+        uint32_t mx = 0;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int c = 8 * (lane + 64 * i);
-        if (c < K) {
-            load8<DT>(x, m * K + c, v[i]);
-        } else {
+        for (int i = 0; i < NC; ++i) {
+            const int c = 8 * (lane + 64 * i);
+            if (c < K) {
+                load8<DT>(x, m * K + c, v[i]);
+            } else {
 #pragma unroll
-            for (int t = 0; t < 8; ++t) v[i][t] = 0.0f;
+                for (int t = 0; t < 8; ++t) v[i][t] = 0.0f;
+            }
+#pragma unroll
+            for (int t = 0; t < 8; ++t) mx = max(mx, __float_as_uint(v[i][t]) & 0x7fffffffu);
         }
 #pragma unroll
-        for (int t = 0; t < 8; ++t) mx = max(mx, __float_as_uint(v[i][t]) & 0x7fffffffu);
-    }
+        for (int o = 32; o > 0; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
+        const Int8Row row(mx);
+        if (lane == 0) scale[m] = row.scale;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
-    const Int8Row row(mx);
-    if (lane == 0) scale[m] = row.scale;
+        for (int i = 0; i < NC; ++i) {
+            const int c = 8 * (lane + 64 * i);
+            if (c >= ldq) continue;
+            uint32_t w[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int c = 8 * (lane + 64 * i);
-        if (c >= ldq) continue;
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int t = 0; t < 8; ++t) w[t >> 2] |= (uint32_t)(row.code(v[i][t]) & 0xff) << (8 * (t & 3));
-        *reinterpret_cast<uint2*>(q + m * ldq + c) = make_uint2(w[0], w[1]);
+            for (int t = 0; t < 8; ++t) w[t >> 2] |= (uint32_t)(row.code(v[i][t]) & 0xff) << (8 * (t & 3));
+            *reinterpret_cast<uint2*>(q + m * ldq + c) = make_uint2(w[0], w[1]);
+        }
     }
 }
 
@@ -359,7 +359,8 @@ template <int DT>
 static hipError_t quantize_dt(const void* x, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale, hipStream_t s) {
     const bool vec = K % 8 == 0 && ldq % 8 == 0 && ldq <= 4096 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
                      reinterpret_cast<uintptr_t>(q) % 8 == 0;
-    const dim3 rows((unsigned)((M + 3) / 4));
+    // at most 2^22 workgroups: a launch's threads are counted in 32 bits
+    const dim3 rows((unsigned)(M < (1LL << 24) ? (M + 3) / 4 : 1LL << 22));
 #define RPFQ_ROWS(NC) hipLaunchKernelGGL((int8_rows_kernel<DT, NC>), rows, dim3(256), 0, s, x, M, (int)K, q, ldq, scale)
     if (vec && ldq <= 512) RPFQ_ROWS(1);
     else if (vec && ldq <= 1024) RPFQ_ROWS(2);

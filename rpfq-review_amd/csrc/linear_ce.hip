@@ -869,35 +869,31 @@ struct GradGo {
     hipStream_t s;
     template <int MB, int WM, int S, int KB>
     hipError_t run() {
-        if constexpr (MB == 1 && WM == 1) {
-            return hipErrorInvalidValue;  // ce_split takes 64 rows at least
-        } else {
-            using X = TileGemm<MB, WM, S, KB, false, true, Mma>;
-            using W = TileGemm<MB, WM, S, KB, true, true, Mma>;
-            static_assert(X::LDS == W::LDS, "one launch");
-            static std::atomic<uint64_t> done{0};
-            const hipError_t e = ce_lds(&ce_grads_kernel<MB, WM, S, KB, Mma, DT>, X::LDS, done);
-            if (e != hipSuccess) return e;
-            double length[2];
-            for (int k = 0; k < 2; ++k) {
-                CeGrad& g = a.g[k];
-                g.tiles_m = (int)((g.M + X::ROWS - 1) / X::ROWS);
-                g.tiles_n = (int)((g.N + 255) / 256);
-                a.units[k] = g.tiles_m * g.tiles_n * g.splits;
-                length[k] = g.splits ? (double)(k ? W::steps(g.rk) : X::steps(g.rk)) / g.splits : 0.0;
-            }
-            a.first = length[1] > length[0];
-            hipLaunchKernelGGL((ce_grads_kernel<MB, WM, S, KB, Mma, DT>), dim3((unsigned)(a.units[0] + a.units[1])),
-                               dim3(X::THREADS), X::LDS, s, a);
-            return hipGetLastError();
+        using X = TileGemm<MB, WM, S, KB, false, true, Mma>;
+        using W = TileGemm<MB, WM, S, KB, true, true, Mma>;
+        static_assert(X::LDS == W::LDS, "one launch");
+        static std::atomic<uint64_t> done{0};
+        const hipError_t e = ce_lds(&ce_grads_kernel<MB, WM, S, KB, Mma, DT>, X::LDS, done);
+        if (e != hipSuccess) return e;
+        double length[2];
+        for (int k = 0; k < 2; ++k) {
+            CeGrad& g = a.g[k];
+            g.tiles_m = (int)((g.M + X::ROWS - 1) / X::ROWS);
+            g.tiles_n = (int)((g.N + 255) / 256);
+            a.units[k] = g.tiles_m * g.tiles_n * g.splits;
+            length[k] = g.splits ? (double)(k ? W::steps(g.rk) : X::steps(g.rk)) / g.splits : 0.0;
         }
+        a.first = length[1] > length[0];
+        hipLaunchKernelGGL((ce_grads_kernel<MB, WM, S, KB, Mma, DT>), dim3((unsigned)(a.units[0] + a.units[1])),
+                           dim3(X::THREADS), X::LDS, s, a);
+        return hipGetLastError();
     }
 };
 static hipError_t ce_grads(int dt, bool direct, TileForm form, CeGrads& g, hipStream_t s) {
-    return direct            ? tile_dispatch(form, GradGo<MmaF32, RPFQ_F32>{g, s})
-           : dt == RPFQ_F16  ? tile_dispatch(form, GradGo<MmaF16, RPFQ_F16>{g, s})
-           : dt == RPFQ_BF16 ? tile_dispatch(form, GradGo<MmaBf16, RPFQ_BF16>{g, s})
-                             : tile_dispatch(form, GradGo<MmaBf16, RPFQ_F32>{g, s});
+    return direct            ? tile_dispatch64(form, GradGo<MmaF32, RPFQ_F32>{g, s})
+           : dt == RPFQ_F16  ? tile_dispatch64(form, GradGo<MmaF16, RPFQ_F16>{g, s})
+           : dt == RPFQ_BF16 ? tile_dispatch64(form, GradGo<MmaBf16, RPFQ_BF16>{g, s})
+                             : tile_dispatch64(form, GradGo<MmaBf16, RPFQ_F32>{g, s});
 }
 
 static hipError_t ce_sum(int dt, const float* part, int parts, int64_t stride, int64_t rows, int64_t N, int64_t ldp,

@@ -86,6 +86,9 @@ int check_ce(const rpfq_ce_desc* d) {
         return fail(RPFQ_ERR_SHAPE, "M=%lld V=%lld D=%lld must be positive", (long long)d->M, (long long)d->V, (long long)d->D);
     if (d->M > (1LL << 22) || d->V > (1LL << 22) || d->D > (1LL << 16))
         return fail(RPFQ_ERR_SHAPE, "M=%lld V=%lld exceed 2^22 or D=%lld 2^16", (long long)d->M, (long long)d->V, (long long)d->D);
+    // a launch's threads, two a row and 256 classes, are counted in 32 bits
+    if (d->M * ((d->V + 255) / 256) >= 1LL << 31)
+        return fail(RPFQ_ERR_SHAPE, "M=%lld V=%lld: more than 2^39 logits", (long long)d->M, (long long)d->V);
     if (!dtype_ok(d->dtype) || !dtype_ok(d->bias_dtype)) return fail(RPFQ_ERR_DTYPE, "unsupported dtype %d / %d", d->dtype, d->bias_dtype);
     if (d->reduction < RPFQ_REDUCE_NONE || d->reduction > RPFQ_REDUCE_SUM) return fail(RPFQ_ERR_VALUE, "unknown reduction %d", d->reduction);
     if (!(d->smoothing >= 0.0f && d->smoothing <= 1.0f)) return fail(RPFQ_ERR_VALUE, "smoothing %g is not within 0 .. 1", d->smoothing);

@@ -281,16 +281,19 @@ inline TileForm tile_form(int64_t M, int64_t N) {
     if (t128 <= cus) return kTile128Deep;
     return 20 * ((t256 + cus - 1) / cus) <= 23 * ((t128 + 2 * cus - 1) / (2 * cus)) ? kTile256 : kTile128;
 }
-// go.run<MB, WM, S, KB>() of a form
+// go.run<MB, WM, S, KB>() of a form of 64 rows or more, or of any
 template <class Go>
-inline hipError_t tile_dispatch(TileForm f, Go go) {
+inline hipError_t tile_dispatch64(TileForm f, Go go) {
     switch (f) {
-        case kTile32: return go.template run<1, 1, 3, 128>();
         case kTile64: return go.template run<1, 2, 3, 128>();
         case kTile128Deep: return go.template run<2, 2, 3, 128>();
         case kTile128: return go.template run<4, 1, 3, 64>();
         default: return go.template run<4, 2, 2, 128>();
     }
+}
+template <class Go>
+inline hipError_t tile_dispatch(TileForm f, Go go) {
+    return f == kTile32 ? go.template run<1, 1, 3, 128>() : tile_dispatch64(f, go);
 }
 
 // One wave's 32 x 64 block through 8 KB of LDS of its own: value(v, column)

@@ -875,7 +875,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     the call as quantize_int8 does, or int8 codes with their x_scale [...]
     (out_dtype then says what y is).  weight int8 [N, K] (read in place where
     its rows lie a multiple of 16 bytes apart that holds K, as a slice of wider
-    rows does; else from a copy of it), weight_scale float32 [N].  K <= 131072.  No gradient."""
+    rows does; else from a copy of it), weight_scale float32 [N].  Codes -127 ..
+    127, K <= 131072.  No gradient."""
     host = N.host()
     if host is not None and x_scale is None:
         y = host.linear_int8(x, weight, weight_scale, bias, out_dtype)
@@ -981,7 +982,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     target ignore_index have loss 0, no gradient and no share of the mean; a
     target that is no class makes its row's loss and the gradients NaN.
     Gradients of x, weight and bias, once differentiable; float32 sums in a
-    fixed order."""
+    fixed order.  Can be captured into a graph, backward too, where no eager
+    graph of the same leaves is alive."""
     host = N.host()
     if host is not None:
         loss = host.linear_cross_entropy(x, weight, target, bias, ignore_index, label_smoothing, N.REDUCTIONS.get(reduction))
@@ -1014,9 +1016,14 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         zero = x.float().sum() + 0.0 * weight[0, 0].float() + (0.0 if bias is None else 0.0 * bias[0].float())
         zero = torch.where(torch.ones_like(zero, dtype=torch.bool), zero.new_zeros(()), zero)
         return zero.expand(lead) if reduction == "none" else zero + math.nan if reduction == "mean" else zero
-    loss = _LinearCrossEntropy.apply(x2, _aligned_rows(weight), None if bias is None else bias.contiguous(),
-                                     target.reshape(-1).contiguous(), int(ignore_index), float(label_smoothing),
-                                     reduction)
+    weight, target = _aligned_rows(weight), target.reshape(-1).contiguous()
+    bias = None if bias is None else bias.contiguous()
+    loss = None
+    if host is not None:  # the operands as the native path takes them
+        with torch.autocast("cuda", enabled=False):
+            loss = host.linear_cross_entropy(x2, weight, target, bias, ignore_index, label_smoothing, N.REDUCTIONS[reduction])
+    if loss is None:
+        loss = _LinearCrossEntropy.apply(x2, weight, bias, target, int(ignore_index), float(label_smoothing), reduction)
     return loss.reshape(lead) if reduction == "none" else loss
 
 
@@ -1037,7 +1044,8 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, step: torch.Tensor, *, lr=1e-3, 
     a number, or a float32 device tensor that is read when the step runs.
     grad_scale, found_inf: float32 device scalars, as torch.amp.GradScaler
     passes them: gradients are divided by the one, a nonzero other leaves
-    parameters, states and step as they are.  The tensors must not overlap."""
+    parameters, states and step as they are.  Parameters or states that overlap
+    are refused."""
     params, grads, ms, vs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     n = len(params)
     small = exp_avg_scales is not None
@@ -1084,9 +1092,10 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, step: torch.Tensor, *, lr=1e-3, 
                     raise ValueError(f"tensor {i}: scales must be contiguous float32, one per {STATE_BLOCK} elements")
             a, b = sm[i].data_ptr(), sv[i].data_ptr()
         flat += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), a, b, size)
-    seen = [q for i in range(n) if flat[7 * i + 6] for q in (flat[7 * i], flat[7 * i + 2], flat[7 * i + 3])]
-    if len(set(seen)) != len(seen):
-        raise ValueError("adamw: a parameter or state is there twice")
+    seen = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                  for i in range(n) for t in (params[i], ms[i], vs[i]) if t.numel())
+    if any(b[0] < a[1] for a, b in zip(seen, seen[1:])):
+        raise ValueError("adamw: a parameter or state is there twice, or two overlap")
     hyper = N.AdamWHyper(0.0 if lr_dev is not None else float(lr), float(betas[0]), float(betas[1]), float(eps),
                          float(weight_decay))
     work = torch.empty(8, dtype=torch.float32, device=device)
@@ -1096,7 +1105,7 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, step: torch.Tensor, *, lr=1e-3, 
             table, n, code, 8 if small else 32, ctypes.byref(hyper), step.data_ptr(), N.ptr(lr_dev), N.ptr(grad_scale),
             N.ptr(found_inf), work.data_ptr(), N.stream_of(step)))
     # written behind torch's back: packed layers tell a changed weight by its version
-    torch.autograd.graph.increment_version(params + ms + vs + sm + sv + [step])
+    torch.autograd.graph.increment_version([t for t in params + ms + vs + sm + sv + [step] if not t.is_inference()])
 
 
 def adamw_state_values(codes, scales) -> list[torch.Tensor]:

@@ -82,7 +82,8 @@ class AdamW(torch.optim.Optimizer):
     element instead of 8.  Parameters on the device, float32, fp16 or bf16
     (moments and update in float32).  lr may be a float32 device tensor of one
     element.  The steps are counted on the device, so step() can be captured
-    into a graph once the states exist; torch.amp.GradScaler's scale and its
+    into a graph once the states exist, for the parameters that the eager step
+    before it took; torch.amp.GradScaler's scale and its
     skipped steps are taken on the device too.  state_dict() and
     load_state_dict() keep the states' types."""
 
@@ -100,9 +101,18 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"betas must be within 0 .. 1, got {betas}")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
 
-    def _new_state(self, p: torch.Tensor, bits: int, steps: dict) -> dict:
-        # parameters that start together share one count (and so a launch)
-        state = {"step": steps.setdefault((p.device, "new"), torch.zeros(1, dtype=torch.float32, device=p.device))}
+    def add_param_group(self, param_group) -> None:
+        if param_group.get("state_bits", 8) not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {param_group['state_bits']}")
+        super().add_param_group(param_group)
+
+    def _new_state(self, p: torch.Tensor, bits: int, call, steps: dict) -> dict:
+        # parameters of one call that start together share one count (and so a launch)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: the states must exist before a step is captured (take one eagerly)")
+        if call not in steps:
+            steps[call] = torch.zeros(1, dtype=torch.float32, device=p.device)
+        state = {"step": steps[call]}
         if bits == 32:
             state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
             state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
@@ -125,9 +135,10 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         grad_scale, found_inf = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
-        # all parameters that share a count, and those of them that step now
-        sharing, stepping, fresh = defaultdict(int), defaultdict(list), {}
-        for group in self.param_groups:
+        # calls: parameters that step now, of one group, type and count; users:
+        # all parameters of a count
+        calls, users, fresh = defaultdict(list), defaultdict(int), {}
+        for k, group in enumerate(self.param_groups):
             for p in group["params"]:
                 if p.grad is not None:
                     if p.grad.is_sparse:
@@ -135,29 +146,20 @@ class AdamW(torch.optim.Optimizer):
                     if not p.is_cuda:
                         raise ValueError("AdamW takes device parameters only")
                     if not self.state[p]:
-                        self.state[p] = self._new_state(p, group["state_bits"], fresh)
-                    stepping[id(self.state[p]["step"])].append(p)
+                        self.state[p] = self._new_state(p, group["state_bits"], (k, p.dtype, p.device), fresh)
+                    calls[k, p.dtype, id(self.state[p]["step"])].append(p)
                 if p in self.state and self.state[p]:
-                    sharing[id(self.state[p]["step"])] += 1
-        for key, params in stepping.items():
-            if len(params) < sharing[key]:  # the others do not step: a count of their own for these
-                count = self.state[params[0]]["step"].clone()
+                    users[id(self.state[p]["step"])] += 1
+        for (k, _, count), params in calls.items():
+            step = self.state[params[0]]["step"]
+            if len(params) < users[count]:  # a count belongs to one call: these take a copy
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("AdamW: a captured step takes the parameters that the step before it took")
+                users[count] -= len(params)
+                step = step.clone()
                 for p in params:
-                    self.state[p]["step"] = count
-        for group in self.param_groups:
-            calls = defaultdict(list)
-            for p in group["params"]:
-                if p.grad is not None:
-                    calls[(id(self.state[p]["step"]), p.dtype)].append(p)
-            for params in calls.values():
-                step = self.state[params[0]]["step"]
-                # a count belongs to one call: another group's or type's takes a copy
-                if any(self.state[q]["step"] is step for g in self.param_groups for q in g["params"]
-                       if q in self.state and self.state[q] and (g is not group or q.dtype != params[0].dtype)):
-                    step = step.clone()
-                    for p in params:
-                        self.state[p]["step"] = step
-                self._launch(ops, params, step, group, grad_scale, found_inf)
+                    self.state[p]["step"] = step
+            self._launch(ops, params, step, self.param_groups[k], grad_scale, found_inf)
         return loss
 
     def _launch(self, ops, params, step, group, grad_scale, found_inf):
@@ -191,19 +193,29 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As torch's, but the states keep their types (codes stay codes,
-        moments float32), and parameters of one count share it again."""
+        moments float32), and parameters of one group, type and count share it
+        again.  Takes what torch.optim.AdamW saved, states of 32 bits, but for
+        its amsgrad and maximize."""
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("AdamW has neither amsgrad nor maximize")
         super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            group.setdefault("state_bits", 32)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
+        params = [(k, p) for k, g in enumerate(self.param_groups) for p in g["params"]]
         counts = {}
-        for i, p in zip(saved, params):
+        for i, (k, p) in zip(saved, params):
             source = state_dict["state"].get(i)
             if not source:
                 continue
             for name, value in source.items():
                 if name == "step":
                     at = float(value)
-                    value = counts.setdefault((p.device, at), torch.full((1,), at, dtype=torch.float32, device=p.device))
+                    call = (k, p.dtype, p.device, at)
+                    if call not in counts:
+                        counts[call] = torch.full((1,), at, dtype=torch.float32, device=p.device)
+                    value = counts[call]
                 elif isinstance(value, torch.Tensor):
                     moved = value.to(p.device)
                     value = torch.empty_strided(p.shape, p.stride(), dtype=value.dtype, device=p.device).copy_(moved) \

@@ -350,3 +350,33 @@ def test_refusals():
     with pytest.raises(ValueError):
         ops.adamw_state_values([step], [step])
     assert ops.adamw_state_values([], []) == []
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_overlapping_tensors_are_refused(bits):
+    from quant_models import ops
+
+    made = _tensors(torch.float32, bits, 1, [(8,), (9,)])
+    wide = torch.zeros(16, device=DEV)
+    step = torch.zeros(1, device=DEV)
+    for k in ("params", "exp_avgs"):
+        t = {n: list(v) for n, v in made.items()}
+        wide_k = wide.to(t[k][0].dtype)
+        t[k] = [wide_k[:8], wide_k[7:]]
+        with pytest.raises(ValueError, match="overlap"):
+            ops.adamw(step=step, **t)
+        t[k] = [wide_k[:8], wide_k[8:][:9].new_zeros(9)]
+        ops.adamw(step=step, **t)
+
+
+@pytest.mark.gpu
+def test_states_made_in_inference_mode():
+    from quant_models import ops
+
+    a, b = (_tensors(torch.float32, 32, 2, [(8,), (300,)]) for _ in range(2))
+    with torch.inference_mode():
+        a["exp_avgs"] = [t.clone() for t in a["exp_avgs"]]
+    for t in (a, b):
+        ops.adamw(step=torch.zeros(1, device=DEV), **t)
+    assert all(torch.equal(p, q) for p, q in zip(a["params"] + a["exp_avgs"], b["params"] + b["exp_avgs"]))

@@ -209,3 +209,16 @@ def test_linear_int8_refusals():
         ops.linear_int8(x.requires_grad_(), w, s)
     with pytest.raises(RuntimeError, match="131072"):
         ops.linear_int8(torch.zeros(1, 131088, device=DEV), torch.zeros(1, 131088, dtype=torch.int8, device=DEV), s[:1])
+
+
+@pytest.mark.gpu
+def test_codes_of_more_rows_than_a_launch_has_waves():
+    """2^24 and a few rows: the waves take more than one each."""
+    from quant_models import ops
+
+    rows = (1 << 24) + 5
+    x = torch.randn(rows, 8, device=DEV, generator=_gen(9), dtype=torch.float16)
+    codes, scale = ops.quantize_int8(x)
+    for part in (slice(0, 300), slice(rows - 300, rows)):
+        c, s = ops.quantize_int8(x[part].contiguous())
+        assert torch.equal(codes[part], c) and torch.equal(scale[part], s)

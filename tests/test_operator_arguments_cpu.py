@@ -118,3 +118,12 @@ def test_adamw_argument_errors():
     assert values(c=None) == 1 and values(s=None) == 1 and values(o=None) == 1
     assert values(n=-1) == 2 and values(count=-1) == 2 and values(s=FAKE + 1) == 3
     assert L.rpfq_adamw_state_values(None, None, None, None, None, 1, None) == 1
+
+
+def test_linear_cross_entropy_takes_at_most_2_39_logits():
+    """A launch's threads, two a row and 256 classes, are counted in 32 bits."""
+    L, N = lib()
+    for backward in (0, 1):
+        size = lambda m, v: L.rpfq_linear_cross_entropy_workspace_bytes(ctypes.byref(_ce(N, M=m, V=v)), backward)  # noqa: E731
+        assert size(1 << 22, (1 << 17) - 256) > 0 and size(1 << 22, 1 << 17) == 0 == size(1 << 18, 1 << 22)
+        assert b"2^39" in L.rpfq_last_error()

@@ -390,3 +390,123 @@ def test_captured_training_step():
         want = step2()
         torch.cuda.synchronize()
         assert torch.equal(got, want) and torch.equal(w1, w2) and torch.equal(b1, b2)
+
+
+def test_optimizer_groups_and_foreign_states_on_the_host():
+    import quant_models as qm
+
+    p, q = nn.Parameter(torch.zeros(4)), nn.Parameter(torch.zeros(4))
+    opt = qm.AdamW([p])
+    with pytest.raises(ValueError, match="state_bits"):
+        opt.add_param_group({"params": [q], "state_bits": 4})
+    for kw in ({"amsgrad": True}, {"maximize": True}):
+        with pytest.raises(ValueError, match="amsgrad"):
+            opt.load_state_dict(torch.optim.AdamW([p], **kw).state_dict())
+
+
+@pytest.mark.gpu
+def test_optimizer_continues_a_torch_run():
+    """States that torch.optim.AdamW saved after two steps, then two steps on
+    either side (bounds as in test_optimizer_follows_torch)."""
+    import quant_models as qm
+
+    a, b, g = _pair(32)
+    theirs = torch.optim.AdamW(b, lr=1e-3)
+    grads = [[torch.randn(p.shape, device=DEV, generator=g) for p in a] for _ in range(4)]
+
+    def go(params, opt, gs):
+        for grad in gs:
+            for p, x in zip(params, grad):
+                p.grad = x.clone()
+            opt.step()
+
+    go(b, theirs, grads[:2])
+    mine = qm.AdamW(a, lr=5.0, state_bits=8)
+    mine.load_state_dict(theirs.state_dict())
+    with torch.no_grad():
+        for p, q in zip(a, b):
+            p.copy_(q)
+    go(a, mine, grads[2:])
+    go(b, theirs, grads[2:])
+    for p, q in zip(a, b):
+        assert float((p - q).abs().max()) <= 2 * 8 * 2.0 ** -24 * (float(q.abs().max()) + 1e-3)
+        assert float(mine.state[p]["step"]) == 4 and mine.state[p]["exp_avg"].dtype == torch.float32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_step_after_loading_counts_on(bits):
+    """Two groups whose counts are equal when they are loaded: each counts for
+    itself from then on, so that nothing of a captured step starts over."""
+    import quant_models as qm
+
+    a, b, g = _pair(bits)
+    groups = lambda p: [{"params": p[:2], "lr": 3e-3}, {"params": p[2:]}]  # noqa: E731
+    first = qm.AdamW(groups(a), state_bits=bits)
+    for p, q in zip(a, b):
+        p.grad = torch.randn(p.shape, device=DEV, generator=g)
+        q.grad = torch.empty_like(q).copy_(p.grad)
+    first.step()
+    saved = copy.deepcopy(first.state_dict())
+    with torch.no_grad():
+        for p, q in zip(a, b):
+            q.copy_(p)
+    again = qm.AdamW(groups(b), state_bits=bits)
+    again.load_state_dict(saved)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again.step()
+    for _ in range(3):
+        graph.replay()
+        first.step()
+        torch.cuda.synchronize()
+        for p, q in zip(a, b):
+            assert torch.equal(p, q) and float(first.state[p]["step"]) == float(again.state[q]["step"])
+
+
+@pytest.mark.gpu
+def test_captured_steps_that_would_start_over_are_refused():
+    import quant_models as qm
+
+    a, _, g = _pair(32)
+    for p in a:
+        p.grad = torch.randn(p.shape, device=DEV, generator=g)
+    opt = qm.AdamW(a)
+    before = [p.detach().clone() for p in a]
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="states must exist"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    opt.state.clear()
+    opt.step()
+    assert all(not torch.equal(p, q) for p, q in zip(a, before))
+    a[0].grad = None
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="the step before"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    opt.step()
+    opt.step()  # the four that step have a count of their own now
+    assert [float(opt.state[p]["step"]) for p in a] == [1.0, 3.0, 3.0, 3.0, 3.0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(8,), (2, 4)])
+def test_captured_backward_beside_an_eager_graph_is_refused(shape):
+    """The eager graph has bound the leaves to the default stream."""
+    from quant_models import ops
+
+    x = torch.randn(*shape, 16, device=DEV)
+    w = nn.Parameter(torch.randn(40, 16, device=DEV))
+    t = torch.randint(0, 40, shape, device=DEV)
+    alive = ops.linear_cross_entropy(x, w, t)
+    ops.linear_cross_entropy(x, w, t).backward()  # eagerly there is nothing against it
+    w.grad.zero_()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(graph):
+            ops.linear_cross_entropy(x, w, t).backward()
+    alive.backward()
+    assert float(w.grad.abs().max()) > 0
