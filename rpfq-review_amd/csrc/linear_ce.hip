@@ -124,6 +124,12 @@ __device__ __forceinline__ void ce_stage_bias(const CeArgs& a, int64_t n0, float
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
+// Bound by the products; the exponentials (16 clocks a wave and value, and as
+// much again for maximum and sum) are 3 us of a 256 x 256 tile's 27 at D = 768.
+// 8,192 x 65,536 x 768 bf16 845 us, 975 TFLOP/s (a library product that writes its
+// logits: 1,031, without the softmax); 500 x 131,072 x 1,024 129 us; 2,048 x 20,000
+// x 1,024 fp16 101 us.  128-row tiles, two workgroups a CU, whose exponentials
+// overlap the other's products: 910 us.
 template <int MB, int WM, int S, int KB, class Mma>
 __global__ void __launch_bounds__(256 * WM, 2) ce_stats_kernel(CeArgs a) {
     extern __shared__ __align__(16) char smem[];
@@ -260,26 +266,41 @@ __global__ void __launch_bounds__(1024) ce_reduce_kernel(CeJoin a) {
     ce_reduce(a, s, n);
 }
 
-// lse and loss of a row from its tiles: 16 threads a row, in a fixed order.
+// lse and loss of a row from its tiles: 16 threads a row, in a fixed order
+// (8,192 rows of 256 tiles 10 us; 500 of 512, in 8 workgroups, 13, and 18 with a
+// tile's read at a time).
 // ALL: one workgroup takes all rows and reduces them.
 template <bool ALL>
 __global__ void __launch_bounds__(1024) ce_join_kernel(CeJoin a) {
     const int c = threadIdx.x & 63, q = threadIdx.x >> 6;  // row, one of 16 parts of the tiles
     __shared__ float sm[3][64][17];
+    constexpr int AHEAD = 8;  // tiles on their way at once
     double total = 0.0;
     int count = 0;
     for (int64_t m0 = ALL ? 0 : (int64_t)blockIdx.x * 64; m0 < (ALL ? a.M : (int64_t)blockIdx.x * 64 + 64); m0 += 64) {
         const int64_t m = m0 + c;
         float mx = -__builtin_inff(), sum = 0.0f, zs = 0.0f;
         if (m < a.M)
-            for (int t = q; t < a.tiles; t += 16) {
-                const float2 p = a.part[(int64_t)t * a.M + m];
-                const float n = fmaxf(mx, p.x), base = n == -__builtin_inff() ? 0.0f : n;
-                // a tile of -inf has sum 0, one with NaN has sum NaN whatever its maximum
-                const float add = p.y == 0.0f || p.y != p.y ? p.y : p.y * __builtin_amdgcn_exp2f(ce_gap(p.x, base));
-                sum = (sum == 0.0f ? 0.0f : sum * __builtin_amdgcn_exp2f(ce_gap(mx, base))) + add;
-                mx = n;
-                if (a.zsum) zs += a.zsum[(int64_t)t * a.M + m];
+            for (int t = q; t < a.tiles; t += 16 * AHEAD) {
+                float2 p[AHEAD];
+                float z[AHEAD];
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int64_t at = (int64_t)(t + 16 * k) * a.M + m;
+                    const bool there = t + 16 * k < a.tiles;
+                    p[k] = there ? a.part[at] : make_float2(0.0f, 0.0f);
+                    z[k] = there && a.zsum ? a.zsum[at] : 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    if (t + 16 * k >= a.tiles) break;
+                    const float n = fmaxf(mx, p[k].x), base = n == -__builtin_inff() ? 0.0f : n, y = p[k].y;
+                    // a tile of -inf has sum 0, one with NaN has sum NaN whatever its maximum
+                    const float add = y == 0.0f || y != y ? y : y * __builtin_amdgcn_exp2f(ce_gap(p[k].x, base));
+                    sum = (sum == 0.0f ? 0.0f : sum * __builtin_amdgcn_exp2f(ce_gap(mx, base))) + add;
+                    mx = n;
+                    zs += z[k];
+                }
             }
         sm[0][c][q] = mx;
         sm[1][c][q] = sum;
@@ -447,6 +468,9 @@ __device__ __forceinline__ float ce_lane_sums(float (&v)[32], int lane) {
 }
 
 // dz of one piece of the classes.  DT: the type of dz (float32: three planes).
+// The logits' product again and M V elements written: 8,192 x 65,536 x 768 bf16
+// 950 us, 870 TFLOP/s and 1.1 TB/s of dz; 2,048 x 20,000 x 1,024 fp16 114 us.  Stores
+// past the caches were slower where a piece of dz stays in them.
 template <int MB, int WM, int S, int KB, class Mma, int DT>
 __global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
     extern __shared__ __align__(16) char smem[];
@@ -638,7 +662,9 @@ __device__ __forceinline__ void ce_grad_unit(const CeGrad& a, int bid, char* sme
 
 // Both products of a piece's dz in one launch: dx (dz in K layout, w in T) and dw
 // (dz and x in T), the longer units first and the others into their last round
-// (2,048 x 20,000 x 1,024 fp16: 1.2 and 1.0 rounds of the chip apart, 227 us).
+// (2,048 x 20,000 x 1,024 fp16: 1.2 and 1.0 rounds of the chip; 227 us in two
+// launches, 200 in one).  8,192 x 65,536 x 768 bf16 1,490 us, 1,107 TFLOP/s (library
+// products of the same shapes: 1,700 us).
 struct CeGrads {
     CeGrad g[2];   // dx, dw; splits = 0: not wanted
     int units[2];
@@ -653,7 +679,8 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_grads_kernel(CeGrads a) {
     else ce_grad_unit<MB, WM, S, KB, true, Mma, DT>(a.g[1], at, smem);
 }
 
-// out = factor * sum of the partials, in their order.
+// out = factor * sum of the partials, in their order.  HBM bound: 8 x 8,192 x 768
+// float32 15.5 us with the factor and rounding.
 template <int DT>
 __global__ void __launch_bounds__(256) ce_sum_kernel(const float* part, int parts, int64_t stride, int64_t rows, int64_t N,
                                                      int64_t ldp, CeFactor factor, void* out, int vec) {

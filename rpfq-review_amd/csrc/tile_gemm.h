@@ -173,12 +173,16 @@ struct TileSide {
 // (w % 4) .. + 63 of rows 32 MB (w / 4) .. + 32 MB - 1, acc[j][i] the 32 x 32
 // block of its columns 32 j and rows 32 i: lane (r, g) holds row r and columns
 // acc_row(v, g).  Both operands go global -> LDS by DMA, in S stages of KB bytes
-// of k, S - 1 steps ahead.  The forms that are used (bf16, normal operands;
-// K = 768 / 8192, K layouts):
-//   256 x 256, KB 128, S 2, one workgroup a CU: 1,215 / 1,294 TFLOP/s.  Half the
-//     LDS fill per product of a 128-row tile, which is bound by it (48 of 64
-//     bytes a clock from the vector cache at full matrix rate);
-//   128 x 256, KB 64, S 3, two a CU: 1,040 / 1,010;
+// of k, S - 1 steps ahead (S = 2: two).  The forms that are used (bf16, normal
+// operands, K layouts, the products alone; 8192 x 65536 x 768 / 8192^3):
+//   256 x 256, KB 128, S 2, one workgroup a CU: 1,213 / 1,290 TFLOP/s, and
+//     1,090 / 1,180 where a step begins with its first reads.  Half the LDS
+//     fill per product of a 128-row tile, which is bound by it (48 of 64 bytes
+//     a clock from the vector cache at full matrix rate).  Four waves of 128 x
+//     128 instead of eight of 128 x 64 read less LDS, but a wave alone on its
+//     SIMD waits more: 1,146 / 1,227;
+//   128 x 256, KB 64, S 3, two a CU: 1,058 / 1,021 (steps overlapped 1,054 /
+//     1,010);
 //   64 x 256 and 128 x 256 of eight waves, KB 128, S 3, one a CU: launches of
 //     fewer tiles than CUs (333 x 10,007 x 2,496: 27 and 34 us; four waves with
 //     S 6 of 64 bytes 40 and 43).
@@ -224,48 +228,85 @@ struct TileGemm {
         uint32_t ra[SUB], ca[SUB];
 #pragma unroll
         for (int u = 0; u < SUB; ++u) ra[u] = R::at(lane, u), ca[u] = C::at(lane, u);
+        uint4 cf[2][2], rf[2][MB];  // of a substep and the next
+        auto read = [&](int st, int u, int p) {
+            const uint32_t rst = lds + st * STAGE, cst = rst + R::BYTES;
 #pragma unroll
-        for (int i = 0; i < S - 1; ++i)
-            if (s0 + i < s1) issue(i);
-        meanwhile();
-        auto step = [&](int s, int st) {
-            // the steps behind s may still be on their way
-            if (s + S - 2 < s1)
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * LOADS) : "memory");
-            else
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            for (int j = 0; j < 2; ++j) cf[p][j] = C::frag(cst, ca, 2 * wc + j, u, lane);
+#pragma unroll
+            for (int i = 0; i < MB; ++i) rf[p][i] = R::frag(rst, ra, MB * wr + i, u, lane);
+        };
+        auto products = [&](int p) {
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[j][i] = Mma::mma(cf[p][j], rf[p][i], acc[j][i]);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        // waits for the DMA of all but the last `behind` steps, and for every wave's
+        auto landed = [&](auto behind) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(behind)::value * LOADS) : "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if (s + S - 1 < s1) issue((st + S - 1) % S);  // read a step ago, by every wave
-            const uint32_t rst = lds + st * STAGE, cst = rst + R::BYTES;
-            uint4 cf[2][2], rf[2][MB];  // of a substep and the next
-            auto read = [&](int u, int p) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) cf[p][j] = C::frag(cst, ca, 2 * wc + j, u, lane);
-#pragma unroll
-                for (int i = 0; i < MB; ++i) rf[p][i] = R::frag(rst, ra, MB * wr + i, u, lane);
-            };
-            read(0, 0);
-#pragma unroll
-            for (int u = 0; u < SUB; ++u) {
-                if (u + 1 < SUB) read(u + 1, (u + 1) & 1);
-#pragma unroll
-                for (int i = 0; i < MB; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[j][i] = Mma::mma(cf[u & 1][j], rf[u & 1][i], acc[j][i]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         };
-        int s = s0;
-        for (; s + S <= s1; s += S)
+        using std::integral_constant;
+        if constexpr (S == 2) {
+            // The steps overlap: while a step's last products run, the next one's
+            // first operands are read and the stage is filled again.
+            if (s0 == s1) return;
+            issue(0);
+            if (s0 + 1 < s1) issue(1);
+            meanwhile();
+            if (s0 + 1 < s1) landed(integral_constant<int, 1>());
+            else landed(integral_constant<int, 0>());
+            read(0, 0, 0);
+            auto step = [&](int s, int st) {
 #pragma unroll
-            for (int i = 0; i < S; ++i) step(s + i, i);
+                for (int u = 0; u + 1 < SUB; ++u) {
+                    read(st, u + 1, (u + 1) & 1);
+                    products(u & 1);
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                landed(integral_constant<int, 0>());
+                if (s + 1 < s1) read(st ^ 1, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (s + 2 < s1) issue(st);
+                products((SUB - 1) & 1);
+            };
+            int s = s0;
+            for (; s + 2 <= s1; s += 2) {
+                step(s, 0);
+                step(s + 1, 1);
+            }
+            if (s < s1) step(s, 0);
+        } else {
 #pragma unroll
-        for (int i = 0; i < S - 1; ++i)
-            if (s + i < s1) step(s + i, i);
-        __builtin_amdgcn_s_barrier();  // the stages are free for the epilogue
-        asm volatile("" ::: "memory");
+            for (int i = 0; i < S - 1; ++i)
+                if (s0 + i < s1) issue(i);
+            meanwhile();
+            auto step = [&](int s, int st) {
+                // the steps behind s may still be on their way
+                if (s + S - 2 < s1) landed(integral_constant<int, S - 2>());
+                else landed(integral_constant<int, 0>());
+                if (s + S - 1 < s1) issue((st + S - 1) % S);  // read a step ago, by every wave
+                read(st, 0, 0);
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) {
+                    if (u + 1 < SUB) read(st, u + 1, (u + 1) & 1);
+                    products(u & 1);
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            };
+            int s = s0;
+            for (; s + S <= s1; s += S)
+#pragma unroll
+                for (int i = 0; i < S; ++i) step(s + i, i);
+#pragma unroll
+            for (int i = 0; i < S - 1; ++i)
+                if (s + i < s1) step(s + i, i);
+            __builtin_amdgcn_s_barrier();  // the stages are free for the epilogue
+            asm volatile("" ::: "memory");
+        }
     }
 };
 
