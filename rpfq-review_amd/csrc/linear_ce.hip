@@ -129,7 +129,7 @@ __device__ __forceinline__ void ce_stage_bias(const CeArgs& a, int64_t n0, float
 // 8,192 x 65,536 x 768 bf16 845 us, 975 TFLOP/s (a library product that writes its
 // logits: 1,031, without the softmax); 500 x 131,072 x 1,024 129 us; 2,048 x 20,000
 // x 1,024 fp16 101 us.  128-row tiles, two workgroups a CU, whose exponentials
-// overlap the other's products: 910 us.
+// overlap the other's products: 930 us.
 template <int MB, int WM, int S, int KB, class Mma>
 __global__ void __launch_bounds__(256 * WM, 2) ce_stats_kernel(CeArgs a) {
     extern __shared__ __align__(16) char smem[];
