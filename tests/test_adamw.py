@@ -380,3 +380,28 @@ def test_states_made_in_inference_mode():
     for t in (a, b):
         ops.adamw(step=torch.zeros(1, device=DEV), **t)
     assert all(torch.equal(p, q) for p, q in zip(a["params"] + a["exp_avgs"], b["params"] + b["exp_avgs"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_than_2_31_elements(bits):
+    """The end and the middle of a tensor are the bits of a step on those alone."""
+    from quant_models import ops
+
+    n, part = (1 << 31) + (1 << 20), 4096 * 25
+    g = _gen(3)
+    t = {"params": [torch.randn(n, device=DEV, generator=g, dtype=torch.bfloat16)],
+         "grads": [torch.randn(n, device=DEV, generator=g, dtype=torch.bfloat16)]}
+    kinds = (torch.float32, torch.float32) if bits == 32 else (torch.int8, torch.uint8)
+    t["exp_avgs"], t["exp_avg_sqs"] = ([torch.zeros(n, device=DEV, dtype=k)] for k in kinds)
+    if bits == 8:
+        t["exp_avg_scales"], t["exp_avg_sq_scales"] = ([torch.zeros(n // 256, device=DEV)] for _ in range(2))
+    at = (0, 1 << 30, (1 << 31) - 4096, n - part)
+    cut = lambda v, a: v[a // (n // v.numel()):(a + part) // (n // v.numel())]  # noqa: E731
+    alone = [{k: [cut(v[0], a).clone()] for k, v in t.items()} for a in at]
+    for call in [t] + alone:
+        for _ in range(2):
+            ops.adamw(step=torch.zeros(1, device=DEV), lr=0.1, **call)
+    for a, call in zip(at, alone):
+        for k, v in call.items():
+            assert torch.equal(cut(t[k][0], a), v[0]), k

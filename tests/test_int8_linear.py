@@ -222,3 +222,22 @@ def test_codes_of_more_rows_than_a_launch_has_waves():
     for part in (slice(0, 300), slice(rows - 300, rows)):
         c, s = ops.quantize_int8(x[part].contiguous())
         assert torch.equal(codes[part], c) and torch.equal(scale[part], s)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """An output and an input of 4.6 GB: rows in the middle and at the end are
+    the bits of calls on those rows alone."""
+    from quant_models import ops
+
+    rows, n = 70001, 32768
+    x = torch.randn(rows, 64, device=DEV, generator=_gen(1), dtype=torch.float16)
+    w, sw = ops.quantize_int8(torch.randn(n, 64, device=DEV, generator=_gen(2)))
+    parts = (slice(0, 40), slice(32700, 33000), slice(65400, 65700), slice(rows - 300, rows))
+    y = ops.linear_int8(x, w, sw)
+    for part in parts:
+        assert torch.equal(y[part], ops.linear_int8(x[part], w, sw))
+    codes, scale = ops.quantize_int8(y)
+    for part in parts:
+        c, s = ops.quantize_int8(y[part])
+        assert torch.equal(codes[part], c) and torch.equal(scale[part], s)

@@ -352,3 +352,34 @@ def test_no_rows_and_refusals():
     (g,) = torch.autograd.grad(ops.linear_cross_entropy(xs, w, t), [xs], create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_weights_of_more_than_4_gb():
+    """1.2 M classes of 2,048 fp16 features; the gradient of some of the first,
+    middle and last classes in 64 bits, times 2^12 to stay fp16 normals.  A
+    logit is off by le = (D + 2) 2^-24 sum |x| |w|, p by twice that of itself
+    and the exponentials' 2^-20 (1 + ln V + |lse|); dz is rounded to 2^-11."""
+    from quant_models import ops
+
+    m, v, d = 64, 1200000, 2048
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randn(m, d, device=DEV, generator=g, dtype=torch.float16).requires_grad_()
+    w = (torch.randn(v, d, device=DEV, generator=g, dtype=torch.float16) / math.sqrt(d)).requires_grad_()
+    t = torch.randint(0, v, (m,), device=DEV, generator=g)
+    t[:3] = torch.tensor([v - 1, v - 200, 0], device=DEV)
+    loss = ops.linear_cross_entropy(x, w, t, reduction="sum")
+    loss.backward(torch.tensor(4096.0, device=DEV))
+    xd = x.detach().double()
+    lse = torch.stack([torch.logsumexp(xd @ c.detach().double().t(), 1) for c in w.split(50000)], 1).logsumexp(1)
+    le = (d + 2) * 2.0 ** -24 * (xd.abs() @ w.detach()[:50000].abs().double().t()).max() * 1.5  # rows of w are alike
+    zt = (xd * w.detach()[t].double()).sum(1)
+    assert abs(float(loss.detach().double() - (lse - zt).sum())) <= m * float(2 * le + 2.0 ** -20 * (1 + math.log(v) + lse.max()))
+    for part in (slice(0, 300), slice(524200, 524500), slice(1048500, 1048800), slice(v - 300, v)):
+        c = torch.arange(v, device=DEV)[part]
+        p = torch.exp(xd @ w.detach()[part].double().t() - lse[:, None])
+        dz = p - (t[:, None] == c).double()
+        off = p * (2 * le + 2.0 ** -20 * (1 + math.log(v) + lse.max())) + 2.0 ** -11 * dz.abs() + 2.0 ** -40
+        want = 4096 * dz.t() @ xd
+        bound = 2.0 ** -11 * want.abs() + 4096 * (off + m * 2.0 ** -24 * dz.abs()).t() @ xd.abs() + 2.0 ** -25
+        assert bool(((w.grad[part].double() - want).abs() <= bound * (1 + 2.0 ** -10)).all()), part
