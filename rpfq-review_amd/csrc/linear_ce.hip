@@ -679,27 +679,42 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_grads_kernel(CeGrads a) {
     else ce_grad_unit<MB, WM, S, KB, true, Mma, DT>(a.g[1], at, smem);
 }
 
-// out = factor * sum of the partials, in their order.  HBM bound: 8 x 8,192 x 768
-// float32 15.5 us with the factor and rounding.
-template <int DT>
-__global__ void __launch_bounds__(256) ce_sum_kernel(const float* part, int parts, int64_t stride, int64_t rows, int64_t N,
-                                                     int64_t ldp, CeFactor factor, void* out, int vec) {
-    const float f = factor();
-    const int64_t per = ldp / 4, total = rows * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+// out = factor * sum of the partials, in their order: of dw, db and dx, those
+// that a piece leaves, in one launch.  HBM bound: 8 x 8,192 x 768 float32 15.5 us
+// with the factor and rounding.
+struct CeSum {
+    const float* part;
+    void* out;
+    int64_t stride, rows, N, ldp;  // of a partial; rows, columns and row length of the sum
+    int parts, dt, vec, blocks;
+};
+struct CeSums {
+    CeSum s[3];
+    CeFactor factor;
+};
+__global__ void __launch_bounds__(256) ce_sums_kernel(CeSums a) {
+    int k = 0, bid = blockIdx.x;
+    while (bid >= a.s[k].blocks) bid -= a.s[k++].blocks;
+    const CeSum j = a.s[k];
+    const float f = a.factor();
+    const int64_t per = j.ldp / 4, total = j.rows * per;
+    for (int64_t i = (int64_t)bid * 256 + threadIdx.x; i < total; i += (int64_t)j.blocks * 256) {
         const int64_t m = i / per, n = (i - m * per) * 4;
-        const f32x4* p = reinterpret_cast<const f32x4*>(part + m * ldp + n);
+        const f32x4* p = reinterpret_cast<const f32x4*>(j.part + m * j.ldp + n);
         f32x4 v = p[0];
         int s = 1;
-        for (; s + 8 <= parts; s += 8) {  // eight loads on their way, added in order
+        for (; s + 8 <= j.parts; s += 8) {  // eight loads on their way, added in order
             f32x4 w[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = p[(s + k) * (stride / 4)];
+            for (int t = 0; t < 8; ++t) w[t] = p[(s + t) * (j.stride / 4)];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v += w[k];
+            for (int t = 0; t < 8; ++t) v += w[t];
         }
-        for (; s < parts; ++s) v += p[s * (stride / 4)];
-        tile_store4<DT>(out, m * N, n, N, vec, v * f);
+        for (; s < j.parts; ++s) v += p[s * (j.stride / 4)];
+        v *= f;
+        if (j.dt == RPFQ_F32) tile_store4<RPFQ_F32>(j.out, m * j.N, n, j.N, j.vec, v);
+        else if (j.dt == RPFQ_F16) tile_store4<RPFQ_F16>(j.out, m * j.N, n, j.N, j.vec, v);
+        else tile_store4<RPFQ_BF16>(j.out, m * j.N, n, j.N, j.vec, v);
     }
 }
 
@@ -923,22 +938,10 @@ static hipError_t ce_grads(int dt, bool direct, TileForm form, CeGrads& g, hipSt
                              : tile_dispatch64(form, GradGo<MmaBf16, RPFQ_F32>{g, s});
 }
 
-static hipError_t ce_sum(int dt, const float* part, int parts, int64_t stride, int64_t rows, int64_t N, int64_t ldp,
-                         CeFactor factor, void* out, hipStream_t s) {
+static CeSum ce_sum(int dt, const float* part, int parts, int64_t stride, int64_t rows, int64_t N, int64_t ldp, void* out) {
     const int es = dt == RPFQ_F32 ? 4 : 2;
-    const int vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * es) == 0;
-    const dim3 grid(blocks_of((rows * (ldp / 4) + 255) / 256));
-    switch (dt) {
-        case RPFQ_F32:
-            hipLaunchKernelGGL(ce_sum_kernel<RPFQ_F32>, grid, dim3(256), 0, s, part, parts, stride, rows, N, ldp, factor, out, vec);
-            break;
-        case RPFQ_F16:
-            hipLaunchKernelGGL(ce_sum_kernel<RPFQ_F16>, grid, dim3(256), 0, s, part, parts, stride, rows, N, ldp, factor, out, vec);
-            break;
-        default:
-            hipLaunchKernelGGL(ce_sum_kernel<RPFQ_BF16>, grid, dim3(256), 0, s, part, parts, stride, rows, N, ldp, factor, out, vec);
-    }
-    return hipGetLastError();
+    return {part, out, stride, rows, N, ldp, parts, dt, N % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * es) == 0,
+            (int)blocks_of((rows * (ldp / 4) + 255) / 256)};
 }
 
 hipError_t launch_linear_ce(const CeCall& c, float* loss, float* stat, float* coef, void* work, hipStream_t s) {
@@ -1043,17 +1046,22 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         dw.out = gw ? reinterpret_cast<char*>(gw) + v0 * c.D * es : nullptr;
         dw.vec = c.D % 4 == 0 && reinterpret_cast<uintptr_t>(dw.out) % (4 * es) == 0;
         if ((gx || gw) && (e = ce_grads(c.dtype, p.es == 4, p.grad.form, both, s)) != hipSuccess) return e;
-        if (gw && dw.part &&
-            (e = ce_sum(c.dtype, dw.part, dw.splits, n * p.ldp, n, c.D, p.ldp, factor, dw.out, s)) != hipSuccess)
-            return e;
-        if (gb) {  // db: the column sums of the row tiles, as one row each
-            const int bs = c.bias_dtype == RPFQ_F32 ? 4 : 2;
-            e = ce_sum(c.bias_dtype, a.colsum, col_rows, a.n8, 1, n, a.n8, factor,
-                       reinterpret_cast<char*>(gb) + v0 * bs, s);
-            if (e != hipSuccess) return e;
+        CeSums sums = {{}, factor};
+        int jobs = 0, blocks = 0;
+        auto add = [&](const CeSum& j) {
+            sums.s[jobs++] = j;
+            blocks += j.blocks;
+        };
+        if (gw && dw.part) add(ce_sum(c.dtype, dw.part, dw.splits, n * p.ldp, n, c.D, p.ldp, dw.out));
+        if (gx && dxp && v0 + n == c.V) add(ce_sum(c.dtype, dxp, p.grad.dx, c.M * p.ldp, c.M, c.D, p.ldp, gx));
+        if (gb)  // the column sums of the row tiles, as one row each
+            add(ce_sum(c.bias_dtype, a.colsum, col_rows, a.n8, 1, n, a.n8,
+                       reinterpret_cast<char*>(gb) + v0 * (c.bias_dtype == RPFQ_F32 ? 4 : 2)));
+        if (jobs) {
+            hipLaunchKernelGGL(ce_sums_kernel, dim3((unsigned)blocks), dim3(256), 0, s, sums);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
         }
     }
-    if (gx && dxp) return ce_sum(c.dtype, dxp, p.grad.dx, c.M * p.ldp, c.M, c.D, p.ldp, factor, gx, s);
     return hipSuccess;
 }
 
