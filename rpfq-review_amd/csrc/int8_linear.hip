@@ -173,7 +173,7 @@ struct Int8Args {
 };
 
 // Bound by the matrix cores' step (tile_gemm.h) and, for a wide output of a small
-// K, by its stores: 50,432 x 1,024 -> 4,096 fp16, 250 to 290 us, 1.5 to 1.7 POP/s and
+// K, by its stores: 50,432 x 1,024 -> 4,096 fp16, 260 to 310 us, 1.4 to 1.6 POP/s and
 // 413 MB of y, which alone are 90 us at a copy's rate and hide behind nothing
 // in their own workgroup.  Workgroups that walk several tiles and load the next
 // one's first step during the stores measured the same (249 us against 253).
