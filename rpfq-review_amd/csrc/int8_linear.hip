@@ -120,14 +120,47 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(const void* x, int64_t M
     }
 }
 
-// Any K and alignment: one workgroup a row, read twice (the second time from L2;
-// 777 x 779 float32 3.8 us).
+// codes [rows, K] of any K and alignment -> rows of ldq bytes, zeros past K: a
+// wave a row, 16 bytes a lane.
+struct Int8Pad {
+    const int8_t* src;
+    int64_t ld, K;
+    int8_t* dst;
+    int64_t ldq, rows;
+    unsigned blocks;
+};
+__device__ __forceinline__ void int8_pad(const Int8Pad& a, unsigned block) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t n = (int64_t)block * 4 + (threadIdx.x >> 6); n < a.rows; n += (int64_t)a.blocks * 4)
+        for (int64_t k = 16 * lane; k < a.ldq; k += 1024) {
+            const int8_t* src = a.src + n * a.ld + k;
+            int8_t e[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+            if (k + 16 <= a.K) {
+                __builtin_memcpy(e, src, 16);
+            } else {
+#pragma unroll
+                for (int t = 0; t < 16; ++t)
+                    if (k + t < a.K) e[t] = src[t];
+            }
+            __builtin_memcpy(a.dst + n * a.ldq + k, e, 16);
+        }
+}
+__global__ void __launch_bounds__(256) int8_pad_kernel(Int8Pad a) { int8_pad(a, blockIdx.x); }
+
+// Any K and alignment: one workgroup a row, read twice (the second time from
+// L2).  The workgroups past `blocks` copy a weight whose rows do not lie as the
+// product reads them, in the same launch (777 and 333 rows of 515: 3.9 us, 6.6
+// in two).
 template <int DT>
 __global__ void __launch_bounds__(256) int8_rows_any_kernel(const void* x, int64_t M, int64_t K, int8_t* q, int64_t ldq,
-                                                           float* scale) {
+                                                           float* scale, unsigned blocks, Int8Pad pad) {
     __shared__ uint32_t sm[4];
+    if (blockIdx.x >= blocks) {
+        int8_pad(pad, blockIdx.x - blocks);
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
+    for (int64_t m = blockIdx.x; m < M; m += blocks) {
         uint32_t mx = 0;
         for (int64_t k = threadIdx.x; k < K; k += 256) mx = max(mx, __float_as_uint(load1<DT>(x, m * K + k)) & 0x7fffffffu);
 #pragma unroll
@@ -140,25 +173,6 @@ __global__ void __launch_bounds__(256) int8_rows_any_kernel(const void* x, int64
             q[m * ldq + k] = (int8_t)(k < K ? row.code(load1<DT>(x, m * K + k)) : 0);
         __syncthreads();
     }
-}
-
-// codes [rows, K] of any K and alignment -> rows of ldq bytes, zeros past K: a
-// wave a row, 16 bytes a lane.
-__global__ void __launch_bounds__(256) int8_pad_kernel(const int8_t* src, int64_t ld, int64_t K, int8_t* dst, int64_t ldq,
-                                                      int64_t rows) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (int64_t)gridDim.x * 4)
-        for (int64_t k = 16 * lane; k < ldq; k += 1024) {
-            int8_t e[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-            if (k + 16 <= K) {
-                __builtin_memcpy(e, src + n * ld + k, 16);
-            } else {
-#pragma unroll
-                for (int t = 0; t < 16; ++t)
-                    if (k + t < K) e[t] = src[n * ld + k + t];
-            }
-            __builtin_memcpy(dst + n * ldq + k, e, 16);
-        }
 }
 
 // ---------------------------------------------------------------------------
@@ -364,31 +378,53 @@ static hipError_t few_y(const Int8Few& a, int ydt, hipStream_t s) {
     }
 }
 
+static Int8Pad pad_of(const int8_t* src, int64_t ld, int64_t K, int64_t rows, int8_t* dst, int64_t ldq) {
+    const int64_t blocks = (rows + 3) / 4;
+    return {src, ld, K, dst, ldq, rows, (unsigned)(blocks < 16384 ? blocks : 16384)};
+}
+static hipError_t pad_codes(const Int8Pad& a, hipStream_t s) {
+    hipLaunchKernelGGL(int8_pad_kernel, dim3(a.blocks), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+// pad: a weight to be copied beside it, or blocks = 0
 template <int DT>
-static hipError_t quantize_dt(const void* x, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale, hipStream_t s) {
+static hipError_t quantize_dt(const void* x, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale, const Int8Pad& pad,
+                              hipStream_t s) {
     const bool vec = K % 8 == 0 && ldq % 8 == 0 && ldq <= 4096 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
                      reinterpret_cast<uintptr_t>(q) % 8 == 0;
+    if (!vec) {
+        const unsigned blocks = (unsigned)(M < 65536 ? M : 65536);
+        hipLaunchKernelGGL((int8_rows_any_kernel<DT>), dim3(blocks + pad.blocks), dim3(256), 0, s, x, M, K, q, ldq, scale, blocks,
+                           pad);
+        return hipGetLastError();
+    }
+    if (pad.blocks) {
+        const hipError_t e = pad_codes(pad, s);
+        if (e != hipSuccess) return e;
+    }
     // at most 2^22 workgroups: a launch's threads are counted in 32 bits
     const dim3 rows((unsigned)(M < (1LL << 24) ? (M + 3) / 4 : 1LL << 22));
 #define RPFQ_ROWS(NC) hipLaunchKernelGGL((int8_rows_kernel<DT, NC>), rows, dim3(256), 0, s, x, M, (int)K, q, ldq, scale)
-    if (vec && ldq <= 512) RPFQ_ROWS(1);
-    else if (vec && ldq <= 1024) RPFQ_ROWS(2);
-    else if (vec && ldq <= 2048) RPFQ_ROWS(4);
-    else if (vec) RPFQ_ROWS(8);
-    else
-        hipLaunchKernelGGL((int8_rows_any_kernel<DT>), dim3((unsigned)(M < 65536 ? M : 65536)), dim3(256), 0, s, x, M, K, q,
-                           ldq, scale);
+    if (ldq <= 512) RPFQ_ROWS(1);
+    else if (ldq <= 1024) RPFQ_ROWS(2);
+    else if (ldq <= 2048) RPFQ_ROWS(4);
+    else RPFQ_ROWS(8);
 #undef RPFQ_ROWS
     return hipGetLastError();
 }
 
+static hipError_t quantize(const void* x, int dt, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale,
+                           const Int8Pad& pad, hipStream_t s) {
+    switch (dt) {
+        case RPFQ_F32: return quantize_dt<RPFQ_F32>(x, M, K, q, ldq, scale, pad, s);
+        case RPFQ_F16: return quantize_dt<RPFQ_F16>(x, M, K, q, ldq, scale, pad, s);
+        default: return quantize_dt<RPFQ_BF16>(x, M, K, q, ldq, scale, pad, s);
+    }
+}
 hipError_t launch_quantize_int8(const void* x, int dt, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale,
                                 hipStream_t s) {
-    switch (dt) {
-        case RPFQ_F32: return quantize_dt<RPFQ_F32>(x, M, K, q, ldq, scale, s);
-        case RPFQ_F16: return quantize_dt<RPFQ_F16>(x, M, K, q, ldq, scale, s);
-        default: return quantize_dt<RPFQ_BF16>(x, M, K, q, ldq, scale, s);
-    }
+    return quantize(x, dt, M, K, q, ldq, scale, Int8Pad{}, s);
 }
 
 template <int YDT>
@@ -436,25 +472,20 @@ Int8Plan int8_plan(const void* x, int xdt, int64_t M, int64_t N, int64_t K, cons
     return p;
 }
 
-static hipError_t pad_codes(const int8_t* src, int64_t ld, int64_t K, int64_t rows, int8_t* dst, int64_t ldq, hipStream_t s) {
-    const int64_t blocks = (rows + 3) / 4;
-    hipLaunchKernelGGL(int8_pad_kernel, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, src, ld, K, dst, ldq,
-                       rows);
-    return hipGetLastError();
-}
-
 hipError_t launch_linear_int8(const void* x, int xdt, const float* sx, const int8_t* w, int64_t ldw, const float* sw,
                               const float* bias, int64_t M, int64_t N, int64_t K, void* y, int ydt, void* work,
                               hipStream_t s) {
     const Int8Plan p = int8_plan(x, xdt, M, N, K, w, ldw);
     char* wk = reinterpret_cast<char*>(work);
     hipError_t e;
+    Int8Pad pad = {};
     if (p.pad_w) {
         int8_t* q = reinterpret_cast<int8_t*>(wk + p.w_at);
-        e = pad_codes(w, ldw, K, N, q, p.ld, s);
-        if (e != hipSuccess) return e;
+        pad = pad_of(w, ldw, K, N, q, p.ld);
         w = q;
         ldw = p.ld;
+        const bool beside = p.copy_x && xdt >= 0;  // with the quantizer's launch
+        if (!beside && (e = pad_codes(pad, s)) != hipSuccess) return e;
     }
     if (p.few) {
         const Int8Few f = {x, w, sw, bias, y, ldw, N, (int)M, (int)K};
@@ -472,8 +503,8 @@ hipError_t launch_linear_int8(const void* x, int xdt, const float* sx, const int
         int8_t* q = reinterpret_cast<int8_t*>(wk + p.x_at);
         float* qs = reinterpret_cast<float*>(wk + p.sx_at);
         // codes that come unaligned are copied as an unaligned weight is
-        e = xdt >= 0 ? launch_quantize_int8(x, xdt, M, K, q, p.ld, qs, s)
-                     : pad_codes(reinterpret_cast<const int8_t*>(x), K, K, M, q, p.ld, s);
+        e = xdt >= 0 ? quantize(x, xdt, M, K, q, p.ld, qs, pad, s)
+                     : pad_codes(pad_of(reinterpret_cast<const int8_t*>(x), K, K, M, q, p.ld), s);
         if (e != hipSuccess) return e;
         a.x = {reinterpret_cast<const char*>(q), p.ld, 0, M};
         if (xdt >= 0) a.sx = qs;
