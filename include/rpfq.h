@@ -708,8 +708,9 @@ int rpfq_linear_cross_entropy(const rpfq_ce_desc* desc, const void* x, const voi
  * bias_dtype (each NULL if not wanted); grad_loss: float32 [1], or [M] with
  * RPFQ_REDUCE_NONE; stat and coef as the forward wrote them.  Rows that are
  * ignored have zero grad_x and no share of the other two, whatever x holds
- * there.  Sums in a fixed order; the logits' gradient is rounded to 16 bits once
- * between its two products (float32: not rounded).
+ * there.  Sums in a fixed order, in float32; between its products the logits'
+ * gradient is two terms of 16-bit operands' type, which lose 2^-16 (bf16) or
+ * 2^-22 (fp16; 2^-40 of the largest at least) of it, and float32 beside float32.
  */
 int rpfq_linear_cross_entropy_grad(const rpfq_ce_desc* desc, const void* x, const void* w, const void* bias,
                                    const int64_t* target, const float* stat, const float* coef, const float* grad_loss,

@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(256 * WM, 2) int8_gemm_kernel(Int8Args a) {
     const int steps = (int)G::steps(a.K);
     // scales and biases of the tile's columns and scales of its rows
     float* col = reinterpret_cast<float*>(smem + G::LDS);
-    G::run(a.x, a.w, (int64_t)mt * G::ROWS, n0, a.K, a.K, steps, false, 0, steps, smem, wave, lane, acc, [&] {
+    G::run(a.x, a.w, (int64_t)mt * G::ROWS, n0, a.K, a.K, steps, 1, 0, steps, smem, wave, lane, acc, [&] {
         for (int c = threadIdx.x; c < 256; c += G::THREADS) {
             const int64_t n = n0 + c;
             col[c] = n < a.N ? a.sw[n] : 0.0f;
@@ -246,7 +246,6 @@ __global__ void __launch_bounds__(256 * WM, 2) int8_gemm_kernel(Int8Args a) {
                     const f32x4 v = (f32x4){(float)v0 * sx, (float)v1 * sx, (float)v2 * sx, (float)v3 * sx} * w + b;
                     return make_uint2(tile_pack2<YDT>(v[0], v[1]), tile_pack2<YDT>(v[2], v[3]));
                 },
-                [] {},
                 [&](int row, int c, uint4 v) {
                     const int64_t m = m0 + 32 * i + row;
                     if (m < a.M) tile_store8(a.y, m * a.N, nw + c, a.N, a.vec, v);

@@ -9,13 +9,19 @@
 // not lse: that one's last bit is 2^-20 of a probability near 1, which is most
 // of dz where p - 1 is small.
 // Backward: the logits are formed again, a piece of the classes at a time; dz
-// of a piece goes to a workspace in 16 bits and meets w and x from there.
+// of a piece goes to a workspace and meets w and x from there.
 //
-// Roundings to 16 bits: dz only, once (bf16 2^-9 of its value; fp16 2^-12, dz
-// times 2^15 so that probabilities down to 2^-29 stay normal), as the matrix
-// cores take it; the sums over classes and rows stay in float32 until the
-// gradients are rounded to their own type.  float32 operands lose nothing:
-// many rows go as three bf16 terms (tile_pair), few as they are (kCeDirectRows).
+// dz as the matrix cores take it: beside 16-bit operands as two terms of their
+// type, what the first leaves (at most 2^-8 of the value in bf16, 2^-11 in fp16)
+// being rounded once more: 2^-16 and 2^-22 of the value are lost, and in fp16,
+// where dz is taken times 2^15 so that probabilities down to 2^-29 stay normal,
+// 2^-40 at least.  One term alone left gradients of 64 rows (1,000 classes, bf16)
+// 2.3e-3 off, where the rounding of the result is 1.7e-3; two leave 1.7e-3 and
+// cost the gradients' products twice (2,048 x 20,000 x 1,024 fp16 loss and
+// gradients 413 -> 614 us, 8,192 x 65,536 x 768 bf16 3,310 -> 5,260).  The sums
+// over classes and rows stay in float32 until the gradients are rounded to their
+// own type.  float32 operands lose nothing: many rows go as three bf16 terms
+// (tile_pair), few as they are (kCeDirectRows).
 #include <cmath>
 
 #include "tile_gemm.h"
@@ -55,7 +61,7 @@ struct CeArgs {
     int64_t M, V;              // rows, classes (w.count: those of a piece)
     int64_t v0;                // first class of the piece
     int64_t kb;                // bytes of k
-    int planes;
+    int pairs;                 // of the planes of x and w
     int tiles_m, tiles_n, group;
     float smooth;
     // forward
@@ -68,7 +74,7 @@ struct CeArgs {
     int64_t ignore;
     float dz_scale;
     char* xz;                  // x without its ignored rows, to be written here; or NULL
-    char* dz;                  // [planes][M][ldz bytes]
+    char* dz;                  // [terms][M][ldz bytes]
     int64_t ldz, dz_plane;
     int64_t n8;                // columns of dz that are written: the piece's, in whole 16 bytes
     float* colsum;             // [row waves][n8] or NULL
@@ -142,9 +148,9 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_stats_kernel(CeArgs a) {
     floatx16 acc[2][MB];
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
-    const int per = (int)G::steps(a.kb), steps = a.planes ? kPairs32 * per : per;
+    const int per = (int)G::steps(a.kb), steps = a.pairs * per;
     float* sb = reinterpret_cast<float*>(smem + G::LDS);
-    G::run(a.x, a.w, m0, n0, a.kb, a.kb, per, a.planes, 0, steps, smem, wave, lane, acc, [&] { ce_stage_bias(a, n0, sb); });
+    G::run(a.x, a.w, m0, n0, a.kb, a.kb, per, a.pairs, 0, steps, smem, wave, lane, acc, [&] { ce_stage_bias(a, n0, sb); });
     float* sp = reinterpret_cast<float*>(smem);  // [4 column waves][rows][max, sum, sum of z]
     if (ce_biased(a, n0)) ce_bias<MB>(acc, sb + 64 * (wave & 3), lane);
 #pragma unroll
@@ -467,7 +473,19 @@ __device__ __forceinline__ float ce_lane_sums(float (&v)[32], int lane) {
     return v[0];
 }
 
-// dz of one piece of the classes.  DT: the type of dz (float32: three planes).
+// A value as two 16-bit terms, both nearest.  What an inf leaves is 0 and not
+// inf - inf.
+template <int DT>
+__device__ __forceinline__ void ce_terms2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = tile_pack2<DT>(a, b);
+    const float ha = DT == RPFQ_F16 ? (float)__builtin_bit_cast(half2v, hi)[0] : bf16_to_f32(hi & 0xffffu);
+    const float hb = DT == RPFQ_F16 ? (float)__builtin_bit_cast(half2v, hi)[1] : bf16_to_f32(hi >> 16);
+    const float la = a - ha, lb = b - hb;
+    lo = tile_pack2<DT>(la == la ? la : 0.0f, lb == lb ? lb : 0.0f);
+}
+
+// dz of one piece of the classes.  DT: the type of dz's terms (float32: itself
+// beside float32 operands, three bf16 terms beside theirs).
 // The logits' product again and M V elements written: 8,192 x 65,536 x 768 bf16
 // 950 us, 870 TFLOP/s and 1.1 TB/s of dz; 2,048 x 20,000 x 1,024 fp16 114 us.  Stores
 // past the caches were slower where a piece of dz stays in them.
@@ -484,10 +502,10 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
     floatx16 acc[2][MB];
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
-    const int per = (int)G::steps(a.kb), steps = a.planes ? kPairs32 * per : per;
+    const int per = (int)G::steps(a.kb), steps = a.pairs * per;
     CeLds<G::ROWS>& sh = *reinterpret_cast<CeLds<G::ROWS>*>(smem + G::LDS);
     const float even = a.smooth / (float)a.V;
-    G::run(a.x, a.w, m0, n0, a.kb, a.kb, per, a.planes, 0, steps, smem, wave, lane, acc, [&] {
+    G::run(a.x, a.w, m0, n0, a.kb, a.kb, per, a.pairs, 0, steps, smem, wave, lane, acc, [&] {
         ce_stage_bias(a, n0, sh.bias);
         if (threadIdx.x < G::ROWS) {
             const int64_t m = m0 + threadIdx.x;
@@ -554,13 +572,11 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
                 for (int v = 0; v < 16; ++v)
                     if (nw + 32 * j + acc_row(v, g) >= a.w.count) acc[j][i][v] = 0.0f;
         }
-        if (DT == RPFQ_F32 || a.colsum) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    if (t == 32 * j + acc_row(v, g)) acc[j][i][v] = dzt;
-        }
+            for (int v = 0; v < 16; ++v)
+                if (t == 32 * j + acc_row(v, g)) acc[j][i][v] = dzt;
         if constexpr (DT == RPFQ_F32) {
             const int64_t n = nw + 4 * (lane & 15);
             tile_rows(epi, acc[0][i], acc[1][i], lane, [](float v, int) { return v; },
@@ -580,19 +596,18 @@ __global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
                           __builtin_memcpy(d + 2 * a.dz_plane, l, 8);
                       });
         } else {
-            tile_rows_half(
-                epi, acc[0][i], acc[1][i], lane,
-                [&](float a0, float a1, float a2, float a3, int, int) {
-                    return make_uint2(tile_pack2<DT>(a0, a1), tile_pack2<DT>(a2, a3));
-                },
-                [&] {
-                    if (t >= 0 && g == 0)
-                        *reinterpret_cast<uint16_t*>(epi + tile_half_at(r, t)) = (uint16_t)tile_pack2<DT>(dzt, 0.0f);
-                },
-                [&](int row, int c, uint4 v) {
-                    const int64_t m = mw + 32 * i + row, n = nw + c;
-                    if (m < a.M && n < a.n8) *reinterpret_cast<uint4*>(a.dz + m * a.ldz + 2 * n) = v;
-                });
+            tile_rows8(epi, acc[0][i], acc[1][i], lane, [&](int row, int c, f32x4 v, f32x4 u) {
+                const int64_t m = mw + 32 * i + row, n = nw + c;
+                if (m >= a.M || n >= a.n8) return;
+                uint4 h, l;
+                ce_terms2<DT>(v[0], v[1], h.x, l.x);
+                ce_terms2<DT>(v[2], v[3], h.y, l.y);
+                ce_terms2<DT>(u[0], u[1], h.z, l.z);
+                ce_terms2<DT>(u[2], u[3], h.w, l.w);
+                char* d = a.dz + m * a.ldz + 2 * n;
+                *reinterpret_cast<uint4*>(d) = h;
+                *reinterpret_cast<uint4*>(d + a.dz_plane) = l;
+            });
         }
     }
     if (a.colsum) {  // the wave's columns over its rows
@@ -615,7 +630,7 @@ struct CeGrad {
     TileOperand r, c;
     int64_t rk, ck;
     int64_t M, N;     // rows, columns of the gradient
-    int planes, splits;
+    int pairs, splits;
     int tiles_m, tiles_n;
     float* part;      // [splits][M][ldp], or NULL: the gradient itself, rounded
     int64_t ldp;
@@ -635,12 +650,12 @@ __device__ __forceinline__ void ce_grad_unit(const CeGrad& a, int bid, char* sme
     int mt, nt;
     group_tile(unit - sp * tiles, a.tiles_m, a.tiles_n, a.tiles_n, mt, nt);
     const int64_t m0 = (int64_t)mt * G::ROWS, mw = m0 + 32 * MB * (wave >> 2), n0 = (int64_t)nt * 256;
-    const int per = (int)G::steps(a.rk), steps = a.planes ? kPairs32 * per : per;
+    const int per = (int)G::steps(a.rk), steps = a.pairs * per;
     const int s0 = (int)((int64_t)steps * sp / a.splits), s1 = (int)((int64_t)steps * (sp + 1) / a.splits);
     floatx16 acc[2][MB];
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[0][i] = acc[1][i] = floatx16{0};
-    G::run(a.r, a.c, m0, n0, a.rk, a.ck, per, a.planes, s0, s1, smem, wave, lane, acc, [] {});
+    G::run(a.r, a.c, m0, n0, a.rk, a.ck, per, a.pairs, s0, s1, smem, wave, lane, acc, [] {});
     const int64_t n = n0 + 64 * (wave & 3) + 4 * (lane & 15);
     const float f = a.part ? 1.0f : a.factor();
     float* part = a.part ? a.part + (int64_t)sp * a.M * a.ldp : nullptr;
@@ -726,9 +741,9 @@ __global__ void __launch_bounds__(256) ce_sums_kernel(CeSums a) {
 // the least time: the longest unit or the chip's share of all and half a unit,
 // in steps of a 256-row tile (0.9 us), and the partials' way through memory
 // (about 5 TB/s, and a launch).
-static CeSplit ce_split(int64_t M, int64_t V, int64_t D, int planes, int es) {
+static CeSplit ce_split(int64_t M, int64_t V, int64_t D, int pairs, int es) {
     // float32 as it is: twice the steps, each eight times as long
-    const int64_t cost16 = planes == 3 ? kPairs32 : es == 4 ? 16 : 1, least = es == 4 ? 16 : 4;
+    const int64_t cost16 = es == 4 ? 16 : pairs, least = es == 4 ? 16 : 4;
     const int64_t cus = device_cus(), tn = (D + 255) / 256, kx = cost16 * ((V + 31) / 32), kw = cost16 * ((M + 31) / 32);
     static constexpr int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64};
     CeSplit best = {kTile128, 1, 1};
@@ -780,11 +795,15 @@ static int64_t ce_ldz(int64_t n, int es) {
 // 10,008 x 768, 64 rows 185 -> 163, 256 both 221, 1,024 492 -> 677).
 constexpr int64_t kCeDirectRows = 256;
 
+// products of dz's terms with those of the other operand
+static int ce_pairs(int terms) { return terms == 3 ? kPairs32 : terms; }
+
 CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool backward) {
     CePlan p = {};
     const bool direct = dt == RPFQ_F32 && M <= kCeDirectRows;
     const int planes = p.planes = dt == RPFQ_F32 && !direct ? 3 : 1;
     const int es = p.es = direct ? 4 : 2;
+    const int terms = p.terms = direct ? 1 : planes == 3 ? 3 : 2;
     p.ldk = planes == 3 ? (D + 31) & ~(int64_t)31 : (D + 7) & ~(int64_t)7;
     p.pad = planes == 3 || D % 8 != 0;
     auto take = [&](int64_t n) {
@@ -807,15 +826,15 @@ CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool back
     if (!p.pad) p.x_at = take(es * M * p.ldk);  // x without its ignored rows
     p.rho_at = take(4 * M);
     p.factor_at = take(4);
-    const int64_t fit = std::max<int64_t>(1, kCePiece / (es * planes * M * 256));
+    const int64_t fit = std::max<int64_t>(1, kCePiece / (es * terms * M * 256));
     p.pieces = (p.tiles_v + fit - 1) / fit;
     p.piece = (p.tiles_v + p.pieces - 1) / p.pieces * 256;  // classes
     if (p.piece > V) p.piece = (V + 7) & ~(int64_t)7;
-    p.dz_at = take(planes * M * (es * p.piece + 256));
+    p.dz_at = take(terms * M * (es * p.piece + 256));
     p.col_at = take(4 * ((M + 31) / 32 + 8) * p.piece);
     // float32 partials, rows of whole 16 bytes
     p.ldp = (D + 3) & ~(int64_t)3;
-    p.grad = ce_split(M, p.piece, D, planes, es);
+    p.grad = ce_split(M, p.piece, D, ce_pairs(p.terms), es);
     p.dx_at = take(p.grad.dx > 1 || p.pieces > 1 ? 4 * p.grad.dx * M * p.ldp : 0);
     p.dw_at = take(p.grad.dw > 1 ? 4 * p.grad.dw * p.piece * p.ldp : 0);
     return p;
@@ -827,7 +846,7 @@ static unsigned blocks_of(int64_t n) { return (unsigned)(n < 1 ? 1 : n > 16384 ?
 // target: rows of x that it ignores are zero there (backward).
 static hipError_t ce_operands(const CePlan& p, const CeCall& c, const int64_t* target, char* wk, CeArgs& a, hipStream_t s) {
     a.kb = p.es * p.ldk;
-    a.planes = p.planes == 3;
+    a.pairs = p.planes == 3 ? kPairs32 : 1;
     a.x = {reinterpret_cast<const char*>(c.x), a.kb, 0, c.M};
     a.w = {reinterpret_cast<const char*>(c.w), a.kb, 0, c.V};
     a.bias = c.bias;
@@ -849,7 +868,7 @@ static hipError_t ce_operands(const CePlan& p, const CeCall& c, const int64_t* t
                       c.ignore,
                       lanes};
     const dim3 grid(blocks_of(((c.M + c.V) * lanes + 255) / 256));
-    if (a.planes) hipLaunchKernelGGL(ce_copy_kernel<1>, grid, dim3(256), 0, s, k);
+    if (p.planes == 3) hipLaunchKernelGGL(ce_copy_kernel<1>, grid, dim3(256), 0, s, k);
     else if (p.es == 4) hipLaunchKernelGGL(ce_copy_kernel<2>, grid, dim3(256), 0, s, k);
     else hipLaunchKernelGGL(ce_copy_kernel<0>, grid, dim3(256), 0, s, k);
     a.x.p = wk + p.x_at;
@@ -1023,7 +1042,7 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         const TileOperand dzk = {a.dz, a.ldz, a.dz_plane, c.M}, dzt = {a.dz, a.ldz, a.dz_plane, n};
         CeGrads both = {};
         CeGrad &dx = both.g[0], &dw = both.g[1];
-        dx.planes = dw.planes = a.planes;
+        dx.pairs = dw.pairs = ce_pairs(p.terms);
         dx.N = dw.N = c.D;
         dx.ldp = dw.ldp = p.ldp;
         dx.factor = dw.factor = factor;

@@ -408,7 +408,7 @@ struct CeSplit {
     int dx, dw;     // parts of their k
 };
 struct CePlan {
-    int es, planes;         // bytes of an operand's element, bf16 terms of a float32
+    int es, planes, terms;  // bytes of an operand's element, planes of x and w (bf16 terms of a float32), of dz
     int64_t ldk, ldp;       // elements of a row of k; of float32 partials
     bool pad;               // x and w are copied (rows of ldk, or three planes of them)
     int64_t tiles_v, piece, pieces;

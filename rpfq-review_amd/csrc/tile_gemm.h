@@ -55,7 +55,7 @@ struct MmaF32 {
 // One operand of a product.  K layout: `count` rows of `k_bytes` at p + row ld.
 // T layout: k rows at p + k ld of `count` elements.  p, ld, k_bytes (K) and the
 // bytes of count (T) are multiples of 16.  Planes (float32 as three bf16
-// terms) lie `plane` bytes apart.
+// terms, or as two of 16 bits) lie `plane` bytes apart.
 struct TileOperand {
     const char* p;
     int64_t ld;
@@ -201,12 +201,13 @@ struct TileGemm {
     static constexpr int64_t steps(int64_t k) { return (k + R::PER - 1) / R::PER; }
 
     // Adds steps s0 .. s1 - 1 of the product; a step is KB bytes of k of one
-    // pair of planes, `per` steps a pair.  rk, ck: k of the operands as issue()
-    // takes it.  meanwhile(): what the epilogue wants in LDS past the stages,
-    // loaded while the first steps are on their way (s0 < s1).
+    // pair of planes, `per` steps a pair.  pairs: 1, kPairs32 of two operands of
+    // three planes, or R's planes, the last (smallest) first.  rk, ck: k of the
+    // operands as issue() takes it.  meanwhile(): what the epilogue wants in LDS
+    // past the stages, loaded while the first steps are on their way (s0 < s1).
     template <class F>
     static __device__ __forceinline__ void run(const TileOperand& ro, const TileOperand& co, int64_t m0, int64_t n0,
-                                               int64_t rk, int64_t ck, int per, bool planes, int s0, int s1, char* smem,
+                                               int64_t rk, int64_t ck, int per, int pairs, int s0, int s1, char* smem,
                                                int wave, int lane, acc_t (&acc)[2][MB], F meanwhile) {
         R rs;
         C cs;
@@ -216,8 +217,8 @@ struct TileGemm {
         const int wc = wave & 3, wr = wave >> 2;
         int pair = s0 / per, ks = s0 - pair * per;
         auto issue = [&](int st) {
-            int rp = 0, cp = 0;
-            if (planes) tile_pair(pair, rp, cp);
+            int rp = pairs - 1 - pair, cp = 0;
+            if (pairs == kPairs32) tile_pair(pair, rp, cp);
             rs.issue(ks, rp, rk, lds + st * STAGE, wave);
             cs.issue(ks, cp, ck, lds + st * STAGE + R::BYTES, wave);
             if (++ks == per) {
@@ -363,12 +364,36 @@ __device__ __forceinline__ void tile_rows(char* epi, const Acc& a0, const Acc& a
     __builtin_amdgcn_wave_barrier();
 }
 
+// The same with 8 columns a lane: out(row, column, 4 values, the 4 behind them).
+template <class Acc, class Out>
+__device__ __forceinline__ void tile_rows8(char* epi, const Acc& a0, const Acc& a1, int lane, Out out) {
+    const int r = lane & 31, g = lane >> 5, c = lane & 7, row8 = lane >> 3;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const Acc& a = j ? a1 : a0;
+            const f32x4 v = {a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+            *reinterpret_cast<f32x4*>(epi + r * 256 + (((8 * j + 2 * q + g) ^ (r & 15)) * 16)) = v;
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int row = 8 * j + row8;
+        const char* from = epi + row * 256;
+        out(row, 8 * c, *reinterpret_cast<const f32x4*>(from + (((2 * c) ^ (row & 15)) * 16)),
+            *reinterpret_cast<const f32x4*>(from + (((2 * c + 1) ^ (row & 15)) * 16)));
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // The same for 16-bit outputs, half the LDS: value4(4 values, column) packs four
-// columns to 8 bytes, patch() may change the staged block (its byte of row r,
-// column c: tile_half_at), out(row, column, 8 values) stores 128-byte pieces.
+// columns to 8 bytes, out(row, column, 8 values) stores 128-byte pieces.
 __device__ __forceinline__ int tile_half_at(int r, int c) { return r * 128 + (((c >> 3) ^ ((r >> 1) & 7)) * 16) + (c & 7) * 2; }
-template <class Acc, class F, class P, class Out>
-__device__ __forceinline__ void tile_rows_half(char* epi, const Acc& a0, const Acc& a1, int lane, F value4, P patch, Out out) {
+template <class Acc, class F, class Out>
+__device__ __forceinline__ void tile_rows_half(char* epi, const Acc& a0, const Acc& a1, int lane, F value4, Out out) {
     const int r = lane & 31, g = lane >> 5;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -378,7 +403,6 @@ __device__ __forceinline__ void tile_rows_half(char* epi, const Acc& a0, const A
             const Acc& a = j ? a1 : a0;
             *reinterpret_cast<uint2*>(epi + tile_half_at(r, c)) = value4(a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3], j, q);
         }
-    patch();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
