@@ -352,24 +352,25 @@ __global__ void __launch_bounds__(1024) ce_join_kernel(CeJoin a) {
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
-// reduction none: rho[m] = grad[m] over the largest of the rows that count, so
-// that dz stays within [-1, 1], and that largest, factor[0].
+// reduction none: rho[m] = grad[m] over the largest finite one of the rows that
+// count, so that their dz stays within [-1, 1], and that largest, factor[0].  A
+// row with inf or NaN keeps it to itself and to grad_w.
 __global__ void __launch_bounds__(1024) ce_rho_kernel(const float* grad, const int64_t* target, int64_t M, int64_t ignore,
                                                       float* rho, float* factor) {
     __shared__ float sm[1024];
     const int t = threadIdx.x;
     float top = 0.0f;
-    for (int64_t m = t; m < M; m += 1024)
-        if (target[m] != ignore) top = fmaxf(top, fabsf(grad[m]));
+    for (int64_t m = t; m < M; m += 1024) {
+        const float g = fabsf(grad[m]);
+        if (target[m] != ignore && g <= 3.40282347e38f) top = fmaxf(top, g);
+    }
     sm[t] = top;
     __syncthreads();
     for (int h = 512; h > 0; h >>= 1) {
         if (t < h) sm[t] = fmaxf(sm[t], sm[t + h]);
         __syncthreads();
     }
-    top = sm[0];
-    // no finite scale: the rows keep their gradients as they are
-    if (!(top > 0.0f) || top > 3.40282347e38f) top = 1.0f;
+    top = sm[0] > 0.0f ? sm[0] : 1.0f;
     for (int64_t m = t; m < M; m += 1024) rho[m] = grad[m] / top;
     if (t == 0) factor[0] = top;
 }

@@ -46,3 +46,32 @@ def test_error_of_a_batch_is_that_of_its_rounding(dtype):
         rounded = float((e.to(dtype).double() - e).norm())
         # as the result's own rounding: the rest is 2^-16 (2^-22) of dz, 2^-4 of a step, and the sums' 2^-20
         assert float((g.double() - e).norm()) <= 1.1 * rounded
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m", [40, 400])
+def test_rows_beside_an_infinite_upstream_gradient(m, dtype, bad):
+    """grad_x of the finite rows is what it is without the other row (whose
+    gradient, here 0 instead, takes no part in theirs), and finite."""
+    from quant_models import ops
+
+    x, w, t, b = base._inputs(m, 300, 64, dtype, True, 0.2)
+    t[3] = 7
+    g = torch.linspace(-900, 900, m, device=DEV)
+    with_bad, without = g.clone(), g.clone()
+    with_bad[3], without[3] = bad, 0.0
+
+    def run(up):
+        leaves = [p.clone().requires_grad_() for p in (x, w, b)]
+        return torch.autograd.grad(ops.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none"), leaves, up)
+
+    got, want = run(with_bad), run(without)
+    rows = torch.arange(m, device=DEV) != 3
+    assert bool(torch.isfinite(got[0][rows]).all()) and torch.equal(got[0][rows], want[0][rows])
+    assert not bool(torch.isfinite(got[0][3]).any()) and not bool(torch.isfinite(got[1][7]).any())
+    base._check(x, w, t, b, 0.0, "none", without)
+    # a row without a label keeps its gradient to itself, whatever it is
+    t[3] = -100
+    assert all(torch.equal(a, e) for a, e in zip(run(with_bad), run(without)))
