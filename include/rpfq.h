@@ -710,7 +710,9 @@ int rpfq_linear_cross_entropy(const rpfq_ce_desc* desc, const void* x, const voi
  * ignored have zero grad_x and no share of the other two, whatever x holds
  * there.  Sums in a fixed order, in float32; between its products the logits'
  * gradient is two terms of 16-bit operands' type, which lose 2^-16 (bf16) or
- * 2^-22 (fp16; 2^-40 of the largest at least) of it, and float32 beside float32.
+ * 2^-22 (fp16; 2^-40 of grad_loss at least) of it, and float32 beside float32.
+ * fp16 with RPFQ_REDUCE_NONE, whose rows' gradients may lie far apart: bf16
+ * terms, 2^-15 of each row's.
  */
 int rpfq_linear_cross_entropy_grad(const rpfq_ce_desc* desc, const void* x, const void* w, const void* bias,
                                    const int64_t* target, const float* stat, const float* coef, const float* grad_loss,

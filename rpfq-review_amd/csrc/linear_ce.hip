@@ -21,7 +21,9 @@
 // gradients 413 -> 614 us, 8,192 x 65,536 x 768 bf16 3,310 -> 5,260).  The sums
 // over classes and rows stay in float32 until the gradients are rounded to their
 // own type.  float32 operands lose nothing: many rows go as three bf16 terms
-// (tile_pair), few as they are (kCeDirectRows).
+// (tile_pair), few as they are (kCeDirectRows).  fp16 rows with upstream gradients
+// of their own have dz in two bf16 terms, with 2^-16 of it for the product of the
+// second terms that is left out (CePlan::wide).
 #include <cmath>
 
 #include "tile_gemm.h"
@@ -390,6 +392,17 @@ __device__ __forceinline__ void split3(float v, uint16_t& h, uint16_t& m, uint16
     l = (uint16_t)(__float_as_uint(r2) >> 16);
 }
 
+// A value as two 16-bit terms, both nearest.  What an inf leaves is 0 and not
+// inf - inf.
+template <int DT>
+__device__ __forceinline__ void ce_terms2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = tile_pack2<DT>(a, b);
+    const float ha = DT == RPFQ_F16 ? (float)__builtin_bit_cast(half2v, hi)[0] : bf16_to_f32(hi & 0xffffu);
+    const float hb = DT == RPFQ_F16 ? (float)__builtin_bit_cast(half2v, hi)[1] : bf16_to_f32(hi >> 16);
+    const float la = a - ha, lb = b - hb;
+    lo = tile_pack2<DT>(la == la ? la : 0.0f, lb == lb ? lb : 0.0f);
+}
+
 // x [M, D] and w [V, D] as operands: rows of ld elements, float32 as three planes
 // of bf16 terms.  target: rows of x that it ignores are zeros, whatever they
 // hold (0 x NaN would reach every class of dw); NULL: all rows as they are.
@@ -402,7 +415,8 @@ struct CeCopy {
     int64_t ignore;
     int lanes;
 };
-// MODE 0: 16-bit rows, 1: planes, 2: float32 rows.  `lanes` (a power of two) take
+// MODE 0: 16-bit rows, 1: planes, 2: float32 rows, 3: fp16 as two bf16 planes
+// (nearest, and what that leaves: 3 bits, exact).  `lanes` (a power of two) take
 // a row, 8 elements each; whole pieces are read at once, at any alignment of
 // their elements.
 template <int MODE>
@@ -416,7 +430,7 @@ __global__ void __launch_bounds__(256) ce_copy_kernel(CeCopy a) {
         for (int i = lane; i < per; i += a.lanes) {
             const int64_t d = 8 * i;
             uint16_t* out = a.dst[k] + (m * a.ld + d) * (MODE == 2 ? 2 : 1);
-            if constexpr (MODE == 0) {
+            if constexpr (MODE == 0 || MODE == 3) {
                 const uint16_t* x = reinterpret_cast<const uint16_t*>(a.src[k]) + m * a.D + d;
                 uint16_t e[8] = {0, 0, 0, 0, 0, 0, 0, 0};
                 if (on && d + 8 <= a.D) {
@@ -425,6 +439,19 @@ __global__ void __launch_bounds__(256) ce_copy_kernel(CeCopy a) {
 #pragma unroll
                     for (int t = 0; t < 8; ++t)
                         if (d + t < a.D) e[t] = x[t];
+                }
+                if constexpr (MODE == 3) {
+                    uint4 h, l;
+                    auto two = [&](int i, uint32_t& hi, uint32_t& lo) {
+                        ce_terms2<RPFQ_BF16>((float)__builtin_bit_cast(_Float16, e[i]), (float)__builtin_bit_cast(_Float16, e[i + 1]),
+                                             hi, lo);
+                    };
+                    two(0, h.x, l.x);
+                    two(2, h.y, l.y);
+                    two(4, h.z, l.z);
+                    two(6, h.w, l.w);
+                    __builtin_memcpy(e, &h, 16);
+                    __builtin_memcpy(out + a.rows[k] * a.ld, &l, 16);
                 }
                 __builtin_memcpy(out, e, 16);
             } else {
@@ -472,17 +499,6 @@ __device__ __forceinline__ float ce_lane_sums(float (&v)[32], int lane) {
     ce_lane_round<2>(v, lane);
     ce_lane_round<1>(v, lane);
     return v[0];
-}
-
-// A value as two 16-bit terms, both nearest.  What an inf leaves is 0 and not
-// inf - inf.
-template <int DT>
-__device__ __forceinline__ void ce_terms2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    hi = tile_pack2<DT>(a, b);
-    const float ha = DT == RPFQ_F16 ? (float)__builtin_bit_cast(half2v, hi)[0] : bf16_to_f32(hi & 0xffffu);
-    const float hb = DT == RPFQ_F16 ? (float)__builtin_bit_cast(half2v, hi)[1] : bf16_to_f32(hi >> 16);
-    const float la = a - ha, lb = b - hb;
-    lo = tile_pack2<DT>(la == la ? la : 0.0f, lb == lb ? lb : 0.0f);
 }
 
 // dz of one piece of the classes.  DT: the type of dz's terms (float32: itself
@@ -797,10 +813,16 @@ static int64_t ce_ldz(int64_t n, int es) {
 constexpr int64_t kCeDirectRows = 256;
 
 // products of dz's terms with those of the other operand
-static int ce_pairs(int terms) { return terms == 3 ? kPairs32 : terms; }
+static int ce_pairs(const CePlan& p) { return p.terms == 3 ? kPairs32 : p.wide ? kPairsHalf : p.terms; }
 
 CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool backward) {
     CePlan p = {};
+    // fp16 rows with upstream gradients of their own: dz, whose rows may lie far
+    // apart, in bf16 terms, and x and w in as many for its products.  Under one
+    // fp16 scale a row 2^-25 of the largest kept three bits.  2,048 x 20,000 x 1,024
+    // loss and gradients 645 -> 809 us, 256 x 10,000 x 768 75 -> 90; through the
+    // six products of float32 operands 1,632 and 192.
+    p.wide = dt == RPFQ_F16 && reduction == RPFQ_REDUCE_NONE && backward;
     const bool direct = dt == RPFQ_F32 && M <= kCeDirectRows;
     const int planes = p.planes = dt == RPFQ_F32 && !direct ? 3 : 1;
     const int es = p.es = direct ? 4 : 2;
@@ -824,7 +846,12 @@ CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool back
         p.rows_at = take(reduction ? 4 * M : 0);
         return p;
     }
-    if (!p.pad) p.x_at = take(es * M * p.ldk);  // x without its ignored rows
+    if (p.wide) {  // two planes of x (without its ignored rows) and w
+        p.x2_at = take(4 * M * p.ldk);
+        p.w2_at = take(4 * V * p.ldk);
+    } else if (!p.pad) {
+        p.x_at = take(es * M * p.ldk);  // x without its ignored rows
+    }
     p.rho_at = take(4 * M);
     p.factor_at = take(4);
     const int64_t fit = std::max<int64_t>(1, kCePiece / (es * terms * M * 256));
@@ -835,13 +862,29 @@ CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool back
     p.col_at = take(4 * ((M + 31) / 32 + 8) * p.piece);
     // float32 partials, rows of whole 16 bytes
     p.ldp = (D + 3) & ~(int64_t)3;
-    p.grad = ce_split(M, p.piece, D, ce_pairs(p.terms), es);
+    p.grad = ce_split(M, p.piece, D, ce_pairs(p), es);
     p.dx_at = take(p.grad.dx > 1 || p.pieces > 1 ? 4 * p.grad.dx * M * p.ldp : 0);
     p.dw_at = take(p.grad.dw > 1 ? 4 * p.grad.dw * p.piece * p.ldp : 0);
     return p;
 }
 
 static unsigned blocks_of(int64_t n) { return (unsigned)(n < 1 ? 1 : n > 16384 ? 16384 : n); }
+
+template <int MODE>
+static hipError_t ce_copy(const CePlan& p, const CeCall& c, const int64_t* target, const char* x, const char* w, hipStream_t s) {
+    int lanes = 1;
+    while (lanes < 64 && 8 * lanes < p.ldk) lanes *= 2;
+    const CeCopy k = {{c.x, c.w},
+                      {reinterpret_cast<uint16_t*>(const_cast<char*>(x)), reinterpret_cast<uint16_t*>(const_cast<char*>(w))},
+                      {c.M, c.V},
+                      c.D,
+                      p.ldk,
+                      target,
+                      c.ignore,
+                      lanes};
+    hipLaunchKernelGGL(ce_copy_kernel<MODE>, dim3(blocks_of(((c.M + c.V) * lanes + 255) / 256)), dim3(256), 0, s, k);
+    return hipGetLastError();
+}
 
 // The operands of the logits: as they are, or padded / split copies in `work`.
 // target: rows of x that it ignores are zero there (backward).
@@ -858,25 +901,13 @@ static hipError_t ce_operands(const CePlan& p, const CeCall& c, const int64_t* t
     a.smooth = c.smooth;
     a.ignore = c.ignore;
     if (!p.pad) return hipSuccess;
-    int lanes = 1;
-    while (lanes < 64 && 8 * lanes < p.ldk) lanes *= 2;
-    const CeCopy k = {{c.x, c.w},
-                      {reinterpret_cast<uint16_t*>(wk + p.x_at), reinterpret_cast<uint16_t*>(wk + p.w_at)},
-                      {c.M, c.V},
-                      c.D,
-                      p.ldk,
-                      target,
-                      c.ignore,
-                      lanes};
-    const dim3 grid(blocks_of(((c.M + c.V) * lanes + 255) / 256));
-    if (p.planes == 3) hipLaunchKernelGGL(ce_copy_kernel<1>, grid, dim3(256), 0, s, k);
-    else if (p.es == 4) hipLaunchKernelGGL(ce_copy_kernel<2>, grid, dim3(256), 0, s, k);
-    else hipLaunchKernelGGL(ce_copy_kernel<0>, grid, dim3(256), 0, s, k);
     a.x.p = wk + p.x_at;
     a.w.p = wk + p.w_at;
     a.x.plane = 2 * c.M * p.ldk;  // planes are 16-bit
     a.w.plane = 2 * c.V * p.ldk;
-    return hipGetLastError();
+    return p.planes == 3 ? ce_copy<1>(p, c, target, a.x.p, a.w.p, s)
+           : p.es == 4   ? ce_copy<2>(p, c, target, a.x.p, a.w.p, s)
+                         : ce_copy<0>(p, c, target, a.x.p, a.w.p, s);
 }
 
 template <class K>
@@ -951,11 +982,13 @@ struct GradGo {
         return hipGetLastError();
     }
 };
-static hipError_t ce_grads(int dt, bool direct, TileForm form, CeGrads& g, hipStream_t s) {
-    return direct            ? tile_dispatch64(form, GradGo<MmaF32, RPFQ_F32>{g, s})
+static hipError_t ce_grads(int dt, const CePlan& p, CeGrads& g, hipStream_t s) {
+    const TileForm form = p.grad.form;
+    return p.terms == 1      ? tile_dispatch64(form, GradGo<MmaF32, RPFQ_F32>{g, s})
+           : p.terms == 3    ? tile_dispatch64(form, GradGo<MmaBf16, RPFQ_F32>{g, s})
+           : p.wide          ? tile_dispatch64(form, GradGo<MmaBf16, RPFQ_F16>{g, s})
            : dt == RPFQ_F16  ? tile_dispatch64(form, GradGo<MmaF16, RPFQ_F16>{g, s})
-           : dt == RPFQ_BF16 ? tile_dispatch64(form, GradGo<MmaBf16, RPFQ_BF16>{g, s})
-                             : tile_dispatch64(form, GradGo<MmaBf16, RPFQ_F32>{g, s});
+                             : tile_dispatch64(form, GradGo<MmaBf16, RPFQ_BF16>{g, s});
 }
 
 static CeSum ce_sum(int dt, const float* part, int parts, int64_t stride, int64_t rows, int64_t N, int64_t ldp, void* out) {
@@ -1003,7 +1036,7 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
     CeArgs a = {};
     hipError_t e = ce_operands(p, c, c.target, wk, a, s);
     if (e != hipSuccess) return e;
-    const float scale = c.dtype == RPFQ_F16 ? 32768.0f : 1.0f;
+    const float scale = c.dtype == RPFQ_F16 && !p.wide ? 32768.0f : 1.0f;
     CeFactor factor = {grad, c.reduction == 1 ? coef : nullptr, 1.0f / scale};
     if (c.reduction == 0) {
         float* rho = reinterpret_cast<float*>(wk + p.rho_at);
@@ -1013,8 +1046,14 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         a.rho = rho;
         factor.grad = top;
     }
-    TileOperand xz = a.x;  // x of dw: its ignored rows as zeros
-    if (gw && !p.pad) {
+    TileOperand xz = a.x, w2 = a.w;  // of the gradients' products; x's ignored rows as zeros
+    if (p.wide) {
+        xz.p = wk + p.x2_at;
+        w2.p = wk + p.w2_at;
+        xz.plane = 2 * c.M * p.ldk;
+        w2.plane = 2 * c.V * p.ldk;
+        if ((e = ce_copy<3>(p, c, c.target, xz.p, w2.p, s)) != hipSuccess) return e;
+    } else if (gw && !p.pad) {
         xz.p = wk + p.x_at;
         a.xz = wk + p.x_at;
     }
@@ -1034,21 +1073,22 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         a.dz_plane = c.M * a.ldz;
         const TileForm form = tile_form(c.M, n);
         int col_rows = 0;
-        e = p.es == 4              ? tile_dispatch(form, DzGo<MmaF32, RPFQ_F32>{a, col_rows, s})
-            : c.dtype == RPFQ_F16  ? tile_dispatch(form, DzGo<MmaF16, RPFQ_F16>{a, col_rows, s})
-            : c.dtype == RPFQ_BF16 ? tile_dispatch(form, DzGo<MmaBf16, RPFQ_BF16>{a, col_rows, s})
-                                   : tile_dispatch(form, DzGo<MmaBf16, RPFQ_F32>{a, col_rows, s});
+        e = p.terms == 1          ? tile_dispatch(form, DzGo<MmaF32, RPFQ_F32>{a, col_rows, s})
+            : p.terms == 3        ? tile_dispatch(form, DzGo<MmaBf16, RPFQ_F32>{a, col_rows, s})
+            : p.wide              ? tile_dispatch(form, DzGo<MmaF16, RPFQ_BF16>{a, col_rows, s})
+            : c.dtype == RPFQ_F16 ? tile_dispatch(form, DzGo<MmaF16, RPFQ_F16>{a, col_rows, s})
+                                  : tile_dispatch(form, DzGo<MmaBf16, RPFQ_BF16>{a, col_rows, s});
         if (e != hipSuccess) return e;
         a.xz = nullptr;  // written with the first piece
         const TileOperand dzk = {a.dz, a.ldz, a.dz_plane, c.M}, dzt = {a.dz, a.ldz, a.dz_plane, n};
         CeGrads both = {};
         CeGrad &dx = both.g[0], &dw = both.g[1];
-        dx.pairs = dw.pairs = ce_pairs(p.terms);
+        dx.pairs = dw.pairs = ce_pairs(p);
         dx.N = dw.N = c.D;
         dx.ldp = dw.ldp = p.ldp;
         dx.factor = dw.factor = factor;
         dx.r = dzk;
-        dx.c = {a.w.p, w.ld, w.plane, p.ldk};
+        dx.c = {w2.p + v0 * w2.ld, w2.ld, w2.plane, p.ldk};
         dx.rk = p.es * a.n8;
         dx.ck = n;
         dx.M = c.M;
@@ -1065,7 +1105,7 @@ hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float
         dw.part = p.grad.dw > 1 ? reinterpret_cast<float*>(wk + p.dw_at) : nullptr;
         dw.out = gw ? reinterpret_cast<char*>(gw) + v0 * c.D * es : nullptr;
         dw.vec = c.D % 4 == 0 && reinterpret_cast<uintptr_t>(dw.out) % (4 * es) == 0;
-        if ((gx || gw) && (e = ce_grads(c.dtype, p.es == 4, p.grad.form, both, s)) != hipSuccess) return e;
+        if ((gx || gw) && (e = ce_grads(c.dtype, p, both, s)) != hipSuccess) return e;
         CeSums sums = {{}, factor};
         int jobs = 0, blocks = 0;
         auto add = [&](const CeSum& j) {

@@ -410,10 +410,10 @@ struct CeSplit {
 struct CePlan {
     int es, planes, terms;  // bytes of an operand's element, planes of x and w (bf16 terms of a float32), of dz
     int64_t ldk, ldp;       // elements of a row of k; of float32 partials
-    bool pad;               // x and w are copied (rows of ldk, or three planes of them)
+    bool pad, wide;         // x and w are copied (rows of ldk, or three planes of them); fp16 with dz in bf16
     int64_t tiles_v, piece, pieces;
     CeSplit grad;
-    size_t x_at, w_at, part_at, zsum_at, zt_at, rows_at, rho_at, factor_at, dz_at, col_at, dx_at, dw_at, bytes;
+    size_t x_at, w_at, part_at, zsum_at, zt_at, rows_at, rho_at, factor_at, dz_at, col_at, dx_at, dw_at, x2_at, w2_at, bytes;
 };
 CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool backward);
 hipError_t launch_linear_ce(const CeCall& c, float* loss, float* stat, float* coef, void* work, hipStream_t s);

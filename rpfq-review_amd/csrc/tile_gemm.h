@@ -67,10 +67,14 @@ struct TileOperand {
 // the nine products the six above 2^-24, smallest first.  The terms keep
 // float32's exponents, so no scales are needed; 6 x the cost of one.
 constexpr int kPairs32 = 6;
-__device__ __forceinline__ void tile_pair(int pair, int& r, int& c) {
+// fp16 products as bf16 ones, where the other operand's exponents pass fp16's: a
+// fp16 is two bf16 terms exactly, the other side two terms of its own; (l,h)
+// (h,l) (h,h), without the one below 2^-16.
+constexpr int kPairsHalf = 3;
+__device__ __forceinline__ void tile_pair(int pairs, int pair, int& r, int& c) {
     // (l,h) (h,l) (m,m) (m,h) (h,m) (h,h); planes h = 0, m = 1, l = 2
-    r = (0x001102 >> (4 * pair)) & 3;
-    c = (0x010120 >> (4 * pair)) & 3;
+    r = ((pairs == kPairs32 ? 0x001102 : 0x001) >> (4 * pair)) & 3;
+    c = ((pairs == kPairs32 ? 0x010120 : 0x010) >> (4 * pair)) & 3;
 }
 
 // LDS DMA through a buffer resource: lanes with an offset past its end write
@@ -201,8 +205,8 @@ struct TileGemm {
     static constexpr int64_t steps(int64_t k) { return (k + R::PER - 1) / R::PER; }
 
     // Adds steps s0 .. s1 - 1 of the product; a step is KB bytes of k of one
-    // pair of planes, `per` steps a pair.  pairs: 1, kPairs32 of two operands of
-    // three planes, or R's planes, the last (smallest) first.  rk, ck: k of the
+    // pair of planes, `per` steps a pair.  pairs: those of tile_pair, or R's
+    // planes, 1 or 2, beside one of C, the second first.  rk, ck: k of the
     // operands as issue() takes it.  meanwhile(): what the epilogue wants in LDS
     // past the stages, loaded while the first steps are on their way (s0 < s1).
     template <class F>
@@ -218,7 +222,7 @@ struct TileGemm {
         int pair = s0 / per, ks = s0 - pair * per;
         auto issue = [&](int st) {
             int rp = pairs - 1 - pair, cp = 0;
-            if (pairs == kPairs32) tile_pair(pair, rp, cp);
+            if (pairs >= kPairsHalf) tile_pair(pairs, pair, rp, cp);
             rs.issue(ks, rp, rk, lds + st * STAGE, wave);
             cs.issue(ks, cp, ck, lds + st * STAGE + R::BYTES, wave);
             if (++ks == per) {

@@ -75,3 +75,33 @@ def test_rows_beside_an_infinite_upstream_gradient(m, dtype, bad):
     # a row without a label keeps its gradient to itself, whatever it is
     t[3] = -100
     assert all(torch.equal(a, e) for a, e in zip(run(with_bad), run(without)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,v,d", [(60, 5000, 64), (60, 301, 61), (400, 5000, 64), (400, 301, 61)])
+def test_rows_far_below_the_largest_upstream_gradient(m, v, d, dtype):
+    """grad_x of rows 2^-25 of the largest's gradient is as exact as theirs."""
+    from quant_models import ops
+
+    x, w, t, b = base._inputs(m, v, d, dtype, True, 0.1)
+    up = torch.logspace(16, -9, m, base=2.0, device=DEV)
+    xs = x.clone().requires_grad_()
+    (got,) = torch.autograd.grad(ops.linear_cross_entropy(xs, w, t, b, reduction="none"), xs, up)
+    xd, wd = x.double(), w.double()
+    z = xd @ wd.t() + b.double()
+    p = torch.softmax(z, 1)
+    q = torch.zeros_like(p)
+    valid = t != -100
+    q[valid, t[valid]] = 1.0
+    dz = torch.where(valid, up.double(), 0.0)[:, None] * (p - q)
+    zerr = (d + 2) * 2.0 ** -24 * (xd.abs() @ wd.abs().t() + b.double().abs()).amax(1)
+    # p's own error, dz's two bf16 terms (2^-16; fp16: and the second terms' product,
+    # 2^-8 of dz times 2^-8 of w), float32 sums of up to six products a class
+    perr = torch.where(valid, up.double(), 0.0)[:, None] * p * (3 * zerr + 2.0 ** -20 * 10)[:, None]
+    size = perr + dz.abs() * ({torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -15, torch.float32: 2.0 ** -22}[dtype] + 6 * v * 2.0 ** -24)
+    want = dz @ wd
+    # fp16's own steps end at 2^-24
+    bound = base.HALF[dtype] * want.abs() + 1.01 * size @ wd.abs() + (2.0 ** -25 if dtype == torch.float16 else 0)
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), (off / bound).amax(1)
