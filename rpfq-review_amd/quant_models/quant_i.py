@@ -835,8 +835,12 @@ class QATLinearComplexPhase(nn.Linear):
         rpfq_layer_norm_act_quant); only valid when packed_act_bits(x) > 0."""
         return self._packed_forward(x, prequantized=True)
 
+    def runs_packed(self, x: torch.Tensor) -> bool:
+        """forward(x) takes the packed path: in eval, on the device."""
+        return x.is_cuda and not self.training and self.use_packed
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if x.is_cuda and not self.training and self.use_packed:
+        if self.runs_packed(x):
             return self._packed_forward(x)
         return self._qat_forward(x)
 

@@ -22,6 +22,9 @@ def head_operands(layer: nn.Module, x: torch.Tensor):
     phase-quantized layer's activations and weight as its training forward
     quantizes them (straight-through gradients), nn.Linear's as they are."""
     if isinstance(layer, QATLinearComplexPhase):
+        if layer._override is not None and layer.runs_packed(x):
+            raise ValueError("classifier_loss: the head runs from supplied codes, not from its float weight; "
+                             "take F.cross_entropy(model(images), labels)")
         return layer.training_operands(x)
     if type(layer) is not nn.Linear:
         raise TypeError(f"classifier_loss takes a linear head, got {type(layer).__name__}")
@@ -35,7 +38,9 @@ def classifier_loss(model: nn.Module, images: torch.Tensor, labels: torch.Tensor
     model's features, then ops.linear_cross_entropy with the head's weight.
     A distilled DeiT's two heads are averaged, as its eval output is; in
     distilled training the model returns two outputs, which this does not
-    take."""
+    take.  In eval, where a head runs packed, its weight is quantized as in
+    training: the same codes and scales.  A head that runs from supplied codes
+    (load_packed) is refused."""
     from . import ops
 
     if isinstance(model, VisionTransformerDistilled):
