@@ -198,9 +198,10 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As torch's, but the states keep their types (codes stay codes,
-        moments float32), and parameters of one group, type and count share it
-        again.  Takes what torch.optim.AdamW saved, states of 32 bits, but for
-        its amsgrad and maximize."""
+        moments are float32), and parameters of one group, type and count share
+        it again.  Takes what torch.optim.AdamW saved (its moments of fp16 and
+        bf16 parameters, kept in their type, as float32), but for its amsgrad and
+        maximize."""
         for group in state_dict["param_groups"]:
             if group.get("amsgrad") or group.get("maximize"):
                 raise ValueError("AdamW has neither amsgrad nor maximize")
@@ -222,6 +223,8 @@ class AdamW(torch.optim.Optimizer):
                         counts[call] = torch.full((1,), at, dtype=torch.float32, device=p.device)
                     value = counts[call]
                 elif isinstance(value, torch.Tensor):
+                    if self.param_groups[k]["state_bits"] == 32:
+                        value = value.float()
                     moved = value.to(p.device)
                     value = torch.empty_strided(p.shape, p.stride(), dtype=value.dtype, device=p.device).copy_(moved) \
                         if value.shape == p.shape and name in ("exp_avg", "exp_avg_sq") else moved.clone()
