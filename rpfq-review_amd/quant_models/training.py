@@ -80,6 +80,11 @@ def _flat(t: torch.Tensor, what: str) -> torch.Tensor:
     return t.as_strided((t.numel(),), (1,))
 
 
+def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Two tensors of one shape have their elements in one order."""
+    return a.stride() == b.stride() or all(s == t for n, s, t in zip(a.shape, a.stride(), b.stride()) if n != 1)
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's step (decoupled weight decay) on the device kernel
     (ops.adamw): one launch per 60 tensors of a type.  state_bits 32: float32
@@ -90,7 +95,8 @@ class AdamW(torch.optim.Optimizer):
     into a graph once the states exist, for the parameters that the eager step
     before it took; torch.amp.GradScaler's scale and its
     skipped steps are taken on the device too.  state_dict() and
-    load_state_dict() keep the states' types."""
+    load_state_dict() keep the states' types.  Moments of 32 bits follow a change
+    of their parameter's memory order; with 8 bits it is refused."""
 
     _step_supports_amp_scaling = True
 
@@ -175,6 +181,7 @@ class AdamW(torch.optim.Optimizer):
                 g = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
             lists["params"].append(_flat(p, "a parameter"))
             lists["grads"].append(_flat(g, "a gradient"))
+            self._follow(p, state, group["state_bits"])
             lists["exp_avgs"].append(_flat(state["exp_avg"], "a state"))
             lists["exp_avg_sqs"].append(_flat(state["exp_avg_sq"], "a state"))
             if group["state_bits"] == 8:
@@ -185,6 +192,20 @@ class AdamW(torch.optim.Optimizer):
         ops.adamw(step=step, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                   grad_scale=there[0], found_inf=there[1], **lists)
 
+    @staticmethod
+    def _follow(p, state, bits):
+        """Lays the moments out as p, whose memory order may have changed since
+        (model.to(memory_format=...))."""
+        moved = [k for k in ("exp_avg", "exp_avg_sq") if not _same_order(state[k], p)]
+        if not moved:
+            return
+        if bits == 8:
+            raise ValueError("AdamW: a parameter's memory order is not the one its 8-bit state was made in, whose blocks follow it")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a parameter's memory order has changed: take a step eagerly before one is captured")
+        for k in moved:
+            state[k] = torch.empty_strided(p.shape, p.stride(), dtype=state[k].dtype, device=p.device).copy_(state[k])
+
     def state_values(self, p: torch.Tensor):
         """(first, second) moment of a parameter as float32 tensors."""
         from . import ops
@@ -194,7 +215,7 @@ class AdamW(torch.optim.Optimizer):
             return state["exp_avg"], state["exp_avg_sq"]
         flat = [_flat(state[k], "a state").reshape(-1) for k in ("exp_avg", "exp_avg_sq")]
         values = ops.adamw_state_values(flat, [state["exp_avg_scale"], state["exp_avg_sq_scale"]])
-        return tuple(v.as_strided(p.shape, p.stride()) for v in values)
+        return tuple(v.as_strided(p.shape, state[k].stride()) for v, k in zip(values, ("exp_avg", "exp_avg_sq")))
 
     def load_state_dict(self, state_dict) -> None:
         """As torch's, but the states keep their types (codes stay codes,
@@ -205,13 +226,17 @@ class AdamW(torch.optim.Optimizer):
         for group in state_dict["param_groups"]:
             if group.get("amsgrad") or group.get("maximize"):
                 raise ValueError("AdamW has neither amsgrad nor maximize")
+        saved = [(i, g.get("state_bits", 32)) for g in state_dict["param_groups"] for i in g["params"]]
+        for (i, bits), p in zip(saved, (p for g in self.param_groups for p in g["params"])):
+            codes = state_dict["state"].get(i, {}).get("exp_avg")
+            if bits == 8 and codes is not None and codes.shape == p.shape and not _same_order(codes, p):
+                raise ValueError("AdamW: an 8-bit state was saved of a parameter in another memory order, which its blocks follow")
         super().load_state_dict(state_dict)
         for group in self.param_groups:
             group.setdefault("state_bits", 32)
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [(k, p) for k, g in enumerate(self.param_groups) for p in g["params"]]
         counts = {}
-        for i, (k, p) in zip(saved, params):
+        for (i, _), (k, p) in zip(saved, params):
             source = state_dict["state"].get(i)
             if not source:
                 continue
