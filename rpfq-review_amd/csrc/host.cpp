@@ -510,7 +510,12 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (code < 0 || scalar[0]->is_inference()) Py_RETURN_NONE;
     std::vector<rpfq_adamw_tensor> table(count);
     std::vector<std::pair<const char*, const char*>> seen;  // what the step writes
-    seen.reserve(3 * count);
+    seen.reserve(5 * count + 1);
+    auto writes = [&](const void* at, int64_t bytes) {
+        const char* c = reinterpret_cast<const char*>(at);
+        if (bytes) seen.emplace_back(c, c + bytes);
+    };
+    writes(scalar[0]->data_ptr(), 4);
     const int64_t es = p[0]->element_size(), ss = small ? 1 : 4;
     for (size_t i = 0; i < count; ++i) {
         const int64_t size = p[i]->numel();
@@ -526,11 +531,9 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 if (s->scalar_type() != at::kFloat || s->numel() != (size + 255) / 256 || s->device() != device) Py_RETURN_NONE;
             t.exp_avg_scale = sm[i]->data_ptr<float>();
             t.exp_avg_sq_scale = sv[i]->data_ptr<float>();
+            writes(t.exp_avg_scale, (size + 255) / 256 * 4);
+            writes(t.exp_avg_sq_scale, (size + 255) / 256 * 4);
         }
-        auto writes = [&](const void* at, int64_t bytes) {
-            const char* c = reinterpret_cast<const char*>(at);
-            if (bytes) seen.emplace_back(c, c + bytes);
-        };
         writes(t.param, size * es);
         writes(t.exp_avg, size * ss);
         writes(t.exp_avg_sq, size * ss);
@@ -538,6 +541,11 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     std::sort(seen.begin(), seen.end());
     for (size_t i = 1; i < seen.size(); ++i)
         if (seen[i].first < seen[i - 1].second) Py_RETURN_NONE;
+    for (const rpfq_adamw_tensor& t : table) {  // gradients may share memory with each other only
+        const char *first = reinterpret_cast<const char*>(t.grad), *last = first + t.numel * es;
+        const auto next = std::lower_bound(seen.begin(), seen.end(), std::make_pair(last, last));
+        if (first < last && next != seen.begin() && std::prev(next)->second > first) Py_RETURN_NONE;
+    }
     int rc;
     {
         Unlocked u;

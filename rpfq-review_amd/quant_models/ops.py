@@ -5,6 +5,7 @@ raises if the library is unavailable or a tensor is on the host.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
 import math
 from dataclasses import dataclass, field
@@ -1046,8 +1047,8 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, step: torch.Tensor, *, lr=1e-3, 
     a number, or a float32 device tensor that is read when the step runs.
     grad_scale, found_inf: float32 device scalars, as torch.amp.GradScaler
     passes them: gradients are divided by the one, a nonzero other leaves
-    parameters, states and step as they are.  Parameters or states that overlap
-    are refused."""
+    parameters, states and step as they are.  Parameters or states (scales and
+    step among them) that overlap each other or a gradient are refused."""
     params, grads, ms, vs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     n = len(params)
     small = exp_avg_scales is not None
@@ -1094,10 +1095,16 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, step: torch.Tensor, *, lr=1e-3, 
                     raise ValueError(f"tensor {i}: scales must be contiguous float32, one per {STATE_BLOCK} elements")
             a, b = sm[i].data_ptr(), sv[i].data_ptr()
         flat += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), a, b, size)
-    seen = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
-                  for i in range(n) for t in (params[i], ms[i], vs[i]) if t.numel())
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
+    seen = sorted(span(t) for t in [step] + params + ms + vs + sm + sv if t.numel())
     if any(b[0] < a[1] for a, b in zip(seen, seen[1:])):
         raise ValueError("adamw: a parameter or state is there twice, or two overlap")
+    for first, last in (span(g) for g in grads if g.numel()):
+        at = bisect.bisect_left(seen, (last, last))
+        if at and seen[at - 1][1] > first:
+            raise ValueError("adamw: a gradient overlaps a parameter or state")
     hyper = N.AdamWHyper(0.0 if lr_dev is not None else float(lr), float(betas[0]), float(betas[1]), float(eps),
                          float(weight_decay))
     work = torch.empty(8, dtype=torch.float32, device=device)
