@@ -909,10 +909,12 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         return y
     x2 = _aligned_rows(x.reshape(-1, k))
     m = x2.shape[0]
-    # rows are read in whole 16 bytes: the last one's too have to be there
-    end = weight.storage_offset() + (n - 1) * weight.stride(0) + -(-k // 16) * 16
-    if weight.stride(1) != 1 and k > 1 or weight.stride(0) < k or end > weight.untyped_storage().nbytes():
-        weight = weight.contiguous()
+    # rows are read in whole 16 bytes: the last one's too have to be there (rows
+    # of exactly K that do not fill them are copied by the library)
+    whole = -(-k // 16) * 16
+    past = weight.storage_offset() + (n - 1) * weight.stride(0) + whole > weight.untyped_storage().nbytes()
+    if weight.stride(1) != 1 and k > 1 or weight.stride(0) < k or weight.stride(0) >= whole and past:
+        weight = weight.clone(memory_format=torch.contiguous_format)  # contiguous() keeps a single row as it is
     weight_scale = weight_scale.contiguous()
     bias = None if bias is None else bias.detach().float().contiguous()
     x_scale = None if x_scale is None else x_scale.contiguous()
