@@ -291,6 +291,7 @@ PyObject* linear_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Py_RETURN_NONE;
     const int64_t out = w->size(0), k = w->size(1), m = x->numel() / k;
     const int64_t ld = out > 1 ? w->stride(0) : std::max(k, w->stride(0));
+    if (ld > 1 << 20) Py_RETURN_NONE;  // rows further apart than the library takes are copied
     // rows are read in whole 16 bytes: the last one's too have to be there (rows
     // of exactly K that do not fill them are copied by the library)
     if (ld >= (k + 15) / 16 * 16 &&

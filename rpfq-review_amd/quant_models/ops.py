@@ -913,7 +913,7 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     # of exactly K that do not fill them are copied by the library)
     whole = -(-k // 16) * 16
     past = weight.storage_offset() + (n - 1) * weight.stride(0) + whole > weight.untyped_storage().nbytes()
-    if weight.stride(1) != 1 and k > 1 or weight.stride(0) < k or weight.stride(0) >= whole and past:
+    if weight.stride(1) != 1 and k > 1 or not k <= weight.stride(0) <= 1 << 20 or weight.stride(0) >= whole and past:
         weight = weight.clone(memory_format=torch.contiguous_format)  # contiguous() keeps a single row as it is
     weight_scale = weight_scale.contiguous()
     bias = None if bias is None else bias.detach().float().contiguous()
