@@ -54,16 +54,22 @@ def to_int8(model: nn.Module, skip=()) -> int:
     """Replace every linear layer of `model` (nn.Linear and phase-quantized
     ones, from their float weights) by its 8-bit baseline Int8Linear, but those
     named in `skip` (names of named_modules(); a name covers what is below
-    it).  For inference; returns the number of layers."""
-    edges = []
+    it).  Other subclasses of nn.Linear, whose forward is their own, stay; a
+    layer that runs from supplied codes is refused, and the model then left as
+    it was.  A layer in several places is one layer afterwards too.  For
+    inference; returns the number of layers."""
+    edges, made = [], {}
     for name, parent in model.named_modules():
-        for child_name, child in parent.named_children():
+        for child_name, child in parent._modules.items():
             full = f"{name}.{child_name}" if name else child_name
-            if isinstance(child, nn.Linear) and not any(full == s or full.startswith(s + ".") for s in skip):
+            if type(child) in (nn.Linear, QATLinearComplexPhase) and not any(full == s or full.startswith(s + ".") for s in skip):
                 edges.append((parent, child_name, child))
+    for _, _, child in edges:
+        if id(child) not in made:
+            made[id(child)] = Int8Linear.from_linear(child)
     for parent, name, child in edges:
-        setattr(parent, name, Int8Linear.from_linear(child))
-    return len(edges)
+        setattr(parent, name, made[id(child)])
+    return len(made)
 
 
 def packed_code_bytes(model: nn.Module) -> int:
