@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/rpfq.h"
@@ -361,19 +362,35 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
         return out;
     }
 
-    // Under capture: whether the engine would next add to a leaf on the default
-    // stream, where an eager graph that is still alive has bound it; joining that
-    // stream to the capture ends the process, not the call.
+    // Under capture: whether the engine, here or further on, would hand a gradient
+    // to a leaf on the default stream, where an eager graph that is still alive has
+    // bound it; joining that stream to the capture ends the process, not the call.
+    // grad() hands it over too, before it takes it out.
     static bool leaves_capture() {
         if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return false;
-        const auto* inputs = torch::autograd::get_current_graph_task_exec_info();
-        const auto node = torch::autograd::get_current_node();
-        if (!node || (inputs && !inputs->empty())) return false;  // autograd.grad adds to no leaf
-        for (const auto& edge : node->next_edges())
-            if (dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) {
-                const auto s = edge.function->stream();
+        const auto* only = torch::autograd::get_current_graph_task_exec_info();  // not empty: of grad() and backward(inputs=)
+        const auto here = torch::autograd::get_current_node();
+        if (!here) return false;
+        std::vector<torch::autograd::Node*> todo{here.get()};
+        std::unordered_set<torch::autograd::Node*> seen;
+        while (!todo.empty()) {
+            const auto* node = todo.back();
+            todo.pop_back();
+            for (const auto& edge : node->next_edges()) {
+                auto* next = edge.function.get();
+                if (!next || !seen.insert(next).second) continue;
+                if (!dynamic_cast<torch::autograd::AccumulateGrad*>(next)) {
+                    todo.push_back(next);
+                    continue;
+                }
+                if (only && !only->empty()) {
+                    const auto found = only->find(next);
+                    if (found == only->end() || !found->second.should_execute()) continue;
+                }
+                const auto s = next->stream();
                 if (s && s->id() == 0) return true;  // the default stream
             }
+        }
         return false;
     }
 

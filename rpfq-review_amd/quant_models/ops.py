@@ -987,8 +987,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     Gradients of x, weight and bias, once differentiable; float32 sums in a
     fixed order, in which the gradient of 16-bit operands' logits takes part as
     two terms of their type (2^-16 of it is lost in bf16, 2^-22 in fp16, 2^-15
-    in fp16 with reduction "none").  Can be captured into a graph, backward too, where no eager
-    graph of the same leaves is alive."""
+    in fp16 with reduction "none").  Can be captured into a graph, backward too,
+    where no eager graph of the same leaves is alive: the native host path
+    refuses such a backward, without it torch ends the process."""
     host = N.host()
     if host is not None:
         loss = host.linear_cross_entropy(x, weight, target, bias, ignore_index, label_smoothing, N.REDUCTIONS.get(reduction))
