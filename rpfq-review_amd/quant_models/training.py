@@ -17,10 +17,18 @@ from .vision_transformer import VisionTransformer, VisionTransformerDistilled
 # ---------------------------------------------------------------------------
 # loss
 # ---------------------------------------------------------------------------
+def _no_hooks(module: nn.Module) -> None:
+    """Hooks of a forward that is not called would be left out, those that form
+    a weight (pruning, spectral norm) among them."""
+    if module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks:
+        raise ValueError(f"classifier_loss does not call {type(module).__name__}.forward, which has hooks")
+
+
 def head_operands(layer: nn.Module, x: torch.Tensor):
     """(x, weight, bias) whose linear map is layer(x) in training: a
     phase-quantized layer's activations and weight as its training forward
     quantizes them (straight-through gradients), nn.Linear's as they are."""
+    _no_hooks(layer)
     if isinstance(layer, QATLinearComplexPhase):
         if layer._override is not None and layer.runs_packed(x):
             raise ValueError("classifier_loss: the head runs from supplied codes, not from its float weight; "
@@ -40,9 +48,11 @@ def classifier_loss(model: nn.Module, images: torch.Tensor, labels: torch.Tensor
     distilled training the model returns two outputs, which this does not
     take.  In eval, where a head runs packed, its weight is quantized as in
     training: the same codes and scales.  A head that runs from supplied codes
-    (load_packed) is refused."""
+    (load_packed) is refused, and so are hooks on the model or its head, whose
+    forward is not called, and models wrapped in another module."""
     from . import ops
 
+    _no_hooks(model)
     if isinstance(model, VisionTransformerDistilled):
         if model.distilled_training and model.training:
             raise ValueError("classifier_loss: distilled training has a loss for each head")
@@ -56,6 +66,7 @@ def classifier_loss(model: nn.Module, images: torch.Tensor, labels: torch.Tensor
     elif isinstance(model, VisionTransformer):
         x, weight, bias = head_operands(model.head, model.forward_head(model.forward_features(images), pre_logits=True))
     elif isinstance(model, SwinTransformer):
+        _no_hooks(model.head)
         x, weight, bias = head_operands(model.head.fc, model.forward_features(images).mean(dim=(1, 2)))
     else:
         raise TypeError(f"classifier_loss takes a VisionTransformer or SwinTransformer, got {type(model).__name__}")

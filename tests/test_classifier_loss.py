@@ -54,3 +54,21 @@ def test_supplied_codes_are_refused_in_eval(name):
     for grad in (False, True):
         with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="supplied codes"):
             qm.classifier_loss(m, x, _labels())
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_hooks_are_refused(name):
+    """On the host: before anything is computed."""
+    import quant_models as qm
+
+    m = _model(name, device="cpu")
+    x, t = torch.randn(2, 3, 32, 32), torch.tensor([1, 2])
+    head = m.head.fc if "swin" in name else m.head
+    for module in (m, m.head, head):
+        for add in (module.register_forward_hook, module.register_forward_pre_hook, module.register_full_backward_hook):
+            handle = add(lambda *a: None)
+            with pytest.raises(ValueError, match="hooks"):
+                qm.classifier_loss(m, x, t)
+            handle.remove()
+    with pytest.raises(TypeError):
+        qm.classifier_loss(torch.nn.Sequential(m), x, t)
