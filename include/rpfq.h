@@ -687,7 +687,9 @@ typedef struct rpfq_ce_desc {
 
 /* Bytes of the device workspace of rpfq_linear_cross_entropy (backward = 0) or
  * its gradient (1): there a piece of the logits' gradient, at most about 1 GiB
- * whatever V is; 0 if the shape is not taken (M or V above 2^22, M V above
+ * whatever V is (or 256 classes of it, where M makes those more), float32 sums
+ * of grad_x where there are several, and copies of x and w where they do not
+ * lie as they are read; 0 if the shape is not taken (M or V above 2^22, M V above
  * 2^39, D above 2^16). */
 size_t rpfq_linear_cross_entropy_workspace_bytes(const rpfq_ce_desc* desc, int backward);
 

@@ -357,14 +357,12 @@ __global__ void __launch_bounds__(256) int8_few_kernel(Int8Few a) {
 // launches
 // ---------------------------------------------------------------------------
 static bool int8_few(int xdt, int64_t M, int64_t K) {
-    return xdt >= 0 && M <= 16 && M * int8_few_pitch(K) <= 140 * 1024 && M * K <= kInt8FewCodes;
+    return xdt >= 0 && M <= 16 && M * K <= kInt8FewCodes;
 }
 
 template <int XDT, int YDT>
 static hipError_t few_go(const Int8Few& a, hipStream_t s) {
-    static std::atomic<uint64_t> attr_done{0};
-    const hipError_t e = set_lds_attr_once(reinterpret_cast<const void*>(&int8_few_kernel<XDT, YDT>), 140 * 1024, attr_done);
-    if (e != hipSuccess) return e;
+    // at most kInt8FewCodes + 16 x 79 bytes
     hipLaunchKernelGGL((int8_few_kernel<XDT, YDT>), dim3((unsigned)((a.N + 15) / 16)), dim3(256), a.M * int8_few_pitch(a.K), s, a);
     return hipGetLastError();
 }
@@ -516,10 +514,10 @@ hipError_t launch_linear_int8(const void* x, int xdt, const float* sx, const int
     a.K = p.ld;
     const int es = ydt == RPFQ_F32 ? 4 : 2;
     a.vec = N % (16 / es) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
-    // an output larger than the 256-MB cache behind the L2 goes past both, which
-    // leaves them to the operands (50,432 x 4,096: 289 -> 277 us); a smaller one
-    // is what the next layer reads
-    if (a.vec && M * N * es > 256LL << 20) a.vec = 2;
+    // a 16-bit output larger than the 256-MB cache behind the L2 goes past both,
+    // which leaves them to the operands (50,432 x 4,096: 289 -> 277 us); a smaller
+    // one is what the next layer reads
+    if (a.vec && es == 2 && M * N * es > 256LL << 20) a.vec = 2;
     switch (ydt) {
         case RPFQ_F32: return gemm_y<RPFQ_F32>(a, s);
         case RPFQ_F16: return gemm_y<RPFQ_F16>(a, s);

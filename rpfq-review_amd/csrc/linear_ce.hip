@@ -815,7 +815,7 @@ constexpr int64_t kCeDirectRows = 256;
 // products of dz's terms with those of the other operand
 static int ce_pairs(const CePlan& p) { return p.terms == 3 ? kPairs32 : p.wide ? kPairsHalf : p.terms; }
 
-CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool backward) {
+CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool smooth, bool backward) {
     CePlan p = {};
     // fp16 rows with upstream gradients of their own: dz, whose rows may lie far
     // apart, in bf16 terms, and x and w in as many for its products.  Under one
@@ -841,7 +841,7 @@ CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool back
     p.tiles_v = (V + 255) / 256;
     if (!backward) {
         p.part_at = take(8 * p.tiles_v * M);
-        p.zsum_at = take(4 * p.tiles_v * M);
+        p.zsum_at = take(smooth ? 4 * p.tiles_v * M : 0);
         p.zt_at = take(4 * M);
         p.rows_at = take(reduction ? 4 * M : 0);
         return p;
@@ -998,7 +998,7 @@ static CeSum ce_sum(int dt, const float* part, int parts, int64_t stride, int64_
 }
 
 hipError_t launch_linear_ce(const CeCall& c, float* loss, float* stat, float* coef, void* work, hipStream_t s) {
-    const CePlan p = ce_plan(c.dtype, c.M, c.V, c.D, c.reduction, false);
+    const CePlan p = ce_plan(c.dtype, c.M, c.V, c.D, c.reduction, c.smooth > 0.0f, false);
     char* wk = reinterpret_cast<char*>(work);
     CeArgs a = {};
     hipError_t e = ce_operands(p, c, nullptr, wk, a, s);
@@ -1030,7 +1030,7 @@ hipError_t launch_linear_ce(const CeCall& c, float* loss, float* stat, float* co
 
 hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float* coef, const float* grad, void* gx, void* gw,
                                  void* gb, void* work, hipStream_t s) {
-    const CePlan p = ce_plan(c.dtype, c.M, c.V, c.D, c.reduction, true);
+    const CePlan p = ce_plan(c.dtype, c.M, c.V, c.D, c.reduction, c.smooth > 0.0f, true);
     char* wk = reinterpret_cast<char*>(work);
     const int es = c.dtype == RPFQ_F32 ? 4 : 2;
     CeArgs a = {};

@@ -802,7 +802,7 @@ int rpfq_linear_int8(const void* x, int x_dtype, const float* x_scale, const int
 
 size_t rpfq_linear_cross_entropy_workspace_bytes(const rpfq_ce_desc* d, int backward) {
     if (check_ce(d) != RPFQ_OK) return 0;
-    return rpfq::ce_plan(d->dtype, d->M, d->V, d->D, d->reduction, backward != 0).bytes;
+    return rpfq::ce_plan(d->dtype, d->M, d->V, d->D, d->reduction, d->smoothing > 0.0f, backward != 0).bytes;
 }
 
 int rpfq_linear_cross_entropy(const rpfq_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* target,

@@ -415,7 +415,7 @@ struct CePlan {
     CeSplit grad;
     size_t x_at, w_at, part_at, zsum_at, zt_at, rows_at, rho_at, factor_at, dz_at, col_at, dx_at, dw_at, x2_at, w2_at, bytes;
 };
-CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool backward);
+CePlan ce_plan(int dt, int64_t M, int64_t V, int64_t D, int reduction, bool smooth, bool backward);
 hipError_t launch_linear_ce(const CeCall& c, float* loss, float* stat, float* coef, void* work, hipStream_t s);
 hipError_t launch_linear_ce_grad(const CeCall& c, const float* stat, const float* coef, const float* grad, void* gx, void* gw,
                                  void* gb, void* work, hipStream_t s);

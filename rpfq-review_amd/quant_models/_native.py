@@ -142,10 +142,6 @@ class AdamWHyper(ctypes.Structure):
     _fields_ = [(name, ctypes.c_double) for name in ("lr", "beta1", "beta2", "eps", "weight_decay")]
 
 
-# fields of struct rpfq_adamw_tensor, all of 8 bytes
-ADAMW_FIELDS = 7
-
-
 class RPFQError(RuntimeError):
     """A C-ABI call returned a non-zero status."""
 

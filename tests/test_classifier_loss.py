@@ -72,3 +72,26 @@ def test_hooks_are_refused(name):
             handle.remove()
     with pytest.raises(TypeError):
         qm.classifier_loss(torch.nn.Sequential(m), x, t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", NAMES)
+def test_eval_loss_of_a_prepared_model(name):
+    """fp16 inference: the model rounds its logits and their loss to 2^-11, this
+    one the head's weight to 2^-11; both meet the same fp16 features."""
+    import quant_models as qm
+    from quant_models.inference import prepare_inference
+
+    m = _model(name)
+    heads = [h for n, h in m.named_modules() if n.startswith("head") and hasattr(h, "quantized_weight")]
+    with torch.no_grad():
+        off = max(float(h.quantized_weight().norm(dim=1).max()) * 1.5 * h.in_features ** 0.5 for h in heads)
+    prepare_inference(m, DEV, torch.float16)
+    x = torch.randn(6, 3, 32, 32, device=DEV, dtype=torch.float16)
+    with torch.no_grad():
+        z = m(x)
+        a, b = qm.classifier_loss(m, x, _labels()), F.cross_entropy(z, _labels())
+    # a logit: the weight's rounding and the packed rows', each 2^-11 |x| |w|, and
+    # its own; the loss: twice that, and its own rounding
+    bound = 2 * (2 * 2.0 ** -11 * off + 2.0 ** -11 * float(z.abs().max())) + 2.0 ** -11 * float(b)
+    assert abs(float(a) - float(b)) <= bound
