@@ -169,6 +169,7 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError("AdamW takes device parameters only")
                     if not self.state[p]:
                         self.state[p] = self._new_state(p, group["state_bits"], (k, p.dtype, p.device), fresh)
+                    self._follow(p, self.state[p], group["state_bits"])
                     calls[k, p.dtype, id(self.state[p]["step"])].append(p)
                 if p in self.state and self.state[p]:
                     users[id(self.state[p]["step"])] += 1
@@ -192,7 +193,6 @@ class AdamW(torch.optim.Optimizer):
                 g = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
             lists["params"].append(_flat(p, "a parameter"))
             lists["grads"].append(_flat(g, "a gradient"))
-            self._follow(p, state, group["state_bits"])
             lists["exp_avgs"].append(_flat(state["exp_avg"], "a state"))
             lists["exp_avg_sqs"].append(_flat(state["exp_avg_sq"], "a state"))
             if group["state_bits"] == 8:
@@ -210,6 +210,7 @@ class AdamW(torch.optim.Optimizer):
         moved = [k for k in ("exp_avg", "exp_avg_sq") if not _same_order(state[k], p)]
         if not moved:
             return
+        _flat(p, "a parameter")  # gaps are another matter
         if bits == 8:
             raise ValueError("AdamW: a parameter's memory order is not the one its 8-bit state was made in, whose blocks follow it")
         if torch.cuda.is_current_stream_capturing():

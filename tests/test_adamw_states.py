@@ -116,7 +116,8 @@ def test_8_bit_states_refuse_another_memory_order():
     import quant_models as qm
 
     a = _Conv(DEV)
-    opt = qm.AdamW(a.parameters(), lr=1e-2, state_bits=8)
+    # the parameter whose order changes is in the second group
+    opt = qm.AdamW([{"params": [a.b, a.point]}, {"params": [a.w]}], lr=1e-2, state_bits=8)
     for p in a.parameters():
         p.grad = torch.randn_like(p)
     opt.step()
@@ -129,7 +130,7 @@ def test_8_bit_states_refuse_another_memory_order():
         opt.step()
     assert all(torch.equal(p, q) for p, q in zip(a.parameters(), old))
     with pytest.raises(ValueError, match="memory order"):
-        qm.AdamW(a.parameters(), state_bits=8).load_state_dict(opt.state_dict())
+        qm.AdamW([{"params": [a.b, a.point]}, {"params": [a.w]}], state_bits=8).load_state_dict(opt.state_dict())
     a.to(memory_format=torch.contiguous_format)
     opt.step()
     assert all(float(opt.state[p]["step"]) == 2 for p in a.parameters())
