@@ -503,9 +503,10 @@ __device__ __forceinline__ float ce_lane_sums(float (&v)[32], int lane) {
 
 // dz of one piece of the classes.  DT: the type of dz's terms (float32: itself
 // beside float32 operands, three bf16 terms beside theirs).
-// The logits' product again and M V elements written: 8,192 x 65,536 x 768 bf16
-// 950 us, 870 TFLOP/s and 1.1 TB/s of dz; 2,048 x 20,000 x 1,024 fp16 114 us.  Stores
-// past the caches were slower where a piece of dz stays in them.
+// The logits' product again and dz's terms written: 8,192 x 65,536 x 768 bf16 1,320
+// us in two pieces, 625 TFLOP/s and 1.6 TB/s of dz; 2,048 x 20,000 x 1,024 fp16 146
+// us.  With one term 950 and 114.  Stores past the caches were slower where a
+// piece of dz stays in them.
 template <int MB, int WM, int S, int KB, class Mma, int DT>
 __global__ void __launch_bounds__(256 * WM, 2) ce_dz_kernel(CeArgs a) {
     extern __shared__ __align__(16) char smem[];
@@ -694,9 +695,10 @@ __device__ __forceinline__ void ce_grad_unit(const CeGrad& a, int bid, char* sme
 
 // Both products of a piece's dz in one launch: dx (dz in K layout, w in T) and dw
 // (dz and x in T), the longer units first and the others into their last round
-// (2,048 x 20,000 x 1,024 fp16: 1.2 and 1.0 rounds of the chip; 227 us in two
-// launches, 200 in one).  8,192 x 65,536 x 768 bf16 1,490 us, 1,107 TFLOP/s (library
-// products of the same shapes: 1,700 us).
+// (2,048 x 20,000 x 1,024 fp16, one term: 1.2 and 1.0 rounds of the chip; 227 us in
+// two launches, 200 in one; 380 with two terms).  8,192 x 65,536 x 768 bf16, two
+// terms, 2,980 us in two pieces, 1,107 TFLOP/s (library products of the same
+// shapes, one term: 1,700 us).
 struct CeGrads {
     CeGrad g[2];   // dx, dw; splits = 0: not wanted
     int units[2];
