@@ -93,7 +93,7 @@ def _flat(t: torch.Tensor, what: str) -> torch.Tensor:
 
 def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Two tensors of one shape have their elements in one order."""
-    return a.stride() == b.stride() or all(s == t for n, s, t in zip(a.shape, a.stride(), b.stride()) if n != 1)
+    return all(s == t for n, s, t in zip(a.shape, a.stride(), b.stride()) if n != 1)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -161,34 +161,37 @@ class AdamW(torch.optim.Optimizer):
         # all parameters of a count
         calls, users, fresh = defaultdict(list), defaultdict(int), {}
         for k, group in enumerate(self.param_groups):
+            bits = group["state_bits"]
             for p in group["params"]:
-                if p.grad is not None:
-                    if p.grad.is_sparse:
+                state, g = self.state.get(p), p.grad
+                if g is not None:
+                    if g.is_sparse:
                         raise RuntimeError("AdamW does not take sparse gradients")
                     if not p.is_cuda:
                         raise ValueError("AdamW takes device parameters only")
-                    if not self.state[p]:
-                        self.state[p] = self._new_state(p, group["state_bits"], (k, p.dtype, p.device), fresh)
-                    self._follow(p, self.state[p], group["state_bits"])
-                    calls[k, p.dtype, id(self.state[p]["step"])].append(p)
-                if p in self.state and self.state[p]:
-                    users[id(self.state[p]["step"])] += 1
-        for (k, _, count), params in calls.items():
-            step = self.state[params[0]]["step"]
-            if len(params) < users[count]:  # a count belongs to one call: these take a copy
+                    if not state:
+                        state = self.state[p] = self._new_state(p, bits, (k, p.dtype, p.device), fresh)
+                    lies = p.stride()
+                    if state["exp_avg"].stride() != lies or state["exp_avg_sq"].stride() != lies:
+                        self._follow(p, state, bits)
+                    calls[k, p.dtype, id(state["step"])].append((p, state, g))
+                if state:
+                    users[id(state["step"])] += 1
+        for (k, _, count), taken in calls.items():
+            step = taken[0][1]["step"]
+            if len(taken) < users[count]:  # a count belongs to one call: these take a copy
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("AdamW: a captured step takes the parameters that the step before it took")
-                users[count] -= len(params)
+                users[count] -= len(taken)
                 step = step.clone()
-                for p in params:
-                    self.state[p]["step"] = step
-            self._launch(ops, params, step, self.param_groups[k], grad_scale, found_inf)
+                for _, state, _ in taken:
+                    state["step"] = step
+            self._launch(ops, taken, step, self.param_groups[k], grad_scale, found_inf)
         return loss
 
-    def _launch(self, ops, params, step, group, grad_scale, found_inf):
+    def _launch(self, ops, taken, step, group, grad_scale, found_inf):
         lists = defaultdict(list)
-        for p in params:
-            state, g = self.state[p], p.grad
+        for p, state, g in taken:
             if g.stride() != p.stride():
                 g = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
             lists["params"].append(_flat(p, "a parameter"))
@@ -198,7 +201,7 @@ class AdamW(torch.optim.Optimizer):
             if group["state_bits"] == 8:
                 lists["exp_avg_scales"].append(state["exp_avg_scale"])
                 lists["exp_avg_sq_scales"].append(state["exp_avg_sq_scale"])
-        device = params[0].device
+        device = step.device
         there = [None if t is None else t.to(device=device, dtype=torch.float32) for t in (grad_scale, found_inf)]
         ops.adamw(step=step, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                   grad_scale=there[0], found_inf=there[1], **lists)
