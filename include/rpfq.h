@@ -763,6 +763,44 @@ int rpfq_adamw_state_values(const void* const* codes, const float* const* scales
                             float* const* out, int64_t count, void* stream);
 
 /*
+ * Root-mean-square norm of rows, with the residual's addition in front of it:
+ *   h = x + residual (rounded to dtype; x itself where residual is NULL),
+ *   y = h / sqrt(mean(h^2) + eps) * weight, rounded once to dtype.
+ * x, residual, y, h [M, C] of dtype; weight [C] of weight_dtype or NULL (ones).
+ * h: NULL without a residual.  rstd [M] (out, or NULL: not wanted): the factor
+ * 1 / sqrt(..) of each row, which the gradient needs.  float32 statistics.
+ * C <= 16384, any alignment of the elements; eps > 0.  No counterpart in the
+ * reference, whose blocks normalize by nn.LayerNorm.
+ */
+int rpfq_rms_norm(const void* x, const void* residual, int dtype, int64_t M, int64_t C, const void* weight,
+                  int weight_dtype, float eps, void* y, void* h, float* rstd, void* stream);
+
+/*
+ * The same with its output in 8 bits, as rpfq_linear_int8 takes it (x_dtype =
+ * RPFQ_I8): codes [M, C] = rint(127 h w / max|h w|) of each row, ties to even, of
+ * the exact products, and scale [M] = max|y| / 127 of the unrounded y; 0 for a row
+ * of zeros, a row with inf or NaN has scale NaN and codes 0.
+ */
+int rpfq_rms_norm_int8(const void* x, const void* residual, int dtype, int64_t M, int64_t C, const void* weight,
+                       int weight_dtype, float eps, int8_t* codes, float* scale, void* h, void* stream);
+
+/* Bytes of the device workspace of rpfq_rms_norm_grad where grad_weight is
+ * wanted; 0 if the shape is not taken. */
+size_t rpfq_rms_norm_grad_workspace_bytes(int64_t M, int64_t C);
+
+/*
+ * Gradient of rpfq_rms_norm: with n = h rstd and g = grad_y weight,
+ *   grad_x = rstd (g - n mean(g n)) + grad_h,  grad_weight = sum over rows of grad_y n.
+ * h: what the forward normalized (its h, or x); grad_y, grad_h (NULL: none),
+ * grad_x [M, C] of dtype; grad_x is the residual's gradient too.  grad_weight [C]
+ * of weight_dtype (NULL: not wanted), float32 sums in a fixed order; work: its
+ * workspace, 256-byte aligned.
+ */
+int rpfq_rms_norm_grad(const void* grad_y, const void* grad_h, const void* h, int dtype, int64_t M, int64_t C,
+                       const void* weight, int weight_dtype, const float* rstd, void* grad_x, void* grad_weight,
+                       void* work, size_t work_bytes, void* stream);
+
+/*
  * rpfq_quantize_wide without a workspace argument and without any device
  * allocation: the float64 partials live in a static device array of this
  * library (64 KiB per GPU, held until the process ends), so the call makes

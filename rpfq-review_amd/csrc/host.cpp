@@ -20,6 +20,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <array>
+#include <cmath>
 #include <cstring>
 #include <unordered_set>
 #include <vector>
@@ -40,7 +42,8 @@ constexpr double kMostOps = 1.5e9;
     X(rpfq_layer_norm_wide_linear_fusable) X(rpfq_layer_norm_wide_linear) X(rpfq_act_quant_wide_linear) \
     X(rpfq_attention) X(rpfq_last_error) X(rpfq_linear_int8_workspace_bytes) X(rpfq_linear_int8)        \
     X(rpfq_linear_cross_entropy_workspace_bytes) X(rpfq_linear_cross_entropy)                           \
-    X(rpfq_linear_cross_entropy_grad) X(rpfq_adamw)
+    X(rpfq_linear_cross_entropy_grad) X(rpfq_adamw) X(rpfq_rms_norm) X(rpfq_rms_norm_int8)             \
+    X(rpfq_rms_norm_grad_workspace_bytes) X(rpfq_rms_norm_grad)
 struct Api {
 #define X(f) decltype(&::f) f;
     RPFQ_HOST_CALLS(X)
@@ -324,6 +327,59 @@ PyObject* linear_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// Under capture: whether the engine, here or further on, would hand a gradient
+// to a leaf on the default stream, where an eager graph that is still alive has
+// bound it; joining that stream to the capture ends the process, not the call.
+// grad() hands it over too, before it takes it out.
+bool leaves_capture() {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return false;
+    const auto* only = torch::autograd::get_current_graph_task_exec_info();  // not empty: of grad() and backward(inputs=)
+    const auto here = torch::autograd::get_current_node();
+    if (!here) return false;
+    std::vector<torch::autograd::Node*> todo{here.get()};
+    std::unordered_set<torch::autograd::Node*> seen;
+    while (!todo.empty()) {
+        const auto* node = todo.back();
+        todo.pop_back();
+        for (const auto& edge : node->next_edges()) {
+            auto* next = edge.function.get();
+            if (!next || !seen.insert(next).second) continue;
+            if (!dynamic_cast<torch::autograd::AccumulateGrad*>(next)) {
+                todo.push_back(next);
+                continue;
+            }
+            if (only && !only->empty()) {
+                const auto found = only->find(next);
+                if (found == only->end() || !found->second.should_execute()) continue;
+            }
+            const auto s = next->stream();
+            if (s && s->id() == 0) return true;  // the default stream
+        }
+    }
+    return false;
+}
+
+void refuse_capture(const char* name) {
+    TORCH_CHECK(!leaves_capture(), name, ": backward under capture while an eager graph of the same leaves is alive: let go of its "
+                "outputs first");
+}
+
+// The gradients of a backward: with create_graph ones that cannot be differentiated again.
+torch::autograd::variable_list once_differentiable(torch::autograd::variable_list out, const char* name) {
+    if (!at::GradMode::is_enabled()) return out;
+    auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " is differentiable once", (int)out.size());
+    torch::autograd::variable_list wrapped(out.size());
+    for (size_t i = 0; i < out.size(); ++i)
+        if (out[i].defined()) {
+            at::Tensor t = out[i].detach();
+            t.requires_grad_(true);
+            wrapped[i] = t;
+        }
+    return (*error)(std::move(wrapped));
+}
+
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
 // The cross entropy of a classifier under autograd, as ops._LinearCrossEntropy.
 struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     static rpfq_ce_desc describe(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, int64_t ignore,
@@ -331,8 +387,6 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
         return {x.size(0), w.size(0), x.size(1), ignore, dtype_code(x.scalar_type()),
                 bias.defined() ? dtype_code(bias.scalar_type()) : RPFQ_F32, (int32_t)reduction, (float)smoothing};
     }
-    static void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-
     // (loss, stat)
     static std::pair<at::Tensor, at::Tensor> loss(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target,
                                                   const at::Tensor& bias, const rpfq_ce_desc& d) {
@@ -362,41 +416,8 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
         return out;
     }
 
-    // Under capture: whether the engine, here or further on, would hand a gradient
-    // to a leaf on the default stream, where an eager graph that is still alive has
-    // bound it; joining that stream to the capture ends the process, not the call.
-    // grad() hands it over too, before it takes it out.
-    static bool leaves_capture() {
-        if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return false;
-        const auto* only = torch::autograd::get_current_graph_task_exec_info();  // not empty: of grad() and backward(inputs=)
-        const auto here = torch::autograd::get_current_node();
-        if (!here) return false;
-        std::vector<torch::autograd::Node*> todo{here.get()};
-        std::unordered_set<torch::autograd::Node*> seen;
-        while (!todo.empty()) {
-            const auto* node = todo.back();
-            todo.pop_back();
-            for (const auto& edge : node->next_edges()) {
-                auto* next = edge.function.get();
-                if (!next || !seen.insert(next).second) continue;
-                if (!dynamic_cast<torch::autograd::AccumulateGrad*>(next)) {
-                    todo.push_back(next);
-                    continue;
-                }
-                if (only && !only->empty()) {
-                    const auto found = only->find(next);
-                    if (found == only->end() || !found->second.should_execute()) continue;
-                }
-                const auto s = next->stream();
-                if (s && s->id() == 0) return true;  // the default stream
-            }
-        }
-        return false;
-    }
-
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-        TORCH_CHECK(!leaves_capture(), "linear_cross_entropy: backward under capture while an eager graph of the same leaves is "
-                    "alive: let go of its outputs first");
+        refuse_capture("linear_cross_entropy");
         const auto saved = ctx->get_saved_variables();
         const at::Tensor &x = saved[0], &w = saved[1], &target = saved[2], &bias = saved[3], &stat = saved[4];
         const c10::DeviceGuard guard(x.device());
@@ -423,19 +444,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
         out[0] = gx;
         out[1] = gw;
         out[3] = gb;
-        if (at::GradMode::is_enabled()) {  // create_graph: these gradients cannot be differentiated again
-            auto error = std::make_shared<torch::autograd::DelayedError>(
-                "linear_cross_entropy is differentiable once", (int)out.size());
-            torch::autograd::variable_list wrapped(out.size());
-            for (size_t i = 0; i < out.size(); ++i)
-                if (out[i].defined()) {
-                    at::Tensor t = out[i].detach();
-                    t.requires_grad_(true);
-                    wrapped[i] = t;
-                }
-            return (*error)(std::move(wrapped));
-        }
-        return out;
+        return once_differentiable(std::move(out), "linear_cross_entropy");
     }
 };
 
@@ -474,6 +483,155 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
             y = CrossEntropy::loss(*x, *w, *t, bias, d).first;
     }
     return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// None (undefined), or a plain tensor of a type and the sizes given.
+bool operand(PyObject* o, at::Tensor* t) {
+    if (o == Py_None) return true;
+    const at::Tensor* p = plain(o);
+    if (!p || dtype_code(p->scalar_type()) < 0 || transformed(*p)) return false;
+    *t = *p;
+    return true;
+}
+
+// Root-mean-square norm under autograd: (x, residual, weight) -> (y[, h]).
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+    static int wdt(const at::Tensor& w) { return w.defined() ? dtype_code(w.scalar_type()) : RPFQ_F32; }
+
+    // y, h (undefined without a residual) and, where it is wanted, rstd
+    static std::array<at::Tensor, 3> norm(const at::Tensor& x, const at::Tensor& res, const at::Tensor& w, double eps, bool stat) {
+        const c10::DeviceGuard guard(x.device());
+        const int64_t c = x.size(-1), m = x.numel() / c;
+        std::array<at::Tensor, 3> out;
+        const auto options = x.options().requires_grad(false);
+        out[0] = at::empty(x.sizes(), options);
+        if (res.defined()) out[1] = at::empty(x.sizes(), options);
+        if (stat) out[2] = at::empty({m}, options.dtype(at::kFloat));
+        const int rc = api.rpfq_rms_norm(x.data_ptr(), ptr(res), dtype_code(x.scalar_type()), m, c, ptr(w), wdt(w), (float)eps,
+                                         out[0].data_ptr(), ptr(out[1]), stat ? out[2].data_ptr<float>() : nullptr, stream_on(x));
+        TORCH_CHECK(rc == RPFQ_OK, "rpfq_rms_norm: ", api.rpfq_last_error());
+        return out;
+    }
+
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                                                  const std::optional<at::Tensor>& res, const std::optional<at::Tensor>& w, double eps) {
+        const at::Tensor none;
+        const at::Tensor& weight = w ? *w : none;
+        auto out = norm(x, res ? *res : none, weight, eps, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({res ? out[1] : x, weight, out[2]});
+        ctx->saved_data["res"] = res.has_value();
+        if (!res) return {out[0]};
+        return {out[0], out[1]};
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        refuse_capture("rms_norm");
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &h = saved[0], &w = saved[1], &rstd = saved[2];
+        const bool res = ctx->saved_data["res"].toBool();  // needs_input_grad counts the tensors that were given
+        const c10::DeviceGuard guard(h.device());
+        torch::autograd::variable_list out(4);
+        {
+            const at::NoGradGuard plain_results;
+            const at::Tensor gh = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
+            at::Tensor gx, gw;
+            if (grads[0].defined()) {
+                const at::Tensor gy = grads[0].contiguous();
+                const int64_t c = h.size(-1), m = h.numel() / c;
+                gx = at::empty(h.sizes(), h.options().requires_grad(false));
+                at::Tensor work;
+                size_t bytes = 0;
+                if (w.defined() && ctx->needs_input_grad(1 + res)) {
+                    gw = at::empty(w.sizes(), w.options().requires_grad(false));
+                    bytes = api.rpfq_rms_norm_grad_workspace_bytes(m, c);
+                    work = at::empty({(int64_t)bytes}, h.options().dtype(at::kByte).requires_grad(false));
+                }
+                const int rc = api.rpfq_rms_norm_grad(gy.data_ptr(), ptr(gh), h.data_ptr(), dtype_code(h.scalar_type()), m, c, ptr(w),
+                                                      wdt(w), rstd.const_data_ptr<float>(), gx.data_ptr(), ptr(gw), ptr(work), bytes,
+                                                      stream_on(h));
+                TORCH_CHECK(rc == RPFQ_OK, "rpfq_rms_norm_grad: ", api.rpfq_last_error());
+            } else {
+                gx = gh;  // only the sum was used
+            }
+            if (ctx->needs_input_grad(0)) out[0] = gx;
+            if (res && ctx->needs_input_grad(1)) out[1] = gx;
+            out[2] = gw;
+        }
+        return once_differentiable(std::move(out), "rms_norm");
+    }
+};
+
+// The operands of a norm as the kernels read them: contiguous x and residual of
+// one shape and type, weight [C], all on one device.
+bool norm_operands(PyObject* const* a, at::Tensor (&t)[3], double* eps) {
+    if (!api.rpfq_rms_norm) return false;
+    for (int i = 0; i < 3; ++i)
+        if (!operand(a[i], &t[i])) return false;
+    *eps = PyFloat_AsDouble(a[3]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    const at::Tensor &x = t[0], &res = t[1], &w = t[2];
+    if (!x.defined() || x.dim() < 1 || x.numel() == 0 || !x.is_contiguous() || x.size(-1) > 16384 || x.numel() / x.size(-1) > 1 << 30 ||
+        !((float)*eps > 0.0f && (float)*eps < INFINITY))
+        return false;
+    if (res.defined() && (res.scalar_type() != x.scalar_type() || res.sizes() != x.sizes() || !res.is_contiguous() ||
+                          res.device() != x.device()))
+        return false;
+    return !w.defined() || (w.dim() == 1 && w.size(0) == x.size(-1) && w.is_contiguous() && w.device() == x.device());
+}
+
+// rms_norm(x, residual, weight, eps): y, or (y, h) with a residual
+PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor t[3];
+    double eps;
+    if (n != 4 || !norm_operands(a, t, &eps)) Py_RETURN_NONE;
+    at::Tensor y, h;
+    {
+        Unlocked u;
+        if (needs_grad(&t[0]) || needs_grad(&t[1]) || needs_grad(&t[2])) {
+            auto given = [](const at::Tensor& o) { return o.defined() ? std::optional<at::Tensor>(o) : std::nullopt; };
+            const auto out = RmsNorm::apply(t[0], given(t[1]), given(t[2]), eps);
+            y = out[0];
+            if (out.size() > 1) h = out[1];
+        } else {
+            auto out = RmsNorm::norm(t[0], t[1], t[2], eps, false);
+            y = out[0];
+            h = out[1];
+        }
+    }
+    if (!h.defined()) return THPVariable_Wrap(y);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(y), THPVariable_Wrap(h));
+    END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_int8(x, residual, weight, eps): (codes, scale), or (codes, scale, h)
+PyObject* rms_norm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor t[3];
+    double eps;
+    if (n != 4 || !norm_operands(a, t, &eps) || needs_grad(&t[0]) || needs_grad(&t[1]) || needs_grad(&t[2])) Py_RETURN_NONE;
+    const at::Tensor &x = t[0], &res = t[1], &w = t[2];
+    at::Tensor codes, scale, h;
+    int rc;
+    {
+        Unlocked u;
+        const c10::DeviceGuard guard(x.device());
+        const auto options = x.options().requires_grad(false);
+        const int64_t c = x.size(-1);
+        codes = at::empty(x.sizes(), options.dtype(at::kChar));
+        scale = at::empty(x.sizes().slice(0, x.dim() - 1), options.dtype(at::kFloat));
+        if (res.defined()) h = at::empty(x.sizes(), options);
+        rc = api.rpfq_rms_norm_int8(x.data_ptr(), ptr(res), dtype_code(x.scalar_type()), x.numel() / c, c, ptr(w), RmsNorm::wdt(w),
+                                    (float)eps, reinterpret_cast<int8_t*>(codes.data_ptr()), scale.data_ptr<float>(), ptr(h), stream_on(x));
+    }
+    if (rc != RPFQ_OK) Py_RETURN_NONE;
+    if (!h.defined()) return Py_BuildValue("(NN)", THPVariable_Wrap(codes), THPVariable_Wrap(scale));
+    return Py_BuildValue("(NNN)", THPVariable_Wrap(codes), THPVariable_Wrap(scale), THPVariable_Wrap(h));
     END_HANDLE_TH_ERRORS
 }
 
@@ -608,6 +766,8 @@ PyMethodDef methods[] = {
     {"linear_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_int8)), METH_FASTCALL, nullptr},
     {"linear_cross_entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_cross_entropy)), METH_FASTCALL, nullptr},
     {"adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw)), METH_FASTCALL, nullptr},
+    {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rms_norm)), METH_FASTCALL, nullptr},
+    {"rms_norm_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rms_norm_int8)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

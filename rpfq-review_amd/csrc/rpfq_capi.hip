@@ -110,6 +110,16 @@ rpfq::CeCall ce_call(const rpfq_ce_desc* d, const void* x, const void* w, const 
     return {x, w, bias, d->dtype, d->bias_dtype, target, d->M, d->V, d->D, d->ignore_index, d->smoothing, d->reduction};
 }
 
+int check_norm(int64_t M, int64_t C, int dtype, int weight_dtype, float eps) {
+    if (!dtype_ok(dtype) || !dtype_ok(weight_dtype)) return fail(RPFQ_ERR_DTYPE, "unsupported dtype %d, weight %d", dtype, weight_dtype);
+    if (M <= 0 || C <= 0 || M > (1LL << 30) || C > rpfq::kNormMaxC)
+        return fail(RPFQ_ERR_SHAPE, "M=%lld must be 1 .. 2^30, C=%lld 1 .. %lld", (long long)M, (long long)C, (long long)rpfq::kNormMaxC);
+    if (!(eps > 0.0f && eps < INFINITY)) return fail(RPFQ_ERR_VALUE, "eps=%g must be positive and finite", (double)eps);
+    return RPFQ_OK;
+}
+
+size_t element(int dtype) { return dtype == RPFQ_F32 ? 4 : 2; }
+
 int check_int8(int64_t M, int64_t N, int64_t K, int x_dtype, int64_t ld_w) {
     if (M <= 0 || N <= 0 || K <= 0)
         return fail(RPFQ_ERR_SHAPE, "M=%lld N=%lld K=%lld must be positive", (long long)M, (long long)N, (long long)K);
@@ -773,6 +783,58 @@ int rpfq_quantize_int8(const void* x, int x_dtype, int64_t M, int64_t K, int8_t*
     if (!aligned(x, x_dtype == RPFQ_F32 ? 4 : 2) || !aligned(scale, 4)) return fail(RPFQ_ERR_ALIGN, "x and scale must be aligned to their elements");
     return hip_status(rpfq::launch_quantize_int8(x, x_dtype, M, K, codes, ld_codes, scale, reinterpret_cast<hipStream_t>(stream)),
                       "rpfq_quantize_int8");
+}
+
+int rpfq_rms_norm(const void* x, const void* residual, int dtype, int64_t M, int64_t C, const void* weight,
+                  int weight_dtype, float eps, void* y, void* h, float* rstd, void* stream) {
+    int rc = check_norm(M, C, dtype, weight_dtype, eps);
+    if (rc) return rc;
+    if (!x || !y) return fail(RPFQ_ERR_NULL, "rpfq_rms_norm: NULL pointer argument");
+    if ((residual != nullptr) != (h != nullptr)) return fail(RPFQ_ERR_NULL, "h goes with a residual, and only with it");
+    const size_t es = element(dtype);
+    if (!aligned(x, es) || !aligned(residual, es) || !aligned(y, es) || !aligned(h, es) || !aligned(weight, element(weight_dtype)) ||
+        !aligned(rstd, 4))
+        return fail(RPFQ_ERR_ALIGN, "operands must be aligned to their elements");
+    return hip_status(rpfq::launch_rms_norm({x, residual, weight, dtype, weight_dtype, M, C, eps}, y, h, rstd, nullptr, nullptr,
+                                            reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_rms_norm");
+}
+
+int rpfq_rms_norm_int8(const void* x, const void* residual, int dtype, int64_t M, int64_t C, const void* weight,
+                       int weight_dtype, float eps, int8_t* codes, float* scale, void* h, void* stream) {
+    int rc = check_norm(M, C, dtype, weight_dtype, eps);
+    if (rc) return rc;
+    if (!x || !codes || !scale) return fail(RPFQ_ERR_NULL, "rpfq_rms_norm_int8: NULL pointer argument");
+    if ((residual != nullptr) != (h != nullptr)) return fail(RPFQ_ERR_NULL, "h goes with a residual, and only with it");
+    const size_t es = element(dtype);
+    if (!aligned(x, es) || !aligned(residual, es) || !aligned(h, es) || !aligned(weight, element(weight_dtype)) || !aligned(scale, 4))
+        return fail(RPFQ_ERR_ALIGN, "operands must be aligned to their elements");
+    return hip_status(rpfq::launch_rms_norm({x, residual, weight, dtype, weight_dtype, M, C, eps}, nullptr, h, nullptr, codes, scale,
+                                            reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_rms_norm_int8");
+}
+
+size_t rpfq_rms_norm_grad_workspace_bytes(int64_t M, int64_t C) {
+    if (check_norm(M, C, RPFQ_F32, RPFQ_F32, 1.0f) != RPFQ_OK) return 0;
+    return (size_t)rpfq::norm_grad_parts(M, C) * C * 4;
+}
+
+int rpfq_rms_norm_grad(const void* grad_y, const void* grad_h, const void* h, int dtype, int64_t M, int64_t C,
+                       const void* weight, int weight_dtype, const float* rstd, void* grad_x, void* grad_weight,
+                       void* work, size_t work_bytes, void* stream) {
+    int rc = check_norm(M, C, dtype, weight_dtype, 1.0f);
+    if (rc) return rc;
+    if (!grad_y || !h || !rstd || !grad_x || (grad_weight && (!weight || !work)))
+        return fail(RPFQ_ERR_NULL, "rpfq_rms_norm_grad: NULL pointer argument");
+    const size_t es = element(dtype), ws = element(weight_dtype);
+    if (!aligned(grad_y, es) || !aligned(grad_h, es) || !aligned(h, es) || !aligned(grad_x, es) || !aligned(weight, ws) ||
+        !aligned(grad_weight, ws) || !aligned(rstd, 4) || !aligned(work, 256))
+        return fail(RPFQ_ERR_ALIGN, "operands must be aligned to their elements and work to 256 bytes");
+    const size_t need = grad_weight ? rpfq_rms_norm_grad_workspace_bytes(M, C) : 0;
+    if (work_bytes < need) return fail(RPFQ_ERR_SHAPE, "workspace holds %zu bytes, need %zu", work_bytes, need);
+    return hip_status(rpfq::launch_rms_norm_grad({h, nullptr, weight, dtype, weight_dtype, M, C, 0.0f}, grad_y, grad_h, rstd, grad_x,
+                                                 grad_weight, work, reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_rms_norm_grad");
 }
 
 size_t rpfq_linear_int8_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t N, int64_t K, const int8_t* w,

@@ -427,6 +427,20 @@ hipError_t launch_adamw(const AdamTensor* t, int64_t count, int pdt, int bits, c
                         const float* lr_dev, const float* grad_scale, const float* found_inf, float* coef, hipStream_t s);
 hipError_t launch_adamw_values(const void* const* codes, const float* const* scales, const int64_t* numel,
                                const int* second, float* const* out, int64_t count, hipStream_t s);
+// root-mean-square norm (rms_norm.hip): rows of up to kNormMaxC values
+constexpr int64_t kNormMaxC = 16384;
+struct NormCall {
+    const void *x, *residual, *weight;  // [M, C], the same or NULL, [C] or NULL
+    int dtype, weight_dtype;
+    int64_t M, C;
+    float eps;
+};
+// y, rstd (NULL: not wanted) or codes, scale; h with a residual
+hipError_t launch_rms_norm(const NormCall& c, void* y, void* h, float* rstd, int8_t* codes, float* scale, hipStream_t s);
+int norm_grad_parts(int64_t M, int64_t C);
+// x: the norm's input, the sum with a residual; gh, gw NULL: none
+hipError_t launch_rms_norm_grad(const NormCall& c, const void* gy, const void* gh, const float* rstd, void* gx, void* gw,
+                                void* work, hipStream_t s);
 // adjoint blob (rpfq_kernels.hip) and the grad_x kernel (wide_adjoint.hip)
 hipError_t launch_wide_pack_adjoint(const rpfq_wide_desc& d, const WideGeom& g, const void* packed, void* adjoint,
                                     hipStream_t s);

@@ -92,6 +92,10 @@ EXPORTED = (
     "rpfq_linear_cross_entropy_grad",
     "rpfq_adamw",
     "rpfq_adamw_state_values",
+    "rpfq_rms_norm",
+    "rpfq_rms_norm_int8",
+    "rpfq_rms_norm_grad_workspace_bytes",
+    "rpfq_rms_norm_grad",
 )
 
 
@@ -231,8 +235,15 @@ def load() -> ctypes.CDLL:
         lib.rpfq_linear_cross_entropy_grad.argtypes = [cp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         lib.rpfq_adamw.argtypes = [vp, i64, i32, i32, ctypes.POINTER(AdamWHyper), vp, vp, vp, vp, vp, vp]
         lib.rpfq_adamw_state_values.argtypes = [vp, vp, vp, vp, vp, i64, vp]
+        f32 = ctypes.c_float
+        lib.rpfq_rms_norm.argtypes = [vp, vp, i32, i64, i64, vp, i32, f32, vp, vp, vp, vp]
+        lib.rpfq_rms_norm_int8.argtypes = [vp, vp, i32, i64, i64, vp, i32, f32, vp, vp, vp, vp]
+        lib.rpfq_rms_norm_grad_workspace_bytes.argtypes = [i64, i64]
+        lib.rpfq_rms_norm_grad_workspace_bytes.restype = sz
+        lib.rpfq_rms_norm_grad.argtypes = [vp, vp, vp, i32, i64, i64, vp, i32, vp, vp, vp, vp, sz, vp]
         for name in EXPORTED[2:]:
-            if name not in ("rpfq_linear_int8_workspace_bytes", "rpfq_linear_cross_entropy_workspace_bytes",
+            if name not in ("rpfq_rms_norm_grad_workspace_bytes", "rpfq_linear_int8_workspace_bytes",
+                            "rpfq_linear_cross_entropy_workspace_bytes",
                             "rpfq_wide_packed_bytes", "rpfq_wide_adjoint_bytes", "rpfq_quantize_workspace_bytes",
                             "rpfq_linear_f32_workspace_bytes", "rpfq_wide_dense_bytes"):
                 getattr(lib, name).restype = i32

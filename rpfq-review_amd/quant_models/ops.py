@@ -1145,6 +1145,107 @@ def adamw_state_values(codes, scales) -> list[torch.Tensor]:
     return out
 
 
+def _no_transforms(name: str, *tensors: torch.Tensor) -> None:
+    """Refuses what stands for other tensors: functorch's, and dual numbers,
+    whose tangents the kernels would drop."""
+    if torch._C._are_functorch_transforms_active():
+        raise RuntimeError(f"{name} takes no part in functorch transforms")
+    if torch.autograd.forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative")
+
+
+def _records(*tensors: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _norm_operands(name, x, weight, eps, residual):
+    """The checks of a norm's arguments; (x, weight, residual) as the kernels
+    read them, x [M, C]."""
+    N.require_same_device(x, weight=weight, residual=residual)
+    _no_transforms(name, x, weight, residual)
+    if x.dim() == 0 or not 1 <= x.shape[-1] <= NORM_MAX_FEATURES:
+        raise ValueError(f"{name} takes rows of 1 .. {NORM_MAX_FEATURES} values, got {tuple(x.shape)}")
+    N.dtype_code(x.dtype)
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"residual must be {x.dtype} of shape {tuple(x.shape)}, got {residual.dtype} {tuple(residual.shape)}")
+    if weight is not None:
+        N.dtype_code(weight.dtype)
+        if weight.shape != x.shape[-1:]:
+            raise ValueError(f"weight must have shape ({x.shape[-1]},), got {tuple(weight.shape)}")
+    if not 0.0 < eps < math.inf:
+        raise ValueError(f"eps must be positive and finite, got {eps}")
+    return x.contiguous(), None if weight is None else weight.contiguous(), None if residual is None else residual.contiguous()
+
+
+NORM_MAX_FEATURES = 16384
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
+             residual: torch.Tensor | None = None):
+    """y = x / sqrt(mean(x^2) + eps) * weight over the last dimension
+    (rpfq_rms_norm): float32 statistics, y rounded once to x's type.  With a
+    residual of x's shape and type: (y, h), h = x + residual in that type, y
+    the norm of h, in one pass.  x: float32, fp16 or bf16 [..., C], C <=
+    NORM_MAX_FEATURES; weight [C] of any of these types.  Gradients of x,
+    residual and weight, once differentiable, float32 sums in a fixed order;
+    can be captured into a graph, backward too, where no eager graph of the
+    same leaves is alive (such a backward is refused).  Gradients need the
+    native host path (csrc/host.cpp)."""
+    host = N.host()
+    if host is not None:
+        out = host.rms_norm(x, residual, weight, eps)
+        if out is not None:
+            return out
+    x2, w, r = _norm_operands("rms_norm", x, weight, eps, residual)
+    if x.numel() == 0:
+        y = x2 if weight is None else (x2 * w).to(x.dtype)
+        return (y + 0.0) if residual is None else (y + 0.0, x2 + r)
+    if host is not None:
+        out = host.rms_norm(x2, r, w, eps)
+        if out is not None:
+            return out
+    if _records(x, weight, residual):
+        raise RuntimeError("rms_norm: gradients need the native host path (csrc/host.cpp)")
+    y = torch.empty_like(x2)
+    h = None if r is None else torch.empty_like(x2)
+    c = x2.shape[-1]
+    with N.on_device(x2):
+        N.check("rpfq_rms_norm", N.load().rpfq_rms_norm(
+            x2.data_ptr(), N.ptr(r), N.dtype_code(x2.dtype), x2.numel() // c, c, N.ptr(w),
+            N.F32 if w is None else N.dtype_code(w.dtype), float(eps), y.data_ptr(), N.ptr(h), None, N.stream_of(x2)))
+    return y if r is None else (y, h)
+
+
+def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
+                  residual: torch.Tensor | None = None):
+    """rms_norm with its output in 8 bits, as linear_int8 takes it
+    (rpfq_rms_norm_int8): (codes int8 [..., C], scale float32 [...]), with a
+    residual (codes, scale, h).  scale = max|y| / 127 of the unrounded y, codes =
+    rint(127 y / max|y|), ties to even: decided by the products h weight, exact
+    in 64 bits.  A row with inf or NaN has scale NaN.  No gradient."""
+    host = N.host()
+    if host is not None:
+        out = host.rms_norm_int8(x, residual, weight, eps)
+        if out is not None:
+            return out
+    x2, w, r = _norm_operands("rms_norm_int8", x, weight, eps, residual)
+    if _records(x, weight, residual):
+        raise RuntimeError("rms_norm_int8 has no gradient: call it under torch.no_grad()")
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    h = None if r is None else torch.empty_like(x2)
+    c = x2.shape[-1]
+    if x2.numel():
+        with N.on_device(x2):
+            N.check("rpfq_rms_norm_int8", N.load().rpfq_rms_norm_int8(
+                x2.data_ptr(), N.ptr(r), N.dtype_code(x2.dtype), x2.numel() // c, c, N.ptr(w),
+                N.F32 if w is None else N.dtype_code(w.dtype), float(eps), codes.data_ptr(), scale.data_ptr(), N.ptr(h),
+                N.stream_of(x2)))
+    return (codes, scale) if r is None else (codes, scale, h)
+
+
 def make_desc(n_complex, k_complex, codebook, stages, block, rotation) -> N.WideDesc:
     d = N.WideDesc()
     d.n_complex = int(n_complex)
