@@ -800,6 +800,34 @@ int rpfq_rms_norm_grad(const void* grad_y, const void* grad_h, const void* h, in
                        const void* weight, int weight_dtype, const float* rstd, void* grad_x, void* grad_weight,
                        void* work, size_t work_bytes, void* stream);
 
+/* Rotary positions of the heads of one or two tensors [B, N, heads[i], D] (the
+ * queries and the keys of a layer), strides in elements between batches, tokens
+ * and heads, the values of a head next to each other. */
+#define RPFQ_POS_I64 0
+#define RPFQ_POS_I32 1
+#define RPFQ_POS_F32 2
+typedef struct rpfq_rotary_desc {
+    int64_t B, N, D;
+    int64_t heads[2]; /* heads[1] = 0: one tensor */
+    int64_t in_stride[2][3], out_stride[2][3];
+    int64_t pos_stride[2]; /* of positions between batches (0: shared) and tokens; the axes lie next to each other */
+    int32_t dtype, pos_dtype;
+    int32_t axes;        /* 1 .. 4 */
+    int32_t sections[4]; /* pairs that each axis turns, one section behind the other; 2 sum(sections) <= D <= 1024 */
+    int32_t interleaved; /* pair j: values 2 j and 2 j + 1; 0: values j and j + sum(sections) */
+    int32_t inverse;     /* turned back: the gradient */
+} rpfq_rotary_desc;
+
+/*
+ * Pair j of every head turned by position[token][axis of j] freqs[j] radians
+ * (freqs [sum(sections)] float64 in device memory; the angle in 64 bits, the rest
+ * float32, rounded once): (u, v) -> (u cos - v sin, v cos + u sin); the values
+ * behind the pairs are copied.  Outputs may be the inputs themselves.  No
+ * counterpart in the reference, whose positions are learned and added.
+ */
+int rpfq_rotary(const rpfq_rotary_desc* desc, const void* q, const void* k, void* q_out, void* k_out,
+                const void* positions, const double* freqs, void* stream);
+
 /*
  * rpfq_quantize_wide without a workspace argument and without any device
  * allocation: the float64 partials live in a static device array of this

@@ -43,7 +43,7 @@ constexpr double kMostOps = 1.5e9;
     X(rpfq_attention) X(rpfq_last_error) X(rpfq_linear_int8_workspace_bytes) X(rpfq_linear_int8)        \
     X(rpfq_linear_cross_entropy_workspace_bytes) X(rpfq_linear_cross_entropy)                           \
     X(rpfq_linear_cross_entropy_grad) X(rpfq_adamw) X(rpfq_rms_norm) X(rpfq_rms_norm_int8)             \
-    X(rpfq_rms_norm_grad_workspace_bytes) X(rpfq_rms_norm_grad)
+    X(rpfq_rms_norm_grad_workspace_bytes) X(rpfq_rms_norm_grad) X(rpfq_rotary)
 struct Api {
 #define X(f) decltype(&::f) f;
     RPFQ_HOST_CALLS(X)
@@ -635,6 +635,118 @@ PyObject* rms_norm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// Rotary positions under autograd: (q[, k]) -> (q[, k]) turned; the gradients turn back.
+struct Rotary : torch::autograd::Function<Rotary> {
+    static void strides(const at::Tensor& t, int64_t (&s)[3]) {
+        for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
+    }
+    // x turned as d says (its sizes, sections and types filled in), in new tensors
+    static torch::autograd::variable_list turn(rpfq_rotary_desc d, const std::array<at::Tensor, 2>& x, const at::Tensor& positions,
+                                               const at::Tensor& freqs) {
+        const c10::DeviceGuard guard(positions.device());
+        torch::autograd::variable_list out;
+        for (int i = 0; i < 2; ++i) {
+            d.heads[i] = x[i].defined() ? x[i].size(2) : 0;
+            if (!x[i].defined()) continue;
+            out.push_back(at::empty(x[i].sizes(), x[i].options().requires_grad(false)));
+            strides(x[i], d.in_stride[i]);
+            strides(out.back(), d.out_stride[i]);
+        }
+        const int rc = api.rpfq_rotary(&d, x[0].data_ptr(), ptr(x[1]), out[0].data_ptr(), out.size() > 1 ? out[1].data_ptr() : nullptr,
+                                       positions.data_ptr(), freqs.const_data_ptr<double>(), stream_on(x[0]));
+        TORCH_CHECK(rc == RPFQ_OK, "rpfq_rotary: ", api.rpfq_last_error());
+        return out;
+    }
+
+    // the descriptor goes to the backward as a tensor of its bytes
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const std::optional<at::Tensor>& k,
+                                                  const at::Tensor& positions, const at::Tensor& freqs, const rpfq_rotary_desc* d) {
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({positions, freqs});
+        ctx->saved_data["desc"] = std::string(reinterpret_cast<const char*>(d), sizeof(*d));
+        return turn(*d, {q, k ? *k : at::Tensor()}, positions, freqs);
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        refuse_capture("rotary");
+        const auto saved = ctx->get_saved_variables();
+        rpfq_rotary_desc d;
+        const std::string bytes = ctx->saved_data["desc"].toStringRef();
+        std::memcpy(&d, bytes.data(), sizeof(d));
+        d.inverse = 1;
+        torch::autograd::variable_list out(5);
+        {
+            const at::NoGradGuard plain_results;
+            std::array<at::Tensor, 2> g;
+            int at_[2], n = 0;
+            for (int i = 0; i < (int)grads.size(); ++i) {
+                if (!grads[i].defined() || !ctx->needs_input_grad(i)) continue;
+                g[n] = grads[i].stride(3) == 1 || grads[i].size(3) == 1 ? grads[i] : grads[i].contiguous();
+                at_[n++] = i;
+            }
+            if (!n) return out;
+            const auto turned = turn(d, g, saved[0], saved[1]);
+            for (int i = 0; i < n; ++i) out[at_[i]] = turned[i];
+        }
+        return once_differentiable(std::move(out), "rotary");
+    }
+};
+
+// rotary(q, k or None, positions [N or B, N, axes], freqs, sections, interleaved): a tuple of the turned
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor q, k;
+    int64_t inter;
+    if (n != 6 || !api.rpfq_rotary || !operand(a[0], &q) || !operand(a[1], &k) || !q.defined() || !number(a[5], &inter) ||
+        !PyTuple_CheckExact(a[4]))
+        Py_RETURN_NONE;
+    const at::Tensor *pos = plain(a[2]), *freqs = plain(a[3]);
+    const Py_ssize_t axes = PyTuple_GET_SIZE(a[4]);
+    if (!pos || !freqs || axes < 1 || axes > 4 || freqs->scalar_type() != at::kDouble || freqs->dim() != 1 || !freqs->is_contiguous() ||
+        q.dim() != 4 || q.numel() == 0 || pos->dim() < 2 || pos->dim() > 3 || pos->size(-1) != axes ||
+        (axes > 1 && pos->stride(-1) != 1) || pos->requires_grad() || freqs->requires_grad())
+        Py_RETURN_NONE;
+    rpfq_rotary_desc d = {};
+    d.B = q.size(0), d.N = q.size(1), d.D = q.size(3);
+    d.dtype = dtype_code(q.scalar_type());
+    switch (pos->scalar_type()) {
+        case at::kLong: d.pos_dtype = RPFQ_POS_I64; break;
+        case at::kInt: d.pos_dtype = RPFQ_POS_I32; break;
+        case at::kFloat: d.pos_dtype = RPFQ_POS_F32; break;
+        default: Py_RETURN_NONE;
+    }
+    d.axes = (int32_t)axes;
+    int64_t pairs = 0;
+    for (Py_ssize_t i = 0; i < axes; ++i) {
+        int64_t v;
+        if (!number(PyTuple_GET_ITEM(a[4], i), &v) || v < 0 || v > 512) Py_RETURN_NONE;
+        d.sections[i] = (int32_t)v;
+        pairs += v;
+    }
+    d.interleaved = inter != 0;
+    d.pos_stride[0] = pos->dim() == 3 ? pos->stride(0) : 0;
+    d.pos_stride[1] = pos->stride(-2);
+    if (freqs->size(0) != pairs || 2 * pairs > d.D || pos->size(-2) != d.N || (pos->dim() == 3 && pos->size(0) != d.B) ||
+        pos->device() != q.device() || freqs->device() != q.device())
+        Py_RETURN_NONE;
+    for (const at::Tensor* t : {&q, &k})
+        if (t->defined() && (t->dim() != 4 || t->size(0) != d.B || t->size(1) != d.N || t->size(3) != d.D || t->size(2) < 1 ||
+                             t->scalar_type() != q.scalar_type() || t->device() != q.device() || (d.D > 1 && t->stride(3) != 1)))
+            Py_RETURN_NONE;
+    if (d.N > (1LL << 30) / d.B || q.size(2) > 1024 || (k.defined() && k.size(2) > 1024)) Py_RETURN_NONE;
+    torch::autograd::variable_list out;
+    {
+        Unlocked u;
+        if (needs_grad(&q) || needs_grad(&k))
+            out = Rotary::apply(q, k.defined() ? std::optional<at::Tensor>(k) : std::nullopt, *pos, *freqs, (const rpfq_rotary_desc*)&d);
+        else
+            out = Rotary::turn(d, {q, k}, *pos, *freqs);
+    }
+    if (out.size() == 1) return Py_BuildValue("(N)", THPVariable_Wrap(out[0]));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(out[0]), THPVariable_Wrap(out[1]));
+    END_HANDLE_TH_ERRORS
+}
+
 // The tensors of a list, or false where it is not a list of plain ones.
 bool tensors(PyObject* list, std::vector<const at::Tensor*>& out) {
     if (!PyList_CheckExact(list)) return false;
@@ -768,6 +880,7 @@ PyMethodDef methods[] = {
     {"adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw)), METH_FASTCALL, nullptr},
     {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rms_norm)), METH_FASTCALL, nullptr},
     {"rms_norm_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rms_norm_int8)), METH_FASTCALL, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -837,6 +837,34 @@ int rpfq_rms_norm_grad(const void* grad_y, const void* grad_h, const void* h, in
                       "rpfq_rms_norm_grad");
 }
 
+int rpfq_rotary(const rpfq_rotary_desc* d, const void* q, const void* k, void* q_out, void* k_out, const void* positions,
+                const double* freqs, void* stream) {
+    if (!d) return fail(RPFQ_ERR_NULL, "desc is NULL");
+    if (!dtype_ok(d->dtype) || d->pos_dtype < RPFQ_POS_I64 || d->pos_dtype > RPFQ_POS_F32)
+        return fail(RPFQ_ERR_DTYPE, "unsupported dtype %d, positions %d", d->dtype, d->pos_dtype);
+    if (d->B <= 0 || d->N <= 0 || d->D <= 0 || d->heads[0] <= 0 || d->heads[1] < 0)
+        return fail(RPFQ_ERR_SHAPE, "B=%lld N=%lld D=%lld heads=%lld,%lld must be positive", (long long)d->B, (long long)d->N,
+                    (long long)d->D, (long long)d->heads[0], (long long)d->heads[1]);
+    if (d->D > 1024 || d->heads[0] > 1024 || d->heads[1] > 1024 || d->N > (1LL << 30) / d->B)
+        return fail(RPFQ_ERR_SHAPE, "takes up to 1024 heads of 1024 values and 2^30 tokens (B=%lld N=%lld D=%lld heads=%lld,%lld)",
+                    (long long)d->B, (long long)d->N, (long long)d->D, (long long)d->heads[0], (long long)d->heads[1]);
+    if (d->axes < 1 || d->axes > 4) return fail(RPFQ_ERR_VALUE, "axes=%d must be 1 .. 4", d->axes);
+    int64_t pairs = 0;
+    for (int i = 0; i < d->axes; ++i) {
+        if (d->sections[i] < 0) return fail(RPFQ_ERR_VALUE, "sections[%d]=%d must not be negative", i, d->sections[i]);
+        pairs += d->sections[i];
+    }
+    if (pairs < 1 || 2 * pairs > d->D) return fail(RPFQ_ERR_SHAPE, "%lld pairs in heads of %lld values", (long long)pairs, (long long)d->D);
+    if ((d->interleaved | d->inverse) & ~1) return fail(RPFQ_ERR_VALUE, "interleaved and inverse must be 0 or 1");
+    const bool two = d->heads[1] > 0;
+    if (!q || !q_out || !positions || !freqs || (two && (!k || !k_out))) return fail(RPFQ_ERR_NULL, "rpfq_rotary: NULL pointer argument");
+    const size_t es = element(d->dtype);
+    if (!aligned(q, es) || !aligned(q_out, es) || !aligned(k, es) || !aligned(k_out, es) || !aligned(freqs, 8) ||
+        !aligned(positions, d->pos_dtype == RPFQ_POS_I64 ? 8 : 4))
+        return fail(RPFQ_ERR_ALIGN, "operands must be aligned to their elements");
+    return hip_status(rpfq::launch_rotary(*d, q, k, q_out, k_out, positions, freqs, reinterpret_cast<hipStream_t>(stream)), "rpfq_rotary");
+}
+
 size_t rpfq_linear_int8_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t N, int64_t K, const int8_t* w,
                                         int64_t ld_w) {
     if (check_int8(M, N, K, x_dtype, ld_w) != RPFQ_OK) return 0;

@@ -441,6 +441,9 @@ int norm_grad_parts(int64_t M, int64_t C);
 // x: the norm's input, the sum with a residual; gh, gw NULL: none
 hipError_t launch_rms_norm_grad(const NormCall& c, const void* gy, const void* gh, const float* rstd, void* gx, void* gw,
                                 void* work, hipStream_t s);
+// rotary positions (rotary.hip)
+hipError_t launch_rotary(const rpfq_rotary_desc& d, const void* q, const void* k, void* q_out, void* k_out, const void* pos,
+                         const double* freqs, hipStream_t s);
 // adjoint blob (rpfq_kernels.hip) and the grad_x kernel (wide_adjoint.hip)
 hipError_t launch_wide_pack_adjoint(const rpfq_wide_desc& d, const WideGeom& g, const void* packed, void* adjoint,
                                     hipStream_t s);

@@ -96,6 +96,7 @@ EXPORTED = (
     "rpfq_rms_norm_int8",
     "rpfq_rms_norm_grad_workspace_bytes",
     "rpfq_rms_norm_grad",
+    "rpfq_rotary",
 )
 
 
@@ -144,6 +145,29 @@ class AdamWHyper(ctypes.Structure):
     """Mirror of struct rpfq_adamw_hyper."""
 
     _fields_ = [(name, ctypes.c_double) for name in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+
+
+class RotaryDesc(ctypes.Structure):
+    """Mirror of struct rpfq_rotary_desc."""
+
+    _fields_ = [
+        ("B", ctypes.c_int64),
+        ("N", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("heads", ctypes.c_int64 * 2),
+        ("in_stride", ctypes.c_int64 * 3 * 2),
+        ("out_stride", ctypes.c_int64 * 3 * 2),
+        ("pos_stride", ctypes.c_int64 * 2),
+        ("dtype", ctypes.c_int32),
+        ("pos_dtype", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * 4),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+    ]
+
+
+POS_DTYPES = {torch.int64: 0, torch.int32: 1, torch.float32: 2}
 
 
 class RPFQError(RuntimeError):
@@ -241,6 +265,7 @@ def load() -> ctypes.CDLL:
         lib.rpfq_rms_norm_grad_workspace_bytes.argtypes = [i64, i64]
         lib.rpfq_rms_norm_grad_workspace_bytes.restype = sz
         lib.rpfq_rms_norm_grad.argtypes = [vp, vp, vp, i32, i64, i64, vp, i32, vp, vp, vp, vp, sz, vp]
+        lib.rpfq_rotary.argtypes = [ctypes.POINTER(RotaryDesc), vp, vp, vp, vp, vp, vp, vp]
         for name in EXPORTED[2:]:
             if name not in ("rpfq_rms_norm_grad_workspace_bytes", "rpfq_linear_int8_workspace_bytes",
                             "rpfq_linear_cross_entropy_workspace_bytes",

@@ -1246,6 +1246,117 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor | None = None, eps: floa
     return (codes, scale) if r is None else (codes, scale, h)
 
 
+def rotary_frequencies(sections, base: float = 10000.0, *, shared: bool = False, device="cuda") -> torch.Tensor:
+    """float64 freqs for rotary(): each axis with its own ladder base^(-j / p), j =
+    0 .. p - 1 over its p pairs; shared=True: one ladder over all pairs, which
+    the axes divide between them."""
+    runs = [sum(sections)] if shared else list(sections)
+    if not sections or min(sections) < 0 or sum(sections) < 1 or not 0.0 < base < math.inf:
+        raise ValueError(f"rotary_frequencies: sections {tuple(sections)} and base {base}")
+    return torch.cat([base ** (-torch.arange(p, dtype=torch.float64) / max(p, 1)) for p in runs]).to(device)
+
+
+def _apart(t: torch.Tensor) -> bool:
+    """Whether t's elements surely lie at places of their own."""
+    span = 1
+    for size, stride in sorted(zip(t.shape, t.stride()), key=lambda e: e[1]):
+        if size > 1:
+            if stride < span:
+                return False
+            span = stride * (size - 1) + span
+    return True
+
+
+def rotary(x, positions: torch.Tensor, freqs: torch.Tensor, sections=None, *, interleaved: bool = False,
+           inplace: bool = False):
+    """Rotary positions of several axes (rpfq_rotary): pair j of every head of x
+    [B, N, heads, D], or of each of a pair of them (q, k), turned by
+    positions[token, axis of j] * freqs[j] radians.  positions [N] (one axis),
+    [N, axes] or [B, N, axes], int64, int32 or float32, at most 4 axes; freqs
+    float64 [pairs] on the device (rotary_frequencies); sections: pairs of each
+    axis, one behind the other (default: all of one axis).  Pair j is the values
+    j and j + pairs of a head, interleaved 2 j and 2 j + 1; values behind the
+    pairs stay as they are.  The angle is formed in 64 bits.  fp16, bf16 or
+    float32, any strides over the heads of a qkv tensor (values of a head next
+    to each other, else a copy).  A token of positions 0 (a class token) is not
+    turned.  inplace: x is turned itself (and returned), which takes no part in
+    autograd.  Gradients of x, once differentiable, need the native host path
+    (csrc/host.cpp); can be captured as rms_norm can."""
+    one = isinstance(x, torch.Tensor)
+    xs = (x,) if one else tuple(x)
+    if not 1 <= len(xs) <= 2:
+        raise ValueError(f"rotary takes one tensor or two, got {len(xs)}")
+    if isinstance(positions, torch.Tensor) and positions.dim() == 1:
+        positions = positions[:, None]
+    if sections is None:
+        sections = (freqs.numel(),)
+    sections = tuple(sections)
+    host = N.host()
+    if host is not None and not inplace:
+        out = host.rotary(xs[0], xs[1] if len(xs) > 1 else None, positions, freqs, sections, interleaved)
+        if out is not None:
+            return out[0] if one else out
+    q = xs[0]
+    N.require_same_device(q, positions=positions, freqs=freqs, k=xs[1] if len(xs) > 1 else None)
+    _no_transforms("rotary", *xs)
+    if not 1 <= len(sections) <= 4 or min(sections) < 0:
+        raise ValueError(f"rotary takes 1 to 4 sections of 0 pairs or more, got {sections}")
+    pairs = sum(sections)
+    for t in xs:
+        N.dtype_code(t.dtype)
+        if t.dim() != 4 or t.shape[2] > 1024 or t.shape[3] > 1024:
+            raise ValueError(f"rotary takes [B, N, heads, D] of at most 1024 heads of 1024 values, got {tuple(t.shape)}")
+        if t.dtype != q.dtype or (t.shape[0], t.shape[1], t.shape[3]) != (q.shape[0], q.shape[1], q.shape[3]):
+            raise ValueError(f"rotary: {t.dtype} {tuple(t.shape)} beside {q.dtype} {tuple(q.shape)}")
+    b, n, _, d = q.shape
+    if pairs < 1 or 2 * pairs > d:
+        raise ValueError(f"rotary: {pairs} pairs in heads of {d} values")
+    if b * n > 1 << 30:
+        raise ValueError(f"rotary takes at most 2^30 tokens, got {b * n}")
+    if freqs.shape != (pairs,) or freqs.dtype != torch.float64:
+        raise ValueError(f"freqs must be float64 of shape ({pairs},), got {freqs.dtype} {tuple(freqs.shape)}")
+    if positions.dtype not in N.POS_DTYPES or tuple(positions.shape) not in ((n, len(sections)), (b, n, len(sections))):
+        raise ValueError(f"positions must be int64, int32 or float32 of shape ({n}, {len(sections)}) or ({b}, {n}, {len(sections)}), "
+                         f"got {positions.dtype} {tuple(positions.shape)}")
+    if _records(positions, freqs):
+        raise RuntimeError("rotary has no gradient of positions and freqs")
+    if inplace:
+        if _records(*xs):
+            raise RuntimeError("rotary: inplace takes no part in autograd")
+        if not all(t.stride(3) == 1 and _apart(t) for t in xs if t.numel()):
+            raise ValueError("rotary: inplace takes tensors whose heads lie in one piece each, none over another")
+    if q.numel() == 0 and (one or xs[1].numel() == 0):
+        out = xs if inplace else tuple(t.clone() for t in xs)
+        return out[0] if one else out
+    if any(t.shape[2] == 0 for t in xs):
+        raise ValueError("rotary: a tensor without heads beside one with heads")
+    positions = positions if len(sections) == 1 or positions.stride(-1) == 1 else positions.contiguous()
+    freqs = freqs.contiguous()
+    ins = tuple(t if t.stride(3) == 1 else t.contiguous() for t in xs)
+    if host is not None and not inplace:
+        out = host.rotary(ins[0], ins[1] if len(ins) > 1 else None, positions, freqs, sections, interleaved)
+        if out is not None:
+            return out[0] if one else out
+    if _records(*xs):
+        raise RuntimeError("rotary: gradients need the native host path (csrc/host.cpp)")
+    outs = ins if inplace else tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in ins)
+    desc = N.RotaryDesc(B=b, N=n, D=d, dtype=N.dtype_code(q.dtype), pos_dtype=N.POS_DTYPES[positions.dtype], axes=len(sections),
+                        interleaved=int(bool(interleaved)))
+    desc.sections[:len(sections)] = sections
+    desc.pos_stride[:] = (positions.stride(0) if positions.dim() == 3 else 0, positions.stride(-2))
+    for i, (t, o) in enumerate(zip(ins, outs)):
+        desc.heads[i] = t.shape[2]
+        desc.in_stride[i][:] = t.stride()[:3]
+        desc.out_stride[i][:] = o.stride()[:3]
+    with N.on_device(q):
+        N.check("rpfq_rotary", N.load().rpfq_rotary(
+            ctypes.byref(desc), ins[0].data_ptr(), ins[1].data_ptr() if len(ins) > 1 else None, outs[0].data_ptr(),
+            outs[1].data_ptr() if len(outs) > 1 else None, positions.data_ptr(), freqs.data_ptr(), N.stream_of(q)))
+    if inplace:
+        torch.autograd.graph.increment_version([t for t in xs if not t.is_inference()])
+    return outs[0] if one else outs
+
+
 def make_desc(n_complex, k_complex, codebook, stages, block, rotation) -> N.WideDesc:
     d = N.WideDesc()
     d.n_complex = int(n_complex)
