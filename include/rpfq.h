@@ -829,6 +829,54 @@ int rpfq_rotary(const rpfq_rotary_desc* desc, const void* q, const void* k, void
                 const void* positions, const double* freqs, void* stream);
 
 /*
+ * Attention with a sliding window and first tokens that stay visible (sinks):
+ * query i sees key j of its sequence where
+ *   causal:  j <= i and (i - j < window or j < sinks),
+ *   else:    |i - j| < window or j < sinks or i < sinks,
+ * out = softmax(scale q k^T) v over what it sees, zeros for a row without any.
+ * q, out [B, N, H, D]; k, v [B, N, KV, D] (cached: [B, M, KV, D]), KV a divisor of
+ * H: query head h reads head h KV / H.  fp16 or bf16, scores and sums float32,
+ * probabilities rounded to 16 bits.  Strides in elements between batches, tokens
+ * and heads, multiples of 8, below 2^22 between tokens; the values of a head
+ * next to each other, D a multiple of 8 up to 128, pointers 16-byte aligned.
+ * lengths [B] (device int32, NULL: all of them N): rows of a sequence that
+ * count, clamped to 0 .. N; those behind give zeros and are not read.
+ * No counterpart in the reference, whose attention sees every token.
+ */
+typedef struct rpfq_window_desc {
+    int64_t B, N, H, KV, D;
+    int64_t M;              /* cached: keys of the cache; else 0 */
+    int64_t window, sinks;  /* window >= 1, sinks >= 0 */
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    int64_t out_stride[3];  /* cached: contiguous */
+    int64_t grad_stride[3]; /* of grad_out */
+    int32_t dtype, causal;
+    float scale;            /* positive and finite */
+} rpfq_window_desc;
+
+/* stat (out, float32, 256-byte aligned, rpfq_window_attention_stat_bytes; NULL: not wanted): what the
+ * gradient needs of each row. */
+int rpfq_window_attention(const rpfq_window_desc* desc, const void* q, const void* k, const void* v,
+                          const int32_t* lengths, void* out, float* stat, void* stream);
+size_t rpfq_window_attention_stat_bytes(const rpfq_window_desc* desc);
+
+/* Gradients, contiguous and of dtype, zeros behind a sequence's end; any of
+ * them NULL: not wanted.  out, stat: the forward's; work: as many bytes as stat,
+ * 256-byte aligned.  Sums in a fixed order. */
+int rpfq_window_attention_grad(const rpfq_window_desc* desc, const void* q, const void* k, const void* v,
+                               const int32_t* lengths, const void* out, const void* grad_out, const float* stat,
+                               void* grad_q, void* grad_k, void* grad_v, void* work, size_t work_bytes, void* stream);
+
+/* The last N tokens of each sequence against a cache of M slots: query t is
+ * token lengths[b] - N + t, causal; lengths [B] (clamped to 0 .. M) counts the new
+ * tokens.  Only slots that some query sees are read.  work: its workspace
+ * (may be 0 bytes), 256-byte aligned; where lengths < N the first queries see
+ * nothing. */
+int rpfq_window_attention_cached(const rpfq_window_desc* desc, const void* q, const void* k_cache, const void* v_cache,
+                                 const int32_t* lengths, void* out, void* work, size_t work_bytes, void* stream);
+size_t rpfq_window_attention_cached_workspace_bytes(const rpfq_window_desc* desc);
+
+/*
  * rpfq_quantize_wide without a workspace argument and without any device
  * allocation: the float64 partials live in a static device array of this
  * library (64 KiB per GPU, held until the process ends), so the call makes

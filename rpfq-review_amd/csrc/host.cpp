@@ -43,7 +43,9 @@ constexpr double kMostOps = 1.5e9;
     X(rpfq_attention) X(rpfq_last_error) X(rpfq_linear_int8_workspace_bytes) X(rpfq_linear_int8)        \
     X(rpfq_linear_cross_entropy_workspace_bytes) X(rpfq_linear_cross_entropy)                           \
     X(rpfq_linear_cross_entropy_grad) X(rpfq_adamw) X(rpfq_rms_norm) X(rpfq_rms_norm_int8)             \
-    X(rpfq_rms_norm_grad_workspace_bytes) X(rpfq_rms_norm_grad) X(rpfq_rotary)
+    X(rpfq_rms_norm_grad_workspace_bytes) X(rpfq_rms_norm_grad) X(rpfq_rotary) \
+    X(rpfq_window_attention) X(rpfq_window_attention_stat_bytes) X(rpfq_window_attention_grad)           \
+    X(rpfq_window_attention_cached) X(rpfq_window_attention_cached_workspace_bytes)
 struct Api {
 #define X(f) decltype(&::f) f;
     RPFQ_HOST_CALLS(X)
@@ -747,6 +749,145 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// What the window's kernels read as it lies: 16-bit heads in one piece each, whole
+// 16-byte pieces from a 16-byte aligned start.
+bool window_rows16(const at::Tensor& t) {
+    return (t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16) && t.dim() == 4 && t.size(3) % 8 == 0 && t.stride(3) == 1 &&
+           (t.stride(0) | t.stride(1) | t.stride(2)) % 8 == 0 && t.stride(1) < 1 << 22 &&
+           reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+void window_strides(const at::Tensor& t, int64_t (&s)[3]) {
+    for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
+}
+
+// Attention with a window under autograd: (q, k, v) -> out.
+struct Window : torch::autograd::Function<Window> {
+    static std::pair<at::Tensor, at::Tensor> attend(rpfq_window_desc& d, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                    const at::Tensor& lengths, bool stat) {
+        const c10::DeviceGuard guard(q.device());
+        const auto options = q.options().requires_grad(false);
+        at::Tensor out = at::empty(q.sizes(), options), st;
+        window_strides(out, d.out_stride);
+        if (stat) st = at::empty({(int64_t)(api.rpfq_window_attention_stat_bytes(&d) / 4)}, options.dtype(at::kFloat));
+        const int rc = api.rpfq_window_attention(&d, q.data_ptr(), k.data_ptr(), v.data_ptr(), static_cast<const int32_t*>(ptr(lengths)),
+                                                 out.data_ptr(), stat ? st.data_ptr<float>() : nullptr, stream_on(q));
+        TORCH_CHECK(rc == RPFQ_OK, "rpfq_window_attention: ", api.rpfq_last_error());
+        return {out, st};
+    }
+
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                              const std::optional<at::Tensor>& lengths, rpfq_window_desc* d) {
+        const at::Tensor len = lengths ? *lengths : at::Tensor();
+        auto [out, stat] = attend(*d, q, k, v, len, true);
+        ctx->save_for_backward({q, k, v, len, out, stat});
+        ctx->saved_data["desc"] = std::string(reinterpret_cast<const char*>(d), sizeof(*d));
+        return out;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        refuse_capture("window_attention");
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &lengths = saved[3], &out = saved[4], &stat = saved[5];
+        const c10::DeviceGuard guard(q.device());
+        rpfq_window_desc d;
+        const std::string bytes = ctx->saved_data["desc"].toStringRef();
+        std::memcpy(&d, bytes.data(), sizeof(d));
+        torch::autograd::variable_list g(5);
+        {
+            const at::NoGradGuard plain_results;
+            const at::Tensor go = window_rows16(grads[0]) ? grads[0] : grads[0].clone(at::MemoryFormat::Contiguous);
+            window_strides(go, d.grad_stride);
+            const at::Tensor* in[3] = {&q, &k, &v};
+            for (int i = 0; i < 3; ++i)
+                if (ctx->needs_input_grad(i)) g[i] = at::empty(in[i]->sizes(), q.options().requires_grad(false));
+            if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return g;
+            at::Tensor work = at::empty(stat.sizes(), stat.options());
+            const int rc = api.rpfq_window_attention_grad(&d, q.data_ptr(), k.data_ptr(), v.data_ptr(), static_cast<const int32_t*>(ptr(lengths)),
+                                                          out.data_ptr(), go.data_ptr(), stat.const_data_ptr<float>(), ptr(g[0]), ptr(g[1]),
+                                                          ptr(g[2]), work.data_ptr(), work.nbytes(), stream_on(q));
+            TORCH_CHECK(rc == RPFQ_OK, "rpfq_window_attention_grad: ", api.rpfq_last_error());
+        }
+        return once_differentiable(std::move(g), "window_attention");
+    }
+};
+
+// q, k, v, lengths (int32 or None), window, sinks, scale of a call that the kernels
+// take as it lies; d's sizes, strides and numbers.
+bool window_operands(PyObject* const* a, at::Tensor (&t)[3], at::Tensor& lengths, rpfq_window_desc& d, bool cached) {
+    if (!api.rpfq_window_attention) return false;
+    for (int i = 0; i < 3; ++i)
+        if (!operand(a[i], &t[i]) || !t[i].defined() || !window_rows16(t[i])) return false;
+    if (a[3] != Py_None) {
+        const at::Tensor* l = plain(a[3]);
+        if (!l || l->scalar_type() != at::kInt || l->dim() != 1 || !l->is_contiguous()) return false;
+        lengths = *l;
+    }
+    const double scale = PyFloat_AsDouble(a[6]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    const at::Tensor &q = t[0], &k = t[1], &v = t[2];
+    if (!number(a[4], &d.window) || !number(a[5], &d.sinks) || d.window < 1 || d.sinks < 0) return false;
+    d.B = q.size(0), d.N = q.size(1), d.H = q.size(2), d.D = q.size(3), d.KV = k.size(2), d.M = cached ? k.size(1) : 0;
+    d.dtype = dtype_code(q.scalar_type());
+    d.scale = (float)scale;
+    for (const at::Tensor* x : {&k, &v})
+        if (x->scalar_type() != q.scalar_type() || x->device() != q.device() || x->size(0) != d.B || x->size(3) != d.D ||
+            x->size(2) != d.KV || x->size(1) != (cached ? d.M : d.N))
+            return false;
+    if (lengths.defined() ? lengths.size(0) != d.B || lengths.device() != q.device() : cached) return false;
+    window_strides(q, d.q_stride);
+    window_strides(k, d.k_stride);
+    window_strides(v, d.v_stride);
+    return true;
+}
+
+// window_attention(q, k, v, lengths, window, sinks, scale, causal)
+PyObject* window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor t[3], lengths;
+    rpfq_window_desc d = {};
+    int64_t causal;
+    if (n != 8 || !number(a[7], &causal) || !window_operands(a, t, lengths, d, false)) Py_RETURN_NONE;
+    d.causal = causal != 0;
+    if (!api.rpfq_window_attention_stat_bytes(&d)) Py_RETURN_NONE;  // shapes that are not taken
+    at::Tensor out;
+    {
+        Unlocked u;
+        if (needs_grad(&t[0]) || needs_grad(&t[1]) || needs_grad(&t[2]))
+            out = Window::apply(t[0], t[1], t[2], lengths.defined() ? std::optional<at::Tensor>(lengths) : std::nullopt, &d);
+        else
+            out = Window::attend(d, t[0], t[1], t[2], lengths, false).first;
+    }
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// window_attention_cached(q, k, v, lengths, window, sinks, scale)
+PyObject* window_attention_cached(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor t[3], lengths;
+    rpfq_window_desc d = {};
+    if (n != 7 || !window_operands(a, t, lengths, d, true) || needs_grad(&t[0]) || needs_grad(&t[1]) || needs_grad(&t[2])) Py_RETURN_NONE;
+    at::Tensor out;
+    int rc;
+    {
+        Unlocked u;
+        const at::Tensor& q = t[0];
+        const c10::DeviceGuard guard(q.device());
+        const auto options = q.options().requires_grad(false);
+        out = at::empty(q.sizes(), options);
+        const size_t bytes = api.rpfq_window_attention_cached_workspace_bytes(&d);
+        at::Tensor work;
+        if (bytes) work = at::empty({(int64_t)bytes}, options.dtype(at::kByte));
+        rc = api.rpfq_window_attention_cached(&d, q.data_ptr(), t[1].data_ptr(), t[2].data_ptr(), lengths.const_data_ptr<int32_t>(),
+                                              out.data_ptr(), ptr(work), bytes, stream_on(q));
+    }
+    return done(rc, out);
+    END_HANDLE_TH_ERRORS
+}
+
 // The tensors of a list, or false where it is not a list of plain ones.
 bool tensors(PyObject* list, std::vector<const at::Tensor*>& out) {
     if (!PyList_CheckExact(list)) return false;
@@ -881,6 +1022,8 @@ PyMethodDef methods[] = {
     {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rms_norm)), METH_FASTCALL, nullptr},
     {"rms_norm_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rms_norm_int8)), METH_FASTCALL, nullptr},
     {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
+    {"window_attention_cached", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(window_attention_cached)), METH_FASTCALL, nullptr},
+    {"window_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(window_attention)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -865,6 +865,81 @@ int rpfq_rotary(const rpfq_rotary_desc* d, const void* q, const void* k, void* q
     return hip_status(rpfq::launch_rotary(*d, q, k, q_out, k_out, positions, freqs, reinterpret_cast<hipStream_t>(stream)), "rpfq_rotary");
 }
 
+static int check_window(const rpfq_window_desc* d, bool cached) {
+    if (!d) return fail(RPFQ_ERR_NULL, "desc is NULL");
+    if (d->dtype != RPFQ_F16 && d->dtype != RPFQ_BF16) return fail(RPFQ_ERR_DTYPE, "unsupported dtype %d: fp16 or bf16", d->dtype);
+    if (d->B <= 0 || d->N <= 0 || d->H <= 0 || d->KV <= 0 || d->D <= 0 || (cached ? d->M <= 0 : d->M != 0))
+        return fail(RPFQ_ERR_SHAPE, "B=%lld N=%lld H=%lld KV=%lld D=%lld M=%lld must be positive (M: cached only)", (long long)d->B,
+                    (long long)d->N, (long long)d->H, (long long)d->KV, (long long)d->D, (long long)d->M);
+    if (d->D > 128 || d->D % 8) return fail(RPFQ_ERR_SHAPE, "D=%lld must be a multiple of 8 up to 128", (long long)d->D);
+    if (d->H > 1024 || d->H % d->KV) return fail(RPFQ_ERR_SHAPE, "H=%lld (up to 1024) must be a multiple of KV=%lld", (long long)d->H, (long long)d->KV);
+    if (d->N > (1LL << 28) || d->M > (1LL << 28) || d->B > (1LL << 24) || d->B * d->H > (1LL << 24) ||
+        d->B * d->H * (d->N / 32 + 4) > (1LL << 30))
+        return fail(RPFQ_ERR_SHAPE, "takes up to 2^28 tokens, 2^24 heads of a batch and 2^30 of 32 rows each (B=%lld N=%lld H=%lld M=%lld)",
+                    (long long)d->B, (long long)d->N, (long long)d->H, (long long)d->M);
+    if (d->window < 1 || d->sinks < 0) return fail(RPFQ_ERR_VALUE, "window=%lld must be positive, sinks=%lld not negative", (long long)d->window, (long long)d->sinks);
+    if (d->causal & ~1) return fail(RPFQ_ERR_VALUE, "causal must be 0 or 1");
+    if (!(d->scale > 0.0f && d->scale < INFINITY)) return fail(RPFQ_ERR_VALUE, "scale=%g must be positive and finite", (double)d->scale);
+    return RPFQ_OK;
+}
+// strides that the kernels index by: whole 16-byte pieces, 128 rows of a tile within 31 bits
+static bool window_strides(const int64_t (&s)[3]) {
+    return (s[0] | s[1] | s[2]) % 8 == 0 && s[0] >= 0 && s[1] >= 0 && s[2] >= 0 && s[1] < (1LL << 22);
+}
+static int check_window_operands(const rpfq_window_desc* d, const void* q, const void* k, const void* v, const void* out, const int32_t* lengths) {
+    if (!q || !k || !v || !out) return fail(RPFQ_ERR_NULL, "rpfq_window_attention: NULL pointer argument");
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(lengths, 4))
+        return fail(RPFQ_ERR_ALIGN, "q, k, v and out must be 16-byte aligned, lengths 4");
+    if (!window_strides(d->q_stride) || !window_strides(d->k_stride) || !window_strides(d->v_stride))
+        return fail(RPFQ_ERR_ALIGN, "strides must be multiples of 8 elements, below 2^22 between tokens");
+    return RPFQ_OK;
+}
+size_t rpfq_window_attention_stat_bytes(const rpfq_window_desc* d) {
+    if (check_window(d, false) != RPFQ_OK) return 0;
+    return (size_t)(d->B * d->H * rpfq::window_rows(d->N)) * 4;
+}
+int rpfq_window_attention(const rpfq_window_desc* d, const void* q, const void* k, const void* v, const int32_t* lengths, void* out,
+                          float* stat, void* stream) {
+    int rc = check_window(d, false);
+    if (!rc) rc = check_window_operands(d, q, k, v, out, lengths);
+    if (rc) return rc;
+    if (!window_strides(d->out_stride) || !aligned(stat, 256)) return fail(RPFQ_ERR_ALIGN, "out's strides or stat's alignment");
+    return hip_status(rpfq::launch_window_attention(*d, q, k, v, lengths, out, stat, reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_window_attention");
+}
+int rpfq_window_attention_grad(const rpfq_window_desc* d, const void* q, const void* k, const void* v, const int32_t* lengths,
+                               const void* out, const void* grad_out, const float* stat, void* grad_q, void* grad_k, void* grad_v,
+                               void* work, size_t work_bytes, void* stream) {
+    int rc = check_window(d, false);
+    if (!rc) rc = check_window_operands(d, q, k, v, out, lengths);
+    if (rc) return rc;
+    if (!grad_out || !stat || !work || (!grad_q && !grad_k && !grad_v))
+        return fail(RPFQ_ERR_NULL, "rpfq_window_attention_grad: NULL pointer argument");
+    if (!window_strides(d->out_stride) || !window_strides(d->grad_stride) || !aligned(grad_out, 16) || !aligned(stat, 256) ||
+        !aligned(grad_q, 16) || !aligned(grad_k, 16) || !aligned(grad_v, 16) || !aligned(work, 256))
+        return fail(RPFQ_ERR_ALIGN, "gradients must be 16-byte aligned, stat and work 256; strides multiples of 8 elements");
+    const size_t need = rpfq_window_attention_stat_bytes(d);
+    if (work_bytes < need) return fail(RPFQ_ERR_SHAPE, "workspace holds %zu bytes, need %zu", work_bytes, need);
+    return hip_status(rpfq::launch_window_attention_grad(*d, q, k, v, lengths, out, grad_out, stat, grad_q, grad_k, grad_v, work,
+                                                         reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_window_attention_grad");
+}
+size_t rpfq_window_attention_cached_workspace_bytes(const rpfq_window_desc* d) {
+    return check_window(d, true) != RPFQ_OK ? 0 : rpfq::window_cached_bytes(*d);
+}
+int rpfq_window_attention_cached(const rpfq_window_desc* d, const void* q, const void* k, const void* v, const int32_t* lengths, void* out,
+                                 void* work, size_t work_bytes, void* stream) {
+    int rc = check_window(d, true);
+    if (!rc) rc = check_window_operands(d, q, k, v, out, lengths);
+    if (rc) return rc;
+    const size_t need = rpfq::window_cached_bytes(*d);
+    if (!lengths || (need && !work)) return fail(RPFQ_ERR_NULL, "rpfq_window_attention_cached: NULL pointer argument");
+    if (!aligned(work, 256)) return fail(RPFQ_ERR_ALIGN, "work must be 256-byte aligned");
+    if (work_bytes < need) return fail(RPFQ_ERR_SHAPE, "workspace holds %zu bytes, need %zu", work_bytes, need);
+    return hip_status(rpfq::launch_window_attention_cached(*d, q, k, v, lengths, out, work, reinterpret_cast<hipStream_t>(stream)),
+                      "rpfq_window_attention_cached");
+}
+
 size_t rpfq_linear_int8_workspace_bytes(const void* x, int x_dtype, int64_t M, int64_t N, int64_t K, const int8_t* w,
                                         int64_t ld_w) {
     if (check_int8(M, N, K, x_dtype, ld_w) != RPFQ_OK) return 0;

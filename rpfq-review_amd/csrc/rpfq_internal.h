@@ -441,6 +441,17 @@ int norm_grad_parts(int64_t M, int64_t C);
 // x: the norm's input, the sum with a residual; gh, gw NULL: none
 hipError_t launch_rms_norm_grad(const NormCall& c, const void* gy, const void* gh, const float* rstd, void* gx, void* gw,
                                 void* work, hipStream_t s);
+// attention with a window (window_attention.hip); statistics of window_rows(N) rows a head
+inline int64_t window_rows(int64_t N) { return (N + 63) / 64 * 64; }
+hipError_t launch_window_attention(const rpfq_window_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths,
+                                   void* out, float* stat, hipStream_t s);
+hipError_t launch_window_attention_grad(const rpfq_window_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths,
+                                        const void* out, const void* grad_out, const float* stat, void* gq, void* gk, void* gv,
+                                        void* work, hipStream_t s);
+size_t window_cached_bytes(const rpfq_window_desc& d);
+hipError_t launch_window_attention_cached(const rpfq_window_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths,
+                                          void* out, void* work, hipStream_t s);
+
 // rotary positions (rotary.hip)
 hipError_t launch_rotary(const rpfq_rotary_desc& d, const void* q, const void* k, void* q_out, void* k_out, const void* pos,
                          const double* freqs, hipStream_t s);

@@ -1,0 +1,919 @@
+// Attention with a sliding window and first tokens that stay visible (sinks),
+// over whole sequences with its gradient, and for the last tokens over a cache.
+// Query i sees key j of its sequence where
+//   causal:  j <= i and (i - j < window or j < sinks),
+//   else:    |i - j| < window or j < sinks or i < sinks;
+//   O = P V,  P = softmax(scale Q K^T) over what is seen, 0 for a row without any.
+// Gradient, with P = exp(S - lse) formed again from the row's statistic:
+//   dV = P^T dO,  dS = P (dO V^T - rowsum(dO O)),  dQ = scale dS K,  dK = scale dS^T Q.
+#include "tile_gemm.h"
+
+namespace rpfq {
+
+// A tile's rows in LDS: DP values of 16 bits (the head's size, rounded up to
+// 32; zeros behind it), chunks of 16 bytes.  Chunk c lies at c ^ swz(row): both
+// reads below fall on all banks, 16 rows of one chunk (a 32 x 32 product's rows)
+// and 4 rows x 64 bytes (the transposed read).
+template <int DP>
+struct Rows {
+    static constexpr int RB = DP <= 32 ? 64 : DP <= 64 ? 128 : 256;  // bytes of a row
+    static constexpr int CH = RB / 16;
+    static constexpr int PER = 1024 / RB;  // rows of one DMA load
+    static __device__ __forceinline__ int swz(int row) {
+        return CH == 16 ? (row & 3) << 2 | ((row >> 2) & 3) : CH == 8 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : (row >> 2) & 3;
+    }
+};
+
+// The loads of a tile of R rows by WAVES waves: row `row` of the tile from
+// base + row ld, rows past `end` bytes and chunks past D as zeros.
+template <int DP, int R, int WAVES>
+struct RowLoads {
+    static constexpr int TOTAL = R / Rows<DP>::PER, LOADS = (TOTAL + WAVES - 1) / WAVES;
+    uint32_t off[LOADS];
+    __device__ __forceinline__ void init(int64_t ld, int D, int wave, int lane) {
+#pragma unroll
+        for (int p = 0; p < LOADS; ++p) {
+            const int row = (wave + p * WAVES) * Rows<DP>::PER + lane / Rows<DP>::CH;
+            const int c = (lane & (Rows<DP>::CH - 1)) ^ Rows<DP>::swz(row);
+            off[p] = 8 * c < D ? (uint32_t)(row * (int)ld + 16 * c) : kTileOut;
+        }
+    }
+    // rows first .. of a tensor whose rows 0 .. n - 1 count
+    __device__ __forceinline__ void issue(const char* base, int64_t ld, int D, int first, int n, uint32_t lds, int wave) const {
+        intx4 rs = tile_rsrc(base + (int64_t)first * ld);
+        const int64_t end = (int64_t)(n - first - 1) * ld + 2 * D;
+        rs[2] = __builtin_amdgcn_readfirstlane(n <= first ? 0 : (int)(end > 0x7fffffff ? 0x7fffffff : end));
+#pragma unroll
+        for (int p = 0; p < LOADS; ++p)
+            if (TOTAL % WAVES == 0 || wave + p * WAVES < TOTAL) dma_buffer(rs, off[p], lds + (wave + p * WAVES) * 1024);
+    }
+};
+
+// Fragments of a tile's 32-row block: rows as they lie (the product's rows, 16
+// values of a row a step), and transposed (the row index is contracted, 16 rows
+// a step: lane half g holds rows 4 g .. + 3 and 8 + 4 g .. + 3, the order in
+// which a 32 x 32 result holds its rows).
+template <int DP>
+struct Frags {
+    uint32_t row[DP / 16], col[DP / 32][2];
+    __device__ __forceinline__ void init(int lane) {
+        using T = Rows<DP>;
+        const int r = lane & 31, g = lane >> 5, i16 = lane & 15, hf = (lane >> 4) & 1;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) row[s] = r * T::RB + (((2 * s + g) ^ T::swz(r)) * 16);
+        const int tr = 4 * g + (i16 >> 2);
+#pragma unroll
+        for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                col[j][h] = (tr + 8 * h) * T::RB + (((4 * j + 2 * hf + ((i16 & 3) >> 1)) ^ T::swz(tr + 8 * h)) * 16) + (i16 & 1) * 8;
+    }
+    __device__ __forceinline__ uint4 rows(uint32_t at, int s) const {
+        return __builtin_bit_cast(uint4, *reinterpret_cast<__attribute__((address_space(3))) const u32x4*>(at + row[s]));
+    }
+    __device__ __forceinline__ uint4 cols(uint32_t at, int j) const {
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)(at + col[j][0]));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)(at + col[j][1]));
+        return __builtin_bit_cast(uint4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
+
+template <bool BF>
+__device__ __forceinline__ floatx16 win_mma(uint4 a, uint4 b, floatx16 c) {
+    if constexpr (BF) return MmaBf16::mma(a, b, c);
+    return MmaF16::mma(a, b, c);
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t win_pack(float lo, float hi) {
+    if constexpr (BF) return pack_bf2(lo, hi);
+    return cvt_pk(lo, hi);
+}
+// 8 values of a 32 x 32 result as the other operand's 16 rows
+template <bool BF>
+__device__ __forceinline__ uint4 win_pack8(const floatx16& s, int u) {
+    return make_uint4(win_pack<BF>(s[8 * u], s[8 * u + 1]), win_pack<BF>(s[8 * u + 2], s[8 * u + 3]),
+                      win_pack<BF>(s[8 * u + 4], s[8 * u + 5]), win_pack<BF>(s[8 * u + 6], s[8 * u + 7]));
+}
+// c + lo + hi of a 16-bit pair
+template <bool BF>
+__device__ __forceinline__ float win_sum2(uint32_t v, float c) {
+    if constexpr (BF) {
+        typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, v), __builtin_bit_cast(bf2, 0x3f803f80u), c, false);
+    } else {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, v), __builtin_bit_cast(half2v, 0x3c003c00u), c, false);
+    }
+}
+// c + a . b of 8 pairs of 16 bits, in float32
+template <bool BF>
+__device__ __forceinline__ float win_dot8(uint4 a, uint4 b, float c) {
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        if (BF) {
+            c = fmaf(bf16_to_f32(x[t] & 0xffffu), bf16_to_f32(y[t] & 0xffffu), c);
+            c = fmaf(bf16_to_f32(x[t] >> 16), bf16_to_f32(y[t] >> 16), c);
+        } else {
+            const half2v h = __builtin_bit_cast(half2v, x[t]), k = __builtin_bit_cast(half2v, y[t]);
+            c = fmaf((float)h[0], (float)k[0], c);
+            c = fmaf((float)h[1], (float)k[1], c);
+        }
+    }
+    return c;
+}
+
+// Probabilities are formed times 2^-kWinShift.  fp16: 2^15, normal down to 2^-29
+// of the row's largest.  bf16 has float32's range and so have its values: 2^-20,
+// so that a million of them stay within float32.
+template <bool BF>
+constexpr float win_shift() { return BF ? 20.0f : -15.0f; }
+
+struct WinArgs {
+    const char *q, *k, *v, *o, *go;     // o: out of the forward, in of the gradient
+    char *out, *gq, *gk, *gv;
+    int64_t qs[3], ks[3], vs[3], os[3], gos[3];  // bytes between batches, tokens, heads
+    const int32_t* lengths;
+    float *stat, *delta;                // [B, H, NP]
+    int B, N, H, KV, D, NP;
+    int window, sinks, causal;
+    int hw, qw, tiles;                  // heads and 32-query blocks of a workgroup; query tiles
+    float scale, scale2;                // scale2 = scale log2(e)
+    // cached
+    int M, rows, blocks, splits;        // keys of the cache; queries of a key head; their 32-row blocks
+    float* part;
+};
+
+__device__ __forceinline__ int win_length(const WinArgs& a, int b, int most) {
+    if (!a.lengths) return most;
+    const int n = a.lengths[b];
+    return n < 0 ? 0 : n > most ? most : n;
+}
+// What a pair sees, without a branch: d = i - j within [-off, span - off), or a
+// sink with d >= least.
+struct WinMask {
+    int off, sinks, least, n, causal;
+    uint32_t span;
+    __device__ __forceinline__ WinMask(const WinArgs& a, int n_)
+        : off(a.causal ? 0 : a.window - 1), sinks(a.sinks), least(a.causal ? 0 : -0x7fffffff), n(n_), causal(a.causal),
+          span(a.causal ? (uint32_t)a.window : 2u * (uint32_t)a.window - 1u) {}
+    __device__ __forceinline__ bool operator()(int i, int j) const {
+        const int d = i - j;
+        const bool near = (uint32_t)(d + off) < span, first = (j < sinks) | ((i < sinks) & !causal);
+        return (j < n) & (near | (first & (d >= least)));
+    }
+};
+// What queries q0 .. q1 see of keys k0 .. k1: 0 nothing, 1 some, 2 all.
+__device__ __forceinline__ int win_class(const WinArgs& a, int q0, int q1, int k0, int k1) {
+    if (a.causal) {
+        if (k0 > q1 || (q0 - k1 >= a.window && k0 >= a.sinks)) return 0;
+        return k1 <= q0 && (q1 - k0 < a.window || k1 < a.sinks) ? 2 : 1;
+    }
+    if ((q0 - k1 >= a.window || k0 - q1 >= a.window) && k0 >= a.sinks && q0 >= a.sinks) return 0;
+    return (q1 - k0 < a.window && k1 - q0 < a.window) || k1 < a.sinks || q1 < a.sinks ? 2 : 1;
+}
+
+// The tiles of T keys that queries q0 .. q1 (< n) see: `first` tiles of the
+// sinks, then [t0, t1).
+struct WinTiles {
+    int first, t0, count;
+    __device__ __forceinline__ int at(int s) const { return s < first ? s : t0 + s - first; }
+};
+template <int T>
+__device__ __forceinline__ WinTiles win_tiles(const WinArgs& a, int q0, int q1, int n) {
+    int lo = q0 - a.window + 1, hi = a.causal ? q1 + 1 : q1 + a.window;
+    if (!a.causal && q0 < a.sinks) lo = 0, hi = n;
+    lo = lo < 0 ? 0 : lo;
+    hi = hi > n ? n : hi;
+    WinTiles t;
+    t.first = ((a.sinks < lo ? a.sinks : lo) + T - 1) / T;
+    t.t0 = lo / T > t.first ? lo / T : t.first;
+    const int t1 = (hi + T - 1) / T;
+    t.count = q1 < q0 ? 0 : t.first + (t1 > t.t0 ? t1 - t.t0 : 0);
+    return t;
+}
+
+// 32 rows of DP results [d][row] as 16-bit values: after trading halves across
+// the 32 lanes each lane has 8 consecutive ones.
+template <int DP, bool BF>
+__device__ __forceinline__ void win_store(const floatx16 (&o)[DP / 32], float f, bool zero, bool inside, char* dst, int D, int g) {
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            uint32_t x[2], y[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                x[e] = win_pack<BF>(o[j][8 * p + 2 * e] * f, o[j][8 * p + 2 * e + 1] * f);
+                y[e] = win_pack<BF>(o[j][8 * p + 4 + 2 * e] * f, o[j][8 * p + 5 + 2 * e] * f);
+                if (zero) x[e] = y[e] = 0;
+            }
+            const auto s0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+            const int d = 32 * j + 16 * p + 8 * g;
+            if (inside && d < D) *reinterpret_cast<uint4*>(dst + 2 * d) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+        }
+}
+
+// A 16-bit row's values 16 s + 8 g .. + 7 (zeros past D or where it is not inside).
+template <int DP>
+__device__ __forceinline__ void win_row(uint4 (&f)[DP / 16], const char* src, bool inside, int D, int g) {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+        f[s] = make_uint4(0, 0, 0, 0);
+        if (inside && 16 * s + 8 * g < D) f[s] = *reinterpret_cast<const uint4*>(src + 32 * s + 16 * g);
+    }
+}
+
+__device__ __forceinline__ void win_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// The running softmax of a lane's query over 32 more keys (two lanes hold one
+// query's 32 scores, half each): `top` the largest score so far, `sub` = top
+// scale2 + shift as it is rounded, the exponent that is subtracted; l the sum.
+struct WinState {
+    float top, sub, l;
+};
+// P of KB blocks of 32 scores in place; returns the factor of what was summed before.
+template <int KB, bool BF>
+__device__ __forceinline__ float win_softmax(floatx16 (&s)[KB], WinState& st, float scale2) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[kb][v]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float top = fmaxf(st.top, mx);
+    const float base = top == -__builtin_inff() ? 0.0f : top;  // nothing seen yet: exp2(-inf) is 0
+    const float sub = fmaf(base, scale2, win_shift<BF>());
+    float f;
+    // scores far from 0: the rounding of `sub` would carry probabilities out of
+    // fp16's range, so the largest is subtracted first
+    if (__any(fabsf(base) * scale2 > 0x1p20f)) {
+        f = __builtin_amdgcn_exp2f((st.top - base) * scale2);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[kb][v] = __builtin_amdgcn_exp2f(fmaf(s[kb][v] - base, scale2, -win_shift<BF>()));
+    } else {
+        f = __builtin_amdgcn_exp2f(st.sub - sub);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[kb][v] = __builtin_amdgcn_exp2f(fmaf(s[kb][v], scale2, -sub));
+    }
+    st.top = top;
+    st.sub = top == -__builtin_inff() ? -__builtin_inff() : sub;
+    st.l *= f;
+    return f;
+}
+
+// Where a workgroup of four waves stands: wave w has head hw h0 + w % hw and the
+// 32-query block w / hw of its tile.  Heads that share keys sit together, so a
+// tile is narrow and its window little wider than one query's.
+struct WinPlace {
+    int b, h, kv, q0, q1, mine, n;  // tile's first and last query (< n), first of this wave
+};
+__device__ __forceinline__ WinPlace win_place(const WinArgs& a, int wave) {
+    WinPlace p;
+    const int u = xcd_tile(blockIdx.x, gridDim.x);
+    const int t = u % a.tiles, rest = u / a.tiles, groups = a.H / a.hw;
+    p.b = rest / groups;
+    const int h0 = (rest - p.b * groups) * a.hw;
+    p.h = h0 + wave % a.hw;
+    p.kv = h0 / (a.H / a.KV);
+    const int tile = a.causal ? a.tiles - 1 - t : t;  // the longest first
+    p.q0 = tile * 32 * a.qw;
+    p.mine = p.q0 + 32 * (wave / a.hw);
+    p.n = win_length(a, p.b, a.N);
+    p.q1 = (p.q0 + 32 * a.qw < p.n ? p.q0 + 32 * a.qw : p.n) - 1;
+    return p;
+}
+
+// Forward.  S^T = K Q^T: a lane holds one query's scores, so the softmax is
+// in-lane but for one exchange, and the probabilities, rounded to 16 bits, are
+// already the operand of O^T = V^T P^T.  K and V tiles of 64 keys go to LDS by
+// DMA, the next one while this one is used.
+template <int DP, bool BF>
+__global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr int T = 64, TILE = T * Rows<DP>::RB;  // K, then V; twice
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const WinPlace p = win_place(a, wave);
+    const int i = p.mine + r, last = (p.mine + 31 < p.n - 1 ? p.mine + 31 : p.n - 1);
+    uint4 q[DP / 16];
+    win_row<DP>(q, a.q + p.b * a.qs[0] + (int64_t)i * a.qs[1] + p.h * a.qs[2], i < p.n, a.D, g);
+    const WinTiles tiles = win_tiles<T>(a, p.q0, p.q1, p.n);
+    RowLoads<DP, T, 4> lk, lv;
+    lk.init(a.ks[1], a.D, wave, lane);
+    lv.init(a.vs[1], a.D, wave, lane);
+    Frags<DP> at;
+    at.init(lane);
+    const char *kbase = a.k + p.b * a.ks[0] + p.kv * a.ks[2], *vbase = a.v + p.b * a.vs[0] + p.kv * a.vs[2];
+    const uint32_t lds = lds_addr(smem);
+    auto issue = [&](int s) {
+        const int first = tiles.at(s) * T;
+        const uint32_t to = lds + (s & 1) * 2 * TILE;
+        lk.issue(kbase, a.ks[1], a.D, first, p.n, to, wave);
+        lv.issue(vbase, a.vs[1], a.D, first, p.n, to + TILE, wave);
+    };
+    const WinMask mask(a, p.n);
+    WinState st = {-__builtin_inff(), -__builtin_inff(), 0.0f};
+    floatx16 o[DP / 32];
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
+    if (tiles.count) issue(0);
+    for (int t = 0; t < tiles.count; ++t) {
+        win_sync();
+        if (t + 1 < tiles.count) issue(t + 1);
+        const int k0 = tiles.at(t) * T;
+        const int seen = last < p.mine ? 0 : win_class(a, p.mine, last, k0, k0 + T - 1);
+        if (!seen) continue;
+        const uint32_t kt = lds + (t & 1) * 2 * TILE, vt = kt + TILE;
+        floatx16 s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            s[kb] = floatx16{0};
+#pragma unroll
+            for (int e = 0; e < DP / 16; ++e) s[kb] = win_mma<BF>(at.rows(kt + kb * 32 * Rows<DP>::RB, e), q[e], s[kb]);
+        }
+        if (seen == 1 || k0 + T > p.n) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
+                    s[kb][v] = in ? s[kb][v] : -__builtin_inff();
+                }
+        }
+        const float f = win_softmax<2, BF>(s, st, a.scale2);
+        if (__any(f != 1.0f)) {
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[j][v] *= f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint4 pr = win_pack8<BF>(s[u >> 1], u & 1);
+            // the sum of the rounded probabilities: their rounding errors then
+            // weigh the values' distance to the output, not the values
+            st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j) o[j] = win_mma<BF>(at.cols(vt + u * 16 * Rows<DP>::RB, j), pr, o[j]);
+        }
+    }
+    const float l = st.l + __shfl_xor(st.l, 32, 64);
+    const bool any = l != 0.0f && i < p.n;
+    // the gradient's probabilities are exp2(S scale2 + stat), times 2^15 in fp16
+    if (a.stat && g == 0 && i < a.NP)
+        a.stat[((int64_t)p.b * a.H + p.h) * a.NP + i] = any ? (BF ? 0.0f : 15.0f) - (st.sub + __builtin_amdgcn_logf(l)) : -__builtin_inff();
+    win_store<DP, BF>(o, any ? 1.0f / l : 0.0f, !any, i < a.N, a.out + p.b * a.os[0] + (int64_t)i * a.os[1] + p.h * a.os[2], a.D, g);
+}
+
+// fp16 gradients: dS is carried times a power of two of its column (one query in
+// dQ, one key in dK), so that the largest so far lies in [2^14, 2^15): the
+// sums are float32 and follow it down where a larger one comes.
+__device__ __forceinline__ float win_lower(float c, float mx) {
+    const int e = 15 - __builtin_amdgcn_frexp_expf(mx);
+    const float to = __builtin_amdgcn_ldexpf(1.0f, e < -126 ? -126 : e > 126 ? 126 : e);
+    return to < c ? to : c;
+}
+template <int DP, bool BF>
+__device__ __forceinline__ void win_scale_ds(floatx16& ds, float& c, floatx16 (&o)[DP / 32]) {
+    if constexpr (!BF) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, fabsf(ds[v]));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        if (__any(mx * c > 0x1p15f)) {
+            const float to = mx * c > 0x1p15f ? win_lower(c, mx) : c, f = to / c;
+            c = to;
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[j][v] *= f;
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) ds[v] *= c;
+    }
+}
+
+// Gradient of the queries, laid out as the forward: S^T = K Q^T and dP^T = V dO^T
+// in one lane's query, dQ^T = K^T dS^T.  Leaves rowsum(dO O) for the other.
+template <int DP, bool BF>
+__global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr int T = 64, TILE = T * Rows<DP>::RB;
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const WinPlace p = win_place(a, wave);
+    const int i = p.mine + r, last = (p.mine + 31 < p.n - 1 ? p.mine + 31 : p.n - 1);
+    const int64_t row = ((int64_t)p.b * a.H + p.h) * a.NP + i;
+    uint4 q[DP / 16], go[DP / 16];
+    win_row<DP>(q, a.q + p.b * a.qs[0] + (int64_t)i * a.qs[1] + p.h * a.qs[2], i < p.n, a.D, g);
+    win_row<DP>(go, a.go + p.b * a.gos[0] + (int64_t)i * a.gos[1] + p.h * a.gos[2], i < p.n, a.D, g);
+    float delta = 0.0f;
+    {
+        uint4 out[DP / 16];
+        win_row<DP>(out, a.o + p.b * a.os[0] + (int64_t)i * a.os[1] + p.h * a.os[2], i < p.n, a.D, g);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) delta = win_dot8<BF>(go[s], out[s], delta);
+        delta += __shfl_xor(delta, 32, 64);
+    }
+    if (g == 0 && i < a.NP) a.delta[row] = delta;
+    const float stat = i < a.NP ? a.stat[row] : -__builtin_inff();
+    if (!a.gq) return;
+    const WinTiles tiles = win_tiles<T>(a, p.q0, p.q1, p.n);
+    RowLoads<DP, T, 4> lk, lv;
+    lk.init(a.ks[1], a.D, wave, lane);
+    lv.init(a.vs[1], a.D, wave, lane);
+    Frags<DP> at;
+    at.init(lane);
+    const char *kbase = a.k + p.b * a.ks[0] + p.kv * a.ks[2], *vbase = a.v + p.b * a.vs[0] + p.kv * a.vs[2];
+    const uint32_t lds = lds_addr(smem);
+    auto issue = [&](int s) {
+        const int first = tiles.at(s) * T;
+        const uint32_t to = lds + (s & 1) * 2 * TILE;
+        lk.issue(kbase, a.ks[1], a.D, first, p.n, to, wave);
+        lv.issue(vbase, a.vs[1], a.D, first, p.n, to + TILE, wave);
+    };
+    const WinMask mask(a, p.n);
+    floatx16 o[DP / 32];
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
+    float c = BF ? 1.0f : 0x1p126f;
+    if (tiles.count) issue(0);
+    for (int t = 0; t < tiles.count; ++t) {
+        win_sync();
+        if (t + 1 < tiles.count) issue(t + 1);
+        const int k0 = tiles.at(t) * T;
+        const int seen = last < p.mine ? 0 : win_class(a, p.mine, last, k0, k0 + T - 1);
+        if (!seen) continue;
+        const bool some = seen == 1 || k0 + T > p.n;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const uint32_t kt = lds + (t & 1) * 2 * TILE + kb * 32 * Rows<DP>::RB, vt = kt + TILE;
+            floatx16 s = floatx16{0}, dp = floatx16{0};
+#pragma unroll
+            for (int e = 0; e < DP / 16; ++e) s = win_mma<BF>(at.rows(kt, e), q[e], s);
+#pragma unroll
+            for (int e = 0; e < DP / 16; ++e) dp = win_mma<BF>(at.rows(vt, e), go[e], dp);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, stat)) * (dp[v] - delta);
+            if (some) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
+                    s[v] = in ? s[v] : 0.0f;
+                }
+            }
+            win_scale_ds<DP, BF>(s, c, o);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint4 ds = win_pack8<BF>(s, u);
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j) o[j] = win_mma<BF>(at.cols(kt + u * 16 * Rows<DP>::RB, j), ds, o[j]);
+            }
+        }
+    }
+    char* dst = a.gq + (((int64_t)p.b * a.N + i) * a.H + p.h) * 2 * a.D;
+    win_store<DP, BF>(o, a.scale * (BF ? 1.0f : 0x1p-15f) / c, i >= p.n, i < a.N, dst, a.D, g);
+}
+
+// Gradient of the keys and values: a workgroup of eight waves has 128 keys, 32 to
+// a wave and its fellow, which take every other 32 of the queries that see them,
+// of all heads that share them.  S = Q K^T and dP = dO V^T with a key to a lane:
+// P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS.  K stays in
+// registers, V in LDS (with both, 128-value heads spill).
+constexpr int kWinKeys = 128, kWinStep = 64;
+template <int DP>
+constexpr int win_grad_lds() {
+    const int rows = Rows<DP>::RB * (kWinKeys + 4 * kWinStep) + 4 * kWinStep * 4;
+    const int sums = 4 * 32 * (DP + 4) * 4;
+    return rows > sums ? rows : sums;
+}
+template <int DP, bool BF>
+__global__ void __launch_bounds__(512, 2) window_grad_kv_kernel(WinArgs a) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr int RB = Rows<DP>::RB, V = kWinKeys * RB, STAGE = 2 * kWinStep * RB;  // V, two stages of Q and dO, their statistics
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), block = wave & 3, half = wave >> 2;
+    const int u = xcd_tile(blockIdx.x, gridDim.x), tiles_n = (a.N + kWinKeys - 1) / kWinKeys;
+    const int tile = u % tiles_n, rest = u / tiles_n, b = rest / a.KV, kv = rest - b * a.KV, group = a.H / a.KV;
+    const int n = win_length(a, b, a.N), k0 = tile * kWinKeys, mine = k0 + 32 * block, key = mine + r;
+    const int klast = (mine + 31 < n - 1 ? mine + 31 : n - 1), kend = (k0 + kWinKeys < n ? k0 + kWinKeys : n) - 1;
+    uint4 kf[DP / 16];
+    win_row<DP>(kf, a.k + b * a.ks[0] + (int64_t)key * a.ks[1] + kv * a.ks[2], key < n, a.D, g);
+    // the queries that see them: first tiles (seeing all), then [t0, t1), for each head
+    int lo = a.causal ? k0 : k0 - a.window + 1, hi = kend + a.window;
+    if (k0 < a.sinks) hi = n, lo = a.causal ? lo : 0;
+    lo = lo < 0 ? 0 : lo;
+    hi = hi > n ? n : hi;
+    WinTiles q;
+    q.first = a.causal ? 0 : ((a.sinks < lo ? a.sinks : lo) + kWinStep - 1) / kWinStep;
+    q.t0 = lo / kWinStep > q.first ? lo / kWinStep : q.first;
+    const int t1 = (hi + kWinStep - 1) / kWinStep;
+    q.count = kend < k0 ? 0 : q.first + (t1 > q.t0 ? t1 - q.t0 : 0);
+    const int steps = q.count * group;
+
+    RowLoads<DP, kWinStep, 8> lq, lo_;
+    lq.init(a.qs[1], a.D, wave, lane);
+    lo_.init(a.gos[1], a.D, wave, lane);
+    Frags<DP> at;
+    at.init(lane);
+    const uint32_t lds = lds_addr(smem), stats = lds + V + 2 * STAGE;
+    int head = 0, qt = 0;  // of the step that is issued next
+    auto issue = [&](int s) {
+        const int h = kv * group + head, first = q.at(qt) * kWinStep;
+        const uint32_t to = lds + V + (s & 1) * STAGE;
+        lq.issue(a.q + b * a.qs[0] + h * a.qs[2], a.qs[1], a.D, first, n, to, wave);
+        lo_.issue(a.go + b * a.gos[0] + h * a.gos[2], a.gos[1], a.D, first, n, to + kWinStep * RB, wave);
+        const int64_t row = ((int64_t)b * a.H + h) * a.NP + first;
+        if (wave == 0) dma_dword(a.stat + row, lane * 4, stats + (s & 1) * 2 * kWinStep * 4);
+        if (wave == 1) dma_dword(a.delta + row, lane * 4, stats + (s & 1) * 2 * kWinStep * 4 + kWinStep * 4);
+        if (++qt == q.count) qt = 0, ++head;
+    };
+    if (steps) {
+        RowLoads<DP, kWinKeys, 8> lv;
+        lv.init(a.vs[1], a.D, wave, lane);
+        lv.issue(a.v + b * a.vs[0] + kv * a.vs[2], a.vs[1], a.D, k0, n, lds, wave);
+        issue(0);
+    }
+    floatx16 ok[DP / 32], ov[DP / 32];
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j) ok[j] = ov[j] = floatx16{0};
+    const WinMask mask(a, n);
+    float c = BF ? 1.0f : 0x1p126f;
+    int ct = 0;
+    for (int t = 0; t < steps; ++t) {
+        win_sync();
+        if (t + 1 < steps) issue(t + 1);
+        const int q0 = q.at(ct) * kWinStep + 32 * half, qlast = (q0 + 31 < n - 1 ? q0 + 31 : n - 1);
+        if (++ct == q.count) ct = 0;
+        const int seen = qlast < q0 || klast < mine ? 0 : win_class(a, q0, qlast, mine, klast);
+        if (!seen) continue;
+        const uint32_t qtile = lds + V + (t & 1) * STAGE + 32 * half * RB, otile = qtile + kWinStep * RB;
+        const uint32_t st = stats + (t & 1) * 2 * kWinStep * 4 + 32 * half * 4 + 16 * g, vt = lds + 32 * block * RB;
+        typedef __attribute__((address_space(3))) const f32x4* lds_f4_t;
+        floatx16 s = floatx16{0}, dp = floatx16{0};
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) s = win_mma<BF>(at.rows(qtile, e), kf[e], s);
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) dp = win_mma<BF>(at.rows(otile, e), at.rows(vt, e), dp);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const f32x4 sv = *reinterpret_cast<lds_f4_t>(st + 32 * w), dv = *reinterpret_cast<lds_f4_t>(st + kWinStep * 4 + 32 * w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = 4 * w + e;
+                s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, sv[e]));
+                dp[v] = s[v] * (dp[v] - dv[e]);
+            }
+        }
+        if (seen == 1) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const bool in = mask(q0 + acc_row(v, g), key);
+                s[v] = in ? s[v] : 0.0f;
+                dp[v] = in ? dp[v] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint4 pr = win_pack8<BF>(s, e);
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j) ov[j] = win_mma<BF>(at.cols(otile + e * 16 * RB, j), pr, ov[j]);
+        }
+        win_scale_ds<DP, BF>(dp, c, ok);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint4 ds = win_pack8<BF>(dp, e);
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j) ok[j] = win_mma<BF>(at.cols(qtile + e * 16 * RB, j), ds, ok[j]);
+        }
+    }
+    // the fellow's sums through LDS, one tensor after the other
+    const float fk = a.scale * (BF ? 1.0f : 0x1p-15f), fv = BF ? 1.0f : 0x1p-15f;
+    float* sums = reinterpret_cast<float*>(smem) + (block * 32 + r) * (DP + 4);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        floatx16(&o)[DP / 32] = w ? ov : ok;
+        const float f = w ? 1.0f : 1.0f / c;
+        win_sync();
+        if (half) {
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; v += 4)
+                    *reinterpret_cast<f32x4*>(sums + 32 * j + acc_row(v, g)) =
+                        (f32x4){o[j][v] * f, o[j][v + 1] * f, o[j][v + 2] * f, o[j][v + 3] * f};
+        }
+        win_sync();
+        if (!half) {
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; v += 4) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(sums + 32 * j + acc_row(v, g));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][v + e] = o[j][v + e] * f + x[e];
+                }
+            char* dst = w ? a.gv : a.gk;
+            if (dst)
+                win_store<DP, BF>(o, w ? fv : fk, key >= n, key < a.N, dst + (((int64_t)b * a.N + key) * a.KV + kv) * 2 * a.D, a.D, g);
+        }
+    }
+}
+
+// The last tokens over a cache.  A workgroup has one key head of one sequence,
+// up to 32 of its rows (queries x heads that share it) and a part of the keys; its
+// waves take tiles of 32 keys in turn, each through LDS of its own, without
+// waiting for each other.  Parts are joined by window_join_kernel.
+template <int DP, bool BF>
+__global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr int T = 32, RB = Rows<DP>::RB, TILE = T * RB, LOADS = T / Rows<DP>::PER;
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = a.H / a.KV;
+    int u = blockIdx.x;
+    const int split = u % a.splits;
+    u /= a.splits;
+    const int blk = u % a.blocks;
+    u /= a.blocks;
+    const int kv = u % a.KV, b = u / a.KV;
+    const int row = 32 * blk + r, tok = row / group, h = kv * group + row - tok * group;
+    const bool inside = row < a.rows;
+    const int len = win_length(a, b, a.M), i = len - a.N + tok;
+    uint4 q[DP / 16];
+    win_row<DP>(q, a.q + b * a.qs[0] + tok * a.qs[1] + h * a.qs[2], inside, a.D, g);
+
+    const int lo = len - a.N - a.window + 1 < 0 ? 0 : len - a.N - a.window + 1;
+    const int sinks = a.sinks < len ? a.sinks : len;
+    const int first = ((sinks < lo ? sinks : lo) + T - 1) / T, t0 = lo / T > first ? lo / T : first;
+    const int t1 = (len + T - 1) / T, count = first + (t1 > t0 ? t1 - t0 : 0);
+    const int from = (int)((int64_t)count * split / a.splits), to = (int)((int64_t)count * (split + 1) / a.splits);
+
+    const uint32_t lds = lds_addr(smem) + wave * 4 * TILE;  // K, V; twice
+    const char *kbase = a.k + b * a.ks[0] + kv * a.ks[2], *vbase = a.v + b * a.vs[0] + kv * a.vs[2];
+    // slots that no query sees are not read: what they hold is not to count
+    auto issue = [&](int s, int buf) {
+        const int j0 = (s < first ? s : t0 + s - first) * T;
+        intx4 rk = tile_rsrc(kbase + (int64_t)j0 * a.ks[1]), rv = tile_rsrc(vbase + (int64_t)j0 * a.vs[1]);
+#pragma unroll
+        for (int p = 0; p < LOADS; ++p) {
+            const int x = p * Rows<DP>::PER + lane / Rows<DP>::CH, j = j0 + x;
+            const int ch = (lane & (Rows<DP>::CH - 1)) ^ Rows<DP>::swz(x);
+            const bool in = 8 * ch < a.D && j < len && (j >= lo || j < sinks);
+            dma_buffer(rk, in ? (uint32_t)(x * (int)a.ks[1] + 16 * ch) : kTileOut, lds + buf * 2 * TILE + p * 1024);
+            dma_buffer(rv, in ? (uint32_t)(x * (int)a.vs[1] + 16 * ch) : kTileOut, lds + buf * 2 * TILE + TILE + p * 1024);
+        }
+    };
+    Frags<DP> at;
+    at.init(lane);
+    WinState st = {-__builtin_inff(), -__builtin_inff(), 0.0f};
+    floatx16 o[DP / 32];
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
+    const WinMask mask(a, len);
+    int s = from + wave, buf = 0;
+    if (s < to) issue(s, 0);
+    for (; s < to; s += 4, buf ^= 1) {
+        if (s + 4 < to) {
+            issue(s + 4, buf ^ 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        const uint32_t kt = lds + buf * 2 * TILE, vt = kt + TILE;
+        const int j0 = (s < first ? s : t0 + s - first) * T;
+        floatx16 sc[1] = {floatx16{0}};
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) sc[0] = win_mma<BF>(at.rows(kt, e), q[e], sc[0]);
+        // all of it seen by every row, or not
+        if (j0 + T > len - a.N + 1 || (len - 1 - j0 >= a.window && j0 + T > sinks)) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const bool in = mask(i, j0 + acc_row(v, g));
+                sc[0][v] = in ? sc[0][v] : -__builtin_inff();
+            }
+        }
+        const float f = win_softmax<1, BF>(sc, st, a.scale2);
+        if (__any(f != 1.0f)) {
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[j][v] *= f;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint4 pr = win_pack8<BF>(sc[0], e);
+            st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j) o[j] = win_mma<BF>(at.cols(vt + e * 16 * RB, j), pr, o[j]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this buffer is free for the next load
+    }
+    // the four waves' sums, in their order
+    st.l += __shfl_xor(st.l, 32, 64);
+    __syncthreads();
+    constexpr int LD = DP + 4;
+    float* sums = reinterpret_cast<float*>(smem);  // [wave][row][LD]
+    float* ml = sums + 4 * 32 * LD;                // [wave][row][2]
+    if (inside) {
+#pragma unroll
+        for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; v += 4)
+                *reinterpret_cast<f32x4*>(sums + (wave * 32 + r) * LD + 32 * j + acc_row(v, g)) =
+                    (f32x4){o[j][v], o[j][v + 1], o[j][v + 2], o[j][v + 3]};
+        if (g == 0) ml[(wave * 32 + r) * 2] = st.sub, ml[(wave * 32 + r) * 2 + 1] = st.l;
+    }
+    __syncthreads();
+    const int rows = a.rows - 32 * blk < 32 ? a.rows - 32 * blk : 32;
+    for (int e = tid; e < rows * (DP / 8); e += 256) {
+        const int x = e / (DP / 8), d = 8 * (e - x * (DP / 8));
+        float m = -__builtin_inff(), l = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[(w * 32 + x) * 2]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float mw = ml[(w * 32 + x) * 2], f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
+            l += f * ml[(w * 32 + x) * 2 + 1];
+            if (mw != -__builtin_inff())
+#pragma unroll
+                for (int t = 0; t < 8; ++t) v[t] = fmaf(f, sums[(w * 32 + x) * LD + d + t], v[t]);
+        }
+        const int orow = 32 * blk + x, ot = orow / group, oh = kv * group + orow - ot * group;
+        if (a.splits > 1) {
+            const int64_t at_ = (((int64_t)b * a.N + ot) * a.H + oh) * a.splits + split;
+            float* dst = a.part + at_ * (DP + 8);  // 8 DP-piece, then the exponent and the sum
+#pragma unroll
+            for (int t = 0; t < 8; t += 4) *reinterpret_cast<f32x4*>(dst + d + t) = (f32x4){v[t], v[t + 1], v[t + 2], v[t + 3]};
+            if (d == 0) dst[DP] = m, dst[DP + 1] = l;
+        } else if (d < a.D) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            char* dst = a.out + (((int64_t)b * a.N + ot) * a.H + oh) * 2 * a.D + 2 * d;
+            *reinterpret_cast<uint4*>(dst) = make_uint4(win_pack<BF>(v[0] * inv, v[1] * inv), win_pack<BF>(v[2] * inv, v[3] * inv),
+                                                        win_pack<BF>(v[4] * inv, v[5] * inv), win_pack<BF>(v[6] * inv, v[7] * inv));
+        }
+    }
+}
+
+// One row of the output a DP / 8 threads: its parts in their order.
+template <int DP, bool BF>
+__global__ void __launch_bounds__(256) window_join_kernel(WinArgs a, int64_t rows) {
+    constexpr int PER = 256 / (DP / 8);
+    const int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / (DP / 8);
+    const int d = 8 * (threadIdx.x % (DP / 8));
+    if (threadIdx.x / (DP / 8) >= PER || row >= rows || d >= a.D) return;
+    const float* src = a.part + row * a.splits * (DP + 8);
+    float m = -__builtin_inff(), l = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, src[s * (DP + 8) + DP]);
+    for (int s = 0; s < a.splits; ++s) {
+        const float* p = src + s * (DP + 8);
+        if (p[DP] == -__builtin_inff()) continue;
+        const float f = __builtin_amdgcn_exp2f(p[DP] - m);
+        l = fmaf(f, p[DP + 1], l);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) v[t] = fmaf(f, p[d + t], v[t]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<uint4*>(a.out + row * 2 * a.D + 2 * d) =
+        make_uint4(win_pack<BF>(v[0] * inv, v[1] * inv), win_pack<BF>(v[2] * inv, v[3] * inv), win_pack<BF>(v[4] * inv, v[5] * inv),
+                   win_pack<BF>(v[6] * inv, v[7] * inv));
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+static WinArgs win_args(const rpfq_window_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths) {
+    WinArgs a = {};
+    a.q = reinterpret_cast<const char*>(q), a.k = reinterpret_cast<const char*>(k), a.v = reinterpret_cast<const char*>(v);
+    for (int i = 0; i < 3; ++i)
+        a.qs[i] = 2 * d.q_stride[i], a.ks[i] = 2 * d.k_stride[i], a.vs[i] = 2 * d.v_stride[i], a.os[i] = 2 * d.out_stride[i],
+        a.gos[i] = 2 * d.grad_stride[i];
+    a.lengths = lengths;
+    a.B = (int)d.B, a.N = (int)d.N, a.H = (int)d.H, a.KV = (int)d.KV, a.D = (int)d.D, a.M = (int)d.M;
+    a.NP = (int)window_rows(d.N);
+    const int64_t most = d.M > d.N ? d.M : d.N;
+    a.window = (int)(d.window < most ? d.window : most);
+    a.sinks = (int)(d.sinks < most ? d.sinks : most);
+    a.causal = d.causal;
+    a.scale = d.scale;
+    a.scale2 = d.scale * 1.4426950408889634f;
+    const int group = a.H / a.KV;
+    a.hw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+    a.qw = 4 / a.hw;
+    a.tiles = (a.NP + 32 * a.qw - 1) / (32 * a.qw);  // the statistics' rows behind N too
+    return a;
+}
+template <class K>
+static hipError_t win_launch(K kernel, std::atomic<uint64_t>& done, const WinArgs& a, int64_t blocks, int threads, int lds, hipStream_t s) {
+    const hipError_t e = set_lds_attr_once(reinterpret_cast<const void*>(kernel), lds, done);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, s, a);
+    return hipGetLastError();
+}
+#define WIN_LAUNCH(kernel, a, blocks, threads, lds, s)                         \
+    [&] {                                                                      \
+        static std::atomic<uint64_t> done{0};                                  \
+        return win_launch(&kernel, done, a, blocks, threads, lds, s);          \
+    }()
+
+struct WinForward {
+    const WinArgs& a;
+    hipStream_t s;
+    template <int DP, bool BF>
+    hipError_t run() {
+        return WIN_LAUNCH((window_forward_kernel<DP, BF>), a, (int64_t)a.B * (a.H / a.hw) * a.tiles, 256, 4 * 64 * Rows<DP>::RB, s);
+    }
+};
+struct WinGrad {
+    const WinArgs& a;
+    hipStream_t s;
+    template <int DP, bool BF>
+    hipError_t run() {
+        const hipError_t e =
+            WIN_LAUNCH((window_grad_q_kernel<DP, BF>), a, (int64_t)a.B * (a.H / a.hw) * a.tiles, 256, 4 * 64 * Rows<DP>::RB, s);
+        if (e != hipSuccess || (!a.gk && !a.gv)) return e;
+        return WIN_LAUNCH((window_grad_kv_kernel<DP, BF>), a, (int64_t)a.B * a.KV * ((a.N + kWinKeys - 1) / kWinKeys), 512,
+                          win_grad_lds<DP>(), s);
+    }
+};
+template <int DP>
+constexpr int win_cached_lds() {
+    const int rings = 4 * 4 * 32 * Rows<DP>::RB, sums = 4 * 32 * (DP + 6) * 4;
+    return rings > sums ? rings : sums;
+}
+struct WinCached {
+    const WinArgs& a;
+    hipStream_t s;
+    template <int DP, bool BF>
+    hipError_t run() {
+        const hipError_t e = WIN_LAUNCH((window_cached_kernel<DP, BF>), a, (int64_t)a.B * a.KV * a.blocks * a.splits, 256, win_cached_lds<DP>(), s);
+        if (e != hipSuccess || a.splits == 1) return e;
+        const int64_t rows = (int64_t)a.B * a.N * a.H;
+        constexpr int PER = 256 / (DP / 8);
+        hipLaunchKernelGGL((window_join_kernel<DP, BF>), dim3((unsigned)((rows + PER - 1) / PER)), dim3(256), 0, s, a, rows);
+        return hipGetLastError();
+    }
+};
+template <bool BF, class Go>
+static hipError_t win_dim(int D, Go go) {
+    if (D <= 32) return go.template run<32, BF>();
+    if (D <= 64) return go.template run<64, BF>();
+    if (D <= 96) return go.template run<96, BF>();
+    return go.template run<128, BF>();
+}
+template <class Go>
+static hipError_t win_dispatch(const rpfq_window_desc& d, Go go) {
+    return d.dtype == RPFQ_BF16 ? win_dim<true>((int)d.D, go) : win_dim<false>((int)d.D, go);
+}
+
+hipError_t launch_window_attention(const rpfq_window_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths,
+                                   void* out, float* stat, hipStream_t s) {
+    WinArgs a = win_args(d, q, k, v, lengths);
+    a.out = reinterpret_cast<char*>(out);
+    a.stat = stat;
+    return win_dispatch(d, WinForward{a, s});
+}
+hipError_t launch_window_attention_grad(const rpfq_window_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths,
+                                        const void* out, const void* grad_out, const float* stat, void* gq, void* gk, void* gv,
+                                        void* work, hipStream_t s) {
+    WinArgs a = win_args(d, q, k, v, lengths);
+    a.o = reinterpret_cast<const char*>(out), a.go = reinterpret_cast<const char*>(grad_out);
+    a.stat = const_cast<float*>(stat);
+    a.delta = reinterpret_cast<float*>(work);
+    a.gq = reinterpret_cast<char*>(gq), a.gk = reinterpret_cast<char*>(gk), a.gv = reinterpret_cast<char*>(gv);
+    return win_dispatch(d, WinGrad{a, s});
+}
+
+// Parts of the keys of one key head: as many as fill the chip four workgroups a
+// CU, each with 4 tiles (a tile a wave) or more.
+int window_splits(const rpfq_window_desc& d) {
+    const int64_t blocks = ((d.H / d.KV) * d.N + 31) / 32, units = d.B * d.KV * blocks;
+    int64_t keys = d.window + d.N - 1 + d.sinks;
+    keys = keys < d.M ? keys : d.M;
+    const int64_t most = (keys + 127) / 128, want = (4 * (int64_t)device_cus() + units - 1) / units;
+    const int64_t s = most < want ? most : want;
+    return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+}
+size_t window_cached_bytes(const rpfq_window_desc& d) {
+    const int s = window_splits(d);
+    if (s == 1) return 0;
+    const size_t dp = (size_t)((d.D + 31) / 32 * 32);
+    return (size_t)d.B * d.N * d.H * s * (dp + 8) * 4;
+}
+hipError_t launch_window_attention_cached(const rpfq_window_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths,
+                                          void* out, void* work, hipStream_t s) {
+    WinArgs a = win_args(d, q, k, v, lengths);
+    a.out = reinterpret_cast<char*>(out);
+    a.part = reinterpret_cast<float*>(work);
+    a.causal = 1;
+    a.rows = a.H / a.KV * a.N;
+    a.blocks = (a.rows + 31) / 32;
+    a.splits = window_splits(d);
+    return win_dispatch(d, WinCached{a, s});
+}
+
+}  // namespace rpfq

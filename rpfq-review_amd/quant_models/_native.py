@@ -97,6 +97,11 @@ EXPORTED = (
     "rpfq_rms_norm_grad_workspace_bytes",
     "rpfq_rms_norm_grad",
     "rpfq_rotary",
+    "rpfq_window_attention",
+    "rpfq_window_attention_stat_bytes",
+    "rpfq_window_attention_grad",
+    "rpfq_window_attention_cached",
+    "rpfq_window_attention_cached_workspace_bytes",
 )
 
 
@@ -164,6 +169,29 @@ class RotaryDesc(ctypes.Structure):
         ("sections", ctypes.c_int32 * 4),
         ("interleaved", ctypes.c_int32),
         ("inverse", ctypes.c_int32),
+    ]
+
+
+class WindowDesc(ctypes.Structure):
+    """Mirror of struct rpfq_window_desc."""
+
+    _fields_ = [
+        ("B", ctypes.c_int64),
+        ("N", ctypes.c_int64),
+        ("H", ctypes.c_int64),
+        ("KV", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("M", ctypes.c_int64),
+        ("window", ctypes.c_int64),
+        ("sinks", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("out_stride", ctypes.c_int64 * 3),
+        ("grad_stride", ctypes.c_int64 * 3),
+        ("dtype", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("scale", ctypes.c_float),
     ]
 
 
@@ -266,8 +294,16 @@ def load() -> ctypes.CDLL:
         lib.rpfq_rms_norm_grad_workspace_bytes.restype = sz
         lib.rpfq_rms_norm_grad.argtypes = [vp, vp, vp, i32, i64, i64, vp, i32, vp, vp, vp, vp, sz, vp]
         lib.rpfq_rotary.argtypes = [ctypes.POINTER(RotaryDesc), vp, vp, vp, vp, vp, vp, vp]
+        wd = ctypes.POINTER(WindowDesc)
+        lib.rpfq_window_attention.argtypes = [wd, vp, vp, vp, vp, vp, vp, vp]
+        lib.rpfq_window_attention_grad.argtypes = [wd, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        lib.rpfq_window_attention_cached.argtypes = [wd, vp, vp, vp, vp, vp, vp, sz, vp]
+        for size in (lib.rpfq_window_attention_stat_bytes, lib.rpfq_window_attention_cached_workspace_bytes):
+            size.argtypes = [wd]
+            size.restype = sz
         for name in EXPORTED[2:]:
-            if name not in ("rpfq_rms_norm_grad_workspace_bytes", "rpfq_linear_int8_workspace_bytes",
+            if name not in ("rpfq_window_attention_stat_bytes", "rpfq_window_attention_cached_workspace_bytes",
+                            "rpfq_rms_norm_grad_workspace_bytes", "rpfq_linear_int8_workspace_bytes",
                             "rpfq_linear_cross_entropy_workspace_bytes",
                             "rpfq_wide_packed_bytes", "rpfq_wide_adjoint_bytes", "rpfq_quantize_workspace_bytes",
                             "rpfq_linear_f32_workspace_bytes", "rpfq_wide_dense_bytes"):

@@ -1357,6 +1357,128 @@ def rotary(x, positions: torch.Tensor, freqs: torch.Tensor, sections=None, *, in
     return outs[0] if one else outs
 
 
+WINDOW_MAX_HEAD = 128
+
+
+def _window_operands(name, q, k, v, lengths, window, sinks, scale, cached):
+    """The checks of a windowed attention's arguments; (q, k, v, lengths, scale) as
+    the kernels read them, heads padded to a multiple of 8 values."""
+    N.require_same_device(q, k=k, v=v, lengths=lengths)
+    _no_transforms(name, q, k, v)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"{name} takes fp16 or bf16, got {q.dtype}")
+    for what, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4 or t.dtype != q.dtype:
+            raise ValueError(f"{what} must be {q.dtype} [B, tokens, heads, D], got {t.dtype} {tuple(t.shape)}")
+    b, n, h, d = q.shape
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d or (not cached and k.shape[1] != n):
+        raise ValueError(f"{name}: k {tuple(k.shape)} and v {tuple(v.shape)} beside q {tuple(q.shape)}")
+    if not 1 <= d <= WINDOW_MAX_HEAD or h < 1 or k.shape[2] < 1 or h % k.shape[2]:
+        raise ValueError(f"{name} takes heads of 1 .. {WINDOW_MAX_HEAD} values, a multiple of k's heads, got {h} of {d} on {k.shape[2]}")
+    if int(window) != window or int(sinks) != sinks or window < 1 or sinks < 0:
+        raise ValueError(f"window must be a whole number above 0, sinks 0 or more, got {window} and {sinks}")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if lengths is not None:
+        if lengths.shape != (b,) or lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"lengths must be int32 or int64 of shape ({b},), got {lengths.dtype} {tuple(lengths.shape)}")
+        if lengths.dtype == torch.int64:  # past int32 they are clamped all the same
+            lengths = lengths.clamp(0, 2 ** 31 - 1)
+        lengths = lengths.to(torch.int32).contiguous()
+
+    def rows(t):
+        if d % 8:
+            return torch.nn.functional.pad(t, (0, -d % 8))
+        if t.numel() and (t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.stride(1) >= 1 << 22 or t.data_ptr() % 16):
+            return t.clone(memory_format=torch.contiguous_format)
+        return t
+
+    return rows(q), rows(k), rows(v), lengths, scale
+
+
+def _window_desc(q, k, v, window, sinks, scale, causal, m=0):
+    b, n, h, d = q.shape
+    desc = N.WindowDesc(B=b, N=n, H=h, KV=k.shape[2], D=d, M=m, window=min(int(window), 1 << 40), sinks=min(int(sinks), 1 << 40),
+                        dtype=N.dtype_code(q.dtype), causal=int(bool(causal)), scale=scale)
+    for at, t in ((desc.q_stride, q), (desc.k_stride, k), (desc.v_stride, v)):
+        at[:] = t.stride()[:3]
+    return desc
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0, *, causal: bool = True,
+                     scale: float | None = None, lengths: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(scale q k^T) v over a sliding window (rpfq_window_attention): query
+    i sees key j where, causal, j <= i and (i - j < window or j < sinks), else
+    |i - j| < window or j < sinks or i < sinks (a class token in front sees and
+    is seen by all: sinks=1).  q [B, N, heads, D], k and v [B, N, kv heads, D],
+    kv heads a divisor of heads, D up to WINDOW_MAX_HEAD, fp16 or bf16, any
+    length; scale: D^-1/2 unless given.  lengths [B] (int32 or int64 on the
+    device): tokens of each sequence that count; the rows behind them give
+    zeros, also in the gradients, and their values are not read.  Parts of a
+    qkv tensor are read as they lie; heads that are not in one 16-byte aligned
+    piece, or of no multiple of 8 values, are copied.  Scores and sums in
+    float32, probabilities rounded to q's type.  A value that is not finite
+    makes the outputs of queries near it NaN too, whether they see it or not.
+    Gradients of q, k and v, once differentiable, sums in a fixed order; they
+    need the native host path (csrc/host.cpp); can be captured as rms_norm can."""
+    host = N.host()
+    if host is not None:
+        given = q.shape[-1] ** -0.5 if scale is None and isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else scale
+        out = host.window_attention(q, k, v, lengths, window, sinks, given, causal)
+        if out is not None:
+            return out
+    q2, k2, v2, lengths, scale = _window_operands("window_attention", q, k, v, lengths, window, sinks, scale, False)
+    if q.numel() == 0:
+        return q2 + 0.0
+    if host is not None:
+        out = host.window_attention(q2, k2, v2, lengths, min(int(window), 1 << 40), min(int(sinks), 1 << 40), scale, causal)
+        if out is not None:
+            return out[..., :q.shape[3]].contiguous()
+    if _records(q, k, v):
+        raise RuntimeError("window_attention: gradients need the native host path (csrc/host.cpp)")
+    desc = _window_desc(q2, k2, v2, window, sinks, scale, causal)
+    out = torch.empty(q2.shape, dtype=q2.dtype, device=q2.device)
+    desc.out_stride[:] = out.stride()[:3]
+    with N.on_device(q2):
+        N.check("rpfq_window_attention", N.load().rpfq_window_attention(
+            ctypes.byref(desc), q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), N.ptr(lengths), out.data_ptr(), None, N.stream_of(q2)))
+    return out[..., :q.shape[3]].contiguous()
+
+
+def window_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, window: int,
+                            sinks: int = 0, *, scale: float | None = None) -> torch.Tensor:
+    """window_attention, causal, of the last tokens of each sequence over a cache
+    (rpfq_window_attention_cached): q [B, T, heads, D], caches [B, slots, kv
+    heads, D], lengths [B] (int32 or int64 on the device, up to slots): tokens
+    in the cache, the T new ones among them, so query t is token lengths - T +
+    t.  Slots that no query sees are not read: what lies behind a sequence's
+    end, or between the sinks and the window, does not count.  Queries in front
+    of the first token (lengths < T) give zeros.  No gradient."""
+    host = N.host()
+    if host is not None:
+        given = q.shape[-1] ** -0.5 if scale is None and isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else scale
+        out = host.window_attention_cached(q, k_cache, v_cache, lengths, window, sinks, given)
+        if out is not None:
+            return out
+    if lengths is None:
+        raise ValueError("window_attention_cached needs lengths")
+    q2, k2, v2, lengths, scale = _window_operands("window_attention_cached", q, k_cache, v_cache, lengths, window, sinks, scale, True)
+    if _records(q, k_cache, v_cache):
+        raise RuntimeError("window_attention_cached has no gradient: call it under torch.no_grad()")
+    out = torch.zeros(q2.shape, dtype=q2.dtype, device=q2.device)
+    if q2.numel() == 0 or k2.numel() == 0:
+        return out[..., :q.shape[3]]
+    desc = _window_desc(q2, k2, v2, window, sinks, scale, True, k2.shape[1])
+    lib = N.load()
+    with N.on_device(q2):
+        work = torch.empty(lib.rpfq_window_attention_cached_workspace_bytes(ctypes.byref(desc)), dtype=torch.uint8, device=q2.device)
+        N.check("rpfq_window_attention_cached", lib.rpfq_window_attention_cached(
+            ctypes.byref(desc), q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), lengths.data_ptr(), out.data_ptr(),
+            work.data_ptr() or None, work.numel(), N.stream_of(q2)))
+    return out[..., :q.shape[3]].contiguous()
+
+
 def make_desc(n_complex, k_complex, codebook, stages, block, rotation) -> N.WideDesc:
     d = N.WideDesc()
     d.n_complex = int(n_complex)
