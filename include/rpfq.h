@@ -854,14 +854,17 @@ typedef struct rpfq_window_desc {
     float scale;            /* positive and finite */
 } rpfq_window_desc;
 
-/* stat (out, float32, 256-byte aligned, rpfq_window_attention_stat_bytes; NULL: not wanted): what the
- * gradient needs of each row. */
+/* stat (out, float32, 256-byte aligned, rpfq_window_attention_stat_bytes; NULL: not
+ * wanted): what the gradient needs of each row.  work: its workspace (may be 0
+ * bytes), 256-byte aligned. */
 int rpfq_window_attention(const rpfq_window_desc* desc, const void* q, const void* k, const void* v,
-                          const int32_t* lengths, void* out, float* stat, void* stream);
+                          const int32_t* lengths, void* out, float* stat, void* work, size_t work_bytes, void* stream);
 size_t rpfq_window_attention_stat_bytes(const rpfq_window_desc* desc);
+/* Bytes of the device workspace of rpfq_window_attention (grad 0) and its gradient. */
+size_t rpfq_window_attention_workspace_bytes(const rpfq_window_desc* desc, int grad);
 
 /* Gradients, contiguous and of dtype, zeros behind a sequence's end; any of
- * them NULL: not wanted.  out, stat: the forward's; work: as many bytes as stat,
+ * them NULL: not wanted.  out, stat: the forward's; work: its workspace,
  * 256-byte aligned.  Sums in a fixed order. */
 int rpfq_window_attention_grad(const rpfq_window_desc* desc, const void* q, const void* k, const void* v,
                                const int32_t* lengths, const void* out, const void* grad_out, const float* stat,

@@ -45,7 +45,8 @@ constexpr double kMostOps = 1.5e9;
     X(rpfq_linear_cross_entropy_grad) X(rpfq_adamw) X(rpfq_rms_norm) X(rpfq_rms_norm_int8)             \
     X(rpfq_rms_norm_grad_workspace_bytes) X(rpfq_rms_norm_grad) X(rpfq_rotary) \
     X(rpfq_window_attention) X(rpfq_window_attention_stat_bytes) X(rpfq_window_attention_grad)           \
-    X(rpfq_window_attention_cached) X(rpfq_window_attention_cached_workspace_bytes)
+    X(rpfq_window_attention_workspace_bytes) X(rpfq_window_attention_cached)                                \
+    X(rpfq_window_attention_cached_workspace_bytes)
 struct Api {
 #define X(f) decltype(&::f) f;
     RPFQ_HOST_CALLS(X)
@@ -769,8 +770,11 @@ struct Window : torch::autograd::Function<Window> {
         at::Tensor out = at::empty(q.sizes(), options), st;
         window_strides(out, d.out_stride);
         if (stat) st = at::empty({(int64_t)(api.rpfq_window_attention_stat_bytes(&d) / 4)}, options.dtype(at::kFloat));
+        const size_t bytes = api.rpfq_window_attention_workspace_bytes(&d, 0);
+        at::Tensor work;
+        if (bytes) work = at::empty({(int64_t)bytes}, options.dtype(at::kByte));
         const int rc = api.rpfq_window_attention(&d, q.data_ptr(), k.data_ptr(), v.data_ptr(), static_cast<const int32_t*>(ptr(lengths)),
-                                                 out.data_ptr(), stat ? st.data_ptr<float>() : nullptr, stream_on(q));
+                                                 out.data_ptr(), stat ? st.data_ptr<float>() : nullptr, ptr(work), bytes, stream_on(q));
         TORCH_CHECK(rc == RPFQ_OK, "rpfq_window_attention: ", api.rpfq_last_error());
         return {out, st};
     }
@@ -801,7 +805,7 @@ struct Window : torch::autograd::Function<Window> {
             for (int i = 0; i < 3; ++i)
                 if (ctx->needs_input_grad(i)) g[i] = at::empty(in[i]->sizes(), q.options().requires_grad(false));
             if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return g;
-            at::Tensor work = at::empty(stat.sizes(), stat.options());
+            at::Tensor work = at::empty({(int64_t)api.rpfq_window_attention_workspace_bytes(&d, 1)}, stat.options().dtype(at::kByte));
             const int rc = api.rpfq_window_attention_grad(&d, q.data_ptr(), k.data_ptr(), v.data_ptr(), static_cast<const int32_t*>(ptr(lengths)),
                                                           out.data_ptr(), go.data_ptr(), stat.const_data_ptr<float>(), ptr(g[0]), ptr(g[1]),
                                                           ptr(g[2]), work.data_ptr(), work.nbytes(), stream_on(q));

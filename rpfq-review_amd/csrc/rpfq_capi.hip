@@ -898,13 +898,20 @@ size_t rpfq_window_attention_stat_bytes(const rpfq_window_desc* d) {
     if (check_window(d, false) != RPFQ_OK) return 0;
     return (size_t)(d->B * d->H * rpfq::window_rows(d->N)) * 4;
 }
+size_t rpfq_window_attention_workspace_bytes(const rpfq_window_desc* d, int grad) {
+    return check_window(d, false) != RPFQ_OK ? 0 : rpfq::window_bytes(*d, grad != 0);
+}
 int rpfq_window_attention(const rpfq_window_desc* d, const void* q, const void* k, const void* v, const int32_t* lengths, void* out,
-                          float* stat, void* stream) {
+                          float* stat, void* work, size_t work_bytes, void* stream) {
     int rc = check_window(d, false);
     if (!rc) rc = check_window_operands(d, q, k, v, out, lengths);
     if (rc) return rc;
-    if (!window_strides(d->out_stride) || !aligned(stat, 256)) return fail(RPFQ_ERR_ALIGN, "out's strides or stat's alignment");
-    return hip_status(rpfq::launch_window_attention(*d, q, k, v, lengths, out, stat, reinterpret_cast<hipStream_t>(stream)),
+    if (!window_strides(d->out_stride) || !aligned(stat, 256) || !aligned(work, 256))
+        return fail(RPFQ_ERR_ALIGN, "out's strides must be multiples of 8 elements, stat and work 256-byte aligned");
+    const size_t need = rpfq::window_bytes(*d, false);
+    if (need && !work) return fail(RPFQ_ERR_NULL, "rpfq_window_attention: NULL pointer argument");
+    if (work_bytes < need) return fail(RPFQ_ERR_SHAPE, "workspace holds %zu bytes, need %zu", work_bytes, need);
+    return hip_status(rpfq::launch_window_attention(*d, q, k, v, lengths, out, stat, work, reinterpret_cast<hipStream_t>(stream)),
                       "rpfq_window_attention");
 }
 int rpfq_window_attention_grad(const rpfq_window_desc* d, const void* q, const void* k, const void* v, const int32_t* lengths,
@@ -918,7 +925,7 @@ int rpfq_window_attention_grad(const rpfq_window_desc* d, const void* q, const v
     if (!window_strides(d->out_stride) || !window_strides(d->grad_stride) || !aligned(grad_out, 16) || !aligned(stat, 256) ||
         !aligned(grad_q, 16) || !aligned(grad_k, 16) || !aligned(grad_v, 16) || !aligned(work, 256))
         return fail(RPFQ_ERR_ALIGN, "gradients must be 16-byte aligned, stat and work 256; strides multiples of 8 elements");
-    const size_t need = rpfq_window_attention_stat_bytes(d);
+    const size_t need = rpfq::window_bytes(*d, true);
     if (work_bytes < need) return fail(RPFQ_ERR_SHAPE, "workspace holds %zu bytes, need %zu", work_bytes, need);
     return hip_status(rpfq::launch_window_attention_grad(*d, q, k, v, lengths, out, grad_out, stat, grad_q, grad_k, grad_v, work,
                                                          reinterpret_cast<hipStream_t>(stream)),

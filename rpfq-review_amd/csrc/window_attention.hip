@@ -8,6 +8,8 @@
 //   dV = P^T dO,  dS = P (dO V^T - rowsum(dO O)),  dQ = scale dS K,  dK = scale dS^T Q.
 #include "tile_gemm.h"
 
+#include <utility>
+
 namespace rpfq {
 
 // A tile's rows in LDS: DP values of 16 bits (the head's size, rounded up to
@@ -128,6 +130,14 @@ __device__ __forceinline__ float win_dot8(uint4 a, uint4 b, float c) {
 template <bool BF>
 constexpr float win_shift() { return BF ? 20.0f : -15.0f; }
 
+// A tile with sinks has far more to go over than the others: every key (sinks as
+// queries, where not causal), every query (sinks as keys).  What lies past the
+// tile's own window is divided into `parts` workgroups of their own; each leaves
+// float32 sums of the sinks' rows (slot 0: the tile's), which a join adds up in
+// their order.  parts = 0: the tile goes over all of it itself, and first.
+struct WinFar {
+    int tiles, rows, parts;  // tiles with sinks, the sinks, parts of a tile
+};
 struct WinArgs {
     const char *q, *k, *v, *o, *go;     // o: out of the forward, in of the gradient
     char *out, *gq, *gk, *gv;
@@ -138,9 +148,10 @@ struct WinArgs {
     int window, sinks, causal;
     int hw, qw, tiles;                  // heads and 32-query blocks of a workgroup; query tiles
     float scale, scale2;                // scale2 = scale log2(e)
+    WinFar far, kfar;                   // of the sinks as queries, as keys
+    float *part, *kpart;
     // cached
-    int M, rows, blocks, splits;        // keys of the cache; queries of a key head; their 32-row blocks
-    float* part;
+    int M, rows, blocks, splits;        // keys of the cache; queries of a key head; their 32-row blocks; parts of a row
 };
 
 __device__ __forceinline__ int win_length(const WinArgs& a, int b, int most) {
@@ -266,26 +277,74 @@ __device__ __forceinline__ float win_softmax(floatx16 (&s)[KB], WinState& st, fl
     return f;
 }
 
+// Unit of a launch over `groups` x `tiles`: (group, tile, part), the parts of the
+// far ranges first, or the long tiles.
+struct WinUnit {
+    int group, tile, part;  // part 0: the tile itself
+};
+__device__ __forceinline__ WinUnit win_unit(const WinFar& f, int groups, int tiles) {
+    const int u = blockIdx.x, first = groups * f.tiles * (f.parts ? f.parts : 1), skip = f.parts ? 0 : f.tiles;
+    if (u < first) {
+        const int p = f.parts ? u % f.parts : 0, v = xcd_tile(f.parts ? u / f.parts : u, groups * f.tiles);
+        return {v / f.tiles, v % f.tiles, f.parts ? 1 + p : 0};
+    }
+    const int v = xcd_tile(u - first, groups * (tiles - skip));
+    return {v / (tiles - skip), skip + v % (tiles - skip), 0};
+}
+static inline int64_t win_units(const WinFar& f, int64_t groups, int tiles) { return groups * (tiles + f.tiles * f.parts); }
+// The tiles that a unit goes over, of all [0, end) and up to `near` by the tile itself.
+__device__ __forceinline__ WinTiles win_share(const WinFar& f, const WinUnit& u, WinTiles t, int near, int end) {
+    if (!f.parts || u.tile >= f.tiles) return t;
+    near = near < end ? near : end;
+    if (!u.part) {
+        if (t.t0 + t.count - t.first > near) t.count = near > t.t0 ? t.first + near - t.t0 : t.first;
+    } else {
+        const int n = end - near;
+        t.first = 0;
+        t.t0 = near + (int)((int64_t)n * (u.part - 1) / f.parts);
+        t.count = near + (int)((int64_t)n * u.part / f.parts) - t.t0;
+    }
+    return t;
+}
+
 // Where a workgroup of four waves stands: wave w has head hw h0 + w % hw and the
 // 32-query block w / hw of its tile.  Heads that share keys sit together, so a
 // tile is narrow and its window little wider than one query's.
 struct WinPlace {
     int b, h, kv, q0, q1, mine, n;  // tile's first and last query (< n), first of this wave
+    WinUnit unit;
 };
 __device__ __forceinline__ WinPlace win_place(const WinArgs& a, int wave) {
     WinPlace p;
-    const int u = xcd_tile(blockIdx.x, gridDim.x);
-    const int t = u % a.tiles, rest = u / a.tiles, groups = a.H / a.hw;
-    p.b = rest / groups;
-    const int h0 = (rest - p.b * groups) * a.hw;
+    const int groups = a.H / a.hw;
+    p.unit = win_unit(a.far, a.B * groups, a.tiles);
+    p.b = p.unit.group / groups;
+    const int h0 = (p.unit.group - p.b * groups) * a.hw;
     p.h = h0 + wave % a.hw;
     p.kv = h0 / (a.H / a.KV);
-    const int tile = a.causal ? a.tiles - 1 - t : t;  // the longest first
+    const int tile = a.causal ? a.tiles - 1 - p.unit.tile : p.unit.tile;  // the longest first
     p.q0 = tile * 32 * a.qw;
     p.mine = p.q0 + 32 * (wave / a.hw);
     p.n = win_length(a, p.b, a.N);
     p.q1 = (p.q0 + 32 * a.qw < p.n ? p.q0 + 32 * a.qw : p.n) - 1;
     return p;
+}
+// Its key tiles of T.
+template <int T>
+__device__ __forceinline__ WinTiles win_keys(const WinArgs& a, const WinPlace& p) {
+    return win_share(a.far, p.unit, win_tiles<T>(a, p.q0, p.q1, p.n), (p.q0 + 32 * a.qw + a.window + T - 1) / T, p.q1 < p.q0 ? 0 : (p.n + T - 1) / T);
+}
+
+// 32 rows of DP results as a slot of their float32 sums: `o` times f, and two
+// numbers behind them.
+template <int DP>
+__device__ __forceinline__ void win_part(float* dst, const floatx16 (&o)[DP / 32], float f, float x, float y, int g) {
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4)
+            *reinterpret_cast<f32x4*>(dst + 32 * j + acc_row(v, g)) = (f32x4){o[j][v] * f, o[j][v + 1] * f, o[j][v + 2] * f, o[j][v + 3] * f};
+    if (g == 0) dst[DP] = x, dst[DP + 1] = y;
 }
 
 // Forward.  S^T = K Q^T: a lane holds one query's scores, so the softmax is
@@ -302,7 +361,7 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
     const int i = p.mine + r, last = (p.mine + 31 < p.n - 1 ? p.mine + 31 : p.n - 1);
     uint4 q[DP / 16];
     win_row<DP>(q, a.q + p.b * a.qs[0] + (int64_t)i * a.qs[1] + p.h * a.qs[2], i < p.n, a.D, g);
-    const WinTiles tiles = win_tiles<T>(a, p.q0, p.q1, p.n);
+    const WinTiles tiles = win_keys<T>(a, p);
     RowLoads<DP, T, 4> lk, lv;
     lk.init(a.ks[1], a.D, wave, lane);
     lv.init(a.vs[1], a.D, wave, lane);
@@ -364,10 +423,16 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
     }
     const float l = st.l + __shfl_xor(st.l, 32, 64);
     const bool any = l != 0.0f && i < p.n;
+    if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
+        const int64_t row = (((int64_t)p.b * a.far.rows + i) * a.H + p.h) * (a.far.parts + 1) + p.unit.part;
+        if (i < a.far.rows) win_part<DP>(a.part + row * (DP + 8), o, 1.0f, any ? st.sub : -__builtin_inff(), l, g);
+    }
+    if (p.unit.part) return;
+    const bool joined = a.far.parts && i < a.far.rows;
     // the gradient's probabilities are exp2(S scale2 + stat), times 2^15 in fp16
-    if (a.stat && g == 0 && i < a.NP)
+    if (a.stat && g == 0 && i < a.NP && !joined)
         a.stat[((int64_t)p.b * a.H + p.h) * a.NP + i] = any ? (BF ? 0.0f : 15.0f) - (st.sub + __builtin_amdgcn_logf(l)) : -__builtin_inff();
-    win_store<DP, BF>(o, any ? 1.0f / l : 0.0f, !any, i < a.N, a.out + p.b * a.os[0] + (int64_t)i * a.os[1] + p.h * a.os[2], a.D, g);
+    win_store<DP, BF>(o, any ? 1.0f / l : 0.0f, !any, i < a.N && !joined, a.out + p.b * a.os[0] + (int64_t)i * a.os[1] + p.h * a.os[2], a.D, g);
 }
 
 // fp16 gradients: dS is carried times a power of two of its column (one query in
@@ -420,10 +485,10 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
         for (int s = 0; s < DP / 16; ++s) delta = win_dot8<BF>(go[s], out[s], delta);
         delta += __shfl_xor(delta, 32, 64);
     }
-    if (g == 0 && i < a.NP) a.delta[row] = delta;
+    if (g == 0 && i < a.NP && !p.unit.part) a.delta[row] = delta;
     const float stat = i < a.NP ? a.stat[row] : -__builtin_inff();
     if (!a.gq) return;
-    const WinTiles tiles = win_tiles<T>(a, p.q0, p.q1, p.n);
+    const WinTiles tiles = win_keys<T>(a, p);
     RowLoads<DP, T, 4> lk, lv;
     lk.init(a.ks[1], a.D, wave, lane);
     lv.init(a.vs[1], a.D, wave, lane);
@@ -476,31 +541,47 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
             }
         }
     }
+    const float f = (BF ? 1.0f : 0x1p-15f) / c;
+    if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
+        const int64_t slot = (((int64_t)p.b * a.far.rows + i) * a.H + p.h) * (a.far.parts + 1) + p.unit.part;
+        if (i < a.far.rows) win_part<DP>(a.part + slot * (DP + 8), o, i < p.n ? f : 0.0f, 0.0f, 1.0f, g);
+    }
+    if (p.unit.part) return;
     char* dst = a.gq + (((int64_t)p.b * a.N + i) * a.H + p.h) * 2 * a.D;
-    win_store<DP, BF>(o, a.scale * (BF ? 1.0f : 0x1p-15f) / c, i >= p.n, i < a.N, dst, a.D, g);
+    win_store<DP, BF>(o, a.scale * f, i >= p.n, i < a.N && !(a.far.parts && i < a.far.rows), dst, a.D, g);
 }
 
-// Gradient of the keys and values: a workgroup of eight waves has 128 keys, 32 to
-// a wave and its fellow, which take every other 32 of the queries that see them,
+// Gradient of the keys and values: a workgroup of four waves has 64 keys, 32 to a
+// wave and its fellow, which take every other 32 of the queries that see them,
 // of all heads that share them.  S = Q K^T and dP = dO V^T with a key to a lane:
 // P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS.  K stays in
-// registers, V in LDS (with both, 128-value heads spill).
-constexpr int kWinKeys = 128, kWinStep = 64;
+// registers, V in LDS (with both, 128-value heads spill); with two stages of Q
+// and dO that is 80 KB, two workgroups a CU.
+constexpr int kWinKeys = 64, kWinStep = 64;
 template <int DP>
 constexpr int win_grad_lds() {
-    const int rows = Rows<DP>::RB * (kWinKeys + 4 * kWinStep) + 4 * kWinStep * 4;
-    const int sums = 4 * 32 * (DP + 4) * 4;
+    const int rows = Rows<DP>::RB * (kWinKeys + 4 * kWinStep), sums = 2 * 32 * (DP + 4) * 4;
     return rows > sums ? rows : sums;
 }
+// The value of lane E of each 16 lanes in all of them.
+template <int E>
+__device__ __forceinline__ float win_lane(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + E, 0xf, 0xf, true));
+}
+// P and dS of a lane's key and 16 queries, whose statistics lie in 16 lanes
+template <int... E>
+__device__ __forceinline__ void win_probs(std::integer_sequence<int, E...>, floatx16& s, floatx16& dp, float scale2, float stat, float delta) {
+    ((s[E] = __builtin_amdgcn_exp2f(s[E] * scale2 + win_lane<E>(stat)), dp[E] = s[E] * (dp[E] - win_lane<E>(delta))), ...);
+}
 template <int DP, bool BF>
-__global__ void __launch_bounds__(512, 2) window_grad_kv_kernel(WinArgs a) {
+__global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
     extern __shared__ __align__(16) char smem[];
-    constexpr int RB = Rows<DP>::RB, V = kWinKeys * RB, STAGE = 2 * kWinStep * RB;  // V, two stages of Q and dO, their statistics
+    constexpr int RB = Rows<DP>::RB, V = kWinKeys * RB, STAGE = 2 * kWinStep * RB;  // V, two stages of Q and dO
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), block = wave & 3, half = wave >> 2;
-    const int u = xcd_tile(blockIdx.x, gridDim.x), tiles_n = (a.N + kWinKeys - 1) / kWinKeys;
-    const int tile = u % tiles_n, rest = u / tiles_n, b = rest / a.KV, kv = rest - b * a.KV, group = a.H / a.KV;
-    const int n = win_length(a, b, a.N), k0 = tile * kWinKeys, mine = k0 + 32 * block, key = mine + r;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), block = wave & 1, half = wave >> 1;
+    const WinUnit unit = win_unit(a.kfar, a.B * a.KV, (a.N + kWinKeys - 1) / kWinKeys);
+    const int b = unit.group / a.KV, kv = unit.group - b * a.KV, group = a.H / a.KV;
+    const int n = win_length(a, b, a.N), k0 = unit.tile * kWinKeys, mine = k0 + 32 * block, key = mine + r;
     const int klast = (mine + 31 < n - 1 ? mine + 31 : n - 1), kend = (k0 + kWinKeys < n ? k0 + kWinKeys : n) - 1;
     uint4 kf[DP / 16];
     win_row<DP>(kf, a.k + b * a.ks[0] + (int64_t)key * a.ks[1] + kv * a.ks[2], key < n, a.D, g);
@@ -514,27 +595,29 @@ __global__ void __launch_bounds__(512, 2) window_grad_kv_kernel(WinArgs a) {
     q.t0 = lo / kWinStep > q.first ? lo / kWinStep : q.first;
     const int t1 = (hi + kWinStep - 1) / kWinStep;
     q.count = kend < k0 ? 0 : q.first + (t1 > q.t0 ? t1 - q.t0 : 0);
+    q = win_share(a.kfar, unit, q, (k0 + kWinKeys + a.window + kWinStep - 1) / kWinStep, kend < k0 ? 0 : (n + kWinStep - 1) / kWinStep);
     const int steps = q.count * group;
 
-    RowLoads<DP, kWinStep, 8> lq, lo_;
+    RowLoads<DP, kWinStep, 4> lq, lo_;
     lq.init(a.qs[1], a.D, wave, lane);
     lo_.init(a.gos[1], a.D, wave, lane);
     Frags<DP> at;
     at.init(lane);
-    const uint32_t lds = lds_addr(smem), stats = lds + V + 2 * STAGE;
+    const uint32_t lds = lds_addr(smem);
     int head = 0, qt = 0;  // of the step that is issued next
+    float stat, delta, stat_next = 0.0f, delta_next = 0.0f;
     auto issue = [&](int s) {
         const int h = kv * group + head, first = q.at(qt) * kWinStep;
         const uint32_t to = lds + V + (s & 1) * STAGE;
         lq.issue(a.q + b * a.qs[0] + h * a.qs[2], a.qs[1], a.D, first, n, to, wave);
         lo_.issue(a.go + b * a.gos[0] + h * a.gos[2], a.gos[1], a.D, first, n, to + kWinStep * RB, wave);
-        const int64_t row = ((int64_t)b * a.H + h) * a.NP + first;
-        if (wave == 0) dma_dword(a.stat + row, lane * 4, stats + (s & 1) * 2 * kWinStep * 4);
-        if (wave == 1) dma_dword(a.delta + row, lane * 4, stats + (s & 1) * 2 * kWinStep * 4 + kWinStep * 4);
+        const int64_t row = ((int64_t)b * a.H + h) * a.NP + first + 32 * half + acc_row(lane & 15, g);
+        stat_next = a.stat[row];
+        delta_next = a.delta[row];
         if (++qt == q.count) qt = 0, ++head;
     };
     if (steps) {
-        RowLoads<DP, kWinKeys, 8> lv;
+        RowLoads<DP, kWinKeys, 4> lv;
         lv.init(a.vs[1], a.D, wave, lane);
         lv.issue(a.v + b * a.vs[0] + kv * a.vs[2], a.vs[1], a.D, k0, n, lds, wave);
         issue(0);
@@ -547,29 +630,20 @@ __global__ void __launch_bounds__(512, 2) window_grad_kv_kernel(WinArgs a) {
     int ct = 0;
     for (int t = 0; t < steps; ++t) {
         win_sync();
+        stat = stat_next, delta = delta_next;
         if (t + 1 < steps) issue(t + 1);
         const int q0 = q.at(ct) * kWinStep + 32 * half, qlast = (q0 + 31 < n - 1 ? q0 + 31 : n - 1);
         if (++ct == q.count) ct = 0;
         const int seen = qlast < q0 || klast < mine ? 0 : win_class(a, q0, qlast, mine, klast);
         if (!seen) continue;
         const uint32_t qtile = lds + V + (t & 1) * STAGE + 32 * half * RB, otile = qtile + kWinStep * RB;
-        const uint32_t st = stats + (t & 1) * 2 * kWinStep * 4 + 32 * half * 4 + 16 * g, vt = lds + 32 * block * RB;
-        typedef __attribute__((address_space(3))) const f32x4* lds_f4_t;
+        const uint32_t vt = lds + 32 * block * RB;
         floatx16 s = floatx16{0}, dp = floatx16{0};
 #pragma unroll
         for (int e = 0; e < DP / 16; ++e) s = win_mma<BF>(at.rows(qtile, e), kf[e], s);
 #pragma unroll
         for (int e = 0; e < DP / 16; ++e) dp = win_mma<BF>(at.rows(otile, e), at.rows(vt, e), dp);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const f32x4 sv = *reinterpret_cast<lds_f4_t>(st + 32 * w), dv = *reinterpret_cast<lds_f4_t>(st + kWinStep * 4 + 32 * w);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int v = 4 * w + e;
-                s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, sv[e]));
-                dp[v] = s[v] * (dp[v] - dv[e]);
-            }
-        }
+        win_probs(std::make_integer_sequence<int, 16>(), s, dp, a.scale2, stat, delta);
         if (seen == 1) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
@@ -593,8 +667,9 @@ __global__ void __launch_bounds__(512, 2) window_grad_kv_kernel(WinArgs a) {
         }
     }
     // the fellow's sums through LDS, one tensor after the other
-    const float fk = a.scale * (BF ? 1.0f : 0x1p-15f), fv = BF ? 1.0f : 0x1p-15f;
+    const float fv = BF ? 1.0f : 0x1p-15f;
     float* sums = reinterpret_cast<float*>(smem) + (block * 32 + r) * (DP + 4);
+    const bool parted = a.kfar.parts && unit.tile < a.kfar.tiles;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         floatx16(&o)[DP / 32] = w ? ov : ok;
@@ -618,9 +693,14 @@ __global__ void __launch_bounds__(512, 2) window_grad_kv_kernel(WinArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[j][v + e] = o[j][v + e] * f + x[e];
                 }
+            if (parted && key < a.kfar.rows) {
+                const int64_t row = ((((int64_t)w * a.B + b) * a.kfar.rows + key) * a.KV + kv) * (a.kfar.parts + 1) + unit.part;
+                win_part<DP>(a.kpart + row * (DP + 8), o, key < n ? fv : 0.0f, 0.0f, 1.0f, g);
+            }
             char* dst = w ? a.gv : a.gk;
-            if (dst)
-                win_store<DP, BF>(o, w ? fv : fk, key >= n, key < a.N, dst + (((int64_t)b * a.N + key) * a.KV + kv) * 2 * a.D, a.D, g);
+            if (dst && !unit.part)
+                win_store<DP, BF>(o, w ? fv : fv * a.scale, key >= n, key < a.N && !(parted && key < a.kfar.rows),
+                                  dst + (((int64_t)b * a.N + key) * a.KV + kv) * 2 * a.D, a.D, g);
         }
     }
 }
@@ -759,26 +839,46 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
     }
 }
 
-// One row of the output a DP / 8 threads: its parts in their order.
-template <int DP, bool BF>
-__global__ void __launch_bounds__(256) window_join_kernel(WinArgs a, int64_t rows) {
-    constexpr int PER = 256 / (DP / 8);
+// Rows [sequence][token][head] from their slots, in their order, DP / 8 threads a
+// row: outputs (a slot: sums, their exponent, their weight), or plain sums times
+// `factor` (GRAD: no exponents).  A slot without any has the exponent -inf.
+struct WinJoin {
+    const float* part;
+    char* out;
+    float* stat;          // [B, heads, NP], or NULL
+    int64_t os[3];
+    int64_t rows;         // sequences x tokens x heads
+    int tokens, heads, slots, D, NP;
+    float factor;
+};
+template <int DP, bool BF, bool GRAD>
+__global__ void __launch_bounds__(256) window_join_kernel(WinJoin a) {
+    constexpr int PER = 256 / (DP / 8), LD = DP + 8;
     const int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / (DP / 8);
     const int d = 8 * (threadIdx.x % (DP / 8));
-    if (threadIdx.x / (DP / 8) >= PER || row >= rows || d >= a.D) return;
-    const float* src = a.part + row * a.splits * (DP + 8);
+    if (threadIdx.x / (DP / 8) >= PER || row >= a.rows || d >= a.D) return;
+    const float* src = a.part + row * a.slots * LD;
     float m = -__builtin_inff(), l = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, src[s * (DP + 8) + DP]);
-    for (int s = 0; s < a.splits; ++s) {
-        const float* p = src + s * (DP + 8);
-        if (p[DP] == -__builtin_inff()) continue;
-        const float f = __builtin_amdgcn_exp2f(p[DP] - m);
-        l = fmaf(f, p[DP + 1], l);
+    if (!GRAD)
+        for (int s = 0; s < a.slots; ++s) m = fmaxf(m, src[s * LD + DP]);
+    for (int s = 0; s < a.slots; ++s) {
+        const float* p = src + s * LD;
+        float f = 1.0f;
+        if (!GRAD) {
+            f = p[DP];
+            if (f == -__builtin_inff()) continue;
+            f = __builtin_amdgcn_exp2f(f - m);
+            l = fmaf(f, p[DP + 1], l);
+        }
 #pragma unroll
         for (int t = 0; t < 8; ++t) v[t] = fmaf(f, p[d + t], v[t]);
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    *reinterpret_cast<uint4*>(a.out + row * 2 * a.D + 2 * d) =
+    const int64_t seq = row / (a.tokens * a.heads);
+    const int rest = (int)(row - seq * a.tokens * a.heads), tok = rest / a.heads, h = rest - tok * a.heads;
+    if (!GRAD && a.stat && d == 0)
+        a.stat[(seq * a.heads + h) * a.NP + tok] = l == 0.0f ? -__builtin_inff() : (BF ? 0.0f : 15.0f) - (m + __builtin_amdgcn_logf(l));
+    const float inv = GRAD ? a.factor : l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<uint4*>(a.out + seq * a.os[0] + tok * a.os[1] + h * a.os[2] + 2 * d) =
         make_uint4(win_pack<BF>(v[0] * inv, v[1] * inv), win_pack<BF>(v[2] * inv, v[3] * inv), win_pack<BF>(v[4] * inv, v[5] * inv),
                    win_pack<BF>(v[6] * inv, v[7] * inv));
 }
@@ -820,12 +920,23 @@ static hipError_t win_launch(K kernel, std::atomic<uint64_t>& done, const WinArg
         return win_launch(&kernel, done, a, blocks, threads, lds, s);          \
     }()
 
+template <int DP, bool BF, bool GRAD>
+static hipError_t win_join(const WinArgs& a, const float* part, char* out, const int64_t (&os)[3], float* stat, int tokens, int heads,
+                           int slots, float factor, hipStream_t s) {
+    const WinJoin j = {part, out, stat, {os[0], os[1], os[2]}, (int64_t)a.B * tokens * heads, tokens, heads, slots, a.D, a.NP, factor};
+    constexpr int PER = 256 / (DP / 8);
+    hipLaunchKernelGGL((window_join_kernel<DP, BF, GRAD>), dim3((unsigned)((j.rows + PER - 1) / PER)), dim3(256), 0, s, j);
+    return hipGetLastError();
+}
 struct WinForward {
     const WinArgs& a;
     hipStream_t s;
     template <int DP, bool BF>
     hipError_t run() {
-        return WIN_LAUNCH((window_forward_kernel<DP, BF>), a, (int64_t)a.B * (a.H / a.hw) * a.tiles, 256, 4 * 64 * Rows<DP>::RB, s);
+        const hipError_t e = WIN_LAUNCH((window_forward_kernel<DP, BF>), a, win_units(a.far, (int64_t)a.B * (a.H / a.hw), a.tiles), 256,
+                                        4 * 64 * Rows<DP>::RB, s);
+        if (e != hipSuccess || !a.far.parts) return e;
+        return win_join<DP, BF, false>(a, a.part, a.out, a.os, a.stat, a.far.rows, a.H, a.far.parts + 1, 0.0f, s);
     }
 };
 struct WinGrad {
@@ -833,11 +944,22 @@ struct WinGrad {
     hipStream_t s;
     template <int DP, bool BF>
     hipError_t run() {
-        const hipError_t e =
-            WIN_LAUNCH((window_grad_q_kernel<DP, BF>), a, (int64_t)a.B * (a.H / a.hw) * a.tiles, 256, 4 * 64 * Rows<DP>::RB, s);
+        hipError_t e = WIN_LAUNCH((window_grad_q_kernel<DP, BF>), a, win_units(a.far, (int64_t)a.B * (a.H / a.hw), a.tiles), 256,
+                                  4 * 64 * Rows<DP>::RB, s);
+        if (e == hipSuccess && a.gq && a.far.parts) {
+            const int64_t os[3] = {(int64_t)a.N * a.H * 2 * a.D, (int64_t)a.H * 2 * a.D, 2 * a.D};
+            e = win_join<DP, BF, true>(a, a.part, a.gq, os, nullptr, a.far.rows, a.H, a.far.parts + 1, a.scale, s);
+        }
         if (e != hipSuccess || (!a.gk && !a.gv)) return e;
-        return WIN_LAUNCH((window_grad_kv_kernel<DP, BF>), a, (int64_t)a.B * a.KV * ((a.N + kWinKeys - 1) / kWinKeys), 512,
-                          win_grad_lds<DP>(), s);
+        e = WIN_LAUNCH((window_grad_kv_kernel<DP, BF>), a, win_units(a.kfar, (int64_t)a.B * a.KV, (a.N + kWinKeys - 1) / kWinKeys), 256,
+                       win_grad_lds<DP>(), s);
+        for (int w = 0; w < 2 && a.kfar.parts && e == hipSuccess; ++w) {
+            char* dst = w ? a.gv : a.gk;
+            const int64_t os[3] = {(int64_t)a.N * a.KV * 2 * a.D, (int64_t)a.KV * 2 * a.D, 2 * a.D};
+            const float* part = a.kpart + (int64_t)w * a.B * a.kfar.rows * a.KV * (a.kfar.parts + 1) * (DP + 8);
+            if (dst) e = win_join<DP, BF, true>(a, part, dst, os, nullptr, a.kfar.rows, a.KV, a.kfar.parts + 1, w ? 1.0f : a.scale, s);
+        }
+        return e;
     }
 };
 template <int DP>
@@ -852,10 +974,8 @@ struct WinCached {
     hipError_t run() {
         const hipError_t e = WIN_LAUNCH((window_cached_kernel<DP, BF>), a, (int64_t)a.B * a.KV * a.blocks * a.splits, 256, win_cached_lds<DP>(), s);
         if (e != hipSuccess || a.splits == 1) return e;
-        const int64_t rows = (int64_t)a.B * a.N * a.H;
-        constexpr int PER = 256 / (DP / 8);
-        hipLaunchKernelGGL((window_join_kernel<DP, BF>), dim3((unsigned)((rows + PER - 1) / PER)), dim3(256), 0, s, a, rows);
-        return hipGetLastError();
+        const int64_t os[3] = {(int64_t)a.N * a.H * 2 * a.D, (int64_t)a.H * 2 * a.D, 2 * a.D};
+        return win_join<DP, BF, false>(a, a.part, a.out, os, nullptr, a.N, a.H, a.splits, 0.0f, s);
     }
 };
 template <bool BF, class Go>
@@ -870,11 +990,41 @@ static hipError_t win_dispatch(const rpfq_window_desc& d, Go go) {
     return d.dtype == RPFQ_BF16 ? win_dim<true>((int)d.D, go) : win_dim<false>((int)d.D, go);
 }
 
+// Whether the tiles with sinks go in parts: where one of them has more steps than
+// a CU's share of them all (`slots` workgroups at once), so that the launch would
+// wait for it; a part is `share` of a tile's own steps.  `rows`, `steps` a tile.
+static WinFar win_far(int64_t sinks, int64_t groups, int64_t tiles, int64_t rows, int64_t window, int64_t N, int heads, int share) {
+    WinFar f = {(int)((sinks + rows - 1) / rows), (int)sinks, 0};
+    const int64_t all = heads * ((N + 63) / 64), near = heads * ((rows + window) / 64 + 1), slots = 2 * device_cus();
+    if (!sinks || sinks > 128 || all <= 2 * near || all * slots <= groups * tiles * near) return f;
+    const int64_t step = near / share > 4 ? near / share : 4, parts = (all - near + step - 1) / step;
+    f.parts = (int)(parts > 64 ? 64 : parts);
+    return f;
+}
+static void win_fars(WinArgs& a) {
+    const int64_t near = 2 * (int64_t)a.window;  // to both sides
+    if (!a.causal) a.far = win_far(a.sinks, (int64_t)a.B * (a.H / a.hw), a.tiles, 32 * a.qw, near, a.N, 1, 4);
+    a.kfar = win_far(a.sinks, (int64_t)a.B * a.KV, (a.N + kWinKeys - 1) / kWinKeys, kWinKeys, a.causal ? a.window : near, a.N, a.H / a.KV, 8);
+}
+static size_t win_part_floats(const WinFar& f, int64_t heads, int64_t B, int64_t D) {
+    return f.parts ? (size_t)B * f.rows * heads * (f.parts + 1) * ((D + 31) / 32 * 32 + 8) : 0;
+}
+// The workspace: rowsum(dO O) (gradient), the sinks' sums as queries, as keys.
+size_t window_bytes(const rpfq_window_desc& d, bool grad) {
+    WinArgs a = win_args(d, nullptr, nullptr, nullptr, nullptr);
+    win_fars(a);
+    size_t n = win_part_floats(a.far, a.H, a.B, a.D);
+    if (grad) n += (size_t)a.B * a.H * a.NP + 2 * win_part_floats(a.kfar, a.KV, a.B, a.D);
+    return 4 * n;
+}
+
 hipError_t launch_window_attention(const rpfq_window_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths,
-                                   void* out, float* stat, hipStream_t s) {
+                                   void* out, float* stat, void* work, hipStream_t s) {
     WinArgs a = win_args(d, q, k, v, lengths);
+    win_fars(a);
     a.out = reinterpret_cast<char*>(out);
     a.stat = stat;
+    a.part = reinterpret_cast<float*>(work);
     return win_dispatch(d, WinForward{a, s});
 }
 hipError_t launch_window_attention_grad(const rpfq_window_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths,
@@ -883,7 +1033,10 @@ hipError_t launch_window_attention_grad(const rpfq_window_desc& d, const void* q
     WinArgs a = win_args(d, q, k, v, lengths);
     a.o = reinterpret_cast<const char*>(out), a.go = reinterpret_cast<const char*>(grad_out);
     a.stat = const_cast<float*>(stat);
+    win_fars(a);
     a.delta = reinterpret_cast<float*>(work);
+    a.part = a.delta + (size_t)a.B * a.H * a.NP;
+    a.kpart = a.part + win_part_floats(a.far, a.H, a.B, a.D);
     a.gq = reinterpret_cast<char*>(gq), a.gk = reinterpret_cast<char*>(gk), a.gv = reinterpret_cast<char*>(gv);
     return win_dispatch(d, WinGrad{a, s});
 }

@@ -99,6 +99,7 @@ EXPORTED = (
     "rpfq_rotary",
     "rpfq_window_attention",
     "rpfq_window_attention_stat_bytes",
+    "rpfq_window_attention_workspace_bytes",
     "rpfq_window_attention_grad",
     "rpfq_window_attention_cached",
     "rpfq_window_attention_cached_workspace_bytes",
@@ -295,14 +296,16 @@ def load() -> ctypes.CDLL:
         lib.rpfq_rms_norm_grad.argtypes = [vp, vp, vp, i32, i64, i64, vp, i32, vp, vp, vp, vp, sz, vp]
         lib.rpfq_rotary.argtypes = [ctypes.POINTER(RotaryDesc), vp, vp, vp, vp, vp, vp, vp]
         wd = ctypes.POINTER(WindowDesc)
-        lib.rpfq_window_attention.argtypes = [wd, vp, vp, vp, vp, vp, vp, vp]
+        lib.rpfq_window_attention.argtypes = [wd, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        lib.rpfq_window_attention_workspace_bytes.argtypes = [wd, i32]
+        lib.rpfq_window_attention_workspace_bytes.restype = sz
         lib.rpfq_window_attention_grad.argtypes = [wd, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         lib.rpfq_window_attention_cached.argtypes = [wd, vp, vp, vp, vp, vp, vp, sz, vp]
         for size in (lib.rpfq_window_attention_stat_bytes, lib.rpfq_window_attention_cached_workspace_bytes):
             size.argtypes = [wd]
             size.restype = sz
         for name in EXPORTED[2:]:
-            if name not in ("rpfq_window_attention_stat_bytes", "rpfq_window_attention_cached_workspace_bytes",
+            if name not in ("rpfq_window_attention_stat_bytes", "rpfq_window_attention_workspace_bytes", "rpfq_window_attention_cached_workspace_bytes",
                             "rpfq_rms_norm_grad_workspace_bytes", "rpfq_linear_int8_workspace_bytes",
                             "rpfq_linear_cross_entropy_workspace_bytes",
                             "rpfq_wide_packed_bytes", "rpfq_wide_adjoint_bytes", "rpfq_quantize_workspace_bytes",

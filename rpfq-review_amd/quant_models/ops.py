@@ -1440,9 +1440,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     desc = _window_desc(q2, k2, v2, window, sinks, scale, causal)
     out = torch.empty(q2.shape, dtype=q2.dtype, device=q2.device)
     desc.out_stride[:] = out.stride()[:3]
+    lib = N.load()
     with N.on_device(q2):
-        N.check("rpfq_window_attention", N.load().rpfq_window_attention(
-            ctypes.byref(desc), q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), N.ptr(lengths), out.data_ptr(), None, N.stream_of(q2)))
+        work = torch.empty(lib.rpfq_window_attention_workspace_bytes(ctypes.byref(desc), 0), dtype=torch.uint8, device=q2.device)
+        N.check("rpfq_window_attention", lib.rpfq_window_attention(
+            ctypes.byref(desc), q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), N.ptr(lengths), out.data_ptr(), None,
+            work.data_ptr() or None, work.numel(), N.stream_of(q2)))
     return out[..., :q.shape[3]].contiguous()
 
 

@@ -113,7 +113,9 @@ def _check(got, want, bound, rounding=0.0):
 SHAPES = [(1, 1, 1, 1, 64, 1, 0, None), (2, 5, 4, 1, 8, 2, 1, [5, 0]), (1, 33, 2, 2, 32, 8, 0, None), (2, 64, 6, 2, 128, 1000, 0, [64, 31]),
           (1, 65, 8, 2, 96, 16, 4, None), (3, 127, 3, 1, 40, 31, 70, [127, 1, 96]), (1, 129, 4, 4, 72, 64, 2, None),
           (2, 200, 4, 2, 17, 50, 3, [200, 129]), (1, 300, 16, 4, 128, 65, 16, None), (2, 257, 2, 2, 64, 1, 1, [1000, -3]),
-          (1, 450, 2, 1, 104, 130, 200, None), (1, 197, 12, 12, 64, 500, 500, None), (2, 130, 5, 5, 24, 7, 0, [66, 130])]
+          (1, 450, 2, 1, 104, 130, 200, None), (1, 197, 12, 12, 64, 500, 500, None), (2, 130, 5, 5, 24, 7, 0, [66, 130]),
+          # sinks whose far ranges are divided among workgroups
+          (1, 1100, 4, 2, 64, 20, 3, None), (2, 900, 4, 1, 32, 9, 65, [900, 333]), (1, 1409, 2, 2, 128, 60, 128, None)]
 
 
 def _inputs(b, n, heads, kv, d, dtype, seed):
@@ -436,8 +438,8 @@ def test_argument_errors():
                 setattr(d, name, v)
         return ctypes.byref(d)
 
-    def fwd(q=at, k=at, v=at, lens=None, out=at, stat=at, **kw):
-        return L.rpfq_window_attention(desc(False, **kw), q, k, v, lens, out, stat, None)
+    def fwd(q=at, k=at, v=at, lens=None, out=at, stat=at, work=at, nb=1 << 40, **kw):
+        return L.rpfq_window_attention(desc(False, **kw), q, k, v, lens, out, stat, work, nb, None)
 
     def grad(q=at, k=at, v=at, lens=None, out=at, go=at, stat=at, gq=at, gk=at, gv=at, work=at, nb=1 << 40, **kw):
         return L.rpfq_window_attention_grad(desc(False, **kw), q, k, v, lens, out, go, stat, gq, gk, gv, work, nb, None)
@@ -445,7 +447,7 @@ def test_argument_errors():
     def cached(q=at, k=at, v=at, lens=at, out=at, work=at, nb=1 << 40, **kw):
         return L.rpfq_window_attention_cached(desc(True, **kw), q, k, v, lens, out, work, nb, None)
 
-    assert L.rpfq_window_attention(None, at, at, at, None, at, at, None) == 1
+    assert L.rpfq_window_attention(None, at, at, at, None, at, at, at, 1 << 40, None) == 1
     for call in (fwd, grad, cached):
         for name in ("q", "k", "v", "out"):
             assert call(**{name: None}) == 1, (call, name)
@@ -465,5 +467,8 @@ def test_argument_errors():
     assert grad(go=at + 8) == 3 and grad(gq=at + 8) == 3 and grad(gk=at + 8) == 3 and grad(gv=at + 8) == 3 and grad(work=at + 64) == 3
     assert grad(grad_stride=(8, 4, 8)) == 3
     size = L.rpfq_window_attention_stat_bytes(desc(False))
-    assert size == 2 * 4 * 64 * 4 and L.rpfq_window_attention_stat_bytes(desc(False, N=0)) == 0 and grad(nb=size - 1) == 2
+    assert size == 2 * 4 * 64 * 4 and L.rpfq_window_attention_stat_bytes(desc(False, N=0)) == 0
+    need = L.rpfq_window_attention_workspace_bytes
+    assert need(desc(False), 0) == 0 and need(desc(False), 1) >= size and need(desc(False, N=0), 1) == 0
+    assert grad(nb=need(desc(False), 1) - 1) == 2
     assert cached(lens=None) == 1 and L.rpfq_window_attention_cached_workspace_bytes(desc(True, window=0)) == 0
