@@ -839,48 +839,70 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
     }
 }
 
-// Rows [sequence][token][head] from their slots, in their order, DP / 8 threads a
-// row: outputs (a slot: sums, their exponent, their weight), or plain sums times
-// `factor` (GRAD: no exponents).  A slot without any has the exponent -inf.
+// Rows [sequence][token][head] from their slots, a workgroup a row: DP / 4 threads
+// hold its values, the others every so many slots (one thread over 49 slots of a
+// gradient's 16 rows: 17 us, so 5).  Outputs (a slot: sums, their exponent,
+// their weight), or plain sums times `factor` (GRAD: no exponents).  A slot
+// without any has the exponent -inf.
+constexpr int kWinSlots = 256;
 struct WinJoin {
     const float* part;
-    char* out;
+    char* out[2];         // GRAD: keys and values, rows of one behind the other's; NULL: not wanted
+    float factor[2];
     float* stat;          // [B, heads, NP], or NULL
     int64_t os[3];
     int64_t rows;         // sequences x tokens x heads
     int tokens, heads, slots, D, NP;
-    float factor;
 };
 template <int DP, bool BF, bool GRAD>
 __global__ void __launch_bounds__(256) window_join_kernel(WinJoin a) {
-    constexpr int PER = 256 / (DP / 8), LD = DP + 8;
-    const int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / (DP / 8);
-    const int d = 8 * (threadIdx.x % (DP / 8));
-    if (threadIdx.x / (DP / 8) >= PER || row >= a.rows || d >= a.D) return;
-    const float* src = a.part + row * a.slots * LD;
-    float m = -__builtin_inff(), l = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (!GRAD)
-        for (int s = 0; s < a.slots; ++s) m = fmaxf(m, src[s * LD + DP]);
-    for (int s = 0; s < a.slots; ++s) {
-        const float* p = src + s * LD;
-        float f = 1.0f;
-        if (!GRAD) {
-            f = p[DP];
-            if (f == -__builtin_inff()) continue;
-            f = __builtin_amdgcn_exp2f(f - m);
-            l = fmaf(f, p[DP + 1], l);
-        }
-#pragma unroll
-        for (int t = 0; t < 8; ++t) v[t] = fmaf(f, p[d + t], v[t]);
+    constexpr int LD = DP + 8, TD = DP / 4, SG = 256 / TD;  // SG slots at once (DP = 96: 10, and threads to spare)
+    __shared__ float weight[kWinSlots], most[4], total[4];
+    __shared__ f32x4 sums[SG][TD];
+    const int tid = threadIdx.x, which = blockIdx.x >= a.rows;
+    const int64_t row = (int64_t)blockIdx.x - (which ? a.rows : 0);
+    char* out = a.out[which];
+    if (!out) return;
+    const float* src = a.part + (int64_t)blockIdx.x * a.slots * LD;
+    float m = 0.0f, l = 0.0f;
+    if (!GRAD) {
+        const float e = tid < a.slots ? src[tid * LD + DP] : -__builtin_inff();
+        m = group_max<64>(e);
+        if ((tid & 63) == 0) most[tid >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        const float f = e == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(e - m);
+        weight[tid] = f;
+        l = group_sum<64>(f != 0.0f ? f * src[tid * LD + DP + 1] : 0.0f);
+        if ((tid & 63) == 0) total[tid >> 6] = l;
+        __syncthreads();
+        l = total[0] + total[1] + total[2] + total[3];
     }
-    const int64_t seq = row / (a.tokens * a.heads);
+    const int d = tid % TD, sg = tid / TD;
+    f32x4 v = {0, 0, 0, 0};
+    if (sg < SG)
+#pragma unroll 4
+        for (int s = sg; s < a.slots; s += SG) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(src + s * LD + 4 * d);
+            const float f = GRAD ? 1.0f : weight[s];
+            if (GRAD || f != 0.0f)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) v[t] = fmaf(f, x[t], v[t]);
+        }
+    if (sg < SG) sums[sg][d] = v;
+    __syncthreads();
+    const int64_t seq = row / ((int64_t)a.tokens * a.heads);
     const int rest = (int)(row - seq * a.tokens * a.heads), tok = rest / a.heads, h = rest - tok * a.heads;
-    if (!GRAD && a.stat && d == 0)
+    if (!GRAD && a.stat && tid == 0)
         a.stat[(seq * a.heads + h) * a.NP + tok] = l == 0.0f ? -__builtin_inff() : (BF ? 0.0f : 15.0f) - (m + __builtin_amdgcn_logf(l));
-    const float inv = GRAD ? a.factor : l == 0.0f ? 0.0f : 1.0f / l;
-    *reinterpret_cast<uint4*>(a.out + seq * a.os[0] + tok * a.os[1] + h * a.os[2] + 2 * d) =
-        make_uint4(win_pack<BF>(v[0] * inv, v[1] * inv), win_pack<BF>(v[2] * inv, v[3] * inv), win_pack<BF>(v[4] * inv, v[5] * inv),
-                   win_pack<BF>(v[6] * inv, v[7] * inv));
+    if (sg || 4 * d >= a.D) return;
+#pragma unroll
+    for (int s = 1; s < SG; ++s)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[t] += sums[s][d][t];
+    const float inv = GRAD ? a.factor[which] : l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<uint2*>(out + seq * a.os[0] + tok * a.os[1] + h * a.os[2] + 8 * d) =
+        make_uint2(win_pack<BF>(v[0] * inv, v[1] * inv), win_pack<BF>(v[2] * inv, v[3] * inv));
 }
 
 // ---------------------------------------------------------------------------
@@ -921,12 +943,17 @@ static hipError_t win_launch(K kernel, std::atomic<uint64_t>& done, const WinArg
     }()
 
 template <int DP, bool BF, bool GRAD>
-static hipError_t win_join(const WinArgs& a, const float* part, char* out, const int64_t (&os)[3], float* stat, int tokens, int heads,
-                           int slots, float factor, hipStream_t s) {
-    const WinJoin j = {part, out, stat, {os[0], os[1], os[2]}, (int64_t)a.B * tokens * heads, tokens, heads, slots, a.D, a.NP, factor};
-    constexpr int PER = 256 / (DP / 8);
-    hipLaunchKernelGGL((window_join_kernel<DP, BF, GRAD>), dim3((unsigned)((j.rows + PER - 1) / PER)), dim3(256), 0, s, j);
+static hipError_t win_join(WinJoin j, hipStream_t s) {
+    hipLaunchKernelGGL((window_join_kernel<DP, BF, GRAD>), dim3((unsigned)(j.rows * (j.out[1] ? 2 : 1))), dim3(256), 0, s, j);
     return hipGetLastError();
+}
+// rows of `tokens` contiguous tokens of n a sequence
+static WinJoin win_joined(const WinArgs& a, const float* part, int tokens, int64_t n, int heads, int slots) {
+    WinJoin j = {part};
+    j.os[0] = n * heads * 2 * a.D, j.os[1] = (int64_t)heads * 2 * a.D, j.os[2] = 2 * a.D;
+    j.rows = (int64_t)a.B * tokens * heads;
+    j.tokens = tokens, j.heads = heads, j.slots = slots, j.D = a.D, j.NP = a.NP;
+    return j;
 }
 struct WinForward {
     const WinArgs& a;
@@ -936,7 +963,10 @@ struct WinForward {
         const hipError_t e = WIN_LAUNCH((window_forward_kernel<DP, BF>), a, win_units(a.far, (int64_t)a.B * (a.H / a.hw), a.tiles), 256,
                                         4 * 64 * Rows<DP>::RB, s);
         if (e != hipSuccess || !a.far.parts) return e;
-        return win_join<DP, BF, false>(a, a.part, a.out, a.os, a.stat, a.far.rows, a.H, a.far.parts + 1, 0.0f, s);
+        WinJoin j = win_joined(a, a.part, a.far.rows, a.N, a.H, a.far.parts + 1);
+        for (int i = 0; i < 3; ++i) j.os[i] = a.os[i];
+        j.out[0] = a.out, j.stat = a.stat;
+        return win_join<DP, BF, false>(j, s);
     }
 };
 struct WinGrad {
@@ -947,19 +977,17 @@ struct WinGrad {
         hipError_t e = WIN_LAUNCH((window_grad_q_kernel<DP, BF>), a, win_units(a.far, (int64_t)a.B * (a.H / a.hw), a.tiles), 256,
                                   4 * 64 * Rows<DP>::RB, s);
         if (e == hipSuccess && a.gq && a.far.parts) {
-            const int64_t os[3] = {(int64_t)a.N * a.H * 2 * a.D, (int64_t)a.H * 2 * a.D, 2 * a.D};
-            e = win_join<DP, BF, true>(a, a.part, a.gq, os, nullptr, a.far.rows, a.H, a.far.parts + 1, a.scale, s);
+            WinJoin j = win_joined(a, a.part, a.far.rows, a.N, a.H, a.far.parts + 1);
+            j.out[0] = a.gq, j.factor[0] = a.scale;
+            e = win_join<DP, BF, true>(j, s);
         }
         if (e != hipSuccess || (!a.gk && !a.gv)) return e;
         e = WIN_LAUNCH((window_grad_kv_kernel<DP, BF>), a, win_units(a.kfar, (int64_t)a.B * a.KV, (a.N + kWinKeys - 1) / kWinKeys), 256,
                        win_grad_lds<DP>(), s);
-        for (int w = 0; w < 2 && a.kfar.parts && e == hipSuccess; ++w) {
-            char* dst = w ? a.gv : a.gk;
-            const int64_t os[3] = {(int64_t)a.N * a.KV * 2 * a.D, (int64_t)a.KV * 2 * a.D, 2 * a.D};
-            const float* part = a.kpart + (int64_t)w * a.B * a.kfar.rows * a.KV * (a.kfar.parts + 1) * (DP + 8);
-            if (dst) e = win_join<DP, BF, true>(a, part, dst, os, nullptr, a.kfar.rows, a.KV, a.kfar.parts + 1, w ? 1.0f : a.scale, s);
-        }
-        return e;
+        if (e != hipSuccess || !a.kfar.parts) return e;
+        WinJoin j = win_joined(a, a.kpart, a.kfar.rows, a.N, a.KV, a.kfar.parts + 1);
+        j.out[0] = a.gk, j.out[1] = a.gv, j.factor[0] = a.scale, j.factor[1] = 1.0f;
+        return win_join<DP, BF, true>(j, s);
     }
 };
 template <int DP>
@@ -974,8 +1002,9 @@ struct WinCached {
     hipError_t run() {
         const hipError_t e = WIN_LAUNCH((window_cached_kernel<DP, BF>), a, (int64_t)a.B * a.KV * a.blocks * a.splits, 256, win_cached_lds<DP>(), s);
         if (e != hipSuccess || a.splits == 1) return e;
-        const int64_t os[3] = {(int64_t)a.N * a.H * 2 * a.D, (int64_t)a.H * 2 * a.D, 2 * a.D};
-        return win_join<DP, BF, false>(a, a.part, a.out, os, nullptr, a.N, a.H, a.splits, 0.0f, s);
+        WinJoin j = win_joined(a, a.part, a.N, a.N, a.H, a.splits);
+        j.out[0] = a.out;
+        return win_join<DP, BF, false>(j, s);
     }
 };
 template <bool BF, class Go>
@@ -1049,7 +1078,7 @@ int window_splits(const rpfq_window_desc& d) {
     keys = keys < d.M ? keys : d.M;
     const int64_t most = (keys + 127) / 128, want = (4 * (int64_t)device_cus() + units - 1) / units;
     const int64_t s = most < want ? most : want;
-    return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+    return (int)(s < 1 ? 1 : s > kWinSlots ? kWinSlots : s);
 }
 size_t window_cached_bytes(const rpfq_window_desc& d) {
     const int s = window_splits(d);
