@@ -80,6 +80,22 @@ struct Frags {
     }
 };
 
+// A step's fragments in the order of their products, PD of them ahead: left to
+// itself the compiler reads each one right before its product and waits.
+template <int N, int PD, class Read, class Use, int... E>
+__device__ __forceinline__ void win_each(uint4 (&ring)[PD], Read read, Use use, std::integer_sequence<int, E...>) {
+    ((use(E, ring[E % PD]), E + PD < N ? (void)(ring[E % PD] = read(E + PD)) : (void)0, __builtin_amdgcn_sched_barrier(0)), ...);
+}
+template <int N, int PD, class Read, class Use>
+__device__ __forceinline__ void win_stream(Read read, Use use) {
+    uint4 ring[PD];
+#pragma unroll
+    for (int e = 0; e < PD; ++e) ring[e] = read(e);
+    __builtin_amdgcn_sched_barrier(0);
+    win_each<N, PD>(ring, read, use, std::make_integer_sequence<int, N>());
+}
+#define WIN_INLINE __attribute__((always_inline))
+
 template <bool BF>
 __device__ __forceinline__ floatx16 win_mma(uint4 a, uint4 b, floatx16 c) {
     if constexpr (BF) return MmaBf16::mma(a, b, c);
@@ -124,11 +140,12 @@ __device__ __forceinline__ float win_dot8(uint4 a, uint4 b, float c) {
     return c;
 }
 
-// Probabilities are formed times 2^-kWinShift.  fp16: 2^15, normal down to 2^-29
-// of the row's largest.  bf16 has float32's range and so have its values: 2^-20,
-// so that a million of them stay within float32.
+// Probabilities are formed times 2^-win_shift.  fp16: 2^7, where they pass 1 by
+// 2^kWinLag at most, normal down to 2^-21 of the row's largest and off by less
+// than 2^-32 of it below.  bf16 has float32's range and so have its values:
+// 2^-28, so that a million of them stay within float32.
 template <bool BF>
-constexpr float win_shift() { return BF ? 20.0f : -15.0f; }
+constexpr float win_shift() { return BF ? 28.0f : -7.0f; }
 
 // A tile with sinks has far more to go over than the others: every key (sinks as
 // queries, where not causal), every query (sinks as keys).  What lies past the
@@ -225,56 +242,76 @@ __device__ __forceinline__ void win_store(const floatx16 (&o)[DP / 32], float f,
         }
 }
 
-// A 16-bit row's values 16 s + 8 g .. + 7 (zeros past D or where it is not inside).
+// A 16-bit row's values 16 s + 8 g .. + 7, zeros past D or where it is not inside:
+// there `base`, a row that is, is read in its place, so that the loads go out
+// together (behind branches the compiler waits for each).
 template <int DP>
-__device__ __forceinline__ void win_row(uint4 (&f)[DP / 16], const char* src, bool inside, int D, int g) {
+__device__ __forceinline__ void win_row(uint4 (&f)[DP / 16], const char* base, int64_t off, bool inside, int D, int g) {
+    const char* src = base + (inside ? off : 0);
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
-        f[s] = make_uint4(0, 0, 0, 0);
-        if (inside && 16 * s + 8 * g < D) f[s] = *reinterpret_cast<const uint4*>(src + 32 * s + 16 * g);
+        const bool in = 16 * s + 8 * g < D;
+        f[s] = *reinterpret_cast<const uint4*>(src + (in ? 32 * s + 16 * g : 0));
+    }
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+        const bool in = (16 * s + 8 * g < D) & inside;
+        f[s] = make_uint4(in ? f[s].x : 0, in ? f[s].y : 0, in ? f[s].z : 0, in ? f[s].w : 0);
     }
 }
 
+// The compiler's wait for a load stands here, and not at its first use: in a loop
+// that would be a wait for the DMA of the next tile too, which it does not count.
+template <int N>
+__device__ __forceinline__ void win_arrived(uint4 (&f)[N]) {
+#pragma unroll
+    for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s].x), "+v"(f[s].y), "+v"(f[s].z), "+v"(f[s].w));
+}
 __device__ __forceinline__ void win_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// The running softmax of a lane's query over 32 more keys (two lanes hold one
-// query's 32 scores, half each): `top` the largest score so far, `sub` = top
-// scale2 + shift as it is rounded, the exponent that is subtracted; l the sum.
+// The running softmax of a lane's query over more keys (two lanes hold one query's
+// scores, half each): `top` the score that is subtracted, `sub` = top scale2 +
+// shift as it is rounded; l the sum.  top follows the largest score only where
+// that passes it by 2^kWinLag, so that the sums are hardly ever scaled anew.
 struct WinState {
     float top, sub, l;
 };
-// P of KB blocks of 32 scores in place; returns the factor of what was summed before.
-template <int KB, bool BF>
-__device__ __forceinline__ float win_softmax(floatx16 (&s)[KB], WinState& st, float scale2) {
+constexpr float kWinLag = 8.0f;
+// P of KB blocks of 32 scores in place; anew(f): what was summed before is scaled.
+template <int KB, bool BF, class Anew>
+__device__ __forceinline__ void win_softmax(floatx16 (&s)[KB], WinState& st, float scale2, Anew anew) {
     float mx = s[0][0];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[kb][v]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float top = fmaxf(st.top, mx);
-    const float base = top == -__builtin_inff() ? 0.0f : top;  // nothing seen yet: exp2(-inf) is 0
-    const float sub = fmaf(base, scale2, win_shift<BF>());
-    float f;
+    if (__any((mx - st.top) * scale2 > kWinLag)) {  // NaN (-inf - -inf): nothing seen yet, nothing to scale
+        const float top = fmaxf(st.top, mx);
+        const float base = top == -__builtin_inff() ? 0.0f : top;
+        const float sub = fmaf(base, scale2, win_shift<BF>());
+        const bool far = fabsf(base) * scale2 > 0x1p20f;
+        const float f = __builtin_amdgcn_exp2f(far ? (st.top - base) * scale2 : st.sub - sub);
+        st.top = top;
+        st.sub = top == -__builtin_inff() ? -__builtin_inff() : sub;
+        st.l *= f;
+        anew(f);
+    }
+    const float base = st.top == -__builtin_inff() ? 0.0f : st.top;  // nothing seen yet: exp2(-inf) is 0
     // scores far from 0: the rounding of `sub` would carry probabilities out of
     // fp16's range, so the largest is subtracted first
     if (__any(fabsf(base) * scale2 > 0x1p20f)) {
-        f = __builtin_amdgcn_exp2f((st.top - base) * scale2);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int v = 0; v < 16; ++v) s[kb][v] = __builtin_amdgcn_exp2f(fmaf(s[kb][v] - base, scale2, -win_shift<BF>()));
     } else {
-        f = __builtin_amdgcn_exp2f(st.sub - sub);
+        const float sub = st.top == -__builtin_inff() ? 0.0f : st.sub;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int v = 0; v < 16; ++v) s[kb][v] = __builtin_amdgcn_exp2f(fmaf(s[kb][v], scale2, -sub));
     }
-    st.top = top;
-    st.sub = top == -__builtin_inff() ? -__builtin_inff() : sub;
-    st.l *= f;
-    return f;
 }
 
 // Unit of a launch over `groups` x `tiles`: (group, tile, part), the parts of the
@@ -360,7 +397,7 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
     const WinPlace p = win_place(a, wave);
     const int i = p.mine + r, last = (p.mine + 31 < p.n - 1 ? p.mine + 31 : p.n - 1);
     uint4 q[DP / 16];
-    win_row<DP>(q, a.q + p.b * a.qs[0] + (int64_t)i * a.qs[1] + p.h * a.qs[2], i < p.n, a.D, g);
+    win_row<DP>(q, a.q + p.b * a.qs[0] + p.h * a.qs[2], i * a.qs[1], i < p.n, a.D, g);
     const WinTiles tiles = win_keys<T>(a, p);
     RowLoads<DP, T, 4> lk, lv;
     lk.init(a.ks[1], a.D, wave, lane);
@@ -380,6 +417,7 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
     floatx16 o[DP / 32];
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
+    win_arrived(q);
     if (tiles.count) issue(0);
     for (int t = 0; t < tiles.count; ++t) {
         win_sync();
@@ -388,38 +426,44 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
         const int seen = last < p.mine ? 0 : win_class(a, p.mine, last, k0, k0 + T - 1);
         if (!seen) continue;
         const uint32_t kt = lds + (t & 1) * 2 * TILE, vt = kt + TILE;
+        constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = DP > 96 ? 8 : 6;
+        auto read = [&](int e) WIN_INLINE {
+            if (e < 2 * NS) return at.rows(kt + e / NS * 32 * RB, e % NS);
+            return at.cols(vt + (e - 2 * NS) / NJ * 16 * RB, (e - 2 * NS) % NJ);
+        };
+        uint4 pr;
         floatx16 s[2];
+        s[0] = s[1] = floatx16{0};
+        win_stream<2 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
+            if (e < 2 * NS) {
+                s[e / NS] = win_mma<BF>(f, q[e % NS], s[e / NS]);
+                if (e < 2 * NS - 1) return;
+                if (seen == 1 || k0 + T > p.n) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            s[kb] = floatx16{0};
+                    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int e = 0; e < DP / 16; ++e) s[kb] = win_mma<BF>(at.rows(kt + kb * 32 * Rows<DP>::RB, e), q[e], s[kb]);
-        }
-        if (seen == 1 || k0 + T > p.n) {
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
-                    s[kb][v] = in ? s[kb][v] : -__builtin_inff();
+                        for (int v = 0; v < 16; ++v) {
+                            const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
+                            s[kb][v] = in ? s[kb][v] : -__builtin_inff();
+                        }
                 }
-        }
-        const float f = win_softmax<2, BF>(s, st, a.scale2);
-        if (__any(f != 1.0f)) {
+                win_softmax<2, BF>(s, st, a.scale2, [&](float f) {
 #pragma unroll
-            for (int j = 0; j < DP / 32; ++j)
+                    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) o[j][v] *= f;
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const uint4 pr = win_pack8<BF>(s[u >> 1], u & 1);
-            // the sum of the rounded probabilities: their rounding errors then
-            // weigh the values' distance to the output, not the values
-            st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
-#pragma unroll
-            for (int j = 0; j < DP / 32; ++j) o[j] = win_mma<BF>(at.cols(vt + u * 16 * Rows<DP>::RB, j), pr, o[j]);
-        }
+                        for (int v = 0; v < 16; ++v) o[j][v] *= f;
+                });
+                return;
+            }
+            const int u = (e - 2 * NS) / NJ, j = (e - 2 * NS) % NJ;
+            if (j == 0) {
+                pr = win_pack8<BF>(s[u >> 1], u & 1);
+                // the sum of the rounded probabilities: their rounding errors then
+                // weigh the values' distance to the output, not the values
+                st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
+            }
+            o[j] = win_mma<BF>(f, pr, o[j]);
+        });
     }
     const float l = st.l + __shfl_xor(st.l, 32, 64);
     const bool any = l != 0.0f && i < p.n;
@@ -475,18 +519,18 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
     const int i = p.mine + r, last = (p.mine + 31 < p.n - 1 ? p.mine + 31 : p.n - 1);
     const int64_t row = ((int64_t)p.b * a.H + p.h) * a.NP + i;
     uint4 q[DP / 16], go[DP / 16];
-    win_row<DP>(q, a.q + p.b * a.qs[0] + (int64_t)i * a.qs[1] + p.h * a.qs[2], i < p.n, a.D, g);
-    win_row<DP>(go, a.go + p.b * a.gos[0] + (int64_t)i * a.gos[1] + p.h * a.gos[2], i < p.n, a.D, g);
+    win_row<DP>(q, a.q + p.b * a.qs[0] + p.h * a.qs[2], i * a.qs[1], i < p.n, a.D, g);
+    win_row<DP>(go, a.go + p.b * a.gos[0] + p.h * a.gos[2], i * a.gos[1], i < p.n, a.D, g);
     float delta = 0.0f;
     {
         uint4 out[DP / 16];
-        win_row<DP>(out, a.o + p.b * a.os[0] + (int64_t)i * a.os[1] + p.h * a.os[2], i < p.n, a.D, g);
+        win_row<DP>(out, a.o + p.b * a.os[0] + p.h * a.os[2], i * a.os[1], i < p.n, a.D, g);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) delta = win_dot8<BF>(go[s], out[s], delta);
         delta += __shfl_xor(delta, 32, 64);
     }
     if (g == 0 && i < a.NP && !p.unit.part) a.delta[row] = delta;
-    const float stat = i < a.NP ? a.stat[row] : -__builtin_inff();
+    float stat = i < a.NP ? a.stat[row] : -__builtin_inff();
     if (!a.gq) return;
     const WinTiles tiles = win_keys<T>(a, p);
     RowLoads<DP, T, 4> lk, lv;
@@ -507,6 +551,9 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
     float c = BF ? 1.0f : 0x1p126f;
+    win_arrived(q);
+    win_arrived(go);
+    asm volatile("" : "+v"(stat), "+v"(delta));
     if (tiles.count) issue(0);
     for (int t = 0; t < tiles.count; ++t) {
         win_sync();
@@ -515,30 +562,40 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
         const int seen = last < p.mine ? 0 : win_class(a, p.mine, last, k0, k0 + T - 1);
         if (!seen) continue;
         const bool some = seen == 1 || k0 + T > p.n;
+        constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = 4;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-            const uint32_t kt = lds + (t & 1) * 2 * TILE + kb * 32 * Rows<DP>::RB, vt = kt + TILE;
+            const uint32_t kt = lds + (t & 1) * 2 * TILE + kb * 32 * RB, vt = kt + TILE;
+            auto read = [&](int e) WIN_INLINE {
+                if (e < 2 * NS) return at.rows(e < NS ? kt : vt, e % NS);
+                return at.cols(kt + (e - 2 * NS) / NJ * 16 * RB, (e - 2 * NS) % NJ);
+            };
+            uint4 ds;
             floatx16 s = floatx16{0}, dp = floatx16{0};
-#pragma unroll
-            for (int e = 0; e < DP / 16; ++e) s = win_mma<BF>(at.rows(kt, e), q[e], s);
-#pragma unroll
-            for (int e = 0; e < DP / 16; ++e) dp = win_mma<BF>(at.rows(vt, e), go[e], dp);
-#pragma unroll
-            for (int v = 0; v < 16; ++v) s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, stat)) * (dp[v] - delta);
-            if (some) {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
-                    s[v] = in ? s[v] : 0.0f;
+            win_stream<2 * NS + 2 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
+                if (e < NS) {
+                    s = win_mma<BF>(f, q[e], s);
+                    return;
                 }
-            }
-            win_scale_ds<DP, BF>(s, c, o);
+                if (e < 2 * NS) {
+                    dp = win_mma<BF>(f, go[e - NS], dp);
+                    if (e < 2 * NS - 1) return;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint4 ds = win_pack8<BF>(s, u);
+                    for (int v = 0; v < 16; ++v) s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, stat)) * (dp[v] - delta);
+                    if (some) {
 #pragma unroll
-                for (int j = 0; j < DP / 32; ++j) o[j] = win_mma<BF>(at.cols(kt + u * 16 * Rows<DP>::RB, j), ds, o[j]);
-            }
+                        for (int v = 0; v < 16; ++v) {
+                            const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
+                            s[v] = in ? s[v] : 0.0f;
+                        }
+                    }
+                    win_scale_ds<DP, BF>(s, c, o);
+                    return;
+                }
+                const int u = (e - 2 * NS) / NJ, j = (e - 2 * NS) % NJ;
+                if (j == 0) ds = win_pack8<BF>(s, u);
+                o[j] = win_mma<BF>(f, ds, o[j]);
+            });
         }
     }
     const float f = (BF ? 1.0f : 0x1p-15f) / c;
@@ -584,7 +641,7 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
     const int n = win_length(a, b, a.N), k0 = unit.tile * kWinKeys, mine = k0 + 32 * block, key = mine + r;
     const int klast = (mine + 31 < n - 1 ? mine + 31 : n - 1), kend = (k0 + kWinKeys < n ? k0 + kWinKeys : n) - 1;
     uint4 kf[DP / 16];
-    win_row<DP>(kf, a.k + b * a.ks[0] + (int64_t)key * a.ks[1] + kv * a.ks[2], key < n, a.D, g);
+    win_row<DP>(kf, a.k + b * a.ks[0] + kv * a.ks[2], key * a.ks[1], key < n, a.D, g);
     // the queries that see them: first tiles (seeing all), then [t0, t1), for each head
     int lo = a.causal ? k0 : k0 - a.window + 1, hi = kend + a.window;
     if (k0 < a.sinks) hi = n, lo = a.causal ? lo : 0;
@@ -628,8 +685,10 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
     const WinMask mask(a, n);
     float c = BF ? 1.0f : 0x1p126f;
     int ct = 0;
+    win_arrived(kf);
     for (int t = 0; t < steps; ++t) {
         win_sync();
+        asm volatile("" : "+v"(stat_next), "+v"(delta_next));
         stat = stat_next, delta = delta_next;
         if (t + 1 < steps) issue(t + 1);
         const int q0 = q.at(ct) * kWinStep + 32 * half, qlast = (q0 + 31 < n - 1 ? q0 + 31 : n - 1);
@@ -638,33 +697,42 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
         if (!seen) continue;
         const uint32_t qtile = lds + V + (t & 1) * STAGE + 32 * half * RB, otile = qtile + kWinStep * RB;
         const uint32_t vt = lds + 32 * block * RB;
+        constexpr int NS = DP / 16, NJ = DP / 32, PD = 4;
+        // Q; dO and V in turn; dO and Q transposed
+        auto read = [&](int e) WIN_INLINE {
+            if (e < NS) return at.rows(qtile, e);
+            if (e < 3 * NS) return at.rows((e - NS) & 1 ? vt : otile, (e - NS) / 2);
+            const int x = e - 3 * NS;
+            return at.cols((x < 2 * NJ ? otile : qtile) + x / NJ % 2 * 16 * RB, x % NJ);
+        };
+        uint4 pr, was;
         floatx16 s = floatx16{0}, dp = floatx16{0};
-#pragma unroll
-        for (int e = 0; e < DP / 16; ++e) s = win_mma<BF>(at.rows(qtile, e), kf[e], s);
-#pragma unroll
-        for (int e = 0; e < DP / 16; ++e) dp = win_mma<BF>(at.rows(otile, e), at.rows(vt, e), dp);
-        win_probs(std::make_integer_sequence<int, 16>(), s, dp, a.scale2, stat, delta);
-        if (seen == 1) {
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const bool in = mask(q0 + acc_row(v, g), key);
-                s[v] = in ? s[v] : 0.0f;
-                dp[v] = in ? dp[v] : 0.0f;
+        win_stream<3 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
+            if (e < NS) {
+                s = win_mma<BF>(f, kf[e], s);
+                return;
             }
-        }
+            if (e < 3 * NS) {
+                if ((e - NS) & 1) dp = win_mma<BF>(was, f, dp);
+                else was = f;
+                if (e < 3 * NS - 1) return;
+                win_probs(std::make_integer_sequence<int, 16>(), s, dp, a.scale2, stat, delta);
+                if (seen == 1) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const uint4 pr = win_pack8<BF>(s, e);
-#pragma unroll
-            for (int j = 0; j < DP / 32; ++j) ov[j] = win_mma<BF>(at.cols(otile + e * 16 * RB, j), pr, ov[j]);
-        }
-        win_scale_ds<DP, BF>(dp, c, ok);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const uint4 ds = win_pack8<BF>(dp, e);
-#pragma unroll
-            for (int j = 0; j < DP / 32; ++j) ok[j] = win_mma<BF>(at.cols(qtile + e * 16 * RB, j), ds, ok[j]);
-        }
+                    for (int v = 0; v < 16; ++v) {
+                        const bool in = mask(q0 + acc_row(v, g), key);
+                        s[v] = in ? s[v] : 0.0f;
+                        dp[v] = in ? dp[v] : 0.0f;
+                    }
+                }
+                return;
+            }
+            const int x = e - 3 * NS, j = x % NJ;
+            if (x == 2 * NJ) win_scale_ds<DP, BF>(dp, c, ok);
+            if (j == 0) pr = win_pack8<BF>(x < 2 * NJ ? s : dp, x / NJ % 2);
+            if (x < 2 * NJ) ov[j] = win_mma<BF>(f, pr, ov[j]);
+            else ok[j] = win_mma<BF>(f, pr, ok[j]);
+        });
     }
     // the fellow's sums through LDS, one tensor after the other
     const float fv = BF ? 1.0f : 0x1p-15f;
@@ -725,7 +793,7 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
     const bool inside = row < a.rows;
     const int len = win_length(a, b, a.M), i = len - a.N + tok;
     uint4 q[DP / 16];
-    win_row<DP>(q, a.q + b * a.qs[0] + tok * a.qs[1] + h * a.qs[2], inside, a.D, g);
+    win_row<DP>(q, a.q + b * a.qs[0], tok * a.qs[1] + h * a.qs[2], inside, a.D, g);
 
     const int lo = len - a.N - a.window + 1 < 0 ? 0 : len - a.N - a.window + 1;
     const int sinks = a.sinks < len ? a.sinks : len;
@@ -756,6 +824,7 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
     for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
     const WinMask mask(a, len);
     int s = from + wave, buf = 0;
+    win_arrived(q);
     if (s < to) issue(s, 0);
     for (; s < to; s += 4, buf ^= 1) {
         if (s + 4 < to) {
@@ -777,13 +846,12 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
                 sc[0][v] = in ? sc[0][v] : -__builtin_inff();
             }
         }
-        const float f = win_softmax<1, BF>(sc, st, a.scale2);
-        if (__any(f != 1.0f)) {
+        win_softmax<1, BF>(sc, st, a.scale2, [&](float f) {
 #pragma unroll
             for (int j = 0; j < DP / 32; ++j)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) o[j][v] *= f;
-        }
+        });
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const uint4 pr = win_pack8<BF>(sc[0], e);
