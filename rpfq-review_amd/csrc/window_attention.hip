@@ -58,17 +58,24 @@ struct RowLoads {
 template <int DP>
 struct Frags {
     uint32_t row[DP / 16], col[DP / 32][2];
-    __device__ __forceinline__ void init(int lane) {
+    __device__ __forceinline__ void init(uint32_t at, int lane) {
         using T = Rows<DP>;
         const int r = lane & 31, g = lane >> 5, i16 = lane & 15, hf = (lane >> 4) & 1;
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) row[s] = r * T::RB + (((2 * s + g) ^ T::swz(r)) * 16);
+        for (int s = 0; s < DP / 16; ++s) row[s] = at + r * T::RB + (((2 * s + g) ^ T::swz(r)) * 16);
         const int tr = 4 * g + (i16 >> 2);
 #pragma unroll
         for (int j = 0; j < DP / 32; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                col[j][h] = (tr + 8 * h) * T::RB + (((4 * j + 2 * hf + ((i16 & 3) >> 1)) ^ T::swz(tr + 8 * h)) * 16) + (i16 & 1) * 8;
+                col[j][h] = at + (tr + 8 * h) * T::RB + (((4 * j + 2 * hf + ((i16 & 3) >> 1)) ^ T::swz(tr + 8 * h)) * 16) + (i16 & 1) * 8;
+    }
+    // to the other stage: once a step, where a read's own sum would be one each
+    __device__ __forceinline__ void move(uint32_t by) {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) row[s] += by;
+#pragma unroll
+        for (int j = 0; j < DP / 32; ++j) col[j][0] += by, col[j][1] += by;
     }
     __device__ __forceinline__ uint4 rows(uint32_t at, int s) const {
         return __builtin_bit_cast(uint4, *reinterpret_cast<__attribute__((address_space(3))) const u32x4*>(at + row[s]));
@@ -269,24 +276,33 @@ __device__ __forceinline__ void win_arrived(uint4 (&f)[N]) {
 }
 __device__ __forceinline__ void win_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// The running softmax of a lane's query over more keys (two lanes hold one query's
-// scores, half each): `top` the score that is subtracted, `sub` = top scale2 +
-// shift as it is rounded; l the sum.  top follows the largest score only where
-// that passes it by 2^kWinLag, so that the sums are hardly ever scaled anew.
+// The larger, the sum, of what lanes l and l + 32 hold.
+__device__ __forceinline__ float half_max(float v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+
+// The running softmax of a lane's query over blocks of 32 keys (two lanes hold one
+// query's scores, half each): `top` the score that is subtracted, `sub` = top
+// scale2 + shift as it is rounded; l the sum.  top follows the largest score only
+// where that passes it by 2^kWinLag, so that the sums are hardly ever scaled anew.
 struct WinState {
     float top, sub, l;
 };
 constexpr float kWinLag = 8.0f;
-// P of KB blocks of 32 scores in place; anew(f): what was summed before is scaled.
-template <int KB, bool BF, class Anew>
-__device__ __forceinline__ void win_softmax(floatx16 (&s)[KB], WinState& st, float scale2, Anew anew) {
-    float mx = s[0][0];
+// The exponent that the block's scores take off; anew(f): what was summed before
+// is scaled.  NaN among them passes by: it ends in the sum.
+template <bool BF, class Anew>
+__device__ __forceinline__ float win_top(floatx16& s, WinState& st, float scale2, Anew anew) {
+    float mx = s[0];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[kb][v]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    if (__any((mx - st.top) * scale2 > kWinLag)) {  // NaN (-inf - -inf): nothing seen yet, nothing to scale
+    for (int v = 1; v < 16; ++v) mx = fmaxf(mx, s[v]);
+    mx = half_max(mx);
+    if (__any((mx - st.top) * scale2 > kWinLag)) {  // -inf - -inf: nothing seen yet, nothing to scale
         const float top = fmaxf(st.top, mx);
         const float base = top == -__builtin_inff() ? 0.0f : top;
         const float sub = fmaf(base, scale2, win_shift<BF>());
@@ -297,22 +313,25 @@ __device__ __forceinline__ void win_softmax(floatx16 (&s)[KB], WinState& st, flo
         st.l *= f;
         anew(f);
     }
-    const float base = st.top == -__builtin_inff() ? 0.0f : st.top;  // nothing seen yet: exp2(-inf) is 0
+    // nothing seen yet: exp2(-inf) is 0
+    const float base = st.top == -__builtin_inff() ? 0.0f : st.top;
     // scores far from 0: the rounding of `sub` would carry probabilities out of
     // fp16's range, so the largest is subtracted first
     if (__any(fabsf(base) * scale2 > 0x1p20f)) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) s[kb][v] = __builtin_amdgcn_exp2f(fmaf(s[kb][v] - base, scale2, -win_shift<BF>()));
-    } else {
-        const float sub = st.top == -__builtin_inff() ? 0.0f : st.sub;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) s[kb][v] = __builtin_amdgcn_exp2f(fmaf(s[kb][v], scale2, -sub));
+        for (int v = 0; v < 16; ++v) s[v] -= base;
+        return win_shift<BF>();
     }
+    return st.top == -__builtin_inff() ? 0.0f : st.sub;
 }
+// P of scores LO .. HI - 1
+__device__ __forceinline__ void win_exp(floatx16& s, int lo, int hi, float scale2, float sub) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v)
+        if (v >= lo && v < hi) s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], scale2, -sub));
+}
+// Where the 16 exponentials of a block stand among N products, the first `from` without.
+constexpr int win_piece(int x, int from, int n) { return x < from ? 0 : x >= n ? 16 : 16 * (x - from) / (n - from); }
 
 // Unit of a launch over `groups` x `tiles`: (group, tile, part), the parts of the
 // far ranges first, or the long tiles.
@@ -402,10 +421,10 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
     RowLoads<DP, T, 4> lk, lv;
     lk.init(a.ks[1], a.D, wave, lane);
     lv.init(a.vs[1], a.D, wave, lane);
-    Frags<DP> at;
-    at.init(lane);
     const char *kbase = a.k + p.b * a.ks[0] + p.kv * a.ks[2], *vbase = a.v + p.b * a.vs[0] + p.kv * a.vs[2];
     const uint32_t lds = lds_addr(smem);
+    Frags<DP> at;
+    at.init(lds, lane);
     auto issue = [&](int s) {
         const int first = tiles.at(s) * T;
         const uint32_t to = lds + (s & 1) * 2 * TILE;
@@ -421,41 +440,61 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
     if (tiles.count) issue(0);
     for (int t = 0; t < tiles.count; ++t) {
         win_sync();
+        if (t) at.move(t & 1 ? 2 * TILE : -2 * TILE);
         if (t + 1 < tiles.count) issue(t + 1);
         const int k0 = tiles.at(t) * T;
         const int seen = last < p.mine ? 0 : win_class(a, p.mine, last, k0, k0 + T - 1);
         if (!seen) continue;
-        const uint32_t kt = lds + (t & 1) * 2 * TILE, vt = kt + TILE;
         constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = DP > 96 ? 8 : 6;
         auto read = [&](int e) WIN_INLINE {
-            if (e < 2 * NS) return at.rows(kt + e / NS * 32 * RB, e % NS);
-            return at.cols(vt + (e - 2 * NS) / NJ * 16 * RB, (e - 2 * NS) % NJ);
+            if (e < 2 * NS) return at.rows(e / NS * 32 * RB, e % NS);
+            return at.cols(TILE + (e - 2 * NS) / NJ * 16 * RB, (e - 2 * NS) % NJ);
+        };
+        auto hide = [&](floatx16& s, int kb) WIN_INLINE {
+            if (seen == 1 || k0 + T > p.n) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
+                    s[v] = in ? s[v] : -__builtin_inff();
+                }
+            }
+        };
+        auto anew = [&](float f) WIN_INLINE {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[j][v] *= f;
         };
         uint4 pr;
         floatx16 s[2];
         s[0] = s[1] = floatx16{0};
+        float take = 0.0f;
+        // The products of one block and the other's softmax side by side: the second
+        // block's scores with the first's exponentials, the first's P V with the
+        // second's.
         win_stream<2 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
-            if (e < 2 * NS) {
-                s[e / NS] = win_mma<BF>(f, q[e % NS], s[e / NS]);
-                if (e < 2 * NS - 1) return;
-                if (seen == 1 || k0 + T > p.n) {
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) {
-                            const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
-                            s[kb][v] = in ? s[kb][v] : -__builtin_inff();
-                        }
-                }
-                win_softmax<2, BF>(s, st, a.scale2, [&](float f) {
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) o[j][v] *= f;
-                });
+            if (e < NS) {
+                s[0] = win_mma<BF>(f, q[e], s[0]);
                 return;
             }
-            const int u = (e - 2 * NS) / NJ, j = (e - 2 * NS) % NJ;
+            if (e < 2 * NS) {
+                const int x = e - NS;
+                s[1] = win_mma<BF>(f, q[x], s[1]);
+                if (x == 1) {
+                    hide(s[0], 0);
+                    take = win_top<BF>(s[0], st, a.scale2, anew);
+                }
+                constexpr int from = NS > 2 ? 2 : 1;
+                win_exp(s[0], win_piece(x, from, NS), win_piece(x + 1, from, NS), a.scale2, take);
+                return;
+            }
+            const int y = e - 2 * NS, u = y / NJ, j = y % NJ;
+            if (y == NJ)  // what is left of the first block is scaled with the rest
+                take = win_top<BF>(s[1], st, a.scale2, [&](float f_) WIN_INLINE {
+                    anew(f_);
+#pragma unroll
+                    for (int v = 8; v < 16; ++v) s[0][v] *= f_;
+                });
             if (j == 0) {
                 pr = win_pack8<BF>(s[u >> 1], u & 1);
                 // the sum of the rounded probabilities: their rounding errors then
@@ -463,9 +502,11 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
                 st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
             }
             o[j] = win_mma<BF>(f, pr, o[j]);
+            if (y == 0) hide(s[1], 1);
+            if (u == 1 || u == 2) win_exp(s[1], 8 * (y - NJ) / NJ, 8 * (y + 1 - NJ) / NJ, a.scale2, take);
         });
     }
-    const float l = st.l + __shfl_xor(st.l, 32, 64);
+    const float l = half_sum(st.l);
     const bool any = l != 0.0f && i < p.n;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
         const int64_t row = (((int64_t)p.b * a.far.rows + i) * a.H + p.h) * (a.far.parts + 1) + p.unit.part;
@@ -493,7 +534,7 @@ __device__ __forceinline__ void win_scale_ds(floatx16& ds, float& c, floatx16 (&
         float mx = 0.0f;
 #pragma unroll
         for (int v = 0; v < 16; ++v) mx = fmaxf(mx, fabsf(ds[v]));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        mx = half_max(mx);
         if (__any(mx * c > 0x1p15f)) {
             const float to = mx * c > 0x1p15f ? win_lower(c, mx) : c, f = to / c;
             c = to;
@@ -527,7 +568,7 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
         win_row<DP>(out, a.o + p.b * a.os[0] + p.h * a.os[2], i * a.os[1], i < p.n, a.D, g);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) delta = win_dot8<BF>(go[s], out[s], delta);
-        delta += __shfl_xor(delta, 32, 64);
+        delta = half_sum(delta);
     }
     if (g == 0 && i < a.NP && !p.unit.part) a.delta[row] = delta;
     float stat = i < a.NP ? a.stat[row] : -__builtin_inff();
@@ -536,10 +577,10 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
     RowLoads<DP, T, 4> lk, lv;
     lk.init(a.ks[1], a.D, wave, lane);
     lv.init(a.vs[1], a.D, wave, lane);
-    Frags<DP> at;
-    at.init(lane);
     const char *kbase = a.k + p.b * a.ks[0] + p.kv * a.ks[2], *vbase = a.v + p.b * a.vs[0] + p.kv * a.vs[2];
     const uint32_t lds = lds_addr(smem);
+    Frags<DP> at;
+    at.init(lds, lane);
     auto issue = [&](int s) {
         const int first = tiles.at(s) * T;
         const uint32_t to = lds + (s & 1) * 2 * TILE;
@@ -557,46 +598,51 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
     if (tiles.count) issue(0);
     for (int t = 0; t < tiles.count; ++t) {
         win_sync();
+        if (t) at.move(t & 1 ? 2 * TILE : -2 * TILE);
         if (t + 1 < tiles.count) issue(t + 1);
         const int k0 = tiles.at(t) * T;
         const int seen = last < p.mine ? 0 : win_class(a, p.mine, last, k0, k0 + T - 1);
         if (!seen) continue;
         const bool some = seen == 1 || k0 + T > p.n;
         constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = 4;
+        // the scores and dP of one block, then the other's, then both blocks' dQ
+        auto read = [&](int e) WIN_INLINE {
+            if (e < 4 * NS) return at.rows((e / NS & 1) * TILE + e / (2 * NS) * 32 * RB, e % NS);
+            return at.cols((e - 4 * NS) / NJ * 16 * RB, (e - 4 * NS) % NJ);
+        };
+        floatx16 s[2], dp = floatx16{0};
+        s[0] = s[1] = floatx16{0};
+        uint4 ds;
+        auto finish = [&](int kb) WIN_INLINE {  // dS from P and dP
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const uint32_t kt = lds + (t & 1) * 2 * TILE + kb * 32 * RB, vt = kt + TILE;
-            auto read = [&](int e) WIN_INLINE {
-                if (e < 2 * NS) return at.rows(e < NS ? kt : vt, e % NS);
-                return at.cols(kt + (e - 2 * NS) / NJ * 16 * RB, (e - 2 * NS) % NJ);
-            };
-            uint4 ds;
-            floatx16 s = floatx16{0}, dp = floatx16{0};
-            win_stream<2 * NS + 2 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
-                if (e < NS) {
-                    s = win_mma<BF>(f, q[e], s);
-                    return;
+            for (int v = 0; v < 16; ++v) s[kb][v] *= dp[v] - delta;
+            if (some) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
+                    s[kb][v] = in ? s[kb][v] : 0.0f;
                 }
-                if (e < 2 * NS) {
-                    dp = win_mma<BF>(f, go[e - NS], dp);
-                    if (e < 2 * NS - 1) return;
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale2, stat)) * (dp[v] - delta);
-                    if (some) {
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) {
-                            const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
-                            s[v] = in ? s[v] : 0.0f;
-                        }
-                    }
-                    win_scale_ds<DP, BF>(s, c, o);
-                    return;
+            }
+            win_scale_ds<DP, BF>(s[kb], c, o);
+            dp = floatx16{0};
+        };
+        win_stream<4 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
+            const int kb = e / (2 * NS), x = e % NS;
+            if (e < 4 * NS) {
+                if (e / NS & 1) {
+                    dp = win_mma<BF>(f, go[x], dp);
+                    win_exp(s[kb], win_piece(x, 1, NS), win_piece(x + 1, 1, NS), a.scale2, -stat);
+                } else {
+                    s[kb] = win_mma<BF>(f, q[x], s[kb]);
+                    if (kb && x == 0) finish(0);
                 }
-                const int u = (e - 2 * NS) / NJ, j = (e - 2 * NS) % NJ;
-                if (j == 0) ds = win_pack8<BF>(s, u);
-                o[j] = win_mma<BF>(f, ds, o[j]);
-            });
-        }
+                return;
+            }
+            const int y = e - 4 * NS, u = y / NJ, j = y % NJ;
+            if (y == (BF ? 1 : 2 * NJ)) finish(1);  // fp16: it may scale what was summed, so behind the first's
+            if (j == 0) ds = win_pack8<BF>(s[u >> 1], u & 1);
+            o[j] = win_mma<BF>(f, ds, o[j]);
+        });
     }
     const float f = (BF ? 1.0f : 0x1p-15f) / c;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
@@ -625,10 +671,14 @@ template <int E>
 __device__ __forceinline__ float win_lane(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + E, 0xf, 0xf, true));
 }
-// P and dS of a lane's key and 16 queries, whose statistics lie in 16 lanes
+// P, and dP - rowsum(dO O), of a lane's key and 16 queries, whose statistics lie in 16 lanes
 template <int... E>
-__device__ __forceinline__ void win_probs(std::integer_sequence<int, E...>, floatx16& s, floatx16& dp, float scale2, float stat, float delta) {
-    ((s[E] = __builtin_amdgcn_exp2f(s[E] * scale2 + win_lane<E>(stat)), dp[E] = s[E] * (dp[E] - win_lane<E>(delta))), ...);
+__device__ __forceinline__ void win_probs(std::integer_sequence<int, E...>, floatx16& s, float scale2, float stat) {
+    ((s[E] = __builtin_amdgcn_exp2f(s[E] * scale2 + win_lane<E>(stat))), ...);
+}
+template <int... E>
+__device__ __forceinline__ void win_diff(std::integer_sequence<int, E...>, floatx16& dp, float delta) {
+    ((dp[E] -= win_lane<E>(delta)), ...);
 }
 template <int DP, bool BF>
 __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
@@ -658,9 +708,9 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
     RowLoads<DP, kWinStep, 4> lq, lo_;
     lq.init(a.qs[1], a.D, wave, lane);
     lo_.init(a.gos[1], a.D, wave, lane);
-    Frags<DP> at;
-    at.init(lane);
     const uint32_t lds = lds_addr(smem);
+    Frags<DP> at;
+    at.init(lds + V + 32 * half * RB, lane);
     int head = 0, qt = 0;  // of the step that is issued next
     float stat, delta, stat_next = 0.0f, delta_next = 0.0f;
     auto issue = [&](int s) {
@@ -690,20 +740,20 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
         win_sync();
         asm volatile("" : "+v"(stat_next), "+v"(delta_next));
         stat = stat_next, delta = delta_next;
+        if (t) at.move(t & 1 ? STAGE : -STAGE);
         if (t + 1 < steps) issue(t + 1);
         const int q0 = q.at(ct) * kWinStep + 32 * half, qlast = (q0 + 31 < n - 1 ? q0 + 31 : n - 1);
         if (++ct == q.count) ct = 0;
         const int seen = qlast < q0 || klast < mine ? 0 : win_class(a, q0, qlast, mine, klast);
         if (!seen) continue;
-        const uint32_t qtile = lds + V + (t & 1) * STAGE + 32 * half * RB, otile = qtile + kWinStep * RB;
-        const uint32_t vt = lds + 32 * block * RB;
-        constexpr int NS = DP / 16, NJ = DP / 32, PD = 4;
+        constexpr int NS = DP / 16, NJ = DP / 32, PD = 4, OUT = kWinStep * RB;
+        const uint32_t vt = 32 * (block - half) * RB - V - (t & 1) * STAGE;  // V's rows from Q's
         // Q; dO and V in turn; dO and Q transposed
         auto read = [&](int e) WIN_INLINE {
-            if (e < NS) return at.rows(qtile, e);
-            if (e < 3 * NS) return at.rows((e - NS) & 1 ? vt : otile, (e - NS) / 2);
+            if (e < NS) return at.rows(0, e);
+            if (e < 3 * NS) return at.rows((e - NS) & 1 ? vt : OUT, (e - NS) / 2);
             const int x = e - 3 * NS;
-            return at.cols((x < 2 * NJ ? otile : qtile) + x / NJ % 2 * 16 * RB, x % NJ);
+            return at.cols((x < 2 * NJ ? OUT : 0) + x / NJ % 2 * 16 * RB, x % NJ);
         };
         uint4 pr, was;
         floatx16 s = floatx16{0}, dp = floatx16{0};
@@ -713,25 +763,41 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
                 return;
             }
             if (e < 3 * NS) {
-                if ((e - NS) & 1) dp = win_mma<BF>(was, f, dp);
-                else was = f;
-                if (e < 3 * NS - 1) return;
-                win_probs(std::make_integer_sequence<int, 16>(), s, dp, a.scale2, stat, delta);
-                if (seen == 1) {
+                if (!((e - NS) & 1)) {
+                    was = f;
+                    return;
+                }
+                dp = win_mma<BF>(was, f, dp);
+                if (e == 3 * NS - 1) {
+                    win_probs(std::make_integer_sequence<int, 16>(), s, a.scale2, stat);
+                    if (seen == 1) {
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) {
-                        const bool in = mask(q0 + acc_row(v, g), key);
-                        s[v] = in ? s[v] : 0.0f;
-                        dp[v] = in ? dp[v] : 0.0f;
+                        for (int v = 0; v < 16; ++v) {
+                            const bool in = mask(q0 + acc_row(v, g), key);
+                            s[v] = in ? s[v] : 0.0f;
+                        }
                     }
                 }
                 return;
             }
             const int x = e - 3 * NS, j = x % NJ;
-            if (x == 2 * NJ) win_scale_ds<DP, BF>(dp, c, ok);
-            if (j == 0) pr = win_pack8<BF>(x < 2 * NJ ? s : dp, x / NJ % 2);
-            if (x < 2 * NJ) ov[j] = win_mma<BF>(f, pr, ov[j]);
-            else ok[j] = win_mma<BF>(f, pr, ok[j]);
+            if (x < 2 * NJ) {
+                if (j == 0) pr = win_pack8<BF>(s, x / NJ);
+                ov[j] = win_mma<BF>(f, pr, ov[j]);
+                if (x == 1) {
+                    win_diff(std::make_integer_sequence<int, 16>(), dp, delta);
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) dp[v] *= s[v];
+                    if (seen == 1) {
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) dp[v] = s[v] == 0.0f ? 0.0f : dp[v];
+                    }
+                }
+            } else {
+                if (x == 2 * NJ) win_scale_ds<DP, BF>(dp, c, ok);
+                if (j == 0) pr = win_pack8<BF>(dp, x / NJ % 2);
+                ok[j] = win_mma<BF>(f, pr, ok[j]);
+            }
         });
     }
     // the fellow's sums through LDS, one tensor after the other
@@ -817,7 +883,7 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
         }
     };
     Frags<DP> at;
-    at.init(lane);
+    at.init(lds, lane);
     WinState st = {-__builtin_inff(), -__builtin_inff(), 0.0f};
     floatx16 o[DP / 32];
 #pragma unroll
@@ -833,36 +899,47 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
-        const uint32_t kt = lds + buf * 2 * TILE, vt = kt + TILE;
         const int j0 = (s < first ? s : t0 + s - first) * T;
-        floatx16 sc[1] = {floatx16{0}};
+        const uint32_t bt = buf * 2 * TILE;
+        constexpr int NS = DP / 16, NJ = DP / 32, PD = 8;
+        auto read = [&](int e) WIN_INLINE {
+            if (e < NS) return at.rows(bt, e);
+            return at.cols(bt + TILE + (e - NS) / NJ * 16 * RB, (e - NS) % NJ);
+        };
+        floatx16 sc = floatx16{0};
+        uint4 pr;
+        win_stream<NS + 2 * NJ, PD < NS + 2 * NJ ? PD : NS + 2 * NJ>(read, [&](int e, uint4 f) WIN_INLINE {
+            if (e < NS) {
+                sc = win_mma<BF>(f, q[e], sc);
+                if (e < NS - 1) return;
+                // all of it seen by every row, or not
+                if (j0 + T > len - a.N + 1 || (len - 1 - j0 >= a.window && j0 + T > sinks)) {
 #pragma unroll
-        for (int e = 0; e < DP / 16; ++e) sc[0] = win_mma<BF>(at.rows(kt, e), q[e], sc[0]);
-        // all of it seen by every row, or not
-        if (j0 + T > len - a.N + 1 || (len - 1 - j0 >= a.window && j0 + T > sinks)) {
+                    for (int v = 0; v < 16; ++v) {
+                        const bool in = mask(i, j0 + acc_row(v, g));
+                        sc[v] = in ? sc[v] : -__builtin_inff();
+                    }
+                }
+                const float take = win_top<BF>(sc, st, a.scale2, [&](float f_) WIN_INLINE {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const bool in = mask(i, j0 + acc_row(v, g));
-                sc[0][v] = in ? sc[0][v] : -__builtin_inff();
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) o[j][v] *= f_;
+                });
+                win_exp(sc, 0, 16, a.scale2, take);
+                return;
             }
-        }
-        win_softmax<1, BF>(sc, st, a.scale2, [&](float f) {
-#pragma unroll
-            for (int j = 0; j < DP / 32; ++j)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) o[j][v] *= f;
+            const int u = (e - NS) / NJ, j = (e - NS) % NJ;
+            if (j == 0) {
+                pr = win_pack8<BF>(sc, u);
+                st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
+            }
+            o[j] = win_mma<BF>(f, pr, o[j]);
         });
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const uint4 pr = win_pack8<BF>(sc[0], e);
-            st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
-#pragma unroll
-            for (int j = 0; j < DP / 32; ++j) o[j] = win_mma<BF>(at.cols(vt + e * 16 * RB, j), pr, o[j]);
-        }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this buffer is free for the next load
     }
     // the four waves' sums, in their order
-    st.l += __shfl_xor(st.l, 32, 64);
+    st.l = half_sum(st.l);
     __syncthreads();
     constexpr int LD = DP + 4;
     float* sums = reinterpret_cast<float*>(smem);  // [wave][row][LD]
