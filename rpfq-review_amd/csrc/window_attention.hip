@@ -8,6 +8,7 @@
 //   dV = P^T dO,  dS = P (dO V^T - rowsum(dO O)),  dQ = scale dS K,  dK = scale dS^T Q.
 #include "tile_gemm.h"
 
+#include <type_traits>
 #include <utility>
 
 namespace rpfq {
@@ -267,6 +268,9 @@ __device__ __forceinline__ void win_row(uint4 (&f)[DP / 16], const char* base, i
     }
 }
 
+// Keeps a rare branch one: without it the compiler computes both sides, the masks
+// of every tile among them.
+__device__ __forceinline__ void win_rare() { asm volatile(""); }
 // The compiler's wait for a load stands here, and not at its first use: in a loop
 // that would be a wait for the DMA of the next tile too, which it does not count.
 template <int N>
@@ -275,6 +279,29 @@ __device__ __forceinline__ void win_arrived(uint4 (&f)[N]) {
     for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s].x), "+v"(f[s].y), "+v"(f[s].z), "+v"(f[s].w));
 }
 __device__ __forceinline__ void win_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// c + a b where some of a are not finite: these count where their factor is not 0.
+template <bool BF>
+__device__ __forceinline__ floatx16 win_mma_some(uint4 a, uint4 b, floatx16 c) {
+    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u, ONE = BF ? 0x3f80u : 0x3c00u;
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+    uint32_t fin[4], odd[4], some[4], any = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const uint32_t lo = (x[t] & E) == E ? 0xffffu : 0u, hi = (x[t] & E << 16) == E << 16 ? 0xffff0000u : 0u;
+        fin[t] = x[t] & ~(lo | hi);
+        odd[t] = (lo | hi) & (ONE | ONE << 16);
+        some[t] = (y[t] & 0x7fffu ? ONE : 0u) | (y[t] & 0x7fff0000u ? ONE << 16 : 0u);
+        any |= lo | hi;
+    }
+    if (!__any(any != 0)) return win_mma<BF>(a, b, c);
+    const floatx16 n = win_mma<BF>(make_uint4(odd[0], odd[1], odd[2], odd[3]), make_uint4(some[0], some[1], some[2], some[3]), floatx16{0});
+    const floatx16 all = win_mma<BF>(a, b, floatx16{0});
+    c = win_mma<BF>(make_uint4(fin[0], fin[1], fin[2], fin[3]), b, c);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) c[v] += n[v] != 0.0f ? all[v] : 0.0f;
+    return c;
+}
 
 // The larger, the sum, of what lanes l and l + 32 hold.
 __device__ __forceinline__ float half_max(float v) {
@@ -295,8 +322,10 @@ struct WinState {
 };
 constexpr float kWinLag = 8.0f;
 // The exponent that the block's scores take off; anew(f): what was summed before
-// is scaled.  NaN among them passes by: it ends in the sum.
-template <bool BF, class Anew>
+// is scaled.  NaN among them passes by: it ends in the sum.  FAR: scores past
+// 2^20, where the rounding of `sub` would carry probabilities out of fp16's range,
+// have the largest subtracted first.
+template <bool BF, bool FAR, class Anew>
 __device__ __forceinline__ float win_top(floatx16& s, WinState& st, float scale2, Anew anew) {
     float mx = s[0];
 #pragma unroll
@@ -306,23 +335,20 @@ __device__ __forceinline__ float win_top(floatx16& s, WinState& st, float scale2
         const float top = fmaxf(st.top, mx);
         const float base = top == -__builtin_inff() ? 0.0f : top;
         const float sub = fmaf(base, scale2, win_shift<BF>());
-        const bool far = fabsf(base) * scale2 > 0x1p20f;
-        const float f = __builtin_amdgcn_exp2f(far ? (st.top - base) * scale2 : st.sub - sub);
+        const float f = __builtin_amdgcn_exp2f(FAR ? (st.top - base) * scale2 : st.sub - sub);
         st.top = top;
         st.sub = top == -__builtin_inff() ? -__builtin_inff() : sub;
         st.l *= f;
         anew(f);
     }
-    // nothing seen yet: exp2(-inf) is 0
-    const float base = st.top == -__builtin_inff() ? 0.0f : st.top;
-    // scores far from 0: the rounding of `sub` would carry probabilities out of
-    // fp16's range, so the largest is subtracted first
-    if (__any(fabsf(base) * scale2 > 0x1p20f)) {
+    const bool none = st.top == -__builtin_inff();  // nothing seen yet: exp2(-inf) is 0
+    if (FAR) {
+        const float base = none ? 0.0f : st.top;
 #pragma unroll
         for (int v = 0; v < 16; ++v) s[v] -= base;
         return win_shift<BF>();
     }
-    return st.top == -__builtin_inff() ? 0.0f : st.sub;
+    return none ? 0.0f : st.sub;
 }
 // P of scores LO .. HI - 1
 __device__ __forceinline__ void win_exp(floatx16& s, int lo, int hi, float scale2, float sub) {
@@ -408,7 +434,7 @@ __device__ __forceinline__ void win_part(float* dst, const floatx16 (&o)[DP / 32
 // already the operand of O^T = V^T P^T.  K and V tiles of 64 keys go to LDS by
 // DMA, the next one while this one is used.
 template <int DP, bool BF>
-__global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
+__global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_forward_kernel(WinArgs a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int T = 64, TILE = T * Rows<DP>::RB;  // K, then V; twice
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
@@ -432,11 +458,14 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
         lv.issue(vbase, a.vs[1], a.D, first, p.n, to + TILE, wave);
     };
     const WinMask mask(a, p.n);
-    WinState st = {-__builtin_inff(), -__builtin_inff(), 0.0f};
+    WinState st;
     floatx16 o[DP / 32];
+    win_arrived(q);
+    auto run = [&](auto careful) WIN_INLINE {
+    constexpr bool FAR = decltype(careful)::value;
+    st = {-__builtin_inff(), -__builtin_inff(), 0.0f};
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
-    win_arrived(q);
     if (tiles.count) issue(0);
     for (int t = 0; t < tiles.count; ++t) {
         win_sync();
@@ -452,6 +481,7 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
         };
         auto hide = [&](floatx16& s, int kb) WIN_INLINE {
             if (seen == 1 || k0 + T > p.n) {
+                win_rare();
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
                     const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
@@ -482,7 +512,7 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
                 s[1] = win_mma<BF>(f, q[x], s[1]);
                 if (x == 1) {
                     hide(s[0], 0);
-                    take = win_top<BF>(s[0], st, a.scale2, anew);
+                    take = win_top<BF, FAR>(s[0], st, a.scale2, anew);
                 }
                 constexpr int from = NS > 2 ? 2 : 1;
                 win_exp(s[0], win_piece(x, from, NS), win_piece(x + 1, from, NS), a.scale2, take);
@@ -490,7 +520,7 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
             }
             const int y = e - 2 * NS, u = y / NJ, j = y % NJ;
             if (y == NJ)  // what is left of the first block is scaled with the rest
-                take = win_top<BF>(s[1], st, a.scale2, [&](float f_) WIN_INLINE {
+                take = win_top<BF, FAR>(s[1], st, a.scale2, [&](float f_) WIN_INLINE {
                     anew(f_);
 #pragma unroll
                     for (int v = 8; v < 16; ++v) s[0][v] *= f_;
@@ -501,11 +531,22 @@ __global__ void __launch_bounds__(256, 2) window_forward_kernel(WinArgs a) {
                 // weigh the values' distance to the output, not the values
                 st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
             }
-            o[j] = win_mma<BF>(f, pr, o[j]);
+            o[j] = FAR ? win_mma_some<BF>(f, pr, o[j]) : win_mma<BF>(f, pr, o[j]);
             if (y == 0) hide(s[1], 1);
             if (u == 1 || u == 2) win_exp(s[1], 8 * (y - NJ) / NJ, 8 * (y + 1 - NJ) / NJ, a.scale2, take);
         });
     }
+    if (tiles.count > 1 && !(tiles.count & 1)) at.move(-2 * TILE);  // to the first stage again
+    };
+    run(std::false_type());
+    // Scores past 2^20, or a value that is not finite (a product with a probability
+    // of 0 in its tile made it everyone's): once more, with care.
+    float odd = st.top * a.scale2 > 0x1p20f || (st.top != -__builtin_inff() && st.top * a.scale2 < -0x1p20f) ? 1.0f : st.l * 0.0f;
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) odd = fmaf(o[j][v], 0.0f, odd);
+    if (__builtin_expect(__syncthreads_or(!(odd == 0.0f)), 0)) run(std::true_type());
     const float l = half_sum(st.l);
     const bool any = l != 0.0f && i < p.n;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
@@ -617,6 +658,7 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) s[kb][v] *= dp[v] - delta;
             if (some) {
+                win_rare();
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
                     const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
@@ -771,6 +813,7 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
                 if (e == 3 * NS - 1) {
                     win_probs(std::make_integer_sequence<int, 16>(), s, a.scale2, stat);
                     if (seen == 1) {
+                        win_rare();
 #pragma unroll
                         for (int v = 0; v < 16; ++v) {
                             const bool in = mask(q0 + acc_row(v, g), key);
@@ -789,6 +832,7 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
 #pragma unroll
                     for (int v = 0; v < 16; ++v) dp[v] *= s[v];
                     if (seen == 1) {
+                        win_rare();
 #pragma unroll
                         for (int v = 0; v < 16; ++v) dp[v] = s[v] == 0.0f ? 0.0f : dp[v];
                     }
@@ -900,6 +944,8 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         const int j0 = (s < first ? s : t0 + s - first) * T;
+        // whether some row does not see all of it
+        const bool some = j0 + T > len - a.N + 1 || (len - 1 - j0 >= a.window && j0 + T > sinks);
         const uint32_t bt = buf * 2 * TILE;
         constexpr int NS = DP / 16, NJ = DP / 32, PD = 8;
         auto read = [&](int e) WIN_INLINE {
@@ -912,15 +958,15 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
             if (e < NS) {
                 sc = win_mma<BF>(f, q[e], sc);
                 if (e < NS - 1) return;
-                // all of it seen by every row, or not
-                if (j0 + T > len - a.N + 1 || (len - 1 - j0 >= a.window && j0 + T > sinks)) {
+                if (some) {
+                    win_rare();
 #pragma unroll
                     for (int v = 0; v < 16; ++v) {
                         const bool in = mask(i, j0 + acc_row(v, g));
                         sc[v] = in ? sc[v] : -__builtin_inff();
                     }
                 }
-                const float take = win_top<BF>(sc, st, a.scale2, [&](float f_) WIN_INLINE {
+                const float take = win_top<BF, true>(sc, st, a.scale2, [&](float f_) WIN_INLINE {
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -934,7 +980,12 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
                 pr = win_pack8<BF>(sc, u);
                 st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
             }
-            o[j] = win_mma<BF>(f, pr, o[j]);
+            if (some && a.N > 1) {
+                win_rare();
+                o[j] = win_mma_some<BF>(f, pr, o[j]);
+            } else {
+                o[j] = win_mma<BF>(f, pr, o[j]);
+            }
         });
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this buffer is free for the next load
     }

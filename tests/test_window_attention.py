@@ -324,6 +324,38 @@ def test_cached_matches_its_definition(b, t, m, heads, kv, d, window, sinks, len
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_values_that_are_not_finite_stay_where_they_are_seen(causal, dtype):
+    """Infinities and NaN among keys and values reach the queries that see them, and no other."""
+    from quant_models import ops
+
+    q, k, v, _ = _inputs(2, 200, 4, 2, 64, dtype, 21)
+    want = _want(q, k, v, 30, 2, causal, 0.125, None)
+    i = torch.arange(200, device=DEV)
+    seen = _seen(i[:, None], i[None], 30, 2, causal)
+    for t, at, what in ((v, 77, math.nan), (v, 130, math.inf), (k, 77, math.nan), (v, 199, -math.inf)):
+        one = t.clone()
+        one[0, at, 0, 5] = what
+        out = ops.window_attention(q, one if t is k else k, one if t is v else v, 30, 2, causal=causal)
+        hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+        hit[0, :, :2] = seen[:, at][:, None, None]
+        if t is v:
+            hit[..., :5] = hit[..., 6:] = False
+        assert not bool(out[hit].isfinite().any())
+        _check(torch.where(hit, 0, out), torch.where(hit, 0, want[0][0]), want[0][1])
+    # three new tokens: the last one's values are not the first ones'
+    lens = torch.tensor([200, 150], dtype=torch.int32, device=DEV)
+    last, worth = q[:, :3].contiguous(), _cache_want(q[:, :3], k, v, [200, 150], 30, 2, 0.125)
+    v[0, 199, 0, 5] = math.nan
+    out = ops.window_attention_cached(last, k, v, lens, 30, 2)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+    hit[0, 2, :2, 5] = True
+    assert bool(out[hit].isnan().all())
+    _check(torch.where(hit, 0, out), torch.where(hit, 0, worth[0]), worth[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_scores_far_from_zero(dtype):
     """Scores past 2^20, where an exponent's rounding would pass fp16's range."""
     from quant_models import ops
