@@ -27,28 +27,46 @@ struct Rows {
     }
 };
 
-// The loads of a tile of R rows by WAVES waves: row `row` of the tile from
-// base + row ld, rows past `end` bytes and chunks past D as zeros.
+// The loads of a tile of R rows by WAVES waves: rows of `ld` bytes, `left` of them
+// from the tile's first on; rows behind those and chunks past D as zeros.  The
+// scalar sums of an address are kept from tile to tile (they took a fifth of the
+// forward's step where each tile formed its own).
 template <int DP, int R, int WAVES>
 struct RowLoads {
     static constexpr int TOTAL = R / Rows<DP>::PER, LOADS = (TOTAL + WAVES - 1) / WAVES;
     uint32_t off[LOADS];
-    __device__ __forceinline__ void init(int64_t ld, int D, int wave, int lane) {
+    uint64_t at;
+    int ld, left, bytes;
+    __device__ __forceinline__ void init(int64_t row_bytes, int D, int wave, int lane) {
+        ld = (int)row_bytes;
+        bytes = 2 * D;
 #pragma unroll
         for (int p = 0; p < LOADS; ++p) {
             const int row = (wave + p * WAVES) * Rows<DP>::PER + lane / Rows<DP>::CH;
             const int c = (lane & (Rows<DP>::CH - 1)) ^ Rows<DP>::swz(row);
-            off[p] = 8 * c < D ? (uint32_t)(row * (int)ld + 16 * c) : kTileOut;
+            off[p] = 8 * c < D ? (uint32_t)(row * ld + 16 * c) : kTileOut;
         }
     }
-    // rows first .. of a tensor whose rows 0 .. n - 1 count
-    __device__ __forceinline__ void issue(const char* base, int64_t ld, int D, int first, int n, uint32_t lds, int wave) const {
-        intx4 rs = tile_rsrc(base + (int64_t)first * ld);
-        const int64_t end = (int64_t)(n - first - 1) * ld + 2 * D;
-        rs[2] = __builtin_amdgcn_readfirstlane(n <= first ? 0 : (int)(end > 0x7fffffff ? 0x7fffffff : end));
+    // to rows first .. of a tensor whose rows 0 .. n - 1 count
+    __device__ __forceinline__ void seek(const char* base, int first, int n) {
+        at = reinterpret_cast<uint64_t>(base) + (uint64_t)first * (uint32_t)ld;
+        left = n - first;
+    }
+    __device__ __forceinline__ void next() {
+        at += (uint32_t)(R * ld);
+        left -= R;
+    }
+    __device__ __forceinline__ void issue(uint32_t lds, int wave) const {
+        const int rows = left < R ? left : R;
+        const intx4 rs = {__builtin_amdgcn_readfirstlane((int)(uint32_t)at), __builtin_amdgcn_readfirstlane((int)((at >> 32) & 0xffff)),
+                          __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * ld + bytes : 0), 0x00027000};
 #pragma unroll
-        for (int p = 0; p < LOADS; ++p)
-            if (TOTAL % WAVES == 0 || wave + p * WAVES < TOTAL) dma_buffer(rs, off[p], lds + (wave + p * WAVES) * 1024);
+        for (int p = 0; p < LOADS; ++p) {
+            if (TOTAL % WAVES && wave + p * WAVES >= TOTAL) continue;
+            const uint32_t to = lds + (wave + p * WAVES) * 1024;
+            if (p == 0) dma_buffer(rs, off[p], to);  // waits for the resource's words, for all of them
+            else asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off[p]), "s"(rs) : "memory", "m0");
+        }
     }
 };
 
@@ -198,21 +216,41 @@ struct WinMask {
         return (j < n) & (near | (first & (d >= least)));
     }
 };
-// What queries q0 .. q1 see of keys k0 .. k1: 0 nothing, 1 some, 2 all.
-__device__ __forceinline__ int win_class(const WinArgs& a, int q0, int q1, int k0, int k1) {
-    if (a.causal) {
-        if (k0 > q1 || (q0 - k1 >= a.window && k0 >= a.sinks)) return 0;
-        return k1 <= q0 && (q1 - k0 < a.window || k1 < a.sinks) ? 2 : 1;
+// What a wave's own queries (keys) see of a run x0 .. x1 of keys (queries): 0
+// nothing, 1 some, 2 all.  Runs within [lo, hi] are seen in part, within [all_lo,
+// all_hi] whole, and those that begin in front of `early` may be.
+struct WinSpan {
+    int lo, hi, all_lo, all_hi, early;
+    // of queries q0 .. q1 (none: q1 < q0) of n
+    static __device__ __forceinline__ WinSpan keys(const WinArgs& a, int q0, int q1, int n) {
+        WinSpan s = {q0 - a.window + 1, a.causal ? q1 : q1 + a.window - 1, q1 - a.window + 1, a.causal ? q0 : q0 + a.window - 1, a.sinks};
+        if (!a.causal && q0 < a.sinks) s.lo = -0x7fffffff, s.hi = 0x7fffffff;
+        if (!a.causal && q1 < a.sinks) s.all_lo = 0, s.all_hi = n;
+        s.all_hi = s.all_hi < n - 1 ? s.all_hi : n - 1;
+        if (q1 < q0) s.lo = 0x7fffffff, s.all_hi = -1, s.early = 0;
+        return s;
     }
-    if ((q0 - k1 >= a.window || k0 - q1 >= a.window) && k0 >= a.sinks && q0 >= a.sinks) return 0;
-    return (q1 - k0 < a.window && k1 - q0 < a.window) || k1 < a.sinks || q1 < a.sinks ? 2 : 1;
-}
+    // of keys k0 .. k1; queries behind the end weigh nothing of themselves
+    static __device__ __forceinline__ WinSpan queries(const WinArgs& a, int k0, int k1) {
+        WinSpan s = {a.causal ? k0 : k0 - a.window + 1, k1 + a.window - 1, a.causal ? k1 : k1 - a.window + 1, k0 + a.window - 1, a.causal ? 0 : a.sinks};
+        if (k0 < a.sinks) s.hi = 0x7fffffff, s.lo = a.causal ? s.lo : -0x7fffffff;
+        if (k1 < a.sinks) s.all_hi = 0x7fffffff, s.all_lo = a.causal ? s.all_lo : -0x7fffffff;
+        if (k1 < k0) s.lo = 0x7fffffff, s.all_hi = -1, s.early = 0;
+        return s;
+    }
+    __device__ __forceinline__ int operator()(int x0, int x1) const {
+        if (x0 >= all_lo && x1 <= all_hi) return 2;
+        return (x0 <= hi && x1 >= lo) || x0 < early;
+    }
+};
 
 // The tiles of T keys that queries q0 .. q1 (< n) see: `first` tiles of the
 // sinks, then [t0, t1).
 struct WinTiles {
     int first, t0, count;
     __device__ __forceinline__ int at(int s) const { return s < first ? s : t0 + s - first; }
+    // whether step s is not the tile behind step s - 1's
+    __device__ __forceinline__ bool leap(int s) const { return s == first && first > 0 && t0 > first; }
 };
 template <int T>
 __device__ __forceinline__ WinTiles win_tiles(const WinArgs& a, int q0, int q1, int n) {
@@ -451,11 +489,17 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     const uint32_t lds = lds_addr(smem);
     Frags<DP> at;
     at.init(lds, lane);
-    auto issue = [&](int s) {
-        const int first = tiles.at(s) * T;
+    const WinSpan span = WinSpan::keys(a, p.mine, last, p.n);
+    auto issue = [&](int s) WIN_INLINE {
         const uint32_t to = lds + (s & 1) * 2 * TILE;
-        lk.issue(kbase, a.ks[1], a.D, first, p.n, to, wave);
-        lv.issue(vbase, a.vs[1], a.D, first, p.n, to + TILE, wave);
+        if (s == 0 || tiles.leap(s)) {
+            lk.seek(kbase, tiles.at(s) * T, p.n);
+            lv.seek(vbase, tiles.at(s) * T, p.n);
+        }
+        lk.issue(to, wave);
+        lv.issue(to + TILE, wave);
+        lk.next();
+        lv.next();
     };
     const WinMask mask(a, p.n);
     WinState st;
@@ -471,8 +515,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
         win_sync();
         if (t) at.move(t & 1 ? 2 * TILE : -2 * TILE);
         if (t + 1 < tiles.count) issue(t + 1);
-        const int k0 = tiles.at(t) * T;
-        const int seen = last < p.mine ? 0 : win_class(a, p.mine, last, k0, k0 + T - 1);
+        const int k0 = tiles.at(t) * T, seen = span(k0, k0 + T - 1);
         if (!seen) continue;
         constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = DP > 96 ? 8 : 6;
         auto read = [&](int e) WIN_INLINE {
@@ -480,7 +523,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
             return at.cols(TILE + (e - 2 * NS) / NJ * 16 * RB, (e - 2 * NS) % NJ);
         };
         auto hide = [&](floatx16& s, int kb) WIN_INLINE {
-            if (seen == 1 || k0 + T > p.n) {
+            if (seen == 1) {
                 win_rare();
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
@@ -622,11 +665,17 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
     const uint32_t lds = lds_addr(smem);
     Frags<DP> at;
     at.init(lds, lane);
-    auto issue = [&](int s) {
-        const int first = tiles.at(s) * T;
+    const WinSpan span = WinSpan::keys(a, p.mine, last, p.n);
+    auto issue = [&](int s) WIN_INLINE {
         const uint32_t to = lds + (s & 1) * 2 * TILE;
-        lk.issue(kbase, a.ks[1], a.D, first, p.n, to, wave);
-        lv.issue(vbase, a.vs[1], a.D, first, p.n, to + TILE, wave);
+        if (s == 0 || tiles.leap(s)) {
+            lk.seek(kbase, tiles.at(s) * T, p.n);
+            lv.seek(vbase, tiles.at(s) * T, p.n);
+        }
+        lk.issue(to, wave);
+        lv.issue(to + TILE, wave);
+        lk.next();
+        lv.next();
     };
     const WinMask mask(a, p.n);
     floatx16 o[DP / 32];
@@ -641,10 +690,8 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
         win_sync();
         if (t) at.move(t & 1 ? 2 * TILE : -2 * TILE);
         if (t + 1 < tiles.count) issue(t + 1);
-        const int k0 = tiles.at(t) * T;
-        const int seen = last < p.mine ? 0 : win_class(a, p.mine, last, k0, k0 + T - 1);
+        const int k0 = tiles.at(t) * T, seen = span(k0, k0 + T - 1);
         if (!seen) continue;
-        const bool some = seen == 1 || k0 + T > p.n;
         constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = 4;
         // the scores and dP of one block, then the other's, then both blocks' dQ
         auto read = [&](int e) WIN_INLINE {
@@ -657,7 +704,7 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
         auto finish = [&](int kb) WIN_INLINE {  // dS from P and dP
 #pragma unroll
             for (int v = 0; v < 16; ++v) s[kb][v] *= dp[v] - delta;
-            if (some) {
+            if (seen == 1) {
                 win_rare();
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
@@ -755,26 +802,37 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
     at.init(lds + V + 32 * half * RB, lane);
     int head = 0, qt = 0;  // of the step that is issued next
     float stat, delta, stat_next = 0.0f, delta_next = 0.0f;
-    auto issue = [&](int s) {
-        const int h = kv * group + head, first = q.at(qt) * kWinStep;
+    const char *qbase = a.q + b * a.qs[0] + kv * group * a.qs[2], *obase = a.go + b * a.gos[0] + kv * group * a.gos[2];
+    int64_t row = 0;
+    auto issue = [&](int s) WIN_INLINE {
         const uint32_t to = lds + V + (s & 1) * STAGE;
-        lq.issue(a.q + b * a.qs[0] + h * a.qs[2], a.qs[1], a.D, first, n, to, wave);
-        lo_.issue(a.go + b * a.gos[0] + h * a.gos[2], a.gos[1], a.D, first, n, to + kWinStep * RB, wave);
-        const int64_t row = ((int64_t)b * a.H + h) * a.NP + first + 32 * half + acc_row(lane & 15, g);
+        if (qt == 0 || q.leap(qt)) {
+            const int first = q.at(qt) * kWinStep;
+            lq.seek(qbase + head * a.qs[2], first, n);
+            lo_.seek(obase + head * a.gos[2], first, n);
+            row = ((int64_t)b * a.H + kv * group + head) * a.NP + first + 32 * half + acc_row(lane & 15, g);
+        }
+        lq.issue(to, wave);
+        lo_.issue(to + kWinStep * RB, wave);
+        lq.next();
+        lo_.next();
         stat_next = a.stat[row];
         delta_next = a.delta[row];
+        row += kWinStep;
         if (++qt == q.count) qt = 0, ++head;
     };
     if (steps) {
         RowLoads<DP, kWinKeys, 4> lv;
         lv.init(a.vs[1], a.D, wave, lane);
-        lv.issue(a.v + b * a.vs[0] + kv * a.vs[2], a.vs[1], a.D, k0, n, lds, wave);
+        lv.seek(a.v + b * a.vs[0] + kv * a.vs[2], k0, n);
+        lv.issue(lds, wave);
         issue(0);
     }
     floatx16 ok[DP / 32], ov[DP / 32];
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) ok[j] = ov[j] = floatx16{0};
     const WinMask mask(a, n);
+    const WinSpan span = WinSpan::queries(a, mine, klast);
     float c = BF ? 1.0f : 0x1p126f;
     int ct = 0;
     win_arrived(kf);
@@ -784,9 +842,8 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
         stat = stat_next, delta = delta_next;
         if (t) at.move(t & 1 ? STAGE : -STAGE);
         if (t + 1 < steps) issue(t + 1);
-        const int q0 = q.at(ct) * kWinStep + 32 * half, qlast = (q0 + 31 < n - 1 ? q0 + 31 : n - 1);
+        const int q0 = q.at(ct) * kWinStep + 32 * half, seen = q0 < n ? span(q0, q0 + 31) : 0;
         if (++ct == q.count) ct = 0;
-        const int seen = qlast < q0 || klast < mine ? 0 : win_class(a, q0, qlast, mine, klast);
         if (!seen) continue;
         constexpr int NS = DP / 16, NJ = DP / 32, PD = 4, OUT = kWinStep * RB;
         const uint32_t vt = 32 * (block - half) * RB - V - (t & 1) * STAGE;  // V's rows from Q's
