@@ -52,21 +52,25 @@ struct RowLoads {
         at = reinterpret_cast<uint64_t>(base) + (uint64_t)first * (uint32_t)ld;
         left = n - first;
     }
-    __device__ __forceinline__ void next() {
+    // the tile's resource, and on to the next tile (off: none of it is loaded)
+    intx4 rsrc;
+    __device__ __forceinline__ void next(bool on) {
+        const int rows = left < R ? left : R;
+        rsrc = (intx4){__builtin_amdgcn_readfirstlane((int)(uint32_t)at), __builtin_amdgcn_readfirstlane((int)((at >> 32) & 0xffff)),
+                       __builtin_amdgcn_readfirstlane(on && rows > 0 ? (rows - 1) * ld + bytes : 0), 0x00027000};
         at += (uint32_t)(R * ld);
         left -= R;
     }
+    // load p of the tile: the first waits for the resource's words, for all of them
+    __device__ __forceinline__ void load(int p, uint32_t lds, int wave) const {
+        if (TOTAL % WAVES && wave + p * WAVES >= TOTAL) return;
+        const uint32_t to = lds + (wave + p * WAVES) * 1024;
+        if (p == 0) dma_buffer(rsrc, off[0], to);
+        else asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off[p]), "s"(rsrc) : "memory", "m0");
+    }
     __device__ __forceinline__ void issue(uint32_t lds, int wave) const {
-        const int rows = left < R ? left : R;
-        const intx4 rs = {__builtin_amdgcn_readfirstlane((int)(uint32_t)at), __builtin_amdgcn_readfirstlane((int)((at >> 32) & 0xffff)),
-                          __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * ld + bytes : 0), 0x00027000};
 #pragma unroll
-        for (int p = 0; p < LOADS; ++p) {
-            if (TOTAL % WAVES && wave + p * WAVES >= TOTAL) continue;
-            const uint32_t to = lds + (wave + p * WAVES) * 1024;
-            if (p == 0) dma_buffer(rs, off[p], to);  // waits for the resource's words, for all of them
-            else asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off[p]), "s"(rs) : "memory", "m0");
-        }
+        for (int p = 0; p < LOADS; ++p) load(p, lds, wave);
     }
 };
 
@@ -74,40 +78,34 @@ struct RowLoads {
 // values of a row a step), and transposed (the row index is contracted, 16 rows
 // a step: lane half g holds rows 4 g .. + 3 and 8 + 4 g .. + 3, the order in
 // which a 32 x 32 result holds its rows).
+// A chunk's number stands in an address as bits, so that the swizzled address of
+// another chunk, or of 8 rows on, is one XOR away: `at` is a multiple of 256.
 template <int DP>
 struct Frags {
-    uint32_t row[DP / 16], col[DP / 32][2];
+    using T = Rows<DP>;
+    uint32_t row, col;
     __device__ __forceinline__ void init(uint32_t at, int lane) {
-        using T = Rows<DP>;
-        const int r = lane & 31, g = lane >> 5, i16 = lane & 15, hf = (lane >> 4) & 1;
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) row[s] = at + r * T::RB + (((2 * s + g) ^ T::swz(r)) * 16);
-        const int tr = 4 * g + (i16 >> 2);
-#pragma unroll
-        for (int j = 0; j < DP / 32; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                col[j][h] = at + (tr + 8 * h) * T::RB + (((4 * j + 2 * hf + ((i16 & 3) >> 1)) ^ T::swz(tr + 8 * h)) * 16) + (i16 & 1) * 8;
+        const int r = lane & 31, g = lane >> 5, i16 = lane & 15, hf = (lane >> 4) & 1, tr = 4 * g + (i16 >> 2);
+        row = at + r * T::RB + ((g ^ T::swz(r)) * 16);
+        col = at + tr * T::RB + (((2 * hf + ((i16 & 3) >> 1)) ^ T::swz(tr)) * 16) + (i16 & 1) * 8;
     }
-    // to the other stage: once a step, where a read's own sum would be one each
-    __device__ __forceinline__ void move(uint32_t by) {
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) row[s] += by;
-#pragma unroll
-        for (int j = 0; j < DP / 32; ++j) col[j][0] += by, col[j][1] += by;
-    }
+    // to the other stage
+    __device__ __forceinline__ void move(uint32_t by) { row += by, col += by; }
     __device__ __forceinline__ uint4 rows(uint32_t at, int s) const {
-        return __builtin_bit_cast(uint4, *reinterpret_cast<__attribute__((address_space(3))) const u32x4*>(at + row[s]));
+        return __builtin_bit_cast(uint4, *reinterpret_cast<__attribute__((address_space(3))) const u32x4*>((row ^ (uint32_t)s << 5) + at));
     }
     __device__ __forceinline__ uint4 cols(uint32_t at, int j) const {
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)(at + col[j][0]));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)(at + col[j][1]));
+        const uint32_t c = col ^ (uint32_t)j << 6;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)(c + at));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)((c ^ 32u) + (at + 8 * T::RB)));
         return __builtin_bit_cast(uint4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 };
 
 // A step's fragments in the order of their products, PD of them ahead: left to
-// itself the compiler reads each one right before its product and waits.
+// itself the compiler reads each one right before its product and waits.  The next
+// tile's loads stand between the products (in one run behind the barrier they
+// held up the forward's wave for 800 of 3,100 clocks a step).
 template <int N, int PD, class Read, class Use, int... E>
 __device__ __forceinline__ void win_each(uint4 (&ring)[PD], Read read, Use use, std::integer_sequence<int, E...>) {
     ((use(E, ring[E % PD]), E + PD < N ? (void)(ring[E % PD] = read(E + PD)) : (void)0, __builtin_amdgcn_sched_barrier(0)), ...);
@@ -316,6 +314,8 @@ __device__ __forceinline__ void win_arrived(uint4 (&f)[N]) {
 #pragma unroll
     for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s].x), "+v"(f[s].y), "+v"(f[s].z), "+v"(f[s].w));
 }
+// No load is on its way to LDS when its workgroup ends.
+__device__ __forceinline__ void win_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void win_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // c + a b where some of a are not finite: these count where their factor is not 0.
@@ -473,7 +473,7 @@ __device__ __forceinline__ void win_part(float* dst, const floatx16 (&o)[DP / 32
 // DMA, the next one while this one is used.
 template <int DP, bool BF>
 __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_forward_kernel(WinArgs a) {
-    extern __shared__ __align__(16) char smem[];
+    extern __shared__ __align__(256) char smem[];
     constexpr int T = 64, TILE = T * Rows<DP>::RB;  // K, then V; twice
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -490,16 +490,26 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     Frags<DP> at;
     at.init(lds, lane);
     const WinSpan span = WinSpan::keys(a, p.mine, last, p.n);
-    auto issue = [&](int s) WIN_INLINE {
-        const uint32_t to = lds + (s & 1) * 2 * TILE;
+    // the loads of step s: ready(s), then load 0 .. 2 LOADS - 1
+    constexpr int LOADS = RowLoads<DP, T, 4>::LOADS;
+    uint32_t to = lds;
+    auto ready = [&](int s) WIN_INLINE {
         if (s == 0 || tiles.leap(s)) {
             lk.seek(kbase, tiles.at(s) * T, p.n);
             lv.seek(vbase, tiles.at(s) * T, p.n);
         }
+        to = lds + (s & 1) * 2 * TILE;
+        lk.next(s < tiles.count);
+        lv.next(s < tiles.count);
+    };
+    auto load = [&](int x) WIN_INLINE {
+        if (x < LOADS) lk.load(x, to, wave);
+        else if (x < 2 * LOADS) lv.load(x - LOADS, to + TILE, wave);
+    };
+    auto issue = [&](int s) WIN_INLINE {
+        ready(s);
         lk.issue(to, wave);
         lv.issue(to + TILE, wave);
-        lk.next();
-        lv.next();
     };
     const WinMask mask(a, p.n);
     WinState st;
@@ -507,6 +517,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     win_arrived(q);
     auto run = [&](auto careful) WIN_INLINE {
     constexpr bool FAR = decltype(careful)::value;
+    win_sync();  // nothing of the run before is on its way to LDS
     st = {-__builtin_inff(), -__builtin_inff(), 0.0f};
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
@@ -514,9 +525,13 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     for (int t = 0; t < tiles.count; ++t) {
         win_sync();
         if (t) at.move(t & 1 ? 2 * TILE : -2 * TILE);
-        if (t + 1 < tiles.count) issue(t + 1);
+        ready(t + 1);
         const int k0 = tiles.at(t) * T, seen = span(k0, k0 + T - 1);
-        if (!seen) continue;
+        if (!seen) {
+            lk.issue(to, wave);
+            lv.issue(to + TILE, wave);
+            continue;
+        }
         constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = DP > 96 ? 8 : 6;
         auto read = [&](int e) WIN_INLINE {
             if (e < 2 * NS) return at.rows(e / NS * 32 * RB, e % NS);
@@ -546,6 +561,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
         // block's scores with the first's exponentials, the first's P V with the
         // second's.
         win_stream<2 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
+            load(e);
             if (e < NS) {
                 s[0] = win_mma<BF>(f, q[e], s[0]);
                 return;
@@ -590,6 +606,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
 #pragma unroll
         for (int v = 0; v < 16; ++v) odd = fmaf(o[j][v], 0.0f, odd);
     if (__builtin_expect(__syncthreads_or(!(odd == 0.0f)), 0)) run(std::true_type());
+    win_landed();
     const float l = half_sum(st.l);
     const bool any = l != 0.0f && i < p.n;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
@@ -636,7 +653,7 @@ __device__ __forceinline__ void win_scale_ds(floatx16& ds, float& c, floatx16 (&
 // in one lane's query, dQ^T = K^T dS^T.  Leaves rowsum(dO O) for the other.
 template <int DP, bool BF>
 __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
-    extern __shared__ __align__(16) char smem[];
+    extern __shared__ __align__(256) char smem[];
     constexpr int T = 64, TILE = T * Rows<DP>::RB;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -666,16 +683,26 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
     Frags<DP> at;
     at.init(lds, lane);
     const WinSpan span = WinSpan::keys(a, p.mine, last, p.n);
-    auto issue = [&](int s) WIN_INLINE {
-        const uint32_t to = lds + (s & 1) * 2 * TILE;
+    // the loads of step s: ready(s), then load 0 .. 2 LOADS - 1
+    constexpr int LOADS = RowLoads<DP, T, 4>::LOADS;
+    uint32_t to = lds;
+    auto ready = [&](int s) WIN_INLINE {
         if (s == 0 || tiles.leap(s)) {
             lk.seek(kbase, tiles.at(s) * T, p.n);
             lv.seek(vbase, tiles.at(s) * T, p.n);
         }
+        to = lds + (s & 1) * 2 * TILE;
+        lk.next(s < tiles.count);
+        lv.next(s < tiles.count);
+    };
+    auto load = [&](int x) WIN_INLINE {
+        if (x < LOADS) lk.load(x, to, wave);
+        else if (x < 2 * LOADS) lv.load(x - LOADS, to + TILE, wave);
+    };
+    auto issue = [&](int s) WIN_INLINE {
+        ready(s);
         lk.issue(to, wave);
         lv.issue(to + TILE, wave);
-        lk.next();
-        lv.next();
     };
     const WinMask mask(a, p.n);
     floatx16 o[DP / 32];
@@ -689,9 +716,13 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
     for (int t = 0; t < tiles.count; ++t) {
         win_sync();
         if (t) at.move(t & 1 ? 2 * TILE : -2 * TILE);
-        if (t + 1 < tiles.count) issue(t + 1);
+        ready(t + 1);
         const int k0 = tiles.at(t) * T, seen = span(k0, k0 + T - 1);
-        if (!seen) continue;
+        if (!seen) {
+            lk.issue(to, wave);
+            lv.issue(to + TILE, wave);
+            continue;
+        }
         constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = 4;
         // the scores and dP of one block, then the other's, then both blocks' dQ
         auto read = [&](int e) WIN_INLINE {
@@ -716,6 +747,7 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
             dp = floatx16{0};
         };
         win_stream<4 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
+            load(e);
             const int kb = e / (2 * NS), x = e % NS;
             if (e < 4 * NS) {
                 if (e / NS & 1) {
@@ -733,6 +765,7 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
             o[j] = win_mma<BF>(f, ds, o[j]);
         });
     }
+    win_landed();
     const float f = (BF ? 1.0f : 0x1p-15f) / c;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
         const int64_t slot = (((int64_t)p.b * a.far.rows + i) * a.H + p.h) * (a.far.parts + 1) + p.unit.part;
@@ -771,7 +804,7 @@ __device__ __forceinline__ void win_diff(std::integer_sequence<int, E...>, float
 }
 template <int DP, bool BF>
 __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
-    extern __shared__ __align__(16) char smem[];
+    extern __shared__ __align__(256) char smem[];
     constexpr int RB = Rows<DP>::RB, V = kWinKeys * RB, STAGE = 2 * kWinStep * RB;  // V, two stages of Q and dO
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), block = wave & 1, half = wave >> 1;
@@ -804,29 +837,41 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
     float stat, delta, stat_next = 0.0f, delta_next = 0.0f;
     const char *qbase = a.q + b * a.qs[0] + kv * group * a.qs[2], *obase = a.go + b * a.gos[0] + kv * group * a.gos[2];
     int64_t row = 0;
-    auto issue = [&](int s) WIN_INLINE {
-        const uint32_t to = lds + V + (s & 1) * STAGE;
-        if (qt == 0 || q.leap(qt)) {
+    constexpr int LOADS = RowLoads<DP, kWinStep, 4>::LOADS;
+    uint32_t to = lds;
+    auto ready = [&](int s) WIN_INLINE {
+        to = lds + V + (s & 1) * STAGE;
+        if (s < steps && (qt == 0 || q.leap(qt))) {
             const int first = q.at(qt) * kWinStep;
             lq.seek(qbase + head * a.qs[2], first, n);
             lo_.seek(obase + head * a.gos[2], first, n);
             row = ((int64_t)b * a.H + kv * group + head) * a.NP + first + 32 * half + acc_row(lane & 15, g);
         }
-        lq.issue(to, wave);
-        lo_.issue(to + kWinStep * RB, wave);
-        lq.next();
-        lo_.next();
-        stat_next = a.stat[row];
-        delta_next = a.delta[row];
+        lq.next(s < steps);
+        lo_.next(s < steps);
+        if (s < steps) {
+            stat_next = a.stat[row];
+            delta_next = a.delta[row];
+        }
         row += kWinStep;
         if (++qt == q.count) qt = 0, ++head;
+    };
+    auto load = [&](int x) WIN_INLINE {
+        if (x < LOADS) lq.load(x, to, wave);
+        else if (x < 2 * LOADS) lo_.load(x - LOADS, to + kWinStep * RB, wave);
+    };
+    auto issue = [&]() WIN_INLINE {
+        lq.issue(to, wave);
+        lo_.issue(to + kWinStep * RB, wave);
     };
     if (steps) {
         RowLoads<DP, kWinKeys, 4> lv;
         lv.init(a.vs[1], a.D, wave, lane);
         lv.seek(a.v + b * a.vs[0] + kv * a.vs[2], k0, n);
+        lv.next(true);
         lv.issue(lds, wave);
-        issue(0);
+        ready(0);
+        issue();
     }
     floatx16 ok[DP / 32], ov[DP / 32];
 #pragma unroll
@@ -841,9 +886,10 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
         asm volatile("" : "+v"(stat_next), "+v"(delta_next));
         stat = stat_next, delta = delta_next;
         if (t) at.move(t & 1 ? STAGE : -STAGE);
-        if (t + 1 < steps) issue(t + 1);
+        ready(t + 1);
         const int q0 = q.at(ct) * kWinStep + 32 * half, seen = q0 < n ? span(q0, q0 + 31) : 0;
         if (++ct == q.count) ct = 0;
+        if (!seen || DP > 96) issue();
         if (!seen) continue;
         constexpr int NS = DP / 16, NJ = DP / 32, PD = 4, OUT = kWinStep * RB;
         const uint32_t vt = 32 * (block - half) * RB - V - (t & 1) * STAGE;  // V's rows from Q's
@@ -857,6 +903,7 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
         uint4 pr, was;
         floatx16 s = floatx16{0}, dp = floatx16{0};
         win_stream<3 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
+            if (DP <= 96) load(e);
             if (e < NS) {
                 s = win_mma<BF>(f, kf[e], s);
                 return;
@@ -946,7 +993,7 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
 // waiting for each other.  Parts are joined by window_join_kernel.
 template <int DP, bool BF>
 __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
-    extern __shared__ __align__(16) char smem[];
+    extern __shared__ __align__(256) char smem[];
     constexpr int T = 32, RB = Rows<DP>::RB, TILE = T * RB, LOADS = T / Rows<DP>::PER;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = a.H / a.KV;
