@@ -34,30 +34,32 @@ struct Rows {
 template <int DP, int R, int WAVES>
 struct RowLoads {
     static constexpr int TOTAL = R / Rows<DP>::PER, LOADS = (TOTAL + WAVES - 1) / WAVES;
-    uint32_t off[LOADS];
+    static_assert(LOADS == 1 || WAVES * Rows<DP>::PER % 16 == 0, "a wave's loads lie alike");
+    uint32_t off;  // of load 0; load p is WAVES p PER rows on
     uint64_t at;
     int ld, left, bytes;
     __device__ __forceinline__ void init(int64_t row_bytes, int D, int wave, int lane) {
         ld = (int)row_bytes;
         bytes = 2 * D;
-#pragma unroll
-        for (int p = 0; p < LOADS; ++p) {
-            const int row = (wave + p * WAVES) * Rows<DP>::PER + lane / Rows<DP>::CH;
-            const int c = (lane & (Rows<DP>::CH - 1)) ^ Rows<DP>::swz(row);
-            off[p] = 8 * c < D ? (uint32_t)(row * ld + 16 * c) : kTileOut;
-        }
+        const int row = wave * Rows<DP>::PER + lane / Rows<DP>::CH, c = (lane & (Rows<DP>::CH - 1)) ^ Rows<DP>::swz(row);
+        off = 8 * c < D ? (uint32_t)(row * ld + 16 * c) : kTileOut;
     }
     // to rows first .. of a tensor whose rows 0 .. n - 1 count
     __device__ __forceinline__ void seek(const char* base, int first, int n) {
         at = reinterpret_cast<uint64_t>(base) + (uint64_t)first * (uint32_t)ld;
         left = n - first;
     }
-    // the tile's resource, and on to the next tile (off: none of it is loaded)
+    // the tile's resource (off: none of it is loaded)
     intx4 rsrc;
-    __device__ __forceinline__ void next(bool on) {
+    __device__ __forceinline__ void resource(bool on) {
         const int rows = left < R ? left : R;
         rsrc = (intx4){__builtin_amdgcn_readfirstlane((int)(uint32_t)at), __builtin_amdgcn_readfirstlane((int)((at >> 32) & 0xffff)),
                        __builtin_amdgcn_readfirstlane(on && rows > 0 ? (rows - 1) * ld + bytes : 0), 0x00027000};
+        asm volatile("" : "+v"(off));  // the loads' own sums stay in the loop: a register, not one each
+    }
+    // and on to the tile behind it
+    __device__ __forceinline__ void next(bool on) {
+        resource(on);
         at += (uint32_t)(R * ld);
         left -= R;
     }
@@ -65,8 +67,9 @@ struct RowLoads {
     __device__ __forceinline__ void load(int p, uint32_t lds, int wave) const {
         if (TOTAL % WAVES && wave + p * WAVES >= TOTAL) return;
         const uint32_t to = lds + (wave + p * WAVES) * 1024;
-        if (p == 0) dma_buffer(rsrc, off[0], to);
-        else asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off[p]), "s"(rsrc) : "memory", "m0");
+        const uint32_t from = off + (uint32_t)(p * WAVES * Rows<DP>::PER * ld);
+        if (p == 0) dma_buffer(rsrc, from, to);
+        else asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(from), "s"(rsrc) : "memory", "m0");
     }
     __device__ __forceinline__ void issue(uint32_t lds, int wave) const {
 #pragma unroll
@@ -200,20 +203,61 @@ __device__ __forceinline__ int win_length(const WinArgs& a, int b, int most) {
     const int n = a.lengths[b];
     return n < 0 ? 0 : n > most ? most : n;
 }
-// What a pair sees, without a branch: d = i - j within [-off, span - off), or a
-// sink with d >= least.
+// Keeps a rare branch one: without it the compiler computes both sides, the masks
+// of every tile among them.
+__device__ __forceinline__ void win_rare() { asm volatile(""); }
+// !seen, as a branch of its own: as the other side of the products' branch it
+// costs a copy of every sum a step.
+__device__ __forceinline__ bool win_unseen(int seen) {
+    seen = __builtin_amdgcn_readfirstlane(seen);
+    asm volatile("" : "+s"(seen));
+    return !seen;
+}
+// What a lane's query (key) sees of the keys (queries) in a block's result: those
+// from lo on, `len` more, and those up to `early` (the sinks).
 struct WinMask {
-    int off, sinks, least, n, causal;
-    uint32_t span;
-    __device__ __forceinline__ WinMask(const WinArgs& a, int n_)
-        : off(a.causal ? 0 : a.window - 1), sinks(a.sinks), least(a.causal ? 0 : -0x7fffffff), n(n_), causal(a.causal),
-          span(a.causal ? (uint32_t)a.window : 2u * (uint32_t)a.window - 1u) {}
-    __device__ __forceinline__ bool operator()(int i, int j) const {
-        const int d = i - j;
-        const bool near = (uint32_t)(d + off) < span, first = (j < sinks) | ((i < sinks) & !causal);
-        return (j < n) & (near | (first & (d >= least)));
+    int lo, early;
+    uint32_t len;
+    __device__ __forceinline__ void within(int from, int to) {
+        from = from < 0 ? 0 : from;
+        lo = to < from ? 0x40000000 : from;
+        len = to < from ? 0u : (uint32_t)(to - from);
+    }
+    // of query i, among keys 0 .. n - 1
+    static __device__ __forceinline__ WinMask keys(const WinArgs& a, int i, int n) {
+        WinMask m;
+        int to = a.causal ? i : i + a.window - 1;
+        to = to < n - 1 ? to : n - 1;
+        m.early = a.sinks - 1 < to || !a.causal ? a.sinks - 1 : to;
+        m.early = m.early < n - 1 ? m.early : n - 1;
+        if (!a.causal && i < a.sinks) m.within(0, n - 1);
+        else m.within(i - a.window + 1, to);
+        return m;
+    }
+    // of key j, among the queries; those behind the end weigh nothing of themselves
+    static __device__ __forceinline__ WinMask queries(const WinArgs& a, int j) {
+        WinMask m;
+        m.early = a.causal ? -1 : a.sinks - 1;
+        m.within(a.causal || j < a.sinks ? (a.causal ? j : 0) : j - a.window + 1, j < a.sinks ? 0x3fffffff : j + a.window - 1);
+        return m;
+    }
+    // hide(v) for the results of rows base .. base + 31 that are not seen; `first`:
+    // the sinks are among them
+    template <class Hide>
+    __device__ __forceinline__ void operator()(int base, int g, bool first, Hide hide) const {
+        const int from = lo - base - 4 * g, last = early - base - 4 * g;
+        if (first) {
+            win_rare();
+#pragma unroll
+            for (int v = 0; v < 16; ++v) hide(v, ((uint32_t)(acc_row(v, 0) - from) <= len) | (acc_row(v, 0) <= last));
+        } else {
+            win_rare();
+#pragma unroll
+            for (int v = 0; v < 16; ++v) hide(v, (uint32_t)(acc_row(v, 0) - from) <= len);
+        }
     }
 };
+
 // What a wave's own queries (keys) see of a run x0 .. x1 of keys (queries): 0
 // nothing, 1 some, 2 all.  Runs within [lo, hi] are seen in part, within [all_lo,
 // all_hi] whole, and those that begin in front of `early` may be.
@@ -304,9 +348,6 @@ __device__ __forceinline__ void win_row(uint4 (&f)[DP / 16], const char* base, i
     }
 }
 
-// Keeps a rare branch one: without it the compiler computes both sides, the masks
-// of every tile among them.
-__device__ __forceinline__ void win_rare() { asm volatile(""); }
 // The compiler's wait for a load stands here, and not at its first use: in a loop
 // that would be a wait for the DMA of the next tile too, which it does not count.
 template <int N>
@@ -511,7 +552,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
         lk.issue(to, wave);
         lv.issue(to + TILE, wave);
     };
-    const WinMask mask(a, p.n);
+    const WinMask mask = WinMask::keys(a, i, p.n);
     WinState st;
     floatx16 o[DP / 32];
     win_arrived(q);
@@ -524,28 +565,17 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     if (tiles.count) issue(0);
     for (int t = 0; t < tiles.count; ++t) {
         win_sync();
-        if (t) at.move(t & 1 ? 2 * TILE : -2 * TILE);
         ready(t + 1);
         const int k0 = tiles.at(t) * T, seen = span(k0, k0 + T - 1);
-        if (!seen) {
-            lk.issue(to, wave);
-            lv.issue(to + TILE, wave);
-            continue;
-        }
+        if (seen) {
         constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = DP > 96 ? 8 : 6;
         auto read = [&](int e) WIN_INLINE {
             if (e < 2 * NS) return at.rows(e / NS * 32 * RB, e % NS);
             return at.cols(TILE + (e - 2 * NS) / NJ * 16 * RB, (e - 2 * NS) % NJ);
         };
         auto hide = [&](floatx16& s, int kb) WIN_INLINE {
-            if (seen == 1) {
-                win_rare();
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
-                    s[v] = in ? s[v] : -__builtin_inff();
-                }
-            }
+            if (seen == 1)
+                mask(k0 + 32 * kb, g, k0 < a.sinks, [&](int v, bool in) WIN_INLINE { s[v] = in ? s[v] : -__builtin_inff(); });
         };
         auto anew = [&](float f) WIN_INLINE {
 #pragma unroll
@@ -594,8 +624,14 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
             if (y == 0) hide(s[1], 1);
             if (u == 1 || u == 2) win_exp(s[1], 8 * (y - NJ) / NJ, 8 * (y + 1 - NJ) / NJ, a.scale2, take);
         });
+        }
+        if (win_unseen(seen)) {
+            lk.issue(to, wave);
+            lv.issue(to + TILE, wave);
+        }
+        at.move(t & 1 ? -2 * TILE : 2 * TILE);
     }
-    if (tiles.count > 1 && !(tiles.count & 1)) at.move(-2 * TILE);  // to the first stage again
+    at.move(tiles.count & 1 ? -2 * TILE : 0);  // to the first stage again
     };
     run(std::false_type());
     // Scores past 2^20, or a value that is not finite (a product with a probability
@@ -652,7 +688,7 @@ __device__ __forceinline__ void win_scale_ds(floatx16& ds, float& c, floatx16 (&
 // Gradient of the queries, laid out as the forward: S^T = K Q^T and dP^T = V dO^T
 // in one lane's query, dQ^T = K^T dS^T.  Leaves rowsum(dO O) for the other.
 template <int DP, bool BF>
-__global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
+__global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(WinArgs a) {
     extern __shared__ __align__(256) char smem[];
     constexpr int T = 64, TILE = T * Rows<DP>::RB;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
@@ -704,7 +740,7 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
         lk.issue(to, wave);
         lv.issue(to + TILE, wave);
     };
-    const WinMask mask(a, p.n);
+    const WinMask mask = WinMask::keys(a, i, p.n);
     floatx16 o[DP / 32];
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
@@ -715,14 +751,9 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
     if (tiles.count) issue(0);
     for (int t = 0; t < tiles.count; ++t) {
         win_sync();
-        if (t) at.move(t & 1 ? 2 * TILE : -2 * TILE);
         ready(t + 1);
         const int k0 = tiles.at(t) * T, seen = span(k0, k0 + T - 1);
-        if (!seen) {
-            lk.issue(to, wave);
-            lv.issue(to + TILE, wave);
-            continue;
-        }
+        if (seen) {
         constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = 4;
         // the scores and dP of one block, then the other's, then both blocks' dQ
         auto read = [&](int e) WIN_INLINE {
@@ -735,14 +766,8 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
         auto finish = [&](int kb) WIN_INLINE {  // dS from P and dP
 #pragma unroll
             for (int v = 0; v < 16; ++v) s[kb][v] *= dp[v] - delta;
-            if (seen == 1) {
-                win_rare();
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const bool in = mask(i, k0 + 32 * kb + acc_row(v, g));
-                    s[kb][v] = in ? s[kb][v] : 0.0f;
-                }
-            }
+            if (seen == 1)
+                mask(k0 + 32 * kb, g, k0 < a.sinks, [&](int v, bool in) WIN_INLINE { s[kb][v] = in ? s[kb][v] : 0.0f; });
             win_scale_ds<DP, BF>(s[kb], c, o);
             dp = floatx16{0};
         };
@@ -764,6 +789,12 @@ __global__ void __launch_bounds__(256, 2) window_grad_q_kernel(WinArgs a) {
             if (j == 0) ds = win_pack8<BF>(s[u >> 1], u & 1);
             o[j] = win_mma<BF>(f, ds, o[j]);
         });
+        }
+        if (win_unseen(seen)) {
+            lk.issue(to, wave);
+            lv.issue(to + TILE, wave);
+        }
+        at.move(t & 1 ? -2 * TILE : 2 * TILE);
     }
     win_landed();
     const float f = (BF ? 1.0f : 0x1p-15f) / c;
@@ -803,7 +834,7 @@ __device__ __forceinline__ void win_diff(std::integer_sequence<int, E...>, float
     ((dp[E] -= win_lane<E>(delta)), ...);
 }
 template <int DP, bool BF>
-__global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
+__global__ void __launch_bounds__(256, DP > 64 ? 2 : 2) window_grad_kv_kernel(WinArgs a) {
     extern __shared__ __align__(256) char smem[];
     constexpr int RB = Rows<DP>::RB, V = kWinKeys * RB, STAGE = 2 * kWinStep * RB;  // V, two stages of Q and dO
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
@@ -833,28 +864,38 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
     const uint32_t lds = lds_addr(smem);
     Frags<DP> at;
     at.init(lds + V + 32 * half * RB, lane);
-    int head = 0, qt = 0;  // of the step that is issued next
-    float stat, delta, stat_next = 0.0f, delta_next = 0.0f;
-    const char *qbase = a.q + b * a.qs[0] + kv * group * a.qs[2], *obase = a.go + b * a.gos[0] + kv * group * a.gos[2];
+    // the step that is loaded next: head `head` of query tile qt; heads go round within a tile
+    int head = 0, qt = 0, q0 = 0, q0_next = 0;
+    float stat = 0.0f, delta = 0.0f, stat_next = 0.0f, delta_next = 0.0f;
+    const int mine_q = 32 * half + acc_row(lane & 15, g);  // whose statistics this lane loads
     int64_t row = 0;
     constexpr int LOADS = RowLoads<DP, kWinStep, 4>::LOADS;
     uint32_t to = lds;
+    auto place = [&]() WIN_INLINE {
+        const int first = q.at(qt) * kWinStep;
+        lq.seek(a.q + b * a.qs[0] + kv * group * a.qs[2], first, n);
+        lo_.seek(a.go + b * a.gos[0] + kv * group * a.gos[2], first, n);
+        row = ((int64_t)b * a.H + kv * group) * a.NP + first;
+        q0_next = first + 32 * half;
+    };
     auto ready = [&](int s) WIN_INLINE {
         to = lds + V + (s & 1) * STAGE;
-        if (s < steps && (qt == 0 || q.leap(qt))) {
-            const int first = q.at(qt) * kWinStep;
-            lq.seek(qbase + head * a.qs[2], first, n);
-            lo_.seek(obase + head * a.gos[2], first, n);
-            row = ((int64_t)b * a.H + kv * group + head) * a.NP + first + 32 * half + acc_row(lane & 15, g);
-        }
-        lq.next(s < steps);
-        lo_.next(s < steps);
+        q0 = q0_next;
         if (s < steps) {
-            stat_next = a.stat[row];
-            delta_next = a.delta[row];
+            if (head == group) {
+                head = 0;
+                ++qt;
+                place();
+            }
+            stat_next = a.stat[row + mine_q];
+            delta_next = a.delta[row + mine_q];
         }
-        row += kWinStep;
-        if (++qt == q.count) qt = 0, ++head;
+        lq.resource(s < steps);
+        lo_.resource(s < steps);
+        lq.at += a.qs[2];
+        lo_.at += a.gos[2];
+        row += a.NP;
+        ++head;
     };
     auto load = [&](int x) WIN_INLINE {
         if (x < LOADS) lq.load(x, to, wave);
@@ -868,29 +909,27 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
         RowLoads<DP, kWinKeys, 4> lv;
         lv.init(a.vs[1], a.D, wave, lane);
         lv.seek(a.v + b * a.vs[0] + kv * a.vs[2], k0, n);
-        lv.next(true);
+        lv.resource(true);
         lv.issue(lds, wave);
+        place();
         ready(0);
         issue();
     }
     floatx16 ok[DP / 32], ov[DP / 32];
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) ok[j] = ov[j] = floatx16{0};
-    const WinMask mask(a, n);
+    const WinMask mask = WinMask::queries(a, key);
     const WinSpan span = WinSpan::queries(a, mine, klast);
     float c = BF ? 1.0f : 0x1p126f;
-    int ct = 0;
     win_arrived(kf);
     for (int t = 0; t < steps; ++t) {
         win_sync();
         asm volatile("" : "+v"(stat_next), "+v"(delta_next));
         stat = stat_next, delta = delta_next;
-        if (t) at.move(t & 1 ? STAGE : -STAGE);
         ready(t + 1);
-        const int q0 = q.at(ct) * kWinStep + 32 * half, seen = q0 < n ? span(q0, q0 + 31) : 0;
-        if (++ct == q.count) ct = 0;
-        if (!seen || DP > 96) issue();
-        if (!seen) continue;
+        const int seen = q0 < n ? span(q0, q0 + 31) : 0;
+        if (DP > 96) issue();  // no registers for them between the products
+        if (seen) {
         constexpr int NS = DP / 16, NJ = DP / 32, PD = 4, OUT = kWinStep * RB;
         const uint32_t vt = 32 * (block - half) * RB - V - (t & 1) * STAGE;  // V's rows from Q's
         // Q; dO and V in turn; dO and Q transposed
@@ -916,14 +955,8 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
                 dp = win_mma<BF>(was, f, dp);
                 if (e == 3 * NS - 1) {
                     win_probs(std::make_integer_sequence<int, 16>(), s, a.scale2, stat);
-                    if (seen == 1) {
-                        win_rare();
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) {
-                            const bool in = mask(q0 + acc_row(v, g), key);
-                            s[v] = in ? s[v] : 0.0f;
-                        }
-                    }
+                    if (seen == 1)
+                        mask(q0, g, !a.causal && q0 < a.sinks, [&](int v, bool in) WIN_INLINE { s[v] = in ? s[v] : 0.0f; });
                 }
                 return;
             }
@@ -947,6 +980,9 @@ __global__ void __launch_bounds__(256, 2) window_grad_kv_kernel(WinArgs a) {
                 ok[j] = win_mma<BF>(f, pr, ok[j]);
             }
         });
+        }
+        if (DP <= 96 && win_unseen(seen)) issue();
+        at.move(t & 1 ? -STAGE : STAGE);
     }
     // the fellow's sums through LDS, one tensor after the other
     const float fv = BF ? 1.0f : 0x1p-15f;
@@ -1036,7 +1072,7 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
     floatx16 o[DP / 32];
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
-    const WinMask mask(a, len);
+    const WinMask mask = WinMask::keys(a, i, len);
     int s = from + wave, buf = 0;
     win_arrived(q);
     if (s < to) issue(s, 0);
@@ -1062,14 +1098,8 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
             if (e < NS) {
                 sc = win_mma<BF>(f, q[e], sc);
                 if (e < NS - 1) return;
-                if (some) {
-                    win_rare();
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) {
-                        const bool in = mask(i, j0 + acc_row(v, g));
-                        sc[v] = in ? sc[v] : -__builtin_inff();
-                    }
-                }
+                if (some)
+                    mask(j0, g, j0 < sinks, [&](int v, bool in) WIN_INLINE { sc[v] = in ? sc[v] : -__builtin_inff(); });
                 const float take = win_top<BF, true>(sc, st, a.scale2, [&](float f_) WIN_INLINE {
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
