@@ -567,7 +567,12 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
         win_sync();
         ready(t + 1);
         const int k0 = tiles.at(t) * T, seen = span(k0, k0 + T - 1);
-        if (seen) {
+        if (!seen) {
+            lk.issue(to, wave);
+            lv.issue(to + TILE, wave);
+            at.move(t & 1 ? -2 * TILE : 2 * TILE);
+            continue;
+        }
         constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = DP > 96 ? 8 : 6;
         auto read = [&](int e) WIN_INLINE {
             if (e < 2 * NS) return at.rows(e / NS * 32 * RB, e % NS);
@@ -624,11 +629,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
             if (y == 0) hide(s[1], 1);
             if (u == 1 || u == 2) win_exp(s[1], 8 * (y - NJ) / NJ, 8 * (y + 1 - NJ) / NJ, a.scale2, take);
         });
-        }
-        if (win_unseen(seen)) {
-            lk.issue(to, wave);
-            lv.issue(to + TILE, wave);
-        }
         at.move(t & 1 ? -2 * TILE : 2 * TILE);
     }
     at.move(tiles.count & 1 ? -2 * TILE : 0);  // to the first stage again
@@ -753,7 +753,12 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
         win_sync();
         ready(t + 1);
         const int k0 = tiles.at(t) * T, seen = span(k0, k0 + T - 1);
-        if (seen) {
+        if (!seen) {
+            lk.issue(to, wave);
+            lv.issue(to + TILE, wave);
+            at.move(t & 1 ? -2 * TILE : 2 * TILE);
+            continue;
+        }
         constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = 4;
         // the scores and dP of one block, then the other's, then both blocks' dQ
         auto read = [&](int e) WIN_INLINE {
@@ -789,11 +794,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
             if (j == 0) ds = win_pack8<BF>(s[u >> 1], u & 1);
             o[j] = win_mma<BF>(f, ds, o[j]);
         });
-        }
-        if (win_unseen(seen)) {
-            lk.issue(to, wave);
-            lv.issue(to + TILE, wave);
-        }
         at.move(t & 1 ? -2 * TILE : 2 * TILE);
     }
     win_landed();
