@@ -72,12 +72,38 @@ __device__ __forceinline__ float norm_round(float v) {
     return v;
 }
 
+// op over the 64 lanes, in all of them: within 16 lanes by DPP, across them by
+// lane swaps.  No LDS: six shuffles wait for it six times, the row's three
+// reductions took a third of the 8-bit norm.
+template <int CTRL>
+__device__ __forceinline__ uint32_t norm_dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <class V, class Op>
+__device__ __forceinline__ V wave_all(V v, Op op) {
+    static_assert(sizeof(V) == 4, "one register");
+    v = op(v, __builtin_bit_cast(V, norm_dpp<0xb1>(__builtin_bit_cast(uint32_t, v))));   // lane ^ 1
+    v = op(v, __builtin_bit_cast(V, norm_dpp<0x4e>(__builtin_bit_cast(uint32_t, v))));   // lane ^ 2
+    v = op(v, __builtin_bit_cast(V, norm_dpp<0x141>(__builtin_bit_cast(uint32_t, v))));  // 7 - lane of 8
+    v = op(v, __builtin_bit_cast(V, norm_dpp<0x140>(__builtin_bit_cast(uint32_t, v))));  // 15 - lane of 16
+    const uint32_t a = __builtin_bit_cast(uint32_t, v);
+    const auto x = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    v = op(__builtin_bit_cast(V, (uint32_t)x[0]), __builtin_bit_cast(V, (uint32_t)x[1]));
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto y = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return op(__builtin_bit_cast(V, (uint32_t)y[0]), __builtin_bit_cast(V, (uint32_t)y[1]));
+}
+template <class Op>
+__device__ __forceinline__ double wave_all(double v, Op op) {  // rare
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+    return v;
+}
 // Sum or maximum over the T threads of a row: a wave, or the workgroup of four
 // through `sm` (a barrier on both sides; every thread of it calls).
 template <int T, class V, class Op>
 __device__ __forceinline__ V row_reduce(V v, V* sm, Op op) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+    v = wave_all(v, op);
     if constexpr (T > 64) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
@@ -145,7 +171,7 @@ __device__ __forceinline__ void norm_codes(const NormArgs& a, const float (&h)[N
         norm_weight8(a.w, a.wdt, col + 8 * T * i, a.C, w);
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-            p[i][t] = col + 8 * T * i + t < a.C ? h[i][t] * lift * w[t] : 0.0f;
+            p[i][t] = h[i][t] * lift * w[t];  // 0 past C, as h and w are
             mx = max(mx, __float_as_uint(p[i][t]) & 0x7fffffffu);
         }
     }
@@ -161,28 +187,59 @@ __device__ __forceinline__ void norm_codes(const NormArgs& a, const float (&h)[N
     if (ok) {
         const float near = top * (1.0f - 0x1p-22f);
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
+        for (int i = 0; i < NC; ++i) {
+            float most = 0.0f;  // one branch for 8: of a row one lane or two take it
+#pragma unroll
+            for (int t = 0; t < 8; ++t) most = fmaxf(most, fabsf(p[i][t]));
+            if (most < near) continue;
 #pragma unroll
             for (int t = 0; t < 8; ++t)
                 if (fabsf(p[i][t]) >= near) topd = fmax(topd, exact(i, t));
+        }
     }
-    topd = row_reduce<T>(topd, sm, Most());
+    // of a wave's row mostly one lane has candidates
+    const uint64_t who = __ballot(topd > 0.0);
+    if (T == 64 && (who & (who - 1)) == 0) {
+        const int lane = who ? __builtin_ctzll(who) : 0;
+        const uint64_t bits = __builtin_bit_cast(uint64_t, topd);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(bits >> 32), lane);
+        topd = __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    } else {
+        topd = row_reduce<T>(topd, sm, Most());
+    }
     if ((threadIdx.x & (T - 1)) == 0) a.scale[m] = fin ? (float)(topd / 127.0 * (double)back) : __uint_as_float(0x7fc00000u);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
         const int c0 = col + 8 * T * i;
         if (c0 >= a.C) continue;
-        uint32_t out[2] = {0, 0};
+        // float32 holds whole numbers around 1.5 2^23: the sum rounds to one, its
+        // low byte is the code
+        constexpr float WHOLE = 0x1.8p23f;
+        uint32_t out[2];
+        float code[8], off = 0.0f;
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-            const float q = fabsf(p[i][t]) * r;
-            float c = __builtin_rintf(q);
-            if (fabsf(fabsf(q - c) - 0.5f) < 1e-4f) {
-                c = floorf(q);
-                const double v = 254.0 * exact(i, t), mid = (2.0 * (double)c + 1.0) * topd;
-                if (v > mid || (v == mid && ((int)c & 1))) c += 1.0f;
+            code[t] = fmaf(p[i][t], r, WHOLE);
+            off = fmaxf(off, fabsf(fmaf(p[i][t], r, -(code[t] - WHOLE))));
+        }
+        if (off > 0.5f - 1e-4f) {  // in the middle of two codes: of 8 values one in 600
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const float q = fabsf(p[i][t]) * r;
+                float c = __builtin_rintf(q);
+                if (fabsf(fabsf(q - c) - 0.5f) < 1e-4f) {
+                    c = floorf(q);
+                    const double v = 254.0 * exact(i, t), mid = (2.0 * (double)c + 1.0) * topd;
+                    if (v > mid || (v == mid && ((int)c & 1))) c += 1.0f;
+                }
+                code[t] = copysignf(c, p[i][t]) + WHOLE;
             }
-            out[t >> 2] |= (uint32_t)((int)copysignf(c, p[i][t]) & 0xff) << (8 * (t & 3));
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(code[4 * e + 1]), __float_as_uint(code[4 * e]), 0x0c0c0400u);
+            const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(code[4 * e + 3]), __float_as_uint(code[4 * e + 2]), 0x04000c0cu);
+            out[e] = fin ? lo | hi : 0u;
         }
         int8_t* dst = a.codes + m * a.C + c0;
         if (c0 + 8 <= a.C) {
@@ -375,7 +432,7 @@ hipError_t launch_rms_norm(const NormCall& c, void* y, void* h, float* rstd, int
 
 // Workgroups of the gradient: each leaves a row of partial sums.
 int norm_grad_parts(int64_t M, int64_t C) {
-    const int64_t rows = C <= 2048 ? 4 : 1, blocks = (M + rows - 1) / rows, most = 2 * device_cus();
+    const int64_t rows = C <= 2048 ? 4 : 1, blocks = (M + rows - 1) / rows, most = 4 * device_cus();
     return (int)(blocks < most ? blocks : most);
 }
 struct NormGradGo {
