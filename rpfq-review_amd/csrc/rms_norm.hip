@@ -7,30 +7,41 @@
 
 namespace rpfq {
 
-// 8 elements of a row from column c on (zeros past C) as float32.  Rows may
+// 8 elements of a row from column c on (zeros past C), as they lie.  Rows may
 // begin at any element: gfx950 loads 16 unaligned bytes with one instruction.
 template <int DT>
-__device__ __forceinline__ void norm_load8(const void* p, int64_t row, int c, int C, float (&v)[8]) {
-    if (c + 8 <= C) {
-        if constexpr (DT == RPFQ_F32) {
-            __builtin_memcpy(v, reinterpret_cast<const float*>(p) + row + c, 32);
-        } else {
-            uint32_t w[4];
-            __builtin_memcpy(w, reinterpret_cast<const uint16_t*>(p) + row + c, 16);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                if (DT == RPFQ_F16) {
-                    const half2v h = __builtin_bit_cast(half2v, w[t]);
-                    v[2 * t] = (float)h[0], v[2 * t + 1] = (float)h[1];
-                } else {
-                    v[2 * t] = bf16_to_f32(w[t] & 0xffffu), v[2 * t + 1] = bf16_to_f32(w[t] >> 16);
-                }
-            }
+struct Norm8 {
+    uint32_t w[DT == RPFQ_F32 ? 8 : 4];
+    __device__ __forceinline__ void load(const void* p, int64_t row, int c, int C) {
+        constexpr int ES = DT == RPFQ_F32 ? 4 : 2;
+        const char* src = reinterpret_cast<const char*>(p) + (row + c) * ES;
+        if (c + 8 <= C) {
+            __builtin_memcpy(w, src, 8 * ES);
+            return;
         }
-        return;
-    }
 #pragma unroll
-    for (int t = 0; t < 8; ++t) v[t] = c + t < C ? load_y1<DT>(p, row + c + t) : 0.0f;
+        for (int t = 0; t < (int)(sizeof(w) / 4); ++t) w[t] = 0;
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+            if (c + t < C) {
+                if (DT == RPFQ_F32) w[t % (sizeof(w) / 4)] = reinterpret_cast<const uint32_t*>(src)[t];
+                else w[t / 2 % (sizeof(w) / 4)] |= (uint32_t)reinterpret_cast<const uint16_t*>(src)[t] << (16 * (t & 1));
+            }
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            if (DT == RPFQ_F32) v[t] = __uint_as_float(w[t % (sizeof(w) / 4)]);
+            else if (DT == RPFQ_F16) v[t] = (float)__builtin_bit_cast(half2v, w[t / 2 % (sizeof(w) / 4)])[t & 1];
+            else v[t] = bf16_to_f32(t & 1 ? w[t / 2 % (sizeof(w) / 4)] >> 16 : w[t / 2 % (sizeof(w) / 4)] & 0xffffu);
+        }
+    }
+};
+template <int DT>
+__device__ __forceinline__ void norm_load8(const void* p, int64_t row, int c, int C, float (&v)[8]) {
+    Norm8<DT> r;
+    r.load(p, row, c, C);
+    r.values(v);
 }
 template <int DT>
 __device__ __forceinline__ uint32_t norm_pack2(float a, float b) {
@@ -158,7 +169,7 @@ __device__ __forceinline__ float norm_rstd(const float (&h)[NC][8], int C, float
 // comparison: 40 bits of 16-bit h).  The largest product is taken among those
 // that float32 rounds to within 2^-22 of the largest.
 template <int T, int NC>
-__device__ __forceinline__ void norm_codes(const NormArgs& a, const float (&h)[NC][8], float rstd, int64_t m, int col, double* sm) {
+__device__ __forceinline__ void norm_codes(const NormArgs& a, const float (&h)[NC][8], const float (&w)[NC][8], float rstd, int64_t m, int col, double* sm) {
     // a power of two near 1 / rms, exact on h: products stay in float32's range
     int e = 1 - __builtin_amdgcn_frexp_expf(rstd);
     e = e < -126 ? -126 : e > 126 ? 126 : e;
@@ -167,22 +178,16 @@ __device__ __forceinline__ void norm_codes(const NormArgs& a, const float (&h)[N
     float p[NC][8];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        float w[8];
-        norm_weight8(a.w, a.wdt, col + 8 * T * i, a.C, w);
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-            p[i][t] = h[i][t] * lift * w[t];  // 0 past C, as h and w are
+            p[i][t] = h[i][t] * lift * w[i][t];  // 0 past C, as h is
             mx = max(mx, __float_as_uint(p[i][t]) & 0x7fffffffu);
         }
     }
     mx = row_reduce<T>(mx, reinterpret_cast<uint32_t*>(sm), Most());
     const bool fin = mx < 0x7f800000u, ok = fin && mx >= 0x00800000u;
     const float top = __uint_as_float(mx), r = ok ? 127.0f / top : 0.0f;
-    auto exact = [&](int i, int t) {
-        float w[8];  // read again: this is rare
-        norm_weight8(a.w, a.wdt, col + 8 * T * i, a.C, w);
-        return (double)(fabsf(h[i][t]) * lift) * (double)fabsf(w[t]);
-    };
+    auto exact = [&](int i, int t) { return (double)(fabsf(h[i][t]) * lift) * (double)fabsf(w[i][t]); };
     double topd = 0.0;
     if (ok) {
         const float near = top * (1.0f - 0x1p-22f);
@@ -192,6 +197,7 @@ __device__ __forceinline__ void norm_codes(const NormArgs& a, const float (&h)[N
 #pragma unroll
             for (int t = 0; t < 8; ++t) most = fmaxf(most, fabsf(p[i][t]));
             if (most < near) continue;
+            asm volatile("");  // the 64-bit products are not formed ahead of the branch
 #pragma unroll
             for (int t = 0; t < 8; ++t)
                 if (fabsf(p[i][t]) >= near) topd = fmax(topd, exact(i, t));
@@ -223,6 +229,7 @@ __device__ __forceinline__ void norm_codes(const NormArgs& a, const float (&h)[N
             off = fmaxf(off, fabsf(fmaf(p[i][t], r, -(code[t] - WHOLE))));
         }
         if (off > 0.5f - 1e-4f) {  // in the middle of two codes: of 8 values one in 600
+            asm volatile("");
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 const float q = fabsf(p[i][t]) * r;
@@ -253,42 +260,50 @@ __device__ __forceinline__ void norm_codes(const NormArgs& a, const float (&h)[N
 }
 
 // A row in the registers of T threads (a wave, or a workgroup of four), 8 NC
-// values each: read once, written once.
+// values each: read once, written once.  A workgroup stays for many rows, with
+// the weights in registers.  Bound by HBM: 50,432 rows of 768 bf16 to codes 60 us
+// (271 MB, 4.5 TB/s; a workgroup a row group 72, with the next row loaded ahead,
+// at half the waves, 79), 16,384 of 4,096 to bf16 88 us (537 MB, 6.1 TB/s).
 template <int DT, int T, int NC, bool CODES>
 __global__ void __launch_bounds__(256) rms_norm_kernel(NormArgs a) {
     __shared__ double sm[4];
     const int col = 8 * (threadIdx.x & (T - 1));
     constexpr int ROWS = 256 / T;
+    float w[NC][8];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) norm_weight8(a.w, a.wdt, col + 8 * T * i, a.C, w[i]);
     for (int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / T; m < a.M; m += (int64_t)gridDim.x * ROWS) {
         const int64_t row = m * a.C;
+        Norm8<DT> x[NC], r[NC];
         float h[NC][8];
 #pragma unroll
-        for (int i = 0; i < NC; ++i) norm_load8<DT>(a.x, row, col + 8 * T * i, a.C, h[i]);
-        if (a.res) {
-            float r[NC][8];
+        for (int i = 0; i < NC; ++i) x[i].load(a.x, row, col + 8 * T * i, a.C);
+        if (a.res)
 #pragma unroll
-            for (int i = 0; i < NC; ++i) norm_load8<DT>(a.res, row, col + 8 * T * i, a.C, r[i]);
+            for (int i = 0; i < NC; ++i) r[i].load(a.res, row, col + 8 * T * i, a.C);
 #pragma unroll
-            for (int i = 0; i < NC; ++i) {
+        for (int i = 0; i < NC; ++i) {
+            x[i].values(h[i]);
+            if (!a.res) continue;
+            float v[8];
+            r[i].values(v);
 #pragma unroll
-                for (int t = 0; t < 8; ++t) h[i][t] = norm_round<DT>(h[i][t] + r[i][t]);
-                if (col + 8 * T * i < a.C) norm_store8<DT>(a.h, row, col + 8 * T * i, a.C, h[i]);
-            }
+            for (int t = 0; t < 8; ++t) h[i][t] = norm_round<DT>(h[i][t] + v[t]);
+            if (col + 8 * T * i < a.C) norm_store8<DT>(a.h, row, col + 8 * T * i, a.C, h[i]);
         }
         const float rstd = norm_rstd<T, NC>(h, a.C, a.eps, sm);
         if constexpr (CODES) {
-            norm_codes<T, NC>(a, h, rstd, m, col, sm);
+            norm_codes<T, NC>(a, h, w, rstd, m, col, sm);
         } else {
             if (a.rstd && (threadIdx.x & (T - 1)) == 0) a.rstd[m] = rstd;
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 const int c = col + 8 * T * i;
                 if (c >= a.C) continue;
-                float w[8];
-                norm_weight8(a.w, a.wdt, c, a.C, w);
+                float y[8];
 #pragma unroll
-                for (int t = 0; t < 8; ++t) w[t] *= h[i][t] * rstd;
-                norm_store8<DT>(a.y, row, c, a.C, w);
+                for (int t = 0; t < 8; ++t) y[t] = w[i][t] * (h[i][t] * rstd);
+                norm_store8<DT>(a.y, row, c, a.C, y);
             }
         }
     }
@@ -314,25 +329,35 @@ __global__ void __launch_bounds__(256) rms_norm_grad_kernel(NormGradArgs a) {
     for (int i = 0; i < NC; ++i)
 #pragma unroll
         for (int t = 0; t < 8; ++t) gw[i][t] = 0.0f;
+    float w[NC][8];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) norm_weight8(a.w, a.wdt, col + 8 * T * i, a.C, w[i]);
     for (int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / T; m < a.M; m += (int64_t)gridDim.x * ROWS) {
         const int64_t row = m * a.C;
+        Norm8<DT> hr[NC], gr[NC], sum[NC];
         float n[NC][8], g[NC][8];
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            norm_load8<DT>(a.h, row, col + 8 * T * i, a.C, n[i]);
-            norm_load8<DT>(a.gy, row, col + 8 * T * i, a.C, g[i]);
+            hr[i].load(a.h, row, col + 8 * T * i, a.C);
+            gr[i].load(a.gy, row, col + 8 * T * i, a.C);
         }
+        if (a.gh)
+#pragma unroll
+            for (int i = 0; i < NC; ++i) sum[i].load(a.gh, row, col + 8 * T * i, a.C);
         const float r = a.rstd[m];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            hr[i].values(n[i]);
+            gr[i].values(g[i]);
+        }
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            float w[8];
-            norm_weight8(a.w, a.wdt, col + 8 * T * i, a.C, w);
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 n[i][t] *= r;
                 gw[i][t] = fmaf(g[i][t], n[i][t], gw[i][t]);
-                g[i][t] *= w[t];
+                g[i][t] *= w[i][t];
                 s = fmaf(g[i][t], n[i][t], s);
             }
         }
@@ -342,7 +367,7 @@ __global__ void __launch_bounds__(256) rms_norm_grad_kernel(NormGradArgs a) {
             const int c = col + 8 * T * i;
             if (c >= a.C) continue;
             float gh[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (a.gh) norm_load8<DT>(a.gh, row, c, a.C, gh);
+            if (a.gh) sum[i].values(gh);
 #pragma unroll
             for (int t = 0; t < 8; ++t) gh[t] = fmaf(r, g[i][t] - n[i][t] * mean, gh[t]);
             norm_store8<DT>(a.gx, row, c, a.C, gh);
@@ -419,7 +444,8 @@ struct NormGo {
     template <int DT, int T, int NC>
     hipError_t run() {
         const int64_t blocks = (a.M + 256 / T - 1) / (256 / T);
-        const dim3 grid((unsigned)(blocks < (1LL << 22) ? blocks : 1LL << 22));
+        const int64_t most = 8 * device_cus();
+        const dim3 grid((unsigned)(blocks < most ? blocks : most));
         if (a.codes) hipLaunchKernelGGL((rms_norm_kernel<DT, T, NC, true>), grid, dim3(256), 0, s, a);
         else hipLaunchKernelGGL((rms_norm_kernel<DT, T, NC, false>), grid, dim3(256), 0, s, a);
         return hipGetLastError();
@@ -430,7 +456,9 @@ hipError_t launch_rms_norm(const NormCall& c, void* y, void* h, float* rstd, int
     return norm_dispatch(c.dtype, c.C, NormGo{a, s});
 }
 
-// Workgroups of the gradient: each leaves a row of partial sums.
+// Workgroups of the gradient: each leaves a row of partial sums.  Four a CU: two
+// leave too few loads on their way (165 us, 4.5 TB/s at four: 16,384 x 4,096 bf16
+// 118 us for 537 MB).
 int norm_grad_parts(int64_t M, int64_t C) {
     const int64_t rows = C <= 2048 ? 4 : 1, blocks = (M + rows - 1) / rows, most = 4 * device_cus();
     return (int)(blocks < most ? blocks : most);

@@ -12,26 +12,25 @@ struct RotaryArgs {
     char* out[2];
     const void* pos;
     const double* freqs;
-    int pairs, tokens, units, total;  // pairs of a head; tokens of a workgroup, units of a head, of all its tokens
+    int pairs, tokens;  // pairs of a head, tokens of a workgroup
+    int turned, units;  // units of V values, or of V pairs, that turn; of a head (the rest are copied)
+    int total;          // units of all its tokens
+    int rest;           // values of a unit that is copied: V, or 1
 };
 
-template <int DT>
-constexpr int rotary_vec() { return DT == RPFQ_F32 ? 4 : 8; }
-
-// V consecutive values as float32: 16 bytes, or one value.
+// V consecutive values as float32, from any element on: gfx950 loads 16 unaligned
+// bytes with one instruction.
 template <int DT, int V>
 __device__ __forceinline__ void rotary_load(const char* p, int64_t at, float (&v)[V]) {
     if constexpr (V == 1) {
         v[0] = load_y1<DT>(p, at);
     } else if constexpr (DT == RPFQ_F32) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(p + 4 * at);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) v[t] = a[t];
+        __builtin_memcpy(v, p + 4 * at, 4 * V);
     } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(p + 2 * at);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        uint32_t w[V / 2];
+        __builtin_memcpy(w, p + 2 * at, 2 * V);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < V / 2; ++t) {
             if (DT == RPFQ_F16) {
                 const half2v h = __builtin_bit_cast(half2v, w[t]);
                 v[2 * t] = (float)h[0], v[2 * t + 1] = (float)h[1];
@@ -46,19 +45,20 @@ __device__ __forceinline__ void rotary_store(char* p, int64_t at, const float (&
     if constexpr (V == 1) {
         store1<DT>(p, at, v[0]);
     } else if constexpr (DT == RPFQ_F32) {
-        *reinterpret_cast<f32x4*>(p + 4 * at) = (f32x4){v[0], v[1], v[2], v[3]};
+        __builtin_memcpy(p + 4 * at, v, 4 * V);
     } else {
-        uint32_t w[4];
+        uint32_t w[V / 2];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) w[t] = DT == RPFQ_F16 ? cvt_pk(v[2 * t], v[2 * t + 1]) : pack_bf2(v[2 * t], v[2 * t + 1]);
-        *reinterpret_cast<uint4*>(p + 2 * at) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int t = 0; t < V / 2; ++t) w[t] = DT == RPFQ_F16 ? cvt_pk(v[2 * t], v[2 * t + 1]) : pack_bf2(v[2 * t], v[2 * t + 1]);
+        __builtin_memcpy(p + 2 * at, w, 2 * V);
     }
 }
 
 // A workgroup takes `tokens` tokens: their cosines and sines go to LDS once, for
 // all heads of both tensors.  The angle is formed in 64 bits and reduced to a
 // part of a turn before it becomes float32, so a position of 2^31 is as exact as
-// 1.  Then a thread takes V pairs at a time (V = 1: any strides and sizes).
+// 1.  Then a thread takes V pairs at a time, or V values of neighbours.
+// Bound by HBM: 32,768 tokens x 20 heads x 128 bf16 60 us (336 MB, 5.5 TB/s).
 template <int DT, int V>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
     extern __shared__ float2 turn[];  // [tokens][pairs]
@@ -94,41 +94,56 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
         const int64_t from = b * d.in_stride[which][0] + n * d.in_stride[which][1] + h * d.in_stride[which][2];
         const int64_t to = b * d.out_stride[which][0] + n * d.out_stride[which][1] + h * d.out_stride[which][2];
         float x[V], y[V];
-        if (u * V >= a.pairs) {  // values behind the pairs: as they are
-            const int at = 2 * a.pairs + u * V - a.pairs;
-            rotary_load<DT, V>(in, from + at, x);
-            rotary_store<DT, V>(out, to + at, x);
+        if (u >= a.turned) {  // values behind the pairs: as they are
+            const int at = 2 * a.pairs + (u - a.turned) * a.rest;
+            if (a.rest == V) {
+                rotary_load<DT, V>(in, from + at, x);
+                rotary_store<DT, V>(out, to + at, x);
+            } else {
+                float one[1];
+                rotary_load<DT, 1>(in, from + at, one);
+                rotary_store<DT, 1>(out, to + at, one);
+            }
+            continue;
+        }
+        if (V > 1 && d.interleaved) {
+            const float2* cs = turn + tok * a.pairs + u * (V / 2);
+            rotary_load<DT, V>(in, from + u * V, x);
+#pragma unroll
+            for (int t = 0; t < V / 2; ++t) {
+                const float2 e = cs[t];
+                y[2 * t] = x[2 * t] * e.x - x[2 * t + 1] * e.y, y[2 * t + 1] = x[2 * t + 1] * e.x + x[2 * t] * e.y;
+            }
+            rotary_store<DT, V>(out, to + u * V, y);
             continue;
         }
         const float2* cs = turn + tok * a.pairs + u * V;
-        const int first = d.interleaved ? 2 * u * V : u * V, second = d.interleaved ? first + V : a.pairs + u * V;
+        const int first = u * V, second = a.pairs + u * V;
         rotary_load<DT, V>(in, from + first, x);
         rotary_load<DT, V>(in, from + second, y);
         float p[V], q[V];
-        if (V > 1 && d.interleaved) {
 #pragma unroll
-            for (int t = 0; t < V / 2; ++t) {
-                const float2 e = cs[t], f = cs[V / 2 + t];
-                p[2 * t] = x[2 * t] * e.x - x[2 * t + 1] * e.y, p[2 * t + 1] = x[2 * t + 1] * e.x + x[2 * t] * e.y;
-                q[2 * t] = y[2 * t] * f.x - y[2 * t + 1] * f.y, q[2 * t + 1] = y[2 * t + 1] * f.x + y[2 * t] * f.y;
-            }
-        } else {
-#pragma unroll
-            for (int t = 0; t < V; ++t) {
-                const float2 e = cs[t];
-                p[t] = x[t] * e.x - y[t] * e.y, q[t] = y[t] * e.x + x[t] * e.y;
-            }
+        for (int t = 0; t < V; ++t) {
+            const float2 e = cs[t];
+            p[t] = x[t] * e.x - y[t] * e.y, q[t] = y[t] * e.x + x[t] * e.y;
         }
         rotary_store<DT, V>(out, to + first, p);
         rotary_store<DT, V>(out, to + second, q);
     }
 }
 
-template <int DT>
-static hipError_t rotary_go(RotaryArgs& a, bool vec, hipStream_t s) {
-    const int v = vec ? rotary_vec<DT>() : 1;
+// V of a call: 16 bytes, or fewer where the pairs are no multiple (26 pairs of
+// neighbours in float32, 1,568 x 2 tokens of 32 heads: 43 us a value at a time, so 21).
+template <int DT, int V>
+static hipError_t rotary_go(RotaryArgs& a, hipStream_t s) {
+    if constexpr (V > 1) {
+        if ((a.d.interleaved ? 2 * a.pairs : a.pairs) % V) return rotary_go<DT, V / 2>(a, s);
+    }
     const int64_t all = a.d.B * a.d.N;
-    a.units = a.pairs / v + (int)(a.d.D - 2 * a.pairs) / v;
+    const int behind = (int)a.d.D - 2 * a.pairs;
+    a.rest = behind % V ? 1 : V;
+    a.turned = V > 1 && a.d.interleaved ? 2 * a.pairs / V : a.pairs / V;
+    a.units = a.turned + behind / a.rest;
     // tokens of a workgroup: an angle a thread, but fewer where the chip would not
     // be filled (2 workgroups a CU)
     const int64_t fill = all / (2 * device_cus()), most = 256 / a.pairs;
@@ -136,9 +151,7 @@ static hipError_t rotary_go(RotaryArgs& a, bool vec, hipStream_t s) {
     if (a.tokens < 1) a.tokens = 1;
     a.total = a.tokens * (int)(a.d.heads[0] + a.d.heads[1]) * a.units;
     const dim3 grid((unsigned)((all + a.tokens - 1) / a.tokens));
-    const size_t lds = (size_t)a.tokens * a.pairs * sizeof(float2);
-    if (vec) hipLaunchKernelGGL((rotary_kernel<DT, rotary_vec<DT>()>), grid, dim3(256), lds, s, a);
-    else hipLaunchKernelGGL((rotary_kernel<DT, 1>), grid, dim3(256), lds, s, a);
+    hipLaunchKernelGGL((rotary_kernel<DT, V>), grid, dim3(256), (size_t)a.tokens * a.pairs * sizeof(float2), s, a);
     return hipGetLastError();
 }
 
@@ -152,18 +165,10 @@ hipError_t launch_rotary(const rpfq_rotary_desc& d, const void* q, const void* k
     a.freqs = freqs;
     for (int i = 0; i < d.axes; ++i) a.pairs += d.sections[i];
     for (int i = d.axes; i < 4; ++i) a.d.sections[i] = 0;
-    const int v = d.dtype == RPFQ_F32 ? 4 : 8;
-    int64_t odd = a.pairs | d.D;  // whether any offset is no multiple of v
-    uintptr_t at = 0;
-    for (int i = 0; i < (d.heads[1] ? 2 : 1); ++i) {
-        for (int j = 0; j < 3; ++j) odd |= d.in_stride[i][j] | d.out_stride[i][j];
-        at |= reinterpret_cast<uintptr_t>(a.in[i]) | reinterpret_cast<uintptr_t>(a.out[i]);
-    }
-    const bool vec = odd % v == 0 && at % 16 == 0;
     switch (d.dtype) {
-        case RPFQ_F32: return rotary_go<RPFQ_F32>(a, vec, s);
-        case RPFQ_F16: return rotary_go<RPFQ_F16>(a, vec, s);
-        default: return rotary_go<RPFQ_BF16>(a, vec, s);
+        case RPFQ_F32: return rotary_go<RPFQ_F32, 4>(a, s);
+        case RPFQ_F16: return rotary_go<RPFQ_F16, 8>(a, s);
+        default: return rotary_go<RPFQ_BF16, 8>(a, s);
     }
 }
 
