@@ -1027,10 +1027,12 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 2) window_grad_kv_kernel(Wi
 // up to 32 of its rows (queries x heads that share it) and a part of the keys; its
 // waves take tiles of 32 keys in turn, each through LDS of its own, without
 // waiting for each other.  Parts are joined by window_join_kernel.
+template <int DP>
+constexpr int win_waves() { return DP > 64 ? 4 : 8; }  // their rings fill 128 KB of LDS at most
 template <int DP, bool BF>
-__global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
+__global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(WinArgs a) {
     extern __shared__ __align__(256) char smem[];
-    constexpr int T = 32, RB = Rows<DP>::RB, TILE = T * RB, LOADS = T / Rows<DP>::PER;
+    constexpr int W = win_waves<DP>(), T = 32, RB = Rows<DP>::RB, TILE = T * RB, LOADS = T / Rows<DP>::PER;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = a.H / a.KV;
     int u = blockIdx.x;
@@ -1076,9 +1078,9 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
     int s = from + wave, buf = 0;
     win_arrived(q);
     if (s < to) issue(s, 0);
-    for (; s < to; s += 4, buf ^= 1) {
-        if (s + 4 < to) {
-            issue(s + 4, buf ^ 1);
+    for (; s < to; s += W, buf ^= 1) {
+        if (s + W < to) {
+            issue(s + W, buf ^ 1);
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1123,12 +1125,12 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
         });
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this buffer is free for the next load
     }
-    // the four waves' sums, in their order
+    // the waves' sums, in their order
     st.l = half_sum(st.l);
     __syncthreads();
     constexpr int LD = DP + 4;
     float* sums = reinterpret_cast<float*>(smem);  // [wave][row][LD]
-    float* ml = sums + 4 * 32 * LD;                // [wave][row][2]
+    float* ml = sums + W * 32 * LD;                // [wave][row][2]
     if (inside) {
 #pragma unroll
         for (int j = 0; j < DP / 32; ++j)
@@ -1140,13 +1142,13 @@ __global__ void __launch_bounds__(256, 1) window_cached_kernel(WinArgs a) {
     }
     __syncthreads();
     const int rows = a.rows - 32 * blk < 32 ? a.rows - 32 * blk : 32;
-    for (int e = tid; e < rows * (DP / 8); e += 256) {
+    for (int e = tid; e < rows * (DP / 8); e += 64 * W) {
         const int x = e / (DP / 8), d = 8 * (e - x * (DP / 8));
         float m = -__builtin_inff(), l = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[(w * 32 + x) * 2]);
+        for (int w = 0; w < W; ++w) m = fmaxf(m, ml[(w * 32 + x) * 2]);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float mw = ml[(w * 32 + x) * 2], f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
             l += f * ml[(w * 32 + x) * 2 + 1];
             if (mw != -__builtin_inff())
@@ -1322,7 +1324,8 @@ struct WinGrad {
 };
 template <int DP>
 constexpr int win_cached_lds() {
-    const int rings = 4 * 4 * 32 * Rows<DP>::RB, sums = 4 * 32 * (DP + 6) * 4;
+    constexpr int W = win_waves<DP>();
+    const int rings = W * 4 * 32 * Rows<DP>::RB, sums = W * 32 * (DP + 6) * 4;
     return rings > sums ? rings : sums;
 }
 struct WinCached {
@@ -1330,7 +1333,8 @@ struct WinCached {
     hipStream_t s;
     template <int DP, bool BF>
     hipError_t run() {
-        const hipError_t e = WIN_LAUNCH((window_cached_kernel<DP, BF>), a, (int64_t)a.B * a.KV * a.blocks * a.splits, 256, win_cached_lds<DP>(), s);
+        const hipError_t e = WIN_LAUNCH((window_cached_kernel<DP, BF>), a, (int64_t)a.B * a.KV * a.blocks * a.splits, 64 * win_waves<DP>(),
+                                        win_cached_lds<DP>(), s);
         if (e != hipSuccess || a.splits == 1) return e;
         WinJoin j = win_joined(a, a.part, a.N, a.N, a.H, a.splits);
         j.out[0] = a.out;
@@ -1400,13 +1404,18 @@ hipError_t launch_window_attention_grad(const rpfq_window_desc& d, const void* q
     return win_dispatch(d, WinGrad{a, s});
 }
 
-// Parts of the keys of one key head: as many as fill the chip four workgroups a
-// CU, each with 4 tiles (a tile a wave) or more.
+// Parts of the keys of one key head.  One where a wave has 5 tiles of 32 keys at
+// most: a second launch, to join, costs more than its share of them (a token of 8
+// streams, 12 heads of 64 over 1,028 slots: 14.8 us in 9 parts, 9.4 in one).
+// Else as many as fill the chip's workgroups, two at least for long ones, whose
+// lengths differ (64 streams, 4 key heads of 128 over 4,100 slots: 106 us in 2
+// parts, 118 in 4, 136 in 9), each of 4 tiles (a tile a wave) or more.
 int window_splits(const rpfq_window_desc& d) {
-    const int64_t blocks = ((d.H / d.KV) * d.N + 31) / 32, units = d.B * d.KV * blocks;
+    const int64_t blocks = ((d.H / d.KV) * d.N + 31) / 32, units = d.B * d.KV * blocks, waves = d.D > 64 ? 4 : 8;
     int64_t keys = d.window + d.N - 1 + d.sinks;
     keys = keys < d.M ? keys : d.M;
-    const int64_t most = (keys + 127) / 128, want = (4 * (int64_t)device_cus() + units - 1) / units;
+    if (keys <= 5 * 32 * waves) return 1;
+    const int64_t most = (keys + 127) / 128, fill = device_cus() / units, want = fill > 2 ? fill : 2;
     const int64_t s = most < want ? most : want;
     return (int)(s < 1 ? 1 : s > kWinSlots ? kWinSlots : s);
 }
