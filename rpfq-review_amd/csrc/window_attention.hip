@@ -206,13 +206,6 @@ __device__ __forceinline__ int win_length(const WinArgs& a, int b, int most) {
 // Keeps a rare branch one: without it the compiler computes both sides, the masks
 // of every tile among them.
 __device__ __forceinline__ void win_rare() { asm volatile(""); }
-// !seen, as a branch of its own: as the other side of the products' branch it
-// costs a copy of every sum a step.
-__device__ __forceinline__ bool win_unseen(int seen) {
-    seen = __builtin_amdgcn_readfirstlane(seen);
-    asm volatile("" : "+s"(seen));
-    return !seen;
-}
 // What a lane's query (key) sees of the keys (queries) in a block's result: those
 // from lo on, `len` more, and those up to `early` (the sinks).
 struct WinMask {
@@ -812,7 +805,8 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
 // of all heads that share them.  S = Q K^T and dP = dO V^T with a key to a lane:
 // P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS.  K stays in
 // registers, V in LDS (with both, 128-value heads spill); with two stages of Q
-// and dO that is 80 KB, two workgroups a CU.
+// and dO that is 80 KB, two workgroups a CU.  Heads up to 64: three, with fewer
+// fragments ahead (96 heads of 64 over 1,025 tokens 47 us, two a CU 53).
 constexpr int kWinKeys = 64, kWinStep = 64;
 template <int DP>
 constexpr int win_grad_lds() {
@@ -834,7 +828,7 @@ __device__ __forceinline__ void win_diff(std::integer_sequence<int, E...>, float
     ((dp[E] -= win_lane<E>(delta)), ...);
 }
 template <int DP, bool BF>
-__global__ void __launch_bounds__(256, DP > 64 ? 2 : 2) window_grad_kv_kernel(WinArgs a) {
+__global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(WinArgs a) {
     extern __shared__ __align__(256) char smem[];
     constexpr int RB = Rows<DP>::RB, V = kWinKeys * RB, STAGE = 2 * kWinStep * RB;  // V, two stages of Q and dO
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
@@ -869,7 +863,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 2) window_grad_kv_kernel(Wi
     float stat = 0.0f, delta = 0.0f, stat_next = 0.0f, delta_next = 0.0f;
     const int mine_q = 32 * half + acc_row(lane & 15, g);  // whose statistics this lane loads
     int64_t row = 0;
-    constexpr int LOADS = RowLoads<DP, kWinStep, 4>::LOADS;
     uint32_t to = lds;
     auto place = [&]() WIN_INLINE {
         const int first = q.at(qt) * kWinStep;
@@ -897,14 +890,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 2) window_grad_kv_kernel(Wi
         row += a.NP;
         ++head;
     };
-    auto load = [&](int x) WIN_INLINE {
-        if (x < LOADS) lq.load(x, to, wave);
-        else if (x < 2 * LOADS) lo_.load(x - LOADS, to + kWinStep * RB, wave);
-    };
-    auto issue = [&]() WIN_INLINE {
-        lq.issue(to, wave);
-        lo_.issue(to + kWinStep * RB, wave);
-    };
     if (steps) {
         RowLoads<DP, kWinKeys, 4> lv;
         lv.init(a.vs[1], a.D, wave, lane);
@@ -913,7 +898,8 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 2) window_grad_kv_kernel(Wi
         lv.issue(lds, wave);
         place();
         ready(0);
-        issue();
+        lq.issue(to, wave);
+        lo_.issue(to + kWinStep * RB, wave);
     }
     floatx16 ok[DP / 32], ov[DP / 32];
 #pragma unroll
@@ -928,9 +914,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 2) window_grad_kv_kernel(Wi
         stat = stat_next, delta = delta_next;
         ready(t + 1);
         const int seen = q0 < n ? span(q0, q0 + 31) : 0;
-        if (DP > 96) issue();  // no registers for them between the products
+        lq.issue(to, wave);  // between the products their sums would need registers
+        lo_.issue(to + kWinStep * RB, wave);
         if (seen) {
-        constexpr int NS = DP / 16, NJ = DP / 32, PD = 4, OUT = kWinStep * RB;
+        constexpr int NS = DP / 16, NJ = DP / 32, PD = DP > 64 ? 4 : 2, OUT = kWinStep * RB;
         const uint32_t vt = 32 * (block - half) * RB - V - (t & 1) * STAGE;  // V's rows from Q's
         // Q; dO and V in turn; dO and Q transposed
         auto read = [&](int e) WIN_INLINE {
@@ -942,7 +929,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 2) window_grad_kv_kernel(Wi
         uint4 pr, was;
         floatx16 s = floatx16{0}, dp = floatx16{0};
         win_stream<3 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
-            if (DP <= 96) load(e);
             if (e < NS) {
                 s = win_mma<BF>(f, kf[e], s);
                 return;
@@ -981,7 +967,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 2) window_grad_kv_kernel(Wi
             }
         });
         }
-        if (DP <= 96 && win_unseen(seen)) issue();
         at.move(t & 1 ? -STAGE : STAGE);
     }
     // the fellow's sums through LDS, one tensor after the other
