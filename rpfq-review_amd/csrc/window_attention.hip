@@ -29,8 +29,7 @@ struct Rows {
 
 // The loads of a tile of R rows by WAVES waves: rows of `ld` bytes, `left` of them
 // from the tile's first on; rows behind those and chunks past D as zeros.  The
-// scalar sums of an address are kept from tile to tile (they took a fifth of the
-// forward's step where each tile formed its own).
+// scalar sums of an address are kept from tile to tile.
 template <int DP, int R, int WAVES>
 struct RowLoads {
     static constexpr int TOTAL = R / Rows<DP>::PER, LOADS = (TOTAL + WAVES - 1) / WAVES;
@@ -49,26 +48,25 @@ struct RowLoads {
         at = reinterpret_cast<uint64_t>(base) + (uint64_t)first * (uint32_t)ld;
         left = n - first;
     }
-    // the tile's resource (off: none of it is loaded)
+    // the tile's resource
     intx4 rsrc;
-    __device__ __forceinline__ void resource(bool on) {
+    __device__ __forceinline__ void resource() {
         const int rows = left < R ? left : R;
         rsrc = (intx4){__builtin_amdgcn_readfirstlane((int)(uint32_t)at), __builtin_amdgcn_readfirstlane((int)((at >> 32) & 0xffff)),
-                       __builtin_amdgcn_readfirstlane(on && rows > 0 ? (rows - 1) * ld + bytes : 0), 0x00027000};
+                       __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * ld + bytes : 0), 0x00027000};
         asm volatile("" : "+v"(off));  // the loads' own sums stay in the loop: a register, not one each
     }
     // and on to the tile behind it
-    __device__ __forceinline__ void next(bool on) {
-        resource(on);
+    __device__ __forceinline__ void next() {
+        resource();
         at += (uint32_t)(R * ld);
         left -= R;
     }
-    // load p of the tile: the first waits for the resource's words, for all of them
     __device__ __forceinline__ void load(int p, uint32_t lds, int wave) const {
         if (TOTAL % WAVES && wave + p * WAVES >= TOTAL) return;
         const uint32_t to = lds + (wave + p * WAVES) * 1024;
         const uint32_t from = off + (uint32_t)(p * WAVES * Rows<DP>::PER * ld);
-        if (p == 0) dma_buffer(rsrc, from, to);
+        if (p == 0) dma_buffer(rsrc, from, to);  // waits for the resource's words, for all of them
         else asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(from), "s"(rsrc) : "memory", "m0");
     }
     __device__ __forceinline__ void issue(uint32_t lds, int wave) const {
@@ -106,9 +104,7 @@ struct Frags {
 };
 
 // A step's fragments in the order of their products, PD of them ahead: left to
-// itself the compiler reads each one right before its product and waits.  The next
-// tile's loads stand between the products (in one run behind the barrier they
-// held up the forward's wave for 800 of 3,100 clocks a step).
+// itself the compiler reads each one right before its product and waits.
 template <int N, int PD, class Read, class Use, int... E>
 __device__ __forceinline__ void win_each(uint4 (&ring)[PD], Read read, Use use, std::integer_sequence<int, E...>) {
     ((use(E, ring[E % PD]), E + PD < N ? (void)(ring[E % PD] = read(E + PD)) : (void)0, __builtin_amdgcn_sched_barrier(0)), ...);
@@ -348,8 +344,6 @@ __device__ __forceinline__ void win_arrived(uint4 (&f)[N]) {
 #pragma unroll
     for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s].x), "+v"(f[s].y), "+v"(f[s].z), "+v"(f[s].w));
 }
-// No load is on its way to LDS when its workgroup ends.
-__device__ __forceinline__ void win_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void win_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // c + a b where some of a are not finite: these count where their factor is not 0.
@@ -524,24 +518,14 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     Frags<DP> at;
     at.init(lds, lane);
     const WinSpan span = WinSpan::keys(a, p.mine, last, p.n);
-    // the loads of step s: ready(s), then load 0 .. 2 LOADS - 1
-    constexpr int LOADS = RowLoads<DP, T, 4>::LOADS;
-    uint32_t to = lds;
-    auto ready = [&](int s) WIN_INLINE {
+    auto issue = [&](int s) WIN_INLINE {
         if (s == 0 || tiles.leap(s)) {
             lk.seek(kbase, tiles.at(s) * T, p.n);
             lv.seek(vbase, tiles.at(s) * T, p.n);
         }
-        to = lds + (s & 1) * 2 * TILE;
-        lk.next(s < tiles.count);
-        lv.next(s < tiles.count);
-    };
-    auto load = [&](int x) WIN_INLINE {
-        if (x < LOADS) lk.load(x, to, wave);
-        else if (x < 2 * LOADS) lv.load(x - LOADS, to + TILE, wave);
-    };
-    auto issue = [&](int s) WIN_INLINE {
-        ready(s);
+        const uint32_t to = lds + (s & 1) * 2 * TILE;
+        lk.next();
+        lv.next();
         lk.issue(to, wave);
         lv.issue(to + TILE, wave);
     };
@@ -550,81 +534,77 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     floatx16 o[DP / 32];
     win_arrived(q);
     auto run = [&](auto careful) WIN_INLINE {
-    constexpr bool FAR = decltype(careful)::value;
-    win_sync();  // nothing of the run before is on its way to LDS
-    st = {-__builtin_inff(), -__builtin_inff(), 0.0f};
+        constexpr bool FAR = decltype(careful)::value;
+        st = {-__builtin_inff(), -__builtin_inff(), 0.0f};
 #pragma unroll
-    for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
-    if (tiles.count) issue(0);
-    for (int t = 0; t < tiles.count; ++t) {
-        win_sync();
-        ready(t + 1);
-        const int k0 = tiles.at(t) * T, seen = span(k0, k0 + T - 1);
-        if (!seen) {
-            lk.issue(to, wave);
-            lv.issue(to + TILE, wave);
-            at.move(t & 1 ? -2 * TILE : 2 * TILE);
-            continue;
-        }
-        constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = DP > 96 ? 8 : 6;
-        auto read = [&](int e) WIN_INLINE {
-            if (e < 2 * NS) return at.rows(e / NS * 32 * RB, e % NS);
-            return at.cols(TILE + (e - 2 * NS) / NJ * 16 * RB, (e - 2 * NS) % NJ);
-        };
-        auto hide = [&](floatx16& s, int kb) WIN_INLINE {
-            if (seen == 1)
-                mask(k0 + 32 * kb, g, k0 < a.sinks, [&](int v, bool in) WIN_INLINE { s[v] = in ? s[v] : -__builtin_inff(); });
-        };
-        auto anew = [&](float f) WIN_INLINE {
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) o[j][v] *= f;
-        };
-        uint4 pr;
-        floatx16 s[2];
-        s[0] = s[1] = floatx16{0};
-        float take = 0.0f;
-        // The products of one block and the other's softmax side by side: the second
-        // block's scores with the first's exponentials, the first's P V with the
-        // second's.
-        win_stream<2 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
-            load(e);
-            if (e < NS) {
-                s[0] = win_mma<BF>(f, q[e], s[0]);
-                return;
+        for (int j = 0; j < DP / 32; ++j) o[j] = floatx16{0};
+        if (tiles.count) issue(0);
+        for (int t = 0; t < tiles.count; ++t) {
+            win_sync();
+            if (t + 1 < tiles.count) issue(t + 1);
+            const int k0 = tiles.at(t) * T, seen = span(k0, k0 + T - 1);
+            if (!seen) {
+                at.move(t & 1 ? -2 * TILE : 2 * TILE);
+                continue;
             }
-            if (e < 2 * NS) {
-                const int x = e - NS;
-                s[1] = win_mma<BF>(f, q[x], s[1]);
-                if (x == 1) {
-                    hide(s[0], 0);
-                    take = win_top<BF, FAR>(s[0], st, a.scale2, anew);
+            constexpr int RB = Rows<DP>::RB, NS = DP / 16, NJ = DP / 32, PD = 4;
+            auto read = [&](int e) WIN_INLINE {
+                if (e < 2 * NS) return at.rows(e / NS * 32 * RB, e % NS);
+                return at.cols(TILE + (e - 2 * NS) / NJ * 16 * RB, (e - 2 * NS) % NJ);
+            };
+            auto hide = [&](floatx16& s, int kb) WIN_INLINE {
+                if (seen == 1)
+                    mask(k0 + 32 * kb, g, k0 < a.sinks, [&](int v, bool in) WIN_INLINE { s[v] = in ? s[v] : -__builtin_inff(); });
+            };
+            auto anew = [&](float f) WIN_INLINE {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) o[j][v] *= f;
+            };
+            uint4 pr;
+            floatx16 s[2];
+            s[0] = s[1] = floatx16{0};
+            float take = 0.0f;
+            // The products of one block and the other's softmax side by side: the second
+            // block's scores with the first's exponentials, the first's P V with the
+            // second's.
+            win_stream<2 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
+                if (e < NS) {
+                    s[0] = win_mma<BF>(f, q[e], s[0]);
+                    return;
                 }
-                constexpr int from = NS > 2 ? 2 : 1;
-                win_exp(s[0], win_piece(x, from, NS), win_piece(x + 1, from, NS), a.scale2, take);
-                return;
-            }
-            const int y = e - 2 * NS, u = y / NJ, j = y % NJ;
-            if (y == NJ)  // what is left of the first block is scaled with the rest
-                take = win_top<BF, FAR>(s[1], st, a.scale2, [&](float f_) WIN_INLINE {
-                    anew(f_);
+                if (e < 2 * NS) {
+                    const int x = e - NS;
+                    s[1] = win_mma<BF>(f, q[x], s[1]);
+                    if (x == 1) {
+                        hide(s[0], 0);
+                        take = win_top<BF, FAR>(s[0], st, a.scale2, anew);
+                    }
+                    constexpr int from = NS > 2 ? 2 : 1;
+                    win_exp(s[0], win_piece(x, from, NS), win_piece(x + 1, from, NS), a.scale2, take);
+                    return;
+                }
+                const int y = e - 2 * NS, u = y / NJ, j = y % NJ;
+                if (y == NJ)  // what is left of the first block is scaled with the rest
+                    take = win_top<BF, FAR>(s[1], st, a.scale2, [&](float f_) WIN_INLINE {
+                        anew(f_);
 #pragma unroll
-                    for (int v = 8; v < 16; ++v) s[0][v] *= f_;
-                });
-            if (j == 0) {
-                pr = win_pack8<BF>(s[u >> 1], u & 1);
-                // the sum of the rounded probabilities: their rounding errors then
-                // weigh the values' distance to the output, not the values
-                st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
-            }
-            o[j] = FAR ? win_mma_some<BF>(f, pr, o[j]) : win_mma<BF>(f, pr, o[j]);
-            if (y == 0) hide(s[1], 1);
-            if (u == 1 || u == 2) win_exp(s[1], 8 * (y - NJ) / NJ, 8 * (y + 1 - NJ) / NJ, a.scale2, take);
-        });
-        at.move(t & 1 ? -2 * TILE : 2 * TILE);
-    }
-    at.move(tiles.count & 1 ? -2 * TILE : 0);  // to the first stage again
+                        for (int v = 8; v < 16; ++v) s[0][v] *= f_;
+                    });
+                if (j == 0) {
+                    pr = win_pack8<BF>(s[u >> 1], u & 1);
+                    // the sum of the rounded probabilities: their rounding errors then
+                    // weigh the values' distance to the output, not the values
+                    st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
+                }
+                o[j] = FAR ? win_mma_some<BF>(f, pr, o[j]) : win_mma<BF>(f, pr, o[j]);
+                if (y == 0) hide(s[1], 1);
+                if (u == 1 || u == 2) win_exp(s[1], 8 * (y - NJ) / NJ, 8 * (y + 1 - NJ) / NJ, a.scale2, take);
+            });
+            at.move(t & 1 ? -2 * TILE : 2 * TILE);
+        }
+        at.move(tiles.count & 1 ? -2 * TILE : 0);  // to the first stage again
     };
     run(std::false_type());
     // Scores past 2^20, or a value that is not finite (a product with a probability
@@ -635,7 +615,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
 #pragma unroll
         for (int v = 0; v < 16; ++v) odd = fmaf(o[j][v], 0.0f, odd);
     if (__builtin_expect(__syncthreads_or(!(odd == 0.0f)), 0)) run(std::true_type());
-    win_landed();
     const float l = half_sum(st.l);
     const bool any = l != 0.0f && i < p.n;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
@@ -712,24 +691,14 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
     Frags<DP> at;
     at.init(lds, lane);
     const WinSpan span = WinSpan::keys(a, p.mine, last, p.n);
-    // the loads of step s: ready(s), then load 0 .. 2 LOADS - 1
-    constexpr int LOADS = RowLoads<DP, T, 4>::LOADS;
-    uint32_t to = lds;
-    auto ready = [&](int s) WIN_INLINE {
+    auto issue = [&](int s) WIN_INLINE {
         if (s == 0 || tiles.leap(s)) {
             lk.seek(kbase, tiles.at(s) * T, p.n);
             lv.seek(vbase, tiles.at(s) * T, p.n);
         }
-        to = lds + (s & 1) * 2 * TILE;
-        lk.next(s < tiles.count);
-        lv.next(s < tiles.count);
-    };
-    auto load = [&](int x) WIN_INLINE {
-        if (x < LOADS) lk.load(x, to, wave);
-        else if (x < 2 * LOADS) lv.load(x - LOADS, to + TILE, wave);
-    };
-    auto issue = [&](int s) WIN_INLINE {
-        ready(s);
+        const uint32_t to = lds + (s & 1) * 2 * TILE;
+        lk.next();
+        lv.next();
         lk.issue(to, wave);
         lv.issue(to + TILE, wave);
     };
@@ -744,11 +713,9 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
     if (tiles.count) issue(0);
     for (int t = 0; t < tiles.count; ++t) {
         win_sync();
-        ready(t + 1);
+        if (t + 1 < tiles.count) issue(t + 1);
         const int k0 = tiles.at(t) * T, seen = span(k0, k0 + T - 1);
         if (!seen) {
-            lk.issue(to, wave);
-            lv.issue(to + TILE, wave);
             at.move(t & 1 ? -2 * TILE : 2 * TILE);
             continue;
         }
@@ -770,7 +737,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
             dp = floatx16{0};
         };
         win_stream<4 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
-            load(e);
             const int kb = e / (2 * NS), x = e % NS;
             if (e < 4 * NS) {
                 if (e / NS & 1) {
@@ -789,7 +755,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
         });
         at.move(t & 1 ? -2 * TILE : 2 * TILE);
     }
-    win_landed();
     const float f = (BF ? 1.0f : 0x1p-15f) / c;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
         const int64_t slot = (((int64_t)p.b * a.far.rows + i) * a.H + p.h) * (a.far.parts + 1) + p.unit.part;
@@ -863,7 +828,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
     float stat = 0.0f, delta = 0.0f, stat_next = 0.0f, delta_next = 0.0f;
     const int mine_q = 32 * half + acc_row(lane & 15, g);  // whose statistics this lane loads
     int64_t row = 0;
-    uint32_t to = lds;
     auto place = [&]() WIN_INLINE {
         const int first = q.at(qt) * kWinStep;
         lq.seek(a.q + b * a.qs[0] + kv * group * a.qs[2], first, n);
@@ -871,20 +835,19 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
         row = ((int64_t)b * a.H + kv * group) * a.NP + first;
         q0_next = first + 32 * half;
     };
-    auto ready = [&](int s) WIN_INLINE {
-        to = lds + V + (s & 1) * STAGE;
-        q0 = q0_next;
-        if (s < steps) {
-            if (head == group) {
-                head = 0;
-                ++qt;
-                place();
-            }
-            stat_next = a.stat[row + mine_q];
-            delta_next = a.delta[row + mine_q];
+    auto issue = [&](int s) WIN_INLINE {
+        const uint32_t to = lds + V + (s & 1) * STAGE;
+        if (head == group) {
+            head = 0;
+            ++qt;
+            place();
         }
-        lq.resource(s < steps);
-        lo_.resource(s < steps);
+        stat_next = a.stat[row + mine_q];
+        delta_next = a.delta[row + mine_q];
+        lq.resource();
+        lo_.resource();
+        lq.issue(to, wave);
+        lo_.issue(to + kWinStep * RB, wave);
         lq.at += a.qs[2];
         lo_.at += a.gos[2];
         row += a.NP;
@@ -894,12 +857,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
         RowLoads<DP, kWinKeys, 4> lv;
         lv.init(a.vs[1], a.D, wave, lane);
         lv.seek(a.v + b * a.vs[0] + kv * a.vs[2], k0, n);
-        lv.resource(true);
+        lv.resource();
         lv.issue(lds, wave);
         place();
-        ready(0);
-        lq.issue(to, wave);
-        lo_.issue(to + kWinStep * RB, wave);
+        issue(0);
     }
     floatx16 ok[DP / 32], ov[DP / 32];
 #pragma unroll
@@ -912,60 +873,59 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
         win_sync();
         asm volatile("" : "+v"(stat_next), "+v"(delta_next));
         stat = stat_next, delta = delta_next;
-        ready(t + 1);
+        q0 = q0_next;
+        if (t + 1 < steps) issue(t + 1);
         const int seen = q0 < n ? span(q0, q0 + 31) : 0;
-        lq.issue(to, wave);  // between the products their sums would need registers
-        lo_.issue(to + kWinStep * RB, wave);
         if (seen) {
-        constexpr int NS = DP / 16, NJ = DP / 32, PD = DP > 64 ? 4 : 2, OUT = kWinStep * RB;
-        const uint32_t vt = 32 * (block - half) * RB - V - (t & 1) * STAGE;  // V's rows from Q's
-        // Q; dO and V in turn; dO and Q transposed
-        auto read = [&](int e) WIN_INLINE {
-            if (e < NS) return at.rows(0, e);
-            if (e < 3 * NS) return at.rows((e - NS) & 1 ? vt : OUT, (e - NS) / 2);
-            const int x = e - 3 * NS;
-            return at.cols((x < 2 * NJ ? OUT : 0) + x / NJ % 2 * 16 * RB, x % NJ);
-        };
-        uint4 pr, was;
-        floatx16 s = floatx16{0}, dp = floatx16{0};
-        win_stream<3 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
-            if (e < NS) {
-                s = win_mma<BF>(f, kf[e], s);
-                return;
-            }
-            if (e < 3 * NS) {
-                if (!((e - NS) & 1)) {
-                    was = f;
+            constexpr int NS = DP / 16, NJ = DP / 32, PD = DP > 64 ? 4 : 2, OUT = kWinStep * RB;
+            const uint32_t vt = 32 * (block - half) * RB - V - (t & 1) * STAGE;  // V's rows from Q's
+            // Q; dO and V in turn; dO and Q transposed
+            auto read = [&](int e) WIN_INLINE {
+                if (e < NS) return at.rows(0, e);
+                if (e < 3 * NS) return at.rows((e - NS) & 1 ? vt : OUT, (e - NS) / 2);
+                const int x = e - 3 * NS;
+                return at.cols((x < 2 * NJ ? OUT : 0) + x / NJ % 2 * 16 * RB, x % NJ);
+            };
+            uint4 pr, was;
+            floatx16 s = floatx16{0}, dp = floatx16{0};
+            win_stream<3 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
+                if (e < NS) {
+                    s = win_mma<BF>(f, kf[e], s);
                     return;
                 }
-                dp = win_mma<BF>(was, f, dp);
-                if (e == 3 * NS - 1) {
-                    win_probs(std::make_integer_sequence<int, 16>(), s, a.scale2, stat);
-                    if (seen == 1)
-                        mask(q0, g, !a.causal && q0 < a.sinks, [&](int v, bool in) WIN_INLINE { s[v] = in ? s[v] : 0.0f; });
-                }
-                return;
-            }
-            const int x = e - 3 * NS, j = x % NJ;
-            if (x < 2 * NJ) {
-                if (j == 0) pr = win_pack8<BF>(s, x / NJ);
-                ov[j] = win_mma<BF>(f, pr, ov[j]);
-                if (x == 1) {
-                    win_diff(std::make_integer_sequence<int, 16>(), dp, delta);
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) dp[v] *= s[v];
-                    if (seen == 1) {
-                        win_rare();
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) dp[v] = s[v] == 0.0f ? 0.0f : dp[v];
+                if (e < 3 * NS) {
+                    if (!((e - NS) & 1)) {
+                        was = f;
+                        return;
                     }
+                    dp = win_mma<BF>(was, f, dp);
+                    if (e == 3 * NS - 1) {
+                        win_probs(std::make_integer_sequence<int, 16>(), s, a.scale2, stat);
+                        if (seen == 1)
+                            mask(q0, g, !a.causal && q0 < a.sinks, [&](int v, bool in) WIN_INLINE { s[v] = in ? s[v] : 0.0f; });
+                    }
+                    return;
                 }
-            } else {
-                if (x == 2 * NJ) win_scale_ds<DP, BF>(dp, c, ok);
-                if (j == 0) pr = win_pack8<BF>(dp, x / NJ % 2);
-                ok[j] = win_mma<BF>(f, pr, ok[j]);
-            }
-        });
+                const int x = e - 3 * NS, j = x % NJ;
+                if (x < 2 * NJ) {
+                    if (j == 0) pr = win_pack8<BF>(s, x / NJ);
+                    ov[j] = win_mma<BF>(f, pr, ov[j]);
+                    if (x == 1) {
+                        win_diff(std::make_integer_sequence<int, 16>(), dp, delta);
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) dp[v] *= s[v];
+                        if (seen == 1) {
+                            win_rare();
+#pragma unroll
+                            for (int v = 0; v < 16; ++v) dp[v] = s[v] == 0.0f ? 0.0f : dp[v];
+                        }
+                    }
+                } else {
+                    if (x == 2 * NJ) win_scale_ds<DP, BF>(dp, c, ok);
+                    if (j == 0) pr = win_pack8<BF>(dp, x / NJ % 2);
+                    ok[j] = win_mma<BF>(f, pr, ok[j]);
+                }
+            });
         }
         at.move(t & 1 ? -STAGE : STAGE);
     }
