@@ -851,7 +851,7 @@ typedef struct rpfq_window_desc {
     int64_t out_stride[3];  /* cached: contiguous */
     int64_t grad_stride[3]; /* of grad_out */
     int32_t dtype, causal;
-    float scale;            /* positive and finite */
+    float scale;            /* positive, below 2^126 */
 } rpfq_window_desc;
 
 /* stat (out, float32, 256-byte aligned, rpfq_window_attention_stat_bytes; NULL: not

@@ -877,9 +877,11 @@ static int check_window(const rpfq_window_desc* d, bool cached) {
         d->B * d->H * (d->N / 32 + 4) > (1LL << 30))
         return fail(RPFQ_ERR_SHAPE, "takes up to 2^28 tokens, 2^24 heads of a batch and 2^30 of 32 rows each (B=%lld N=%lld H=%lld M=%lld)",
                     (long long)d->B, (long long)d->N, (long long)d->H, (long long)d->M);
+    if (cached && d->N * d->H > (1LL << 30))
+        return fail(RPFQ_ERR_SHAPE, "cached: takes up to 2^30 rows of a sequence (N=%lld H=%lld)", (long long)d->N, (long long)d->H);
     if (d->window < 1 || d->sinks < 0) return fail(RPFQ_ERR_VALUE, "window=%lld must be positive, sinks=%lld not negative", (long long)d->window, (long long)d->sinks);
     if (d->causal & ~1) return fail(RPFQ_ERR_VALUE, "causal must be 0 or 1");
-    if (!(d->scale > 0.0f && d->scale < INFINITY)) return fail(RPFQ_ERR_VALUE, "scale=%g must be positive and finite", (double)d->scale);
+    if (!(d->scale > 0.0f && d->scale < 0x1p126f)) return fail(RPFQ_ERR_VALUE, "scale=%g must be positive and below 2^126", (double)d->scale);
     return RPFQ_OK;
 }
 // strides that the kernels index by: whole 16-byte pieces, 128 rows of a tile within 31 bits

@@ -1419,7 +1419,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     qkv tensor are read as they lie; heads that are not in one 16-byte aligned
     piece, or of no multiple of 8 values, are copied.  Scores and sums in
     float32, probabilities rounded to q's type.  A value that is not finite
-    makes the outputs of queries near it NaN too, whether they see it or not.
+    reaches the outputs of the queries that see it and no others; gradients of
+    rows near it may be NaN too.
     Gradients of q, k and v, once differentiable, sums in a fixed order; they
     need the native host path (csrc/host.cpp); can be captured as rms_norm can."""
     host = N.host()
@@ -1430,7 +1431,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
             return out
     q2, k2, v2, lengths, scale = _window_operands("window_attention", q, k, v, lengths, window, sinks, scale, False)
     if q.numel() == 0:
-        return q2 + 0.0
+        return q + 0.0 * (k.sum() + v.sum())
     if host is not None:
         out = host.window_attention(q2, k2, v2, lengths, min(int(window), 1 << 40), min(int(sinks), 1 << 40), scale, causal)
         if out is not None:

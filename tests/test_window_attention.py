@@ -250,7 +250,7 @@ def test_strides_streams_and_odd_layouts(dtype, host_path):
         got = ops.window_attention(*parts, 20, 2)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got, want)
-    for empty in (qkv[:0], qkv[:, :0]):
+    for empty in (qkv[:0], qkv[:, :0], qkv[:0, ..., :17]):
         assert ops.window_attention(*empty.unbind(2), 20, 2).shape == empty[:, :, 0].shape
     # a window and sinks past every length, past 32 bits and past 64
     for far in (70, 1 << 33, 1 << 70):
@@ -493,6 +493,7 @@ def test_argument_errors():
         for name in ("q_stride", "k_stride", "v_stride"):
             assert call(**{name: (1, 256, 64)}) == 3 and call(**{name: (8, 1 << 22, 64)}) == 3 and call(**{name: (8, -8, 64)}) == 3
         assert call(lens=at + 2) == 3
+    assert cached(N=1 << 21, H=1024, KV=1) == 2 and fwd(scale=2.0 ** 126) == 6
     assert fwd(M=5) == 2 and grad(M=5) == 2 and cached(M=0) == 2 and cached(M=1 << 29) == 2
     assert fwd(stat=at + 64) == 3 and fwd(out_stride=(8, 4, 8)) == 3
     assert grad(go=None) == 1 and grad(stat=None) == 1 and grad(work=None) == 1 and grad(gq=None, gk=None, gv=None) == 1
