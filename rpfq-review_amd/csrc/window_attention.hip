@@ -877,7 +877,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
         if (t + 1 < steps) issue(t + 1);
         const int seen = q0 < n ? span(q0, q0 + 31) : 0;
         if (seen) {
-            constexpr int NS = DP / 16, NJ = DP / 32, PD = DP > 64 ? 4 : 2, OUT = kWinStep * RB;
+            constexpr int NS = DP / 16, NJ = DP / 32, PD = 2, OUT = kWinStep * RB;
             const uint32_t vt = 32 * (block - half) * RB - V - (t & 1) * STAGE;  // V's rows from Q's
             // Q; dO and V in turn; dO and Q transposed
             auto read = [&](int e) WIN_INLINE {
