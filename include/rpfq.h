@@ -822,7 +822,7 @@ typedef struct rpfq_rotary_desc {
  * Pair j of every head turned by position[token][axis of j] freqs[j] radians
  * (freqs [sum(sections)] float64 in device memory; the angle in 64 bits, the rest
  * float32, rounded once): (u, v) -> (u cos - v sin, v cos + u sin); the values
- * behind the pairs are copied.  Outputs may be the inputs themselves.  No
+ * behind the pairs are copied.  Outputs may be the inputs themselves, if these share no element.  No
  * counterpart in the reference, whose positions are learned and added.
  */
 int rpfq_rotary(const rpfq_rotary_desc* desc, const void* q, const void* k, void* q_out, void* k_out,

@@ -498,7 +498,10 @@ __device__ __forceinline__ void win_part(float* dst, const floatx16 (&o)[DP / 32
 // Forward.  S^T = K Q^T: a lane holds one query's scores, so the softmax is
 // in-lane but for one exchange, and the probabilities, rounded to 16 bits, are
 // already the operand of O^T = V^T P^T.  K and V tiles of 64 keys go to LDS by
-// DMA, the next one while this one is used.
+// DMA, the next one while this one is used.  Bound by the products for heads of
+// 128 (8,192 tokens, 16 heads on 4, window 1,024, bf16: 88 us, 0.87 PFLOP/s of what
+// the tiles compute), by exponentials, masks and first loads for heads of 64 (96
+// heads, 1,025 tokens, 127 to both sides: 29 us).
 template <int DP, bool BF>
 __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_forward_kernel(WinArgs a) {
     extern __shared__ __align__(256) char smem[];
@@ -658,7 +661,8 @@ __device__ __forceinline__ void win_scale_ds(floatx16& ds, float& c, floatx16 (&
 }
 
 // Gradient of the queries, laid out as the forward: S^T = K Q^T and dP^T = V dO^T
-// in one lane's query, dQ^T = K^T dS^T.  Leaves rowsum(dO O) for the other.
+// in one lane's query, dQ^T = K^T dS^T.  Leaves rowsum(dO O) for the other.  Of
+// the forward's sizes 114 us (1.0 PFLOP/s) and 39.
 template <int DP, bool BF>
 __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(WinArgs a) {
     extern __shared__ __align__(256) char smem[];
@@ -771,7 +775,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
 // P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS.  K stays in
 // registers, V in LDS (with both, 128-value heads spill); with two stages of Q
 // and dO that is 80 KB, two workgroups a CU.  Heads up to 64: three, with fewer
-// fragments ahead (96 heads of 64 over 1,025 tokens 47 us, two a CU 53).
+// fragments ahead (96 heads of 64 over 1,025 tokens 46 us, two a CU 53).  The long
+// case of the forward 170 us (0.87 PFLOP/s), its sinks' far queries in parts (in
+// their tile's own workgroup: 1,276).  Statistics come by lane broadcasts: a
+// 128-bit LDS read of one address by half a wave took 24 clocks.
 constexpr int kWinKeys = 64, kWinStep = 64;
 template <int DP>
 constexpr int win_grad_lds() {
@@ -971,7 +978,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
 // The last tokens over a cache.  A workgroup has one key head of one sequence,
 // up to 32 of its rows (queries x heads that share it) and a part of the keys; its
 // waves take tiles of 32 keys in turn, each through LDS of its own, without
-// waiting for each other.  Parts are joined by window_join_kernel.
+// waiting for each other.  Parts are joined by window_join_kernel.  Bound by HBM
+// (64 streams, 4 key heads of 128, 4,100 slots, bf16: 102 us, 5.3 TB/s), at few
+// heads by a wave's tiles, one read's latency behind the other (8 streams, 12 heads
+// of 64, 1,028 slots 10 us).
 template <int DP>
 constexpr int win_waves() { return DP > 64 ? 4 : 8; }  // their rings fill 128 KB of LDS at most
 template <int DP, bool BF>

@@ -1267,6 +1267,31 @@ def _apart(t: torch.Tensor) -> bool:
     return True
 
 
+def _apart_from(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether a's and b's elements surely share none: other memory, or, with the
+    same strides, places of their own side by side (q and k of a qkv tensor)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return True
+
+    def ends(t):
+        return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+    (a0, a1), (b0, b1) = ends(a), ends(b)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    if a.stride() != b.stride() or a0 == b0:
+        return False
+    shape = [2, *(max(n, m) for n, m in zip(a.shape, b.shape))]
+    stride = [abs(a0 - b0) // a.element_size(), *a.stride()]
+    span = 1
+    for size, step in sorted(zip(shape, stride), key=lambda e: e[1]):
+        if size > 1:
+            if step < span:
+                return False
+            span += step * (size - 1)
+    return True
+
+
 def rotary(x, positions: torch.Tensor, freqs: torch.Tensor, sections=None, *, interleaved: bool = False,
            inplace: bool = False):
     """Rotary positions of several axes (rpfq_rotary): pair j of every head of x
@@ -1325,6 +1350,8 @@ def rotary(x, positions: torch.Tensor, freqs: torch.Tensor, sections=None, *, in
             raise RuntimeError("rotary: inplace takes no part in autograd")
         if not all(t.stride(3) == 1 and _apart(t) for t in xs if t.numel()):
             raise ValueError("rotary: inplace takes tensors whose heads lie in one piece each, none over another")
+        if len(xs) > 1 and not _apart_from(*xs):
+            raise ValueError("rotary: inplace takes q and k that share no elements")
     if q.numel() == 0 and (one or xs[1].numel() == 0):
         out = xs if inplace else tuple(t.clone() for t in xs)
         return out[0] if one else out

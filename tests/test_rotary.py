@@ -245,3 +245,24 @@ def test_argument_errors():
     assert call(sections=(0, 0)) == 2 and call(sections=(-1, 9)) == 6 and call(axes=0) == 6 and call(axes=5) == 6
     assert call(interleaved=2) == 6 and call(inverse=-1) == 6
     assert call(q=at + 1) == 3 and call(ko=at + 1) == 3 and call(freqs=at + 4) == 3 and call(pos=at + 4) == 3
+
+
+@pytest.mark.gpu
+def test_inplace_refuses_tensors_over_each_other(host_path):
+    """q and k that share elements would be turned twice, or not, as it comes."""
+    from quant_models import ops
+
+    freqs, pos = _freqs((8,)), torch.arange(6, device=DEV)
+    qkv = torch.randn(2, 6, 3, 4, 16, device=DEV)
+    packed = torch.randn(2, 6, 8, 16, device=DEV)  # 4 heads of q, 2 of k, 2 of v
+    q, k = qkv[:, :, 0], qkv[:, :, 1]
+    for pair in ((q, q), (qkv[:, :, 0], qkv[:, :, 0, :2]), (packed[:, :, :4], packed[:, :, 3:5]),
+                 (packed[:, :4, :4], packed[:, 2:, :4])):
+        with pytest.raises(ValueError, match="inplace"):
+            n = pair[0].shape[1]
+            ops.rotary(pair, pos[:n], freqs, inplace=True)
+    for pair in ((q, k), (packed[:, :, :4], packed[:, :, 4:6]), (qkv[0:1, :, 0], qkv[1:2, :, 0]), (qkv[:, :3, 0], qkv[:, 3:, 0])):
+        n = pair[0].shape[1]
+        want = ops.rotary(tuple(t.clone() for t in pair), pos[:n], freqs)
+        ops.rotary(pair, pos[:n], freqs, inplace=True)
+        assert all(torch.equal(t, w) for t, w in zip(pair, want))

@@ -505,3 +505,41 @@ def test_argument_errors():
     assert need(desc(False), 0) == 0 and need(desc(False), 1) >= size and need(desc(False, N=0), 1) == 0
     assert grad(nb=need(desc(False), 1) - 1) == 2
     assert cached(lens=None) == 1 and L.rpfq_window_attention_cached_workspace_bytes(desc(True, window=0)) == 0
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A sequence inside a qkv tensor of more than 4 GiB, and caches as long: the last
+    rows against the definition on what they see."""
+    from quant_models import ops
+
+    n, heads, d, window, sinks = 960_000, 12, 64, 40, 3
+    g = _gen(31)
+    qkv = torch.randn(1, n, 3, heads, d, generator=g, device=DEV, dtype=torch.float16)
+    assert qkv.numel() * 2 > 1 << 32
+    q, k, v = qkv.unbind(2)
+    tail = 2 * window
+    near = torch.cat([torch.arange(sinks, device=DEV), torch.arange(n - tail, n, device=DEV)])
+    i = torch.arange(n - window, n, device=DEV)
+    seen = _seen(i[:, None], near[None], window, sinks, True)
+    want = [_head(q[0, i, y].double(), k[0, near, y].double(), v[0, near, y].double(), seen, d ** -0.5, HALF[q.dtype])[0] for y in range(heads)]
+    values, bounds = (torch.stack([w[t] for w in want], 1)[None] for t in range(2))
+    with torch.no_grad():
+        out = ops.window_attention(q, k, v, window, sinks)
+        _check(out[:, -window:], values, bounds)
+        assert bool(out[:, :: n // 64].isfinite().all())
+        del out
+        lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+        got = ops.window_attention_cached(q[:, -window:], k, v, lens, window, sinks)
+    _check(got, values, bounds)
+    # the gradient of the last row: of its own window's keys, and of the sinks
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    go = torch.zeros(1, n, heads, d, device=DEV, dtype=torch.float16)
+    go[:, -1] = torch.randn(heads, d, generator=g, device=DEV).half()
+    grads = torch.autograd.grad(ops.window_attention(*leaves, window, sinks), leaves, go)
+    for y in range(heads):
+        one = _head(q[0, -1:, y].double(), k[0, near, y].double(), v[0, near, y].double(), seen[-1:], d ** -0.5, HALF[q.dtype], go[0, -1:, y].double())
+        _check(grads[0][0, -1:, y], *one[1], rounding=HALF[q.dtype])
+        for got, w in zip(grads[1:], one[2:]):
+            _check(got[0, near, y], *w, rounding=HALF[q.dtype])
+    assert not bool(grads[1][0, sinks:n - tail:9973].any()) and not bool(grads[0][0, : n - 1 : 9973].any())
