@@ -822,8 +822,9 @@ typedef struct rpfq_rotary_desc {
  * Pair j of every head turned by position[token][axis of j] freqs[j] radians
  * (freqs [sum(sections)] float64 in device memory; the angle in 64 bits, the rest
  * float32, rounded once): (u, v) -> (u cos - v sin, v cos + u sin); the values
- * behind the pairs are copied.  Outputs may be the inputs themselves, if these share no element.  No
- * counterpart in the reference, whose positions are learned and added.
+ * behind the pairs are copied.  Outputs may be the inputs themselves, if q and k
+ * share no element.  No counterpart in the reference, whose positions are learned
+ * and added.
  */
 int rpfq_rotary(const rpfq_rotary_desc* desc, const void* q, const void* k, void* q_out, void* k_out,
                 const void* positions, const double* freqs, void* stream);
