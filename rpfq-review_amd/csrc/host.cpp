@@ -769,7 +769,10 @@ struct Window : torch::autograd::Function<Window> {
         const auto options = q.options().requires_grad(false);
         at::Tensor out = at::empty(q.sizes(), options), st;
         window_strides(out, d.out_stride);
-        if (stat) st = at::empty({(int64_t)(api.rpfq_window_attention_stat_bytes(&d) / 4)}, options.dtype(at::kFloat));
+        if (stat) {  // both of its arrays
+            st = at::empty({2, (int64_t)(api.rpfq_window_attention_stat_bytes(&d) / 4)}, options.dtype(at::kFloat));
+            d.top = st[1].data_ptr<float>();
+        }
         const size_t bytes = api.rpfq_window_attention_workspace_bytes(&d, 0);
         at::Tensor work;
         if (bytes) work = at::empty({(int64_t)bytes}, options.dtype(at::kByte));
@@ -801,6 +804,7 @@ struct Window : torch::autograd::Function<Window> {
             const at::NoGradGuard plain_results;
             const at::Tensor go = window_rows16(grads[0]) ? grads[0] : grads[0].clone(at::MemoryFormat::Contiguous);
             window_strides(go, d.grad_stride);
+            d.top = const_cast<float*>(stat.const_data_ptr<float>()) + stat.size(1);
             const at::Tensor* in[3] = {&q, &k, &v};
             for (int i = 0; i < 3; ++i)
                 if (ctx->needs_input_grad(i)) g[i] = at::empty(in[i]->sizes(), q.options().requires_grad(false));

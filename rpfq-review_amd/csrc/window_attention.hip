@@ -4,7 +4,9 @@
 //   causal:  j <= i and (i - j < window or j < sinks),
 //   else:    |i - j| < window or j < sinks or i < sinks;
 //   O = P V,  P = softmax(scale Q K^T) over what is seen, 0 for a row without any.
-// Gradient, with P = exp(S - lse) formed again from the row's statistic:
+// Gradient, with P formed again from two numbers a row, a score and log2 of the
+// sum relative to it: P = exp2((S - top) scale2 - lg), scale2 = scale log2(e).
+// Their sum in one number would be rounded at the scores' size, and P with it.
 //   dV = P^T dO,  dS = P (dO V^T - rowsum(dO O)),  dQ = scale dS K,  dK = scale dS^T Q.
 #include "tile_gemm.h"
 
@@ -183,7 +185,7 @@ struct WinArgs {
     char *out, *gq, *gk, *gv;
     int64_t qs[3], ks[3], vs[3], os[3], gos[3];  // bytes between batches, tokens, heads
     const int32_t* lengths;
-    float *stat, *delta;                // [B, H, NP]
+    float *top, *stat, *delta;          // [B, H, NP]; stat: lg
     int B, N, H, KV, D, NP;
     int window, sinks, causal;
     int hw, qw, tiles;                  // heads and 32-query blocks of a workgroup; query tiles
@@ -381,7 +383,7 @@ __device__ __forceinline__ float half_sum(float v) {
 
 // The running softmax of a lane's query over blocks of 32 keys (two lanes hold one
 // query's scores, half each): `top` the score that is subtracted, `sub` = top
-// scale2 + shift as it is rounded; l the sum.  top follows the largest score only
+// scale2 + shift as it is rounded; l the sum, times 2^-win_rel relative to top.  top follows the largest score only
 // where that passes it by 2^kWinLag, so that the sums are hardly ever scaled anew.
 struct WinState {
     float top, sub, l;
@@ -416,11 +418,22 @@ __device__ __forceinline__ float win_top(floatx16& s, WinState& st, float scale2
     }
     return none ? 0.0f : st.sub;
 }
+// log2 of what a block's sums stand under, from exp2((S - top) scale2) on: the shift,
+// with the rounding of `sub` where that was subtracted.
+template <bool BF, bool FAR>
+__device__ __forceinline__ float win_rel(const WinState& st, float scale2) {
+    return FAR || st.top == -__builtin_inff() ? win_shift<BF>() : fmaf(-st.top, scale2, st.sub);
+}
 // P of scores LO .. HI - 1
 __device__ __forceinline__ void win_exp(floatx16& s, int lo, int hi, float scale2, float sub) {
 #pragma unroll
     for (int v = 0; v < 16; ++v)
         if (v >= lo && v < hi) s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], scale2, -sub));
+}
+__device__ __forceinline__ void win_exp_from(floatx16& s, int lo, int hi, float top, float scale2, float lg) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v)
+        if (v >= lo && v < hi) s[v] = __builtin_amdgcn_exp2f(fmaf(s[v] - top, scale2, -lg));
 }
 // Where the 16 exponentials of a block stand among N products, the first `from` without.
 constexpr int win_piece(int x, int from, int n) { return x < from ? 0 : x >= n ? 16 : 16 * (x - from) / (n - from); }
@@ -483,16 +496,25 @@ __device__ __forceinline__ WinTiles win_keys(const WinArgs& a, const WinPlace& p
     return win_share(a.far, p.unit, win_tiles<T>(a, p.q0, p.q1, p.n), (p.q0 + 32 * a.qw + a.window + T - 1) / T, p.q1 < p.q0 ? 0 : (p.n + T - 1) / T);
 }
 
-// 32 rows of DP results as a slot of their float32 sums: `o` times f, and two
-// numbers behind them.
+// A row's two numbers for the gradient's probabilities, which fp16 has times 2^15;
+// a row without any has probabilities of 0.
+template <bool BF>
+__device__ __forceinline__ void win_stat(float* top, float* stat, int64_t at, bool any, float score, float lg) {
+    top[at] = any ? score : 0.0f;
+    stat[at] = any ? lg - (BF ? 0.0f : 15.0f) : __builtin_inff();
+}
+
+// 32 rows of DP results as a slot of their float32 sums: `o` times f, and three
+// numbers behind them: the score and the sum that they are relative to, and what
+// win_rel differs from the shift by.
 template <int DP>
-__device__ __forceinline__ void win_part(float* dst, const floatx16 (&o)[DP / 32], float f, float x, float y, int g) {
+__device__ __forceinline__ void win_part(float* dst, const floatx16 (&o)[DP / 32], float f, float top, float l, float rel, int g) {
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j)
 #pragma unroll
         for (int v = 0; v < 16; v += 4)
             *reinterpret_cast<f32x4*>(dst + 32 * j + acc_row(v, g)) = (f32x4){o[j][v] * f, o[j][v + 1] * f, o[j][v + 2] * f, o[j][v + 3] * f};
-    if (g == 0) dst[DP] = x, dst[DP + 1] = y;
+    if (g == 0) dst[DP] = top, dst[DP + 1] = l, dst[DP + 2] = rel;
 }
 
 // Forward.  S^T = K Q^T: a lane holds one query's scores, so the softmax is
@@ -534,6 +556,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     };
     const WinMask mask = WinMask::keys(a, i, p.n);
     WinState st;
+    float rel;
     floatx16 o[DP / 32];
     win_arrived(q);
     auto run = [&](auto careful) WIN_INLINE {
@@ -608,6 +631,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
             at.move(t & 1 ? -2 * TILE : 2 * TILE);
         }
         at.move(tiles.count & 1 ? -2 * TILE : 0);  // to the first stage again
+        rel = win_rel<BF, FAR>(st, a.scale2);
     };
     run(std::false_type());
     // Scores past 2^20, or a value that is not finite (a product with a probability
@@ -622,13 +646,12 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     const bool any = l != 0.0f && i < p.n;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
         const int64_t row = (((int64_t)p.b * a.far.rows + i) * a.H + p.h) * (a.far.parts + 1) + p.unit.part;
-        if (i < a.far.rows) win_part<DP>(a.part + row * (DP + 8), o, 1.0f, any ? st.sub : -__builtin_inff(), l, g);
+        if (i < a.far.rows) win_part<DP>(a.part + row * (DP + 8), o, 1.0f, any ? st.top : -__builtin_inff(), l, rel - win_shift<BF>(), g);
     }
     if (p.unit.part) return;
     const bool joined = a.far.parts && i < a.far.rows;
-    // the gradient's probabilities are exp2(S scale2 + stat), times 2^15 in fp16
     if (a.stat && g == 0 && i < a.NP && !joined)
-        a.stat[((int64_t)p.b * a.H + p.h) * a.NP + i] = any ? (BF ? 0.0f : 15.0f) - (st.sub + __builtin_amdgcn_logf(l)) : -__builtin_inff();
+        win_stat<BF>(a.top, a.stat, ((int64_t)p.b * a.H + p.h) * a.NP + i, any, st.top, rel + __builtin_amdgcn_logf(l));
     win_store<DP, BF>(o, any ? 1.0f / l : 0.0f, !any, i < a.N && !joined, a.out + p.b * a.os[0] + (int64_t)i * a.os[1] + p.h * a.os[2], a.D, g);
 }
 
@@ -684,7 +707,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
         delta = half_sum(delta);
     }
     if (g == 0 && i < a.NP && !p.unit.part) a.delta[row] = delta;
-    float stat = i < a.NP ? a.stat[row] : -__builtin_inff();
+    float top = i < a.NP ? a.top[row] : 0.0f, stat = i < a.NP ? a.stat[row] : __builtin_inff();
     if (!a.gq) return;
     const WinTiles tiles = win_keys<T>(a, p);
     RowLoads<DP, T, 4> lk, lv;
@@ -713,7 +736,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
     float c = BF ? 1.0f : 0x1p126f;
     win_arrived(q);
     win_arrived(go);
-    asm volatile("" : "+v"(stat), "+v"(delta));
+    asm volatile("" : "+v"(top), "+v"(stat), "+v"(delta));
     if (tiles.count) issue(0);
     for (int t = 0; t < tiles.count; ++t) {
         win_sync();
@@ -745,7 +768,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
             if (e < 4 * NS) {
                 if (e / NS & 1) {
                     dp = win_mma<BF>(f, go[x], dp);
-                    win_exp(s[kb], win_piece(x, 1, NS), win_piece(x + 1, 1, NS), a.scale2, -stat);
+                    win_exp_from(s[kb], win_piece(x, 1, NS), win_piece(x + 1, 1, NS), top, a.scale2, stat);
                 } else {
                     s[kb] = win_mma<BF>(f, q[x], s[kb]);
                     if (kb && x == 0) finish(0);
@@ -762,7 +785,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
     const float f = (BF ? 1.0f : 0x1p-15f) / c;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
         const int64_t slot = (((int64_t)p.b * a.far.rows + i) * a.H + p.h) * (a.far.parts + 1) + p.unit.part;
-        if (i < a.far.rows) win_part<DP>(a.part + slot * (DP + 8), o, i < p.n ? f : 0.0f, 0.0f, 1.0f, g);
+        if (i < a.far.rows) win_part<DP>(a.part + slot * (DP + 8), o, i < p.n ? f : 0.0f, 0.0f, 1.0f, 0.0f, g);
     }
     if (p.unit.part) return;
     char* dst = a.gq + (((int64_t)p.b * a.N + i) * a.H + p.h) * 2 * a.D;
@@ -792,8 +815,8 @@ __device__ __forceinline__ float win_lane(float v) {
 }
 // P, and dP - rowsum(dO O), of a lane's key and 16 queries, whose statistics lie in 16 lanes
 template <int... E>
-__device__ __forceinline__ void win_probs(std::integer_sequence<int, E...>, floatx16& s, float scale2, float stat) {
-    ((s[E] = __builtin_amdgcn_exp2f(s[E] * scale2 + win_lane<E>(stat))), ...);
+__device__ __forceinline__ void win_probs(std::integer_sequence<int, E...>, floatx16& s, float top, float scale2, float stat) {
+    ((s[E] = __builtin_amdgcn_exp2f((s[E] - win_lane<E>(top)) * scale2 - win_lane<E>(stat))), ...);
 }
 template <int... E>
 __device__ __forceinline__ void win_diff(std::integer_sequence<int, E...>, floatx16& dp, float delta) {
@@ -832,7 +855,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
     at.init(lds + V + 32 * half * RB, lane);
     // the step that is loaded next: head `head` of query tile qt; heads go round within a tile
     int head = 0, qt = 0, q0 = 0, q0_next = 0;
-    float stat = 0.0f, delta = 0.0f, stat_next = 0.0f, delta_next = 0.0f;
+    float top = 0.0f, stat = 0.0f, delta = 0.0f, top_next = 0.0f, stat_next = 0.0f, delta_next = 0.0f;
     const int mine_q = 32 * half + acc_row(lane & 15, g);  // whose statistics this lane loads
     int64_t row = 0;
     auto place = [&]() WIN_INLINE {
@@ -849,6 +872,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
             ++qt;
             place();
         }
+        top_next = a.top[row + mine_q];
         stat_next = a.stat[row + mine_q];
         delta_next = a.delta[row + mine_q];
         lq.resource();
@@ -878,8 +902,8 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
     win_arrived(kf);
     for (int t = 0; t < steps; ++t) {
         win_sync();
-        asm volatile("" : "+v"(stat_next), "+v"(delta_next));
-        stat = stat_next, delta = delta_next;
+        asm volatile("" : "+v"(top_next), "+v"(stat_next), "+v"(delta_next));
+        top = top_next, stat = stat_next, delta = delta_next;
         q0 = q0_next;
         if (t + 1 < steps) issue(t + 1);
         const int seen = q0 < n ? span(q0, q0 + 31) : 0;
@@ -907,7 +931,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
                     }
                     dp = win_mma<BF>(was, f, dp);
                     if (e == 3 * NS - 1) {
-                        win_probs(std::make_integer_sequence<int, 16>(), s, a.scale2, stat);
+                        win_probs(std::make_integer_sequence<int, 16>(), s, top, a.scale2, stat);
                         if (seen == 1)
                             mask(q0, g, !a.causal && q0 < a.sinks, [&](int v, bool in) WIN_INLINE { s[v] = in ? s[v] : 0.0f; });
                     }
@@ -965,7 +989,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
                 }
             if (parted && key < a.kfar.rows) {
                 const int64_t row = ((((int64_t)w * a.B + b) * a.kfar.rows + key) * a.KV + kv) * (a.kfar.parts + 1) + unit.part;
-                win_part<DP>(a.kpart + row * (DP + 8), o, key < n ? fv : 0.0f, 0.0f, 1.0f, g);
+                win_part<DP>(a.kpart + row * (DP + 8), o, key < n ? fv : 0.0f, 0.0f, 1.0f, 0.0f, g);
             }
             char* dst = w ? a.gv : a.gk;
             if (dst && !unit.part)
@@ -1093,7 +1117,7 @@ __global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(
             for (int v = 0; v < 16; v += 4)
                 *reinterpret_cast<f32x4*>(sums + (wave * 32 + r) * LD + 32 * j + acc_row(v, g)) =
                     (f32x4){o[j][v], o[j][v + 1], o[j][v + 2], o[j][v + 3]};
-        if (g == 0) ml[(wave * 32 + r) * 2] = st.sub, ml[(wave * 32 + r) * 2 + 1] = st.l;
+        if (g == 0) ml[(wave * 32 + r) * 2] = st.top, ml[(wave * 32 + r) * 2 + 1] = st.l;
     }
     __syncthreads();
     const int rows = a.rows - 32 * blk < 32 ? a.rows - 32 * blk : 32;
@@ -1104,7 +1128,7 @@ __global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(
         for (int w = 0; w < W; ++w) m = fmaxf(m, ml[(w * 32 + x) * 2]);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            const float mw = ml[(w * 32 + x) * 2], f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
+            const float mw = ml[(w * 32 + x) * 2], f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((mw - m) * a.scale2);
             l += f * ml[(w * 32 + x) * 2 + 1];
             if (mw != -__builtin_inff())
 #pragma unroll
@@ -1113,10 +1137,10 @@ __global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(
         const int orow = 32 * blk + x, ot = orow / group, oh = kv * group + orow - ot * group;
         if (a.splits > 1) {
             const int64_t at_ = (((int64_t)b * a.N + ot) * a.H + oh) * a.splits + split;
-            float* dst = a.part + at_ * (DP + 8);  // 8 DP-piece, then the exponent and the sum
+            float* dst = a.part + at_ * (DP + 8);  // as win_part
 #pragma unroll
             for (int t = 0; t < 8; t += 4) *reinterpret_cast<f32x4*>(dst + d + t) = (f32x4){v[t], v[t + 1], v[t + 2], v[t + 3]};
-            if (d == 0) dst[DP] = m, dst[DP + 1] = l;
+            if (d == 0) dst[DP] = m, dst[DP + 1] = l, dst[DP + 2] = 0.0f;
         } else if (d < a.D) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             char* dst = a.out + (((int64_t)b * a.N + ot) * a.H + oh) * 2 * a.D + 2 * d;
@@ -1128,15 +1152,15 @@ __global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(
 
 // Rows [sequence][token][head] from their slots, a workgroup a row: DP / 4 threads
 // hold its values, the others every so many slots (one thread over 49 slots of a
-// gradient's 16 rows: 17 us, so 5).  Outputs (a slot: sums, their exponent,
-// their weight), or plain sums times `factor` (GRAD: no exponents).  A slot
-// without any has the exponent -inf.
+// gradient's 16 rows: 17 us, so 5).  Outputs (a slot as win_part leaves it), or
+// plain sums times `factor` (GRAD).  A slot without any has the score -inf.
 constexpr int kWinSlots = 256;
 struct WinJoin {
     const float* part;
     char* out[2];         // GRAD: keys and values, rows of one behind the other's; NULL: not wanted
     float factor[2];
-    float* stat;          // [B, heads, NP], or NULL
+    float *top, *stat;    // [B, heads, NP], or NULL
+    float scale2;
     int64_t os[3];
     int64_t rows;         // sequences x tokens x heads
     int tokens, heads, slots, D, NP;
@@ -1158,7 +1182,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(WinJoin a) {
         if ((tid & 63) == 0) most[tid >> 6] = m;
         __syncthreads();
         m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-        const float f = e == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(e - m);
+        const float f = e == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fmaf(e - m, a.scale2, src[tid * LD + DP + 2]));
         weight[tid] = f;
         l = group_sum<64>(f != 0.0f ? f * src[tid * LD + DP + 1] : 0.0f);
         if ((tid & 63) == 0) total[tid >> 6] = l;
@@ -1181,7 +1205,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(WinJoin a) {
     const int64_t seq = row / ((int64_t)a.tokens * a.heads);
     const int rest = (int)(row - seq * a.tokens * a.heads), tok = rest / a.heads, h = rest - tok * a.heads;
     if (!GRAD && a.stat && tid == 0)
-        a.stat[(seq * a.heads + h) * a.NP + tok] = l == 0.0f ? -__builtin_inff() : (BF ? 0.0f : 15.0f) - (m + __builtin_amdgcn_logf(l));
+        win_stat<BF>(a.top, a.stat, (seq * a.heads + h) * a.NP + tok, l != 0.0f, m, win_shift<BF>() + __builtin_amdgcn_logf(l));
     if (sg || 4 * d >= a.D) return;
 #pragma unroll
     for (int s = 1; s < SG; ++s)
@@ -1210,6 +1234,7 @@ static WinArgs win_args(const rpfq_window_desc& d, const void* q, const void* k,
     a.causal = d.causal;
     a.scale = d.scale;
     a.scale2 = d.scale * 1.4426950408889634f;
+    a.top = d.top;
     const int group = a.H / a.KV;
     a.hw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
     a.qw = 4 / a.hw;
@@ -1240,6 +1265,7 @@ static WinJoin win_joined(const WinArgs& a, const float* part, int tokens, int64
     j.os[0] = n * heads * 2 * a.D, j.os[1] = (int64_t)heads * 2 * a.D, j.os[2] = 2 * a.D;
     j.rows = (int64_t)a.B * tokens * heads;
     j.tokens = tokens, j.heads = heads, j.slots = slots, j.D = a.D, j.NP = a.NP;
+    j.scale2 = a.scale2;
     return j;
 }
 struct WinForward {
@@ -1252,7 +1278,7 @@ struct WinForward {
         if (e != hipSuccess || !a.far.parts) return e;
         WinJoin j = win_joined(a, a.part, a.far.rows, a.N, a.H, a.far.parts + 1);
         for (int i = 0; i < 3; ++i) j.os[i] = a.os[i];
-        j.out[0] = a.out, j.stat = a.stat;
+        j.out[0] = a.out, j.top = a.top, j.stat = a.stat;
         return win_join<DP, BF, false>(j, s);
     }
 };

@@ -193,6 +193,7 @@ class WindowDesc(ctypes.Structure):
         ("dtype", ctypes.c_int32),
         ("causal", ctypes.c_int32),
         ("scale", ctypes.c_float),
+        ("top", ctypes.c_void_p),
     ]
 
 
