@@ -506,14 +506,17 @@ __device__ __forceinline__ void win_stat(float* top, float* stat, int64_t at, bo
 
 // 32 rows of DP results as a slot of their float32 sums: `o` times f, and three
 // numbers behind them: the score and the sum that they are relative to, and what
-// win_rel differs from the shift by.
+// win_rel differs from the shift by.  Rows behind a sequence's end leave zeros,
+// whatever the products of their zeros with its values were.
 template <int DP>
-__device__ __forceinline__ void win_part(float* dst, const floatx16 (&o)[DP / 32], float f, float top, float l, float rel, int g) {
+__device__ __forceinline__ void win_part(float* dst, const floatx16 (&o)[DP / 32], float f, bool inside, float top, float l, float rel, int g) {
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j)
 #pragma unroll
-        for (int v = 0; v < 16; v += 4)
-            *reinterpret_cast<f32x4*>(dst + 32 * j + acc_row(v, g)) = (f32x4){o[j][v] * f, o[j][v + 1] * f, o[j][v + 2] * f, o[j][v + 3] * f};
+        for (int v = 0; v < 16; v += 4) {
+            const f32x4 x = (f32x4){o[j][v] * f, o[j][v + 1] * f, o[j][v + 2] * f, o[j][v + 3] * f};
+            *reinterpret_cast<f32x4*>(dst + 32 * j + acc_row(v, g)) = inside ? x : (f32x4){0, 0, 0, 0};
+        }
     if (g == 0) dst[DP] = top, dst[DP + 1] = l, dst[DP + 2] = rel;
 }
 
@@ -646,7 +649,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     const bool any = l != 0.0f && i < p.n;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
         const int64_t row = (((int64_t)p.b * a.far.rows + i) * a.H + p.h) * (a.far.parts + 1) + p.unit.part;
-        if (i < a.far.rows) win_part<DP>(a.part + row * (DP + 8), o, 1.0f, any ? st.top : -__builtin_inff(), l, rel - win_shift<BF>(), g);
+        if (i < a.far.rows) win_part<DP>(a.part + row * (DP + 8), o, 1.0f, i < p.n, any ? st.top : -__builtin_inff(), l, rel - win_shift<BF>(), g);
     }
     if (p.unit.part) return;
     const bool joined = a.far.parts && i < a.far.rows;
@@ -785,7 +788,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
     const float f = (BF ? 1.0f : 0x1p-15f) / c;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
         const int64_t slot = (((int64_t)p.b * a.far.rows + i) * a.H + p.h) * (a.far.parts + 1) + p.unit.part;
-        if (i < a.far.rows) win_part<DP>(a.part + slot * (DP + 8), o, i < p.n ? f : 0.0f, 0.0f, 1.0f, 0.0f, g);
+        if (i < a.far.rows) win_part<DP>(a.part + slot * (DP + 8), o, f, i < p.n, 0.0f, 1.0f, 0.0f, g);
     }
     if (p.unit.part) return;
     char* dst = a.gq + (((int64_t)p.b * a.N + i) * a.H + p.h) * 2 * a.D;
@@ -989,7 +992,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
                 }
             if (parted && key < a.kfar.rows) {
                 const int64_t row = ((((int64_t)w * a.B + b) * a.kfar.rows + key) * a.KV + kv) * (a.kfar.parts + 1) + unit.part;
-                win_part<DP>(a.kpart + row * (DP + 8), o, key < n ? fv : 0.0f, 0.0f, 1.0f, 0.0f, g);
+                win_part<DP>(a.kpart + row * (DP + 8), o, fv, key < n, 0.0f, 1.0f, 0.0f, g);
             }
             char* dst = w ? a.gv : a.gk;
             if (dst && !unit.part)
