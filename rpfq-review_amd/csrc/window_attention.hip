@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     const bool any = l != 0.0f && i < p.n;
     if (a.far.parts && p.unit.tile < a.far.tiles && p.mine < a.far.rows) {
         const int64_t row = (((int64_t)p.b * a.far.rows + i) * a.H + p.h) * (a.far.parts + 1) + p.unit.part;
-        if (i < a.far.rows) win_part<DP>(a.part + row * (DP + 8), o, 1.0f, i < p.n, any ? st.top : -__builtin_inff(), l, rel - win_shift<BF>(), g);
+        if (i < a.far.rows) win_part<DP>(a.part + row * (DP + 8), o, 1.0f, i < p.n, any ? st.top : -__builtin_inff(), i < p.n ? l : 0.0f, rel - win_shift<BF>(), g);
     }
     if (p.unit.part) return;
     const bool joined = a.far.parts && i < a.far.rows;
@@ -1133,9 +1133,8 @@ __global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(
         for (int w = 0; w < W; ++w) {
             const float mw = ml[(w * 32 + x) * 2], f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((mw - m) * a.scale2);
             l += f * ml[(w * 32 + x) * 2 + 1];
-            if (mw != -__builtin_inff())
 #pragma unroll
-                for (int t = 0; t < 8; ++t) v[t] = fmaf(f, sums[(w * 32 + x) * LD + d + t], v[t]);
+            for (int t = 0; t < 8; ++t) v[t] = fmaf(f, sums[(w * 32 + x) * LD + d + t], v[t]);
         }
         const int orow = 32 * blk + x, ot = orow / group, oh = kv * group + orow - ot * group;
         if (a.splits > 1) {
@@ -1156,7 +1155,9 @@ __global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(
 // Rows [sequence][token][head] from their slots, a workgroup a row: DP / 4 threads
 // hold its values, the others every so many slots (one thread over 49 slots of a
 // gradient's 16 rows: 17 us, so 5).  Outputs (a slot as win_part leaves it), or
-// plain sums times `factor` (GRAD).  A slot without any has the score -inf.
+// plain sums times `factor` (GRAD).  A slot without any has the score -inf and sums
+// of 0; one whose scores are all NaN has it too, and a sum of NaN, so no slot is
+// passed over for its weight of 0.
 constexpr int kWinSlots = 256;
 struct WinJoin {
     const float* part;
@@ -1187,7 +1188,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(WinJoin a) {
         m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
         const float f = e == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fmaf(e - m, a.scale2, src[tid * LD + DP + 2]));
         weight[tid] = f;
-        l = group_sum<64>(f != 0.0f ? f * src[tid * LD + DP + 1] : 0.0f);
+        l = group_sum<64>(tid < a.slots ? f * src[tid * LD + DP + 1] : 0.0f);
         if ((tid & 63) == 0) total[tid >> 6] = l;
         __syncthreads();
         l = total[0] + total[1] + total[2] + total[3];
@@ -1199,9 +1200,8 @@ __global__ void __launch_bounds__(256) window_join_kernel(WinJoin a) {
         for (int s = sg; s < a.slots; s += SG) {
             const f32x4 x = *reinterpret_cast<const f32x4*>(src + s * LD + 4 * d);
             const float f = GRAD ? 1.0f : weight[s];
-            if (GRAD || f != 0.0f)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) v[t] = fmaf(f, x[t], v[t]);
+            for (int t = 0; t < 4; ++t) v[t] = fmaf(f, x[t], v[t]);
         }
     if (sg < SG) sums[sg][d] = v;
     __syncthreads();

@@ -29,3 +29,61 @@ def test_gradients_behind_the_end_of_divided_sinks(which, causal, dtype):
     for grad in torch.autograd.grad(out, leaves, go):
         assert bool(grad[0].isfinite().all())
         assert not bool(grad[1, 20:].any())  # any() of NaN is true
+
+
+# batch, new tokens, slots, heads, kv heads, values, window, sinks, lengths: one part, and several
+CACHES = [(2, 1, 300, 4, 2, 64, 200, 2, [300, 77]), (2, 1, 5000, 4, 2, 64, 4100, 4, [4999, 4000]), (2, 3, 2500, 4, 2, 128, 2500, 0, [2500, 1700])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", W.DTYPES)
+@pytest.mark.parametrize("b,t,m,heads,kv,d,window,sinks,lengths", CACHES)
+def test_nan_over_a_cache_is_not_lost_where_parts_are_joined(b, t, m, heads, kv, d, window, sinks, lengths, dtype):
+    from quant_models import ops
+
+    g = W._gen(m)
+    q, k, v = W._normal(g, b, t, heads, d, dtype=dtype), W._normal(g, b, m, kv, d, dtype=dtype), W._normal(g, b, m, kv, d, dtype=dtype)
+    lens = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    want, bound = W._cache_want(q, k, v, lengths, window, sinks, d ** -0.5)
+    # a query that is not a number: every score of its row
+    one = q.clone()
+    one[0, -1, 1, 3] = math.nan
+    out = ops.window_attention_cached(one, k, v, lens, window, sinks)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+    hit[0, -1, 1] = True
+    assert bool(out[hit].isnan().all())
+    W._check(torch.where(hit, 0, out), torch.where(hit, 0, want), bound)
+    # a stretch of keys that are none, all that some parts see
+    lo = max(0, lengths[0] - window)
+    one = k.clone()
+    one[0, lo:lo + (lengths[0] - lo) * 2 // 3, 0] = math.nan
+    out = ops.window_attention_cached(q, one, v, lens, window, sinks)
+    hit[:] = False
+    hit[0, :, :heads // kv] = True
+    assert bool(out[hit].isnan().all())
+    W._check(torch.where(hit, 0, out), torch.where(hit, 0, want), bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", W.DTYPES)
+def test_nan_is_not_lost_where_sinks_are_divided(dtype):
+    from quant_models import ops
+
+    n, heads, kv, d, window, sinks = 1100, 4, 2, 64, 20, 3
+    q, k, v, _ = W._inputs(1, n, heads, kv, d, dtype, 11)
+    want = W._want(q, k, v, window, sinks, False, d ** -0.5, None)[0]
+    one = q.clone()
+    one[0, 1, 2, 3] = math.nan
+    out = ops.window_attention(one, k, v, window, sinks, causal=False)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+    hit[0, 1, 2] = True
+    assert bool(out[hit].isnan().all())
+    W._check(torch.where(hit, 0, out), torch.where(hit, 0, want[0]), want[1])
+    one = k.clone()
+    one[0, 300:900, 0] = math.nan  # all that some of the parts see
+    out = ops.window_attention(q, one, v, window, sinks, causal=False)
+    i = torch.arange(n, device=DEV)
+    hit[:] = False
+    hit[0, :, :2] = W._seen(i[:, None], i[None, 300:900], window, sinks, False).any(1)[:, None, None]
+    assert bool(hit[0, 0, 0].all()) and bool(out[hit].isnan().all())
+    W._check(torch.where(hit, 0, out), torch.where(hit, 0, want[0]), want[1])
