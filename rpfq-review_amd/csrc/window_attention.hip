@@ -348,18 +348,19 @@ __device__ __forceinline__ void win_arrived(uint4 (&f)[N]) {
 }
 __device__ __forceinline__ void win_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// c + a b where some of a are not finite: these count where their factor is not 0.
+// c + a b where some of a are not finite: these count where they are seen (the bits
+// of `seen`, b's 8 values), a factor that was rounded to 0 among them.
 template <bool BF>
-__device__ __forceinline__ floatx16 win_mma_some(uint4 a, uint4 b, floatx16 c) {
+__device__ __forceinline__ floatx16 win_mma_some(uint4 a, uint4 b, uint32_t seen, floatx16 c) {
     constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u, ONE = BF ? 0x3f80u : 0x3c00u;
-    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w};
     uint32_t fin[4], odd[4], some[4], any = 0;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         const uint32_t lo = (x[t] & E) == E ? 0xffffu : 0u, hi = (x[t] & E << 16) == E << 16 ? 0xffff0000u : 0u;
         fin[t] = x[t] & ~(lo | hi);
         odd[t] = (lo | hi) & (ONE | ONE << 16);
-        some[t] = (y[t] & 0x7fffu ? ONE : 0u) | (y[t] & 0x7fff0000u ? ONE << 16 : 0u);
+        some[t] = (seen >> 2 * t & 1 ? ONE : 0u) | (seen >> (2 * t + 1) & 1 ? ONE << 16 : 0u);
         any |= lo | hi;
     }
     if (!__any(any != 0)) return win_mma<BF>(a, b, c);
@@ -581,9 +582,14 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
                 if (e < 2 * NS) return at.rows(e / NS * 32 * RB, e % NS);
                 return at.cols(TILE + (e - 2 * NS) / NJ * 16 * RB, (e - 2 * NS) % NJ);
             };
+            uint32_t sees[2] = {0xffffu, 0xffffu};  // FAR: of each block's 16 keys of a lane
             auto hide = [&](floatx16& s, int kb) WIN_INLINE {
-                if (seen == 1)
-                    mask(k0 + 32 * kb, g, k0 < a.sinks, [&](int v, bool in) WIN_INLINE { s[v] = in ? s[v] : -__builtin_inff(); });
+                if (seen != 1) return;
+                if (FAR) sees[kb] = 0;
+                mask(k0 + 32 * kb, g, k0 < a.sinks, [&](int v, bool in) WIN_INLINE {
+                    s[v] = in ? s[v] : -__builtin_inff();
+                    if (FAR) sees[kb] |= (uint32_t)in << v;
+                });
             };
             auto anew = [&](float f) WIN_INLINE {
 #pragma unroll
@@ -627,7 +633,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
                     // weigh the values' distance to the output, not the values
                     st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
                 }
-                o[j] = FAR ? win_mma_some<BF>(f, pr, o[j]) : win_mma<BF>(f, pr, o[j]);
+                o[j] = FAR ? win_mma_some<BF>(f, pr, sees[u >> 1] >> 8 * (u & 1), o[j]) : win_mma<BF>(f, pr, o[j]);
                 if (y == 0) hide(s[1], 1);
                 if (u == 1 || u == 2) win_exp(s[1], 8 * (y - NJ) / NJ, 8 * (y + 1 - NJ) / NJ, a.scale2, take);
             });
@@ -1078,12 +1084,16 @@ __global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(
         };
         floatx16 sc = floatx16{0};
         uint4 pr;
+        uint32_t sees = 0;
         win_stream<NS + 2 * NJ, PD < NS + 2 * NJ ? PD : NS + 2 * NJ>(read, [&](int e, uint4 f) WIN_INLINE {
             if (e < NS) {
                 sc = win_mma<BF>(f, q[e], sc);
                 if (e < NS - 1) return;
                 if (some)
-                    mask(j0, g, j0 < sinks, [&](int v, bool in) WIN_INLINE { sc[v] = in ? sc[v] : -__builtin_inff(); });
+                    mask(j0, g, j0 < sinks, [&](int v, bool in) WIN_INLINE {
+                        sc[v] = in ? sc[v] : -__builtin_inff();
+                        sees |= (uint32_t)in << v;
+                    });
                 const float take = win_top<BF, true>(sc, st, a.scale2, [&](float f_) WIN_INLINE {
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
@@ -1100,7 +1110,7 @@ __global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(
             }
             if (some && a.N > 1) {
                 win_rare();
-                o[j] = win_mma_some<BF>(f, pr, o[j]);
+                o[j] = win_mma_some<BF>(f, pr, sees >> 8 * u, o[j]);
             } else {
                 o[j] = win_mma<BF>(f, pr, o[j]);
             }

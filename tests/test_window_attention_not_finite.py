@@ -87,3 +87,36 @@ def test_nan_is_not_lost_where_sinks_are_divided(dtype):
     hit[0, :, :2] = W._seen(i[:, None], i[None, 300:900], window, sinks, False).any(1)[:, None, None]
     assert bool(hit[0, 0, 0].all()) and bool(out[hit].isnan().all())
     W._check(torch.where(hit, 0, out), torch.where(hit, 0, want[0]), want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", W.DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_values_of_no_weight_reach_what_sees_them(causal, dtype):
+    """A key 300 above the others: their probabilities are 0 in any type, but a value
+    that is not finite among them is seen all the same."""
+    from quant_models import ops
+
+    n, heads, kv, d, window, sinks = 200, 4, 2, 64, 30, 2
+    q, k, v, _ = W._inputs(1, n, heads, kv, d, dtype, 5)
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[:, 110::50, :, 0] = 300.0  # keys 110 and 160, scores 300
+    want = W._want(q, k, v, window, sinks, causal, 0.125, None)[0]
+    i = torch.arange(n, device=DEV)
+    seen = W._seen(i[:, None], i[None], window, sinks, causal)
+    for at, what in ((120, math.inf), (100, math.nan), (1, -math.inf), (158, math.nan)):
+        one = v.clone()
+        one[0, at, 0, 5] = what
+        out = ops.window_attention(q, k, one, window, sinks, causal=causal, scale=0.125)
+        hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+        hit[0, :, :2, 5] = seen[:, at][:, None]
+        assert not bool(out[hit].isfinite().any())
+        W._check(torch.where(hit, 0, out), torch.where(hit, 0, want[0]), want[1])
+        for t in (1, 3):  # the last tokens, up to 190
+            last, worth = q[:, 190 - t:190].contiguous(), W._cache_want(q[:, 190 - t:190], k, v, [190], window, sinks, 0.125)
+            got = ops.window_attention_cached(last, k, one, torch.tensor([190], dtype=torch.int32, device=DEV), window, sinks, scale=0.125)
+            near = W._seen(i[190 - t:190], torch.tensor(at, device=DEV), window, sinks, True)
+            hit = torch.zeros(got.shape, dtype=torch.bool, device=DEV)
+            hit[0, :, :2, 5] = near[:, None]
+            assert not bool(got[hit].isfinite().any())
+            W._check(torch.where(hit, 0, got), torch.where(hit, 0, worth[0]), worth[1])
