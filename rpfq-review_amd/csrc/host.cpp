@@ -707,7 +707,8 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Py_ssize_t axes = PyTuple_GET_SIZE(a[4]);
     if (!pos || !freqs || axes < 1 || axes > 4 || freqs->scalar_type() != at::kDouble || freqs->dim() != 1 || !freqs->is_contiguous() ||
         q.dim() != 4 || q.numel() == 0 || pos->dim() < 2 || pos->dim() > 3 || pos->size(-1) != axes ||
-        (axes > 1 && pos->stride(-1) != 1) || pos->requires_grad() || freqs->requires_grad())
+        (axes > 1 && pos->stride(-1) != 1) || pos->requires_grad() || freqs->requires_grad() || transformed(*pos) ||
+        transformed(*freqs))
         Py_RETURN_NONE;
     rpfq_rotary_desc d = {};
     d.B = q.size(0), d.N = q.size(1), d.D = q.size(3);
@@ -827,7 +828,7 @@ bool window_operands(PyObject* const* a, at::Tensor (&t)[3], at::Tensor& lengths
         if (!operand(a[i], &t[i]) || !t[i].defined() || !window_rows16(t[i])) return false;
     if (a[3] != Py_None) {
         const at::Tensor* l = plain(a[3]);
-        if (!l || l->scalar_type() != at::kInt || l->dim() != 1 || !l->is_contiguous()) return false;
+        if (!l || l->scalar_type() != at::kInt || l->dim() != 1 || !l->is_contiguous() || transformed(*l)) return false;
         lengths = *l;
     }
     const double scale = PyFloat_AsDouble(a[6]);

@@ -1323,7 +1323,7 @@ def rotary(x, positions: torch.Tensor, freqs: torch.Tensor, sections=None, *, in
             return out[0] if one else out
     q = xs[0]
     N.require_same_device(q, positions=positions, freqs=freqs, k=xs[1] if len(xs) > 1 else None)
-    _no_transforms("rotary", *xs)
+    _no_transforms("rotary", *xs, positions, freqs)
     if not 1 <= len(sections) <= 4 or min(sections) < 0:
         raise ValueError(f"rotary takes 1 to 4 sections of 0 pairs or more, got {sections}")
     pairs = sum(sections)
