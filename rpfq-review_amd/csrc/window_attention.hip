@@ -1406,8 +1406,8 @@ hipError_t launch_window_attention_grad(const rpfq_window_desc& d, const void* q
 // parts, 118 in 4, 136 in 9), each of 4 tiles (a tile a wave) or more.
 int window_splits(const rpfq_window_desc& d) {
     const int64_t blocks = ((d.H / d.KV) * d.N + 31) / 32, units = d.B * d.KV * blocks, waves = d.D > 64 ? 4 : 8;
-    int64_t keys = d.window + d.N - 1 + d.sinks;
-    keys = keys < d.M ? keys : d.M;
+    const int64_t window = d.window < d.M ? d.window : d.M, sinks = d.sinks < d.M ? d.sinks : d.M;  // any int64: clamped before they are added
+    const int64_t all = window + d.N - 1 + sinks, keys = all < d.M ? all : d.M;
     if (keys <= 5 * 32 * waves) return 1;
     const int64_t most = (keys + 127) / 128, fill = device_cus() / units, want = fill > 2 ? fill : 2;
     const int64_t s = most < want ? most : want;
