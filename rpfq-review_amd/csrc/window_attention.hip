@@ -1403,12 +1403,16 @@ hipError_t launch_window_attention_grad(const rpfq_window_desc& d, const void* q
 // streams, 12 heads of 64 over 1,028 slots: 14.8 us in 9 parts, 9.4 in one).
 // Else as many as fill the chip's workgroups, two at least for long ones, whose
 // lengths differ (64 streams, 4 key heads of 128 over 4,100 slots: 106 us in 2
-// parts, 118 in 4, 136 in 9), each of 4 tiles (a tile a wave) or more.
+// parts, 118 in 4, 136 in 9), each of 4 tiles (a tile a wave) or more.  Several
+// blocks of rows a key head that fill the chip: one, since every row's float32 sums
+// go through memory twice (4 key heads of 128, bf16: 8 x 64 new tokens over 4,096
+// slots 60 us in 2 parts, 50 in one; 8 x 2,048 3.2 ms and 2.6, and 0.3 GB less).
 int window_splits(const rpfq_window_desc& d) {
     const int64_t blocks = ((d.H / d.KV) * d.N + 31) / 32, units = d.B * d.KV * blocks, waves = d.D > 64 ? 4 : 8;
     const int64_t window = d.window < d.M ? d.window : d.M, sinks = d.sinks < d.M ? d.sinks : d.M;  // any int64: clamped before they are added
     const int64_t all = window + d.N - 1 + sinks, keys = all < d.M ? all : d.M;
     if (keys <= 5 * 32 * waves) return 1;
+    if (blocks > 1 && units >= device_cus()) return 1;
     const int64_t most = (keys + 127) / 128, fill = device_cus() / units, want = fill > 2 ? fill : 2;
     const int64_t s = most < want ? most : want;
     return (int)(s < 1 ? 1 : s > kWinSlots ? kWinSlots : s);

@@ -24,3 +24,16 @@ def test_a_window_or_sinks_of_any_size_divide_a_cache_alike(d):
         assert size(_desc(D=d, window=far)) == want
         assert size(_desc(D=d, window=1, sinks=far)) == want
         assert size(_desc(D=d, window=far, sinks=far)) == want
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_new_tokens_over_a_cache_take_no_workspace(d):
+    """Where the rows fill the chip, no float32 sums of them go through memory; the last
+    tokens of a few streams over a long cache still go in parts."""
+    from quant_models import _native as N
+
+    size = N.load().rpfq_window_attention_cached_workspace_bytes
+    for b, n, heads, kv in ((8, 2048, 32, 8), (1, 4096, 16, 4), (1, 1 << 20, 16, 4), (64, 64, 12, 12)):
+        assert size(_desc(B=b, N=n, H=heads, KV=kv, D=d)) == 0
+    for b, n in ((1, 1), (8, 1), (8, 3), (300, 1), (1, 300)):
+        assert size(_desc(B=b, N=n, H=8, KV=2, D=d)) > 0
