@@ -842,6 +842,9 @@ int rpfq_rotary(const rpfq_rotary_desc* desc, const void* q, const void* k, void
  * next to each other, D a multiple of 8 up to 128, pointers 16-byte aligned.
  * lengths [B] (device int32, NULL: all of them N): rows of a sequence that
  * count, clamped to 0 .. N; those behind give zeros and are not read.
+ * Up to 2^28 tokens and 1,024 heads, and what fits one launch: fewer than 2^24
+ * workgroups, which have 128 rows of queries (heads that share keys together, each
+ * padded to 64) or 64 of keys, cached 32 rows (2^23 where D <= 64).
  * No counterpart in the reference, whose attention sees every token.
  */
 typedef struct rpfq_window_desc {

@@ -865,7 +865,7 @@ int rpfq_rotary(const rpfq_rotary_desc* d, const void* q, const void* k, void* q
     return hip_status(rpfq::launch_rotary(*d, q, k, q_out, k_out, positions, freqs, reinterpret_cast<hipStream_t>(stream)), "rpfq_rotary");
 }
 
-static int check_window(const rpfq_window_desc* d, bool cached) {
+static int check_window(const rpfq_window_desc* d, bool cached, bool grad) {
     if (!d) return fail(RPFQ_ERR_NULL, "desc is NULL");
     if (d->dtype != RPFQ_F16 && d->dtype != RPFQ_BF16) return fail(RPFQ_ERR_DTYPE, "unsupported dtype %d: fp16 or bf16", d->dtype);
     if (d->B <= 0 || d->N <= 0 || d->H <= 0 || d->KV <= 0 || d->D <= 0 || (cached ? d->M <= 0 : d->M != 0))
@@ -882,6 +882,10 @@ static int check_window(const rpfq_window_desc* d, bool cached) {
     if (d->window < 1 || d->sinks < 0) return fail(RPFQ_ERR_VALUE, "window=%lld must be positive, sinks=%lld not negative", (long long)d->window, (long long)d->sinks);
     if (d->causal & ~1) return fail(RPFQ_ERR_VALUE, "causal must be 0 or 1");
     if (!(d->scale > 0.0f && d->scale < 0x1p126f)) return fail(RPFQ_ERR_VALUE, "scale=%g must be positive and below 2^126", (double)d->scale);
+    if (rpfq::window_threads(*d, cached, grad) >> 32)
+        return fail(RPFQ_ERR_SHAPE, "more than a launch holds, %s (B=%lld N=%lld H=%lld KV=%lld)",
+                    cached ? "2^32 threads, 256 or 512 for 32 rows of a key head" : "2^32 threads, 256 for 128 rows of queries or 64 of keys",
+                    (long long)d->B, (long long)d->N, (long long)d->H, (long long)d->KV);
     return RPFQ_OK;
 }
 // strides that the kernels index by: whole 16-byte pieces, 128 rows of a tile within 31 bits
@@ -897,15 +901,15 @@ static int check_window_operands(const rpfq_window_desc* d, const void* q, const
     return RPFQ_OK;
 }
 size_t rpfq_window_attention_stat_bytes(const rpfq_window_desc* d) {
-    if (check_window(d, false) != RPFQ_OK) return 0;
+    if (check_window(d, false, true) != RPFQ_OK) return 0;
     return (size_t)(d->B * d->H * rpfq::window_rows(d->N)) * 4;
 }
 size_t rpfq_window_attention_workspace_bytes(const rpfq_window_desc* d, int grad) {
-    return check_window(d, false) != RPFQ_OK ? 0 : rpfq::window_bytes(*d, grad != 0);
+    return check_window(d, false, grad != 0) != RPFQ_OK ? 0 : rpfq::window_bytes(*d, grad != 0);
 }
 int rpfq_window_attention(const rpfq_window_desc* d, const void* q, const void* k, const void* v, const int32_t* lengths, void* out,
                           float* stat, void* work, size_t work_bytes, void* stream) {
-    int rc = check_window(d, false);
+    int rc = check_window(d, false, stat != nullptr);
     if (!rc) rc = check_window_operands(d, q, k, v, out, lengths);
     if (rc) return rc;
     if (!window_strides(d->out_stride) || !aligned(stat, 256) || !aligned(d->top, 256) || !aligned(work, 256))
@@ -920,7 +924,7 @@ int rpfq_window_attention(const rpfq_window_desc* d, const void* q, const void* 
 int rpfq_window_attention_grad(const rpfq_window_desc* d, const void* q, const void* k, const void* v, const int32_t* lengths,
                                const void* out, const void* grad_out, const float* stat, void* grad_q, void* grad_k, void* grad_v,
                                void* work, size_t work_bytes, void* stream) {
-    int rc = check_window(d, false);
+    int rc = check_window(d, false, true);
     if (!rc) rc = check_window_operands(d, q, k, v, out, lengths);
     if (rc) return rc;
     if (!grad_out || !stat || !work || (!grad_q && !grad_k && !grad_v))
@@ -936,11 +940,11 @@ int rpfq_window_attention_grad(const rpfq_window_desc* d, const void* q, const v
                       "rpfq_window_attention_grad");
 }
 size_t rpfq_window_attention_cached_workspace_bytes(const rpfq_window_desc* d) {
-    return check_window(d, true) != RPFQ_OK ? 0 : rpfq::window_cached_bytes(*d);
+    return check_window(d, true, false) != RPFQ_OK ? 0 : rpfq::window_cached_bytes(*d);
 }
 int rpfq_window_attention_cached(const rpfq_window_desc* d, const void* q, const void* k, const void* v, const int32_t* lengths, void* out,
                                  void* work, size_t work_bytes, void* stream) {
-    int rc = check_window(d, true);
+    int rc = check_window(d, true, false);
     if (!rc) rc = check_window_operands(d, q, k, v, out, lengths);
     if (rc) return rc;
     const size_t need = rpfq::window_cached_bytes(*d);

@@ -446,6 +446,7 @@ inline int64_t window_rows(int64_t N) { return (N + 63) / 64 * 64; }
 hipError_t launch_window_attention(const rpfq_window_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths,
                                    void* out, float* stat, void* work, hipStream_t s);
 size_t window_bytes(const rpfq_window_desc& d, bool grad);
+int64_t window_threads(const rpfq_window_desc& d, bool cached, bool grad);
 hipError_t launch_window_attention_grad(const rpfq_window_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths,
                                         const void* out, const void* grad_out, const float* stat, void* gq, void* gk, void* gv,
                                         void* work, hipStream_t s);

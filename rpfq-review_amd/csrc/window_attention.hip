@@ -1162,7 +1162,7 @@ __global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(
     }
 }
 
-// Rows [sequence][token][head] from their slots, a workgroup a row: DP / 4 threads
+// Rows [sequence][token][head] from their slots, a workgroup a row at a time: DP / 4 threads
 // hold its values, the others every so many slots (one thread over 49 slots of a
 // gradient's 16 rows: 17 us, so 5).  Outputs (a slot as win_part leaves it), or
 // plain sums times `factor` (GRAD).  A slot without any has the score -inf and sums
@@ -1176,7 +1176,7 @@ struct WinJoin {
     float *top, *stat;    // [B, heads, NP], or NULL
     float scale2;
     int64_t os[3];
-    int64_t rows;         // sequences x tokens x heads
+    int64_t rows, all;    // sequences x tokens x heads; of both tensors
     int tokens, heads, slots, D, NP;
 };
 template <int DP, bool BF, bool GRAD>
@@ -1184,49 +1184,53 @@ __global__ void __launch_bounds__(256) window_join_kernel(WinJoin a) {
     constexpr int LD = DP + 8, TD = DP / 4, SG = 256 / TD;  // SG slots at once (DP = 96: 10, and threads to spare)
     __shared__ float weight[kWinSlots], most[4], total[4];
     __shared__ f32x4 sums[SG][TD];
-    const int tid = threadIdx.x, which = blockIdx.x >= a.rows;
-    const int64_t row = (int64_t)blockIdx.x - (which ? a.rows : 0);
-    char* out = a.out[which];
-    if (!out) return;
-    const float* src = a.part + (int64_t)blockIdx.x * a.slots * LD;
-    float m = 0.0f, l = 0.0f;
-    if (!GRAD) {
-        const float e = tid < a.slots ? src[tid * LD + DP] : -__builtin_inff();
-        m = group_max<64>(e);
-        if ((tid & 63) == 0) most[tid >> 6] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-        const float f = e == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fmaf(e - m, a.scale2, src[tid * LD + DP + 2]));
-        weight[tid] = f;
-        l = group_sum<64>(tid < a.slots ? f * src[tid * LD + DP + 1] : 0.0f);
-        if ((tid & 63) == 0) total[tid >> 6] = l;
-        __syncthreads();
-        l = total[0] + total[1] + total[2] + total[3];
-    }
-    const int d = tid % TD, sg = tid / TD;
-    f32x4 v = {0, 0, 0, 0};
-    if (sg < SG)
-#pragma unroll 4
-        for (int s = sg; s < a.slots; s += SG) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(src + s * LD + 4 * d);
-            const float f = GRAD ? 1.0f : weight[s];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) v[t] = fmaf(f, x[t], v[t]);
+    const int tid = threadIdx.x;
+    for (int64_t at = blockIdx.x; at < a.all; at += gridDim.x) {
+        const int which = at >= a.rows;
+        const int64_t row = at - (which ? a.rows : 0);
+        char* out = a.out[which];
+        if (!out) continue;
+        __syncthreads();  // the row before has been read
+        const float* src = a.part + at * a.slots * LD;
+        float m = 0.0f, l = 0.0f;
+        if (!GRAD) {
+            const float e = tid < a.slots ? src[tid * LD + DP] : -__builtin_inff();
+            m = group_max<64>(e);
+            if ((tid & 63) == 0) most[tid >> 6] = m;
+            __syncthreads();
+            m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+            const float f = e == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(fmaf(e - m, a.scale2, src[tid * LD + DP + 2]));
+            weight[tid] = f;
+            l = group_sum<64>(tid < a.slots ? f * src[tid * LD + DP + 1] : 0.0f);
+            if ((tid & 63) == 0) total[tid >> 6] = l;
+            __syncthreads();
+            l = total[0] + total[1] + total[2] + total[3];
         }
-    if (sg < SG) sums[sg][d] = v;
-    __syncthreads();
-    const int64_t seq = row / ((int64_t)a.tokens * a.heads);
-    const int rest = (int)(row - seq * a.tokens * a.heads), tok = rest / a.heads, h = rest - tok * a.heads;
-    if (!GRAD && a.stat && tid == 0)
-        win_stat<BF>(a.top, a.stat, (seq * a.heads + h) * a.NP + tok, l != 0.0f, m, win_shift<BF>() + __builtin_amdgcn_logf(l));
-    if (sg || 4 * d >= a.D) return;
+        const int d = tid % TD, sg = tid / TD;
+        f32x4 v = {0, 0, 0, 0};
+        if (sg < SG)
+#pragma unroll 4
+            for (int s = sg; s < a.slots; s += SG) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(src + s * LD + 4 * d);
+                const float f = GRAD ? 1.0f : weight[s];
 #pragma unroll
-    for (int s = 1; s < SG; ++s)
+                for (int t = 0; t < 4; ++t) v[t] = fmaf(f, x[t], v[t]);
+            }
+        if (sg < SG) sums[sg][d] = v;
+        __syncthreads();
+        const int64_t seq = row / ((int64_t)a.tokens * a.heads);
+        const int rest = (int)(row - seq * a.tokens * a.heads), tok = rest / a.heads, h = rest - tok * a.heads;
+        if (!GRAD && a.stat && tid == 0)
+            win_stat<BF>(a.top, a.stat, (seq * a.heads + h) * a.NP + tok, l != 0.0f, m, win_shift<BF>() + __builtin_amdgcn_logf(l));
+        if (sg || 4 * d >= a.D) continue;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) v[t] += sums[s][d][t];
-    const float inv = GRAD ? a.factor[which] : l == 0.0f ? 0.0f : 1.0f / l;
-    *reinterpret_cast<uint2*>(out + seq * a.os[0] + tok * a.os[1] + h * a.os[2] + 8 * d) =
-        make_uint2(win_pack<BF>(v[0] * inv, v[1] * inv), win_pack<BF>(v[2] * inv, v[3] * inv));
+        for (int s = 1; s < SG; ++s)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) v[t] += sums[s][d][t];
+        const float inv = GRAD ? a.factor[which] : l == 0.0f ? 0.0f : 1.0f / l;
+        *reinterpret_cast<uint2*>(out + seq * a.os[0] + tok * a.os[1] + h * a.os[2] + 8 * d) =
+            make_uint2(win_pack<BF>(v[0] * inv, v[1] * inv), win_pack<BF>(v[2] * inv, v[3] * inv));
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -1269,7 +1273,9 @@ static hipError_t win_launch(K kernel, std::atomic<uint64_t>& done, const WinArg
 
 template <int DP, bool BF, bool GRAD>
 static hipError_t win_join(WinJoin j, hipStream_t s) {
-    hipLaunchKernelGGL((window_join_kernel<DP, BF, GRAD>), dim3((unsigned)(j.rows * (j.out[1] ? 2 : 1))), dim3(256), 0, s, j);
+    j.all = j.rows * (j.out[1] ? 2 : 1);
+    const int64_t most = 1 << 20;
+    hipLaunchKernelGGL((window_join_kernel<DP, BF, GRAD>), dim3((unsigned)(j.all < most ? j.all : most)), dim3(256), 0, s, j);
     return hipGetLastError();
 }
 // rows of `tokens` contiguous tokens of n a sequence
@@ -1408,7 +1414,7 @@ hipError_t launch_window_attention_grad(const rpfq_window_desc& d, const void* q
 // go through memory twice (4 key heads of 128, bf16: 8 x 64 new tokens over 4,096
 // slots 60 us in 2 parts, 50 in one; 8 x 2,048 3.2 ms and 2.6, and 0.3 GB less).
 int window_splits(const rpfq_window_desc& d) {
-    const int64_t blocks = ((d.H / d.KV) * d.N + 31) / 32, units = d.B * d.KV * blocks, waves = d.D > 64 ? 4 : 8;
+    const int64_t blocks = ((d.H / d.KV) * d.N + 31) / 32, units = d.B * d.KV * blocks, waves = d.D > 64 ? win_waves<128>() : win_waves<64>();
     const int64_t window = d.window < d.M ? d.window : d.M, sinks = d.sinks < d.M ? d.sinks : d.M;  // any int64: clamped before they are added
     const int64_t all = window + d.N - 1 + sinks, keys = all < d.M ? all : d.M;
     if (keys <= 5 * 32 * waves) return 1;
@@ -1416,6 +1422,15 @@ int window_splits(const rpfq_window_desc& d) {
     const int64_t most = (keys + 127) / 128, fill = device_cus() / units, want = fill > 2 ? fill : 2;
     const int64_t s = most < want ? most : want;
     return (int)(s < 1 ? 1 : s > kWinSlots ? kWinSlots : s);
+}
+// Threads of the largest launch of a call: a grid of 2^32 or more is none.
+int64_t window_threads(const rpfq_window_desc& d, bool cached, bool grad) {
+    if (cached) return d.B * d.KV * ((d.H / d.KV * d.N + 31) / 32) * window_splits(d) * 64 * (d.D > 64 ? win_waves<128>() : win_waves<64>());
+    WinArgs a = win_args(d, nullptr, nullptr, nullptr, nullptr);
+    win_fars(a);
+    const int64_t q = win_units(a.far, (int64_t)a.B * (a.H / a.hw), a.tiles);
+    const int64_t k = grad ? win_units(a.kfar, (int64_t)a.B * a.KV, (a.N + kWinKeys - 1) / kWinKeys) : 0;
+    return 256 * (q > k ? q : k);
 }
 size_t window_cached_bytes(const rpfq_window_desc& d) {
     const int s = window_splits(d);
