@@ -16,6 +16,7 @@ struct RotaryArgs {
     int turned, units;  // units of V values, or of V pairs, that turn; of a head (the rest are copied)
     int total;          // units of all its tokens
     int rest;           // values of a unit that is copied: V, or 1
+    int64_t first;      // the launch's first token
 };
 
 // V consecutive values as float32, from any element on: gfx950 loads 16 unaligned
@@ -63,7 +64,7 @@ template <int DT, int V>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
     extern __shared__ float2 turn[];  // [tokens][pairs]
     const rpfq_rotary_desc& d = a.d;
-    const int64_t t0 = (int64_t)blockIdx.x * a.tokens, all = d.B * d.N;
+    const int64_t t0 = a.first + (int64_t)blockIdx.x * a.tokens, all = d.B * d.N;
     for (int i = threadIdx.x; i < a.tokens * a.pairs; i += 256) {
         const int tok = i / a.pairs, j = i - tok * a.pairs;
         const int64_t t = t0 + tok;
@@ -150,9 +151,16 @@ static hipError_t rotary_go(RotaryArgs& a, hipStream_t s) {
     a.tokens = (int)(most < fill ? most : fill);
     if (a.tokens < 1) a.tokens = 1;
     a.total = a.tokens * (int)(a.d.heads[0] + a.d.heads[1]) * a.units;
-    const dim3 grid((unsigned)((all + a.tokens - 1) / a.tokens));
-    hipLaunchKernelGGL((rotary_kernel<DT, V>), grid, dim3(256), (size_t)a.tokens * a.pairs * sizeof(float2), s, a);
-    return hipGetLastError();
+    // a grid has fewer than 2^32 threads: 2^23 workgroups of 256 a launch
+    const int64_t most_blocks = 1 << 23;
+    for (a.first = 0; a.first < all; a.first += most_blocks * a.tokens) {
+        const int64_t blocks = (all - a.first + a.tokens - 1) / a.tokens;
+        const dim3 grid((unsigned)(blocks < most_blocks ? blocks : most_blocks));
+        hipLaunchKernelGGL((rotary_kernel<DT, V>), grid, dim3(256), (size_t)a.tokens * a.pairs * sizeof(float2), s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_rotary(const rpfq_rotary_desc& d, const void* q, const void* k, void* q_out, void* k_out, const void* pos,
