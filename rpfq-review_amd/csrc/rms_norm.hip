@@ -165,8 +165,9 @@ __device__ __forceinline__ float norm_rstd(const float (&h)[NC][8], int C, float
 // Codes of a row, rint(127 p / max|p|) of p = h w: 1 / rms cancels, so they are
 // decided by the stored h and w alone, ties to even.  float32's own quotient is
 // within 2e-5; where it is within 1e-4 of the middle of two codes, 254 |p| is
-// compared with (2 c + 1) max|p| in 64 bits, which hold the products (and the
-// comparison: 40 bits of 16-bit h).  The largest product is taken among those
+// compared with (2 c + 1) max|p| exactly: 64 bits hold the products (48 of their
+// 53 bits), not always their multiples, so the difference is formed by fma, with
+// what (2 c + 1) max|p| was rounded by.  The largest product is taken among those
 // that float32 rounds to within 2^-22 of the largest.
 template <int T, int NC>
 __device__ __forceinline__ void norm_codes(const NormArgs& a, const float (&h)[NC][8], const float (&w)[NC][8], float rstd, int64_t m, int col, double* sm) {
@@ -236,8 +237,9 @@ __device__ __forceinline__ void norm_codes(const NormArgs& a, const float (&h)[N
                 float c = __builtin_rintf(q);
                 if (fabsf(fabsf(q - c) - 0.5f) < 1e-4f) {
                     c = floorf(q);
-                    const double v = 254.0 * exact(i, t), mid = (2.0 * (double)c + 1.0) * topd;
-                    if (v > mid || (v == mid && ((int)c & 1))) c += 1.0f;
+                    const double odd = 2.0 * (double)c + 1.0, mid = odd * topd;
+                    const double past = fma(254.0, exact(i, t), -mid), rest = fma(odd, topd, -mid);
+                    if (past > rest || (past == rest && ((int)c & 1))) c += 1.0f;
                 }
                 code[t] = copysignf(c, p[i][t]) + WHOLE;
             }
