@@ -837,7 +837,8 @@ int rpfq_rotary(const rpfq_rotary_desc* desc, const void* q, const void* k, void
  * out = softmax(scale q k^T) v over what it sees, zeros for a row without any.
  * q, out [B, N, H, D]; k, v [B, N, KV, D] (cached: [B, M, KV, D]), KV a divisor of
  * H: query head h reads head h KV / H.  fp16 or bf16, scores and sums float32,
- * probabilities rounded to 16 bits.  Strides in elements between batches, tokens
+ * probabilities rounded to 16 bits (cached: two terms of 16 bits, as exact as the
+ * output's type).  Strides in elements between batches, tokens
  * and heads, multiples of 8, below 2^22 between tokens; the values of a head
  * next to each other, D a multiple of 8 up to 128, pointers 16-byte aligned.
  * lengths [B] (device int32, NULL: all of them N): rows of a sequence that

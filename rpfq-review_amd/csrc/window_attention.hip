@@ -137,6 +137,19 @@ __device__ __forceinline__ uint4 win_pack8(const floatx16& s, int u) {
     return make_uint4(win_pack<BF>(s[8 * u], s[8 * u + 1]), win_pack<BF>(s[8 * u + 2], s[8 * u + 3]),
                       win_pack<BF>(s[8 * u + 4], s[8 * u + 5]), win_pack<BF>(s[8 * u + 6], s[8 * u + 7]));
 }
+// What win_pack8 rounded off, as 16-bit values in the same order.
+template <bool BF>
+__device__ __forceinline__ uint4 win_rest8(const floatx16& s, int u, uint4 p) {
+    const uint32_t x[4] = {p.x, p.y, p.z, p.w};
+    uint32_t y[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const half2v h = __builtin_bit_cast(half2v, x[t]);
+        const float lo = BF ? bf16_to_f32(x[t] & 0xffffu) : (float)h[0], hi = BF ? bf16_to_f32(x[t] >> 16) : (float)h[1];
+        y[t] = win_pack<BF>(s[8 * u + 2 * t] - lo, s[8 * u + 2 * t + 1] - hi);
+    }
+    return make_uint4(y[0], y[1], y[2], y[3]);
+}
 // c + lo + hi of a 16-bit pair
 template <bool BF>
 __device__ __forceinline__ float win_sum2(uint32_t v, float c) {
@@ -1011,10 +1024,13 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
 // The last tokens over a cache.  A workgroup has one key head of one sequence,
 // up to 32 of its rows (queries x heads that share it) and a part of the keys; its
 // waves take tiles of 32 keys in turn, each through LDS of its own, without
-// waiting for each other.  Parts are joined by window_join_kernel.  Bound by HBM
-// (64 streams, 4 key heads of 128, 4,100 slots, bf16: 102 us, 5.3 TB/s), at few
-// heads by a wave's tiles, one read's latency behind the other (8 streams, 12 heads
-// of 64, 1,028 slots 10 us).
+// waiting for each other.  Parts are joined by window_join_kernel.  P goes into P V
+// as two 16-bit terms: the matrix units wait for memory here, and with one the
+// rounding of P is half of the output's error (bf16 2.3e-3 of it, with two 1.65e-3,
+// its own rounding).  Bound by HBM (64 streams, 4 key heads of 128, 4,100 slots,
+// bf16: 103 us, 5.2 TB/s, with one term 99), at few heads by a wave's tiles, one
+// read's latency behind the other (8 streams, 12 heads of 64, 1,028 slots 9.7 us,
+// with one 9.0).
 template <int DP>
 constexpr int win_waves() { return DP > 64 ? 4 : 8; }  // their rings fill 128 KB of LDS at most
 template <int DP, bool BF>
@@ -1083,7 +1099,7 @@ __global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(
             return at.cols(bt + TILE + (e - NS) / NJ * 16 * RB, (e - NS) % NJ);
         };
         floatx16 sc = floatx16{0};
-        uint4 pr;
+        uint4 pr, rest;
         uint32_t sees = 0;
         win_stream<NS + 2 * NJ, PD < NS + 2 * NJ ? PD : NS + 2 * NJ>(read, [&](int e, uint4 f) WIN_INLINE {
             if (e < NS) {
@@ -1106,13 +1122,17 @@ __global__ void __launch_bounds__(64 * win_waves<DP>(), 1) window_cached_kernel(
             const int u = (e - NS) / NJ, j = (e - NS) % NJ;
             if (j == 0) {
                 pr = win_pack8<BF>(sc, u);
-                st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
+                rest = win_rest8<BF>(sc, u, pr);
+#pragma unroll
+                for (int v = 0; v < 8; ++v) st.l += sc[8 * u + v];
             }
             if (some && a.N > 1) {
                 win_rare();
                 o[j] = win_mma_some<BF>(f, pr, sees >> 8 * u, o[j]);
+                o[j] = win_mma_some<BF>(f, rest, sees >> 8 * u, o[j]);
             } else {
                 o[j] = win_mma<BF>(f, pr, o[j]);
+                o[j] = win_mma<BF>(f, rest, o[j]);
             }
         });
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this buffer is free for the next load

@@ -1485,7 +1485,9 @@ def window_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     in the cache, the T new ones among them, so query t is token lengths - T +
     t.  Slots that no query sees are not read: what lies behind a sequence's
     end, or between the sinks and the window, does not count.  Queries in front
-    of the first token (lengths < T) give zeros.  No gradient."""
+    of the first token (lengths < T) give zeros.  Probabilities go into the product
+    with v as two 16-bit terms: the output's error is its own rounding.  No
+    gradient."""
     host = N.host()
     if host is not None:
         given = q.shape[-1] ** -0.5 if scale is None and isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else scale
