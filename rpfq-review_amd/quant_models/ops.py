@@ -1279,17 +1279,27 @@ def _apart_from(a: torch.Tensor, b: torch.Tensor) -> bool:
     (a0, a1), (b0, b1) = ends(a), ends(b)
     if a1 <= b0 or b1 <= a0:
         return True
-    if a.stride() != b.stride() or a0 == b0:
+    low, high = (a, b) if a0 < b0 else (b, a)
+    gap, odd = divmod(abs(a0 - b0), a.element_size())
+    if gap == 0 or odd:
         return False
-    shape = [2, *(max(n, m) for n, m in zip(a.shape, b.shape))]
-    stride = [abs(a0 - b0) // a.element_size(), *a.stride()]
-    span = 1
-    for size, step in sorted(zip(shape, stride), key=lambda e: e[1]):
-        if size > 1:
-            if step < span:
-                return False
-            span += step * (size - 1)
-    return True
+    dims = []
+    for n, m, s, t in zip(low.shape, high.shape, low.stride(), high.stride()):
+        if n > 1 and m > 1 and s != t:
+            return False
+        dims.append((s if n > 1 else t, n, m))
+    # what lies within the gap: the lower one's pieces have to end there; behind it
+    # the two are one piece, which no larger stride may fold onto itself
+    below, above, span = 1, 1, 0
+    for step, n, m in sorted(d for d in dims if max(d[1:]) > 1):
+        if step < gap or (n == 1 and not span):
+            below, above = below + step * (n - 1), above + step * (m - 1)
+            continue
+        span = span or gap + above
+        if step < span:
+            return False
+        span += step * (max(n, m) - 1)
+    return below <= gap
 
 
 def rotary(x, positions: torch.Tensor, freqs: torch.Tensor, sections=None, *, interleaved: bool = False,
