@@ -858,12 +858,14 @@ typedef struct rpfq_window_desc {
     int32_t dtype, causal;
     float scale;            /* positive, below 2^126 */
     float* top;             /* goes with stat: a second array of its size, out of the forward, in of the gradient */
+    void* rests;            /* goes with stat: of dtype, contiguous [B, N, H, D], 16-byte aligned */
 } rpfq_window_desc;
 
 /* stat, desc->top (out, float32, 256-byte aligned, rpfq_window_attention_stat_bytes
- * each; both NULL: not wanted): what the gradient needs of each row, log2 of its
- * softmax's sum relative to a score, and that score.  work: its workspace (may be
- * 0 bytes), 256-byte aligned. */
+ * each) and desc->rests; all NULL: not wanted: what the gradient needs of each row,
+ * log2 of its softmax's sum relative to a score, that score, and what out was
+ * rounded by (so that rowsum(grad_out out) is float32's; with it P V takes two
+ * 16-bit terms of P).  work: its workspace (may be 0 bytes), 256-byte aligned. */
 int rpfq_window_attention(const rpfq_window_desc* desc, const void* q, const void* k, const void* v,
                           const int32_t* lengths, void* out, float* stat, void* work, size_t work_bytes, void* stream);
 size_t rpfq_window_attention_stat_bytes(const rpfq_window_desc* desc);
@@ -871,7 +873,7 @@ size_t rpfq_window_attention_stat_bytes(const rpfq_window_desc* desc);
 size_t rpfq_window_attention_workspace_bytes(const rpfq_window_desc* desc, int grad);
 
 /* Gradients, contiguous and of dtype, zeros behind a sequence's end; any of
- * them NULL: not wanted.  out, stat, desc->top: the forward's; work: its workspace,
+ * them NULL: not wanted.  out, stat, desc->top, desc->rests: the forward's; work: its workspace,
  * 256-byte aligned.  Sums in a fixed order. */
 int rpfq_window_attention_grad(const rpfq_window_desc* desc, const void* q, const void* k, const void* v,
                                const int32_t* lengths, const void* out, const void* grad_out, const float* stat,

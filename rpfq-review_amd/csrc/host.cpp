@@ -764,15 +764,17 @@ void window_strides(const at::Tensor& t, int64_t (&s)[3]) {
 
 // Attention with a window under autograd: (q, k, v) -> out.
 struct Window : torch::autograd::Function<Window> {
-    static std::pair<at::Tensor, at::Tensor> attend(rpfq_window_desc& d, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    static std::array<at::Tensor, 3> attend(rpfq_window_desc& d, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                     const at::Tensor& lengths, bool stat) {
         const c10::DeviceGuard guard(q.device());
         const auto options = q.options().requires_grad(false);
-        at::Tensor out = at::empty(q.sizes(), options), st;
+        at::Tensor out = at::empty(q.sizes(), options), st, rests;
         window_strides(out, d.out_stride);
         if (stat) {  // both of its arrays
             st = at::empty({2, (int64_t)(api.rpfq_window_attention_stat_bytes(&d) / 4)}, options.dtype(at::kFloat));
             d.top = st[1].data_ptr<float>();
+            rests = at::empty(q.sizes(), options);
+            d.rests = rests.data_ptr();
         }
         const size_t bytes = api.rpfq_window_attention_workspace_bytes(&d, 0);
         at::Tensor work;
@@ -780,14 +782,14 @@ struct Window : torch::autograd::Function<Window> {
         const int rc = api.rpfq_window_attention(&d, q.data_ptr(), k.data_ptr(), v.data_ptr(), static_cast<const int32_t*>(ptr(lengths)),
                                                  out.data_ptr(), stat ? st.data_ptr<float>() : nullptr, ptr(work), bytes, stream_on(q));
         TORCH_CHECK(rc == RPFQ_OK, "rpfq_window_attention: ", api.rpfq_last_error());
-        return {out, st};
+        return {out, st, rests};
     }
 
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                               const std::optional<at::Tensor>& lengths, rpfq_window_desc* d) {
         const at::Tensor len = lengths ? *lengths : at::Tensor();
-        auto [out, stat] = attend(*d, q, k, v, len, true);
-        ctx->save_for_backward({q, k, v, len, out, stat});
+        auto [out, stat, rests] = attend(*d, q, k, v, len, true);
+        ctx->save_for_backward({q, k, v, len, out, stat, rests});
         ctx->saved_data["desc"] = std::string(reinterpret_cast<const char*>(d), sizeof(*d));
         return out;
     }
@@ -806,6 +808,7 @@ struct Window : torch::autograd::Function<Window> {
             const at::Tensor go = window_rows16(grads[0]) ? grads[0] : grads[0].clone(at::MemoryFormat::Contiguous);
             window_strides(go, d.grad_stride);
             d.top = const_cast<float*>(stat.const_data_ptr<float>()) + stat.size(1);
+            d.rests = saved[6].data_ptr();
             const at::Tensor* in[3] = {&q, &k, &v};
             for (int i = 0; i < 3; ++i)
                 if (ctx->needs_input_grad(i)) g[i] = at::empty(in[i]->sizes(), q.options().requires_grad(false));
@@ -867,7 +870,7 @@ PyObject* window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (needs_grad(&t[0]) || needs_grad(&t[1]) || needs_grad(&t[2]))
             out = Window::apply(t[0], t[1], t[2], lengths.defined() ? std::optional<at::Tensor>(lengths) : std::nullopt, &d);
         else
-            out = Window::attend(d, t[0], t[1], t[2], lengths, false).first;
+            out = Window::attend(d, t[0], t[1], t[2], lengths, false)[0];
     }
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS

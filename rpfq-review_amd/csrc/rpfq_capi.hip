@@ -912,9 +912,10 @@ int rpfq_window_attention(const rpfq_window_desc* d, const void* q, const void* 
     int rc = check_window(d, false, stat != nullptr);
     if (!rc) rc = check_window_operands(d, q, k, v, out, lengths);
     if (rc) return rc;
-    if (!window_strides(d->out_stride) || !aligned(stat, 256) || !aligned(d->top, 256) || !aligned(work, 256))
-        return fail(RPFQ_ERR_ALIGN, "out's strides must be multiples of 8 elements, stat, desc->top and work 256-byte aligned");
-    if ((stat != nullptr) != (d->top != nullptr)) return fail(RPFQ_ERR_NULL, "desc->top goes with stat, and only with it");
+    if (!window_strides(d->out_stride) || !aligned(stat, 256) || !aligned(d->top, 256) || !aligned(d->rests, 16) || !aligned(work, 256))
+        return fail(RPFQ_ERR_ALIGN, "out's strides must be multiples of 8 elements, stat, desc->top and work 256-byte aligned, desc->rests 16");
+    if ((stat != nullptr) != (d->top != nullptr) || (stat != nullptr) != (d->rests != nullptr))
+        return fail(RPFQ_ERR_NULL, "desc->top and desc->rests go with stat, and only with it");
     const size_t need = rpfq::window_bytes(*d, false);
     if (need && !work) return fail(RPFQ_ERR_NULL, "rpfq_window_attention: NULL pointer argument");
     if (work_bytes < need) return fail(RPFQ_ERR_SHAPE, "workspace holds %zu bytes, need %zu", work_bytes, need);
@@ -930,11 +931,11 @@ int rpfq_window_attention_grad(const rpfq_window_desc* d, const void* q, const v
     if (!grad_out || !stat || !work || (!grad_q && !grad_k && !grad_v))
         return fail(RPFQ_ERR_NULL, "rpfq_window_attention_grad: NULL pointer argument");
     if (!window_strides(d->out_stride) || !window_strides(d->grad_stride) || !aligned(grad_out, 16) || !aligned(stat, 256) ||
-        !aligned(d->top, 256) || !aligned(grad_q, 16) || !aligned(grad_k, 16) || !aligned(grad_v, 16) || !aligned(work, 256))
-        return fail(RPFQ_ERR_ALIGN, "gradients must be 16-byte aligned, stat, desc->top and work 256; strides multiples of 8 elements");
+        !aligned(d->top, 256) || !aligned(d->rests, 16) || !aligned(grad_q, 16) || !aligned(grad_k, 16) || !aligned(grad_v, 16) || !aligned(work, 256))
+        return fail(RPFQ_ERR_ALIGN, "gradients must be 16-byte aligned, stat, desc->top and work 256, desc->rests 16; strides multiples of 8 elements");
     const size_t need = rpfq::window_bytes(*d, true);
     if (work_bytes < need) return fail(RPFQ_ERR_SHAPE, "workspace holds %zu bytes, need %zu", work_bytes, need);
-    if (!d->top) return fail(RPFQ_ERR_NULL, "the gradient needs desc->top beside stat");
+    if (!d->top || !d->rests) return fail(RPFQ_ERR_NULL, "the gradient needs desc->top and desc->rests beside stat");
     return hip_status(rpfq::launch_window_attention_grad(*d, q, k, v, lengths, out, grad_out, stat, grad_q, grad_k, grad_v, work,
                                                          reinterpret_cast<hipStream_t>(stream)),
                       "rpfq_window_attention_grad");

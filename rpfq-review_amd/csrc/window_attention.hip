@@ -195,7 +195,7 @@ struct WinFar {
 };
 struct WinArgs {
     const char *q, *k, *v, *o, *go;     // o: out of the forward, in of the gradient
-    char *out, *gq, *gk, *gv;
+    char *out, *gq, *gk, *gv, *rests;   // rests: out of the forward, in of the gradient, contiguous
     int64_t qs[3], ks[3], vs[3], os[3], gos[3];  // bytes between batches, tokens, heads
     const int32_t* lengths;
     float *top, *stat, *delta;          // [B, H, NP]; stat: lg
@@ -313,24 +313,37 @@ __device__ __forceinline__ WinTiles win_tiles(const WinArgs& a, int q0, int q1, 
 }
 
 // 32 rows of DP results [d][row] as 16-bit values: after trading halves across
-// the 32 lanes each lane has 8 consecutive ones.
-template <int DP, bool BF>
-__device__ __forceinline__ void win_store(const floatx16 (&o)[DP / 32], float f, bool zero, bool inside, char* dst, int D, int g) {
+// the 32 lanes each lane has 8 consecutive ones.  RESTS: what that rounds off too.
+template <bool BF>
+__device__ __forceinline__ uint32_t win_pack_rest(float lo, float hi, uint32_t p) {
+    const half2v h = __builtin_bit_cast(half2v, p);
+    return win_pack<BF>(lo - (BF ? bf16_to_f32(p & 0xffffu) : (float)h[0]), hi - (BF ? bf16_to_f32(p >> 16) : (float)h[1]));
+}
+template <int DP, bool BF, bool RESTS = false>
+__device__ __forceinline__ void win_store(const floatx16 (&o)[DP / 32], float f, bool zero, bool inside, char* dst, int D, int g, char* rests = nullptr) {
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-            uint32_t x[2], y[2];
+            uint32_t x[2], y[2], xr[2], yr[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                x[e] = win_pack<BF>(o[j][8 * p + 2 * e] * f, o[j][8 * p + 2 * e + 1] * f);
-                y[e] = win_pack<BF>(o[j][8 * p + 4 + 2 * e] * f, o[j][8 * p + 5 + 2 * e] * f);
+                const float a = o[j][8 * p + 2 * e] * f, b = o[j][8 * p + 2 * e + 1] * f;
+                const float c = o[j][8 * p + 4 + 2 * e] * f, h = o[j][8 * p + 5 + 2 * e] * f;
+                x[e] = win_pack<BF>(a, b);
+                y[e] = win_pack<BF>(c, h);
+                if (RESTS) xr[e] = zero ? 0 : win_pack_rest<BF>(a, b, x[e]), yr[e] = zero ? 0 : win_pack_rest<BF>(c, h, y[e]);
                 if (zero) x[e] = y[e] = 0;
             }
             const auto s0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
             const auto s1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
             const int d = 32 * j + 16 * p + 8 * g;
             if (inside && d < D) *reinterpret_cast<uint4*>(dst + 2 * d) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+            if constexpr (RESTS) {
+                const auto r0 = __builtin_amdgcn_permlane32_swap(xr[0], yr[0], false, false);
+                const auto r1 = __builtin_amdgcn_permlane32_swap(xr[1], yr[1], false, false);
+                if (inside && d < D) *reinterpret_cast<uint4*>(rests + 2 * d) = make_uint4(r0[0], r1[0], r0[1], r1[1]);
+            }
         }
 }
 
@@ -539,9 +552,13 @@ __device__ __forceinline__ void win_part(float* dst, const floatx16 (&o)[DP / 32
 // already the operand of O^T = V^T P^T.  K and V tiles of 64 keys go to LDS by
 // DMA, the next one while this one is used.  Bound by the products for heads of
 // 128 (8,192 tokens, 16 heads on 4, window 1,024, bf16: 88 us, 0.87 PFLOP/s of what
-// the tiles compute), by exponentials, masks and first loads for heads of 64 (96
-// heads, 1,025 tokens, 127 to both sides: 29 us).
-template <int DP, bool BF>
+// the tiles compute), by few and short walks over the keys for heads of 64 (96
+// heads, 1,025 tokens, 127 to both sides: 29 us).  P goes into P V rounded to 16
+// bits, which costs the output up to 0.4 of its own rounding.  TWO, where a gradient
+// is wanted: with the rest as a second term (112 and 36 us), since rowsum(dO O) is
+// subtracted from values as large, and what O is off by is much of what is left.
+// The careful pass keeps one term.
+template <int DP, bool BF, bool TWO>
 __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_forward_kernel(WinArgs a) {
     extern __shared__ __align__(256) char smem[];
     constexpr int T = 64, TILE = T * Rows<DP>::RB;  // K, then V; twice
@@ -610,7 +627,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
 #pragma unroll
                     for (int v = 0; v < 16; ++v) o[j][v] *= f;
             };
-            uint4 pr;
+            uint4 pr, rest;
             floatx16 s[2];
             s[0] = s[1] = floatx16{0};
             float take = 0.0f;
@@ -644,9 +661,16 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
                     pr = win_pack8<BF>(s[u >> 1], u & 1);
                     // the sum of the rounded probabilities: their rounding errors then
                     // weigh the values' distance to the output, not the values
-                    st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
+                    if (TWO && !FAR) {
+                        rest = win_rest8<BF>(s[u >> 1], u & 1, pr);
+#pragma unroll
+                        for (int v = 0; v < 8; ++v) st.l += s[u >> 1][8 * (u & 1) + v];
+                    } else {
+                        st.l = win_sum2<BF>(pr.x, win_sum2<BF>(pr.y, win_sum2<BF>(pr.z, win_sum2<BF>(pr.w, st.l))));
+                    }
                 }
                 o[j] = FAR ? win_mma_some<BF>(f, pr, sees[u >> 1] >> 8 * (u & 1), o[j]) : win_mma<BF>(f, pr, o[j]);
+                if (TWO && !FAR) o[j] = win_mma<BF>(f, rest, o[j]);
                 if (y == 0) hide(s[1], 1);
                 if (u == 1 || u == 2) win_exp(s[1], 8 * (y - NJ) / NJ, 8 * (y + 1 - NJ) / NJ, a.scale2, take);
             });
@@ -674,7 +698,8 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
     const bool joined = a.far.parts && i < a.far.rows;
     if (a.stat && g == 0 && i < a.NP && !joined)
         win_stat<BF>(a.top, a.stat, ((int64_t)p.b * a.H + p.h) * a.NP + i, any, st.top, rel + __builtin_amdgcn_logf(l));
-    win_store<DP, BF>(o, any ? 1.0f / l : 0.0f, !any, i < a.N && !joined, a.out + p.b * a.os[0] + (int64_t)i * a.os[1] + p.h * a.os[2], a.D, g);
+    win_store<DP, BF, TWO>(o, any ? 1.0f / l : 0.0f, !any, i < a.N && !joined, a.out + p.b * a.os[0] + (int64_t)i * a.os[1] + p.h * a.os[2], a.D, g,
+                           a.rests + (((int64_t)p.b * a.N + i) * a.H + p.h) * 2 * a.D);
 }
 
 // fp16 gradients: dS is carried times a power of two of its column (one query in
@@ -708,7 +733,7 @@ __device__ __forceinline__ void win_scale_ds(floatx16& ds, float& c, floatx16 (&
 // Gradient of the queries, laid out as the forward: S^T = K Q^T and dP^T = V dO^T
 // in one lane's query, dQ^T = K^T dS^T.  Leaves rowsum(dO O) for the other.  Of
 // the forward's sizes 114 us (1.0 PFLOP/s) and 39.
-template <int DP, bool BF>
+template <int DP, bool BF, bool TWO>
 __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(WinArgs a) {
     extern __shared__ __align__(256) char smem[];
     constexpr int T = 64, TILE = T * Rows<DP>::RB;
@@ -722,10 +747,11 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
     win_row<DP>(go, a.go + p.b * a.gos[0] + p.h * a.gos[2], i * a.gos[1], i < p.n, a.D, g);
     float delta = 0.0f;
     {
-        uint4 out[DP / 16];
+        uint4 out[DP / 16], rest[DP / 16];
         win_row<DP>(out, a.o + p.b * a.os[0] + p.h * a.os[2], i * a.os[1], i < p.n, a.D, g);
+        win_row<DP>(rest, a.rests + ((int64_t)p.b * a.N * a.H + p.h) * 2 * a.D, (int64_t)i * a.H * 2 * a.D, i < p.n, a.D, g);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) delta = win_dot8<BF>(go[s], out[s], delta);
+        for (int s = 0; s < DP / 16; ++s) delta = win_dot8<BF>(go[s], rest[s], win_dot8<BF>(go[s], out[s], delta));
         delta = half_sum(delta);
     }
     if (g == 0 && i < a.NP && !p.unit.part) a.delta[row] = delta;
@@ -776,7 +802,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
         };
         floatx16 s[2], dp = floatx16{0};
         s[0] = s[1] = floatx16{0};
-        uint4 ds;
+        uint4 ds, rest;
         auto finish = [&](int kb) WIN_INLINE {  // dS from P and dP
 #pragma unroll
             for (int v = 0; v < 16; ++v) s[kb][v] *= dp[v] - delta;
@@ -799,8 +825,12 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
             }
             const int y = e - 4 * NS, u = y / NJ, j = y % NJ;
             if (y == (BF ? 1 : 2 * NJ)) finish(1);  // fp16: it may scale what was summed, so behind the first's
-            if (j == 0) ds = win_pack8<BF>(s[u >> 1], u & 1);
+            if (j == 0) {
+                ds = win_pack8<BF>(s[u >> 1], u & 1);
+                if (TWO) rest = win_rest8<BF>(s[u >> 1], u & 1, ds);
+            }
             o[j] = win_mma<BF>(f, ds, o[j]);
+            if (TWO) o[j] = win_mma<BF>(f, rest, o[j]);
         });
         at.move(t & 1 ? -2 * TILE : 2 * TILE);
     }
@@ -844,7 +874,7 @@ template <int... E>
 __device__ __forceinline__ void win_diff(std::integer_sequence<int, E...>, floatx16& dp, float delta) {
     ((dp[E] -= win_lane<E>(delta)), ...);
 }
-template <int DP, bool BF>
+template <int DP, bool BF, bool TWO>
 __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(WinArgs a) {
     extern __shared__ __align__(256) char smem[];
     constexpr int RB = Rows<DP>::RB, V = kWinKeys * RB, STAGE = 2 * kWinStep * RB;  // V, two stages of Q and dO
@@ -939,7 +969,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
                 const int x = e - 3 * NS;
                 return at.cols((x < 2 * NJ ? OUT : 0) + x / NJ % 2 * 16 * RB, x % NJ);
             };
-            uint4 pr, was;
+            uint4 pr, was, rest;
             floatx16 s = floatx16{0}, dp = floatx16{0};
             win_stream<3 * NS + 4 * NJ, PD>(read, [&](int e, uint4 f) WIN_INLINE {
                 if (e < NS) {
@@ -961,8 +991,12 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
                 }
                 const int x = e - 3 * NS, j = x % NJ;
                 if (x < 2 * NJ) {
-                    if (j == 0) pr = win_pack8<BF>(s, x / NJ);
+                    if (j == 0) {
+                        pr = win_pack8<BF>(s, x / NJ);
+                        if (TWO) rest = win_rest8<BF>(s, x / NJ, pr);
+                    }
                     ov[j] = win_mma<BF>(f, pr, ov[j]);
+                    if (TWO) ov[j] = win_mma<BF>(f, rest, ov[j]);
                     if (x == 1) {
                         win_diff(std::make_integer_sequence<int, 16>(), dp, delta);
 #pragma unroll
@@ -975,8 +1009,12 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
                     }
                 } else {
                     if (x == 2 * NJ) win_scale_ds<DP, BF>(dp, c, ok);
-                    if (j == 0) pr = win_pack8<BF>(dp, x / NJ % 2);
+                    if (j == 0) {
+                        pr = win_pack8<BF>(dp, x / NJ % 2);
+                        if (TWO) rest = win_rest8<BF>(dp, x / NJ % 2, pr);
+                    }
                     ok[j] = win_mma<BF>(f, pr, ok[j]);
+                    if (TWO) ok[j] = win_mma<BF>(f, rest, ok[j]);
                 }
             });
         }
@@ -1192,12 +1230,13 @@ constexpr int kWinSlots = 256;
 struct WinJoin {
     const float* part;
     char* out[2];         // GRAD: keys and values, rows of one behind the other's; NULL: not wanted
+    char* rests;          // of the output, contiguous, or NULL
     float factor[2];
     float *top, *stat;    // [B, heads, NP], or NULL
     float scale2;
     int64_t os[3];
     int64_t rows, all;    // sequences x tokens x heads; of both tensors
-    int tokens, heads, slots, D, NP;
+    int tokens, heads, slots, D, N, NP;
 };
 template <int DP, bool BF, bool GRAD>
 __global__ void __launch_bounds__(256) window_join_kernel(WinJoin a) {
@@ -1248,8 +1287,11 @@ __global__ void __launch_bounds__(256) window_join_kernel(WinJoin a) {
 #pragma unroll
             for (int t = 0; t < 4; ++t) v[t] += sums[s][d][t];
         const float inv = GRAD ? a.factor[which] : l == 0.0f ? 0.0f : 1.0f / l;
-        *reinterpret_cast<uint2*>(out + seq * a.os[0] + tok * a.os[1] + h * a.os[2] + 8 * d) =
-            make_uint2(win_pack<BF>(v[0] * inv, v[1] * inv), win_pack<BF>(v[2] * inv, v[3] * inv));
+        const uint2 x = make_uint2(win_pack<BF>(v[0] * inv, v[1] * inv), win_pack<BF>(v[2] * inv, v[3] * inv));
+        *reinterpret_cast<uint2*>(out + seq * a.os[0] + tok * a.os[1] + h * a.os[2] + 8 * d) = x;
+        if (!GRAD && a.rests)
+            *reinterpret_cast<uint2*>(a.rests + ((seq * a.N + tok) * a.heads + h) * 2 * a.D + 8 * d) =
+                make_uint2(win_pack_rest<BF>(v[0] * inv, v[1] * inv, x.x), win_pack_rest<BF>(v[2] * inv, v[3] * inv, x.y));
     }
 }
 
@@ -1272,6 +1314,7 @@ static WinArgs win_args(const rpfq_window_desc& d, const void* q, const void* k,
     a.scale = d.scale;
     a.scale2 = d.scale * 1.4426950408889634f;
     a.top = d.top;
+    a.rests = reinterpret_cast<char*>(d.rests);
     const int group = a.H / a.KV;
     a.hw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
     a.qw = 4 / a.hw;
@@ -1303,7 +1346,7 @@ static WinJoin win_joined(const WinArgs& a, const float* part, int tokens, int64
     WinJoin j = {part};
     j.os[0] = n * heads * 2 * a.D, j.os[1] = (int64_t)heads * 2 * a.D, j.os[2] = 2 * a.D;
     j.rows = (int64_t)a.B * tokens * heads;
-    j.tokens = tokens, j.heads = heads, j.slots = slots, j.D = a.D, j.NP = a.NP;
+    j.tokens = tokens, j.heads = heads, j.slots = slots, j.D = a.D, j.N = a.N, j.NP = a.NP;
     j.scale2 = a.scale2;
     return j;
 }
@@ -1312,21 +1355,34 @@ struct WinForward {
     hipStream_t s;
     template <int DP, bool BF>
     hipError_t run() {
-        const hipError_t e = WIN_LAUNCH((window_forward_kernel<DP, BF>), a, win_units(a.far, (int64_t)a.B * (a.H / a.hw), a.tiles), 256,
-                                        4 * 64 * Rows<DP>::RB, s);
+        const int64_t units = win_units(a.far, (int64_t)a.B * (a.H / a.hw), a.tiles);
+        const hipError_t e = a.rests ? WIN_LAUNCH((window_forward_kernel<DP, BF, true>), a, units, 256, 4 * 64 * Rows<DP>::RB, s)
+                                     : WIN_LAUNCH((window_forward_kernel<DP, BF, false>), a, units, 256, 4 * 64 * Rows<DP>::RB, s);
         if (e != hipSuccess || !a.far.parts) return e;
         WinJoin j = win_joined(a, a.part, a.far.rows, a.N, a.H, a.far.parts + 1);
         for (int i = 0; i < 3; ++i) j.os[i] = a.os[i];
-        j.out[0] = a.out, j.top = a.top, j.stat = a.stat;
+        j.out[0] = a.out, j.rests = a.rests, j.top = a.top, j.stat = a.stat;
         return win_join<DP, BF, false>(j, s);
     }
 };
+// P and dS go into the gradients' products as one 16-bit term: over many rows what
+// that rounds off adds up to as much as the results' own rounding (together 1.41 of
+// it).  Over few rows it does not even out, and the results were off by up to 1.7
+// of it: up to 8,192 rows (tokens x heads) have a second term each.  With it always,
+// 8,192 tokens of 16 heads of 128 on 4 take 455 us forward and backward, with one
+// 396; 512 tokens of 12 heads of 64 (6,144 rows) take 53 in a graph and with one 46,
+// both less than the host's time without a graph.
+constexpr int64_t kWinFewRows = 8192;
 struct WinGrad {
     const WinArgs& a;
     hipStream_t s;
     template <int DP, bool BF>
     hipError_t run() {
-        hipError_t e = WIN_LAUNCH((window_grad_q_kernel<DP, BF>), a, win_units(a.far, (int64_t)a.B * (a.H / a.hw), a.tiles), 256,
+        return (int64_t)a.B * a.H * a.N <= kWinFewRows ? go<DP, BF, true>() : go<DP, BF, false>();
+    }
+    template <int DP, bool BF, bool TWO>
+    hipError_t go() {
+        hipError_t e = WIN_LAUNCH((window_grad_q_kernel<DP, BF, TWO>), a, win_units(a.far, (int64_t)a.B * (a.H / a.hw), a.tiles), 256,
                                   4 * 64 * Rows<DP>::RB, s);
         if (e == hipSuccess && a.gq && a.far.parts) {
             WinJoin j = win_joined(a, a.part, a.far.rows, a.N, a.H, a.far.parts + 1);
@@ -1334,7 +1390,7 @@ struct WinGrad {
             e = win_join<DP, BF, true>(j, s);
         }
         if (e != hipSuccess || (!a.gk && !a.gv)) return e;
-        e = WIN_LAUNCH((window_grad_kv_kernel<DP, BF>), a, win_units(a.kfar, (int64_t)a.B * a.KV, (a.N + kWinKeys - 1) / kWinKeys), 256,
+        e = WIN_LAUNCH((window_grad_kv_kernel<DP, BF, TWO>), a, win_units(a.kfar, (int64_t)a.B * a.KV, (a.N + kWinKeys - 1) / kWinKeys), 256,
                        win_grad_lds<DP>(), s);
         if (e != hipSuccess || !a.kfar.parts) return e;
         WinJoin j = win_joined(a, a.kpart, a.kfar.rows, a.N, a.KV, a.kfar.parts + 1);

@@ -194,6 +194,7 @@ class WindowDesc(ctypes.Structure):
         ("causal", ctypes.c_int32),
         ("scale", ctypes.c_float),
         ("top", ctypes.c_void_p),
+        ("rests", ctypes.c_void_p),
     ]
 
 

@@ -130,25 +130,26 @@ def test_far_scores_over_a_cache(b, t, m, heads, kv, d, window, sinks, lengths, 
     W._check(ops.window_attention_cached(q, k, v, torch.tensor(lengths, dtype=torch.int32, device=DEV), window, sinks, scale=scale), *want)
 
 
-def test_the_statistic_has_two_arrays():
-    """stat and desc.top go together, and both are checked before anything is launched."""
+def test_what_goes_with_the_statistic():
+    """stat, desc.top and desc.rests go together, and are checked before anything is launched."""
     import ctypes
 
     from quant_models import _native as N
 
     L, at = N.load(), 1 << 20
 
-    def desc(top):
-        d = N.WindowDesc(B=2, N=50, H=4, KV=2, D=64, window=9, sinks=1, dtype=1, causal=1, scale=0.125, top=top)
+    def desc(top, rests):
+        d = N.WindowDesc(B=2, N=50, H=4, KV=2, D=64, window=9, sinks=1, dtype=1, causal=1, scale=0.125, top=top, rests=rests)
         for s in ("q_stride", "k_stride", "v_stride", "out_stride", "grad_stride"):
             getattr(d, s)[:] = (50 * 256, 256, 64)
         return ctypes.byref(d)
 
-    def fwd(top, stat):
-        return L.rpfq_window_attention(desc(top), at, at, at, None, at, stat, at, 1 << 40, None)
+    def fwd(top, rests, stat):
+        return L.rpfq_window_attention(desc(top, rests), at, at, at, None, at, stat, at, 1 << 40, None)
 
-    def grad(top):
-        return L.rpfq_window_attention_grad(desc(top), at, at, at, None, at, at, at, at, at, at, at, 1 << 40, None)
+    def grad(top, rests):
+        return L.rpfq_window_attention_grad(desc(top, rests), at, at, at, None, at, at, at, at, at, at, at, 1 << 40, None)
 
-    assert fwd(None, at) == 1 and fwd(at, None) == 1 and fwd(at + 64, at) == 3
-    assert grad(None) == 1 and grad(at + 64) == 3
+    assert fwd(None, at, at) == 1 and fwd(at, None, at) == 1 and fwd(at, at, None) == 1 and fwd(at, None, None) == 1 and fwd(None, at, None) == 1
+    assert fwd(at + 64, at, at) == 3 and fwd(at, at + 8, at) == 3
+    assert grad(None, at) == 1 and grad(at, None) == 1 and grad(at + 64, at) == 3 and grad(at, at + 8) == 3
