@@ -383,6 +383,15 @@ torch::autograd::variable_list once_differentiable(torch::autograd::variable_lis
 
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// A saved tensor as the kernels read it: hooks on saved tensors (offloading,
+// recomputation) may give it back in another memory order than it was saved in.
+at::Tensor packed(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
+    if (!t.defined()) return t;
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == type && t.sizes() == sizes, "a saved tensor came back as another one");
+    const at::NoGradGuard no_graph;
+    return t.contiguous();
+}
+
 // The cross entropy of a classifier under autograd, as ops._LinearCrossEntropy.
 struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     static rpfq_ce_desc describe(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, int64_t ignore,
@@ -532,7 +541,9 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         refuse_capture("rms_norm");
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &h = saved[0], &w = saved[1], &rstd = saved[2];
+        const at::Tensor h = packed(saved[0], saved[0].sizes(), saved[0].scalar_type());
+        const at::Tensor w = saved[1].defined() ? packed(saved[1], {h.size(-1)}, saved[1].scalar_type()) : saved[1];
+        const at::Tensor rstd = packed(saved[2], {h.numel() / h.size(-1)}, at::kFloat);
         const bool res = ctx->saved_data["res"].toBool();  // needs_input_grad counts the tensors that were given
         const c10::DeviceGuard guard(h.device());
         torch::autograd::variable_list out(4);
@@ -541,6 +552,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
             const at::Tensor gh = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
             at::Tensor gx, gw;
             if (grads[0].defined()) {
+                TORCH_CHECK(grads[0].sizes() == h.sizes() && grads[0].scalar_type() == h.scalar_type(), "a saved tensor came back as another one");
                 const at::Tensor gy = grads[0].contiguous();
                 const int64_t c = h.size(-1), m = h.numel() / c;
                 gx = at::empty(h.sizes(), h.options().requires_grad(false));
@@ -643,6 +655,21 @@ struct Rotary : torch::autograd::Function<Rotary> {
     static void strides(const at::Tensor& t, int64_t (&s)[3]) {
         for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
     }
+    // type and strides of positions [N or B, N, axes]; false where they are none
+    static bool place(const at::Tensor& positions, rpfq_rotary_desc& d) {
+        switch (positions.scalar_type()) {
+            case at::kLong: d.pos_dtype = RPFQ_POS_I64; break;
+            case at::kInt: d.pos_dtype = RPFQ_POS_I32; break;
+            case at::kFloat: d.pos_dtype = RPFQ_POS_F32; break;
+            default: return false;
+        }
+        if (positions.dim() < 2 || positions.dim() > 3 || positions.size(-1) != d.axes || positions.size(-2) != d.N ||
+            (positions.dim() == 3 && positions.size(0) != d.B) || (d.axes > 1 && positions.stride(-1) != 1))
+            return false;
+        d.pos_stride[0] = positions.dim() == 3 ? positions.stride(0) : 0;
+        d.pos_stride[1] = positions.stride(-2);
+        return true;
+    }
     // x turned as d says (its sizes, sections and types filled in), in new tensors
     static torch::autograd::variable_list turn(rpfq_rotary_desc d, const std::array<at::Tensor, 2>& x, const at::Tensor& positions,
                                                const at::Tensor& freqs) {
@@ -677,6 +704,11 @@ struct Rotary : torch::autograd::Function<Rotary> {
         const std::string bytes = ctx->saved_data["desc"].toStringRef();
         std::memcpy(&d, bytes.data(), sizeof(d));
         d.inverse = 1;
+        int64_t pairs = 0;
+        for (int i = 0; i < d.axes; ++i) pairs += d.sections[i];
+        const at::Tensor freqs = packed(saved[1], {pairs}, at::kDouble);
+        const at::Tensor positions = saved[0].stride(-1) != 1 ? saved[0].contiguous() : saved[0];
+        TORCH_CHECK(positions.is_cuda() && place(positions, d), "a saved tensor came back as another one");
         torch::autograd::variable_list out(5);
         {
             const at::NoGradGuard plain_results;
@@ -688,7 +720,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
                 at_[n++] = i;
             }
             if (!n) return out;
-            const auto turned = turn(d, g, saved[0], saved[1]);
+            const auto turned = turn(d, g, positions, freqs);
             for (int i = 0; i < n; ++i) out[at_[i]] = turned[i];
         }
         return once_differentiable(std::move(out), "rotary");
@@ -706,19 +738,12 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor *pos = plain(a[2]), *freqs = plain(a[3]);
     const Py_ssize_t axes = PyTuple_GET_SIZE(a[4]);
     if (!pos || !freqs || axes < 1 || axes > 4 || freqs->scalar_type() != at::kDouble || freqs->dim() != 1 || !freqs->is_contiguous() ||
-        q.dim() != 4 || q.numel() == 0 || pos->dim() < 2 || pos->dim() > 3 || pos->size(-1) != axes ||
-        (axes > 1 && pos->stride(-1) != 1) || pos->requires_grad() || freqs->requires_grad() || transformed(*pos) ||
+        q.dim() != 4 || q.numel() == 0 || pos->requires_grad() || freqs->requires_grad() || transformed(*pos) ||
         transformed(*freqs))
         Py_RETURN_NONE;
     rpfq_rotary_desc d = {};
     d.B = q.size(0), d.N = q.size(1), d.D = q.size(3);
     d.dtype = dtype_code(q.scalar_type());
-    switch (pos->scalar_type()) {
-        case at::kLong: d.pos_dtype = RPFQ_POS_I64; break;
-        case at::kInt: d.pos_dtype = RPFQ_POS_I32; break;
-        case at::kFloat: d.pos_dtype = RPFQ_POS_F32; break;
-        default: Py_RETURN_NONE;
-    }
     d.axes = (int32_t)axes;
     int64_t pairs = 0;
     for (Py_ssize_t i = 0; i < axes; ++i) {
@@ -728,10 +753,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         pairs += v;
     }
     d.interleaved = inter != 0;
-    d.pos_stride[0] = pos->dim() == 3 ? pos->stride(0) : 0;
-    d.pos_stride[1] = pos->stride(-2);
-    if (freqs->size(0) != pairs || 2 * pairs > d.D || pos->size(-2) != d.N || (pos->dim() == 3 && pos->size(0) != d.B) ||
-        pos->device() != q.device() || freqs->device() != q.device())
+    if (!Rotary::place(*pos, d) || freqs->size(0) != pairs || 2 * pairs > d.D || pos->device() != q.device() || freqs->device() != q.device())
         Py_RETURN_NONE;
     for (const at::Tensor* t : {&q, &k})
         if (t->defined() && (t->dim() != 4 || t->size(0) != d.B || t->size(1) != d.N || t->size(3) != d.D || t->size(2) < 1 ||
@@ -797,18 +819,31 @@ struct Window : torch::autograd::Function<Window> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         refuse_capture("window_attention");
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &lengths = saved[3], &out = saved[4], &stat = saved[5];
-        const c10::DeviceGuard guard(q.device());
         rpfq_window_desc d;
         const std::string bytes = ctx->saved_data["desc"].toStringRef();
         std::memcpy(&d, bytes.data(), sizeof(d));
+        const auto type = d.dtype == RPFQ_BF16 ? at::kBFloat16 : at::kHalf;
+        const std::array<int64_t, 4> like_q{d.B, d.N, d.H, d.D}, like_k{d.B, d.N, d.KV, d.D};
+        // in the memory order that they have now, which hooks on saved tensors may have changed
+        auto rows = [&](const at::Tensor& t, const std::array<int64_t, 4>& sizes, int64_t (&strides)[3]) {
+            TORCH_CHECK(t.is_cuda() && t.scalar_type() == type && t.sizes() == at::IntArrayRef(sizes), "a saved tensor came back as another one");
+            const at::NoGradGuard no_graph;
+            const at::Tensor r = window_rows16(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+            window_strides(r, strides);
+            return r;
+        };
+        const at::Tensor q = rows(saved[0], like_q, d.q_stride), k = rows(saved[1], like_k, d.k_stride), v = rows(saved[2], like_k, d.v_stride);
+        const at::Tensor out = rows(saved[4], like_q, d.out_stride), lengths = packed(saved[3], {d.B}, at::kInt);
+        const at::Tensor stat = packed(saved[5], {2, saved[5].size(-1)}, at::kFloat), rests = packed(saved[6], like_q, type);
+        TORCH_CHECK(stat.nbytes() >= 2 * api.rpfq_window_attention_stat_bytes(&d), "a saved tensor came back as another one");
+        const c10::DeviceGuard guard(q.device());
         torch::autograd::variable_list g(5);
         {
             const at::NoGradGuard plain_results;
             const at::Tensor go = window_rows16(grads[0]) ? grads[0] : grads[0].clone(at::MemoryFormat::Contiguous);
             window_strides(go, d.grad_stride);
             d.top = const_cast<float*>(stat.const_data_ptr<float>()) + stat.size(1);
-            d.rests = saved[6].data_ptr();
+            d.rests = rests.data_ptr();
             const at::Tensor* in[3] = {&q, &k, &v};
             for (int i = 0; i < 3; ++i)
                 if (ctx->needs_input_grad(i)) g[i] = at::empty(in[i]->sizes(), q.options().requires_grad(false));
