@@ -431,7 +431,10 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         refuse_capture("linear_cross_entropy");
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &x = saved[0], &w = saved[1], &target = saved[2], &bias = saved[3], &stat = saved[4];
+        const at::Tensor x = packed(saved[0], saved[0].sizes(), saved[0].scalar_type());
+        const at::Tensor w = packed(saved[1], {saved[1].size(0), x.size(1)}, x.scalar_type()), target = packed(saved[2], {x.size(0)}, at::kLong);
+        const at::Tensor bias = saved[3].defined() ? packed(saved[3], {w.size(0)}, saved[3].scalar_type()) : saved[3];
+        const at::Tensor stat = packed(saved[4], {3 * x.size(0) + 1}, at::kFloat);
         const c10::DeviceGuard guard(x.device());
         const rpfq_ce_desc d = describe(x, w, bias, ctx->saved_data["ignore"].toInt(), ctx->saved_data["smoothing"].toDouble(),
                                         ctx->saved_data["reduction"].toInt());

@@ -954,8 +954,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, bias, target, stat = ctx.saved_tensors
         desc = ctx.desc
+        m, d, v = desc.M, desc.D, desc.V
+        x, weight, bias, target, stat = (  # hooks may give them back in another memory order
+            t if t is None else t.contiguous() for t in ctx.saved_tensors)
+        if (x.shape, weight.shape, target.shape, stat.shape) != ((m, d), (v, d), (m,), (3 * m + 1,)) or x.dtype != weight.dtype \
+                or N.dtype_code(x.dtype) != desc.dtype or target.dtype != torch.int64 or stat.dtype != torch.float32 \
+                or (bias is not None and (bias.shape != (v,) or N.dtype_code(bias.dtype) != desc.bias_dtype)):
+            raise RuntimeError("linear_cross_entropy: a saved tensor came back as another one")
         want = ctx.needs_input_grad
         gx = torch.empty_like(x) if want[0] else None
         gw = torch.empty_like(weight) if want[1] else None

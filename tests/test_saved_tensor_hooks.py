@@ -63,3 +63,36 @@ def test_another_tensor_is_refused(name):
             outs = call()
         with pytest.raises(RuntimeError, match="another"):
             torch.autograd.grad([o.sum() for o in outs], leaves)
+
+
+@pytest.fixture(params=["native", "ctypes"])
+def host_path(request, monkeypatch):
+    if request.param == "ctypes":
+        from quant_models import _native
+
+        monkeypatch.setattr(_native, "host", lambda: None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hook", sorted(HOOKS))
+@pytest.mark.parametrize("bias", [False, True])
+def test_the_loss_through_hooks(bias, hook, host_path):
+    from quant_models import ops
+
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, w, b = (torch.randn(*s, generator=g, device=DEV).half().requires_grad_() for s in ((40, 64), (90, 64), (90,)))
+    target = torch.randint(0, 90, (40,), generator=g, device=DEV)
+    leaves = [x, w, b] if bias else [x, w]
+
+    def call():
+        return ops.linear_cross_entropy(x, w, target, b if bias else None)
+
+    want = torch.autograd.grad(call(), leaves)
+    with HOOKS[hook]():
+        loss = call()
+    assert all(torch.equal(a, e) for a, e in zip(torch.autograd.grad(loss, leaves), want))
+    for change in (lambda t: t[:1], lambda t: t.double()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            loss = call()
+        with pytest.raises((RuntimeError, ValueError, TypeError)):
+            torch.autograd.grad(loss, leaves)
