@@ -837,10 +837,12 @@ int rpfq_rotary(const rpfq_rotary_desc* desc, const void* q, const void* k, void
  * out = softmax(scale q k^T) v over what it sees, zeros for a row without any.
  * q, out [B, N, H, D]; k, v [B, N, KV, D] (cached: [B, M, KV, D]), KV a divisor of
  * H: query head h reads head h KV / H.  fp16 or bf16, scores and sums float32,
- * probabilities rounded to 16 bits (cached: two terms of 16 bits, as exact as the
- * output's type).  Strides in elements between batches, tokens
- * and heads, multiples of 8, below 2^22 between tokens; the values of a head
- * next to each other, D a multiple of 8 up to 128, pointers 16-byte aligned.
+ * probabilities rounded to 16 bits; where a gradient is wanted, and over a cache, as
+ * two terms of 16 bits (the output's error is then its own rounding).  The
+ * gradients' products take probabilities and dS as one term, up to B N H = 8192 as
+ * two.  Strides in elements between batches, tokens and heads, multiples of 8,
+ * below 2^22 between tokens; the values of a head next to each other, D a multiple
+ * of 8 up to 128, pointers 16-byte aligned.
  * lengths [B] (device int32, NULL: all of them N): rows of a sequence that
  * count, clamped to 0 .. N; those behind give zeros and are not read.
  * Up to 2^28 tokens and 1,024 heads, and what fits one launch: fewer than 2^24
@@ -881,7 +883,9 @@ int rpfq_window_attention_grad(const rpfq_window_desc* desc, const void* q, cons
 
 /* The last N tokens of each sequence against a cache of M slots: query t is
  * token lengths[b] - N + t, causal; lengths [B] (clamped to 0 .. M) counts the new
- * tokens.  Only slots that some query sees are read.  work: its workspace
+ * tokens.  Only slots that some query sees are read; every 32 rows of a key head go
+ * over all that the N tokens see (for many of them, rpfq_window_attention is the
+ * faster).  work: its workspace
  * (may be 0 bytes), 256-byte aligned; where lengths < N the first queries see
  * nothing. */
 int rpfq_window_attention_cached(const rpfq_window_desc* desc, const void* q, const void* k_cache, const void* v_cache,

@@ -555,7 +555,7 @@ __device__ __forceinline__ void win_part(float* dst, const floatx16 (&o)[DP / 32
 // the tiles compute), by few and short walks over the keys for heads of 64 (96
 // heads, 1,025 tokens, 127 to both sides: 29 us).  P goes into P V rounded to 16
 // bits, which costs the output up to 0.4 of its own rounding.  TWO, where a gradient
-// is wanted: with the rest as a second term (112 and 36 us), since rowsum(dO O) is
+// is wanted: with the rest as a second term (115 and 36 us), since rowsum(dO O) is
 // subtracted from values as large, and what O is off by is much of what is left.
 // The careful pass keeps one term.
 template <int DP, bool BF, bool TWO>
@@ -732,7 +732,7 @@ __device__ __forceinline__ void win_scale_ds(floatx16& ds, float& c, floatx16 (&
 
 // Gradient of the queries, laid out as the forward: S^T = K Q^T and dP^T = V dO^T
 // in one lane's query, dQ^T = K^T dS^T.  Leaves rowsum(dO O) for the other.  Of
-// the forward's sizes 114 us (1.0 PFLOP/s) and 39.
+// the forward's sizes 120 us (0.95 PFLOP/s) and 42.
 template <int DP, bool BF, bool TWO>
 __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(WinArgs a) {
     extern __shared__ __align__(256) char smem[];
@@ -850,9 +850,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_q_kernel(Win
 // P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS.  K stays in
 // registers, V in LDS (with both, 128-value heads spill); with two stages of Q
 // and dO that is 80 KB, two workgroups a CU.  Heads up to 64: three, with fewer
-// fragments ahead (96 heads of 64 over 1,025 tokens 46 us, two a CU 53).  The long
-// case of the forward 170 us (0.87 PFLOP/s), its sinks' far queries in parts (in
-// their tile's own workgroup: 1,276).  Statistics come by lane broadcasts: a
+// fragments ahead (96 heads of 64 over 1,025 tokens 49 us, with two a CU 7 more; a
+// few registers spill, outside the products).  The long case of the forward 175 us
+// (0.85 PFLOP/s), its sinks' far queries in parts (in their tile's own workgroup
+// seven times that).  Statistics come by lane broadcasts: a
 // 128-bit LDS read of one address by half a wave took 24 clocks.
 constexpr int kWinKeys = 64, kWinStep = 64;
 template <int DP>
@@ -1060,9 +1061,11 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : 3) window_grad_kv_kernel(Wi
 }
 
 // The last tokens over a cache.  A workgroup has one key head of one sequence,
-// up to 32 of its rows (queries x heads that share it) and a part of the keys; its
-// waves take tiles of 32 keys in turn, each through LDS of its own, without
-// waiting for each other.  Parts are joined by window_join_kernel.  P goes into P V
+// up to 32 of its rows (queries x heads that share it) and a part of the keys that
+// any of the sequence's new tokens sees (so 32 rows of many new tokens go over all
+// of theirs: 2,048 with a window of 128, 16 heads of 128 on 4, 0.32 ms, the whole
+// form 13 us); its waves take tiles of 32 keys in turn, each through LDS of its
+// own, without waiting for each other.  Parts are joined by window_join_kernel.  P goes into P V
 // as two 16-bit terms: the matrix units wait for memory here, and with one the
 // rounding of P is half of the output's error (bf16 2.3e-3 of it, with two 1.65e-3,
 // its own rounding).  Bound by HBM (64 streams, 4 key heads of 128, 4,100 slots,
@@ -1432,6 +1435,9 @@ static hipError_t win_dispatch(const rpfq_window_desc& d, Go go) {
 // Whether the tiles with sinks go in parts: where one of them has more steps than
 // a CU's share of them all (`slots` workgroups at once), so that the launch would
 // wait for it; a part is `share` of a tile's own steps.  `rows`, `steps` a tile.
+// Up to 128 sinks: the parts' float32 sums grow with them (16 heads of 128: 72 MB
+// then). With more a tile goes over its range alone: 8,192 tokens, 16 heads of 128
+// on 4, window 1,024, forward and backward 0.43 ms with 128 and 1.0 with 129.
 static WinFar win_far(int64_t sinks, int64_t groups, int64_t tiles, int64_t rows, int64_t window, int64_t N, int heads, int share) {
     WinFar f = {(int)((sinks + rows - 1) / rows), (int)sinks, 0};
     const int64_t all = heads * ((N + 63) / 64), near = heads * ((rows + window) / 64 + 1), slots = 2 * device_cus();

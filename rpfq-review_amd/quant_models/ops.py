@@ -1461,11 +1461,16 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     zeros, also in the gradients, and their values are not read.  Parts of a
     qkv tensor are read as they lie; heads that are not in one 16-byte aligned
     piece, or of no multiple of 8 values, are copied.  Scores and sums in
-    float32, probabilities rounded to q's type.  A value that is not finite
-    reaches the outputs of the queries that see it and no others; gradients of
-    rows near it may be NaN too.
+    float32, probabilities rounded to q's type for their product with v (as two
+    such terms where a gradient is wanted).  A value that is not finite reaches
+    the outputs of the queries that see it and no others; gradients of rows near
+    it may be NaN too.
     Gradients of q, k and v, once differentiable, sums in a fixed order; they
-    need the native host path (csrc/host.cpp); can be captured as rms_norm can."""
+    need the native host path (csrc/host.cpp); can be captured as rms_norm can.
+    Probabilities and the scores' gradient are rounded to q's type in their
+    products: up to B N heads = 8,192 as two terms, over more rows as one, whose
+    error is that of the results' own rounding again.  The backward keeps q, k,
+    v, the output, 16 bits more a value of it and 8 bytes a row and head."""
     host = N.host()
     if host is not None:
         given = q.shape[-1] ** -0.5 if scale is None and isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else scale
