@@ -1372,8 +1372,8 @@ struct WinForward {
 // that rounds off adds up to as much as the results' own rounding (together 1.41 of
 // it).  Over few rows it does not even out, and the results were off by up to 1.7
 // of it: up to 8,192 rows (tokens x heads) have a second term each.  With it always,
-// 8,192 tokens of 16 heads of 128 on 4 take 455 us forward and backward, with one
-// 396; 512 tokens of 12 heads of 64 (6,144 rows) take 53 in a graph and with one 46,
+// 8,192 tokens of 16 heads of 128 on 4 take 474 us forward and backward, with one
+// 401; 512 tokens of 12 heads of 64 (6,144 rows) take 53 in a graph and with one 46,
 // both less than the host's time without a graph.
 constexpr int64_t kWinFewRows = 8192;
 struct WinGrad {
