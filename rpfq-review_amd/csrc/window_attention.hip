@@ -137,18 +137,16 @@ __device__ __forceinline__ uint4 win_pack8(const floatx16& s, int u) {
     return make_uint4(win_pack<BF>(s[8 * u], s[8 * u + 1]), win_pack<BF>(s[8 * u + 2], s[8 * u + 3]),
                       win_pack<BF>(s[8 * u + 4], s[8 * u + 5]), win_pack<BF>(s[8 * u + 6], s[8 * u + 7]));
 }
-// What win_pack8 rounded off, as 16-bit values in the same order.
+// What win_pack, and win_pack8, rounded off, as 16-bit values in the same order.
+template <bool BF>
+__device__ __forceinline__ uint32_t win_rest(float lo, float hi, uint32_t p) {
+    const half2v h = __builtin_bit_cast(half2v, p);
+    return win_pack<BF>(lo - (BF ? bf16_to_f32(p & 0xffffu) : (float)h[0]), hi - (BF ? bf16_to_f32(p >> 16) : (float)h[1]));
+}
 template <bool BF>
 __device__ __forceinline__ uint4 win_rest8(const floatx16& s, int u, uint4 p) {
-    const uint32_t x[4] = {p.x, p.y, p.z, p.w};
-    uint32_t y[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const half2v h = __builtin_bit_cast(half2v, x[t]);
-        const float lo = BF ? bf16_to_f32(x[t] & 0xffffu) : (float)h[0], hi = BF ? bf16_to_f32(x[t] >> 16) : (float)h[1];
-        y[t] = win_pack<BF>(s[8 * u + 2 * t] - lo, s[8 * u + 2 * t + 1] - hi);
-    }
-    return make_uint4(y[0], y[1], y[2], y[3]);
+    return make_uint4(win_rest<BF>(s[8 * u], s[8 * u + 1], p.x), win_rest<BF>(s[8 * u + 2], s[8 * u + 3], p.y),
+                      win_rest<BF>(s[8 * u + 4], s[8 * u + 5], p.z), win_rest<BF>(s[8 * u + 6], s[8 * u + 7], p.w));
 }
 // c + lo + hi of a 16-bit pair
 template <bool BF>
@@ -314,11 +312,6 @@ __device__ __forceinline__ WinTiles win_tiles(const WinArgs& a, int q0, int q1, 
 
 // 32 rows of DP results [d][row] as 16-bit values: after trading halves across
 // the 32 lanes each lane has 8 consecutive ones.  RESTS: what that rounds off too.
-template <bool BF>
-__device__ __forceinline__ uint32_t win_pack_rest(float lo, float hi, uint32_t p) {
-    const half2v h = __builtin_bit_cast(half2v, p);
-    return win_pack<BF>(lo - (BF ? bf16_to_f32(p & 0xffffu) : (float)h[0]), hi - (BF ? bf16_to_f32(p >> 16) : (float)h[1]));
-}
 template <int DP, bool BF, bool RESTS = false>
 __device__ __forceinline__ void win_store(const floatx16 (&o)[DP / 32], float f, bool zero, bool inside, char* dst, int D, int g, char* rests = nullptr) {
 #pragma unroll
@@ -332,7 +325,7 @@ __device__ __forceinline__ void win_store(const floatx16 (&o)[DP / 32], float f,
                 const float c = o[j][8 * p + 4 + 2 * e] * f, h = o[j][8 * p + 5 + 2 * e] * f;
                 x[e] = win_pack<BF>(a, b);
                 y[e] = win_pack<BF>(c, h);
-                if (RESTS) xr[e] = zero ? 0 : win_pack_rest<BF>(a, b, x[e]), yr[e] = zero ? 0 : win_pack_rest<BF>(c, h, y[e]);
+                if (RESTS) xr[e] = zero ? 0 : win_rest<BF>(a, b, x[e]), yr[e] = zero ? 0 : win_rest<BF>(c, h, y[e]);
                 if (zero) x[e] = y[e] = 0;
             }
             const auto s0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
@@ -410,8 +403,9 @@ __device__ __forceinline__ float half_sum(float v) {
 
 // The running softmax of a lane's query over blocks of 32 keys (two lanes hold one
 // query's scores, half each): `top` the score that is subtracted, `sub` = top
-// scale2 + shift as it is rounded; l the sum, times 2^-win_rel relative to top.  top follows the largest score only
-// where that passes it by 2^kWinLag, so that the sums are hardly ever scaled anew.
+// scale2 + shift as it is rounded; l the sum, times 2^-win_rel relative to top.  top
+// follows the largest score only where that passes it by 2^kWinLag, so that the
+// sums are hardly ever scaled anew.
 struct WinState {
     float top, sub, l;
 };
@@ -659,8 +653,8 @@ __global__ void __launch_bounds__(256, DP > 64 ? 2 : DP > 32 ? 3 : 4) window_for
                     });
                 if (j == 0) {
                     pr = win_pack8<BF>(s[u >> 1], u & 1);
-                    // the sum of the rounded probabilities: their rounding errors then
-                    // weigh the values' distance to the output, not the values
+                    // with one term the sum of the rounded probabilities: their rounding errors
+                    // then weigh the values' distance to the output, not the values
                     if (TWO && !FAR) {
                         rest = win_rest8<BF>(s[u >> 1], u & 1, pr);
 #pragma unroll
@@ -1294,7 +1288,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(WinJoin a) {
         *reinterpret_cast<uint2*>(out + seq * a.os[0] + tok * a.os[1] + h * a.os[2] + 8 * d) = x;
         if (!GRAD && a.rests)
             *reinterpret_cast<uint2*>(a.rests + ((seq * a.N + tok) * a.heads + h) * 2 * a.D + 8 * d) =
-                make_uint2(win_pack_rest<BF>(v[0] * inv, v[1] * inv, x.x), win_pack_rest<BF>(v[2] * inv, v[3] * inv, x.y));
+                make_uint2(win_rest<BF>(v[0] * inv, v[1] * inv, x.x), win_rest<BF>(v[2] * inv, v[3] * inv, x.y));
     }
 }
 
